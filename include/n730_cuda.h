@@ -163,6 +163,73 @@ int n730_qweight_load_blocks(const char* path, int n, const int64_t* offsets, vo
 int n730_quantize_grouped(const float* d_w, int rows, int cols, int bits, int group, uint8_t* d_codes,
                           uint16_t* d_scales16, uint16_t* d_zeros16, void* stream);
 
+/* ---- key/value cache in 8 bits (no counterpart in the reference) ----
+ * A paged cache of one layer.  Codes lie as [n_pages][n_kv][page_size][head_dim] bytes, int8 or
+ * e4m3; `block` (16, 32 or 64, dividing page_size) consecutive positions of a page and KV head
+ * share one fp32 scale, [n_pages][n_kv][page_size / block]; a value is code * scale.  Position p of
+ * sequence b lies in page block_table[b * max_pages + p / page_size]; an id outside [0, n_pages) is
+ * no page: rows for it are dropped, reads of it give zeros, attention does not see its positions.
+ * All pointers are device memory of the current device and belong to the caller; code pools are
+ * 16-byte aligned, head_dim is 64 or 128.  Pages may be shared between sequences as long as no
+ * call writes them (append, evict).  The calls are asynchronous on `stream`, allocate nothing and
+ * can be captured into a graph.  Lengths and counts are read on the device (below 0 counts as 0,
+ * above the table's max_pages * page_size positions as that).  `dtype` is the type of the caller's
+ * rows; row strides are in elements, token t of sequence b is row b * tokens + t. */
+enum { N730_KV8_INT8 = 0, N730_KV8_E4M3 = 1 };
+enum { N730_F32 = 0, N730_F16 = 1, N730_BF16 = 2 };
+typedef struct N730KV8Cache {
+  void* k_codes;
+  void* v_codes;
+  float* k_scales;
+  float* v_scales;
+  const int32_t* block_table;
+  int32_t n_pages, max_pages, n_kv, head_dim, page_size, block, code;
+} N730KV8Cache;
+/* Append d_new[b] (all `tokens` when d_new is null) rows of K and V, [n_kv][head_dim] each, behind
+ * the d_lens[b] cached positions of sequence b; d_lens is not changed.  A block's scale is
+ * amax / 127 (int8) or amax / 448 (e4m3) over its rows, the older scale where that is larger; when
+ * it grows, the block's older codes are rounded to it.  Codes round to nearest, ties to even.
+ * amax is over finite values; NaN becomes 0, an infinity the largest code.  Rows past the table's
+ * capacity are dropped. */
+int n730_kv8_append(const N730KV8Cache* c, const void* d_k, const void* d_v, int dtype, int64_t ld, int batch,
+                    int tokens, const int32_t* d_lens, const int32_t* d_new, void* stream);
+/* Values of positions [d_first[b], d_first[b] + tokens) (from 0 when d_first is null) as rows
+ * [n_kv][head_dim] of d_k and d_v; positions outside [0, d_lens[b]) give zeros. */
+int n730_kv8_read(const N730KV8Cache* c, void* d_k, void* d_v, int dtype, int64_t ld, int batch, int tokens,
+                  const int32_t* d_first, const int32_t* d_lens, void* stream);
+/* Bytes of workspace of n730_kv8_attention (negative: a return code).  Zero the workspace once;
+ * each call leaves it ready for the next.  Calls that may overlap in time need one each. */
+int64_t n730_kv8_attention_ws(const N730KV8Cache* c, int batch, int tokens, int n_heads, int weights);
+/* Attention of the `tokens` newest rows of each sequence (d_new[b] of them) over its cached
+ * positions: query t of sequence b, RoPE applied, sees positions [0, d_lens[b] + t] - call it after
+ * n730_kv8_append with the same d_lens and d_new.  d_q and d_out rows are [n_heads][head_dim]
+ * (query head i reads KV head i / (n_heads / n_kv)); out rows from d_new[b] on are left as they
+ * were; a query that sees no position gives zeros.  Scores are scaled by `scale`.  fp32 rows keep
+ * fp32 accuracy; 16-bit rows round the softmax weights to fp16.
+ * d_w_out (may be null) [batch][n_kv][ldw]: for positions below d_lens[b] + d_new[b], d_w (null:
+ * zeros; may equal d_w_out) plus the softmax weights summed over the KV head's queries; positions
+ * that are new count from zero.  ldw >= max_pages * page_size. */
+int n730_kv8_attention(const N730KV8Cache* c, const void* d_q, int dtype, int64_t ldq, int batch, int tokens,
+                       int n_heads, float scale, const int32_t* d_lens, const int32_t* d_new, void* d_out,
+                       int64_t ldo, const float* d_w, float* d_w_out, int64_t ldw, void* d_ws, int64_t ws_bytes,
+                       void* stream);
+/* Bytes of workspace of n730_kv8_evict (negative: a return code); its contents do not matter. */
+int64_t n730_kv8_evict_ws(const N730KV8Cache* c, int batch, int keep);
+/* Cut every sequence of more than `keep` (a multiple of the block) cached slots to `keep`, per KV
+ * head: the slots of positions below `first` and of the last `recent` of the d_seen[b] positions
+ * seen so far stay, then those of the largest accumulated weight (ties: the lowest slot; NaN
+ * counts least).  Kept slots at or behind `keep` move into the holes before it, in order; the other
+ * rows keep their place and codes.  A block that takes rows in gets the largest scale of its rows
+ * and codes rounded to it.  d_pos [batch][n_kv][ldw] holds each slot's position (start with 0, 1,
+ * 2, ...); d_w and d_pos move along, and from `keep` on d_w_out is 0 and d_pos_out the positions
+ * that tokens appended there will have (d_seen[b], d_seen[b] + 1, ...).  d_lens_out[b] is the new
+ * length.  Outputs may be the same arrays as their inputs.  Sequences within `keep` stay as they
+ * are.  Attention over an evicted cache sees every kept slot: RoPE of the next token goes by
+ * d_seen, its slot by d_lens_out. */
+int n730_kv8_evict(const N730KV8Cache* c, int batch, int keep, int first, int recent, const int32_t* d_seen,
+                   const int32_t* d_lens, int32_t* d_lens_out, const float* d_w, float* d_w_out,
+                   const int32_t* d_pos, int32_t* d_pos_out, int64_t ldw, void* d_ws, int64_t ws_bytes, void* stream);
+
 /* ---- whole-model engine (replaces N730CudaTransformer.forward's per-op loop,
  * src-code/inference.py:259-669) ---- */
 typedef struct N730ModelConfig {

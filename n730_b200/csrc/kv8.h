@@ -1,0 +1,73 @@
+// Paged key/value cache in 8 bits: shared definitions of its kernels.
+//
+// Codes lie as [pages][n_kv][page_size][head_dim] bytes, int8 or e4m3; `block` consecutive
+// positions of a page and KV head share one fp32 scale, [pages][n_kv][page_size / block]; a
+// value is code * scale.  Position p of sequence b lies in page block_table[b * max_pages +
+// p / page_size]; an id outside [0, n_pages) is no page.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+#include "n730_cuda.h"
+
+namespace n730 {
+
+int kv8_check(const N730KV8Cache* c, int batch, const char* what);
+int kv8_append_launch(const N730KV8Cache& c, const void* k, const void* v, int dtype, int64_t ld, int batch,
+                      int tokens, const int* lens, const int* n_new, bool pdl, cudaStream_t st);
+
+struct KV8AttnCall {
+  N730KV8Cache c;
+  const void* q; void* out;
+  int dtype;
+  int64_t ldq, ldo;
+  int batch, tokens, heads;
+  float scale;
+  const int* lens; const int* n_new;
+  const float* w_in; float* w_out;
+  int64_t ldw;
+  void* ws; int64_t ws_bytes;
+  bool pdl;
+};
+int64_t kv8_attention_ws(const N730KV8Cache& c, int batch, int tokens, int heads, bool weights);
+int kv8_attention_launch(const KV8AttnCall& a, cudaStream_t st);
+
+// one element of a row in the caller's type, widened to fp32
+__device__ __forceinline__ float kv8_load1(const void* p, int64_t i, int dtype) {
+  if (dtype == N730_F32) return reinterpret_cast<const float*>(p)[i];
+  if (dtype == N730_F16) return __half2float(reinterpret_cast<const __half*>(p)[i]);
+  return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void kv8_store1(void* p, int64_t i, int dtype, float x) {
+  if (dtype == N730_F32) reinterpret_cast<float*>(p)[i] = x;
+  else if (dtype == N730_F16) reinterpret_cast<__half*>(p)[i] = __float2half_rn(x);
+  else reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
+}
+inline int kv8_esize(int dtype) { return dtype == N730_F32 ? 4 : 2; }
+
+// cached positions of a sequence before a call's new rows, within the table's capacity
+__device__ __forceinline__ int kv8_len(const int* lens, int b, int cap) { return min(max(lens[b], 0), cap); }
+// new rows of a sequence (all `tokens` without a count array)
+__device__ __forceinline__ int kv8_new(const int* n_new, int b, int tokens) {
+  return n_new ? min(max(n_new[b], 0), tokens) : tokens;
+}
+
+// Launch with or without programmatic dependent launch.
+template <typename... KArgs, typename... Args>
+int kv8_launch(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  N730_CUDA(cudaLaunchKernelEx(&cfg, k, args...));
+  return N730_OK;
+}
+
+}  // namespace n730
