@@ -3,26 +3,31 @@
 //   out[b, t, head] = softmax_p(scale q . k_p) v_p,  positions p <= lens[b] + t of KV head head / G
 //
 // Split kernel (single tokens and few rows).  The rows of an item (sequence, KV head) are its
-// tokens x G query heads, up to RG = 16 at a time (8 for fp32 queries).  All items' 16-position
-// tiles form one line that the CTAs cut into equal runs, so ragged lengths and few sequences load
-// every SM alike; a run that covers part of an item leaves its (max, sum, output) in the workspace,
-// and the last CTA to finish an item joins the parts in run order (the result does not depend on
-// which CTA that is).  Within a CTA each warp takes every fourth tile.
+// tokens x G query heads, 8 or 16 at a time.  All items' 16-position tiles form one line that the
+// CTAs cut into equal runs, so ragged lengths and few sequences load every SM alike; a run that
+// covers part of an item leaves its (max, sum, output) in the workspace, and the last CTA to finish
+// an item joins the parts in run order (the result does not depend on which CTA that is).  Within a
+// CTA each warp takes every fourth tile, two of them at a time.
 //
+// The products are transposed, so that a key or a channel is a row of mma.m16n8k16's A and the few
+// query rows are its 8 columns: no half of an instruction works on rows that are not there.
+//   S^T = K Q^T: the order of the channels in the sum is free, so lane (g, t) feeds 16 contiguous
+//      bytes of keys g and g + 8, each 4 of them one k-step's slots.
+//   O^T = V^T P^T: lane (g, t) feeds 16 contiguous channels of keys 2t, 2t+1, 2t+8, 2t+9,
+//      interleaved by byte permutes; P^T comes from S^T by an 8x8 transposition between lanes.
 // A lane copies into shared memory, with cp.async, exactly the bytes that it later feeds to the
-// tensor cores, so tiles need no CTA barrier and no transposition through shared memory:
-//   K: S = Q K^T by mma.m16n8k16.  The order of the channels in the sum is free, so lane (g, t)
-//      reads 16 contiguous bytes of row g's key and each 4 of them are one k-step's slots.
-//   V: the order of the keys is free too.  Lane (g, t) owns keys 4t..4t+3 in both products: P
-//      passes from the accumulators of the first to the operand of the second in registers, and V
-//      needs 16 contiguous channels of those four keys, interleaved by byte permutes.
+// tensor cores: tiles need no CTA barrier and no transposition through shared memory.
 // int8 codes become fp16 exactly (1024 + 128 + q by a byte permute, then one subtraction), e4m3
-// codes by a conversion; K's scale multiplies the scores, V's scale goes into the exponent.
+// codes by a conversion.  K's scale multiplies the scores, V's scale the weights.
 //
-// Numerics.  Queries are scaled by a power of two per row so that a 16-bit query is exact in fp16;
-// an fp32 query is split into two fp16 terms that fill rows 0-7 and 8-15 of the same product, and
-// so is P: fp32 calls lose about 2^-22.  For 16-bit calls P is rounded to fp16 (2^-11 of each weight,
-// below the rounding of the output).  Maxima, sums and outputs are fp32.
+// Softmax.  Weights are kept against a reference that follows the maximum only when a score is more
+// than 2^8 above it, so a tile costs one vote and no reduction; a second reference does the same for
+// weight x V scale, which has to fit fp16 whatever the scales are.
+//
+// Numerics.  Queries are scaled by a power of two per row so that a 16-bit query is exact in fp16; an
+// fp32 query is split into two fp16 terms, and so is P: fp32 calls lose about 2^-22.  For 16-bit calls P
+// is rounded to fp16 (2^-11 of each weight, below the rounding of the output).  Maxima, sums and
+// outputs are fp32.
 #include <algorithm>
 
 #include "kv8.h"
@@ -31,11 +36,12 @@ namespace n730 {
 
 constexpr int KD_WARPS = 4;
 constexpr int KD_THREADS = KD_WARPS * 32;
-constexpr int KD_STAGES = 4;
-constexpr int KD_TILE = 16;
+constexpr int KD_STAGES = 4;     // tile buffers of a warp
+constexpr int KD_TILE = 16;      // positions
 constexpr int KD_CTAS_PER_SM = 3;
 constexpr int KD_MIN_UNITS = 8;  // tiles of a run: fewer would leave warps idle and joins to do
 constexpr int KD_MAX_BATCH = 4096;
+constexpr float KD_SLACK = 8.f;  // log2 of how far a weight may exceed its reference
 
 struct KDArgs {
   N730KV8Cache c;
@@ -58,13 +64,13 @@ struct KDGeom {
   static constexpr int VB = HD / 8;                   // V bytes per lane and key
   static constexpr int K_BYTES = 2 * KCH * 512;       // per tile
   static constexpr int TILE_BYTES = K_BYTES + 4 * VB * 32;
-  static constexpr int OSTRIDE = HD + 8;              // padded output row (bank spread)
+  static constexpr int OSTRIDE = HD + 4;              // padded output row (bank spread, 16-byte rows)
 };
 
 template <int HD>
 struct KDSmem {
   uint8_t ring[KD_WARPS][KD_STAGES][KDGeom<HD>::TILE_BYTES];
-  uint4 qf[HD / 16][32];           // Q as the A operand, by k-step and lane
+  uint2 qf[2][HD / 16][32];        // Q^T as the B operand by k-step and lane: rows 8-15 or low terms second
   float sc[KD_WARPS][KD_STAGES][2];
   int ok[KD_WARPS][KD_STAGES];
   float rowmul[16];
@@ -91,6 +97,12 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint4& a, uint32_t
                "{%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+// 8x8 matrix of 16-bit elements, one row of two columns a lane: transposed between the lanes
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 template <int BYTES>
 __device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool pred) {
@@ -127,14 +139,16 @@ __device__ __forceinline__ int kd_units(const KDArgs& a, int b, int cap) {
   return (tot + KD_TILE - 1) / KD_TILE;
 }
 
-// HL: fp32 queries, 8 rows as high and low fp16 halves; else 16 rows.
-template <int HD, int CODE, bool HL>
+// NB: 8-row groups of an item's rows worked on together; LO: fp32 rows in two fp16 terms.
+template <int HD, int CODE, int NB, bool LO>
 __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(const KDArgs a) {
   using G = KDGeom<HD>;
-  constexpr int RG = HL ? 8 : 16, NT = HD / 8, ST = KD_STAGES;
+  constexpr int RG = 8 * NB, KS = HD / 16, MT = HD / 16, ST = KD_STAGES;
+  constexpr int TT = NB == 1 ? 2 : 1;  // tiles worked on together: independent chains for the tensor cores
   extern __shared__ __align__(128) uint8_t kd_raw[];
   KDSmem<HD>& sm = *reinterpret_cast<KDSmem<HD>*>(kd_raw);
   static_assert(sizeof(float) * KD_WARPS * RG * G::OSTRIDE <= sizeof(sm.ring), "per-warp outputs fit the ring");
+  static_assert(ST % TT == 0 && ST > TT, "whole groups of tiles in flight");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   const N730KV8Cache& c = a.c;
   const int cap = c.max_pages * c.page_size;
@@ -206,18 +220,17 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
       const int row = __shfl_sync(0xffffffffu, rows_now, qi & 31);
       const bool ok = row >= 0;
       const int64_t r0 = ok ? row : 0;
-      const uint32_t dst = ring + st * G::TILE_BYTES + lane * 16;
-      const uint8_t* kc = reinterpret_cast<const uint8_t*>(c.k_codes) + r0 * HD;
-      const uint8_t* vc = reinterpret_cast<const uint8_t*>(c.v_codes) + r0 * HD;
+      const uint32_t dst = ring + st * G::TILE_BYTES;
+      const uint8_t* kc = reinterpret_cast<const uint8_t*>(c.k_codes) + r0 * HD + g * HD + t4 * 16;
+      const uint8_t* vc = reinterpret_cast<const uint8_t*>(c.v_codes) + r0 * HD + 2 * t4 * HD + g * G::VB;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < G::KCH; ++j)
-          cp_async<16>(dst + (i * G::KCH + j) * 512, kc + (4 * (g >> 1) + 2 * i + (g & 1)) * HD + j * 64 + t4 * 16, ok);
+          cp_async<16>(dst + (i * G::KCH + j) * 512 + lane * 16, kc + 8 * i * HD + j * 64, ok);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        cp_async<G::VB>(ring + st * G::TILE_BYTES + G::K_BYTES + i * 32 * G::VB + lane * G::VB,
-                        vc + (4 * t4 + i) * HD + g * G::VB, ok);
+        cp_async<G::VB>(dst + G::K_BYTES + i * 32 * G::VB + lane * G::VB, vc + ((i & 1) + 8 * (i >> 1)) * HD, ok);
       if (lane < 2) {
         const float* s = (lane ? c.v_scales : c.k_scales) + (r0 >> a.log_block);
         cp_async<4>(smem_u32(&sm.sc[warp][st][lane]), s, ok);
@@ -225,12 +238,12 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
       if (lane == 0) sm.ok[warp][st] = ok;
     };
 #pragma unroll
-    for (int s = 0; s < ST - 1; ++s) {
+    for (int s = 0; s < ST - TT; ++s) {  // one group per TT tiles
       if (s < n_tile) issue(s);
-      cp_commit();
+      if (s % TT == TT - 1) cp_commit();
     }
 
-    // ---- Q: a row per warp at a time, scaled by a power of two, as the A operand ----
+    // ---- Q: a row per warp at a time, scaled by a power of two, as the B operand ----
     for (int r = warp; r < RG; r += KD_WARPS) {
       constexpr int E = HD / 32;  // channels a lane
       float x[E];
@@ -252,190 +265,247 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const int dch = lane * E + e, ks = (dch >> 6) * 4 + ((dch >> 2) & 3), tt = (dch >> 4) & 3, w = dch & 3;
-        __half* slot = reinterpret_cast<__half*>(&sm.qf[ks][(r & 7) * 4 + tt]);  // a0, a1, a2, a3 as 8 halves
         const float y = x[e] * mul;
         const __half hi = __float2half_rn(y);
-        const int at = (w >> 1) * 4 + (w & 1);  // a0 or a2
-        if (HL) {
-          slot[at] = hi;
-          slot[at + 2] = __float2half_rn(y - __half2float(hi));  // an infinite y gives NaN, as it should
-        } else {
-          slot[at + (r >> 3) * 2] = hi;
-        }
+        reinterpret_cast<__half*>(&sm.qf[LO ? 0 : r >> 3][ks][(r & 7) * 4 + tt])[w] = hi;
+        if (LO)  // an infinite y gives NaN, as it should
+          reinterpret_cast<__half*>(&sm.qf[1][ks][(r & 7) * 4 + tt])[w] = __float2half_rn(y - __half2float(hi));
       }
     }
     __syncthreads();
-    float rm[2];
-    int vis[2];  // positions below vis are seen by the row
+    uint2 qreg[NB == 1 && !LO ? KS : 1];  // one row group's Q stays in registers, two are read as needed
+    if (NB == 1 && !LO)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = g + 8 * i;
-      const bool live = r < nrow;  // HL: row 1 of the lane is the low half of row 0
-      rm[i] = live ? sm.rowmul[HL ? g : r] : 0.f;
-      vis[i] = live ? (int)min((int64_t)L + (f0 + r) / a.group + 1, (int64_t)cap) : 0;
-    }
+      for (int k = 0; k < KS; ++k) qreg[k] = sm.qf[0][k][lane];
+    float rm[NB][2];
+    int vis[NB][2];  // positions below vis are seen by the row
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = n * 8 + 2 * t4 + e;
+        const bool live = r < nrow;
+        rm[n][e] = live ? sm.rowmul[r] : 0.f;
+        vis[n][e] = live ? (int)min((int64_t)L + (f0 + r) / a.group + 1, (int64_t)cap) : 0;
+      }
     const int all_see = (int)min((int64_t)L + f0 / a.group + 1, (int64_t)cap);  // positions every row sees
+    float* score_row = a.scores ? a.scores + (((int64_t)b * c.n_kv + h) * a.rows + f0) * cap : nullptr;
 
-    float o[NT][4];
+    float o[NB][MT][4];  // O^T: channels g HD/8 + 2 u, + 1 (c0 c1, c2 c3) of rows 2 t4, 2 t4 + 1
 #pragma unroll
-    for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-    constexpr int NR = HL ? 1 : 2;  // rows a lane answers for
-    float m_run[NR], mo_run[NR], l_run[NR];
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
-    for (int i = 0; i < NR; ++i) { m_run[i] = mo_run[i] = -INFINITY; l_run[i] = 0.f; }
+      for (int k = 0; k < MT; ++k) o[n][k][0] = o[n][k][1] = o[n][k][2] = o[n][k][3] = 0.f;
+    float m_ref[NB][2], mo_ref[NB][2], fm[NB][2], l_run[NB][2];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) { m_ref[n][e] = mo_ref[n][e] = -INFINITY; fm[n][e] = l_run[n][e] = 0.f; }
 
-    for (int qi = 0; qi < n_tile; ++qi) {
-      cp_wait<ST - 2>();
-      __syncwarp();
-      const int st = qi % ST;
-      const uint8_t* kt = sm.ring[warp][st];
-      const uint8_t* vt = kt + G::K_BYTES;
-      const float ksc = sm.sc[warp][st][0], vsc = sm.sc[warp][st][1];
-      const bool tile_ok = sm.ok[warp][st];
-      const int p0 = (ta + warp + qi * KD_WARPS) * KD_TILE;
-
-      // ---- S = Q K^T ----
-      float s[2][4];
+    for (int qi = 0; qi < n_tile; qi += TT) {
+      __syncwarp();  // every lane is done with the buffers that the next copies go to
 #pragma unroll
-      for (int i = 0; i < 2; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
-#pragma unroll
-      for (int j = 0; j < G::KCH; ++j) {
-        const uint4 k0 = *reinterpret_cast<const uint4*>(kt + j * 512 + lane * 16);
-        const uint4 k1 = *reinterpret_cast<const uint4*>(kt + (G::KCH + j) * 512 + lane * 16);
-        const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint4 qa = sm.qf[j * 4 + e][lane];
-          const uint32_t x0 = code_word<CODE>(w0[e]), x1 = code_word<CODE>(w1[e]);
-          mma16816(s[0], qa, codes2<CODE, 0>(x0), codes2<CODE, 1>(x0));
-          mma16816(s[1], qa, codes2<CODE, 0>(x1), codes2<CODE, 1>(x1));
-        }
-      }
-      // ---- base-2 scores x of keys p0 + 4 t4 + 0..3 ----
-      float x[NR][4];
-#pragma unroll
-      for (int i = 0; i < NR; ++i) {
-        const float f = rm[i] * ksc;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float raw = HL ? s[e >> 1][e & 1] + s[e >> 1][2 + (e & 1)] : s[e >> 1][2 * i + (e & 1)];
-          x[i][e] = raw * f;
-        }
-      }
-      if (p0 + KD_TILE > all_see || !tile_ok) {
-#pragma unroll
-        for (int i = 0; i < NR; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (p0 + 4 * t4 + e >= vis[i] || !tile_ok) x[i][e] = -INFINITY;
-      }
-      if (a.scores) {
-#pragma unroll
-        for (int i = 0; i < NR; ++i)
-          if (g + 8 * i < nrow)
-            *reinterpret_cast<float4*>(a.scores + (((int64_t)b * c.n_kv + h) * a.rows + f0 + g + 8 * i) * cap + p0 + 4 * t4) =
-                make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
-      }
-      // ---- online softmax: sums against m_run, weights times V's scale against mo_run ----
-      const float lv = lg2(vsc);
-      float w[NR][4];
-      bool grew = false;
-      float al[NR];
-#pragma unroll
-      for (int i = 0; i < NR; ++i) {
-        float mt = fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3]));
-        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
-        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
-        const float mn = fmaxf(m_run[i], mt), ms = mn == -INFINITY ? 0.f : mn;
-        float ps = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) ps += ex2(x[i][e] - ms);
-        l_run[i] = l_run[i] * ex2(m_run[i] - ms) + ps;
-        m_run[i] = mn;
-        const float mo = fmaxf(mo_run[i], mt + lv), mos = mo == -INFINITY ? 0.f : mo;
-        al[i] = ex2(mo_run[i] - mos);
-        grew |= mo > mo_run[i];
-        mo_run[i] = mo;
-        const float off = lv - mos;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[i][e] = ex2(x[i][e] + off);
-      }
-      if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          o[n][0] *= al[0]; o[n][1] *= al[0];
-          o[n][2] *= al[NR - 1]; o[n][3] *= al[NR - 1];
-        }
-      }
-      uint4 pa;  // a0, a1: keys 4 t4, 4 t4 + 1 of rows g, g + 8; a2, a3: keys 4 t4 + 2, + 3
-      if (HL) {
-        pa.x = pack_h2(w[0][0], w[0][1]);
-        pa.z = pack_h2(w[0][2], w[0][3]);
-        const float2 f0h = __half22float2(*reinterpret_cast<__half2*>(&pa.x)), f1h = __half22float2(*reinterpret_cast<__half2*>(&pa.z));
-        pa.y = pack_h2(w[0][0] - f0h.x, w[0][1] - f0h.y);
-        pa.w = pack_h2(w[0][2] - f1h.x, w[0][3] - f1h.y);
-      } else {
-        pa.x = pack_h2(w[0][0], w[0][1]); pa.y = pack_h2(w[NR - 1][0], w[NR - 1][1]);
-        pa.z = pack_h2(w[0][2], w[0][3]); pa.w = pack_h2(w[NR - 1][2], w[NR - 1][3]);
-      }
-      // ---- O += P V ----
-      constexpr int VW = G::VB / 4;  // words a key
-      uint32_t v[4][VW];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t* src = vt + i * 32 * G::VB + lane * G::VB;
-        if (VW == 4) {
-          const uint4 y = *reinterpret_cast<const uint4*>(src);
-          v[i][0] = y.x; v[i][1] = y.y; v[i][VW - 2] = y.z; v[i][VW - 1] = y.w;
-        } else {
-          const uint2 y = *reinterpret_cast<const uint2*>(src);
-          v[i][0] = y.x; v[i][1] = y.y;
-        }
-        if (p0 + KD_TILE > total && p0 + 4 * t4 + i >= total) {  // rows never written may hold NaN codes
-#pragma unroll
-          for (int k = 0; k < VW; ++k) v[i][k] = 0u;
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < VW; ++k) {
-        const uint32_t v0 = code_word<CODE>(v[0][k]), v1 = code_word<CODE>(v[1][k]);
-        const uint32_t v2 = code_word<CODE>(v[2][k]), v3 = code_word<CODE>(v[3][k]);
-        const uint32_t a01 = __byte_perm(v0, v1, 0x5140), b01 = __byte_perm(v0, v1, 0x7362);
-        const uint32_t a23 = __byte_perm(v2, v3, 0x5140), b23 = __byte_perm(v2, v3, 0x7362);
-        mma16816(o[4 * k + 0], pa, codes2<CODE, 0>(a01), codes2<CODE, 0>(a23));
-        mma16816(o[4 * k + 1], pa, codes2<CODE, 1>(a01), codes2<CODE, 1>(a23));
-        mma16816(o[4 * k + 2], pa, codes2<CODE, 0>(b01), codes2<CODE, 0>(b23));
-        mma16816(o[4 * k + 3], pa, codes2<CODE, 1>(b01), codes2<CODE, 1>(b23));
-      }
-      __syncwarp();  // every lane is done with the buffer that the next copies go to
-      if (qi + ST - 1 < n_tile) issue(qi + ST - 1);
+      for (int tt = 0; tt < TT; ++tt)
+        if (qi + ST - TT + tt < n_tile) issue(qi + ST - TT + tt);
       cp_commit();
+      cp_wait<ST / TT - 1>();  // the group of tiles qi.. has landed
+      __syncwarp();
+      float y[TT][NB][4];  // base-2 scores: key g (0, 1) and g + 8 (2, 3) of rows 2 t4, 2 t4 + 1
+      float vsc[TT], lv[TT];
+      int p0[TT];
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) {
+        const int st = (qi + tt) % ST;
+        const bool live = qi + tt < n_tile;
+        const bool seen = live && sm.ok[warp][st];
+        p0[tt] = live ? (ta + warp + (qi + tt) * KD_WARPS) * KD_TILE : 0x40000000;
+        const float ksc = seen ? sm.sc[warp][st][0] : 0.f;
+        vsc[tt] = seen ? sm.sc[warp][st][1] : 0.f;
+        lv[tt] = lg2(vsc[tt]);
+        const uint8_t* kt = sm.ring[warp][st];
+        float s[G::KCH][NB][4];
+#pragma unroll
+        for (int j = 0; j < G::KCH; ++j) {
+#pragma unroll
+          for (int n = 0; n < NB; ++n) s[j][n][0] = s[j][n][1] = s[j][n][2] = s[j][n][3] = 0.f;
+          const uint4 k0 = *reinterpret_cast<const uint4*>(kt + j * 512 + lane * 16);
+          const uint4 k1 = *reinterpret_cast<const uint4*>(kt + (G::KCH + j) * 512 + lane * 16);
+          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t x0 = code_word<CODE>(w0[e]), x1 = code_word<CODE>(w1[e]);
+            const uint4 ka = make_uint4(codes2<CODE, 0>(x0), codes2<CODE, 0>(x1), codes2<CODE, 1>(x0), codes2<CODE, 1>(x1));
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+              const uint2 q = NB == 1 && !LO ? qreg[NB == 1 && !LO ? j * 4 + e : 0] : sm.qf[n][j * 4 + e][lane];
+              mma16816(s[j][n], ka, q.x, q.y);
+              if (LO) {
+                const uint2 ql = sm.qf[1][j * 4 + e][lane];
+                mma16816(s[j][n], ka, ql.x, ql.y);
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float raw = G::KCH == 2 ? s[0][n][e] + s[G::KCH - 1][n][e] : s[0][n][e];
+            y[tt][n][e] = raw * (rm[n][e & 1] * ksc);
+          }
+        if (p0[tt] + KD_TILE > all_see || !seen) {
+#pragma unroll
+          for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (p0[tt] + g + 8 * (e >> 1) >= vis[n][e & 1] || !seen) y[tt][n][e] = -INFINITY;
+        }
+        if (score_row && live) {
+#pragma unroll
+          for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int r = n * 8 + 2 * t4 + (e & 1);
+              if (r < nrow) score_row[(int64_t)r * cap + p0[tt] + g + 8 * (e >> 1)] = y[tt][n][e];
+            }
+        }
+      }
+      // ---- move the references when a weight would exceed them by 2^KD_SLACK ----
+      bool move = false;
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = -INFINITY, mv = -INFINITY;
+#pragma unroll
+          for (int tt = 0; tt < TT; ++tt) {
+            const float x = fmaxf(y[tt][n][e], y[tt][n][e + 2]);
+            mx = fmaxf(mx, x);
+            mv = fmaxf(mv, x + lv[tt]);
+          }
+          move |= mx > m_ref[n][e] + KD_SLACK || mv > mo_ref[n][e] + KD_SLACK;
+        }
+      if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = m_ref[n][e], mv = mo_ref[n][e];
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) {
+              const float x = fmaxf(y[tt][n][e], y[tt][n][e + 2]);
+              mx = fmaxf(mx, x);
+              mv = fmaxf(mv, x + lv[tt]);
+            }
+#pragma unroll
+            for (int k = 4; k < 32; k <<= 1) {
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+              mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, k));
+            }
+            if (mx != m_ref[n][e]) {  // from -infinity: the sums are still 0
+              l_run[n][e] *= ex2(m_ref[n][e] - mx);
+              m_ref[n][e] = mx;
+            }
+            if (mv != mo_ref[n][e]) {
+              const float f = ex2(mo_ref[n][e] - mv);
+#pragma unroll
+              for (int k = 0; k < MT; ++k) { o[n][k][e] *= f; o[n][k][e + 2] *= f; }
+              mo_ref[n][e] = mv;
+            }
+            fm[n][e] = mv == -INFINITY ? 0.f : ex2(mx - mv);
+          }
+      }
+      // ---- O^T += V^T P^T ----
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) {
+        const uint8_t* vt = sm.ring[warp][(qi + tt) % ST] + G::K_BYTES;
+        uint32_t pb[NB][2], pl[NB][2];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float m = m_ref[n][e & 1];
+            const float pe = ex2(y[tt][n][e] - (m == -INFINITY ? 0.f : m));
+            l_run[n][e & 1] += pe;
+            w[e] = pe * (vsc[tt] * fm[n][e & 1]);
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t hi = pack_h2(w[2 * i], w[2 * i + 1]);
+            pb[n][i] = transpose8(hi);
+            if (LO) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+              pl[n][i] = transpose8(pack_h2(w[2 * i] - f.x, w[2 * i + 1] - f.y));
+            }
+          }
+        }
+        constexpr int VW = G::VB / 4;  // words a key
+        uint32_t v[4][VW];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint8_t* src = vt + i * 32 * G::VB + lane * G::VB;
+          if (VW == 4) {
+            const uint4 x = *reinterpret_cast<const uint4*>(src);
+            v[i][0] = x.x; v[i][1] = x.y; v[i][VW - 2] = x.z; v[i][VW - 1] = x.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(src);
+            v[i][0] = x.x; v[i][1] = x.y;
+          }
+        }
+        if (p0[tt] + KD_TILE > total) {  // rows never written may hold NaN codes
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (p0[tt] + 2 * t4 + (i & 1) + 8 * (i >> 1) >= total)
+#pragma unroll
+              for (int k = 0; k < VW; ++k) v[i][k] = 0u;
+        }
+#pragma unroll
+        for (int k = 0; k < VW; ++k) {
+          const uint32_t v0 = code_word<CODE>(v[0][k]), v1 = code_word<CODE>(v[1][k]);
+          const uint32_t v2 = code_word<CODE>(v[2][k]), v3 = code_word<CODE>(v[3][k]);
+          const uint32_t a01 = __byte_perm(v0, v1, 0x5140), b01 = __byte_perm(v0, v1, 0x7362);
+          const uint32_t a23 = __byte_perm(v2, v3, 0x5140), b23 = __byte_perm(v2, v3, 0x7362);
+          const uint4 va = make_uint4(codes2<CODE, 0>(a01), codes2<CODE, 1>(a01), codes2<CODE, 0>(a23), codes2<CODE, 1>(a23));
+          const uint4 vb = make_uint4(codes2<CODE, 0>(b01), codes2<CODE, 1>(b01), codes2<CODE, 0>(b23), codes2<CODE, 1>(b23));
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            mma16816(o[n][2 * k], va, pb[n][0], pb[n][1]);
+            mma16816(o[n][2 * k + 1], vb, pb[n][0], pb[n][1]);
+            if (LO) {
+              mma16816(o[n][2 * k], va, pl[n][0], pl[n][1]);
+              mma16816(o[n][2 * k + 1], vb, pl[n][0], pl[n][1]);
+            }
+          }
+        }
+      }
     }
     cp_wait<0>();
 
     // ---- join the warps ----
 #pragma unroll
-    for (int i = 0; i < NR; ++i) {
-      l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 1);
-      l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 2);
-      if (t4 == 0) {
-        sm.wm[warp][g + 8 * i] = m_run[i];
-        sm.wmo[warp][g + 8 * i] = mo_run[i];
-        sm.wl[warp][g + 8 * i] = l_run[i];
-      }
-    }
-    __syncthreads();  // all tiles are read: the ring takes the outputs
-    float* wo = reinterpret_cast<float*>(&sm.ring[0][0][0]);  // [warp][row][OSTRIDE], channel n VB + u at u * 8 + n
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float* d0 = wo + (warp * RG + g) * G::OSTRIDE + n * 8 + 2 * t4;
-      if (HL) {
-        *reinterpret_cast<float2*>(d0) = make_float2(o[n][0] + o[n][2], o[n][1] + o[n][3]);
-      } else {
-        *reinterpret_cast<float2*>(d0) = make_float2(o[n][0], o[n][1]);
-        *reinterpret_cast<float2*>(d0 + 8 * G::OSTRIDE) = make_float2(o[n][2], o[n][3]);
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int k = 4; k < 32; k <<= 1) l_run[n][e] += __shfl_xor_sync(0xffffffffu, l_run[n][e], k);
+        if (g == 0) {
+          const int r = n * 8 + 2 * t4 + e;
+          sm.wm[warp][r] = m_ref[n][e];
+          sm.wmo[warp][r] = mo_ref[n][e];
+          sm.wl[warp][r] = l_run[n][e];
+        }
       }
-    }
+    __syncthreads();  // all tiles are read: the ring takes the outputs
+    float* wo = reinterpret_cast<float*>(&sm.ring[0][0][0]);  // [warp][row][OSTRIDE]
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int k = 0; k < MT; ++k)
+          *reinterpret_cast<float2*>(wo + (warp * RG + n * 8 + 2 * t4 + e) * G::OSTRIDE + g * G::VB + 2 * k) =
+              make_float2(o[n][k][e], o[n][k][e + 2]);
     __syncthreads();
     const bool whole = ta == 0 && te == units;
     const int slot = 2 * cta + (ta == 0 ? 1 : 0);
@@ -450,31 +520,36 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
         sm.wmo[k][tid] = ex2(sm.wmo[k][tid] - mos);
       }
       sm.tot[tid][0] = Mo; sm.tot[tid][1] = M; sm.tot[tid][2] = l;
-      if (!whole && tid < nrow) {
-        float* ml = a.part_ml + ((int64_t)slot * RG + tid) * 4;
-        ml[0] = Mo; ml[1] = M; ml[2] = l;
-      }
+      if (!whole && tid < nrow)
+        *reinterpret_cast<float4*>(a.part_ml + ((int64_t)slot * RG + tid) * 4) = make_float4(Mo, M, l, 0.f);
     }
     __syncthreads();
     const int64_t ob = (int64_t)b * a.tokens;
-    auto finish = [&](int r, int d, float num) {  // the answer of row r, channel d
+    auto finish = [&](int r, int d, const float4& num) {  // the answer of row r, channels d..d + 3
       const float Mo = sm.tot[r][0], M = sm.tot[r][1], l = sm.tot[r][2];
-      const float y = l == 0.f ? 0.f : num * (Mo == -INFINITY ? 0.f : ex2(Mo - M)) / l;  // a NaN query: NaN
-      const int f = f0 + r;
-      kv8_store1(a.out, (ob + f / a.group) * a.ldo + (int64_t)(h * a.group + f % a.group) * HD + d, a.dtype, y);
+      const float f = l == 0.f ? 0.f : (Mo == -INFINITY ? 0.f : ex2(Mo - M)) / l;  // a NaN query: NaN
+      const int64_t at = (ob + (f0 + r) / a.group) * a.ldo + (int64_t)(h * a.group + (f0 + r) % a.group) * HD + d;
+      kv8_store1(a.out, at, a.dtype, num.x * f);
+      kv8_store1(a.out, at + 1, a.dtype, num.y * f);
+      kv8_store1(a.out, at + 2, a.dtype, num.z * f);
+      kv8_store1(a.out, at + 3, a.dtype, num.w * f);
     };
     auto store_lse = [&]() {
       if (a.lse && tid < nrow)
         a.lse[((int64_t)b * c.n_kv + h) * a.rows + f0 + tid] =
             sm.tot[tid][2] == 0.f ? INFINITY : sm.tot[tid][1] + lg2(sm.tot[tid][2]);
     };
-    for (int i = tid; i < nrow * HD; i += KD_THREADS) {
-      const int r = i / HD, d = i % HD, at = (d % G::VB) * 8 + d / G::VB;
-      float num = 0.f;
+    for (int i = tid; i < nrow * (HD / 4); i += KD_THREADS) {
+      const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+      float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int k = 0; k < KD_WARPS; ++k) num = fmaf(wo[(k * RG + r) * G::OSTRIDE + at], sm.wmo[k][r], num);
+      for (int k = 0; k < KD_WARPS; ++k) {
+        const float4 x = *reinterpret_cast<const float4*>(wo + (k * RG + r) * G::OSTRIDE + d);
+        const float f = sm.wmo[k][r];
+        num.x = fmaf(x.x, f, num.x); num.y = fmaf(x.y, f, num.y); num.z = fmaf(x.z, f, num.z); num.w = fmaf(x.w, f, num.w);
+      }
       if (whole) finish(r, d, num);
-      else a.part[((int64_t)slot * RG + r) * HD + d] = num;
+      else *reinterpret_cast<float4*>(a.part + ((int64_t)slot * RG + r) * HD + d) = num;
     }
     if (whole) {
       store_lse();
@@ -493,27 +568,35 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
     if (!sm.flag) continue;
     __threadfence();
     float* wts = wo;  // [row][part]
+    auto part_of = [&](int k) { return (int64_t)(2 * (c0 + k) + (k == 0)) * RG; };  // its first row
     for (int r = warp; r < nrow; r += KD_WARPS) {
-      auto ml = [&](int k, int j) { return __ldcg(a.part_ml + ((int64_t)(2 * (c0 + k) + (k == 0)) * RG + r) * 4 + j); };
       float M = -INFINITY, Mo = -INFINITY, l = 0.f;
-      for (int k = lane; k < parts; k += 32) { Mo = fmaxf(Mo, ml(k, 0)); M = fmaxf(M, ml(k, 1)); }
+      for (int k = lane; k < parts; k += 32) {
+        const float4 ml = __ldcg(reinterpret_cast<const float4*>(a.part_ml) + part_of(k) + r);
+        Mo = fmaxf(Mo, ml.x);
+        M = fmaxf(M, ml.y);
+      }
       M = warp_max(M);
       Mo = warp_max(Mo);
       const float ms = M == -INFINITY ? 0.f : M, mos = Mo == -INFINITY ? 0.f : Mo;
       for (int k = lane; k < parts; k += 32) {
-        l += ml(k, 2) * ex2(ml(k, 1) - ms);
-        wts[r * parts + k] = ex2(ml(k, 0) - mos);
+        const float4 ml = __ldcg(reinterpret_cast<const float4*>(a.part_ml) + part_of(k) + r);
+        l += ml.z * ex2(ml.y - ms);
+        wts[r * parts + k] = ex2(ml.x - mos);
       }
       l = warp_sum(l);
       if (lane == 0) { sm.tot[r][0] = Mo; sm.tot[r][1] = M; sm.tot[r][2] = l; }
     }
     __syncthreads();
-    for (int i = tid; i < nrow * HD; i += KD_THREADS) {
-      const int r = i / HD, d = i % HD;
-      float num = 0.f;
+    for (int i = tid; i < nrow * (HD / 4); i += KD_THREADS) {
+      const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+      float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-      for (int k = 0; k < parts; ++k)
-        num = fmaf(__ldcg(a.part + ((int64_t)(2 * (c0 + k) + (k == 0)) * RG + r) * HD + d), wts[r * parts + k], num);
+      for (int k = 0; k < parts; ++k) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(a.part + (part_of(k) + r) * HD + d));
+        const float f = wts[r * parts + k];
+        num.x = fmaf(x.x, f, num.x); num.y = fmaf(x.y, f, num.y); num.z = fmaf(x.z, f, num.z); num.w = fmaf(x.w, f, num.w);
+      }
       finish(r, d, num);
     }
     store_lse();
@@ -560,7 +643,8 @@ struct KDPlan {
 static KDPlan kd_plan(const N730KV8Cache& c, int batch, int tokens, int heads, int dtype, bool weights) {
   KDPlan p{};
   const int64_t rows = (int64_t)tokens * (heads / c.n_kv);
-  p.rg = dtype == N730_F32 ? 8 : 16;
+  // fp32 rows take both terms' products, and up to 8 rows need no second group of columns
+  p.rg = dtype == N730_F32 || rows <= 8 ? 8 : 16;
   p.nrg = (int)((rows + p.rg - 1) / p.rg);
   p.n_cta = KD_CTAS_PER_SM * num_sms();
   auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
@@ -589,11 +673,11 @@ int64_t kv8_attention_ws(const N730KV8Cache& c, int batch, int tokens, int heads
                   kd_plan(c, batch, tokens, heads, N730_F16, weights).bytes);
 }
 
-template <int HD, int CODE, bool HL>
+template <int HD, int CODE, int NB, bool LO>
 static int split_launch(const KDArgs& a, bool pdl, cudaStream_t st) {
   const size_t smem = sizeof(KDSmem<HD>) + (size_t)a.batch * 4;
-  if (int rc = smem_attr_once<kv8_split_kernel<HD, CODE, HL>>((int)(sizeof(KDSmem<HD>) + KD_MAX_BATCH * 4))) return rc;
-  return kv8_launch(kv8_split_kernel<HD, CODE, HL>, dim3(a.n_cta), dim3(KD_THREADS), smem, st, pdl, a);
+  if (int rc = smem_attr_once<kv8_split_kernel<HD, CODE, NB, LO>>((int)(sizeof(KDSmem<HD>) + KD_MAX_BATCH * 4))) return rc;
+  return kv8_launch(kv8_split_kernel<HD, CODE, NB, LO>, dim3(a.n_cta), dim3(KD_THREADS), smem, st, pdl, a);
 }
 
 int kv8_attention_launch(const KV8AttnCall& k, cudaStream_t st) {
@@ -615,9 +699,11 @@ int kv8_attention_launch(const KV8AttnCall& k, cudaStream_t st) {
   a.scores = weights ? reinterpret_cast<float*>(ws + p.scores) : nullptr;
   a.n_cta = p.n_cta;
   a.log_block = c.block == 16 ? 4 : c.block == 32 ? 5 : 6;
-  const bool hl = k.dtype == N730_F32;
   int rc;
-#define N730_SPLIT(HD, CODE) (hl ? split_launch<HD, CODE, true>(a, k.pdl, st) : split_launch<HD, CODE, false>(a, k.pdl, st))
+#define N730_SPLIT(HD, CODE)                                                 \
+  (k.dtype == N730_F32 ? split_launch<HD, CODE, 1, true>(a, k.pdl, st)       \
+   : p.rg == 8         ? split_launch<HD, CODE, 1, false>(a, k.pdl, st)      \
+                       : split_launch<HD, CODE, 2, false>(a, k.pdl, st))
   if (c.head_dim == 128) rc = c.code == N730_KV8_INT8 ? N730_SPLIT(128, N730_KV8_INT8) : N730_SPLIT(128, N730_KV8_E4M3);
   else rc = c.code == N730_KV8_INT8 ? N730_SPLIT(64, N730_KV8_INT8) : N730_SPLIT(64, N730_KV8_E4M3);
 #undef N730_SPLIT
