@@ -3,11 +3,11 @@
 //   out[b, t, head] = softmax_p(scale q . k_p) v_p,  positions p <= lens[b] + t of KV head head / G
 //
 // Split kernel (single tokens and few rows).  The rows of an item (sequence, KV head) are its
-// tokens x G query heads, 8 or 16 at a time.  All items' 16-position tiles form one line that the
+// tokens x G query heads, 8 or 16 at a time.  All items' 32-position tiles form one line that the
 // CTAs cut into equal runs, so ragged lengths and few sequences load every SM alike; a run that
 // covers part of an item leaves its (max, sum, output) in the workspace, and the last CTA to finish
 // an item joins the parts in run order (the result does not depend on which CTA that is).  Within a
-// CTA each warp takes every fourth tile, two of them at a time.
+// CTA each warp takes every fourth tile.
 //
 // The products are transposed, so that a key or a channel is a row of mma.m16n8k16's A and the few
 // query rows are its 8 columns: no half of an instruction works on rows that are not there.
@@ -15,8 +15,10 @@
 //      bytes of keys g and g + 8, each 4 of them one k-step's slots.
 //   O^T = V^T P^T: lane (g, t) feeds 16 contiguous channels of keys 2t, 2t+1, 2t+8, 2t+9,
 //      interleaved by byte permutes; P^T comes from S^T by an 8x8 transposition between lanes.
-// A lane copies into shared memory, with cp.async, exactly the bytes that it later feeds to the
-// tensor cores: tiles need no CTA barrier and no transposition through shared memory.
+// Each warp fills its own two tile buffers with tensor copies (no barrier between warps in the loop).
+// Rows of 128 (64) bytes lie swizzled, and the order of the 16 keys of a product is chosen so that
+// the lanes of one shared-memory wavefront meet no bank twice in either product (key_of).  Copies
+// of 16 bytes per lane (cp.async) in fragment order reached 4.1 TB/s even without any arithmetic.
 // int8 codes become fp16 exactly (1024 + 128 + q by a byte permute, then one subtraction), e4m3
 // codes by a conversion.  K's scale multiplies the scores, V's scale the weights.
 //
@@ -29,6 +31,10 @@
 // is rounded to fp16 (2^-11 of each weight, below the rounding of the output).  Maxima, sums and
 // outputs are fp32.
 #include <algorithm>
+#include <mutex>
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
 
 #include "kv8.h"
 
@@ -36,12 +42,13 @@ namespace n730 {
 
 constexpr int KD_WARPS = 4;
 constexpr int KD_THREADS = KD_WARPS * 32;
-constexpr int KD_STAGES = 4;     // tile buffers of a warp
-constexpr int KD_TILE = 16;      // positions
+constexpr int KD_STAGES = 2;     // tile buffers of a warp
+constexpr int KD_TILE = 32;      // positions
 constexpr int KD_CTAS_PER_SM = 3;
-constexpr int KD_MIN_UNITS = 8;  // tiles of a run: fewer would leave warps idle and joins to do
+constexpr int KD_MIN_UNITS = 4;  // tiles of a run: fewer would leave warps idle and joins to do
 constexpr int KD_MAX_BATCH = 4096;
 constexpr float KD_SLACK = 8.f;  // log2 of how far a weight may exceed its reference
+constexpr uint64_t KD_WAIT_NS = 1000000000;  // bound of a wait for copies
 
 struct KDArgs {
   N730KV8Cache c;
@@ -50,29 +57,40 @@ struct KDArgs {
   int dtype, batch, tokens, heads, group, rows, nrg;  // rows = tokens * group; nrg row groups of RG
   float scale_log2e;
   const int* lens; const int* n_new;
+  int* status;         // set when a wait ran out
   unsigned* cnt;       // [batch][n_kv][nrg] arrivals, zero between calls
   float* part;         // [2 * n_cta][RG][HD]
   float* part_ml;      // [2 * n_cta][RG][4]: reference of the output, max, sum
   float* lse;          // [batch][n_kv][rows] log2 of the softmax sum, +inf for an empty row (weights only)
   float* scores;       // [batch][n_kv][rows][cap] base-2 scores (weights only)
-  int n_cta, log_block;
+  int n_cta, log_block, box;  // box: rows of a copy, 32, or 16 where pages are no multiples of 32
 };
 
 template <int HD>
 struct KDGeom {
-  static constexpr int KCH = HD / 64;                 // 16-byte K chunks per lane and 8 keys
+  static constexpr int KCH = HD / 64;                 // 16-byte K chunks per lane and key
   static constexpr int VB = HD / 8;                   // V bytes per lane and key
-  static constexpr int K_BYTES = 2 * KCH * 512;       // per tile
-  static constexpr int TILE_BYTES = K_BYTES + 4 * VB * 32;
+  static constexpr int KV_BYTES = KD_TILE * HD;       // K (or V) codes of a tile
+  static constexpr int TILE_BYTES = 2 * KV_BYTES;
   static constexpr int OSTRIDE = HD + 4;              // padded output row (bank spread, 16-byte rows)
+  // byte of 16-byte chunk c of row r: the copies' 128-byte (64-byte) swizzle
+  static __device__ __forceinline__ int chunk(int r, int c) {
+    return HD == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+  }
+  // row of the i-th key of the first 8 of a product (the second 8: + 8)
+  static __device__ __forceinline__ int key_of(int i) {
+    const int e = HD == 128 ? i & 6 : ((i >> 1) & 1) + ((i >> 2) << 2);  // even i: 0 2 4 6, or 0 1 4 5
+    return (i & 1) == 0 ? e : HD == 128 ? (e ^ 4) + 1 : e ^ 3;
+  }
 };
 
 template <int HD>
 struct KDSmem {
   uint8_t ring[KD_WARPS][KD_STAGES][KDGeom<HD>::TILE_BYTES];
   uint2 qf[2][HD / 16][32];        // Q^T as the B operand by k-step and lane: rows 8-15 or low terms second
-  float sc[KD_WARPS][KD_STAGES][2];
-  int ok[KD_WARPS][KD_STAGES];
+  uint64_t full[KD_WARPS][KD_STAGES];
+  float sc[KD_WARPS][KD_STAGES][4];  // scales of K, V of the tile's two halves
+  int ok[KD_WARPS][KD_STAGES];     // bit i: half i has a page
   float rowmul[16];
   float wm[KD_WARPS][16], wmo[KD_WARPS][16], wl[KD_WARPS][16];
   float tot[16][4];
@@ -103,6 +121,20 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
+}
+// 2-D tensor copy (no multicast) of the box whose first row is `row`, completing on `bar`
+__device__ __forceinline__ void copy_rows(uint32_t dst, const CUtensorMap* map, int row, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(smem_u32(bar)) : "memory");
+}
+// Bounded wait for the phase of `bar`; no time is spent once a wait of the thread has run out.
+__device__ __forceinline__ bool wait_copies(uint64_t* bar, uint32_t parity, bool lost) {
+  if (mbar_try_wait(bar, parity)) return true;
+  auto now = [] { uint64_t t; asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t)); return t; };
+  const uint64_t t0 = now();
+  while (!mbar_try_wait(bar, parity))
+    if (lost || now() - t0 > KD_WAIT_NS) return false;
+  return true;
 }
 template <int BYTES>
 __device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool pred) {
@@ -141,17 +173,23 @@ __device__ __forceinline__ int kd_units(const KDArgs& a, int b, int cap) {
 
 // NB: 8-row groups of an item's rows worked on together; LO: fp32 rows in two fp16 terms.
 template <int HD, int CODE, int NB, bool LO>
-__global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(const KDArgs a) {
+__global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(const KDArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using G = KDGeom<HD>;
   constexpr int RG = 8 * NB, KS = HD / 16, MT = HD / 16, ST = KD_STAGES;
-  constexpr int TT = NB == 1 ? 2 : 1;  // tiles worked on together: independent chains for the tensor cores
-  extern __shared__ __align__(128) uint8_t kd_raw[];
-  KDSmem<HD>& sm = *reinterpret_cast<KDSmem<HD>*>(kd_raw);
+  constexpr int TT = NB == 1 ? 2 : 1;  // halves of a tile worked on together: independent chains for the tensor cores
+  extern __shared__ __align__(1024) uint8_t kd_raw[];
+  KDSmem<HD>& sm = *reinterpret_cast<KDSmem<HD>*>((reinterpret_cast<uintptr_t>(kd_raw) + 1023) & ~uintptr_t(1023));
   static_assert(sizeof(float) * KD_WARPS * RG * G::OSTRIDE <= sizeof(sm.ring), "per-warp outputs fit the ring");
-  static_assert(ST % TT == 0 && ST > TT, "whole groups of tiles in flight");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   const N730KV8Cache& c = a.c;
   const int cap = c.max_pages * c.page_size;
+  if (lane == 0) {
+    for (int s = 0; s < ST; ++s) mbar_init(&sm.full[warp][s], 1);
+    fence_mbar_init();
+  }
+  bool lost = false;   // a wait ran out
+  uint32_t fills = 0;  // tiles this warp has asked for, and used: buffer and phase go by them
+  uint32_t uses = 0;
   pdl_wait();
 
   // ---- prefix sums of the sequences' tiles ----
@@ -200,47 +238,58 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
     const int nrow = min(RG, rows_b - f0);
     const int total = (int)min((int64_t)L + n_new, (int64_t)cap);  // positions cached with the new rows
 
-    __syncthreads();  // shared memory of the previous run is free
+    // shared memory of the previous run is free; what its threads wrote there comes before new copies
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
     // ---- the warp's tiles ----
     const int n_tile = te - ta > warp ? (te - ta - warp + KD_WARPS - 1) / KD_WARPS : 0;
     const int* bt = c.block_table + (int64_t)b * c.max_pages;
-    // pool row of tile q0 + lane of this warp (-1: no page), looked up 32 tiles at a time
+    // pool row of half tile q0 + lane of this warp (-1: no page), looked up 16 tiles at a time
     auto lookup = [&](int q0) {
-      const int qi = q0 + lane;
-      if (qi >= n_tile) return -1;
-      const int p = (ta + warp + qi * KD_WARPS) * KD_TILE;
+      const int p = (ta + warp + ((q0 + lane) >> 1) * KD_WARPS) * KD_TILE + (lane & 1) * 16;
+      if (((q0 + lane) >> 1) >= n_tile || p >= total) return -1;
       const int page = bt[p / c.page_size];
       return (unsigned)page < (unsigned)c.n_pages ? (page * c.n_kv + h) * c.page_size + p % c.page_size : -1;
     };
     int rows_now = lookup(0), rows_next = lookup(32);
-    const uint32_t ring = smem_u32(sm.ring[warp]);
     auto issue = [&](int qi) {
-      const int st = qi % ST;
-      if (qi && (qi & 31) == 0) { rows_now = rows_next; rows_next = lookup(qi + 32); }
-      const int row = __shfl_sync(0xffffffffu, rows_now, qi & 31);
-      const bool ok = row >= 0;
-      const int64_t r0 = ok ? row : 0;
-      const uint32_t dst = ring + st * G::TILE_BYTES;
-      const uint8_t* kc = reinterpret_cast<const uint8_t*>(c.k_codes) + r0 * HD + g * HD + t4 * 16;
-      const uint8_t* vc = reinterpret_cast<const uint8_t*>(c.v_codes) + r0 * HD + 2 * t4 * HD + g * G::VB;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < G::KCH; ++j)
-          cp_async<16>(dst + (i * G::KCH + j) * 512 + lane * 16, kc + 8 * i * HD + j * 64, ok);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        cp_async<G::VB>(dst + G::K_BYTES + i * 32 * G::VB + lane * G::VB, vc + ((i & 1) + 8 * (i >> 1)) * HD, ok);
-      if (lane < 2) {
-        const float* s = (lane ? c.v_scales : c.k_scales) + (r0 >> a.log_block);
-        cp_async<4>(smem_u32(&sm.sc[warp][st][lane]), s, ok);
+      const int st = fills % ST;
+      ++fills;
+      if (qi && (qi & 15) == 0) { rows_now = rows_next; rows_next = lookup(2 * qi + 32); }
+      const int row0 = __shfl_sync(0xffffffffu, rows_now, (2 * qi) & 31);
+      const int row1 = __shfl_sync(0xffffffffu, rows_now, (2 * qi + 1) & 31);
+      if (lane == 0) {
+        const uint32_t dst = smem_u32(sm.ring[warp][st]);
+        uint64_t* bar = &sm.full[warp][st];
+        sm.ok[warp][st] = (row0 >= 0 ? 1 : 0) | (row1 >= 0 ? 2 : 0);
+        if (a.box == KD_TILE) {
+          mbar_arrive_expect_tx(bar, row0 >= 0 ? G::TILE_BYTES : 0);
+          if (row0 >= 0) {
+            copy_rows(dst, &kmap, row0, bar);
+            copy_rows(dst + G::KV_BYTES, &vmap, row0, bar);
+          }
+        } else {
+          mbar_arrive_expect_tx(bar, (row0 >= 0 ? G::KV_BYTES : 0) + (row1 >= 0 ? G::KV_BYTES : 0));
+          if (row0 >= 0) {
+            copy_rows(dst, &kmap, row0, bar);
+            copy_rows(dst + G::KV_BYTES, &vmap, row0, bar);
+          }
+          if (row1 >= 0) {
+            copy_rows(dst + G::KV_BYTES / 2, &kmap, row1, bar);
+            copy_rows(dst + G::KV_BYTES * 3 / 2, &vmap, row1, bar);
+          }
+        }
       }
-      if (lane == 0) sm.ok[warp][st] = ok;
+      if (lane < 4) {
+        const int row = lane < 2 ? row0 : row1;
+        const float* s = ((lane & 1) ? c.v_scales : c.k_scales) + (max(row, 0) >> a.log_block);
+        cp_async<4>(smem_u32(&sm.sc[warp][st][lane]), s, row >= 0);
+      }
     };
 #pragma unroll
-    for (int s = 0; s < ST - TT; ++s) {  // one group per TT tiles
+    for (int s = 0; s < ST - 1; ++s) {
       if (s < n_tile) issue(s);
-      if (s % TT == TT - 1) cp_commit();
+      cp_commit();
     }
 
     // ---- Q: a row per warp at a time, scaled by a power of two, as the B operand ----
@@ -289,6 +338,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
         vis[n][e] = live ? (int)min((int64_t)L + (f0 + r) / a.group + 1, (int64_t)cap) : 0;
       }
     const int all_see = (int)min((int64_t)L + f0 / a.group + 1, (int64_t)cap);  // positions every row sees
+    const int kg = G::key_of(g), kv0 = G::key_of(2 * t4), kv1 = G::key_of(2 * t4 + 1);
     float* score_row = a.scores ? a.scores + (((int64_t)b * c.n_kv + h) * a.rows + f0) * cap : nullptr;
 
     float o[NB][MT][4];  // O^T: channels g HD/8 + 2 u, + 1 (c0 c1, c2 c3) of rows 2 t4, 2 t4 + 1
@@ -302,34 +352,37 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
 #pragma unroll
       for (int e = 0; e < 2; ++e) { m_ref[n][e] = mo_ref[n][e] = -INFINITY; fm[n][e] = l_run[n][e] = 0.f; }
 
-    for (int qi = 0; qi < n_tile; qi += TT) {
-      __syncwarp();  // every lane is done with the buffers that the next copies go to
-#pragma unroll
-      for (int tt = 0; tt < TT; ++tt)
-        if (qi + ST - TT + tt < n_tile) issue(qi + ST - TT + tt);
+    for (int qi = 0; qi < n_tile; ++qi) {
+      __syncwarp();  // every lane is done with the buffer that the next copies go to
+      if (qi + ST - 1 < n_tile) issue(qi + ST - 1);
       cp_commit();
-      cp_wait<ST / TT - 1>();  // the group of tiles qi.. has landed
+      const int st = uses % ST;
+      if (!wait_copies(&sm.full[warp][st], (uses / ST) & 1, lost)) lost = true;
+      ++uses;
+      cp_wait<ST - 1>();
       __syncwarp();
-      float y[TT][NB][4];  // base-2 scores: key g (0, 1) and g + 8 (2, 3) of rows 2 t4, 2 t4 + 1
+      const int okm = sm.ok[warp][st];
+#pragma unroll
+      for (int t0 = 0; t0 < 2; t0 += TT) {
+      float y[TT][NB][4];  // base-2 scores: keys key_of(g) (0, 1) and + 8 (2, 3) of rows 2 t4, 2 t4 + 1
       float vsc[TT], lv[TT];
       int p0[TT];
 #pragma unroll
       for (int tt = 0; tt < TT; ++tt) {
-        const int st = (qi + tt) % ST;
-        const bool live = qi + tt < n_tile;
-        const bool seen = live && sm.ok[warp][st];
-        p0[tt] = live ? (ta + warp + (qi + tt) * KD_WARPS) * KD_TILE : 0x40000000;
-        const float ksc = seen ? sm.sc[warp][st][0] : 0.f;
-        vsc[tt] = seen ? sm.sc[warp][st][1] : 0.f;
+        const int half = t0 + tt;
+        const bool seen = (okm >> half) & 1;
+        p0[tt] = (ta + warp + qi * KD_WARPS) * KD_TILE + half * 16;
+        const float ksc = seen ? sm.sc[warp][st][2 * half] : 0.f;
+        vsc[tt] = seen ? sm.sc[warp][st][2 * half + 1] : 0.f;
         lv[tt] = lg2(vsc[tt]);
-        const uint8_t* kt = sm.ring[warp][st];
+        const uint8_t* kt = sm.ring[warp][st] + half * 16 * HD;
         float s[G::KCH][NB][4];
 #pragma unroll
         for (int j = 0; j < G::KCH; ++j) {
 #pragma unroll
           for (int n = 0; n < NB; ++n) s[j][n][0] = s[j][n][1] = s[j][n][2] = s[j][n][3] = 0.f;
-          const uint4 k0 = *reinterpret_cast<const uint4*>(kt + j * 512 + lane * 16);
-          const uint4 k1 = *reinterpret_cast<const uint4*>(kt + (G::KCH + j) * 512 + lane * 16);
+          const uint4 k0 = *reinterpret_cast<const uint4*>(kt + G::chunk(kg, j * 4 + t4));
+          const uint4 k1 = *reinterpret_cast<const uint4*>(kt + 8 * HD + G::chunk(kg, j * 4 + t4));
           const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -353,20 +406,20 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
             const float raw = G::KCH == 2 ? s[0][n][e] + s[G::KCH - 1][n][e] : s[0][n][e];
             y[tt][n][e] = raw * (rm[n][e & 1] * ksc);
           }
-        if (p0[tt] + KD_TILE > all_see || !seen) {
+        if (p0[tt] + 16 > all_see || !seen) {
 #pragma unroll
           for (int n = 0; n < NB; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (p0[tt] + g + 8 * (e >> 1) >= vis[n][e & 1] || !seen) y[tt][n][e] = -INFINITY;
+              if (p0[tt] + kg + 8 * (e >> 1) >= vis[n][e & 1] || !seen) y[tt][n][e] = -INFINITY;
         }
-        if (score_row && live) {
+        if (score_row && p0[tt] < cap) {
 #pragma unroll
           for (int n = 0; n < NB; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int r = n * 8 + 2 * t4 + (e & 1);
-              if (r < nrow) score_row[(int64_t)r * cap + p0[tt] + g + 8 * (e >> 1)] = y[tt][n][e];
+              if (r < nrow) score_row[(int64_t)r * cap + p0[tt] + kg + 8 * (e >> 1)] = y[tt][n][e];
             }
         }
       }
@@ -418,7 +471,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
       // ---- O^T += V^T P^T ----
 #pragma unroll
       for (int tt = 0; tt < TT; ++tt) {
-        const uint8_t* vt = sm.ring[warp][(qi + tt) % ST] + G::K_BYTES;
+        const uint8_t* vt = sm.ring[warp][st] + G::KV_BYTES + (t0 + tt) * 16 * HD;
         uint32_t pb[NB][2], pl[NB][2];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
@@ -444,7 +497,8 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
         uint32_t v[4][VW];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint8_t* src = vt + i * 32 * G::VB + lane * G::VB;
+          const int r = (i & 1) ? kv1 : kv0;
+          const uint8_t* src = vt + 8 * (i >> 1) * HD + (HD == 128 ? G::chunk(r, g) : G::chunk(r, g >> 1) + (g & 1) * 8);
           if (VW == 4) {
             const uint4 x = *reinterpret_cast<const uint4*>(src);
             v[i][0] = x.x; v[i][1] = x.y; v[i][VW - 2] = x.z; v[i][VW - 1] = x.w;
@@ -453,10 +507,10 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
             v[i][0] = x.x; v[i][1] = x.y;
           }
         }
-        if (p0[tt] + KD_TILE > total) {  // rows never written may hold NaN codes
+        if (p0[tt] + 16 > total || !((okm >> (t0 + tt)) & 1)) {  // rows never written may hold NaN codes
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (p0[tt] + 2 * t4 + (i & 1) + 8 * (i >> 1) >= total)
+            if (p0[tt] + ((i & 1) ? kv1 : kv0) + 8 * (i >> 1) >= total || !((okm >> (t0 + tt)) & 1))
 #pragma unroll
               for (int k = 0; k < VW; ++k) v[i][k] = 0u;
         }
@@ -479,8 +533,10 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
           }
         }
       }
+      }
     }
     cp_wait<0>();
+    if (lost && lane == 0) *a.status = 1;
 
     // ---- join the warps ----
 #pragma unroll
@@ -638,7 +694,7 @@ __global__ void __launch_bounds__(128) kv8_weights_kernel(const KWArgs a) {
 // ---------------------------------------------------------------------------
 struct KDPlan {
   int rg, nrg, n_cta;
-  int64_t cnt, part, ml, lse, scores, bytes;  // offsets
+  int64_t part, ml, lse, scores, bytes;  // offsets; the status word is at 0, the arrivals at 256
 };
 static KDPlan kd_plan(const N730KV8Cache& c, int batch, int tokens, int heads, int dtype, bool weights) {
   KDPlan p{};
@@ -648,7 +704,7 @@ static KDPlan kd_plan(const N730KV8Cache& c, int batch, int tokens, int heads, i
   p.nrg = (int)((rows + p.rg - 1) / p.rg);
   p.n_cta = KD_CTAS_PER_SM * num_sms();
   auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-  p.part = up((int64_t)batch * c.n_kv * p.nrg * 4);
+  p.part = 256 + up((int64_t)batch * c.n_kv * p.nrg * 4);
   p.ml = p.part + up((int64_t)2 * p.n_cta * p.rg * c.head_dim * 4);
   p.lse = p.ml + up((int64_t)2 * p.n_cta * p.rg * 16);
   p.scores = p.lse + (weights ? up((int64_t)batch * c.n_kv * rows * 4) : 0);
@@ -673,11 +729,44 @@ int64_t kv8_attention_ws(const N730KV8Cache& c, int batch, int tokens, int heads
                   kd_plan(c, batch, tokens, heads, N730_F16, weights).bytes);
 }
 
+// cuTensorMapEncodeTiled through the runtime's driver entry point (no libcuda link).
+static PFN_cuTensorMapEncodeTiled_v12000 kv8_encoder() {
+  static std::once_flag once;
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+    else
+      cudaGetLastError();
+  });
+  return fn;
+}
+
+// A code pool as a 2-D tensor of bytes, one row per position and KV head of a page; a copy takes
+// `box` whole rows (x is always 0), swizzled over the row's 128 or 64 bytes.
+static int kv8_map(const N730KV8Cache& c, const void* codes, int box, CUtensorMap* out) {
+  auto enc = kv8_encoder();
+  N730_REQUIRE(enc, N730_CUDA_ERR, "kv8_attention: cuTensorMapEncodeTiled is not available");
+  const cuuint64_t dims[2] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.n_pages * c.n_kv * c.page_size};
+  const cuuint64_t strides[1] = {(cuuint64_t)c.head_dim};
+  const cuuint32_t boxes[2] = {(cuuint32_t)c.head_dim, (cuuint32_t)box};
+  const cuuint32_t es[2] = {1, 1};
+  N730_REQUIRE(enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, boxes, es,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, c.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS,
+               N730_CUDA_ERR, "kv8_attention: cuTensorMapEncodeTiled failed");
+  return N730_OK;
+}
+
 template <int HD, int CODE, int NB, bool LO>
-static int split_launch(const KDArgs& a, bool pdl, cudaStream_t st) {
-  const size_t smem = sizeof(KDSmem<HD>) + (size_t)a.batch * 4;
-  if (int rc = smem_attr_once<kv8_split_kernel<HD, CODE, NB, LO>>((int)(sizeof(KDSmem<HD>) + KD_MAX_BATCH * 4))) return rc;
-  return kv8_launch(kv8_split_kernel<HD, CODE, NB, LO>, dim3(a.n_cta), dim3(KD_THREADS), smem, st, pdl, a);
+static int split_launch(const KDArgs& a, const CUtensorMap& km, const CUtensorMap& vm, bool pdl, cudaStream_t st) {
+  const size_t fixed = sizeof(KDSmem<HD>) + 1024;
+  if (int rc = smem_attr_once<kv8_split_kernel<HD, CODE, NB, LO>>((int)(fixed + KD_MAX_BATCH * 4))) return rc;
+  return kv8_launch(kv8_split_kernel<HD, CODE, NB, LO>, dim3(a.n_cta), dim3(KD_THREADS), fixed + (size_t)a.batch * 4, st,
+                    pdl, a, km, vm);
 }
 
 int kv8_attention_launch(const KV8AttnCall& k, cudaStream_t st) {
@@ -692,18 +781,23 @@ int kv8_attention_launch(const KV8AttnCall& k, cudaStream_t st) {
   a.rows = k.tokens * a.group; a.nrg = p.nrg;
   a.scale_log2e = k.scale * 1.4426950408889634f;
   a.lens = k.lens; a.n_new = k.n_new;
-  a.cnt = reinterpret_cast<unsigned*>(ws);
+  a.status = reinterpret_cast<int*>(ws);
+  a.cnt = reinterpret_cast<unsigned*>(ws + 256);
   a.part = reinterpret_cast<float*>(ws + p.part);
   a.part_ml = reinterpret_cast<float*>(ws + p.ml);
   a.lse = weights ? reinterpret_cast<float*>(ws + p.lse) : nullptr;
   a.scores = weights ? reinterpret_cast<float*>(ws + p.scores) : nullptr;
   a.n_cta = p.n_cta;
   a.log_block = c.block == 16 ? 4 : c.block == 32 ? 5 : 6;
-  int rc;
+  a.box = c.page_size % KD_TILE == 0 ? KD_TILE : 16;
+  CUtensorMap km, vm;
+  int rc = kv8_map(c, c.k_codes, a.box, &km);
+  if (!rc) rc = kv8_map(c, c.v_codes, a.box, &vm);
+  if (rc) return rc;
 #define N730_SPLIT(HD, CODE)                                                 \
-  (k.dtype == N730_F32 ? split_launch<HD, CODE, 1, true>(a, k.pdl, st)       \
-   : p.rg == 8         ? split_launch<HD, CODE, 1, false>(a, k.pdl, st)      \
-                       : split_launch<HD, CODE, 2, false>(a, k.pdl, st))
+  (k.dtype == N730_F32 ? split_launch<HD, CODE, 1, true>(a, km, vm, k.pdl, st)       \
+   : p.rg == 8         ? split_launch<HD, CODE, 1, false>(a, km, vm, k.pdl, st)      \
+                       : split_launch<HD, CODE, 2, false>(a, km, vm, k.pdl, st))
   if (c.head_dim == 128) rc = c.code == N730_KV8_INT8 ? N730_SPLIT(128, N730_KV8_INT8) : N730_SPLIT(128, N730_KV8_E4M3);
   else rc = c.code == N730_KV8_INT8 ? N730_SPLIT(64, N730_KV8_INT8) : N730_SPLIT(64, N730_KV8_E4M3);
 #undef N730_SPLIT
