@@ -5,9 +5,12 @@
 // Split kernel (single tokens and few rows).  The rows of an item (sequence, KV head) are its
 // tokens x G query heads, 8 or 16 at a time.  All items' 32-position tiles form one line that the
 // CTAs cut into equal runs, so ragged lengths and few sequences load every SM alike; a run that
-// covers part of an item leaves its (max, sum, output) in the workspace, and the last CTA to finish
-// an item joins the parts in run order (the result does not depend on which CTA that is).  Within a
-// CTA each warp takes every fourth tile.
+// covers part of an item leaves its (max, sum, output) in the workspace, and the finishing kernel
+// joins an item's parts in run order, with as many CTAs as there are items.  Within a
+// CTA each warp takes every fourth tile.  An item counts for KD_ITEM_COST tiles more than it has, the
+// time that starting and ending one takes: without that the CTAs that meet many short sequences were
+// the last to finish (batch of 128 ragged lengths: see KD_ITEM_COST).  The next run's first tile is
+// asked for before this one's outputs are joined.
 //
 // The products are transposed, so that a key or a channel is a row of mma.m16n8k16's A and the few
 // query rows are its 8 columns: no half of an instruction works on rows that are not there.
@@ -45,6 +48,7 @@ constexpr int KD_THREADS = KD_WARPS * 32;
 constexpr int KD_STAGES = 2;     // tile buffers of a warp
 constexpr int KD_TILE = 32;      // positions
 constexpr int KD_CTAS_PER_SM = 3;
+constexpr int KD_ITEM_COST = 6;  // tiles
 constexpr int KD_MIN_UNITS = 4;  // tiles of a run: fewer would leave warps idle and joins to do
 constexpr int KD_MAX_BATCH = 4096;
 constexpr float KD_SLACK = 8.f;  // log2 of how far a weight may exceed its reference
@@ -58,10 +62,10 @@ struct KDArgs {
   float scale_log2e;
   const int* lens; const int* n_new;
   int* status;         // set when a wait ran out
-  unsigned* cnt;       // [batch][n_kv][nrg] arrivals, zero between calls
+  int* line;           // [batch + 1] prefix sums of the line, for the finishing kernel
   float* part;         // [2 * n_cta][RG][HD]
   float* part_ml;      // [2 * n_cta][RG][4]: reference of the output, max, sum
-  float* lse;          // [batch][n_kv][rows] log2 of the softmax sum, +inf for an empty row (weights only)
+  float* lse;          // [batch][n_kv][rows] log2 of the softmax sum, +inf for an empty row (items of one run)
   float* scores;       // [batch][n_kv][rows][cap] base-2 scores (weights only)
   int n_cta, log_block, box;  // box: rows of a copy, 32, or 16 where pages are no multiples of 32
 };
@@ -72,7 +76,6 @@ struct KDGeom {
   static constexpr int VB = HD / 8;                   // V bytes per lane and key
   static constexpr int KV_BYTES = KD_TILE * HD;       // K (or V) codes of a tile
   static constexpr int TILE_BYTES = 2 * KV_BYTES;
-  static constexpr int OSTRIDE = HD + 4;              // padded output row (bank spread, 16-byte rows)
   // byte of 16-byte chunk c of row r: the copies' 128-byte (64-byte) swizzle
   static __device__ __forceinline__ int chunk(int r, int c) {
     return HD == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
@@ -82,6 +85,15 @@ struct KDGeom {
     const int e = HD == 128 ? i & 6 : ((i >> 1) & 1) + ((i >> 2) << 2);  // even i: 0 2 4 6, or 0 1 4 5
     return (i & 1) == 0 ? e : HD == 128 ? (e ^ 4) + 1 : e ^ 3;
   }
+};
+
+// one CTA's run through one item
+struct KDSeg {
+  int valid;
+  int b, h, rg;         // sequence, KV head, row group
+  int ta, te, units;    // tiles [ta, te) of the item's `units`
+  int L, total;         // positions cached before the call, with the new rows
+  int f0, nrow;         // first row, rows
 };
 
 template <int HD>
@@ -94,8 +106,9 @@ struct KDSmem {
   float rowmul[16];
   float wm[KD_WARPS][16], wmo[KD_WARPS][16], wl[KD_WARPS][16];
   float tot[16][4];
-  int flag;
-  int pre[1];                      // [batch + 1] prefix sums of the sequences' tiles
+  int out_at[KD_WARPS];            // buffer of each warp's outputs
+  KDSeg seg[3];                    // this run, the next, and the last one's, which slow warps may still read
+  int pre[1];                      // [batch + 1] prefix sums of the line, then [batch] lengths, [batch] new rows
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -163,12 +176,23 @@ __device__ __forceinline__ uint32_t codes2(uint32_t x) {
 template <int CODE>
 __device__ __forceinline__ uint32_t code_word(uint32_t x) { return CODE == N730_KV8_INT8 ? x ^ 0x80808080u : x; }
 
-// tiles of sequence b: at least one when it has new rows (they need an answer)
-__device__ __forceinline__ int kd_units(const KDArgs& a, int b, int cap) {
-  const int n = kv8_new(a.n_new, b, a.tokens);
-  if (n == 0) return 0;
-  const int tot = (int)min((int64_t)kv8_len(a.lens, b, cap) + n, (int64_t)cap);
-  return (tot + KD_TILE - 1) / KD_TILE;
+// tiles of a sequence with new rows
+__device__ __forceinline__ int kd_units(int L, int n_new, int cap) {
+  return (int)((min((int64_t)L + n_new, (int64_t)cap) + KD_TILE - 1) / KD_TILE);
+}
+
+// the CTA of N whose part of the line of U holds tile u
+__device__ __forceinline__ int kd_owner(int64_t u, int64_t U, int64_t N) { return (int)(((u + 1) * N - 1) / U); }
+
+// The answer of row f, channels d..d + 3: sums of weight x V against Mo, of weights l against M.
+template <int HD>
+__device__ __forceinline__ void kd_answer(const KDArgs& a, int b, int h, int f, int d, const float4& num, float Mo, float M, float l) {
+  const float s = l == 0.f ? 0.f : (Mo == -INFINITY ? 0.f : ex2(Mo - M)) / l;  // a NaN query: NaN
+  const int64_t at = ((int64_t)b * a.tokens + f / a.group) * a.ldo + (int64_t)(h * a.group + f % a.group) * HD + d;
+  kv8_store1(a.out, at, a.dtype, num.x * s);
+  kv8_store1(a.out, at + 1, a.dtype, num.y * s);
+  kv8_store1(a.out, at + 2, a.dtype, num.z * s);
+  kv8_store1(a.out, at + 3, a.dtype, num.w * s);
 }
 
 // NB: 8-row groups of an item's rows worked on together; LO: fp32 rows in two fp16 terms.
@@ -179,7 +203,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
   constexpr int TT = NB == 1 ? 2 : 1;  // halves of a tile worked on together: independent chains for the tensor cores
   extern __shared__ __align__(1024) uint8_t kd_raw[];
   KDSmem<HD>& sm = *reinterpret_cast<KDSmem<HD>*>((reinterpret_cast<uintptr_t>(kd_raw) + 1023) & ~uintptr_t(1023));
-  static_assert(sizeof(float) * KD_WARPS * RG * G::OSTRIDE <= sizeof(sm.ring), "per-warp outputs fit the ring");
+  static_assert(ST == 2 && sizeof(float) * RG * HD <= G::TILE_BYTES, "a warp's outputs fit the buffer that is not being filled");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   const N730KV8Cache& c = a.c;
   const int cap = c.max_pages * c.page_size;
@@ -192,105 +216,134 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
   uint32_t uses = 0;
   pdl_wait();
 
-  // ---- prefix sums of the sequences' tiles ----
+  // ---- the line: prefix sums of items x (tiles + KD_ITEM_COST) / items ----
+  int* const len_of = sm.pre + a.batch + 1;
+  int* const new_of = len_of + a.batch;
   if (warp == 0) {
     int run = 0;
     if (lane == 0) sm.pre[0] = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 32) {
-      int v = b0 + lane < a.batch ? kd_units(a, b0 + lane, cap) : 0;
+      const int b = b0 + lane;
+      int v = 0;
+      if (b < a.batch) {
+        const int n = kv8_new(a.n_new, b, a.tokens), L = kv8_len(a.lens, b, cap);
+        len_of[b] = L;
+        new_of[b] = n;
+        v = n ? kd_units(L, n, cap) + KD_ITEM_COST : 0;
+      }
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int n = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += n;
       }
-      if (b0 + lane < a.batch) sm.pre[b0 + lane + 1] = run + v;
+      if (b < a.batch) sm.pre[b + 1] = run + v;
       run += __shfl_sync(0xffffffffu, v, 31);
     }
   }
   __syncthreads();
+  pdl_launch_dependents();  // the finishing kernel waits for this grid's end
+  if (blockIdx.x == 0)
+    for (int i = tid; i <= a.batch; i += KD_THREADS) a.line[i] = sm.pre[i];
   const int items = c.n_kv * a.nrg;  // per sequence
   const int64_t U = (int64_t)sm.pre[a.batch] * items;
   const int64_t N = min((int64_t)a.n_cta, (U + KD_MIN_UNITS - 1) / KD_MIN_UNITS);
   const int cta = blockIdx.x;
   if (cta >= N) return;
+  // one thread walks the CTA's part [u, u1) of the line
   int64_t u = U * cta / N;
   const int64_t u1 = U * (cta + 1) / N;
-  int b = 0;
-  {
-    int lo = 0, hi = a.batch - 1;  // the last b with pre[b] * items <= u
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if ((int64_t)sm.pre[mid] * items <= u) lo = mid; else hi = mid - 1;
+  int at_b = -1;
+  auto next_run = [&](KDSeg& s) {
+    s.valid = 0;
+    if (at_b < 0) {
+      int lo = 0, hi = a.batch - 1;  // the last b with pre[b] * items <= u
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if ((int64_t)sm.pre[mid] * items <= u) lo = mid; else hi = mid - 1;
+      }
+      at_b = lo;
     }
-    b = lo;
-  }
+    while (u < u1) {
+      while ((int64_t)sm.pre[at_b + 1] * items <= u) ++at_b;  // past sequences without tiles
+      const int b = at_b, span = sm.pre[b + 1] - sm.pre[b];
+      const int64_t base = (int64_t)sm.pre[b] * items, ub = u - base;
+      const int item = (int)(ub / span), off = (int)(ub - (int64_t)item * span);
+      const int end = (int)min((int64_t)span, off + (u1 - u));
+      u += end - off;
+      s.f0 = item % a.nrg * RG;
+      s.nrow = min(RG, new_of[b] * a.group - s.f0);
+      s.ta = max(0, off - KD_ITEM_COST);
+      s.te = end - KD_ITEM_COST;
+      if (s.te <= s.ta || s.nrow <= 0) continue;  // only the item's cost, or rows behind the sequence's new ones
+      s.valid = 1;
+      s.b = b; s.h = item / a.nrg; s.rg = item % a.nrg;
+      s.units = span - KD_ITEM_COST;
+      s.L = len_of[b];
+      s.total = (int)min((int64_t)s.L + new_of[b], (int64_t)cap);
+      break;
+    }
+  };
+  constexpr int WALKER = KD_THREADS - 32;  // its first lane walks
+  if (tid == WALKER) next_run(sm.seg[0]);
+  __syncthreads();
 
-  while (u < u1) {
-    while ((int64_t)sm.pre[b + 1] * items <= u) ++b;  // past sequences without tiles
-    const int units = sm.pre[b + 1] - sm.pre[b];
-    const int64_t ub = u - (int64_t)sm.pre[b] * items;
-    const int item = (int)(ub / units), ta = (int)(ub % units), te = (int)min((int64_t)units, ta + (u1 - u));
-    u += te - ta;
-    const int h = item / a.nrg, rg = item % a.nrg;
-    const int L = kv8_len(a.lens, b, cap), n_new = kv8_new(a.n_new, b, a.tokens);
-    const int rows_b = n_new * a.group, f0 = rg * RG;
-    if (f0 >= rows_b) continue;  // a row group behind this sequence's new rows
-    const int nrow = min(RG, rows_b - f0);
-    const int total = (int)min((int64_t)L + n_new, (int64_t)cap);  // positions cached with the new rows
-
-    // shared memory of the previous run is free; what its threads wrote there comes before new copies
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncthreads();
-    // ---- the warp's tiles ----
-    const int n_tile = te - ta > warp ? (te - ta - warp + KD_WARPS - 1) / KD_WARPS : 0;
-    const int* bt = c.block_table + (int64_t)b * c.max_pages;
-    // pool row of half tile q0 + lane of this warp (-1: no page), looked up 16 tiles at a time
-    auto lookup = [&](int q0) {
-      const int p = (ta + warp + ((q0 + lane) >> 1) * KD_WARPS) * KD_TILE + (lane & 1) * 16;
-      if (((q0 + lane) >> 1) >= n_tile || p >= total) return -1;
-      const int page = bt[p / c.page_size];
-      return (unsigned)page < (unsigned)c.n_pages ? (page * c.n_kv + h) * c.page_size + p % c.page_size : -1;
-    };
-    int rows_now = lookup(0), rows_next = lookup(32);
-    auto issue = [&](int qi) {
-      const int st = fills % ST;
-      ++fills;
-      if (qi && (qi & 15) == 0) { rows_now = rows_next; rows_next = lookup(2 * qi + 32); }
-      const int row0 = __shfl_sync(0xffffffffu, rows_now, (2 * qi) & 31);
-      const int row1 = __shfl_sync(0xffffffffu, rows_now, (2 * qi + 1) & 31);
-      if (lane == 0) {
-        const uint32_t dst = smem_u32(sm.ring[warp][st]);
-        uint64_t* bar = &sm.full[warp][st];
-        sm.ok[warp][st] = (row0 >= 0 ? 1 : 0) | (row1 >= 0 ? 2 : 0);
-        if (a.box == KD_TILE) {
-          mbar_arrive_expect_tx(bar, row0 >= 0 ? G::TILE_BYTES : 0);
-          if (row0 >= 0) {
-            copy_rows(dst, &kmap, row0, bar);
-            copy_rows(dst + G::KV_BYTES, &vmap, row0, bar);
-          }
-        } else {
-          mbar_arrive_expect_tx(bar, (row0 >= 0 ? G::KV_BYTES : 0) + (row1 >= 0 ? G::KV_BYTES : 0));
-          if (row0 >= 0) {
-            copy_rows(dst, &kmap, row0, bar);
-            copy_rows(dst + G::KV_BYTES, &vmap, row0, bar);
-          }
-          if (row1 >= 0) {
-            copy_rows(dst + G::KV_BYTES / 2, &kmap, row1, bar);
-            copy_rows(dst + G::KV_BYTES * 3 / 2, &vmap, row1, bar);
-          }
+  // ---- the warp's tiles of a run: every KD_WARPS-th ----
+  auto tiles_of = [&](const KDSeg& s) { return s.te - s.ta > warp ? (s.te - s.ta - warp + KD_WARPS - 1) / KD_WARPS : 0; };
+  // pool row of half tile q0 + lane (-1: no page), looked up 16 tiles at a time
+  auto lookup = [&](const KDSeg& s, int q0) {
+    const int p = (s.ta + warp + ((q0 + lane) >> 1) * KD_WARPS) * KD_TILE + (lane & 1) * 16;
+    if (p >= min(s.total, s.te * KD_TILE)) return -1;
+    const int page = c.block_table[(int64_t)s.b * c.max_pages + p / c.page_size];
+    return (unsigned)page < (unsigned)c.n_pages ? (page * c.n_kv + s.h) * c.page_size + p % c.page_size : -1;
+  };
+  // ask for a tile whose half rows are lanes 2 i, 2 i + 1 of `rows`
+  auto issue = [&](int rows, int i) {
+    const int st = fills % ST;
+    ++fills;
+    const int row0 = __shfl_sync(0xffffffffu, rows, 2 * i), row1 = __shfl_sync(0xffffffffu, rows, 2 * i + 1);
+    if (lane == 0) {
+      const uint32_t dst = smem_u32(sm.ring[warp][st]);
+      uint64_t* bar = &sm.full[warp][st];
+      sm.ok[warp][st] = (row0 >= 0 ? 1 : 0) | (row1 >= 0 ? 2 : 0);
+      if (a.box == KD_TILE) {
+        mbar_arrive_expect_tx(bar, row0 >= 0 ? G::TILE_BYTES : 0);
+        if (row0 >= 0) {
+          copy_rows(dst, &kmap, row0, bar);
+          copy_rows(dst + G::KV_BYTES, &vmap, row0, bar);
+        }
+      } else {
+        mbar_arrive_expect_tx(bar, (row0 >= 0 ? G::KV_BYTES : 0) + (row1 >= 0 ? G::KV_BYTES : 0));
+        if (row0 >= 0) {
+          copy_rows(dst, &kmap, row0, bar);
+          copy_rows(dst + G::KV_BYTES, &vmap, row0, bar);
+        }
+        if (row1 >= 0) {
+          copy_rows(dst + G::KV_BYTES / 2, &kmap, row1, bar);
+          copy_rows(dst + G::KV_BYTES * 3 / 2, &vmap, row1, bar);
         }
       }
-      if (lane < 4) {
-        const int row = lane < 2 ? row0 : row1;
-        const float* s = ((lane & 1) ? c.v_scales : c.k_scales) + (max(row, 0) >> a.log_block);
-        cp_async<4>(smem_u32(&sm.sc[warp][st][lane]), s, row >= 0);
-      }
-    };
-#pragma unroll
-    for (int s = 0; s < ST - 1; ++s) {
-      if (s < n_tile) issue(s);
-      cp_commit();
     }
+    if (lane < 4) {
+      const int row = lane < 2 ? row0 : row1;
+      const float* s = ((lane & 1) ? c.v_scales : c.k_scales) + (max(row, 0) >> a.log_block);
+      cp_async<4>(smem_u32(&sm.sc[warp][st][lane]), s, row >= 0);
+    }
+  };
+  int rows_now = -1;
+  if (sm.seg[0].valid) {
+    rows_now = lookup(sm.seg[0], 0);
+    if (tiles_of(sm.seg[0])) issue(rows_now, 0);
+  }
+  cp_commit();
+
+  for (int turn = 0;; ++turn) {
+    const KDSeg& run = sm.seg[turn % 3];
+    const KDSeg& after = sm.seg[(turn + 1) % 3];
+    if (!run.valid) break;
+    const int b = run.b, h = run.h, f0 = run.f0, nrow = run.nrow, L = run.L, total = run.total, ta = run.ta;
+    const int n_tile = tiles_of(run);
+    int rows_next = lookup(run, 32);
+    if (tid == WALKER) next_run(sm.seg[(turn + 1) % 3]);
 
     // ---- Q: a row per warp at a time, scaled by a power of two, as the B operand ----
     for (int r = warp; r < RG; r += KD_WARPS) {
@@ -321,7 +374,10 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
           reinterpret_cast<__half*>(&sm.qf[1][ks][(r & 7) * 4 + tt])[w] = __float2half_rn(y - __half2float(hi));
       }
     }
+    // what the last run's threads did to shared memory comes before the copies of this one's loop
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
+    const int rows_after = after.valid ? lookup(after, 0) : -1;
     uint2 qreg[NB == 1 && !LO ? KS : 1];  // one row group's Q stays in registers, two are read as needed
     if (NB == 1 && !LO)
 #pragma unroll
@@ -354,7 +410,10 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
 
     for (int qi = 0; qi < n_tile; ++qi) {
       __syncwarp();  // every lane is done with the buffer that the next copies go to
-      if (qi + ST - 1 < n_tile) issue(qi + ST - 1);
+      if (qi + 1 < n_tile) {
+        if (((qi + 1) & 15) == 0) { rows_now = rows_next; rows_next = lookup(run, 2 * (qi + 1) + 32); }
+        issue(rows_now, (qi + 1) & 15);
+      }
       cp_commit();
       const int st = uses % ST;
       if (!wait_copies(&sm.full[warp][st], (uses / ST) & 1, lost)) lost = true;
@@ -535,8 +594,13 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
       }
       }
     }
-    cp_wait<0>();
     if (lost && lane == 0) *a.status = 1;
+    __syncwarp();
+    // the next run's first tile goes into one buffer, this run's outputs into the other
+    rows_now = rows_after;
+    if (after.valid && tiles_of(after)) issue(rows_now, 0);
+    cp_commit();
+    float* const mine = reinterpret_cast<float*>(sm.ring[warp][fills % ST]);  // [row][HD], 16-byte groups spread by row
 
     // ---- join the warps ----
 #pragma unroll
@@ -552,18 +616,19 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
           sm.wl[warp][r] = l_run[n][e];
         }
       }
-    __syncthreads();  // all tiles are read: the ring takes the outputs
-    float* wo = reinterpret_cast<float*>(&sm.ring[0][0][0]);  // [warp][row][OSTRIDE]
+    if (lane == 0) sm.out_at[warp] = fills % ST;
+    // 16-byte group q of row r lies at q ^ (r & 7): the lanes of a store meet few banks twice
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int k = 0; k < MT; ++k)
-          *reinterpret_cast<float2*>(wo + (warp * RG + n * 8 + 2 * t4 + e) * G::OSTRIDE + g * G::VB + 2 * k) =
-              make_float2(o[n][k][e], o[n][k][e + 2]);
+        for (int k = 0; k < MT; ++k) {
+          const int r = n * 8 + 2 * t4 + e, d = g * G::VB + 2 * k;
+          *reinterpret_cast<float2*>(mine + r * HD + (((d >> 2) ^ (r & 7)) << 2) + (d & 2)) = make_float2(o[n][k][e], o[n][k][e + 2]);
+        }
     __syncthreads();
-    const bool whole = ta == 0 && te == units;
+    const bool whole = ta == 0 && run.te == run.units;
     const int slot = 2 * cta + (ta == 0 ? 1 : 0);
     if (tid < RG) {
       float M = -INFINITY, Mo = -INFINITY, l = 0.f;
@@ -580,113 +645,152 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
         *reinterpret_cast<float4*>(a.part_ml + ((int64_t)slot * RG + tid) * 4) = make_float4(Mo, M, l, 0.f);
     }
     __syncthreads();
-    const int64_t ob = (int64_t)b * a.tokens;
-    auto finish = [&](int r, int d, const float4& num) {  // the answer of row r, channels d..d + 3
-      const float Mo = sm.tot[r][0], M = sm.tot[r][1], l = sm.tot[r][2];
-      const float f = l == 0.f ? 0.f : (Mo == -INFINITY ? 0.f : ex2(Mo - M)) / l;  // a NaN query: NaN
-      const int64_t at = (ob + (f0 + r) / a.group) * a.ldo + (int64_t)(h * a.group + (f0 + r) % a.group) * HD + d;
-      kv8_store1(a.out, at, a.dtype, num.x * f);
-      kv8_store1(a.out, at + 1, a.dtype, num.y * f);
-      kv8_store1(a.out, at + 2, a.dtype, num.z * f);
-      kv8_store1(a.out, at + 3, a.dtype, num.w * f);
-    };
-    auto store_lse = [&]() {
-      if (a.lse && tid < nrow)
-        a.lse[((int64_t)b * c.n_kv + h) * a.rows + f0 + tid] =
-            sm.tot[tid][2] == 0.f ? INFINITY : sm.tot[tid][1] + lg2(sm.tot[tid][2]);
-    };
     for (int i = tid; i < nrow * (HD / 4); i += KD_THREADS) {
       const int r = i / (HD / 4), d = i % (HD / 4) * 4;
       float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int k = 0; k < KD_WARPS; ++k) {
-        const float4 x = *reinterpret_cast<const float4*>(wo + (k * RG + r) * G::OSTRIDE + d);
+        const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm.ring[k][sm.out_at[k]]) + r * HD +
+                                                          (((d >> 2) ^ (r & 7)) << 2));
         const float f = sm.wmo[k][r];
         num.x = fmaf(x.x, f, num.x); num.y = fmaf(x.y, f, num.y); num.z = fmaf(x.z, f, num.z); num.w = fmaf(x.w, f, num.w);
       }
-      if (whole) finish(r, d, num);
+      if (whole) kd_answer<HD>(a, b, h, f0 + r, d, num, sm.tot[r][0], sm.tot[r][1], sm.tot[r][2]);
       else *reinterpret_cast<float4*>(a.part + ((int64_t)slot * RG + r) * HD + d) = num;
     }
-    if (whole) {
-      store_lse();
-      continue;
-    }
-    // ---- parts: the last CTA of the item joins them ----
-    const int64_t i0 = (int64_t)sm.pre[b] * items + (int64_t)item * units;  // the item's first tile on the line
-    const int c0 = (int)(((i0 + 1) * N - 1) / U), c1 = (int)(((i0 + units) * N - 1) / U), parts = c1 - c0 + 1;
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) {
-      unsigned* cnt = a.cnt + ((int64_t)b * c.n_kv + h) * a.nrg + rg;
-      sm.flag = atomicInc(cnt, (unsigned)(parts - 1)) == (unsigned)(parts - 1);  // wraps to 0: ready for the next call
-    }
-    __syncthreads();
-    if (!sm.flag) continue;
-    __threadfence();
-    float* wts = wo;  // [row][part]
-    auto part_of = [&](int k) { return (int64_t)(2 * (c0 + k) + (k == 0)) * RG; };  // its first row
-    for (int r = warp; r < nrow; r += KD_WARPS) {
-      float M = -INFINITY, Mo = -INFINITY, l = 0.f;
-      for (int k = lane; k < parts; k += 32) {
-        const float4 ml = __ldcg(reinterpret_cast<const float4*>(a.part_ml) + part_of(k) + r);
-        Mo = fmaxf(Mo, ml.x);
-        M = fmaxf(M, ml.y);
-      }
-      M = warp_max(M);
-      Mo = warp_max(Mo);
-      const float ms = M == -INFINITY ? 0.f : M, mos = Mo == -INFINITY ? 0.f : Mo;
-      for (int k = lane; k < parts; k += 32) {
-        const float4 ml = __ldcg(reinterpret_cast<const float4*>(a.part_ml) + part_of(k) + r);
-        l += ml.z * ex2(ml.y - ms);
-        wts[r * parts + k] = ex2(ml.x - mos);
-      }
-      l = warp_sum(l);
-      if (lane == 0) { sm.tot[r][0] = Mo; sm.tot[r][1] = M; sm.tot[r][2] = l; }
-    }
-    __syncthreads();
-    for (int i = tid; i < nrow * (HD / 4); i += KD_THREADS) {
-      const int r = i / (HD / 4), d = i % (HD / 4) * 4;
-      float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int k = 0; k < parts; ++k) {
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(a.part + (part_of(k) + r) * HD + d));
-        const float f = wts[r * parts + k];
-        num.x = fmaf(x.x, f, num.x); num.y = fmaf(x.y, f, num.y); num.z = fmaf(x.z, f, num.z); num.w = fmaf(x.w, f, num.w);
-      }
-      finish(r, d, num);
-    }
-    store_lse();
+    if (whole && a.lse && tid < nrow)
+      a.lse[((int64_t)b * c.n_kv + h) * a.rows + f0 + tid] =
+          sm.tot[tid][2] == 0.f ? INFINITY : sm.tot[tid][1] + lg2(sm.tot[tid][2]);
   }
+  cp_wait<0>();
 }
 
 // ---------------------------------------------------------------------------
-// accumulated weights: w[b, h, p] += sum over the KV head's rows of exp2(score - lse)
+// Finishing: joins the parts of items that several CTAs worked on, and accumulates the softmax weights:
+//   w[b, h, p] += sum over the KV head's rows of exp2(score - lse), in row order.
+// The first rg / rb blocks of each row group join rb of its rows of (head y, sequence z), with as many of
+// the block's 4 warps on a row as rb leaves; blocks behind them take 512 positions each.
 // ---------------------------------------------------------------------------
-struct KWArgs {
-  N730KV8Cache c;
-  int batch, tokens, group, rows;
-  const int* lens; const int* n_new;
-  const float* scores; const float* lse;
+constexpr int KF_THREADS = 128;
+constexpr int KF_POSITIONS = 4 * KF_THREADS;
+
+struct KFArgs {
+  KDArgs d;
+  int rg, rb;
   const float* w_in; float* w_out;
   int64_t ldw;
 };
 
-// A thread sums one position over the rows in row order.
-__global__ void __launch_bounds__(128) kv8_weights_kernel(const KWArgs a) {
-  pdl_wait();
-  const N730KV8Cache& c = a.c;
-  const int b = blockIdx.z, h = blockIdx.y;
+// An item's parts: slots c0 .. c0 + n - 1 (the first CTA's second slot, the others' first).
+struct KFParts { int c0, n; };
+__device__ __forceinline__ KFParts kf_parts(const KFArgs& a, int b, int h, int rg) {
+  const KDArgs& d = a.d;
+  const int items = d.c.n_kv * d.nrg, span = d.line[b + 1] - d.line[b];
+  const int64_t U = (int64_t)d.line[d.batch] * items;
+  const int64_t N = min((int64_t)d.n_cta, (U + KD_MIN_UNITS - 1) / KD_MIN_UNITS);
+  const int64_t u0 = (int64_t)d.line[b] * items + (int64_t)(h * d.nrg + rg) * span;
+  const int c0 = kd_owner(u0 + KD_ITEM_COST, U, N);
+  return {c0, kd_owner(u0 + span - 1, U, N) - c0 + 1};
+}
+__device__ __forceinline__ int64_t kf_row(const KFArgs& a, const KFParts& p, int k, int r) {
+  return (int64_t)(2 * (p.c0 + k) + (k == 0)) * a.rg + r;
+}
+// A warp's (reference of the outputs, maximum, sum) of row r over the parts.
+__device__ __forceinline__ float4 kf_totals(const KFArgs& a, const KFParts& p, int r) {
+  float Mo = -INFINITY, M = -INFINITY, l = 0.f;
+  for (int k = threadIdx.x & 31; k < p.n; k += 32) {
+    const float4 ml = reinterpret_cast<const float4*>(a.d.part_ml)[kf_row(a, p, k, r)];
+    Mo = fmaxf(Mo, ml.x);
+    const float m = fmaxf(M, ml.y), ms = m == -INFINITY ? 0.f : m;
+    l = l * ex2(M - ms) + ml.z * ex2(ml.y - ms);
+    M = m;
+  }
+  const float m = warp_max(M), ms = m == -INFINITY ? 0.f : m;
+  return make_float4(warp_max(Mo), m, warp_sum(l * ex2(M - ms)), 0.f);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(KF_THREADS) kv8_finish_kernel(const KFArgs a) {
+  constexpr int LPP = HD / 4, WARPS = KF_THREADS / 32;  // lanes that a part of a row takes
+  extern __shared__ float kf_lse[];
+  __shared__ float4 share[KF_THREADS];
+  const KDArgs& d = a.d;
+  const N730KV8Cache& c = d.c;
+  const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cap = c.max_pages * c.page_size;
-  const int L = kv8_len(a.lens, b, cap), n = kv8_new(a.n_new, b, a.tokens);
-  const int total = (int)min((int64_t)L + n, (int64_t)cap);
-  const int p = blockIdx.x * 128 + threadIdx.x;
-  if (p >= total) return;
+  pdl_wait();
+  const int n_new = kv8_new(d.n_new, b, d.tokens), rows_b = n_new * d.group;
+  const int joins = d.nrg * (a.rg / a.rb);
+  if ((int)blockIdx.x < joins) {
+    const int rg = blockIdx.x / (a.rg / a.rb), first = blockIdx.x % (a.rg / a.rb) * a.rb, f0 = rg * a.rg;
+    if (f0 + first >= rows_b) return;
+    const KFParts p = kf_parts(a, b, h, rg);
+    if (p.n == 1) return;  // its CTA gave the answer
+    const int per_row = a.rb >= WARPS ? 1 : WARPS / a.rb;  // warps
+    const int shares = per_row * (32 / LPP), mine = warp % per_row * (32 / LPP) + lane / LPP, d4 = lane % LPP;
+    for (int i = 0; i < a.rb; i += WARPS / per_row) {
+      const int r = first + i + warp / per_row;
+      const bool live = f0 + r < rows_b;
+      float4 t = make_float4(0.f, 0.f, 0.f, 0.f), num = t;
+      if (live) {
+        t = kf_totals(a, p, r);
+        const float mos = t.x == -INFINITY ? 0.f : t.x;
+#pragma unroll 8
+        for (int k = mine; k < p.n; k += shares) {
+          const int64_t at = kf_row(a, p, k, r);
+          const float f = ex2(d.part_ml[at * 4] - mos);
+          const float4 x = reinterpret_cast<const float4*>(d.part + at * HD)[d4];
+          num.x = fmaf(x.x, f, num.x); num.y = fmaf(x.y, f, num.y); num.z = fmaf(x.z, f, num.z); num.w = fmaf(x.w, f, num.w);
+        }
+      }
+      __syncthreads();
+      share[tid] = num;
+      __syncthreads();
+      if (live && mine == 0) {  // the shares in order
+        for (int k = 1; k < shares; ++k) {
+          const float4 x = share[tid + k * LPP];
+          num.x += x.x; num.y += x.y; num.z += x.z; num.w += x.w;
+        }
+        kd_answer<HD>(d, b, h, f0 + r, d4 * 4, num, t.x, t.y, t.z);
+      }
+    }
+    return;
+  }
+  // ---- weights ----
+  const int L = kv8_len(d.lens, b, cap), total = (int)min((int64_t)L + n_new, (int64_t)cap);
+  const int p0 = ((int)blockIdx.x - joins) * KF_POSITIONS;
+  if (p0 >= total) return;
   const int64_t head = (int64_t)b * c.n_kv + h;
-  const float* s = a.scores + head * a.rows * cap + p;
-  const float* lse = a.lse + head * a.rows;
-  float sum = 0.f;
-  for (int f = 0; f < n * a.group; ++f) sum += ex2(s[(int64_t)f * cap] - lse[f]);
-  a.w_out[head * a.ldw + p] = (a.w_in && p < L ? a.w_in[head * a.ldw + p] : 0.f) + sum;
+  for (int rg = 0; rg * a.rg < rows_b; ++rg) {
+    const KFParts p = kf_parts(a, b, h, rg);
+    const int nrow = min(a.rg, rows_b - rg * a.rg);
+    for (int r = warp; r < nrow; r += KF_THREADS / 32) {
+      float lse;
+      if (p.n == 1) {
+        lse = d.lse[head * d.rows + rg * a.rg + r];
+      } else {
+        const float4 t = kf_totals(a, p, r);
+        lse = t.z == 0.f ? INFINITY : t.y + lg2(t.z);
+      }
+      if (lane == 0) kf_lse[rg * a.rg + r] = lse;
+    }
+  }
+  __syncthreads();
+  const int at = p0 + 4 * tid;  // cap is a multiple of 16: four positions are there or none
+  if (at >= total) return;
+  const float* s = d.scores + head * d.rows * cap + at;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int f = 0; f < rows_b; ++f) {
+    const float4 x = *reinterpret_cast<const float4*>(s + (int64_t)f * cap);
+    const float lse = kf_lse[f];
+    sum.x += ex2(x.x - lse); sum.y += ex2(x.y - lse); sum.z += ex2(x.z - lse); sum.w += ex2(x.w - lse);
+  }
+  const float w[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (at + e < total)
+      a.w_out[head * a.ldw + at + e] = (a.w_in && at + e < L ? a.w_in[head * a.ldw + at + e] : 0.f) + w[e];
 }
 
 // ---------------------------------------------------------------------------
@@ -694,7 +798,7 @@ __global__ void __launch_bounds__(128) kv8_weights_kernel(const KWArgs a) {
 // ---------------------------------------------------------------------------
 struct KDPlan {
   int rg, nrg, n_cta;
-  int64_t part, ml, lse, scores, bytes;  // offsets; the status word is at 0, the arrivals at 256
+  int64_t part, ml, lse, scores, bytes;  // offsets; the status word is at 0, the line at 256
 };
 static KDPlan kd_plan(const N730KV8Cache& c, int batch, int tokens, int heads, int dtype, bool weights) {
   KDPlan p{};
@@ -704,7 +808,7 @@ static KDPlan kd_plan(const N730KV8Cache& c, int batch, int tokens, int heads, i
   p.nrg = (int)((rows + p.rg - 1) / p.rg);
   p.n_cta = KD_CTAS_PER_SM * num_sms();
   auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-  p.part = 256 + up((int64_t)batch * c.n_kv * p.nrg * 4);
+  p.part = 256 + up((int64_t)(batch + 1) * 4);
   p.ml = p.part + up((int64_t)2 * p.n_cta * p.rg * c.head_dim * 4);
   p.lse = p.ml + up((int64_t)2 * p.n_cta * p.rg * 16);
   p.scores = p.lse + (weights ? up((int64_t)batch * c.n_kv * rows * 4) : 0);
@@ -764,8 +868,8 @@ static int kv8_map(const N730KV8Cache& c, const void* codes, int box, CUtensorMa
 template <int HD, int CODE, int NB, bool LO>
 static int split_launch(const KDArgs& a, const CUtensorMap& km, const CUtensorMap& vm, bool pdl, cudaStream_t st) {
   const size_t fixed = sizeof(KDSmem<HD>) + 1024;
-  if (int rc = smem_attr_once<kv8_split_kernel<HD, CODE, NB, LO>>((int)(fixed + KD_MAX_BATCH * 4))) return rc;
-  return kv8_launch(kv8_split_kernel<HD, CODE, NB, LO>, dim3(a.n_cta), dim3(KD_THREADS), fixed + (size_t)a.batch * 4, st,
+  if (int rc = smem_attr_once<kv8_split_kernel<HD, CODE, NB, LO>>((int)(fixed + KD_MAX_BATCH * 12))) return rc;
+  return kv8_launch(kv8_split_kernel<HD, CODE, NB, LO>, dim3(a.n_cta), dim3(KD_THREADS), fixed + (size_t)a.batch * 12, st,
                     pdl, a, km, vm);
 }
 
@@ -782,7 +886,7 @@ int kv8_attention_launch(const KV8AttnCall& k, cudaStream_t st) {
   a.scale_log2e = k.scale * 1.4426950408889634f;
   a.lens = k.lens; a.n_new = k.n_new;
   a.status = reinterpret_cast<int*>(ws);
-  a.cnt = reinterpret_cast<unsigned*>(ws + 256);
+  a.line = reinterpret_cast<int*>(ws + 256);
   a.part = reinterpret_cast<float*>(ws + p.part);
   a.part_ml = reinterpret_cast<float*>(ws + p.ml);
   a.lse = weights ? reinterpret_cast<float*>(ws + p.lse) : nullptr;
@@ -801,15 +905,24 @@ int kv8_attention_launch(const KV8AttnCall& k, cudaStream_t st) {
   if (c.head_dim == 128) rc = c.code == N730_KV8_INT8 ? N730_SPLIT(128, N730_KV8_INT8) : N730_SPLIT(128, N730_KV8_E4M3);
   else rc = c.code == N730_KV8_INT8 ? N730_SPLIT(64, N730_KV8_INT8) : N730_SPLIT(64, N730_KV8_E4M3);
 #undef N730_SPLIT
-  if (rc || !weights) return rc;
-  KWArgs w{};
-  w.c = c;
-  w.batch = k.batch; w.tokens = k.tokens; w.group = a.group; w.rows = a.rows;
-  w.lens = k.lens; w.n_new = k.n_new;
-  w.scores = a.scores; w.lse = a.lse;
-  w.w_in = k.w_in; w.w_out = k.w_out; w.ldw = k.ldw;
+  if (rc) return rc;
+  KFArgs f{};
+  f.d = a;
+  f.rg = p.rg;
+  f.w_in = k.w_in; f.w_out = k.w_out; f.ldw = k.ldw;
   const int cap = c.max_pages * c.page_size;
-  return kv8_launch(kv8_weights_kernel, dim3((cap + 127) / 128, c.n_kv, k.batch), dim3(128), 0, st, true, w);
+  // rows of a block: one where that leaves the SMs few blocks, more where most items have one part
+  const int64_t all_rows = (int64_t)k.batch * c.n_kv * p.nrg * p.rg;
+  f.rb = 1;
+  while (f.rb < p.rg && all_rows / f.rb > 8 * num_sms()) f.rb *= 2;
+  const dim3 grid(p.nrg * (p.rg / f.rb) + (weights ? (cap + KF_POSITIONS - 1) / KF_POSITIONS : 0), c.n_kv, k.batch);
+  const size_t smem = weights ? (size_t)p.nrg * p.rg * 4 : 0;
+  if (c.head_dim == 128) {
+    if (int e = smem_attr_once<kv8_finish_kernel<128>>(200 << 10)) return e;
+    return kv8_launch(kv8_finish_kernel<128>, grid, dim3(KF_THREADS), smem, st, true, f);
+  }
+  if (int e = smem_attr_once<kv8_finish_kernel<64>>(200 << 10)) return e;
+  return kv8_launch(kv8_finish_kernel<64>, grid, dim3(KF_THREADS), smem, st, true, f);
 }
 
 }  // namespace n730
