@@ -62,7 +62,7 @@ struct KDArgs {
   float scale_log2e;
   const int* lens; const int* n_new;
   int* status;         // set when a wait ran out
-  int* line;           // [batch + 1] prefix sums of the line, for the finishing kernel
+  int2* parts;         // [batch][n_kv][nrg] first CTA and number of parts of an item, for the finishing kernel
   float* part;         // [2 * n_cta][RG][HD]
   float* part_ml;      // [2 * n_cta][RG][4]: reference of the output, max, sum
   float* lse;          // [batch][n_kv][rows] log2 of the softmax sum, +inf for an empty row (items of one run)
@@ -181,8 +181,12 @@ __device__ __forceinline__ int kd_units(int L, int n_new, int cap) {
   return (int)((min((int64_t)L + n_new, (int64_t)cap) + KD_TILE - 1) / KD_TILE);
 }
 
+// a / b for 0 <= a, 0 < b: by 32 bits where that is enough (a 64-bit division is a long sequence)
+__device__ __forceinline__ int64_t kd_div(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
 // the CTA of N whose part of the line of U holds tile u
-__device__ __forceinline__ int kd_owner(int64_t u, int64_t U, int64_t N) { return (int)(((u + 1) * N - 1) / U); }
+__device__ __forceinline__ int kd_owner(int64_t u, int64_t U, int64_t N) { return (int)kd_div((u + 1) * N - 1, U); }
 
 // The answer of row f, channels d..d + 3: sums of weight x V against Mo, of weights l against M.
 template <int HD>
@@ -242,16 +246,14 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
   }
   __syncthreads();
   pdl_launch_dependents();  // the finishing kernel waits for this grid's end
-  if (blockIdx.x == 0)
-    for (int i = tid; i <= a.batch; i += KD_THREADS) a.line[i] = sm.pre[i];
   const int items = c.n_kv * a.nrg;  // per sequence
   const int64_t U = (int64_t)sm.pre[a.batch] * items;
   const int64_t N = min((int64_t)a.n_cta, (U + KD_MIN_UNITS - 1) / KD_MIN_UNITS);
   const int cta = blockIdx.x;
   if (cta >= N) return;
   // one thread walks the CTA's part [u, u1) of the line
-  int64_t u = U * cta / N;
-  const int64_t u1 = U * (cta + 1) / N;
+  int64_t u = kd_div(U * cta, N);
+  const int64_t u1 = kd_div(U * (cta + 1), N);
   int at_b = -1;
   auto next_run = [&](KDSeg& s) {
     s.valid = 0;
@@ -267,7 +269,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
       while ((int64_t)sm.pre[at_b + 1] * items <= u) ++at_b;  // past sequences without tiles
       const int b = at_b, span = sm.pre[b + 1] - sm.pre[b];
       const int64_t base = (int64_t)sm.pre[b] * items, ub = u - base;
-      const int item = (int)(ub / span), off = (int)(ub - (int64_t)item * span);
+      const int item = (int)kd_div(ub, span), off = (int)(ub - (int64_t)item * span);
       const int end = (int)min((int64_t)span, off + (u1 - u));
       u += end - off;
       s.f0 = item % a.nrg * RG;
@@ -280,6 +282,9 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
       s.units = span - KD_ITEM_COST;
       s.L = len_of[b];
       s.total = (int)min((int64_t)s.L + new_of[b], (int64_t)cap);
+      if (s.ta == 0)
+        a.parts[((int64_t)b * c.n_kv + s.h) * a.nrg + s.rg] =
+            make_int2(cta, kd_owner(base + (int64_t)(item + 1) * span - 1, U, N) - cta + 1);
       break;
     }
   };
@@ -329,9 +334,23 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
       cp_async<4>(smem_u32(&sm.sc[warp][st][lane]), s, row >= 0);
     }
   };
+  // the warp's rows of a run's queries: asked for a run ahead and ahead of tiles (two row groups
+  // have no registers for that)
+  constexpr int QR = RG / KD_WARPS, QE = HD / 32;  // rows a warp, channels a lane
+  float qx[QR][QE];
+  auto load_q = [&](const KDSeg& s) {
+#pragma unroll
+    for (int i = 0; i < QR; ++i) {
+      const int r = warp + i * KD_WARPS, f = s.f0 + r;
+      const int64_t qb = ((int64_t)s.b * a.tokens + f / a.group) * a.ldq + (int64_t)(s.h * a.group + f % a.group) * HD + lane * QE;
+#pragma unroll
+      for (int e = 0; e < QE; ++e) qx[i][e] = r < s.nrow ? kv8_load1(a.q, qb + e, a.dtype) : 0.f;
+    }
+  };
   int rows_now = -1;
   if (sm.seg[0].valid) {
     rows_now = lookup(sm.seg[0], 0);
+    if (NB == 1) load_q(sm.seg[0]);
     if (tiles_of(sm.seg[0])) issue(rows_now, 0);
   }
   cp_commit();
@@ -346,17 +365,13 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
     if (tid == WALKER) next_run(sm.seg[(turn + 1) % 3]);
 
     // ---- Q: a row per warp at a time, scaled by a power of two, as the B operand ----
-    for (int r = warp; r < RG; r += KD_WARPS) {
-      constexpr int E = HD / 32;  // channels a lane
-      float x[E];
-      float m = 0.f;
-      const int f = f0 + r;
-      const int64_t qb = r < nrow ? ((int64_t)b * a.tokens + f / a.group) * a.ldq + (int64_t)(h * a.group + f % a.group) * HD : 0;
+    if (NB == 2) load_q(run);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        x[e] = r < nrow ? kv8_load1(a.q, qb + lane * E + e, a.dtype) : 0.f;
-        m = fmaxf(m, fabsf(x[e]));
-      }
+    for (int i = 0; i < QR; ++i) {
+      const int r = warp + i * KD_WARPS;
+      float m = 0.f;
+#pragma unroll
+      for (int e = 0; e < QE; ++e) m = fmaxf(m, fabsf(qx[i][e]));
       m = warp_max(m);
       // the largest magnitude goes into [2^13, 2^14); rows of zeros or with an infinity stay
       const int ex = (int)((__float_as_uint(m) >> 23) & 255u);
@@ -365,9 +380,9 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
       const float mul = __uint_as_float((uint32_t)(127 + sh) << 23);
       if (lane == 0) sm.rowmul[r] = a.scale_log2e * __uint_as_float((uint32_t)(127 - sh) << 23);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int dch = lane * E + e, ks = (dch >> 6) * 4 + ((dch >> 2) & 3), tt = (dch >> 4) & 3, w = dch & 3;
-        const float y = x[e] * mul;
+      for (int e = 0; e < QE; ++e) {
+        const int dch = lane * QE + e, ks = (dch >> 6) * 4 + ((dch >> 2) & 3), tt = (dch >> 4) & 3, w = dch & 3;
+        const float y = qx[i][e] * mul;
         const __half hi = __float2half_rn(y);
         reinterpret_cast<__half*>(&sm.qf[LO ? 0 : r >> 3][ks][(r & 7) * 4 + tt])[w] = hi;
         if (LO)  // an infinite y gives NaN, as it should
@@ -598,7 +613,10 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
     __syncwarp();
     // the next run's first tile goes into one buffer, this run's outputs into the other
     rows_now = rows_after;
-    if (after.valid && tiles_of(after)) issue(rows_now, 0);
+    if (after.valid) {
+      if (NB == 1) load_q(after);
+      if (tiles_of(after)) issue(rows_now, 0);
+    }
     cp_commit();
     float* const mine = reinterpret_cast<float*>(sm.ring[warp][fills % ST]);  // [row][HD], 16-byte groups spread by row
 
@@ -681,39 +699,41 @@ struct KFArgs {
   int64_t ldw;
 };
 
-// An item's parts: slots c0 .. c0 + n - 1 (the first CTA's second slot, the others' first).
-struct KFParts { int c0, n; };
-__device__ __forceinline__ KFParts kf_parts(const KFArgs& a, int b, int h, int rg) {
-  const KDArgs& d = a.d;
-  const int items = d.c.n_kv * d.nrg, span = d.line[b + 1] - d.line[b];
-  const int64_t U = (int64_t)d.line[d.batch] * items;
-  const int64_t N = min((int64_t)d.n_cta, (U + KD_MIN_UNITS - 1) / KD_MIN_UNITS);
-  const int64_t u0 = (int64_t)d.line[b] * items + (int64_t)(h * d.nrg + rg) * span;
-  const int c0 = kd_owner(u0 + KD_ITEM_COST, U, N);
-  return {c0, kd_owner(u0 + span - 1, U, N) - c0 + 1};
+// An item's parts: row r of part k lies in the first CTA's second slot (k = 0), the others' first.
+__device__ __forceinline__ int64_t kf_row(const KFArgs& a, const int2& p, int k, int r) {
+  return (int64_t)(2 * (p.x + k) + (k == 0)) * a.rg + r;
 }
-__device__ __forceinline__ int64_t kf_row(const KFArgs& a, const KFParts& p, int k, int r) {
-  return (int64_t)(2 * (p.c0 + k) + (k == 0)) * a.rg + r;
-}
-// A warp's (reference of the outputs, maximum, sum) of row r over the parts.
-__device__ __forceinline__ float4 kf_totals(const KFArgs& a, const KFParts& p, int r) {
-  float Mo = -INFINITY, M = -INFINITY, l = 0.f;
-  for (int k = threadIdx.x & 31; k < p.n; k += 32) {
+// A warp's log2 of the softmax sum of row r over the parts (+inf for an empty row).
+__device__ __forceinline__ float kf_lse_of(const KFArgs& a, const int2& p, int r) {
+  float M = -INFINITY, l = 0.f;
+  for (int k = threadIdx.x & 31; k < p.y; k += 32) {
     const float4 ml = reinterpret_cast<const float4*>(a.d.part_ml)[kf_row(a, p, k, r)];
-    Mo = fmaxf(Mo, ml.x);
     const float m = fmaxf(M, ml.y), ms = m == -INFINITY ? 0.f : m;
     l = l * ex2(M - ms) + ml.z * ex2(ml.y - ms);
     M = m;
   }
   const float m = warp_max(M), ms = m == -INFINITY ? 0.f : m;
-  return make_float4(warp_max(Mo), m, warp_sum(l * ex2(M - ms)), 0.f);
+  l = warp_sum(l * ex2(M - ms));
+  return l == 0.f ? INFINITY : m + lg2(l);
+}
+
+// sums of weight x V against mo, and of weights l against m, of two sets of parts
+struct KFSum { float4 num; float mo, m, l; };
+__device__ __forceinline__ void kf_add(KFSum& s, const float4& x, float mo, float m, float l) {
+  const float o1 = fmaxf(s.mo, mo), os = o1 == -INFINITY ? 0.f : o1, m1 = fmaxf(s.m, m), ms = m1 == -INFINITY ? 0.f : m1;
+  const float f = ex2(s.mo - os), g = ex2(mo - os);
+  s.num.x = fmaf(x.x, g, s.num.x * f); s.num.y = fmaf(x.y, g, s.num.y * f);
+  s.num.z = fmaf(x.z, g, s.num.z * f); s.num.w = fmaf(x.w, g, s.num.w * f);
+  s.l = s.l * ex2(s.m - ms) + l * ex2(m - ms);
+  s.mo = o1;
+  s.m = m1;
 }
 
 template <int HD>
 __global__ void __launch_bounds__(KF_THREADS) kv8_finish_kernel(const KFArgs a) {
   constexpr int LPP = HD / 4, WARPS = KF_THREADS / 32;  // lanes that a part of a row takes
   extern __shared__ float kf_lse[];
-  __shared__ float4 share[KF_THREADS];
+  __shared__ KFSum share[KF_THREADS];
   const KDArgs& d = a.d;
   const N730KV8Cache& c = d.c;
   const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -724,34 +744,36 @@ __global__ void __launch_bounds__(KF_THREADS) kv8_finish_kernel(const KFArgs a) 
   if ((int)blockIdx.x < joins) {
     const int rg = blockIdx.x / (a.rg / a.rb), first = blockIdx.x % (a.rg / a.rb) * a.rb, f0 = rg * a.rg;
     if (f0 + first >= rows_b) return;
-    const KFParts p = kf_parts(a, b, h, rg);
-    if (p.n == 1) return;  // its CTA gave the answer
+    const int2 p = d.parts[((int64_t)b * c.n_kv + h) * d.nrg + rg];
+    if (p.y == 1) return;  // its CTA gave the answer
     const int per_row = a.rb >= WARPS ? 1 : WARPS / a.rb;  // warps
     const int shares = per_row * (32 / LPP), mine = warp % per_row * (32 / LPP) + lane / LPP, d4 = lane % LPP;
     for (int i = 0; i < a.rb; i += WARPS / per_row) {
       const int r = first + i + warp / per_row;
       const bool live = f0 + r < rows_b;
-      float4 t = make_float4(0.f, 0.f, 0.f, 0.f), num = t;
-      if (live) {
-        t = kf_totals(a, p, r);
-        const float mos = t.x == -INFINITY ? 0.f : t.x;
-#pragma unroll 8
-        for (int k = mine; k < p.n; k += shares) {
-          const int64_t at = kf_row(a, p, k, r);
-          const float f = ex2(d.part_ml[at * 4] - mos);
-          const float4 x = reinterpret_cast<const float4*>(d.part + at * HD)[d4];
-          num.x = fmaf(x.x, f, num.x); num.y = fmaf(x.y, f, num.y); num.z = fmaf(x.z, f, num.z); num.w = fmaf(x.w, f, num.w);
+      KFSum sum{make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, -INFINITY, 0.f};
+      constexpr int CH = 8;  // parts asked for together
+      for (int k0 = mine; live && k0 < p.y; k0 += CH * shares) {
+        float4 ml[CH], x[CH];
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+          const int64_t at = kf_row(a, p, min(k0 + j * shares, p.y - 1), r);
+          ml[j] = reinterpret_cast<const float4*>(d.part_ml)[at];
+          x[j] = reinterpret_cast<const float4*>(d.part + at * HD)[d4];
         }
+#pragma unroll
+        for (int j = 0; j < CH; ++j)
+          if (k0 + j * shares < p.y) kf_add(sum, x[j], ml[j].x, ml[j].y, ml[j].z);
       }
       __syncthreads();
-      share[tid] = num;
+      share[tid] = sum;
       __syncthreads();
       if (live && mine == 0) {  // the shares in order
         for (int k = 1; k < shares; ++k) {
-          const float4 x = share[tid + k * LPP];
-          num.x += x.x; num.y += x.y; num.z += x.z; num.w += x.w;
+          const KFSum& t = share[tid + k * LPP];
+          kf_add(sum, t.num, t.mo, t.m, t.l);
         }
-        kd_answer<HD>(d, b, h, f0 + r, d4 * 4, num, t.x, t.y, t.z);
+        kd_answer<HD>(d, b, h, f0 + r, d4 * 4, sum.num, sum.mo, sum.m, sum.l);
       }
     }
     return;
@@ -761,36 +783,39 @@ __global__ void __launch_bounds__(KF_THREADS) kv8_finish_kernel(const KFArgs a) 
   const int p0 = ((int)blockIdx.x - joins) * KF_POSITIONS;
   if (p0 >= total) return;
   const int64_t head = (int64_t)b * c.n_kv + h;
-  for (int rg = 0; rg * a.rg < rows_b; ++rg) {
-    const KFParts p = kf_parts(a, b, h, rg);
-    const int nrow = min(a.rg, rows_b - rg * a.rg);
-    for (int r = warp; r < nrow; r += KF_THREADS / 32) {
-      float lse;
-      if (p.n == 1) {
-        lse = d.lse[head * d.rows + rg * a.rg + r];
-      } else {
-        const float4 t = kf_totals(a, p, r);
-        lse = t.z == 0.f ? INFINITY : t.y + lg2(t.z);
+  const int at = p0 + 4 * tid;  // cap is a multiple of 16: four positions are there or none
+  const float* s = d.scores + head * d.rows * cap + min(at, cap - 4);
+  const float* w_in = a.w_in ? a.w_in + head * a.ldw : nullptr;
+  constexpr int CH = 8;  // rows asked for together, the first ones before the sums are known
+  float4 x[CH];
+  auto load = [&](int f) {
+#pragma unroll
+    for (int j = 0; j < CH; ++j) x[j] = *reinterpret_cast<const float4*>(s + (int64_t)min(f + j, rows_b - 1) * cap);
+  };
+  float w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = w_in && at + e < min(L, total) ? w_in[at + e] : 0.f;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  if (rows_b) {
+    load(0);
+    for (int f = warp; f < rows_b; f += KF_THREADS / 32) {
+      const int2 p = d.parts[head * d.nrg + f / a.rg];
+      const float lse = p.y == 1 ? d.lse[head * d.rows + f] : kf_lse_of(a, p, f % a.rg);
+      if (lane == 0) kf_lse[f] = lse;
+    }
+    __syncthreads();
+    for (int f = 0; f < rows_b; f += CH) {
+      if (f) load(f);
+#pragma unroll
+      for (int j = 0; j < CH; ++j) {
+        const float lse = f + j < rows_b ? kf_lse[f + j] : INFINITY;
+        sum[0] += ex2(x[j].x - lse); sum[1] += ex2(x[j].y - lse); sum[2] += ex2(x[j].z - lse); sum[3] += ex2(x[j].w - lse);
       }
-      if (lane == 0) kf_lse[rg * a.rg + r] = lse;
     }
   }
-  __syncthreads();
-  const int at = p0 + 4 * tid;  // cap is a multiple of 16: four positions are there or none
-  if (at >= total) return;
-  const float* s = d.scores + head * d.rows * cap + at;
-  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int f = 0; f < rows_b; ++f) {
-    const float4 x = *reinterpret_cast<const float4*>(s + (int64_t)f * cap);
-    const float lse = kf_lse[f];
-    sum.x += ex2(x.x - lse); sum.y += ex2(x.y - lse); sum.z += ex2(x.z - lse); sum.w += ex2(x.w - lse);
-  }
-  const float w[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (at + e < total)
-      a.w_out[head * a.ldw + at + e] = (a.w_in && at + e < L ? a.w_in[head * a.ldw + at + e] : 0.f) + w[e];
+    if (at + e < total) a.w_out[head * a.ldw + at + e] = w[e] + sum[e];
 }
 
 // ---------------------------------------------------------------------------
@@ -798,7 +823,7 @@ __global__ void __launch_bounds__(KF_THREADS) kv8_finish_kernel(const KFArgs a) 
 // ---------------------------------------------------------------------------
 struct KDPlan {
   int rg, nrg, n_cta;
-  int64_t part, ml, lse, scores, bytes;  // offsets; the status word is at 0, the line at 256
+  int64_t part, ml, lse, scores, bytes;  // offsets; the status word is at 0, the parts table at 256
 };
 static KDPlan kd_plan(const N730KV8Cache& c, int batch, int tokens, int heads, int dtype, bool weights) {
   KDPlan p{};
@@ -808,7 +833,7 @@ static KDPlan kd_plan(const N730KV8Cache& c, int batch, int tokens, int heads, i
   p.nrg = (int)((rows + p.rg - 1) / p.rg);
   p.n_cta = KD_CTAS_PER_SM * num_sms();
   auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-  p.part = 256 + up((int64_t)(batch + 1) * 4);
+  p.part = 256 + up((int64_t)batch * c.n_kv * p.nrg * 8);
   p.ml = p.part + up((int64_t)2 * p.n_cta * p.rg * c.head_dim * 4);
   p.lse = p.ml + up((int64_t)2 * p.n_cta * p.rg * 16);
   p.scores = p.lse + (weights ? up((int64_t)batch * c.n_kv * rows * 4) : 0);
@@ -886,7 +911,7 @@ int kv8_attention_launch(const KV8AttnCall& k, cudaStream_t st) {
   a.scale_log2e = k.scale * 1.4426950408889634f;
   a.lens = k.lens; a.n_new = k.n_new;
   a.status = reinterpret_cast<int*>(ws);
-  a.line = reinterpret_cast<int*>(ws + 256);
+  a.parts = reinterpret_cast<int2*>(ws + 256);
   a.part = reinterpret_cast<float*>(ws + p.part);
   a.part_ml = reinterpret_cast<float*>(ws + p.ml);
   a.lse = weights ? reinterpret_cast<float*>(ws + p.lse) : nullptr;
