@@ -33,6 +33,14 @@ struct KV8AttnCall {
 int64_t kv8_attention_ws(const N730KV8Cache& c, int batch, int tokens, int heads, bool weights);
 int kv8_attention_launch(const KV8AttnCall& a, cudaStream_t st);
 
+// The tensor-memory kernel for prompts (kv8_prompt.cu): 256 rows of an item a CTA, the positions in
+// `splits` shares whose parts lie as [item tile][split][rg rows].
+struct KV8PromptPlan { int rows, tiles, splits, rg; };
+KV8PromptPlan kv8_prompt_plan(const N730KV8Cache& c, int batch, int tokens, int heads);
+int kv8_prompt_launch(const KV8AttnCall& k, const KV8PromptPlan& p, int* status, float* part, float* part_ml, float* lse,
+                      cudaStream_t st);
+int kv8_prompt_weights_launch(const KV8AttnCall& k, const KV8PromptPlan& p, int* status, float* lse, cudaStream_t st);
+
 // one element of a row in the caller's type, widened to fp32
 __device__ __forceinline__ float kv8_load1(const void* p, int64_t i, int dtype) {
   if (dtype == N730_F32) return reinterpret_cast<const float*>(p)[i];
@@ -52,6 +60,32 @@ __device__ __forceinline__ int kv8_len(const int* lens, int b, int cap) { return
 __device__ __forceinline__ int kv8_new(const int* n_new, int b, int tokens) {
   return n_new ? min(max(n_new[b], 0), tokens) : tokens;
 }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+// two codes (the bytes of x selected by SEL: low or high pair) as fp16
+template <int CODE, int HIGH>
+__device__ __forceinline__ uint32_t codes2(uint32_t x) {
+  if (CODE == N730_KV8_INT8) {  // x has its sign bits flipped: bytes 128 + q
+    const uint32_t y = __byte_perm(x, 0x64646464u, HIGH ? 0x4342 : 0x4140);
+    return h2_bits(__hsub2(*reinterpret_cast<const __half2*>(&y), __float2half2_rn(1152.f)));
+  }
+  uint32_t y;
+  asm("{\n .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %1;\n cvt.rn.f16x2.e4m3x2 %0, %2;\n}"
+      : "=r"(y) : "r"(x), "h"((uint16_t)(HIGH ? x >> 16 : x)));
+  return y;
+}
+template <int CODE>
+__device__ __forceinline__ uint32_t code_word(uint32_t x) { return CODE == N730_KV8_INT8 ? x ^ 0x80808080u : x; }
 
 // Launch with or without programmatic dependent launch.
 template <typename... KArgs, typename... Args>

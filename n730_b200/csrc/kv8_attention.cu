@@ -58,7 +58,8 @@ struct KDArgs {
   N730KV8Cache c;
   const void* q; void* out;
   int64_t ldq, ldo;
-  int dtype, batch, tokens, heads, group, rows, nrg;  // rows = tokens * group; nrg row groups of RG
+  int dtype, batch, tokens, heads, group, rows, nrg;  // rows = chunk * group; nrg row groups of RG
+  int t0, chunk;       // the call's tokens [t0, t0 + chunk) of each sequence
   float scale_log2e;
   const int* lens; const int* n_new;
   int* status;         // set when a wait ran out
@@ -111,17 +112,6 @@ struct KDSmem {
   int pre[1];                      // [batch + 1] prefix sums of the line, then [batch] lengths, [batch] new rows
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float lg2(float x) {
-  float y;
-  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) { return h2_bits(__floats2half2_rn(lo, hi)); }
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
@@ -161,21 +151,13 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
 
-// two codes (the bytes of x selected by SEL: low or high pair) as fp16
-template <int CODE, int HIGH>
-__device__ __forceinline__ uint32_t codes2(uint32_t x) {
-  if (CODE == N730_KV8_INT8) {  // x has its sign bits flipped: bytes 128 + q
-    const uint32_t y = __byte_perm(x, 0x64646464u, HIGH ? 0x4342 : 0x4140);
-    return h2_bits(__hsub2(*reinterpret_cast<const __half2*>(&y), __float2half2_rn(1152.f)));
-  }
-  uint32_t y;
-  asm("{\n .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %1;\n cvt.rn.f16x2.e4m3x2 %0, %2;\n}"
-      : "=r"(y) : "r"(x), "h"((uint16_t)(HIGH ? x >> 16 : x)));
-  return y;
+// a sequence's new rows among tokens [t0, t0 + chunk), and the positions cached before them
+__device__ __forceinline__ int kd_new(const KDArgs& a, int b) {
+  return min(max(kv8_new(a.n_new, b, a.tokens) - a.t0, 0), a.chunk);
 }
-template <int CODE>
-__device__ __forceinline__ uint32_t code_word(uint32_t x) { return CODE == N730_KV8_INT8 ? x ^ 0x80808080u : x; }
-
+__device__ __forceinline__ int kd_len(const KDArgs& a, int b, int cap) {
+  return (int)min((int64_t)kv8_len(a.lens, b, cap) + a.t0, (int64_t)cap);
+}
 // tiles of a sequence with new rows
 __device__ __forceinline__ int kd_units(int L, int n_new, int cap) {
   return (int)((min((int64_t)L + n_new, (int64_t)cap) + KD_TILE - 1) / KD_TILE);
@@ -192,7 +174,7 @@ __device__ __forceinline__ int kd_owner(int64_t u, int64_t U, int64_t N) { retur
 template <int HD>
 __device__ __forceinline__ void kd_answer(const KDArgs& a, int b, int h, int f, int d, const float4& num, float Mo, float M, float l) {
   const float s = l == 0.f ? 0.f : (Mo == -INFINITY ? 0.f : ex2(Mo - M)) / l;  // a NaN query: NaN
-  const int64_t at = ((int64_t)b * a.tokens + f / a.group) * a.ldo + (int64_t)(h * a.group + f % a.group) * HD + d;
+  const int64_t at = ((int64_t)b * a.tokens + a.t0 + f / a.group) * a.ldo + (int64_t)(h * a.group + f % a.group) * HD + d;
   kv8_store1(a.out, at, a.dtype, num.x * s);
   kv8_store1(a.out, at + 1, a.dtype, num.y * s);
   kv8_store1(a.out, at + 2, a.dtype, num.z * s);
@@ -230,7 +212,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
       const int b = b0 + lane;
       int v = 0;
       if (b < a.batch) {
-        const int n = kv8_new(a.n_new, b, a.tokens), L = kv8_len(a.lens, b, cap);
+        const int n = kd_new(a, b), L = kd_len(a, b, cap);
         len_of[b] = L;
         new_of[b] = n;
         v = n ? kd_units(L, n, cap) + KD_ITEM_COST : 0;
@@ -342,7 +324,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
 #pragma unroll
     for (int i = 0; i < QR; ++i) {
       const int r = warp + i * KD_WARPS, f = s.f0 + r;
-      const int64_t qb = ((int64_t)s.b * a.tokens + f / a.group) * a.ldq + (int64_t)(s.h * a.group + f % a.group) * HD + lane * QE;
+      const int64_t qb = ((int64_t)s.b * a.tokens + a.t0 + f / a.group) * a.ldq + (int64_t)(s.h * a.group + f % a.group) * HD + lane * QE;
 #pragma unroll
       for (int e = 0; e < QE; ++e) qx[i][e] = r < s.nrow ? kv8_load1(a.q, qb + e, a.dtype) : 0.f;
     }
@@ -695,13 +677,17 @@ constexpr int KF_POSITIONS = 4 * KF_THREADS;
 struct KFArgs {
   KDArgs d;
   int rg, rb;
+  int splits;  // parts of every item, one behind the other (prompts); 0: by the table
   const float* w_in; float* w_out;
   int64_t ldw;
 };
 
 // An item's parts: row r of part k lies in the first CTA's second slot (k = 0), the others' first.
 __device__ __forceinline__ int64_t kf_row(const KFArgs& a, const int2& p, int k, int r) {
-  return (int64_t)(2 * (p.x + k) + (k == 0)) * a.rg + r;
+  return (a.splits ? (int64_t)(p.x + k) : (int64_t)(2 * (p.x + k) + (k == 0))) * a.rg + r;
+}
+__device__ __forceinline__ int2 kf_parts(const KFArgs& a, int64_t item) {
+  return a.splits ? make_int2((int)item * a.splits, a.splits) : a.d.parts[item];
 }
 // A warp's log2 of the softmax sum of row r over the parts (+inf for an empty row).
 __device__ __forceinline__ float kf_lse_of(const KFArgs& a, const int2& p, int r) {
@@ -739,12 +725,12 @@ __global__ void __launch_bounds__(KF_THREADS) kv8_finish_kernel(const KFArgs a) 
   const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cap = c.max_pages * c.page_size;
   pdl_wait();
-  const int n_new = kv8_new(d.n_new, b, d.tokens), rows_b = n_new * d.group;
+  const int n_new = kd_new(d, b), rows_b = n_new * d.group;
   const int joins = d.nrg * (a.rg / a.rb);
   if ((int)blockIdx.x < joins) {
     const int rg = blockIdx.x / (a.rg / a.rb), first = blockIdx.x % (a.rg / a.rb) * a.rb, f0 = rg * a.rg;
     if (f0 + first >= rows_b) return;
-    const int2 p = d.parts[((int64_t)b * c.n_kv + h) * d.nrg + rg];
+    const int2 p = kf_parts(a, ((int64_t)b * c.n_kv + h) * d.nrg + rg);
     if (p.y == 1) return;  // its CTA gave the answer
     const int per_row = a.rb >= WARPS ? 1 : WARPS / a.rb;  // warps
     const int shares = per_row * (32 / LPP), mine = warp % per_row * (32 / LPP) + lane / LPP, d4 = lane % LPP;
@@ -774,12 +760,15 @@ __global__ void __launch_bounds__(KF_THREADS) kv8_finish_kernel(const KFArgs a) 
           kf_add(sum, t.num, t.mo, t.m, t.l);
         }
         kd_answer<HD>(d, b, h, f0 + r, d4 * 4, sum.num, sum.mo, sum.m, sum.l);
+        if (a.splits && d.lse && d4 == 0)  // for the prompt's weights
+          d.lse[((int64_t)b * c.n_kv + h) * d.rows + f0 + r] = sum.l == 0.f ? INFINITY : sum.m + lg2(sum.l);
       }
     }
     return;
   }
   // ---- weights ----
-  const int L = kv8_len(d.lens, b, cap), total = (int)min((int64_t)L + n_new, (int64_t)cap);
+  if (d.t0 && n_new == 0) return;  // a later chunk without rows of this sequence
+  const int L = kd_len(d, b, cap), total = (int)min((int64_t)L + n_new, (int64_t)cap);
   const int p0 = ((int)blockIdx.x - joins) * KF_POSITIONS;
   if (p0 >= total) return;
   const int64_t head = (int64_t)b * c.n_kv + h;
@@ -799,7 +788,7 @@ __global__ void __launch_bounds__(KF_THREADS) kv8_finish_kernel(const KFArgs a) 
   if (rows_b) {
     load(0);
     for (int f = warp; f < rows_b; f += KF_THREADS / 32) {
-      const int2 p = d.parts[head * d.nrg + f / a.rg];
+      const int2 p = kf_parts(a, head * d.nrg + f / a.rg);
       const float lse = p.y == 1 ? d.lse[head * d.rows + f] : kf_lse_of(a, p, f % a.rg);
       if (lane == 0) kf_lse[f] = lse;
     }
@@ -821,23 +810,44 @@ __global__ void __launch_bounds__(KF_THREADS) kv8_finish_kernel(const KFArgs a) 
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
+// Rows of an item from which the prompt kernel takes a call: below, its 256-row tiles are mostly empty and
+// the split kernel's 16-row groups read K and V few enough times.
+constexpr int KD_ROWS_MAX = 64;
+
 struct KDPlan {
+  bool prompt;
+  int chunk;  // tokens a launch: fp32 rows keep to the split kernel, which has both their terms
+  KV8PromptPlan pp;
   int rg, nrg, n_cta;
   int64_t part, ml, lse, scores, bytes;  // offsets; the status word is at 0, the parts table at 256
 };
 static KDPlan kd_plan(const N730KV8Cache& c, int batch, int tokens, int heads, int dtype, bool weights) {
   KDPlan p{};
-  const int64_t rows = (int64_t)tokens * (heads / c.n_kv);
-  // fp32 rows take both terms' products, and up to 8 rows need no second group of columns
-  p.rg = dtype == N730_F32 || rows <= 8 ? 8 : 16;
-  p.nrg = (int)((rows + p.rg - 1) / p.rg);
-  p.n_cta = KD_CTAS_PER_SM * num_sms();
+  const int group = heads / c.n_kv;
+  const int64_t items = (int64_t)batch * c.n_kv;
+  p.prompt = (int64_t)tokens * group > KD_ROWS_MAX && dtype != N730_F32;
+  p.chunk = p.prompt || (int64_t)tokens * group <= KD_ROWS_MAX ? tokens : std::max(1, KD_ROWS_MAX / group);
+  const int64_t rows = (int64_t)p.chunk * group;
   auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-  p.part = 256 + up((int64_t)batch * c.n_kv * p.nrg * 8);
-  p.ml = p.part + up((int64_t)2 * p.n_cta * p.rg * c.head_dim * 4);
-  p.lse = p.ml + up((int64_t)2 * p.n_cta * p.rg * 16);
-  p.scores = p.lse + (weights ? up((int64_t)batch * c.n_kv * rows * 4) : 0);
-  p.bytes = p.scores + (weights ? (int64_t)batch * c.n_kv * rows * c.max_pages * c.page_size * 4 : 0);
+  int64_t slots;
+  if (p.prompt) {
+    p.pp = kv8_prompt_plan(c, batch, tokens, heads);
+    p.rg = p.pp.rg;
+    p.nrg = p.pp.tiles;
+    p.part = 256;
+    slots = p.pp.splits > 1 ? items * p.nrg * p.pp.splits : 0;
+  } else {
+    // fp32 rows take both terms' products, and up to 8 rows need no second group of columns
+    p.rg = dtype == N730_F32 || rows <= 8 ? 8 : 16;
+    p.nrg = (int)((rows + p.rg - 1) / p.rg);
+    p.n_cta = KD_CTAS_PER_SM * num_sms();
+    p.part = 256 + up(items * p.nrg * 8);
+    slots = 2 * p.n_cta;
+  }
+  p.ml = p.part + up(slots * p.rg * c.head_dim * 4);
+  p.lse = p.ml + up(slots * p.rg * 16);
+  p.scores = p.lse + (weights ? up(items * rows * 4) : 0);
+  p.bytes = p.scores + (weights && !p.prompt ? items * rows * c.max_pages * c.page_size * 4 : 0);
   return p;
 }
 
@@ -898,6 +908,25 @@ static int split_launch(const KDArgs& a, const CUtensorMap& km, const CUtensorMa
                     pdl, a, km, vm);
 }
 
+static int finish_launch(const KV8AttnCall& k, const KDPlan& p, const KDArgs& a, cudaStream_t st) {
+  const float* w_in = a.t0 ? k.w_out : k.w_in;  // a later chunk adds to the ones before
+  const bool weights = k.w_out && !p.prompt;
+  KFArgs f{};
+  f.d = a;
+  f.rg = p.rg;
+  f.splits = p.prompt ? p.pp.splits : 0;
+  f.w_in = w_in; f.w_out = k.w_out; f.ldw = k.ldw;
+  const int cap = k.c.max_pages * k.c.page_size;
+  // rows of a block: one where that leaves the SMs few blocks, more where most items have one part
+  const int64_t all_rows = (int64_t)k.batch * k.c.n_kv * p.nrg * p.rg;
+  f.rb = 1;
+  while (f.rb < p.rg && all_rows / f.rb > 8 * num_sms()) f.rb *= 2;
+  const dim3 grid(p.nrg * (p.rg / f.rb) + (weights ? (cap + KF_POSITIONS - 1) / KF_POSITIONS : 0), k.c.n_kv, k.batch);
+  const size_t smem = weights ? (size_t)p.nrg * p.rg * 4 : 0;
+  if (k.c.head_dim == 128) return kv8_launch(kv8_finish_kernel<128>, grid, dim3(KF_THREADS), smem, st, true, f);
+  return kv8_launch(kv8_finish_kernel<64>, grid, dim3(KF_THREADS), smem, st, true, f);
+}
+
 int kv8_attention_launch(const KV8AttnCall& k, cudaStream_t st) {
   const N730KV8Cache& c = k.c;
   const bool weights = k.w_out != nullptr;
@@ -907,7 +936,8 @@ int kv8_attention_launch(const KV8AttnCall& k, cudaStream_t st) {
   a.c = c;
   a.q = k.q; a.out = k.out; a.ldq = k.ldq; a.ldo = k.ldo; a.dtype = k.dtype;
   a.batch = k.batch; a.tokens = k.tokens; a.heads = k.heads; a.group = k.heads / c.n_kv;
-  a.rows = k.tokens * a.group; a.nrg = p.nrg;
+  a.rows = p.chunk * a.group; a.nrg = p.nrg;
+  a.chunk = p.chunk;
   a.scale_log2e = k.scale * 1.4426950408889634f;
   a.lens = k.lens; a.n_new = k.n_new;
   a.status = reinterpret_cast<int*>(ws);
@@ -915,10 +945,16 @@ int kv8_attention_launch(const KV8AttnCall& k, cudaStream_t st) {
   a.part = reinterpret_cast<float*>(ws + p.part);
   a.part_ml = reinterpret_cast<float*>(ws + p.ml);
   a.lse = weights ? reinterpret_cast<float*>(ws + p.lse) : nullptr;
-  a.scores = weights ? reinterpret_cast<float*>(ws + p.scores) : nullptr;
+  a.scores = weights && !p.prompt ? reinterpret_cast<float*>(ws + p.scores) : nullptr;
   a.n_cta = p.n_cta;
   a.log_block = c.block == 16 ? 4 : c.block == 32 ? 5 : 6;
   a.box = c.page_size % KD_TILE == 0 ? KD_TILE : 16;
+  if (p.prompt) {
+    if (int rc = kv8_prompt_launch(k, p.pp, a.status, a.part, a.part_ml, a.lse, st)) return rc;
+    if (p.pp.splits > 1)
+      if (int rc = finish_launch(k, p, a, st)) return rc;
+    return weights ? kv8_prompt_weights_launch(k, p.pp, a.status, a.lse, st) : N730_OK;
+  }
   CUtensorMap km, vm;
   int rc = kv8_map(c, c.k_codes, a.box, &km);
   if (!rc) rc = kv8_map(c, c.v_codes, a.box, &vm);
@@ -927,27 +963,14 @@ int kv8_attention_launch(const KV8AttnCall& k, cudaStream_t st) {
   (k.dtype == N730_F32 ? split_launch<HD, CODE, 1, true>(a, km, vm, k.pdl, st)       \
    : p.rg == 8         ? split_launch<HD, CODE, 1, false>(a, km, vm, k.pdl, st)      \
                        : split_launch<HD, CODE, 2, false>(a, km, vm, k.pdl, st))
-  if (c.head_dim == 128) rc = c.code == N730_KV8_INT8 ? N730_SPLIT(128, N730_KV8_INT8) : N730_SPLIT(128, N730_KV8_E4M3);
-  else rc = c.code == N730_KV8_INT8 ? N730_SPLIT(64, N730_KV8_INT8) : N730_SPLIT(64, N730_KV8_E4M3);
-#undef N730_SPLIT
-  if (rc) return rc;
-  KFArgs f{};
-  f.d = a;
-  f.rg = p.rg;
-  f.w_in = k.w_in; f.w_out = k.w_out; f.ldw = k.ldw;
-  const int cap = c.max_pages * c.page_size;
-  // rows of a block: one where that leaves the SMs few blocks, more where most items have one part
-  const int64_t all_rows = (int64_t)k.batch * c.n_kv * p.nrg * p.rg;
-  f.rb = 1;
-  while (f.rb < p.rg && all_rows / f.rb > 8 * num_sms()) f.rb *= 2;
-  const dim3 grid(p.nrg * (p.rg / f.rb) + (weights ? (cap + KF_POSITIONS - 1) / KF_POSITIONS : 0), c.n_kv, k.batch);
-  const size_t smem = weights ? (size_t)p.nrg * p.rg * 4 : 0;
-  if (c.head_dim == 128) {
-    if (int e = smem_attr_once<kv8_finish_kernel<128>>(200 << 10)) return e;
-    return kv8_launch(kv8_finish_kernel<128>, grid, dim3(KF_THREADS), smem, st, true, f);
+  for (; a.t0 < k.tokens; a.t0 += p.chunk) {
+    if (c.head_dim == 128) rc = c.code == N730_KV8_INT8 ? N730_SPLIT(128, N730_KV8_INT8) : N730_SPLIT(128, N730_KV8_E4M3);
+    else rc = c.code == N730_KV8_INT8 ? N730_SPLIT(64, N730_KV8_INT8) : N730_SPLIT(64, N730_KV8_E4M3);
+    if (!rc) rc = finish_launch(k, p, a, st);
+    if (rc) return rc;
   }
-  if (int e = smem_attr_once<kv8_finish_kernel<64>>(200 << 10)) return e;
-  return kv8_launch(kv8_finish_kernel<64>, grid, dim3(KF_THREADS), smem, st, true, f);
+#undef N730_SPLIT
+  return N730_OK;
 }
 
 }  // namespace n730

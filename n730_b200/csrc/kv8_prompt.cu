@@ -1,0 +1,714 @@
+// Prompt attention over the 8-bit paged key/value cache on the 5th-generation tensor cores.
+//
+//   out[b, t, head] = softmax_p(scale q . k_p) v_p,  positions p <= lens[b] + t of KV head head / G
+//
+// The rows of an item (sequence, KV head) are its tokens x G query heads, row = token * G + head, so
+// every row of a tile reads the same K and V.  One CTA takes 256 rows (two 128-row tiles, A and B) and
+// walks over the positions in tiles of 128:
+//   warps 8-11  load the tile's codes (16 bytes a lane, whole 128-byte rows), turn them into fp16
+//               exactly and store them swizzled: K as [64-channel block][position][128 B], the K-major
+//               operand of S = Q K^T; V in the same layout, which is the MN-major operand of O += P V.
+//               Each conversion serves 256 rows;
+//   warp 12     issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory) of
+//               A and B in turn, so that one's products run while the other's softmax does;
+//   warps 0-3   softmax of A, warps 4-7 of B: a thread owns a row (TMEM lane).  P, fp16, overwrites the
+//               tile's scores in place.
+// Tensor memory: scores of A and B, 128 columns each, outputs of A and B, head_dim columns each.
+//
+// Softmax.  The weight x V scale of a position is formed by one FMA and one exp2: its exponent is
+// score * (row, block factor) + log2(V scale) - reference, and the sum of weights gets each block's sum
+// times 2^(reference - maximum) / V scale.  Both references follow the largest values lazily (2^8 of
+// slack), so outputs in tensor memory are rescaled only when a row's maximum has grown by that much.
+//
+// Bounds: per 128x128 tile 2 x 1024 cycles of tensor work for head_dim 128 against 1024 of exp2 and about
+// as many of issue slots on the 4 schedulers, for each of A and B.
+//
+// Numerics: 16-bit queries are exact in fp16 after a power-of-two scaling of their row; the softmax
+// weights are rounded to fp16 (2^-11 of each, below the rounding of a 16-bit output).  Sums and outputs are
+// fp32.  fp32 queries do not come here.
+// Every wait is bounded; one that runs out sets the workspace's status word, ends the CTA's work and
+// still frees the tensor memory.
+#include "kv8.h"
+#include "tcgen05.cuh"
+
+namespace n730 {
+
+constexpr int KP_ROWS = 256;      // query rows of a CTA
+constexpr int KP_KEYS = 128;      // positions of a tile
+constexpr int KP_THREADS = 13 * 32;
+constexpr int KP_RING = 4;        // tiles whose scales are kept: two more than tiles of codes
+constexpr float KP_SLACK = 8.f;   // log2 of how far a weight may exceed its reference
+
+template <int HD>
+struct KPCfg {
+  static constexpr int NB = HD / 64;                           // 64-channel blocks
+  static constexpr int QB = KP_ROWS * 128, KB = KP_KEYS * 128;  // bytes of a block of Q, of K or V
+  static constexpr int KV = NB * KB;                           // bytes of a tile of K or V
+  static constexpr uint32_t TMEM = 512;
+  static constexpr uint32_t S0 = 0, O0 = 2 * KP_KEYS;           // columns: scores of A, B; outputs of A, B
+  // kind::f16: D fp32, A = B = fp16, M = 128
+  static constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(KP_KEYS >> 3) << 17) | (8u << 24);
+  static constexpr uint32_t IDESC_O = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);  // B is MN-major
+};
+
+template <int HD>
+struct KPSmem {
+  uint8_t q[KPCfg<HD>::NB * KPCfg<HD>::QB];
+  uint8_t k[2][KPCfg<HD>::KV];
+  uint8_t v[2][KPCfg<HD>::KV];
+  float sc[KP_RING][2][8];   // scales of K and of V by block of 16 positions; K's -infinity: no page
+  float rowmul[KP_ROWS];
+  uint64_t kfull[2], vfull[2], kfree[2], vfree[2], sfull[2], pready[2], odone[2], drain;
+  uint32_t tmem;
+  int abort;
+};
+
+// MN-major operand, 128-byte swizzle: atoms of 64 elements x 8 k; the next 64 elements lie `lead` bytes on,
+// the next 8 k 1024 bytes on.
+__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t saddr, uint32_t lead) {
+  uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)(lead >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+// D[tmem_d] (+)= A . B with both operands in shared memory
+template <uint32_t IDESC>
+__device__ __forceinline__ void tc_mma_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t accumulate) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+               :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(IDESC), "r"(accumulate) : "memory");
+}
+
+// HD / 32 consecutive channels of a row as fp32; `vec`: rows lie on whole 16 bytes
+template <int E>
+__device__ __forceinline__ void kp_load(const void* p, int64_t i, int dtype, bool vec, float (&x)[E]) {
+  if (vec && dtype != N730_F32) {
+    uint32_t w[E / 2];
+    if (E == 4) {
+      const uint2 y = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p) + i);
+      w[0] = y.x; w[E / 2 - 1] = y.y;
+    } else {
+      w[0] = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint16_t*>(p) + i);
+    }
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) {
+      if (dtype == N730_F16) {
+        const float2 f = __half22float2(u2h(w[e]));
+        x[2 * e] = f.x; x[2 * e + 1] = f.y;
+      } else {
+        x[2 * e] = __uint_as_float(w[e] << 16);
+        x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = kv8_load1(p, i + e, dtype);
+  }
+}
+// One row of queries (a warp, E channels a lane) scaled by a power of two and written as row r of a K-major,
+// swizzled operand with `block` bytes between 64-channel blocks; returns what scores of it are to be multiplied by.
+template <int E>
+__device__ __forceinline__ float kp_put_row(const float (&x)[E], float sign, float scale, uint8_t* dst, int block, int r) {
+  const int lane = threadIdx.x & 31, d = lane * E;
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) m = fmaxf(m, fabsf(x[e]));
+  m = warp_max(m);
+  // the largest magnitude goes into [2^13, 2^14); rows of zeros or with an infinity stay
+  const int ex = (int)((__float_as_uint(m) >> 23) & 255u);
+  const int sh = ex == 0 || ex == 255 ? 0 : min(max(140 - ex, -126), 126);
+  const float mul = __uint_as_float((uint32_t)(127 + sh) << 23) * sign;
+  uint8_t* at = dst + (d >> 6) * block + r * 128 + ((((d >> 3) & 7) ^ (r & 7)) << 4) + (d & 7) * 2;
+  if (E == 4)
+    *reinterpret_cast<uint2*>(at) = make_uint2(h2u(__floats2half2_rn(x[0] * mul, x[1] * mul)),
+                                               h2u(__floats2half2_rn(x[E - 2] * mul, x[E - 1] * mul)));
+  else
+    *reinterpret_cast<uint32_t*>(at) = h2u(__floats2half2_rn(x[0] * mul, x[1] * mul));
+  return scale * __uint_as_float((uint32_t)(127 - sh) << 23);
+}
+// 16 codes (chunk of a row) as fp16 into row r of a swizzled operand
+template <int CODE>
+__device__ __forceinline__ void kp_put_codes(const uint4& x, uint8_t* dst, int block, int r, int chunk) {
+  const uint32_t wd[4] = {x.x, x.y, x.z, x.w};
+  uint32_t y[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t z = code_word<CODE>(wd[e]);
+    y[2 * e] = codes2<CODE, 0>(z);
+    y[2 * e + 1] = codes2<CODE, 1>(z);
+  }
+  uint8_t* rowp = dst + (chunk >> 2) * block + r * 128;
+  const int c0 = (chunk & 3) * 2, swap = chunk >> 2;  // the second block's lanes store their halves in the other order
+  const uint4 lo = make_uint4(y[0], y[1], y[2], y[3]), hi = make_uint4(y[4], y[5], y[6], y[7]);
+  *reinterpret_cast<uint4*>(rowp + (((c0 + swap) ^ (r & 7)) << 4)) = swap ? hi : lo;
+  *reinterpret_cast<uint4*>(rowp + (((c0 + 1 - swap) ^ (r & 7)) << 4)) = swap ? lo : hi;
+}
+
+struct KPArgs {
+  N730KV8Cache c;
+  const void* q; void* out;
+  int64_t ldq, ldo;
+  int dtype, tokens, group, rows, tiles;  // rows = tokens * group; tiles of KP_ROWS rows
+  int splits;                             // shares of the positions, each a CTA
+  bool vec, qvec;                         // out rows, query rows are 16-byte aligned
+  float scale_log2e;                      // its absolute value; the sign goes with the queries
+  float sign;
+  const int* lens; const int* n_new;
+  int* status;
+  float* part; float* part_ml;            // [item tile][split][KP_ROWS] rows, as the split kernel's (splits > 1)
+  float* lse;                             // [batch][n_kv][rows] (may be null)
+};
+
+template <int HD, int CODE>
+__global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs a) {
+  using Cfg = KPCfg<HD>;
+  extern __shared__ __align__(1024) uint8_t kp_raw[];
+  KPSmem<HD>& sm = *reinterpret_cast<KPSmem<HD>*>((reinterpret_cast<uintptr_t>(kp_raw) + 1023) & ~uintptr_t(1023));
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const N730KV8Cache& c = a.c;
+  const int b = blockIdx.z, h = blockIdx.y;
+  const int tile = a.tiles - 1 - (int)blockIdx.x / a.splits, split = (int)blockIdx.x % a.splits;  // the longest first
+  const int cap = c.max_pages * c.page_size;
+  pdl_wait();
+  pdl_launch_dependents();  // the finishing kernel waits for this grid's end
+  const int L = kv8_len(a.lens, b, cap), n_new = kv8_new(a.n_new, b, a.tokens);
+  const int f0 = tile * KP_ROWS, nrow = min(KP_ROWS, n_new * a.group - f0);
+  if (nrow <= 0) return;
+  // positions [p_lo, p_hi) of this share: what the tile's last row sees, cut into whole tiles
+  const int sees_last = (int)min((int64_t)L + (f0 + nrow - 1) / a.group + 1, (int64_t)cap);
+  const int sees_all = (int)min((int64_t)L + f0 / a.group + 1, (int64_t)cap);
+  const int all_tiles = (sees_last + KP_KEYS - 1) / KP_KEYS;
+  const int j0 = (int)((int64_t)all_tiles * split / a.splits), nt = (int)((int64_t)all_tiles * (split + 1) / a.splits) - j0;
+  const int64_t head = (int64_t)b * c.n_kv + h;
+
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.kfull[i], 4);
+      mbar_init(&sm.vfull[i], 4);
+      mbar_init(&sm.kfree[i], 1);
+      mbar_init(&sm.vfree[i], 1);
+      mbar_init(&sm.sfull[i], 1);
+      mbar_init(&sm.pready[i], 4);
+      mbar_init(&sm.odone[i], 1);
+    }
+    mbar_init(&sm.drain, 1);
+    fence_mbar_init();
+    sm.abort = 0;
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 :: "r"(smem_u32(&sm.tmem)), "r"(Cfg::TMEM) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // ---- Q: a row per warp at a time, scaled by a power of two, K-major and swizzled ----
+#pragma unroll 4
+  for (int r = warp; r < KP_ROWS; r += KP_THREADS / 32) {
+    constexpr int E = HD / 32;  // channels a lane
+    float x[E] = {};
+    const int f = f0 + r;
+    if (r < nrow)
+      kp_load<E>(a.q, ((int64_t)b * a.tokens + f / a.group) * a.ldq + (int64_t)(h * a.group + f % a.group) * HD + lane * E,
+                 a.dtype, a.qvec, x);
+    const float rm = kp_put_row<E>(x, a.sign, a.scale_log2e, sm.q, Cfg::QB, r);
+    if (lane == 0) sm.rowmul[r] = rm;
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem;
+  volatile int* abortf = &sm.abort;
+
+  if (warp >= 8 && warp < 12) {
+    // ---------------- codes to fp16 ----------------
+    constexpr int LPR = HD / 16, RPI = 32 / LPR, NI = 32 / RPI;  // lanes a row, rows an instruction, instructions
+    const int w = warp - 8, row0 = w * 32 + lane / LPR, chunk = lane % LPR;
+    const int* bt = c.block_table + (int64_t)b * c.max_pages;
+    // pool rows of the warp's two blocks of 16 positions of tile j (-1: no page)
+    auto lookup = [&](int j, int i) {
+      const int p = (j0 + j) * KP_KEYS + w * 32 + i * 16;
+      if (j >= nt || p >= sees_last) return -1;
+      const int page = bt[p / c.page_size];
+      return (unsigned)page < (unsigned)c.n_pages ? (page * c.n_kv + h) * c.page_size + p % c.page_size : -1;
+    };
+    uint4 kx[NI], vx[NI];  // asked for a tile ahead
+    auto load = [&](uint4 (&x)[NI], const void* pool, int j, int r_lo, int r_hi) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int r = row0 + i * RPI - w * 32;  // within the warp's 32
+        const int base = r < 16 ? r_lo : r_hi;
+        const bool in = base >= 0 && (j0 + j) * KP_KEYS + w * 32 + r < sees_last;  // rows never written may hold anything
+        x[i] = in ? *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(pool) + ((int64_t)base + (r & 15)) * HD + chunk * 16)
+                  : make_uint4(0, 0, 0, 0);
+      }
+    };
+    // K's and V's scale of the two blocks, lanes 0 - 3
+    auto load_scale = [&](int r_lo, int r_hi) {
+      const int row = lane < 2 ? r_lo : r_hi;
+      if (lane >= 4 || row < 0) return lane & 1 ? 0.f : -INFINITY;
+      return ((lane & 1) ? c.v_scales : c.k_scales)[row / c.block];
+    };
+    auto store = [&](const uint4 (&x)[NI], uint8_t* dst) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) kp_put_codes<CODE>(x[i], dst, Cfg::KB, row0 + i * RPI, chunk);
+    };
+    auto ready = [&](uint64_t* bar) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive1(bar);
+    };
+    int lo = lookup(0, 0), hi = lookup(0, 1), lo1 = lookup(1, 0), hi1 = lookup(1, 1);
+    load(kx, c.k_codes, 0, lo, hi);
+    load(vx, c.v_codes, 0, lo, hi);
+    float scale = load_scale(lo, hi);
+    for (int j = 0; j < nt; ++j) {
+      const int s = j & 1;
+      const int lo2 = lookup(j + 2, 0), hi2 = lookup(j + 2, 1);
+      int go = 1;
+      if (lane == 0 && j >= 2) go = tc_wait(&sm.kfree[s], (uint32_t)((j / 2 - 1) & 1), abortf);
+      if (!__shfl_sync(0xffffffffu, go, 0)) break;
+      store(kx, sm.k[s]);
+      if (lane < 4) sm.sc[j % KP_RING][lane & 1][w * 2 + (lane >> 1)] = scale;
+      ready(&sm.kfull[s]);
+      load(kx, c.k_codes, j + 1, lo1, hi1);
+      scale = load_scale(lo1, hi1);
+      if (lane == 0 && j >= 2) go = tc_wait(&sm.vfree[s], (uint32_t)((j / 2 - 1) & 1), abortf);
+      if (!__shfl_sync(0xffffffffu, go, 0)) break;
+      store(vx, sm.v[s]);
+      ready(&sm.vfull[s]);
+      load(vx, c.v_codes, j + 1, lo1, hi1);
+      lo1 = lo2;
+      hi1 = hi2;
+    }
+  } else if (warp == 12) {
+    // ---------------- products ----------------
+    if (lane == 0) {
+      const uint32_t qs = smem_u32(sm.q);
+      auto scores = [&](int x, int s) {
+        const uint32_t ks = smem_u32(sm.k[s]);
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+          tc_mma_ss<Cfg::IDESC_S>(tmem + Cfg::S0 + x * KP_KEYS,
+                                  umma_desc_sw128(qs + (k >> 2) * Cfg::QB + x * (KP_ROWS / 2) * 128 + (k & 3) * 32),
+                                  umma_desc_sw128(ks + (k >> 2) * Cfg::KB + (k & 3) * 32), k > 0);
+        tc_commit(&sm.sfull[x]);
+      };
+      auto outputs = [&](int x, int s, bool first) {
+        const uint32_t vs = smem_u32(sm.v[s]);
+#pragma unroll
+        for (int k = 0; k < KP_KEYS / 16; ++k)
+          tc_mma_ts<Cfg::IDESC_O>(tmem + Cfg::O0 + x * HD, tmem + Cfg::S0 + x * KP_KEYS + k * 8,
+                                  umma_desc_mn_sw128(vs + k * 2048, Cfg::KB), !(first && k == 0));
+      };
+      bool go = nt > 0 && tc_wait(&sm.kfull[0], 0, abortf);
+      if (go) {
+        tc_fence_after();
+        scores(0, 0);
+        scores(1, 0);
+        tc_commit(&sm.kfree[0]);
+      }
+      for (int j = 0; go && j < nt; ++j) {
+        const int s = j & 1, s1 = s ^ 1;
+        const uint32_t ph = (uint32_t)((j / 2) & 1), ph1 = (uint32_t)(((j + 1) / 2) & 1);
+        go = tc_wait(&sm.vfull[s], ph, abortf);
+        for (int x = 0; go && x < 2; ++x) {
+          go = tc_wait(&sm.pready[x], (uint32_t)(j & 1), abortf);
+          if (!go) break;
+          tc_fence_after();
+          outputs(x, s, j == 0);
+          if (x == 1) tc_commit(&sm.vfree[s]);
+          if (j + 1 < nt) {
+            if (x == 0) go = tc_wait(&sm.kfull[s1], ph1, abortf);
+            if (!go) break;
+            tc_fence_after();
+            scores(x, s1);
+            if (x == 1) tc_commit(&sm.kfree[s1]);
+          } else {
+            tc_commit(&sm.odone[x]);
+          }
+        }
+      }
+      if (!go && nt > 0) {  // what is in flight ends before the tensor memory is freed
+        *abortf = 1;
+        tc_commit(&sm.drain);
+        wait_bar(&sm.drain, 0);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------- softmax: warps 0-3 of A, 4-7 of B, a thread a row ----------------
+    const int x = warp >> 2, q = warp & 3, r = x * (KP_ROWS / 2) + q * 32 + lane, f = f0 + r;
+    const bool live = r < nrow;
+    const int vis = live ? (int)min((int64_t)L + f / a.group + 1, (int64_t)cap) : 0;
+    const float rm = sm.rowmul[r];
+    const uint32_t ts = tmem + ((uint32_t)(q * 32) << 16) + Cfg::S0 + x * KP_KEYS;
+    const uint32_t to = tmem + ((uint32_t)(q * 32) << 16) + Cfg::O0 + x * HD;
+    float m_ref = -INFINITY, mo_ref = -INFINITY, l = 0.f;
+    bool go = true;
+    for (int j = 0; j < nt; ++j) {
+      int ok1 = 1;
+      if (lane == 0) ok1 = tc_wait(&sm.sfull[x], (uint32_t)(j & 1), abortf);
+      if (!__shfl_sync(0xffffffffu, ok1, 0)) { go = false; break; }
+      tc_fence_after();
+      const float* ksc = sm.sc[j % KP_RING][0];
+      const float* vsc = sm.sc[j % KP_RING][1];
+      const int p0 = (j0 + j) * KP_KEYS;
+      const bool masked = p0 + KP_KEYS > sees_all;  // some row of the CTA does not see all of the tile
+      // largest score, and largest score + log2(V scale)
+      float mx = -INFINITY, mv = -INFINITY;
+#pragma unroll 1
+      for (int cc = 0; cc < 4; ++cc) {
+        float v[32];
+        tc_ld32(ts + cc * 32, v);
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (p0 + cc * 32 + i >= vis) v[i] = -INFINITY;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float m = v[16 * e];
+#pragma unroll
+          for (int i = 1; i < 16; ++i) m = fmaxf(m, v[16 * e + i]);
+          const float ks = ksc[2 * cc + e], vs = vsc[2 * cc + e];
+          const bool none = ks == -INFINITY;  // no page: not seen
+          const float y = m == -INFINITY || none ? -INFINITY : m * (rm * ks);
+          mx = fmaxf(mx, y);
+          mv = fmaxf(mv, y + lg2(vs));
+        }
+      }
+      const bool move = mx > m_ref + KP_SLACK || mv > mo_ref + KP_SLACK;
+      if (__any_sync(0xffffffffu, move)) {
+        const float mn = fmaxf(m_ref, mx), mon = fmaxf(mo_ref, mv);
+        if (mn != m_ref) l *= ex2(m_ref - mn);
+        const float fo = mon != mo_ref ? ex2(mo_ref - mon) : 1.f;
+        m_ref = mn;
+        mo_ref = mon;
+        if (j > 0) {
+#pragma unroll 1
+          for (int cc = 0; cc < HD / 32; ++cc) {
+            float v[32];
+            uint32_t w[32];
+            tc_ld32(to + cc * 32, v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i] * fo);
+            tc_st32(to + cc * 32, w);
+          }
+        }
+      }
+      const float mos = mo_ref == -INFINITY ? 0.f : mo_ref, ms = m_ref == -INFINITY ? 0.f : m_ref;
+#pragma unroll 1
+      for (int c2 = 0; c2 < 2; ++c2) {  // 64 positions: 32 columns of P over the scores read
+        uint32_t w[32];
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          float v[32];
+          tc_ld32(ts + c2 * 64 + hh * 32, v);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int blk = c2 * 4 + hh * 2 + e;
+            const float ks = ksc[blk], vs = vsc[blk], lv = lg2(vs);
+            const bool none = ks == -INFINITY, zero = vs == 0.f;
+            // zero V: the weights count in the sum, their product with V is zero
+            const float fk = rm * ks, off = zero ? -ms : lv - mos, back = zero ? 1.f : ex2(mos - ms - lv);
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              float p = ex2(fmaf(v[16 * e + i], fk, off)), p1 = ex2(fmaf(v[16 * e + i + 1], fk, off));
+              if (masked || none) {
+                const int pos = p0 + blk * 16 + i;
+                if (pos >= vis || none) p = 0.f;
+                if (pos + 1 >= vis || none) p1 = 0.f;
+              }
+              sum += p + p1;
+              w[hh * 16 + e * 8 + i / 2] = zero ? 0u : h2u(__floats2half2_rn(p, p1));
+            }
+            l = fmaf(sum, back, l);
+          }
+        }
+        tc_st32(ts + c2 * 32, w);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive1(&sm.pready[x]);
+    }
+    if (go && nt > 0) {
+      int ok1 = 1;
+      if (lane == 0) ok1 = tc_wait(&sm.odone[x], 0, abortf);
+      go = __shfl_sync(0xffffffffu, ok1, 0);
+      tc_fence_after();
+    }
+    if (go) {
+      const float s = l == 0.f ? 0.f : (mo_ref == -INFINITY ? 0.f : ex2(mo_ref - m_ref)) / l;  // a NaN query: NaN
+      const int64_t at = ((int64_t)b * a.tokens + f / a.group) * a.ldo + (int64_t)(h * a.group + f % a.group) * HD;
+      const int64_t slot = ((head * a.tiles + tile) * a.splits + split) * KP_ROWS + r;
+#pragma unroll 1
+      for (int cc = 0; cc < HD / 32; ++cc) {
+        float v[32];
+        if (nt > 0) {
+          tc_ld32(to + cc * 32, v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0.f;
+        }
+        if (!live) continue;
+        if (a.splits > 1) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(a.part + slot * HD + cc * 32 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        } else if (a.vec && a.dtype != N730_F32) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float y0 = v[i + 2 * e] * s, y1 = v[i + 2 * e + 1] * s;
+              if (a.dtype == N730_F16) {
+                w[e] = h2u(__floats2half2_rn(y0, y1));
+              } else {
+                const __nv_bfloat162 y = __floats2bfloat162_rn(y0, y1);
+                w[e] = *reinterpret_cast<const uint32_t*>(&y);
+              }
+            }
+            *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + at + cc * 32 + i) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) kv8_store1(a.out, at + cc * 32 + i, a.dtype, v[i] * s);
+        }
+      }
+      if (live && a.splits > 1) reinterpret_cast<float4*>(a.part_ml)[slot] = make_float4(mo_ref, m_ref, l, 0.f);
+      if (live && a.lse && a.splits == 1) a.lse[head * a.rows + f] = l == 0.f ? INFINITY : m_ref + lg2(l);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (*abortf && tid == 0) *a.status = 1;
+  if (warp == 12)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(Cfg::TMEM) : "memory");
+}
+
+// ---------------------------------------------------------------------------
+// accumulated weights of a prompt: w[b, h, p] += sum over the KV head's rows of exp2(score - lse)
+// ---------------------------------------------------------------------------
+// One CTA per 128 positions of a KV head walks over the rows that see them, 128 at a time, and forms
+// S^T = K Q^T, so that a position is a TMEM lane and its sum over the rows stays in one thread: warps 8-11
+// bring the rows' queries into shared memory, warp 12 issues the products, warps 0-3 sum the even row
+// tiles, 4-7 the odd ones; the two sums are added at the end (always in the same order).
+template <int HD>
+struct KWSmem {
+  uint8_t k[KPCfg<HD>::KV];
+  uint8_t q[2][KPCfg<HD>::KV];
+  float2 row[2][KP_KEYS];    // multiplier, lse
+  float sum[KP_KEYS];
+  uint64_t qfull[2], qfree[2], sfull[2], sread[2], drain;
+  uint32_t tmem;
+  int abort;
+};
+
+template <int HD, int CODE>
+__global__ void __launch_bounds__(KP_THREADS, 1)
+kv8_prompt_weights_kernel(const KPArgs a, const float* w_in, float* w_out, int64_t ldw) {
+  using Cfg = KPCfg<HD>;
+  constexpr int E = HD / 32, RT = KP_KEYS;  // rows of a tile
+  constexpr uint32_t COLS = 2 * RT;         // tensor memory: two score tiles
+  extern __shared__ __align__(1024) uint8_t kp_raw[];
+  KWSmem<HD>& sm = *reinterpret_cast<KWSmem<HD>*>((reinterpret_cast<uintptr_t>(kp_raw) + 1023) & ~uintptr_t(1023));
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const N730KV8Cache& c = a.c;
+  const int b = blockIdx.z, h = blockIdx.y, p0 = blockIdx.x * KP_KEYS;
+  const int cap = c.max_pages * c.page_size;
+  pdl_wait();
+  const int L = kv8_len(a.lens, b, cap), n_new = kv8_new(a.n_new, b, a.tokens), rows = n_new * a.group;
+  const int total = (int)min((int64_t)L + n_new, (int64_t)cap);
+  if (p0 >= total) return;
+  const int64_t head = (int64_t)b * c.n_kv + h;
+  // row tiles [i0, i0 + n): the first whose last row sees position p0
+  const int i0 = max(0, p0 - L) * a.group / RT, n = (rows + RT - 1) / RT - i0;
+  const int* bt = c.block_table + (int64_t)b * c.max_pages;
+  auto row_of = [&](int p) -> int64_t {
+    if (p >= total) return -1;
+    const int page = bt[p / c.page_size];
+    return (unsigned)page < (unsigned)c.n_pages ? ((int64_t)page * c.n_kv + h) * c.page_size + p % c.page_size : -1;
+  };
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.qfull[i], 4);
+      mbar_init(&sm.qfree[i], 1);
+      mbar_init(&sm.sfull[i], 1);
+      mbar_init(&sm.sread[i], 4);
+    }
+    mbar_init(&sm.drain, 1);
+    fence_mbar_init();
+    sm.abort = 0;
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 :: "r"(smem_u32(&sm.tmem)), "r"(COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  for (int i = tid; i < KP_KEYS * (HD / 16); i += KP_THREADS) {
+    const int r = i / (HD / 16), chunk = i % (HD / 16);
+    const int64_t row = row_of(p0 + r);
+    kp_put_codes<CODE>(row >= 0 ? *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(c.k_codes) + row * HD + chunk * 16)
+                                : make_uint4(0, 0, 0, 0), sm.k, Cfg::KB, r, chunk);
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem;
+  volatile int* abortf = &sm.abort;
+  float sum = 0.f;
+
+  if (warp >= 8 && warp < 12) {
+    const int w = warp - 8;
+    for (int i = 0; i < n; ++i) {
+      const int s = i & 1;
+      int go = 1;
+      if (lane == 0 && i >= 2) {  // the products of the tile before are done, and its factors read
+        go = tc_wait(&sm.qfree[s], (uint32_t)((i / 2 - 1) & 1), abortf);
+        if (go) go = tc_wait(&sm.sread[s], (uint32_t)((i / 2 - 1) & 1), abortf);
+      }
+      if (!__shfl_sync(0xffffffffu, go, 0)) break;
+#pragma unroll 4
+      for (int r = w; r < RT; r += 4) {
+        const int f = (i0 + i) * RT + r;
+        float x[E] = {};
+        if (f < rows)
+          kp_load<E>(a.q, ((int64_t)b * a.tokens + f / a.group) * a.ldq + (int64_t)(h * a.group + f % a.group) * HD + lane * E,
+                     a.dtype, a.qvec, x);
+        const float rm = kp_put_row<E>(x, a.sign, a.scale_log2e, sm.q[s], Cfg::KB, r);
+        if (lane == 0) sm.row[s][r] = make_float2(rm, f < rows ? a.lse[head * a.rows + f] : INFINITY);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive1(&sm.qfull[s]);
+    }
+  } else if (warp == 12) {
+    if (lane == 0) {
+      bool go = true;
+      for (int i = 0; go && i < n; ++i) {
+        const int s = i & 1;
+        go = tc_wait(&sm.qfull[s], (uint32_t)((i / 2) & 1), abortf);  // implies that the scores before in this buffer are read
+        if (!go) break;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+          tc_mma_ss<Cfg::IDESC_S>(tmem + s * RT, umma_desc_sw128(smem_u32(sm.k) + (k >> 2) * Cfg::KB + (k & 3) * 32),
+                                  umma_desc_sw128(smem_u32(sm.q[s]) + (k >> 2) * Cfg::KB + (k & 3) * 32), k > 0);
+        tc_commit(&sm.qfree[s]);
+        tc_commit(&sm.sfull[s]);
+      }
+      if (!go) {
+        *abortf = 1;
+        tc_commit(&sm.drain);
+        wait_bar(&sm.drain, 0);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int x = warp >> 2, q = warp & 3, p = p0 + q * 32 + lane;
+    const int64_t row = row_of(p);
+    const float ks = row >= 0 ? c.k_scales[row / c.block] : 0.f;
+    const uint32_t ts = tmem + ((uint32_t)(q * 32) << 16) + x * RT;
+    for (int i = x; i < n; i += 2) {
+      int ok1 = 1;
+      if (lane == 0) ok1 = tc_wait(&sm.sfull[x], (uint32_t)((i / 2) & 1), abortf);
+      if (!__shfl_sync(0xffffffffu, ok1, 0)) break;
+      tc_fence_after();
+      const int f0 = (i0 + i) * RT;
+      const int first_seen = p0 + KP_KEYS - 1 <= L + f0 / a.group ? 0 : max(0, p - L) * a.group - f0;  // rows before it do not see p
+#pragma unroll 1
+      for (int cc = 0; cc < RT / 32; ++cc) {
+        float v[32];
+        tc_ld32(ts + cc * 32, v);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float2 m = sm.row[x][cc * 32 + e];
+          const float y = ex2(fmaf(v[e] * ks, m.x, -m.y));
+          sum += cc * 32 + e < first_seen ? 0.f : y;
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive1(&sm.sread[x]);
+    }
+    if (row < 0) sum = 0.f;
+    if (x == 1) sm.sum[q * 32 + lane] = sum;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (*abortf && tid == 0) *a.status = 1;
+  if (warp < 4 && p0 + tid < total) {
+    const int p = p0 + tid;
+    w_out[head * ldw + p] = (w_in && p < L ? w_in[head * ldw + p] : 0.f) + (sum + sm.sum[tid]);
+  }
+  if (warp == 12)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(COLS) : "memory");
+}
+
+KV8PromptPlan kv8_prompt_plan(const N730KV8Cache& c, int batch, int tokens, int heads) {
+  KV8PromptPlan p{};
+  p.rows = tokens * (heads / c.n_kv);
+  p.tiles = (p.rows + KP_ROWS - 1) / KP_ROWS;
+  p.rg = KP_ROWS;
+  const int64_t ctas = (int64_t)batch * c.n_kv * p.tiles;
+  const int64_t key_tiles = ((int64_t)c.max_pages * c.page_size + KP_KEYS - 1) / KP_KEYS;
+  // shares of the positions while the SMs would stand idle, of four tiles at least
+  p.splits = 1;
+  while (ctas * (p.splits + 1) <= num_sms() && key_tiles / (p.splits + 1) >= 4) ++p.splits;
+  return p;
+}
+
+static KPArgs kp_args(const KV8AttnCall& k, const KV8PromptPlan& p, int* status, float* part, float* part_ml, float* lse) {
+  KPArgs a{};
+  a.c = k.c;
+  a.q = k.q; a.out = k.out; a.ldq = k.ldq; a.ldo = k.ldo; a.dtype = k.dtype;
+  a.tokens = k.tokens; a.group = k.heads / k.c.n_kv; a.rows = p.rows; a.tiles = p.tiles; a.splits = p.splits;
+  a.vec = ((uintptr_t)k.out & 15) == 0 && k.ldo * kv8_esize(k.dtype) % 16 == 0;
+  a.qvec = ((uintptr_t)k.q & 15) == 0 && k.ldq * kv8_esize(k.dtype) % 16 == 0;
+  a.scale_log2e = fabsf(k.scale) * 1.4426950408889634f;
+  a.sign = k.scale < 0.f ? -1.f : 1.f;
+  a.lens = k.lens; a.n_new = k.n_new;
+  a.status = status; a.part = part; a.part_ml = part_ml; a.lse = lse;
+  return a;
+}
+
+template <int HD, int CODE>
+static int prompt_launch(const KPArgs& a, int batch, bool pdl, cudaStream_t st) {
+  const size_t smem = sizeof(KPSmem<HD>) + 1024;
+  if (int rc = smem_attr_once<kv8_prompt_kernel<HD, CODE>>((int)smem)) return rc;
+  return kv8_launch(kv8_prompt_kernel<HD, CODE>, dim3(a.tiles * a.splits, a.c.n_kv, batch), dim3(KP_THREADS), smem, st, pdl, a);
+}
+template <int HD, int CODE>
+static int prompt_weights_launch(const KPArgs& a, const KV8AttnCall& k, cudaStream_t st) {
+  const size_t smem = sizeof(KWSmem<HD>) + 1024;
+  if (int rc = smem_attr_once<kv8_prompt_weights_kernel<HD, CODE>>((int)smem)) return rc;
+  const int cap = a.c.max_pages * a.c.page_size;
+  return kv8_launch(kv8_prompt_weights_kernel<HD, CODE>, dim3((cap + KP_KEYS - 1) / KP_KEYS, a.c.n_kv, k.batch),
+                    dim3(KP_THREADS), smem, st, false, a, k.w_in, k.w_out, k.ldw);
+}
+
+int kv8_prompt_launch(const KV8AttnCall& k, const KV8PromptPlan& p, int* status, float* part, float* part_ml, float* lse,
+                      cudaStream_t st) {
+  const KPArgs a = kp_args(k, p, status, part, part_ml, lse);
+  const bool i8 = k.c.code == N730_KV8_INT8;
+  if (k.c.head_dim == 128)
+    return i8 ? prompt_launch<128, N730_KV8_INT8>(a, k.batch, k.pdl, st) : prompt_launch<128, N730_KV8_E4M3>(a, k.batch, k.pdl, st);
+  return i8 ? prompt_launch<64, N730_KV8_INT8>(a, k.batch, k.pdl, st) : prompt_launch<64, N730_KV8_E4M3>(a, k.batch, k.pdl, st);
+}
+
+int kv8_prompt_weights_launch(const KV8AttnCall& k, const KV8PromptPlan& p, int* status, float* lse, cudaStream_t st) {
+  const KPArgs a = kp_args(k, p, status, nullptr, nullptr, lse);
+  const bool i8 = k.c.code == N730_KV8_INT8;
+  if (k.c.head_dim == 128)
+    return i8 ? prompt_weights_launch<128, N730_KV8_INT8>(a, k, st) : prompt_weights_launch<128, N730_KV8_E4M3>(a, k, st);
+  return i8 ? prompt_weights_launch<64, N730_KV8_INT8>(a, k, st) : prompt_weights_launch<64, N730_KV8_E4M3>(a, k, st);
+}
+
+}  // namespace n730
