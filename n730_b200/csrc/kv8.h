@@ -41,6 +41,10 @@ int kv8_prompt_launch(const KV8AttnCall& k, const KV8PromptPlan& p, int* status,
                       cudaStream_t st);
 int kv8_prompt_weights_launch(const KV8AttnCall& k, const KV8PromptPlan& p, int* status, float* lse, cudaStream_t st);
 
+// The first 1024-byte boundary of dynamic shared memory.  Formed by an offset, not by rounding the pointer: the
+// compiler would lose sight of the address space and fall back to generic loads and stores.
+__device__ __forceinline__ uint8_t* aligned_smem(uint8_t* raw) { return raw + ((0u - smem_u32(raw)) & 1023u); }
+
 // one element of a row in the caller's type, widened to fp32
 __device__ __forceinline__ float kv8_load1(const void* p, int64_t i, int dtype) {
   if (dtype == N730_F32) return reinterpret_cast<const float*>(p)[i];

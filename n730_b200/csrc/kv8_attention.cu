@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
   constexpr int RG = 8 * NB, KS = HD / 16, MT = HD / 16, ST = KD_STAGES;
   constexpr int TT = NB == 1 ? 2 : 1;  // halves of a tile worked on together: independent chains for the tensor cores
   extern __shared__ __align__(1024) uint8_t kd_raw[];
-  KDSmem<HD>& sm = *reinterpret_cast<KDSmem<HD>*>((reinterpret_cast<uintptr_t>(kd_raw) + 1023) & ~uintptr_t(1023));
+  KDSmem<HD>& sm = *reinterpret_cast<KDSmem<HD>*>(aligned_smem(kd_raw));
   static_assert(ST == 2 && sizeof(float) * RG * HD <= G::TILE_BYTES, "a warp's outputs fit the buffer that is not being filled");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   const N730KV8Cache& c = a.c;

@@ -5,11 +5,11 @@
 // The rows of an item (sequence, KV head) are its tokens x G query heads, row = token * G + head, so
 // every row of a tile reads the same K and V.  One CTA takes 256 rows (two 128-row tiles, A and B) and
 // walks over the positions in tiles of 128:
-//   warps 8-11  load the tile's codes (16 bytes a lane, whole 128-byte rows), turn them into fp16
+//   warps 8-10  load the tile's codes (16 bytes a lane, whole 128-byte rows), turn them into fp16
 //               exactly and store them swizzled: K as [64-channel block][position][128 B], the K-major
 //               operand of S = Q K^T; V in the same layout, which is the MN-major operand of O += P V.
 //               Each conversion serves 256 rows;
-//   warp 12     issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory) of
+//   warp 11     issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory) of
 //               A and B in turn, so that one's products run while the other's softmax does;
 //   warps 0-3   softmax of A, warps 4-7 of B: a thread owns a row (TMEM lane).  P, fp16, overwrites the
 //               tile's scores in place.
@@ -35,9 +35,14 @@ namespace n730 {
 
 constexpr int KP_ROWS = 256;      // query rows of a CTA
 constexpr int KP_KEYS = 128;      // positions of a tile
-constexpr int KP_THREADS = 13 * 32;
+// Twelve warps leave 168 registers a thread: the softmax holds a row's 128 scores (reading tensor memory twice
+// cost as much as the arithmetic).
+constexpr int KP_THREADS = 12 * 32;
+constexpr int KP_CODE_WARPS = 3, KP_MMA_WARP = 11;
+constexpr int KW_THREADS = 13 * 32;
 constexpr int KP_RING = 4;        // tiles whose scales are kept: two more than tiles of codes
-constexpr float KP_SLACK = 8.f;   // log2 of how far a weight may exceed its reference
+constexpr float KP_SLACK = 8.f;   // log2 of how far a weight x V scale may exceed its reference (fp16: 2^16)
+constexpr float KP_SUM_SLACK = 64.f;  // and of how far a weight in the sum (fp32)
 
 template <int HD>
 struct KPCfg {
@@ -56,13 +61,34 @@ struct KPSmem {
   uint8_t q[KPCfg<HD>::NB * KPCfg<HD>::QB];
   uint8_t k[2][KPCfg<HD>::KV];
   uint8_t v[2][KPCfg<HD>::KV];
-  float sc[KP_RING][2][8];   // scales of K and of V by block of 16 positions; K's -infinity: no page
+  float sc[KP_RING][3][8];   // by block of 16 positions: K's scale (-infinity: no page), log2 of V's scale, 1 / V's scale
+  int odd[KP_RING][4];       // by warp of the codes: some block has no page, or a V scale of 0
   float rowmul[KP_ROWS];
   uint64_t kfull[2], vfull[2], kfree[2], vfree[2], sfull[2], pready[2], odone[2], drain;
   uint32_t tmem;
   int abort;
 };
 
+// Bounded wait of one lane that also gives up when another role raised the CTA's abort flag, and raises it
+// itself after 2 s.  The clock is read once in 64 polls: reading it takes longer than most of these waits.
+__device__ __forceinline__ bool kp_wait(uint64_t* bar, uint32_t parity, volatile int* abortf) {
+  uint64_t t0 = 0;
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*abortf) return false;
+    if (!t0) t0 = gtimer();
+    else if (gtimer() - t0 > 2000000000ull) { *abortf = 1; return false; }
+  }
+}
+// The same by a whole warp, which goes on together: with one lane waiting for the others the compiler kept that lane
+// apart, and what followed ran twice.
+__device__ __forceinline__ bool kp_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abortf) {
+  const bool ok = __all_sync(0xffffffffu, kp_wait(bar, parity, abortf));
+  __syncwarp();
+  return ok;
+}
 // MN-major operand, 128-byte swizzle: atoms of 64 elements x 8 k; the next 64 elements lie `lead` bytes on,
 // the next 8 k 1024 bytes on.
 __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t saddr, uint32_t lead) {
@@ -72,6 +98,14 @@ __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t saddr, uint32_t 
   d |= (uint64_t)1 << 46;
   d |= (uint64_t)2 << 61;
   return d;
+}
+// One lane of a warp that runs together.  Products are issued under this, with descriptors that are the same in
+// every lane: from code that one lane runs by itself an instruction took 180 cycles to issue instead of the 64 that a
+// 128x128x16 product lasts.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
 }
 // D[tmem_d] (+)= A . B with both operands in shared memory
 template <uint32_t IDESC>
@@ -128,9 +162,10 @@ __device__ __forceinline__ float kp_put_row(const float (&x)[E], float sign, flo
     *reinterpret_cast<uint32_t*>(at) = h2u(__floats2half2_rn(x[0] * mul, x[1] * mul));
   return scale * __uint_as_float((uint32_t)(127 - sh) << 23);
 }
-// 16 codes (chunk of a row) as fp16 into row r of a swizzled operand
+// 16 codes as fp16 into a row of a swizzled operand, at the row's 128 bytes in the 64-channel block of `chunk`;
+// r7: the row's number mod 8.
 template <int CODE>
-__device__ __forceinline__ void kp_put_codes(const uint4& x, uint8_t* dst, int block, int r, int chunk) {
+__device__ __forceinline__ void kp_put_codes(const uint4& x, uint8_t* rowp, int r7, int chunk) {
   const uint32_t wd[4] = {x.x, x.y, x.z, x.w};
   uint32_t y[8];
 #pragma unroll
@@ -139,11 +174,170 @@ __device__ __forceinline__ void kp_put_codes(const uint4& x, uint8_t* dst, int b
     y[2 * e] = codes2<CODE, 0>(z);
     y[2 * e + 1] = codes2<CODE, 1>(z);
   }
-  uint8_t* rowp = dst + (chunk >> 2) * block + r * 128;
-  const int c0 = (chunk & 3) * 2, swap = chunk >> 2;  // the second block's lanes store their halves in the other order
-  const uint4 lo = make_uint4(y[0], y[1], y[2], y[3]), hi = make_uint4(y[4], y[5], y[6], y[7]);
-  *reinterpret_cast<uint4*>(rowp + (((c0 + swap) ^ (r & 7)) << 4)) = swap ? hi : lo;
-  *reinterpret_cast<uint4*>(rowp + (((c0 + 1 - swap) ^ (r & 7)) << 4)) = swap ? lo : hi;
+  // the two halves lie in neighbouring 16 bytes; lanes of the second 64-channel block store them in the other
+  // order, or they would meet the banks of the first block's
+  const bool swap = chunk >= 4;
+  const int at = (((chunk & 3) * 2 + swap) ^ r7) << 4;
+  *reinterpret_cast<uint4*>(rowp + at) = swap ? make_uint4(y[4], y[5], y[6], y[7]) : make_uint4(y[0], y[1], y[2], y[3]);
+  *reinterpret_cast<uint4*>(rowp + (at ^ 16)) = swap ? make_uint4(y[0], y[1], y[2], y[3]) : make_uint4(y[4], y[5], y[6], y[7]);
+}
+
+// a * b + c and a + b of two fp32 pairs
+__device__ __forceinline__ float2 fma2(const float2& a, const float2& b, const float2& c) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(const float2& a, const float2& b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 w, x, y;\n"
+      " mov.b64 {%0, %1}, w;\n}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// 8 consecutive columns of this thread's TMEM lane multiplied by f
+__device__ __forceinline__ void tc_scale8(uint32_t taddr, float f) {
+  float v[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n tcgen05.wait::ld.sync.aligned;"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "r"(taddr) : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] *= f;
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n tcgen05.wait::st.sync.aligned;"
+               :: "r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+// 64 consecutive columns of this thread's TMEM lane
+__device__ __forceinline__ void tc_ld64(uint32_t taddr, float* v) {
+  uint32_t r[64];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+               "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
+               "%24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, "
+               "%46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63"
+               "}, [%64];\n tcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), 
+                 "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), 
+                 "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), 
+                 "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), 
+                 "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), 
+                 "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), 
+                 "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), 
+                 "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+               : "r"(taddr) : "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Moves a row's references to the largest score mx and the largest score + log2(V scale) mv of a tile where those
+// are larger; sums and, when there are any, outputs (at to) are rescaled.  A warp at a time.
+template <int HD>
+__device__ __forceinline__ void kp_move(uint32_t to, bool outputs, float mx, float mv, float& m_ref, float& mo_ref, float& l) {
+  const float mn = fmaxf(m_ref, mx), mon = fmaxf(mo_ref, mv);
+  if (mn != m_ref) l *= ex2(m_ref - mn);
+  const float f = mon != mo_ref ? ex2(mo_ref - mon) : 1.f;
+  m_ref = mn;
+  mo_ref = mon;
+  if (!outputs) return;
+#pragma unroll 1
+  for (int cc = 0; cc < HD; cc += 8) tc_scale8(to + cc, f);  // few registers: a row's scores are held meanwhile
+}
+
+// One tile of a row: moves the references when a weight would be too large against them, then writes the weights
+// (fp16) over the scores at ts and adds their sum to l.  This is the short way: every row sees all of the tile, every
+// block has a page and a V scale.
+template <int HD>
+__device__ __forceinline__ void kp_softmax(uint32_t ts, uint32_t to, const float* ksc, const float* lvs, float rm,
+                                           bool outputs, float& m_ref, float& mo_ref, float& l) {
+  float v[KP_KEYS];
+  tc_ld64(ts, v);
+  tc_ld64(ts + 64, v + 64);
+  float mx = -INFINITY, mv = -INFINITY;
+#pragma unroll
+  for (int blk = 0; blk < KP_KEYS / 16; ++blk) {
+    float m = v[16 * blk];
+#pragma unroll
+    for (int i = 16 * blk + 1; i < 16 * blk + 16; ++i) m = fmaxf(m, v[i]);
+    const float y = m * (rm * ksc[blk]);
+    mx = fmaxf(mx, y);
+    mv = fmaxf(mv, y + lvs[blk]);
+  }
+  if (__any_sync(0xffffffffu, mx > m_ref + KP_SUM_SLACK || mv > mo_ref + KP_SLACK))
+    kp_move<HD>(to, outputs, mx, mv, m_ref, mo_ref, l);
+  const float mos = mo_ref == -INFINITY ? 0.f : mo_ref, ms = m_ref == -INFINITY ? 0.f : m_ref, back0 = ex2(mos - ms);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {  // 64 positions: 32 columns of P
+    uint32_t w[32];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int blk = half * 4 + k;
+      const float fk = rm * ksc[blk], off = lvs[blk] - mos;
+      float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float2 y = fma2(make_float2(v[16 * blk + i], v[16 * blk + i + 1]), make_float2(fk, fk), make_float2(off, off));
+        const float2 p = make_float2(ex2(y.x), ex2(y.y));
+        sum = add2(sum, p);
+        w[8 * k + i / 2] = h2u(__floats2half2_rn(p.x, p.y));
+      }
+      l = fmaf(sum.x + sum.y, back0 * lvs[8 + blk], l);
+    }
+    tc_st32(ts + half * 32, w);
+  }
+}
+
+// The same for any tile: the first `sees` positions are seen, blocks may have no page or a V scale of 0.
+template <int HD>
+__device__ __forceinline__ void kp_softmax_any(uint32_t ts, uint32_t to, const float* ksc, const float* lvs, float rm, int sees,
+                                               bool outputs, float& m_ref, float& mo_ref, float& l) {
+  float mx = -INFINITY, mv = -INFINITY;
+#pragma unroll 1
+  for (int cc = 0; cc < 4; ++cc) {
+    float v[32];
+    tc_ld32(ts + cc * 32, v);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float m = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) m = fmaxf(m, cc * 32 + 16 * e + i < sees ? v[16 * e + i] : -INFINITY);
+      const float ks = ksc[2 * cc + e];
+      const float y = m == -INFINITY || ks == -INFINITY ? -INFINITY : m * (rm * ks);
+      mx = fmaxf(mx, y);
+      mv = fmaxf(mv, y + lvs[2 * cc + e]);
+    }
+  }
+  if (__any_sync(0xffffffffu, mx > m_ref + KP_SUM_SLACK || mv > mo_ref + KP_SLACK))
+    kp_move<HD>(to, outputs, mx, mv, m_ref, mo_ref, l);
+  const float mos = mo_ref == -INFINITY ? 0.f : mo_ref, ms = m_ref == -INFINITY ? 0.f : m_ref, back0 = ex2(mos - ms);
+#pragma unroll 1
+  for (int c2 = 0; c2 < 2; ++c2) {  // 64 positions: 32 columns of P over scores that have been read
+    uint32_t w[32];
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      float v[32];
+      tc_ld32(ts + c2 * 64 + hh * 32, v);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int blk = c2 * 4 + hh * 2 + e;
+        const float ks = ksc[blk], lv = lvs[blk];
+        // zero V: the weights count in the sum, their product with V is zero
+        const bool none = ks == -INFINITY, zero = lv == -INFINITY;  // the same for all rows
+        const float fk = rm * ks, off = zero ? -ms : lv - mos, back = zero ? 1.f : back0 * lvs[8 + blk];
+        const int n = none ? 0 : sees - blk * 16;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const float p0 = i < n ? ex2(fmaf(v[16 * e + i], fk, off)) : 0.f;
+          const float p1 = i + 1 < n ? ex2(fmaf(v[16 * e + i + 1], fk, off)) : 0.f;
+          sum += p0 + p1;
+          w[hh * 16 + e * 8 + i / 2] = zero ? 0u : h2u(__floats2half2_rn(p0, p1));
+        }
+        l = fmaf(sum, back, l);
+      }
+    }
+    tc_st32(ts + c2 * 32, w);
+  }
 }
 
 struct KPArgs {
@@ -151,6 +345,7 @@ struct KPArgs {
   const void* q; void* out;
   int64_t ldq, ldo;
   int dtype, tokens, group, rows, tiles;  // rows = tokens * group; tiles of KP_ROWS rows
+  int log_block;
   int splits;                             // shares of the positions, each a CTA
   bool vec, qvec;                         // out rows, query rows are 16-byte aligned
   float scale_log2e;                      // its absolute value; the sign goes with the queries
@@ -165,7 +360,7 @@ template <int HD, int CODE>
 __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs a) {
   using Cfg = KPCfg<HD>;
   extern __shared__ __align__(1024) uint8_t kp_raw[];
-  KPSmem<HD>& sm = *reinterpret_cast<KPSmem<HD>*>((reinterpret_cast<uintptr_t>(kp_raw) + 1023) & ~uintptr_t(1023));
+  KPSmem<HD>& sm = *reinterpret_cast<KPSmem<HD>*>(aligned_smem(kp_raw));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const N730KV8Cache& c = a.c;
   const int b = blockIdx.z, h = blockIdx.y;
@@ -185,8 +380,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&sm.kfull[i], 4);
-      mbar_init(&sm.vfull[i], 4);
+      mbar_init(&sm.kfull[i], KP_CODE_WARPS);
+      mbar_init(&sm.vfull[i], KP_CODE_WARPS);
       mbar_init(&sm.kfree[i], 1);
       mbar_init(&sm.vfree[i], 1);
       mbar_init(&sm.sfull[i], 1);
@@ -197,7 +392,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
     fence_mbar_init();
     sm.abort = 0;
   }
-  if (warp == 12) {
+  if (warp == KP_MMA_WARP) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                  :: "r"(smem_u32(&sm.tmem)), "r"(Cfg::TMEM) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -221,122 +416,183 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
   const uint32_t tmem = sm.tmem;
   volatile int* abortf = &sm.abort;
 
-  if (warp >= 8 && warp < 12) {
+  if (warp >= 8 && warp < 8 + KP_CODE_WARPS) {
     // ---------------- codes to fp16 ----------------
-    constexpr int LPR = HD / 16, RPI = 32 / LPR, NI = 32 / RPI;  // lanes a row, rows an instruction, instructions
-    const int w = warp - 8, row0 = w * 32 + lane / LPR, chunk = lane % LPR;
+    // A warp takes every third block of 16 positions (each in a page), a lane 16 bytes of every RPI-th row.
+    constexpr int LPR = HD / 16, RPI = 32 / LPR, NI = 16 / RPI;  // lanes a row, rows an instruction, instructions a block
+    constexpr int BLOCKS = KP_KEYS / 16, MINE = (BLOCKS + KP_CODE_WARPS - 1) / KP_CODE_WARPS;
+    const int w = warp - 8, lrow = lane / LPR, chunk = lane % LPR;
     const int* bt = c.block_table + (int64_t)b * c.max_pages;
-    // pool rows of the warp's two blocks of 16 positions of tile j (-1: no page)
-    auto lookup = [&](int j, int i) {
-      const int p = (j0 + j) * KP_KEYS + w * 32 + i * 16;
-      if (j >= nt || p >= sees_last) return -1;
-      const int page = bt[p / c.page_size];
-      return (unsigned)page < (unsigned)c.n_pages ? (page * c.n_kv + h) * c.page_size + p % c.page_size : -1;
-    };
-    uint4 kx[NI], vx[NI];  // asked for a tile ahead
-    auto load = [&](uint4 (&x)[NI], const void* pool, int j, int r_lo, int r_hi) {
+    auto block = [&](int i) { return w + KP_CODE_WARPS * i; };
+    // Walks over the warp's blocks, tile by tile: the page (-1 behind the last position) is looked up a tile before
+    // its row is needed, page and offset advance without divisions.
+    struct Walk { int p, idx, off, page; };
+    const int step_idx = KP_KEYS / c.page_size, step_off = KP_KEYS % c.page_size;
+    const int p_end = min(sees_last, (j0 + nt) * KP_KEYS);
+    Walk walk[MINE];
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int r = row0 + i * RPI - w * 32;  // within the warp's 32
-        const int base = r < 16 ? r_lo : r_hi;
-        const bool in = base >= 0 && (j0 + j) * KP_KEYS + w * 32 + r < sees_last;  // rows never written may hold anything
-        x[i] = in ? *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(pool) + ((int64_t)base + (r & 15)) * HD + chunk * 16)
-                  : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < MINE; ++i) {
+      const int p = j0 * KP_KEYS + block(i) * 16;
+      walk[i] = {p, p / c.page_size, p % c.page_size, block(i) < BLOCKS && p < p_end ? bt[p / c.page_size] : -1};
+    }
+    auto next_rows = [&](int (&row)[MINE]) {  // the rows of the pages looked up last; then the next ones' pages
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+        Walk& k = walk[i];
+        row[i] = (unsigned)k.page < (unsigned)c.n_pages ? (k.page * c.n_kv + h) * c.page_size + k.off : -1;
+        k.p += KP_KEYS;
+        k.idx += step_idx;
+        k.off += step_off;
+        if (k.off >= c.page_size) { k.off -= c.page_size; ++k.idx; }
+        k.page = block(i) < BLOCKS && k.p < p_end ? bt[k.idx] : -1;
       }
     };
-    // K's and V's scale of the two blocks, lanes 0 - 3
-    auto load_scale = [&](int r_lo, int r_hi) {
-      const int row = lane < 2 ? r_lo : r_hi;
-      if (lane >= 4 || row < 0) return lane & 1 ? 0.f : -INFINITY;
-      return ((lane & 1) ? c.v_scales : c.k_scales)[row / c.block];
-    };
-    auto store = [&](const uint4 (&x)[NI], uint8_t* dst) {
+    uint4 x[MINE][NI];  // the next fill's codes, asked for when the last one's have been stored
+    auto load = [&](const void* pool, const int (&row)[MINE]) {
 #pragma unroll
-      for (int i = 0; i < NI; ++i) kp_put_codes<CODE>(x[i], dst, Cfg::KB, row0 + i * RPI, chunk);
+      for (int k = 0; k < MINE; ++k) {
+        if (block(k) >= BLOCKS) break;
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(pool) + ((int64_t)max(row[k], 0) + lrow) * HD + chunk * 16;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) x[k][i] = *reinterpret_cast<const uint4*>(src + i * RPI * HD);
+      }
+    };
+    // lanes 2 i, 2 i + 1: K's and V's scale of block i; its row
+    auto lane_row = [&](const int (&row)[MINE]) {
+      int r = -1;
+#pragma unroll
+      for (int i = 0; i < MINE; ++i)
+        if (lane >> 1 == i) r = row[i];
+      return r;
+    };
+    auto load_scale = [&](const int (&row)[MINE]) {
+      const int r = lane_row(row);
+      return r >= 0 ? ((lane & 1) ? c.v_scales : c.k_scales)[r >> a.log_block] : -1.f;
+    };
+    const int at0 = lrow * 128 + (chunk >> 2) * Cfg::KB;
+    auto store = [&](uint8_t* dst, int j, const int (&row)[MINE]) {
+#pragma unroll
+      for (int k = 0; k < MINE; ++k) {
+        if (block(k) >= BLOCKS) break;
+        const int seen = sees_last - (j0 + j) * KP_KEYS - block(k) * 16;  // rows behind may hold anything, as may those without a page
+        if (seen < 16 || row[k] < 0)
+#pragma unroll
+          for (int i = 0; i < NI; ++i)
+            if (lrow + i * RPI >= seen || row[k] < 0) x[k][i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) kp_put_codes<CODE>(x[k][i], dst + at0 + (block(k) * 16 + i * RPI) * 128, (lrow + i * RPI) & 7, chunk);
+      }
     };
     auto ready = [&](uint64_t* bar) {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive1(bar);
     };
-    int lo = lookup(0, 0), hi = lookup(0, 1), lo1 = lookup(1, 0), hi1 = lookup(1, 1);
-    load(kx, c.k_codes, 0, lo, hi);
-    load(vx, c.v_codes, 0, lo, hi);
-    float scale = load_scale(lo, hi);
-    for (int j = 0; j < nt; ++j) {
-      const int s = j & 1;
-      const int lo2 = lookup(j + 2, 0), hi2 = lookup(j + 2, 1);
-      int go = 1;
-      if (lane == 0 && j >= 2) go = tc_wait(&sm.kfree[s], (uint32_t)((j / 2 - 1) & 1), abortf);
-      if (!__shfl_sync(0xffffffffu, go, 0)) break;
-      store(kx, sm.k[s]);
-      if (lane < 4) sm.sc[j % KP_RING][lane & 1][w * 2 + (lane >> 1)] = scale;
-      ready(&sm.kfull[s]);
-      load(kx, c.k_codes, j + 1, lo1, hi1);
-      scale = load_scale(lo1, hi1);
-      if (lane == 0 && j >= 2) go = tc_wait(&sm.vfree[s], (uint32_t)((j / 2 - 1) & 1), abortf);
-      if (!__shfl_sync(0xffffffffu, go, 0)) break;
-      store(vx, sm.v[s]);
-      ready(&sm.vfull[s]);
-      load(vx, c.v_codes, j + 1, lo1, hi1);
-      lo1 = lo2;
-      hi1 = hi2;
+    // fills in the order K0 K1 V0 K2 V1 ...: the next tile's scores go ahead of this one's outputs
+    int row_v[MINE], row_k[MINE];
+    next_rows(row_k);
+    float scale = load_scale(row_k);
+    load(c.k_codes, row_k);
+#pragma unroll 1
+    for (int f = 0; f < 2 * nt; ++f) {
+      // (K?, tile) of a fill
+      auto is_key = [&](int i) { return i == 0 || ((i & 1) && i < 2 * nt - 1); };
+      auto tile_of = [&](int i) { return is_key(i) ? (i + 1) >> 1 : i == 2 * nt - 1 ? nt - 1 : (i >> 1) - 1; };
+      const bool is_k = is_key(f);
+      const int j = tile_of(f), s = j & 1;
+      if (j >= 2 && !kp_wait_warp(is_k ? &sm.kfree[s] : &sm.vfree[s], (uint32_t)((j / 2 - 1) & 1), abortf)) break;
+      int row[MINE];
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) row[i] = is_k ? row_k[i] : row_v[i];
+      store(is_k ? sm.k[s] : sm.v[s], j, row);
+      if (is_k) {
+        const bool mine = lane < 2 * MINE && block(lane >> 1) < BLOCKS, none = lane_row(row) < 0;
+        if (mine) {
+          float* at = &sm.sc[j % KP_RING][lane & 1][block(lane >> 1)];
+          at[0] = none ? -INFINITY : lane & 1 ? lg2(scale) : scale;
+          if (lane & 1) at[8] = none || scale == 0.f ? 0.f : __frcp_rn(scale);
+        }
+        // whether every block has a page and a V scale
+        const bool odd = __any_sync(0xffffffffu, mine && (none || ((lane & 1) && scale == 0.f)));
+        if (lane == 0) sm.odd[j % KP_RING][w] = odd;
+      }
+      ready(is_k ? &sm.kfull[s] : &sm.vfull[s]);
+      if (f + 1 == 2 * nt) break;
+      const bool next_k = is_key(f + 1);
+      if (next_k || tile_of(f + 1) == nt - 1) {  // V follows a tile behind
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) row_v[i] = row_k[i];
+      }
+      if (next_k) {
+        next_rows(row_k);
+        scale = load_scale(row_k);
+        load(c.k_codes, row_k);
+      } else {
+        load(c.v_codes, row_v);
+      }
     }
-  } else if (warp == 12) {
+  } else if (warp == KP_MMA_WARP) {
     // ---------------- products ----------------
-    if (lane == 0) {
-      const uint32_t qs = smem_u32(sm.q);
-      auto scores = [&](int x, int s) {
-        const uint32_t ks = smem_u32(sm.k[s]);
+    // descriptors advance by constants from each tile's first (addresses are in units of 16 bytes)
+    const uint64_t qd = umma_desc_sw128(smem_u32(sm.q)), kd = umma_desc_sw128(smem_u32(sm.k[0]));
+    const uint64_t vd = umma_desc_mn_sw128(smem_u32(sm.v[0]), Cfg::KB);
+    auto scores = [&](int x, int s) {  // S = Q K^T
+      const uint64_t q0 = qd + (uint64_t)(x * (KP_ROWS / 2) * 128 / 16), k0 = kd + (uint64_t)(s * Cfg::KV / 16);
+      if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k)
-          tc_mma_ss<Cfg::IDESC_S>(tmem + Cfg::S0 + x * KP_KEYS,
-                                  umma_desc_sw128(qs + (k >> 2) * Cfg::QB + x * (KP_ROWS / 2) * 128 + (k & 3) * 32),
-                                  umma_desc_sw128(ks + (k >> 2) * Cfg::KB + (k & 3) * 32), k > 0);
+          tc_mma_ss<Cfg::IDESC_S>(tmem + Cfg::S0 + x * KP_KEYS, q0 + (uint64_t)(((k >> 2) * Cfg::QB + (k & 3) * 32) / 16),
+                                  k0 + (uint64_t)(((k >> 2) * Cfg::KB + (k & 3) * 32) / 16), k > 0);
         tc_commit(&sm.sfull[x]);
-      };
-      auto outputs = [&](int x, int s, bool first) {
-        const uint32_t vs = smem_u32(sm.v[s]);
+        if (x == 1) tc_commit(&sm.kfree[s]);
+      }
+      __syncwarp();
+    };
+    auto outputs = [&](int x, int s, bool first) {  // O += P V
+      const uint64_t v0 = vd + (uint64_t)(s * Cfg::KV / 16);
+      if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < KP_KEYS / 16; ++k)
-          tc_mma_ts<Cfg::IDESC_O>(tmem + Cfg::O0 + x * HD, tmem + Cfg::S0 + x * KP_KEYS + k * 8,
-                                  umma_desc_mn_sw128(vs + k * 2048, Cfg::KB), !(first && k == 0));
-      };
-      bool go = nt > 0 && tc_wait(&sm.kfull[0], 0, abortf);
-      if (go) {
-        tc_fence_after();
-        scores(0, 0);
-        scores(1, 0);
-        tc_commit(&sm.kfree[0]);
+          tc_mma_ts<Cfg::IDESC_O>(tmem + Cfg::O0 + x * HD, tmem + Cfg::S0 + x * KP_KEYS + k * 8, v0 + (uint64_t)(k * 2048 / 16),
+                                  !(first && k == 0));
+        if (x == 1) tc_commit(&sm.vfree[s]);
       }
-      for (int j = 0; go && j < nt; ++j) {
-        const int s = j & 1, s1 = s ^ 1;
-        const uint32_t ph = (uint32_t)((j / 2) & 1), ph1 = (uint32_t)(((j + 1) / 2) & 1);
-        go = tc_wait(&sm.vfull[s], ph, abortf);
-        for (int x = 0; go && x < 2; ++x) {
-          go = tc_wait(&sm.pready[x], (uint32_t)(j & 1), abortf);
+      __syncwarp();
+    };
+    bool go = nt > 0 && kp_wait_warp(&sm.kfull[0], 0, abortf);
+    if (go) {
+      tc_fence_after();
+      scores(0, 0);
+      scores(1, 0);
+    }
+#pragma unroll 1
+    for (int j = 0; go && j < nt; ++j) {
+      const int s = j & 1, s1 = s ^ 1;
+      const uint32_t ph = (uint32_t)((j / 2) & 1), ph1 = (uint32_t)(((j + 1) / 2) & 1);
+      go = kp_wait_warp(&sm.vfull[s], ph, abortf);
+#pragma unroll 1
+      for (int x = 0; go && x < 2; ++x) {
+        go = kp_wait_warp(&sm.pready[x], (uint32_t)(j & 1), abortf);
+        if (!go) break;
+        tc_fence_after();
+        outputs(x, s, j == 0);
+        if (j + 1 < nt) {
+          if (x == 0) go = kp_wait_warp(&sm.kfull[s1], ph1, abortf);
           if (!go) break;
           tc_fence_after();
-          outputs(x, s, j == 0);
-          if (x == 1) tc_commit(&sm.vfree[s]);
-          if (j + 1 < nt) {
-            if (x == 0) go = tc_wait(&sm.kfull[s1], ph1, abortf);
-            if (!go) break;
-            tc_fence_after();
-            scores(x, s1);
-            if (x == 1) tc_commit(&sm.kfree[s1]);
-          } else {
-            tc_commit(&sm.odone[x]);
-          }
+          scores(x, s1);
+        } else {
+          if (elect_one()) tc_commit(&sm.odone[x]);
+          __syncwarp();
         }
       }
-      if (!go && nt > 0) {  // what is in flight ends before the tensor memory is freed
-        *abortf = 1;
-        tc_commit(&sm.drain);
-        wait_bar(&sm.drain, 0);
-      }
     }
-    __syncwarp();
+    if (!go && nt > 0) {  // what is in flight ends before the tensor memory is freed
+      if (lane == 0) *abortf = 1;
+      if (elect_one()) tc_commit(&sm.drain);
+      wait_bar(&sm.drain, 0);
+      __syncwarp();
+    }
   } else {
     // ---------------- softmax: warps 0-3 of A, 4-7 of B, a thread a row ----------------
     const int x = warp >> 2, q = warp & 3, r = x * (KP_ROWS / 2) + q * 32 + lane, f = f0 + r;
@@ -348,96 +604,23 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
     float m_ref = -INFINITY, mo_ref = -INFINITY, l = 0.f;
     bool go = true;
     for (int j = 0; j < nt; ++j) {
-      int ok1 = 1;
-      if (lane == 0) ok1 = tc_wait(&sm.sfull[x], (uint32_t)(j & 1), abortf);
-      if (!__shfl_sync(0xffffffffu, ok1, 0)) { go = false; break; }
+      if (!kp_wait_warp(&sm.sfull[x], (uint32_t)(j & 1), abortf)) { go = false; break; }
       tc_fence_after();
       const float* ksc = sm.sc[j % KP_RING][0];
-      const float* vsc = sm.sc[j % KP_RING][1];
+      const float* lvs = sm.sc[j % KP_RING][1];
       const int p0 = (j0 + j) * KP_KEYS;
       const bool masked = p0 + KP_KEYS > sees_all;  // some row of the CTA does not see all of the tile
-      // largest score, and largest score + log2(V scale)
-      float mx = -INFINITY, mv = -INFINITY;
-#pragma unroll 1
-      for (int cc = 0; cc < 4; ++cc) {
-        float v[32];
-        tc_ld32(ts + cc * 32, v);
-        if (masked) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (p0 + cc * 32 + i >= vis) v[i] = -INFINITY;
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float m = v[16 * e];
-#pragma unroll
-          for (int i = 1; i < 16; ++i) m = fmaxf(m, v[16 * e + i]);
-          const float ks = ksc[2 * cc + e], vs = vsc[2 * cc + e];
-          const bool none = ks == -INFINITY;  // no page: not seen
-          const float y = m == -INFINITY || none ? -INFINITY : m * (rm * ks);
-          mx = fmaxf(mx, y);
-          mv = fmaxf(mv, y + lg2(vs));
-        }
-      }
-      const bool move = mx > m_ref + KP_SLACK || mv > mo_ref + KP_SLACK;
-      if (__any_sync(0xffffffffu, move)) {
-        const float mn = fmaxf(m_ref, mx), mon = fmaxf(mo_ref, mv);
-        if (mn != m_ref) l *= ex2(m_ref - mn);
-        const float fo = mon != mo_ref ? ex2(mo_ref - mon) : 1.f;
-        m_ref = mn;
-        mo_ref = mon;
-        if (j > 0) {
-#pragma unroll 1
-          for (int cc = 0; cc < HD / 32; ++cc) {
-            float v[32];
-            uint32_t w[32];
-            tc_ld32(to + cc * 32, v);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i] * fo);
-            tc_st32(to + cc * 32, w);
-          }
-        }
-      }
-      const float mos = mo_ref == -INFINITY ? 0.f : mo_ref, ms = m_ref == -INFINITY ? 0.f : m_ref;
-#pragma unroll 1
-      for (int c2 = 0; c2 < 2; ++c2) {  // 64 positions: 32 columns of P over the scores read
-        uint32_t w[32];
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          float v[32];
-          tc_ld32(ts + c2 * 64 + hh * 32, v);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int blk = c2 * 4 + hh * 2 + e;
-            const float ks = ksc[blk], vs = vsc[blk], lv = lg2(vs);
-            const bool none = ks == -INFINITY, zero = vs == 0.f;
-            // zero V: the weights count in the sum, their product with V is zero
-            const float fk = rm * ks, off = zero ? -ms : lv - mos, back = zero ? 1.f : ex2(mos - ms - lv);
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              float p = ex2(fmaf(v[16 * e + i], fk, off)), p1 = ex2(fmaf(v[16 * e + i + 1], fk, off));
-              if (masked || none) {
-                const int pos = p0 + blk * 16 + i;
-                if (pos >= vis || none) p = 0.f;
-                if (pos + 1 >= vis || none) p1 = 0.f;
-              }
-              sum += p + p1;
-              w[hh * 16 + e * 8 + i / 2] = zero ? 0u : h2u(__floats2half2_rn(p, p1));
-            }
-            l = fmaf(sum, back, l);
-          }
-        }
-        tc_st32(ts + c2 * 32, w);
-      }
+      const int4 odd4 = *reinterpret_cast<const int4*>(sm.odd[j % KP_RING]);
+      if (!masked && !(odd4.x | odd4.y | odd4.z))
+        kp_softmax<HD>(ts, to, ksc, lvs, rm, j > 0, m_ref, mo_ref, l);
+      else
+        kp_softmax_any<HD>(ts, to, ksc, lvs, rm, masked ? vis - p0 : KP_KEYS, j > 0, m_ref, mo_ref, l);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive1(&sm.pready[x]);
     }
     if (go && nt > 0) {
-      int ok1 = 1;
-      if (lane == 0) ok1 = tc_wait(&sm.odone[x], 0, abortf);
-      go = __shfl_sync(0xffffffffu, ok1, 0);
+      go = kp_wait_warp(&sm.odone[x], 0, abortf);
       tc_fence_after();
     }
     if (go) {
@@ -487,7 +670,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
   __syncthreads();
   tc_fence_after();
   if (*abortf && tid == 0) *a.status = 1;
-  if (warp == 12)
+  if (warp == KP_MMA_WARP)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(Cfg::TMEM) : "memory");
 }
 
@@ -510,13 +693,13 @@ struct KWSmem {
 };
 
 template <int HD, int CODE>
-__global__ void __launch_bounds__(KP_THREADS, 1)
+__global__ void __launch_bounds__(KW_THREADS, 1)
 kv8_prompt_weights_kernel(const KPArgs a, const float* w_in, float* w_out, int64_t ldw) {
   using Cfg = KPCfg<HD>;
   constexpr int E = HD / 32, RT = KP_KEYS;  // rows of a tile
   constexpr uint32_t COLS = 2 * RT;         // tensor memory: two score tiles
   extern __shared__ __align__(1024) uint8_t kp_raw[];
-  KWSmem<HD>& sm = *reinterpret_cast<KWSmem<HD>*>((reinterpret_cast<uintptr_t>(kp_raw) + 1023) & ~uintptr_t(1023));
+  KWSmem<HD>& sm = *reinterpret_cast<KWSmem<HD>*>(aligned_smem(kp_raw));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const N730KV8Cache& c = a.c;
   const int b = blockIdx.z, h = blockIdx.y, p0 = blockIdx.x * KP_KEYS;
@@ -550,11 +733,11 @@ kv8_prompt_weights_kernel(const KPArgs a, const float* w_in, float* w_out, int64
                  :: "r"(smem_u32(&sm.tmem)), "r"(COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  for (int i = tid; i < KP_KEYS * (HD / 16); i += KP_THREADS) {
+  for (int i = tid; i < KP_KEYS * (HD / 16); i += KW_THREADS) {
     const int r = i / (HD / 16), chunk = i % (HD / 16);
     const int64_t row = row_of(p0 + r);
     kp_put_codes<CODE>(row >= 0 ? *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(c.k_codes) + row * HD + chunk * 16)
-                                : make_uint4(0, 0, 0, 0), sm.k, Cfg::KB, r, chunk);
+                                : make_uint4(0, 0, 0, 0), sm.k + (chunk >> 2) * Cfg::KB + r * 128, r & 7, chunk);
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   tc_fence_before();
@@ -568,12 +751,10 @@ kv8_prompt_weights_kernel(const KPArgs a, const float* w_in, float* w_out, int64
     const int w = warp - 8;
     for (int i = 0; i < n; ++i) {
       const int s = i & 1;
-      int go = 1;
-      if (lane == 0 && i >= 2) {  // the products of the tile before are done, and its factors read
-        go = tc_wait(&sm.qfree[s], (uint32_t)((i / 2 - 1) & 1), abortf);
-        if (go) go = tc_wait(&sm.sread[s], (uint32_t)((i / 2 - 1) & 1), abortf);
-      }
-      if (!__shfl_sync(0xffffffffu, go, 0)) break;
+      // the products of the tile before are done, and its factors read
+      if (i >= 2 && !(kp_wait_warp(&sm.qfree[s], (uint32_t)((i / 2 - 1) & 1), abortf) &&
+                      kp_wait_warp(&sm.sread[s], (uint32_t)((i / 2 - 1) & 1), abortf)))
+        break;
 #pragma unroll 4
       for (int r = w; r < RT; r += 4) {
         const int f = (i0 + i) * RT + r;
@@ -589,36 +770,39 @@ kv8_prompt_weights_kernel(const KPArgs a, const float* w_in, float* w_out, int64
       if (lane == 0) mbar_arrive1(&sm.qfull[s]);
     }
   } else if (warp == 12) {
-    if (lane == 0) {
-      bool go = true;
-      for (int i = 0; go && i < n; ++i) {
-        const int s = i & 1;
-        go = tc_wait(&sm.qfull[s], (uint32_t)((i / 2) & 1), abortf);  // implies that the scores before in this buffer are read
-        if (!go) break;
-        tc_fence_after();
+    const uint64_t kd = umma_desc_sw128(smem_u32(sm.k)), qd = umma_desc_sw128(smem_u32(sm.q[0]));
+    bool go = true;
+#pragma unroll 1
+    for (int i = 0; go && i < n; ++i) {
+      const int s = i & 1;
+      go = kp_wait_warp(&sm.qfull[s], (uint32_t)((i / 2) & 1), abortf);  // implies that the scores before in this buffer are read
+      if (!go) break;
+      tc_fence_after();
+      const uint64_t q0 = qd + (uint64_t)(s * Cfg::KV / 16);
+      if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < HD / 16; ++k)
-          tc_mma_ss<Cfg::IDESC_S>(tmem + s * RT, umma_desc_sw128(smem_u32(sm.k) + (k >> 2) * Cfg::KB + (k & 3) * 32),
-                                  umma_desc_sw128(smem_u32(sm.q[s]) + (k >> 2) * Cfg::KB + (k & 3) * 32), k > 0);
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint64_t at = (uint64_t)(((k >> 2) * Cfg::KB + (k & 3) * 32) / 16);
+          tc_mma_ss<Cfg::IDESC_S>(tmem + s * RT, kd + at, q0 + at, k > 0);
+        }
         tc_commit(&sm.qfree[s]);
         tc_commit(&sm.sfull[s]);
       }
-      if (!go) {
-        *abortf = 1;
-        tc_commit(&sm.drain);
-        wait_bar(&sm.drain, 0);
-      }
+      __syncwarp();
     }
-    __syncwarp();
+    if (!go) {
+      if (lane == 0) *abortf = 1;
+      if (elect_one()) tc_commit(&sm.drain);
+      wait_bar(&sm.drain, 0);
+      __syncwarp();
+    }
   } else {
     const int x = warp >> 2, q = warp & 3, p = p0 + q * 32 + lane;
     const int64_t row = row_of(p);
     const float ks = row >= 0 ? c.k_scales[row / c.block] : 0.f;
     const uint32_t ts = tmem + ((uint32_t)(q * 32) << 16) + x * RT;
     for (int i = x; i < n; i += 2) {
-      int ok1 = 1;
-      if (lane == 0) ok1 = tc_wait(&sm.sfull[x], (uint32_t)((i / 2) & 1), abortf);
-      if (!__shfl_sync(0xffffffffu, ok1, 0)) break;
+      if (!kp_wait_warp(&sm.sfull[x], (uint32_t)((i / 2) & 1), abortf)) break;
       tc_fence_after();
       const int f0 = (i0 + i) * RT;
       const int first_seen = p0 + KP_KEYS - 1 <= L + f0 / a.group ? 0 : max(0, p - L) * a.group - f0;  // rows before it do not see p
@@ -675,6 +859,7 @@ static KPArgs kp_args(const KV8AttnCall& k, const KV8PromptPlan& p, int* status,
   a.scale_log2e = fabsf(k.scale) * 1.4426950408889634f;
   a.sign = k.scale < 0.f ? -1.f : 1.f;
   a.lens = k.lens; a.n_new = k.n_new;
+  a.log_block = k.c.block == 16 ? 4 : k.c.block == 32 ? 5 : 6;
   a.status = status; a.part = part; a.part_ml = part_ml; a.lse = lse;
   return a;
 }
@@ -691,7 +876,7 @@ static int prompt_weights_launch(const KPArgs& a, const KV8AttnCall& k, cudaStre
   if (int rc = smem_attr_once<kv8_prompt_weights_kernel<HD, CODE>>((int)smem)) return rc;
   const int cap = a.c.max_pages * a.c.page_size;
   return kv8_launch(kv8_prompt_weights_kernel<HD, CODE>, dim3((cap + KP_KEYS - 1) / KP_KEYS, a.c.n_kv, k.batch),
-                    dim3(KP_THREADS), smem, st, false, a, k.w_in, k.w_out, k.ldw);
+                    dim3(KW_THREADS), smem, st, false, a, k.w_in, k.w_out, k.ldw);
 }
 
 int kv8_prompt_launch(const KV8AttnCall& k, const KV8PromptPlan& p, int* status, float* part, float* part_ml, float* lse,
