@@ -115,52 +115,59 @@ __device__ __forceinline__ void tc_mma_ss(uint32_t tmem_d, uint64_t adesc, uint6
                :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(IDESC), "r"(accumulate) : "memory");
 }
 
-// HD / 32 consecutive channels of a row as fp32; `vec`: rows lie on whole 16 bytes
-template <int E>
-__device__ __forceinline__ void kp_load(const void* p, int64_t i, int dtype, bool vec, float (&x)[E]) {
-  if (vec && dtype != N730_F32) {
-    uint32_t w[E / 2];
-    if (E == 4) {
-      const uint2 y = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p) + i);
-      w[0] = y.x; w[E / 2 - 1] = y.y;
-    } else {
-      w[0] = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint16_t*>(p) + i);
-    }
+// Brings a warp's share of query rows into shared memory: row r (of 32) is scaled by a power of two, so that its largest magnitude lies in [2^13, 2^14) (rows of zeros or with an
+// infinity stay), and written as row r of a K-major, swizzled operand with `block` bytes between 64-channel blocks.
+// A lane takes 8 channels; `put(r, mul)` is called by one lane a row with what scores of it are to be multiplied by,
+// `at(r)` gives the row's first element, negative for rows that are not there.
+template <int HD, class At, class Put>
+__device__ __forceinline__ void kp_put_rows(const void* q, int dtype, bool vec, float sign, float scale, uint8_t* dst, int block,
+                                            int first, At at, Put put) {
+  constexpr int LPR = HD / 8, RPI = 32 / LPR, U = 4;  // lanes a row, rows an instruction, instructions in flight
+  const int lane = threadIdx.x & 31, sub = lane / LPR, ch = lane % LPR;
+#pragma unroll 1
+  for (int r0 = first; r0 < first + 32; r0 += U * RPI) {
+    float x[U][8];
 #pragma unroll
-    for (int e = 0; e < E / 2; ++e) {
-      if (dtype == N730_F16) {
-        const float2 f = __half22float2(u2h(w[e]));
-        x[2 * e] = f.x; x[2 * e + 1] = f.y;
-      } else {
-        x[2 * e] = __uint_as_float(w[e] << 16);
-        x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = at(r0 + u * RPI + sub);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[u][e] = 0.f;
+      if (i >= 0 && vec && dtype != N730_F32) {
+        const uint4 y = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(q) + i + ch * 8);
+        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (dtype == N730_F16) {
+            const float2 f = __half22float2(u2h(w[e]));
+            x[u][2 * e] = f.x; x[u][2 * e + 1] = f.y;
+          } else {
+            x[u][2 * e] = __uint_as_float(w[e] << 16);
+            x[u][2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+          }
+        }
+      } else if (i >= 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[u][e] = kv8_load1(q, i + ch * 8 + e, dtype);
       }
     }
-  } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = kv8_load1(p, i + e, dtype);
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + u * RPI + sub;
+      float m = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[u][e]));
+#pragma unroll
+      for (int k = 1; k < LPR; k <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+      const int ex = (int)((__float_as_uint(m) >> 23) & 255u);
+      const int sh = ex == 0 || ex == 255 ? 0 : min(max(140 - ex, -126), 126);
+      const float mul = __uint_as_float((uint32_t)(127 + sh) << 23) * sign;
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = h2u(__floats2half2_rn(x[u][2 * e] * mul, x[u][2 * e + 1] * mul));
+      *reinterpret_cast<uint4*>(dst + (ch >> 3) * block + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (ch == 0) put(r, scale * __uint_as_float((uint32_t)(127 - sh) << 23));
+    }
   }
-}
-// One row of queries (a warp, E channels a lane) scaled by a power of two and written as row r of a K-major,
-// swizzled operand with `block` bytes between 64-channel blocks; returns what scores of it are to be multiplied by.
-template <int E>
-__device__ __forceinline__ float kp_put_row(const float (&x)[E], float sign, float scale, uint8_t* dst, int block, int r) {
-  const int lane = threadIdx.x & 31, d = lane * E;
-  float m = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) m = fmaxf(m, fabsf(x[e]));
-  m = warp_max(m);
-  // the largest magnitude goes into [2^13, 2^14); rows of zeros or with an infinity stay
-  const int ex = (int)((__float_as_uint(m) >> 23) & 255u);
-  const int sh = ex == 0 || ex == 255 ? 0 : min(max(140 - ex, -126), 126);
-  const float mul = __uint_as_float((uint32_t)(127 + sh) << 23) * sign;
-  uint8_t* at = dst + (d >> 6) * block + r * 128 + ((((d >> 3) & 7) ^ (r & 7)) << 4) + (d & 7) * 2;
-  if (E == 4)
-    *reinterpret_cast<uint2*>(at) = make_uint2(h2u(__floats2half2_rn(x[0] * mul, x[1] * mul)),
-                                               h2u(__floats2half2_rn(x[E - 2] * mul, x[E - 1] * mul)));
-  else
-    *reinterpret_cast<uint32_t*>(at) = h2u(__floats2half2_rn(x[0] * mul, x[1] * mul));
-  return scale * __uint_as_float((uint32_t)(127 - sh) << 23);
 }
 // 16 codes as fp16 into a row of a swizzled operand, at the row's 128 bytes in the 64-channel block of `chunk`;
 // r7: the row's number mod 8.
@@ -398,17 +405,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   // ---- Q: a row per warp at a time, scaled by a power of two, K-major and swizzled ----
-#pragma unroll 4
-  for (int r = warp; r < KP_ROWS; r += KP_THREADS / 32) {
-    constexpr int E = HD / 32;  // channels a lane
-    float x[E] = {};
-    const int f = f0 + r;
-    if (r < nrow)
-      kp_load<E>(a.q, ((int64_t)b * a.tokens + f / a.group) * a.ldq + (int64_t)(h * a.group + f % a.group) * HD + lane * E,
-                 a.dtype, a.qvec, x);
-    const float rm = kp_put_row<E>(x, a.sign, a.scale_log2e, sm.q, Cfg::QB, r);
-    if (lane == 0) sm.rowmul[r] = rm;
-  }
+  if (warp < 8)  // 32 rows each
+    kp_put_rows<HD>(a.q, a.dtype, a.qvec, a.sign, a.scale_log2e, sm.q, Cfg::QB, warp * 32,
+                    [&](int r) -> int64_t {
+                      const int f = f0 + r;
+                      return r < nrow ? ((int64_t)b * a.tokens + f / a.group) * a.ldq + (int64_t)(h * a.group + f % a.group) * HD : -1;
+                    },
+                    [&](int r, float mul) { sm.rowmul[r] = mul; });
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   tc_fence_before();
   __syncthreads();
@@ -696,7 +699,7 @@ template <int HD, int CODE>
 __global__ void __launch_bounds__(KW_THREADS, 1)
 kv8_prompt_weights_kernel(const KPArgs a, const float* w_in, float* w_out, int64_t ldw) {
   using Cfg = KPCfg<HD>;
-  constexpr int E = HD / 32, RT = KP_KEYS;  // rows of a tile
+  constexpr int RT = KP_KEYS;               // rows of a tile
   constexpr uint32_t COLS = 2 * RT;         // tensor memory: two score tiles
   extern __shared__ __align__(1024) uint8_t kp_raw[];
   KWSmem<HD>& sm = *reinterpret_cast<KWSmem<HD>*>(aligned_smem(kp_raw));
@@ -755,16 +758,15 @@ kv8_prompt_weights_kernel(const KPArgs a, const float* w_in, float* w_out, int64
       if (i >= 2 && !(kp_wait_warp(&sm.qfree[s], (uint32_t)((i / 2 - 1) & 1), abortf) &&
                       kp_wait_warp(&sm.sread[s], (uint32_t)((i / 2 - 1) & 1), abortf)))
         break;
-#pragma unroll 4
-      for (int r = w; r < RT; r += 4) {
-        const int f = (i0 + i) * RT + r;
-        float x[E] = {};
-        if (f < rows)
-          kp_load<E>(a.q, ((int64_t)b * a.tokens + f / a.group) * a.ldq + (int64_t)(h * a.group + f % a.group) * HD + lane * E,
-                     a.dtype, a.qvec, x);
-        const float rm = kp_put_row<E>(x, a.sign, a.scale_log2e, sm.q[s], Cfg::KB, r);
-        if (lane == 0) sm.row[s][r] = make_float2(rm, f < rows ? a.lse[head * a.rows + f] : INFINITY);
-      }
+      const int first = (i0 + i) * RT;
+      kp_put_rows<HD>(a.q, a.dtype, a.qvec, a.sign, a.scale_log2e, sm.q[s], Cfg::KB, w * 32,
+                      [&](int r) -> int64_t {
+                        const int f = first + r;
+                        return f < rows ? ((int64_t)b * a.tokens + f / a.group) * a.ldq + (int64_t)(h * a.group + f % a.group) * HD : -1;
+                      },
+                      [&](int r, float mul) {
+                        sm.row[s][r] = make_float2(mul, first + r < rows ? a.lse[head * a.rows + first + r] : INFINITY);
+                      });
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive1(&sm.qfull[s]);
