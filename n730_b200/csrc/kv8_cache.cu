@@ -197,24 +197,26 @@ __global__ void __launch_bounds__(KV8_THREADS) kv8_append_kernel(const KV8Append
   const int p0 = (L / c.block + j) * c.block;
   if (p0 >= end || L >= end) return;
   const int page = c.block_table[(int64_t)b * c.max_pages + p0 / c.page_size];
+  const void* x = which ? a.x[1] : a.x[0];
+  const int chunk = tid % CPR, r0 = tid / CPR;
+  const bool had = p0 < L;
+  float v[NP][16];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {  // the rows do not wait for the page
+    const int r = r0 + i * RPP, p = p0 + r;
+    if (r < c.block && p >= L && p < end)
+      kv8_load16(x, ((int64_t)b * a.tokens + (p - L)) * a.ld + (int64_t)h * HD + chunk * 16, a.dtype, a.vec, v[i]);
+    else
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[i][e] = 0.f;
+  }
   if ((unsigned)page >= (unsigned)c.n_pages) return;  // no page: its rows are dropped
   const int64_t row0 = ((int64_t)page * c.n_kv + h) * c.page_size + p0 % c.page_size;
   uint8_t* codes = reinterpret_cast<uint8_t*>(which ? c.v_codes : c.k_codes) + row0 * HD;
   float* scale = (which ? c.v_scales : c.k_scales) + row0 / c.block;
-  const void* x = which ? a.x[1] : a.x[0];
-  const int chunk = tid % CPR, r0 = tid / CPR;
-  const bool had = p0 < L;
-
-  float v[NP][16];
   float m = 0.f;
 #pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const int r = r0 + i * RPP, p = p0 + r;
-    if (r < c.block && p >= L && p < end) {
-      kv8_load16(x, ((int64_t)b * a.tokens + (p - L)) * a.ld + (int64_t)h * HD + chunk * 16, a.dtype, a.vec, v[i]);
-      m = fmaxf(m, kv8_amax(v[i]));
-    }
-  }
+  for (int i = 0; i < NP; ++i) m = fmaxf(m, kv8_amax(v[i]));
   const float s0 = had ? *scale : 0.f;
   m = warp_max(m);
   if ((tid & 31) == 0) red[tid >> 5] = m;
@@ -263,42 +265,60 @@ int kv8_append_launch(const N730KV8Cache& c, const void* k, const void* v, int d
 struct KV8ReadArgs {
   N730KV8Cache c;
   void* y[2];
-  int dtype, tokens;
+  int dtype, tokens, log_block;
   int64_t ld;
   bool vec;
   const int* first; const int* lens;
 };
 
-// A thread takes 16 channels of one position (a 16-byte load); consecutive threads walk along a
-// head's rows, which are contiguous in a page.  Bound by HBM: 1 byte read, 2 or 4 written a value.
+// A thread takes 16 channels of RD_ROWS positions, a warp's lanes whole rows one behind the other (contiguous in a
+// page); its loads do not wait for one another.  Bound by HBM: 1 byte read, 2 or 4 written a value.  With one
+// position a thread 8192 positions of 8 sequences and heads took 67 us (5.1 TB/s), too few bytes in flight.
+constexpr int RD_ROWS = 4;
+
 template <int HD, int CODE>
 __global__ void __launch_bounds__(KV8_THREADS) kv8_read_kernel(const KV8ReadArgs a) {
-  constexpr int CPR = HD / 16;
+  constexpr int CPR = HD / 16, RPP = KV8_THREADS / CPR;  // chunks a row, rows a pass
   const N730KV8Cache& c = a.c;
   const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1;
-  const int64_t i = (int64_t)blockIdx.x * KV8_THREADS + threadIdx.x;
-  const int64_t t = i / CPR;
-  const int chunk = (int)(i % CPR);
-  if (t >= a.tokens) return;
+  const int chunk = threadIdx.x % CPR;
+  const int64_t t0 = (int64_t)blockIdx.x * (RPP * RD_ROWS) + threadIdx.x / CPR;
   const int cap = c.max_pages * c.page_size;
   const int L = kv8_len(a.lens, b, cap);
-  const int64_t p = (a.first ? a.first[b] : 0) + t;
-  float y[16];
+  const int64_t p0 = (a.first ? a.first[b] : 0) + t0;
+  const uint8_t* codes = reinterpret_cast<const uint8_t*>(which ? c.v_codes : c.k_codes);
+  const float* scales = which ? c.v_scales : c.k_scales;
+  int64_t row[RD_ROWS];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) y[e] = 0.f;
-  if (p >= 0 && p < L) {
-    const int page = c.block_table[(int64_t)b * c.max_pages + (int)p / c.page_size];
-    if ((unsigned)page < (unsigned)c.n_pages) {
-      const int64_t row = ((int64_t)page * c.n_kv + h) * c.page_size + (int)p % c.page_size;
-      const uint8_t* codes = reinterpret_cast<const uint8_t*>(which ? c.v_codes : c.k_codes);
-      const float s = (which ? c.v_scales : c.k_scales)[row / c.block];
-      kv8_unpack<CODE>(*reinterpret_cast<const uint4*>(codes + row * HD + chunk * 16), y);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) y[e] *= s;
+  for (int i = 0; i < RD_ROWS; ++i) {
+    const int64_t p = p0 + i * RPP;
+    row[i] = -1;
+    if (p >= 0 && p < L && t0 + i * RPP < a.tokens) {
+      const int page = c.block_table[(int64_t)b * c.max_pages + (int)p / c.page_size];
+      if ((unsigned)page < (unsigned)c.n_pages) row[i] = ((int64_t)page * c.n_kv + h) * c.page_size + (int)p % c.page_size;
     }
   }
-  kv8_store16(which ? a.y[1] : a.y[0], ((int64_t)b * a.tokens + t) * a.ld + (int64_t)h * HD + chunk * 16, a.dtype, a.vec,
-              y);
+  uint4 q[RD_ROWS];
+  float s[RD_ROWS];
+#pragma unroll
+  for (int i = 0; i < RD_ROWS; ++i) {
+    q[i] = make_uint4(0, 0, 0, 0);
+    s[i] = 0.f;
+    if (row[i] >= 0) {
+      q[i] = __ldcs(reinterpret_cast<const uint4*>(codes + row[i] * HD + chunk * 16));
+      s[i] = scales[row[i] >> a.log_block];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < RD_ROWS; ++i) {
+    const int64_t t = t0 + i * RPP;
+    if (t >= a.tokens) break;
+    float y[16];
+    kv8_unpack<CODE>(q[i], y);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) y[e] = row[i] >= 0 ? y[e] * s[i] : 0.f;
+    kv8_store16(which ? a.y[1] : a.y[0], ((int64_t)b * a.tokens + t) * a.ld + (int64_t)h * HD + chunk * 16, a.dtype, a.vec, y);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -310,21 +330,28 @@ __global__ void __launch_bounds__(KV8_THREADS) kv8_read_kernel(const KV8ReadArgs
 // j-th; all others stay where they are with the codes they have.  A cache in order would have to
 // move, and requantise, nearly every row at every call; attention does not ask for order.
 //
-// Two kernels: the selection (one CTA per sequence and head) writes src[slot], the slot whose row
-// belongs at `slot` (or -1 in the first entry: nothing to move); the move rewrites the blocks that
-// take rows in.  Rows read from behind `keep` (a multiple of the block) are written by nobody.
+// Two kernels: the selection (one CTA per sequence and head) writes src[slot], the pool row whose
+// codes belong at `slot` (-1 without a page, -2 in the first entry when nothing is to move); the move
+// rewrites the blocks that take rows in.  Rows read from behind `keep` (a multiple of the block) are
+// written by nobody.
+//
+// Selection: the keys are read once into shared memory (up to EV_KEYS of them; longer contexts read
+// them again), the keep-th largest is found 11 bits at a time, and ranks of ties, holes and movers come
+// from ballots: a warp owns a run of slots, one scan over the warps' counts a pass.
 struct KV8EvictArgs {
   N730KV8Cache c;
-  int keep, first, recent;
+  int keep, first, recent, log_block;
   int64_t ldw;
   const int* seen; const int* lens_in; int* lens_out;
   const float* w_in; float* w_out;
   const int* pos_in; int* pos_out;
-  int* src;  // [batch][n_kv][keep]
+  int* src;  // [batch][n_kv][keep] pool rows, then as many slots
+  int keys;  // of a row held in shared memory: all that the table can hold, or none
 };
 
 constexpr int EV_THREADS = 1024;
-constexpr int EV_BINS = 2048;  // 11 bits a pass, three passes over the 32-bit key
+constexpr int EV_BINS = 2048;   // 11 bits a pass, three passes over the 32-bit key
+constexpr int EV_KEYS = 50000;  // 200 KB
 
 // Order of the kept: protected slots first, then by weight (NaN as the smallest, -0 as 0).
 __device__ __forceinline__ uint32_t ev_key(float w, int pos, int first, int last) {
@@ -363,6 +390,7 @@ __device__ __forceinline__ int ev_scan(int v, int* wsum, int* total) {
 }
 
 __global__ void __launch_bounds__(EV_THREADS) kv8_evict_select_kernel(const KV8EvictArgs a) {
+  extern __shared__ uint32_t ev_keys[];
   __shared__ int hist[EV_BINS];
   __shared__ int wsum[33];
   __shared__ int pick_bin, pick_above;
@@ -377,7 +405,7 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_select_kernel(const KV8E
   int* pos_out = a.pos_out + head * a.ldw;
   int* src = a.src + head * a.keep;
   if (L <= a.keep) {
-    if (tid == 0) src[0] = -1;
+    if (tid == 0) src[0] = -2;
     for (int64_t i = tid; i < a.ldw; i += EV_THREADS) {
       w_out[i] = i < L ? w_in[i] : 0.f;
       pos_out[i] = pos_in[i];
@@ -385,6 +413,9 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_select_kernel(const KV8E
     return;
   }
   const int seen = a.seen[b], last = seen - a.recent;
+  const int lane = tid & 31, warp = tid >> 5;
+  for (int i = tid; i < min(L, a.keys); i += EV_THREADS) ev_keys[i] = ev_key(w_in[i], pos_in[i], a.first, last);
+  auto key = [&](int i) { return a.keys ? ev_keys[i] : ev_key(w_in[i], pos_in[i], a.first, last); };
   // the keep-th largest key, 11 + 11 + 10 bits at a time
   uint32_t prefix = 0;
   int want = a.keep;  // of the slots whose key has the chosen prefix
@@ -394,7 +425,7 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_select_kernel(const KV8E
     for (int i = tid; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
     __syncthreads();
     for (int i = tid; i < L; i += EV_THREADS) {
-      const uint32_t k = ev_key(w_in[i], pos_in[i], a.first, last);
+      const uint32_t k = key(i);
       if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1);
     }
     __syncthreads();
@@ -410,47 +441,62 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_select_kernel(const KV8E
     __syncthreads();
   }
   const uint32_t cut = prefix;  // slots above it stay, and the first `want` equal to it
-  // each thread a run of consecutive slots: ties, then holes and movers, by block scans
-  const int run = (L + EV_THREADS - 1) / EV_THREADS, i0 = min(L, tid * run), i1 = min(L, i0 + run);
+  // each warp a run of slots, 32 at a time; counts(flag) is how many of the warps before have it
+  const int run = ((L + EV_THREADS - 1) / EV_THREADS) * 32, i0 = min(L, warp * run), i1 = min(L, i0 + run);
+  const uint32_t before = (1u << lane) - 1u;
+  auto counts = [&](int n) {
+    int total;
+    const int mine = ev_scan(lane == 0 ? n : 0, wsum, &total);
+    return __shfl_sync(0xffffffffu, mine, 0);
+  };
   int ties = 0;
-  for (int i = i0; i < i1; ++i) ties += ev_key(w_in[i], pos_in[i], a.first, last) == cut;
-  int total;
-  const int tie0 = ev_scan(ties, wsum, &total);
+  for (int i = i0; i < i1; i += 32) ties += __popc(__ballot_sync(0xffffffffu, i + lane < i1 && key(i + lane) == cut));
+  const int tie0 = counts(ties);
+  // stays(i): called for i = i0 + lane, + 32, ... with the ties so far in t
+  auto stays = [&](int i, int& t) {
+    const uint32_t k = i < i1 ? key(i) : 0u;
+    const uint32_t tie = __ballot_sync(0xffffffffu, i < i1 && k == cut);
+    const bool yes = i < i1 && (k > cut || (k == cut && t + __popc(tie & before) < want));
+    t += __popc(tie);
+    return yes;
+  };
   int holes = 0, movers = 0, t = tie0;
-  for (int i = i0; i < i1; ++i) {
-    const uint32_t k = ev_key(w_in[i], pos_in[i], a.first, last);
-    const bool stays = k > cut || (k == cut && t++ < want);
-    holes += !stays && i < a.keep;
-    movers += stays && i >= a.keep;
+  for (int i = i0 + lane; i - lane < i1; i += 32) {
+    const bool yes = stays(i, t);
+    holes += __popc(__ballot_sync(0xffffffffu, i < i1 && !yes && i < a.keep));
+    movers += __popc(__ballot_sync(0xffffffffu, yes && i >= a.keep));
   }
-  const int hole0 = ev_scan(holes, wsum, &total);
-  __syncthreads();
-  const int mover0 = ev_scan(movers, wsum, &total);
-  // the j-th hole's slot into src[keep - 1 - j] would overwrite; keep the holes in their own places:
-  // holes first note their rank, movers then look their hole up through the list below
-  int* list = a.src + (int64_t)gridDim.y * c.n_kv * a.keep + head * a.keep;  // hole slots by rank
+  const int hole0 = counts(holes);
+  const int mover0 = counts(movers);
+  // slots before the budget: their own, or (holes, listed by rank) a mover's
+  int* from = a.src + (int64_t)gridDim.y * c.n_kv * a.keep + head * a.keep;  // the slot that comes to a slot
+  int* list = src;                                                            // holes by rank, until the rows go there
   t = tie0;
   int hr = hole0;
-  for (int i = i0; i < i1 && i < a.keep; ++i) {
-    const uint32_t k = ev_key(w_in[i], pos_in[i], a.first, last);
-    const bool stays = k > cut || (k == cut && t++ < want);
-    if (stays) src[i] = i;
-    else list[hr++] = i;
+  for (int i = i0 + lane; i - lane < i1; i += 32) {
+    const bool yes = stays(i, t), hole = i < i1 && !yes && i < a.keep;
+    const uint32_t m = __ballot_sync(0xffffffffu, hole);
+    if (yes && i < a.keep) from[i] = i;
+    if (hole) list[hr + __popc(m & before)] = i;
+    hr += __popc(m);
   }
   __syncthreads();
   t = tie0;
   int mr = mover0;
-  for (int i = i0; i < i1; ++i) {
-    const uint32_t k = ev_key(w_in[i], pos_in[i], a.first, last);
-    const bool stays = k > cut || (k == cut && t++ < want);
-    if (stays && i >= a.keep) src[list[mr++]] = i;
+  for (int i = i0 + lane; i - lane < i1; i += 32) {
+    const bool mover = stays(i, t) && i >= a.keep;
+    const uint32_t m = __ballot_sync(0xffffffffu, mover);
+    if (mover) from[list[mr + __popc(m & before)]] = i;
+    mr += __popc(m);
   }
   __syncthreads();
   // weights and positions; in and out may be the same arrays: sources are never slots written before
+  const int* bt = c.block_table + (int64_t)b * c.max_pages;
   for (int i = tid; i < a.keep; i += EV_THREADS) {
-    const int s = src[i];
+    const int s = from[i], page = bt[s / c.page_size];
     w_out[i] = w_in[s];
     pos_out[i] = pos_in[s];
+    src[i] = (unsigned)page < (unsigned)c.n_pages ? (page * c.n_kv + h) * c.page_size + s % c.page_size : -1;
   }
   __syncthreads();
   for (int64_t i = a.keep + tid; i < a.ldw; i += EV_THREADS) {
@@ -465,65 +511,60 @@ __global__ void __launch_bounds__(KV8_THREADS) kv8_evict_move_kernel(const KV8Ev
   constexpr int CPR = HD / 16, RPP = KV8_THREADS / CPR;
   const N730KV8Cache& c = a.c;
   const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
+  pdl_wait();
   if (blockIdx.x == 0 && h == 0 && tid == 0)
     a.lens_out[b] = min(kv8_len(a.lens_in, b, c.max_pages * c.page_size), a.keep);
   const int64_t head = (int64_t)b * c.n_kv + h;
   const int* src = a.src + head * a.keep;
-  if (src[0] < 0) return;
   const int p0 = blockIdx.x * c.block;
-  const int* bt = c.block_table + (int64_t)b * c.max_pages;
-  auto row_of = [&](int slot) -> int64_t {  // row in the pool, -1 without a page
-    const int page = bt[slot / c.page_size];
-    return (unsigned)page < (unsigned)c.n_pages ? ((int64_t)page * c.n_kv + h) * c.page_size + slot % c.page_size : -1;
-  };
-  const int64_t row0 = row_of(p0);
-  const int chunk = tid % CPR, r0 = tid / CPR;
-  // the block's rows: does any come from elsewhere, and the largest scale among them
-  const int lane = tid & 31;
-  bool any = false;
+  const int chunk = tid % CPR, r0 = tid / CPR, lane = tid & 31;
+  // the block's own rows, and those that belong there
+  const int page = c.block_table[(int64_t)b * c.max_pages + p0 / c.page_size];
+  int row[NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) row[i] = r0 + i * RPP < c.block ? src[p0 + r0 + i * RPP] : -1;
+  const int lr0 = lane < c.block ? src[p0 + lane] : -1, lr1 = lane + 32 < c.block ? src[p0 + 32 + lane] : -1;
+  if (src[0] == -2) return;
+  const int row0 = (unsigned)page < (unsigned)c.n_pages ? (page * c.n_kv + h) * c.page_size + p0 % c.page_size : -1;
+  // does any come from elsewhere, and the largest scale among them: every warp on its own
+  bool any = lane < c.block && lr0 != row0 + lane;
+  any |= lane + 32 < c.block && lr1 != row0 + 32 + lane;
   float sk = 0.f, sv = 0.f;
-  for (int r = lane; r < c.block; r += 32) {  // every warp on its own
-    const int s = src[p0 + r];
-    any |= s != p0 + r;
-    const int64_t row = row_of(s);
-    if (row >= 0) {
-      sk = fmaxf(sk, c.k_scales[row / c.block]);
-      sv = fmaxf(sv, c.v_scales[row / c.block]);
-    }
-  }
+  if (lr0 >= 0) { sk = c.k_scales[lr0 >> a.log_block]; sv = c.v_scales[lr0 >> a.log_block]; }
+  if (lr1 >= 0) { sk = fmaxf(sk, c.k_scales[lr1 >> a.log_block]); sv = fmaxf(sv, c.v_scales[lr1 >> a.log_block]); }
   any = __any_sync(0xffffffffu, any);
   if (!any || row0 < 0) return;  // the same in every warp
-  sk = warp_max(sk);
-  sv = warp_max(sv);
   float sf[NP][2];
   uint4 q[NP][2];
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    const int r = r0 + i * RPP;
     q[i][0] = q[i][1] = make_uint4(0, 0, 0, 0);
-    sf[i][0] = sk; sf[i][1] = sv;
-    if (r >= c.block) continue;
-    const int64_t row = row_of(src[p0 + r]);
-    if (row < 0) continue;  // a row without a page reads as zeros
-    sf[i][0] = c.k_scales[row / c.block];
-    sf[i][1] = c.v_scales[row / c.block];
-    q[i][0] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(c.k_codes) + row * HD + chunk * 16);
-    q[i][1] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(c.v_codes) + row * HD + chunk * 16);
+    sf[i][0] = sf[i][1] = -1.f;
+    if (row[i] < 0) continue;  // a row without a page reads as zeros
+    sf[i][0] = c.k_scales[row[i] >> a.log_block];
+    sf[i][1] = c.v_scales[row[i] >> a.log_block];
+    q[i][0] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(c.k_codes) + (int64_t)row[i] * HD + chunk * 16);
+    q[i][1] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(c.v_codes) + (int64_t)row[i] * HD + chunk * 16);
   }
+  sk = warp_max(sk);
+  sv = warp_max(sv);
   __syncthreads();  // every thread has read the block's old scales
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     const int r = r0 + i * RPP;
     if (r >= c.block) continue;
-    const int64_t at = (row0 + r) * HD + chunk * 16;
-    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(c.k_codes) + at) =
-        sf[i][0] == sk ? q[i][0] : kv8_recode<CODE>(q[i][0], sf[i][0], sk);
-    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(c.v_codes) + at) =
-        sf[i][1] == sv ? q[i][1] : kv8_recode<CODE>(q[i][1], sf[i][1], sv);
+    const int64_t at = ((int64_t)row0 + r) * HD + chunk * 16;
+    const bool stays = row[i] == row0 + r;  // rows in place are written only where the scale grows
+    if (!stays || sf[i][0] != sk)
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(c.k_codes) + at) =
+          sf[i][0] == sk || row[i] < 0 ? q[i][0] : kv8_recode<CODE>(q[i][0], sf[i][0], sk);
+    if (!stays || sf[i][1] != sv)
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(c.v_codes) + at) =
+          sf[i][1] == sv || row[i] < 0 ? q[i][1] : kv8_recode<CODE>(q[i][1], sf[i][1], sv);
   }
   if (tid == 0) {
-    c.k_scales[row0 / c.block] = sk;
-    c.v_scales[row0 / c.block] = sv;
+    c.k_scales[row0 >> a.log_block] = sk;
+    c.v_scales[row0 >> a.log_block] = sv;
   }
 }
 
@@ -557,8 +598,9 @@ N730_API int n730_kv8_read(const N730KV8Cache* c, void* d_k, void* d_v, int dtyp
   a.dtype = dtype; a.tokens = tokens; a.ld = ld;
   a.vec = (((uintptr_t)d_k | (uintptr_t)d_v) & 15) == 0 && ld * kv8_esize(dtype) % 16 == 0;
   a.first = d_first; a.lens = d_lens;
-  const int64_t n = (int64_t)tokens * (c->head_dim / 16);
-  const dim3 grid((unsigned)((n + KV8_THREADS - 1) / KV8_THREADS), 2 * c->n_kv, batch);
+  a.log_block = c->block == 16 ? 4 : c->block == 32 ? 5 : 6;
+  const int rows = KV8_THREADS / (c->head_dim / 16) * RD_ROWS;
+  const dim3 grid((unsigned)(((int64_t)tokens + rows - 1) / rows), 2 * c->n_kv, batch);
   cudaStream_t st = (cudaStream_t)stream;
   if (c->head_dim == 128) {
     if (c->code == N730_KV8_INT8) return kv8_launch(kv8_read_kernel<128, N730_KV8_INT8>, grid, dim3(KV8_THREADS), 0, st, false, a);
@@ -601,11 +643,16 @@ N730_API int n730_kv8_evict(const N730KV8Cache* c, int batch, int keep, int firs
   a.seen = d_seen; a.lens_in = d_lens; a.lens_out = d_lens_out;
   a.w_in = d_w; a.w_out = d_w_out; a.pos_in = d_pos; a.pos_out = d_pos_out;
   a.src = reinterpret_cast<int*>(d_ws);
+  a.log_block = c->block == 16 ? 4 : c->block == 32 ? 5 : 6;
+  const int cap = c->max_pages * c->page_size;
+  a.keys = cap <= EV_KEYS ? cap : 0;
   cudaStream_t st = (cudaStream_t)stream;
-  if (int rc = kv8_launch(kv8_evict_select_kernel, dim3(c->n_kv, batch), dim3(EV_THREADS), 0, st, false, a)) return rc;
+  if (int rc = smem_attr_once<kv8_evict_select_kernel>(EV_KEYS * 4)) return rc;
+  if (int rc = kv8_launch(kv8_evict_select_kernel, dim3(c->n_kv, batch), dim3(EV_THREADS), (size_t)a.keys * 4, st, false, a))
+    return rc;
   const dim3 grid(keep / c->block, c->n_kv, batch);
   const int np = (c->block * (c->head_dim / 16) + KV8_THREADS - 1) / KV8_THREADS;
-#define N730_MOVE(HD, CODE, NP) kv8_launch(kv8_evict_move_kernel<HD, CODE, NP>, grid, dim3(KV8_THREADS), 0, st, false, a)
+#define N730_MOVE(HD, CODE, NP) kv8_launch(kv8_evict_move_kernel<HD, CODE, NP>, grid, dim3(KV8_THREADS), 0, st, true, a)
 #define N730_MOVE_CODE(CODE)                                                     \
   if (c->head_dim == 128)                                                        \
     return np == 1 ? N730_MOVE(128, CODE, 1) : np == 2 ? N730_MOVE(128, CODE, 2) : N730_MOVE(128, CODE, 4); \
