@@ -137,13 +137,28 @@ __device__ __forceinline__ void kv8_unpack(const uint4& c, float (&y)[16]) {
     }
   }
 }
+// Quotients by one scale: with r the rounded reciprocal and y = x r rounded, y + (x - y s) r, each by one FMA, is the
+// rounded quotient unless s's significand is all ones (P. Markstein, "Computation of elementary functions on the
+// IBM RISC System/6000 processor", 1990, theorem on correctly rounded quotients).  It needs the remainder to be
+// exact, so the scale is asked to lie in [2^-60, 2^60]: quotients of rows too small for that are codes of 0.  Other
+// scales take the division (which cost more than the row's memory traffic: 4096 rows of 8 heads 13.9 us).
 template <int CODE>
 __device__ __forceinline__ uint4 kv8_encode(const float (&x)[16], float s) {
   float y[16];
+  if (s >= 0x1p-60f && s <= 0x1p60f && (__float_as_uint(s) & 0x7fffffu) != 0x7fffffu) {
+    const float r = __frcp_rn(s), most = 1024.f * s;  // past the largest code either way
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const float v = CODE == N730_KV8_E4M3 && isnan(x[e]) ? 0.f : x[e];
-    y[e] = s > 0.f ? __fdiv_rn(v, s) : 0.f;
+    for (int e = 0; e < 16; ++e) {
+      const float v = x[e] == x[e] ? fminf(fmaxf(x[e], -most), most) : 0.f;
+      const float q = __fmul_rn(v, r);
+      y[e] = __fmaf_rn(__fmaf_rn(-q, s, v), r, q);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float v = x[e] == x[e] ? x[e] : 0.f;
+      y[e] = s > 0.f ? __fdiv_rn(v, s) : 0.f;
+    }
   }
   return kv8_pack<CODE>(y);
 }
@@ -346,7 +361,8 @@ struct KV8EvictArgs {
   const float* w_in; float* w_out;
   const int* pos_in; int* pos_out;
   int* src;  // [batch][n_kv][keep] pool rows, then as many slots
-  int keys;  // of a row held in shared memory: all that the table can hold, or none
+  int keys;   // of a row held in shared memory: all that the table can hold, or none
+  int lists;  // whether the lists of slots are held there too
 };
 
 constexpr int EV_THREADS = 1024;
@@ -361,38 +377,22 @@ __device__ __forceinline__ uint32_t ev_key(float w, int pos, int first, int last
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// exclusive scan of one int per thread over the CTA
-__device__ __forceinline__ int ev_scan(int v, int* wsum, int* total) {
+// Sum over the warps before the caller's of one count a warp (the same in its lanes).  One barrier: every warp adds up
+// the counts by itself; `buf` is not used by the call before.
+__device__ __forceinline__ long long ev_before(long long n, long long* buf) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int inc = v;
+  if (lane == 0) buf[warp] = n;
+  __syncthreads();
+  long long v = lane < warp ? buf[lane] : 0;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int n = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += n;
-  }
-  __syncthreads();
-  if (lane == 31) wsum[warp] = inc;
-  __syncthreads();
-  if (warp == 0) {
-    const int w = wsum[lane];
-    int wi = w;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int n = __shfl_up_sync(0xffffffffu, wi, o);
-      if (lane >= o) wi += n;
-    }
-    wsum[lane] = wi - w;
-    if (lane == 31) wsum[32] = wi;
-  }
-  __syncthreads();
-  *total = wsum[32];
-  return wsum[warp] + inc - v;
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
 __global__ void __launch_bounds__(EV_THREADS) kv8_evict_select_kernel(const KV8EvictArgs a) {
   extern __shared__ uint32_t ev_keys[];
   __shared__ int hist[EV_BINS];
-  __shared__ int wsum[33];
+  __shared__ long long sums[2][EV_THREADS / 32];
   __shared__ int pick_bin, pick_above;
   const N730KV8Cache& c = a.c;
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
@@ -414,7 +414,10 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_select_kernel(const KV8E
   }
   const int seen = a.seen[b], last = seen - a.recent;
   const int lane = tid & 31, warp = tid >> 5;
+  for (int i = tid; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
+#pragma unroll 4
   for (int i = tid; i < min(L, a.keys); i += EV_THREADS) ev_keys[i] = ev_key(w_in[i], pos_in[i], a.first, last);
+  __syncthreads();
   auto key = [&](int i) { return a.keys ? ev_keys[i] : ev_key(w_in[i], pos_in[i], a.first, last); };
   // the keep-th largest key, 11 + 11 + 10 bits at a time
   uint32_t prefix = 0;
@@ -422,8 +425,6 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_select_kernel(const KV8E
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-    for (int i = tid; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
-    __syncthreads();
     for (int i = tid; i < L; i += EV_THREADS) {
       const uint32_t k = key(i);
       if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1);
@@ -431,27 +432,27 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_select_kernel(const KV8E
     __syncthreads();
     // bins from the top: thread t holds bins 2047 - 2t and 2046 - 2t
     const int hi = hist[EV_BINS - 1 - 2 * tid], lo = hist[EV_BINS - 2 - 2 * tid];
-    int total;
-    const int above = ev_scan(hi + lo, wsum, &total);
+    hist[EV_BINS - 1 - 2 * tid] = hist[EV_BINS - 2 - 2 * tid] = 0;  // for the next pass
+    int inc = hi + lo;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int n = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += n;
+    }
+    const int above = (int)ev_before(__shfl_sync(0xffffffffu, inc, 31), sums[pass & 1]) + inc - hi - lo;
     if (above < want && above + hi >= want) { pick_bin = EV_BINS - 1 - 2 * tid; pick_above = above; }
     else if (above + hi < want && above + hi + lo >= want) { pick_bin = EV_BINS - 2 - 2 * tid; pick_above = above + hi; }
     __syncthreads();
     prefix = (prefix << bits) | (uint32_t)pick_bin;
     want -= pick_above;
-    __syncthreads();
   }
   const uint32_t cut = prefix;  // slots above it stay, and the first `want` equal to it
   // each warp a run of slots, 32 at a time; counts(flag) is how many of the warps before have it
   const int run = ((L + EV_THREADS - 1) / EV_THREADS) * 32, i0 = min(L, warp * run), i1 = min(L, i0 + run);
   const uint32_t before = (1u << lane) - 1u;
-  auto counts = [&](int n) {
-    int total;
-    const int mine = ev_scan(lane == 0 ? n : 0, wsum, &total);
-    return __shfl_sync(0xffffffffu, mine, 0);
-  };
   int ties = 0;
   for (int i = i0; i < i1; i += 32) ties += __popc(__ballot_sync(0xffffffffu, i + lane < i1 && key(i + lane) == cut));
-  const int tie0 = counts(ties);
+  const int tie0 = (int)ev_before(ties, sums[1]);
   // stays(i): called for i = i0 + lane, + 32, ... with the ties so far in t
   auto stays = [&](int i, int& t) {
     const uint32_t k = i < i1 ? key(i) : 0u;
@@ -466,11 +467,12 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_select_kernel(const KV8E
     holes += __popc(__ballot_sync(0xffffffffu, i < i1 && !yes && i < a.keep));
     movers += __popc(__ballot_sync(0xffffffffu, yes && i >= a.keep));
   }
-  const int hole0 = counts(holes);
-  const int mover0 = counts(movers);
+  const long long ranks = ev_before(((long long)holes << 32) | (unsigned)movers, sums[0]);
+  const int hole0 = (int)(ranks >> 32), mover0 = (int)(ranks & 0xffffffff);
   // slots before the budget: their own, or (holes, listed by rank) a mover's
-  int* from = a.src + (int64_t)gridDim.y * c.n_kv * a.keep + head * a.keep;  // the slot that comes to a slot
-  int* list = src;                                                            // holes by rank, until the rows go there
+  // from: the slot that comes to a slot; list: the holes by rank (in global memory until the rows go there)
+  int* from = a.lists ? reinterpret_cast<int*>(ev_keys + a.keys) : a.src + (int64_t)gridDim.y * c.n_kv * a.keep + head * a.keep;
+  int* list = a.lists ? from + a.keep : src;
   t = tie0;
   int hr = hole0;
   for (int i = i0 + lane; i - lane < i1; i += 32) {
@@ -492,6 +494,7 @@ __global__ void __launch_bounds__(EV_THREADS) kv8_evict_select_kernel(const KV8E
   __syncthreads();
   // weights and positions; in and out may be the same arrays: sources are never slots written before
   const int* bt = c.block_table + (int64_t)b * c.max_pages;
+#pragma unroll 2
   for (int i = tid; i < a.keep; i += EV_THREADS) {
     const int s = from[i], page = bt[s / c.page_size];
     w_out[i] = w_in[s];
@@ -646,9 +649,11 @@ N730_API int n730_kv8_evict(const N730KV8Cache* c, int batch, int keep, int firs
   a.log_block = c->block == 16 ? 4 : c->block == 32 ? 5 : 6;
   const int cap = c->max_pages * c->page_size;
   a.keys = cap <= EV_KEYS ? cap : 0;
+  a.lists = (int64_t)a.keys + 2 * (int64_t)keep <= EV_KEYS;
+  const size_t smem = ((size_t)a.keys + (a.lists ? 2 * (size_t)keep : 0)) * 4;
   cudaStream_t st = (cudaStream_t)stream;
   if (int rc = smem_attr_once<kv8_evict_select_kernel>(EV_KEYS * 4)) return rc;
-  if (int rc = kv8_launch(kv8_evict_select_kernel, dim3(c->n_kv, batch), dim3(EV_THREADS), (size_t)a.keys * 4, st, false, a))
+  if (int rc = kv8_launch(kv8_evict_select_kernel, dim3(c->n_kv, batch), dim3(EV_THREADS), smem, st, false, a))
     return rc;
   const dim3 grid(keep / c->block, c->n_kv, batch);
   const int np = (c->block * (c->head_dim / 16) + KV8_THREADS - 1) / KV8_THREADS;
