@@ -265,6 +265,9 @@ typedef struct N730ModelConfig {
   int32_t kv_pool_pages; /* pages in the KV pool shared by the sequences (0: max_batch x pages per
                             sequence); a sequence takes pages as it grows and returns them when
                             released (n730_model_seq_release) */
+  int32_t kv_bits;       /* 0 or 16: fp16 cache.  8: int8 codes with an fp32 scale per 16 positions
+                            and KV head (n730_kv8_*): half the cache's bytes, decode with one kernel
+                            per op; page_size must be a multiple of 16 */
 } N730ModelConfig;
 
 /* weight slots (n730_model_set_qweight); EMBED/LMHEAD take layer = -1 */

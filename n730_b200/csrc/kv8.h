@@ -17,6 +17,13 @@ int kv8_check(const N730KV8Cache* c, int batch, const char* what);
 int kv8_append_launch(const N730KV8Cache& c, const void* k, const void* v, int dtype, int64_t ld, int batch,
                       int tokens, const int* lens, const int* n_new, bool pdl, cudaStream_t st);
 
+// RoPE of q and k (rotate_half, in place) in rows [heads | n_kv | ...] of fp32 qkv; row r is at position
+// *pos + r (one sequence) or pos[r] (a row per sequence).  q16 (may be null): q rounded to fp16 instead.
+int kv8_rope_launch(float* qkv, int64_t ld, int rows, int heads, int n_kv, int head_dim, const float* cos_t,
+                    const float* sin_t, const int* pos, bool per_row, __half* q16, bool pdl, cudaStream_t st);
+// fp16 -> fp32
+int kv8_widen_launch(const __half* x, float* y, int64_t n, bool pdl, cudaStream_t st);
+
 struct KV8AttnCall {
   N730KV8Cache c;
   const void* q; void* out;
@@ -31,6 +38,7 @@ struct KV8AttnCall {
   bool pdl;
 };
 int64_t kv8_attention_ws(const N730KV8Cache& c, int batch, int tokens, int heads, bool weights);
+int64_t kv8_attention_ws_upto(const N730KV8Cache& c, int batch, int tokens, int heads);
 int kv8_attention_launch(const KV8AttnCall& a, cudaStream_t st);
 
 // The tensor-memory kernel for prompts (kv8_prompt.cu): 256 rows of an item a CTA, the positions in

@@ -900,6 +900,13 @@ static int kv8_map(const N730KV8Cache& c, const void* codes, int box, CUtensorMa
   return N730_OK;
 }
 
+// of every call of up to `tokens` tokens: the need does not grow with them (other kernels, other shares)
+int64_t kv8_attention_ws_upto(const N730KV8Cache& c, int batch, int tokens, int heads) {
+  int64_t most = 0;
+  for (int t = 1; t <= tokens; ++t) most = std::max(most, kv8_attention_ws(c, batch, t, heads, false));
+  return most;
+}
+
 template <int HD, int CODE, int NB, bool LO>
 static int split_launch(const KDArgs& a, const CUtensorMap& km, const CUtensorMap& vm, bool pdl, cudaStream_t st) {
   const size_t fixed = sizeof(KDSmem<HD>) + 1024;
@@ -931,6 +938,8 @@ int kv8_attention_launch(const KV8AttnCall& k, cudaStream_t st) {
   const N730KV8Cache& c = k.c;
   const bool weights = k.w_out != nullptr;
   const KDPlan p = kd_plan(c, k.batch, k.tokens, k.heads, k.dtype, weights);
+  N730_REQUIRE(k.ws_bytes >= p.bytes, N730_BAD_ARG, "kv8_attention: workspace of %lld bytes, %lld needed",
+               (long long)k.ws_bytes, (long long)p.bytes);
   uint8_t* ws = reinterpret_cast<uint8_t*>(k.ws);
   KDArgs a{};
   a.c = c;

@@ -571,6 +571,48 @@ __global__ void __launch_bounds__(KV8_THREADS) kv8_evict_move_kernel(const KV8Ev
   }
 }
 
+// ---------------------------------------------------------------------------
+// the model's own steps around the cache
+// ---------------------------------------------------------------------------
+__global__ void kv8_rope_kernel(float* qkv, int64_t ld, int heads, int n_kv, int head_dim, const float* cos_t,
+                                const float* sin_t, const int* pos, int per_row, __half* q16) {
+  pdl_wait();
+  const int r = blockIdx.x, h2 = head_dim / 2;
+  const int p = per_row ? pos[r] : pos[0] + r;
+  float* row = qkv + (int64_t)r * ld;
+  const float* cs = cos_t + (int64_t)p * h2;
+  const float* sn = sin_t + (int64_t)p * h2;
+  for (int i = threadIdx.x; i < (heads + n_kv) * h2; i += blockDim.x) {
+    const int h = i / h2, j = i % h2;
+    float* x = row + (int64_t)h * head_dim;
+    const float x0 = x[j], x1 = x[j + h2], y0 = x0 * cs[j] - x1 * sn[j], y1 = x1 * cs[j] + x0 * sn[j];
+    if (q16 && h < heads) {
+      __half* q = q16 + ((int64_t)r * heads + h) * head_dim;
+      q[j] = __float2half_rn(y0);
+      q[j + h2] = __float2half_rn(y1);
+    } else {
+      x[j] = y0;
+      x[j + h2] = y1;
+    }
+  }
+}
+
+int kv8_rope_launch(float* qkv, int64_t ld, int rows, int heads, int n_kv, int head_dim, const float* cos_t,
+                    const float* sin_t, const int* pos, bool per_row, __half* q16, bool pdl, cudaStream_t st) {
+  return kv8_launch(kv8_rope_kernel, dim3(rows), dim3(256), 0, st, pdl, qkv, ld, heads, n_kv, head_dim, cos_t, sin_t, pos,
+                    (int)per_row, q16);
+}
+
+__global__ void kv8_widen_kernel(const __half* x, float* y, int64_t n) {
+  pdl_wait();
+  const int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 2;  // n is even: rows of head_dim
+  if (i < n) *reinterpret_cast<float2*>(y + i) = __half22float2(*reinterpret_cast<const __half2*>(x + i));
+}
+
+int kv8_widen_launch(const __half* x, float* y, int64_t n, bool pdl, cudaStream_t st) {
+  return kv8_launch(kv8_widen_kernel, dim3((unsigned)((n / 2 + 255) / 256)), dim3(256), 0, st, pdl, x, y, n);
+}
+
 }  // namespace n730
 
 using namespace n730;

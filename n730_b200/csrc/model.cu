@@ -23,6 +23,7 @@
 
 #include "attention.h"
 #include "decode_persist.h"
+#include "kv8.h"
 #include "tp_allreduce.h"
 #include "n730_cuda.h"
 #include "qweight.h"
@@ -57,6 +58,8 @@ __global__ void advance_seq_kernel(int* seq_lens, int batch, int by) {
   if (b < batch) seq_lens[b] += by;
 }
 
+constexpr int KV8_MODEL_BLOCK = 16;  // positions that share a scale in the model's 8-bit cache
+
 struct Layer {
   QWeight* qkv = nullptr;
   QWeight* o = nullptr;
@@ -69,6 +72,7 @@ struct Layer {
   float* gate_up_bias = nullptr;
   float* down_bias = nullptr;
   KVLayer kv{};
+  N730KV8Cache kv8{};  // kv_bits 8: the layer's 8-bit cache (block table of sequence 0)
 };
 
 struct Model {
@@ -84,6 +88,11 @@ struct Model {
   std::vector<void*> allocs;
   float *cos_t = nullptr, *sin_t = nullptr;
   __half *k_pool = nullptr, *v_pool = nullptr;
+  // 8-bit cache (kv_bits 8): attention workspace, prefill's first position, fp16 queries and outputs
+  uint8_t* kv8_ws = nullptr;
+  int64_t kv8_ws_bytes = 0;
+  int* kv8_pos0 = nullptr;
+  __half *kv8_q = nullptr, *kv8_out = nullptr;
   int* block_table = nullptr;
   int* seq_lens = nullptr;
   std::vector<int> h_seq;
@@ -659,11 +668,29 @@ static int finalize(Model* m) {
   const size_t pages = c.kv_pool_pages > 0 ? std::min(table, (size_t)c.kv_pool_pages) : table;
   m->pool_pages = (int)pages;
   const size_t per_layer = pages * c.kv_heads * c.page_size * c.head_dim;
-  if (int rc = m->alloc(&m->k_pool, per_layer * nl)) return rc;
-  if (int rc = m->alloc(&m->v_pool, per_layer * nl)) return rc;
-  N730_CUDA(cudaMemsetAsync(m->k_pool, 0, per_layer * nl * sizeof(__half), m->st));
-  N730_CUDA(cudaMemsetAsync(m->v_pool, 0, per_layer * nl * sizeof(__half), m->st));
-  for (int l = 0; l < nl; ++l) m->L[l].kv = KVLayer{m->k_pool + per_layer * l, m->v_pool + per_layer * l};
+  if (c.kv_bits == 8) {
+    // a layer: codes of K and V, then their scales
+    const size_t scales = per_layer / c.head_dim / KV8_MODEL_BLOCK, layer_bytes = 2 * (per_layer + scales * sizeof(float));
+    uint8_t* pool = nullptr;
+    if (int rc = m->alloc(&pool, layer_bytes * nl)) return rc;
+    N730_CUDA(cudaMemsetAsync(pool, 0, layer_bytes * nl, m->st));
+    for (int l = 0; l < nl; ++l) {
+      N730KV8Cache& k = m->L[l].kv8;
+      uint8_t* at = pool + layer_bytes * l;
+      k.k_codes = at;
+      k.v_codes = at + per_layer;
+      k.k_scales = reinterpret_cast<float*>(at + 2 * per_layer);
+      k.v_scales = k.k_scales + scales;
+      k.n_pages = (int)pages; k.max_pages = m->max_pages; k.n_kv = c.kv_heads; k.head_dim = c.head_dim;
+      k.page_size = c.page_size; k.block = KV8_MODEL_BLOCK; k.code = N730_KV8_INT8;
+    }
+  } else {
+    if (int rc = m->alloc(&m->k_pool, per_layer * nl)) return rc;
+    if (int rc = m->alloc(&m->v_pool, per_layer * nl)) return rc;
+    N730_CUDA(cudaMemsetAsync(m->k_pool, 0, per_layer * nl * sizeof(__half), m->st));
+    N730_CUDA(cudaMemsetAsync(m->v_pool, 0, per_layer * nl * sizeof(__half), m->st));
+    for (int l = 0; l < nl; ++l) m->L[l].kv = KVLayer{m->k_pool + per_layer * l, m->v_pool + per_layer * l};
+  }
   {
     // unassigned entries point at page 0 (in bounds); kernels read entries below a sequence's length only
     m->h_bt.assign(table, 0);
@@ -672,6 +699,19 @@ static int finalize(Model* m) {
     m->free_pages.resize(pages);
     for (size_t i = 0; i < pages; ++i) m->free_pages[i] = (int)(pages - 1 - i);  // page 0 handed out first
     m->seq_pages.assign(c.max_batch, {});
+  }
+  if (c.kv_bits == 8) {
+    for (int l = 0; l < nl; ++l) {
+      m->L[l].kv8.block_table = m->block_table;
+      if (int rc = kv8_check(&m->L[l].kv8, c.max_batch, "model: 8-bit cache")) return rc;
+    }
+    m->kv8_ws_bytes = std::max(kv8_attention_ws(m->L[0].kv8, c.max_batch, 1, c.heads, false),
+                               kv8_attention_ws_upto(m->L[0].kv8, 1, c.max_prefill, c.heads));
+    if (int rc = m->alloc(&m->kv8_ws, (size_t)m->kv8_ws_bytes)) return rc;
+    N730_CUDA(cudaMemsetAsync(m->kv8_ws, 0, (size_t)m->kv8_ws_bytes, m->st));
+    if (int rc = m->alloc(&m->kv8_pos0, 1)) return rc;
+    if (int rc = m->alloc(&m->kv8_q, (size_t)c.max_prefill * c.heads * c.head_dim)) return rc;
+    if (int rc = m->alloc(&m->kv8_out, (size_t)c.max_prefill * c.heads * c.head_dim)) return rc;
   }
   if (int rc = m->alloc(&m->seq_lens, c.max_batch)) return rc;
   N730_CUDA(cudaMemsetAsync(m->seq_lens, 0, c.max_batch * 4, m->st));
@@ -706,7 +746,7 @@ static int finalize(Model* m) {
   if (int rc = m->alloc(&m->pmlp, (size_t)P * c.ffn)) return rc;
   N730_CUDA(cudaMallocHost(&m->h_tok, (size_t)std::max(B, P) * 4));
   N730_CUDA(cudaMallocHost(&m->h_logits, (size_t)B * c.vocab * 4));
-  if (c.per_op_decode <= 0)
+  if (c.per_op_decode <= 0 && c.kv_bits != 8)  // the persistent kernel reads fp16 pages
     if (int rc = plan_persistent(m)) return rc;
   if (c.tp_size > 1)
     if (int rc = agree_decode_path(m)) return rc;
@@ -830,6 +870,39 @@ static AttnDims dims(const Model* m) {
   return d;
 }
 
+__global__ void set_int_kernel(int* p, int v) { *p = v; }
+
+// Attention of `rows` new rows of qkv (RoPE'd here) over an 8-bit layer cache that takes their K and V:
+// a row of each of `batch` sequences (tokens 1), or the `tokens` next ones of one (table, lens: its own).
+static int kv8_attend(Model* m, const Layer& y, const int* table, const int* lens, float* qkv, int batch, int tokens,
+                      float* out) {
+  const N730ModelConfig& c = m->c;
+  const int ad = c.heads * c.head_dim, rows = batch * tokens;
+  const bool f16 = tokens > 1;  // prompts: fp16 queries and outputs, which o_proj's GEMM rounds to anyway
+  N730KV8Cache kv = y.kv8;
+  kv.block_table = table;
+  if (int rc = kv8_rope_launch(qkv, m->qkv_dim, rows, c.heads, c.kv_heads, c.head_dim, m->cos_t, m->sin_t, lens, batch > 1,
+                               f16 ? m->kv8_q : nullptr, c.use_pdl, m->st))
+    return rc;
+  if (int rc = kv8_append_launch(kv, qkv + ad, qkv + ad + c.kv_heads * c.head_dim, N730_F32, m->qkv_dim, batch, tokens, lens,
+                                 nullptr, c.use_pdl, m->st))
+    return rc;
+  KV8AttnCall k{};
+  k.c = kv;
+  k.q = f16 ? (const void*)m->kv8_q : qkv;
+  k.out = f16 ? (void*)m->kv8_out : out;
+  k.dtype = f16 ? N730_F16 : N730_F32;
+  k.ldq = f16 ? ad : m->qkv_dim;
+  k.ldo = ad;
+  k.batch = batch; k.tokens = tokens; k.heads = c.heads;
+  k.scale = 1.0f / sqrtf((float)c.head_dim);
+  k.lens = lens;
+  k.ws = m->kv8_ws; k.ws_bytes = m->kv8_ws_bytes;
+  k.pdl = c.use_pdl;
+  if (int rc = kv8_attention_launch(k, m->st)) return rc;
+  return f16 ? kv8_widen_launch(m->kv8_out, out, (int64_t)rows * ad, c.use_pdl, m->st) : N730_OK;
+}
+
 // Enqueue one decode step for sequences [0, B) on m->st (tokens in m->d_tokens).
 static int enqueue_decode(Model* m, int B) {
   const N730ModelConfig& c = m->c;
@@ -849,11 +922,15 @@ static int enqueue_decode(Model* m, int B) {
     LayerW lw;
     if (int rc = stream_acquire(m, l, &lw)) return rc;
     if (int rc = gemv(m, lw.qkv, m->x, h, B, m->qkv, m->qkv_dim, y.qkv_bias, nullptr, 0, y.ln1, 0)) return rc;
-    DecodeAttnArgs a = {};
-    a.qkv = m->qkv; a.ld_qkv = m->qkv_dim; a.cos_t = m->cos_t; a.sin_t = m->sin_t;
-    a.seq_lens = m->seq_lens; a.block_table = m->block_table; a.kv = y.kv; a.d = dims(m);
-    a.out = m->attn; a.batch = B; a.pdl = c.use_pdl;
-    if (int rc = attn_decode_launch(a, m->st)) return rc;
+    if (c.kv_bits == 8) {
+      if (int rc = kv8_attend(m, y, m->block_table, m->seq_lens, m->qkv, B, 1, m->attn)) return rc;
+    } else {
+      DecodeAttnArgs a = {};
+      a.qkv = m->qkv; a.ld_qkv = m->qkv_dim; a.cos_t = m->cos_t; a.sin_t = m->sin_t;
+      a.seq_lens = m->seq_lens; a.block_table = m->block_table; a.kv = y.kv; a.d = dims(m);
+      a.out = m->attn; a.batch = B; a.pdl = c.use_pdl;
+      if (int rc = attn_decode_launch(a, m->st)) return rc;
+    }
     if (int rc = rowsplit_linear(m, lw.o, m->attn, ad, B, m->x, h, y.o_bias)) return rc;
     if (int rc = gemv(m, lw.gate_up, m->x, h, B, m->mlp, c.ffn, y.gate_up_bias, nullptr, 0, y.ln2, 1)) return rc;
     if (int rc = rowsplit_linear(m, lw.down, m->mlp, c.ffn, B, m->x, h, y.down_bias)) return rc;
@@ -930,6 +1007,10 @@ static int prefill(Model* m, int seq, const int32_t* d_tok, int T, float* d_logi
     const int n = std::min(c.max_prefill, T - done);
     const int pos0 = m->h_seq[seq] + done;
     m->ss_of = nullptr;  // px is rewritten by the embedding
+    if (c.kv_bits == 8) {
+      set_int_kernel<<<1, 1, 0, m->st>>>(m->kv8_pos0, pos0);
+      N730_CHECK_LAUNCH();
+    }
     if (int rc = embed_launch(*m->embed, d_tok + done, n, m->px, m->st)) return rc;
     if (int rc = stream_begin(m)) return rc;
     for (int l = 0; l < c.layers; ++l) {
@@ -937,6 +1018,10 @@ static int prefill(Model* m, int seq, const int32_t* d_tok, int T, float* d_logi
       LayerW lw;
       if (int rc = stream_acquire(m, l, &lw)) return rc;
       if (int rc = gemv(m, lw.qkv, m->px, h, n, m->pqkv, m->qkv_dim, y.qkv_bias, nullptr, 0, y.ln1, 0)) return rc;
+      if (c.kv_bits == 8) {
+        if (int rc = kv8_attend(m, y, m->block_table + (size_t)seq * m->max_pages, m->kv8_pos0, m->pqkv, 1, n, m->pattn))
+          return rc;
+      } else {
       KVWriteArgs kw = {};
       kw.qkv = m->pqkv; kw.ld_qkv = m->qkv_dim; kw.cos_t = m->cos_t; kw.sin_t = m->sin_t;
       kw.block_table = m->block_table + (size_t)seq * m->max_pages; kw.kv = y.kv; kw.d = dims(m);
@@ -946,6 +1031,7 @@ static int prefill(Model* m, int seq, const int32_t* d_tok, int T, float* d_logi
       pa.qkv = m->pqkv; pa.ld_qkv = m->qkv_dim; pa.block_table = kw.block_table; pa.kv = y.kv; pa.d = dims(m);
       pa.T = n; pa.pos0 = pos0; pa.out = m->pattn; pa.pdl = c.use_pdl;
       if (int rc = attn_prefill_launch(pa, m->st)) return rc;
+      }
       if (int rc = rowsplit_linear(m, lw.o, m->pattn, ad, n, m->px, h, y.o_bias)) return rc;
       if (int rc = gemv(m, lw.gate_up, m->px, h, n, m->pmlp, c.ffn, y.gate_up_bias, nullptr, 0, y.ln2, 1)) return rc;
       if (int rc = rowsplit_linear(m, lw.down, m->pmlp, c.ffn, n, m->px, h, y.down_bias)) return rc;
@@ -974,6 +1060,8 @@ N730_API int n730_model_create(const N730ModelConfig* cfg, void** out) {
   N730_REQUIRE(c.head_dim == 64 || c.head_dim == 128, N730_UNSUPPORTED, "model_create: head_dim %d", c.head_dim);
   N730_REQUIRE(c.stream_depth >= 0 && c.stream_depth <= 16, N730_BAD_ARG, "model_create: stream_depth %d",
                c.stream_depth);
+  N730_REQUIRE(c.kv_bits == 0 || c.kv_bits == 16 || (c.kv_bits == 8 && (c.page_size <= 0 || c.page_size % KV8_MODEL_BLOCK == 0)),
+               N730_BAD_ARG, "model_create: kv_bits %d with pages of %d positions", c.kv_bits, c.page_size);
   Model* m = new Model();
   m->c = c;
   if (m->c.page_size <= 0) m->c.page_size = 64;
@@ -1432,6 +1520,8 @@ N730_API int n730_model_info(void* p, int64_t* info) {
   for (auto& y : m->L) wb += bytes(y.qkv) + bytes(y.o) + bytes(y.gate_up) + bytes(y.down);
   info[0] = wb;
   info[1] = (int64_t)m->c.layers * 2 * m->c.kv_heads * m->c.head_dim * 2;
+  if (m->c.kv_bits == 8)  // codes, and a scale per KV8_MODEL_BLOCK positions
+    info[1] = (int64_t)m->c.layers * 2 * m->c.kv_heads * (m->c.head_dim * KV8_MODEL_BLOCK + 4) / KV8_MODEL_BLOCK;
   info[2] = info[1] * (int64_t)m->pool_pages * m->c.page_size;
   info[3] = m->n_split;
   info[4] = m->qkv_dim;

@@ -33,7 +33,7 @@ class N730ModelConfig(C.Structure):
                [(n, C.c_int32) for n in ("max_ctx", "max_batch", "page_size", "max_prefill", "tie_embeddings",
                                          "tp_rank", "tp_size", "use_graphs", "use_pdl", "exact_gemv",
                                          "per_op_decode", "stream_depth", "ffn_fuse", "tp_allreduce",
-                                         "kv_pool_pages")]
+                                         "kv_pool_pages", "kv_bits")]
 
 
 def _sigs(lib):
@@ -172,14 +172,15 @@ class Engine:
     def __init__(self, shape: ModelShape, max_ctx: int = 4096, max_batch: int = 1, page_size: int = 64,
                  max_prefill: int = 512, use_graphs: bool = True, use_pdl: bool = True,
                  tp_rank: int = 0, tp_size: int = 1, exact_gemv: bool = False, per_op_decode: int = 0,
-                 stream_depth: int = 0, ffn_fuse: int = 0, tp_allreduce: int = 1, kv_pool_pages: int = 0):
+                 stream_depth: int = 0, ffn_fuse: int = 0, tp_allreduce: int = 1, kv_pool_pages: int = 0,
+                 kv_bits: int = 16):
         self.lib = _sigs(_lib.cuda())
         self.shape = shape
         c = N730ModelConfig(shape.hidden, shape.layers, shape.heads, shape.kv_heads, shape.head_dim, shape.ffn,
                             shape.vocab, shape.rms_eps, shape.rope_theta, max_ctx, max_batch, page_size,
                             max_prefill, int(shape.tie_embeddings), tp_rank, tp_size, int(use_graphs),
                             int(use_pdl), int(exact_gemv), int(per_op_decode), int(stream_depth), int(ffn_fuse),
-                            int(tp_allreduce), int(kv_pool_pages))
+                            int(tp_allreduce), int(kv_pool_pages), int(kv_bits))
         self.cfg = c
         self.h = C.c_void_p()
         _lib.check(self.lib.n730_model_create(C.byref(c), C.byref(self.h)), "model_create")
@@ -265,7 +266,8 @@ class Engine:
         return tuple(getattr(c, f) for f in ("hidden", "layers", "heads", "kv_heads", "head_dim", "vocab",
                                               "max_ctx", "max_batch", "page_size", "max_prefill",
                                               "tie_embeddings", "tp_size", "use_graphs", "use_pdl",
-                                              "exact_gemv", "per_op_decode", "ffn_fuse", "tp_allreduce")) + \
+                                              "exact_gemv", "per_op_decode", "ffn_fuse", "tp_allreduce",
+                                              "kv_bits")) + \
             (round(float(c.rms_eps), 12), float(c.rope_theta))
 
     @staticmethod
