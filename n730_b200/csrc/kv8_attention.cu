@@ -9,7 +9,7 @@
 // joins an item's parts in run order, with as many CTAs as there are items.  Within a
 // CTA each warp takes every fourth tile.  An item counts for KD_ITEM_COST tiles more than it has, the
 // time that starting and ending one takes: without that the CTAs that meet many short sequences were
-// the last to finish (batch of 128 ragged lengths: see KD_ITEM_COST).  The next run's first tile is
+// the last to finish.  The next run's first tile is
 // asked for before this one's outputs are joined.
 //
 // The products are transposed, so that a key or a channel is a row of mma.m16n8k16's A and the few
@@ -48,7 +48,10 @@ constexpr int KD_THREADS = KD_WARPS * 32;
 constexpr int KD_STAGES = 2;     // tile buffers of a warp
 constexpr int KD_TILE = 32;      // positions
 constexpr int KD_CTAS_PER_SM = 3;
-constexpr int KD_ITEM_COST = 6;  // tiles
+// What starting and ending an item counts for on the line, in tiles.  Batch of 128 ragged sequences up to 4096 (72B
+// heads): 3 131.8 us, 6 124.9, 10 120.5, 16 116.1, 24 117.1, 40 121.1; batch of 32 with weights 55.6, 53.9, 53.4,
+// 52.7, 53.2, 54.7.
+constexpr int KD_ITEM_COST = 16;
 constexpr int KD_MIN_UNITS = 4;  // tiles of a run: fewer would leave warps idle and joins to do
 constexpr int KD_MAX_BATCH = 4096;
 constexpr float KD_SLACK = 8.f;  // log2 of how far a weight may exceed its reference
