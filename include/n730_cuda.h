@@ -171,10 +171,12 @@ int n730_quantize_grouped(const float* d_w, int rows, int cols, int bits, int gr
  * no page: rows for it are dropped, reads of it give zeros, attention does not see its positions.
  * All pointers are device memory of the current device and belong to the caller; code pools are
  * 16-byte aligned, head_dim is 64 or 128.  Pages may be shared between sequences as long as no
- * call writes them (append, evict).  The calls are asynchronous on `stream`, allocate nothing and
- * can be captured into a graph.  Lengths and counts are read on the device (below 0 counts as 0,
- * above the table's max_pages * page_size positions as that).  `dtype` is the type of the caller's
- * rows; row strides are in elements, token t of sequence b is row b * tokens + t. */
+ * call writes them (append, evict).  Scales are not negative; V scales below 2^-100 count as 0 in
+ * attention.  The calls are asynchronous on `stream`, allocate nothing and can be captured into a
+ * graph; calls that may overlap in time need a workspace each.  Lengths and counts are read on the
+ * device (below 0 counts as 0, above the table's max_pages * page_size positions as that).  `dtype` is
+ * the type of the caller's rows; row strides are in elements, token t of sequence b is row
+ * b * tokens + t. */
 enum { N730_KV8_INT8 = 0, N730_KV8_E4M3 = 1 };
 enum { N730_F32 = 0, N730_F16 = 1, N730_BF16 = 2 };
 typedef struct N730KV8Cache {
@@ -197,15 +199,17 @@ int n730_kv8_append(const N730KV8Cache* c, const void* d_k, const void* d_v, int
  * [n_kv][head_dim] of d_k and d_v; positions outside [0, d_lens[b]) give zeros. */
 int n730_kv8_read(const N730KV8Cache* c, void* d_k, void* d_v, int dtype, int64_t ld, int batch, int tokens,
                   const int32_t* d_first, const int32_t* d_lens, void* stream);
-/* Bytes of workspace of n730_kv8_attention (negative: a return code).  Zero the workspace once;
- * each call leaves it ready for the next.  Calls that may overlap in time need one each. */
+/* Bytes of workspace (16-byte aligned) of an n730_kv8_attention call of this size (negative: a return
+ * code).  Zero it once: its first int32 becomes 1 if a device wait ever runs out (the call's outputs
+ * are not valid then), the rest does not matter from call to call. */
 int64_t n730_kv8_attention_ws(const N730KV8Cache* c, int batch, int tokens, int n_heads, int weights);
 /* Attention of the `tokens` newest rows of each sequence (d_new[b] of them) over its cached
  * positions: query t of sequence b, RoPE applied, sees positions [0, d_lens[b] + t] - call it after
  * n730_kv8_append with the same d_lens and d_new.  d_q and d_out rows are [n_heads][head_dim]
  * (query head i reads KV head i / (n_heads / n_kv)); out rows from d_new[b] on are left as they
- * were; a query that sees no position gives zeros.  Scores are scaled by `scale`.  fp32 rows keep
- * fp32 accuracy; 16-bit rows round the softmax weights to fp16.
+ * were; a query that sees no position gives zeros.  Scores are scaled by `scale`.  16-bit rows round
+ * the softmax weights to fp16, and more than 64 rows of a KV head run on the tcgen05 tensor cores;
+ * fp32 rows keep fp32 accuracy and run 64 rows of a KV head at a time.
  * d_w_out (may be null) [batch][n_kv][ldw]: for positions below d_lens[b] + d_new[b], d_w (null:
  * zeros; may equal d_w_out) plus the softmax weights summed over the KV head's queries; positions
  * that are new count from zero.  ldw >= max_pages * page_size. */

@@ -64,6 +64,11 @@ __device__ __forceinline__ void kv8_store1(void* p, int64_t i, int dtype, float 
   else if (dtype == N730_F16) reinterpret_cast<__half*>(p)[i] = __float2half_rn(x);
   else reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
 }
+// V scales below this count as 0: quotients by them would leave fp32's range
+constexpr float KV8_TINY = 0x1p-100f;
+// whether pointers lie on whole elements of `size` bytes (null ones do)
+template <class... P>
+inline bool kv8_aligned(int size, const P*... p) { return ((0 | ... | reinterpret_cast<uintptr_t>(p)) & (uintptr_t)(size - 1)) == 0; }
 inline int kv8_esize(int dtype) { return dtype == N730_F32 ? 4 : 2; }
 
 // cached positions of a sequence before a call's new rows, within the table's capacity

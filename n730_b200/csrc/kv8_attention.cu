@@ -433,6 +433,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
         p0[tt] = (ta + warp + qi * KD_WARPS) * KD_TILE + half * 16;
         const float ksc = seen ? sm.sc[warp][st][2 * half] : 0.f;
         vsc[tt] = seen ? sm.sc[warp][st][2 * half + 1] : 0.f;
+        if (vsc[tt] < KV8_TINY) vsc[tt] = 0.f;
         lv[tt] = lg2(vsc[tt]);
         const uint8_t* kt = sm.ring[warp][st] + half * 16 * HD;
         float s[G::KCH][NB][4];
@@ -860,6 +861,11 @@ static int kv8_attention_check(const N730KV8Cache* c, int batch, int tokens, int
   N730_REQUIRE(tokens >= 1 && tokens <= (1 << 20), N730_BAD_ARG, "kv8_attention: tokens %d", tokens);
   N730_REQUIRE(heads >= 1 && heads <= 65535 && heads % c->n_kv == 0, N730_BAD_ARG,
                "kv8_attention: %d heads over %d KV heads", heads, c->n_kv);
+  // a token's queries of a KV head keep their sums in the finishing kernel's shared memory
+  N730_REQUIRE(heads / c->n_kv <= 8192, N730_BAD_ARG, "kv8_attention: %d heads over %d KV heads", heads, c->n_kv);
+  // the sequences' tiles are counted in 32 bits on the device
+  N730_REQUIRE((int64_t)batch * ((int64_t)c->max_pages * c->page_size / KD_TILE + 1 + KD_ITEM_COST) < (1ll << 31), N730_BAD_ARG,
+               "kv8_attention: %d sequences of up to %d pages", batch, c->max_pages);
   N730_REQUIRE((int64_t)tokens * (heads / c->n_kv) <= (1 << 23), N730_BAD_ARG,
                "kv8_attention: %d tokens of %d heads over %d KV heads", tokens, heads, c->n_kv);
   return N730_OK;
@@ -1001,6 +1007,8 @@ N730_API int n730_kv8_attention(const N730KV8Cache* c, const void* d_q, int dtyp
   if (int rc = kv8_attention_check(c, batch, tokens, n_heads)) return rc;
   N730_REQUIRE(dtype == N730_F32 || dtype == N730_F16 || dtype == N730_BF16, N730_BAD_ARG, "kv8_attention: dtype %d", dtype);
   N730_REQUIRE(d_q && d_out && d_lens && d_ws, N730_NULL, "kv8_attention: null pointer");
+  N730_REQUIRE(kv8_aligned(kv8_esize(dtype), (const char*)d_q, (const char*)d_out) && kv8_aligned(4, d_lens, d_new) &&
+                   kv8_aligned(4, d_w, d_w_out), N730_BAD_ARG, "kv8_attention: pointers must lie on whole elements");
   const int64_t row = (int64_t)n_heads * c->head_dim;
   N730_REQUIRE(ldq >= row && ldo >= row, N730_BAD_ARG, "kv8_attention: row strides %lld, %lld < %d heads x %d",
                (long long)ldq, (long long)ldo, n_heads, c->head_dim);

@@ -36,6 +36,8 @@ int kv8_check(const N730KV8Cache* c, int batch, const char* what) {
                "%s: a sequence's pages hold more than 2^30 positions", what);
   N730_REQUIRE((((uintptr_t)c->k_codes | (uintptr_t)c->v_codes) & 15) == 0, N730_BAD_ARG,
                "%s: code pools must be 16-byte aligned", what);
+  N730_REQUIRE(kv8_aligned(4, c->k_scales, c->v_scales, c->block_table), N730_BAD_ARG,
+               "%s: scales and block table must lie on whole elements", what);
   N730_REQUIRE(batch >= 1 && batch <= 65535, N730_BAD_ARG, "%s: batch %d", what, batch);
   return N730_OK;
 }
@@ -622,6 +624,8 @@ N730_API int n730_kv8_append(const N730KV8Cache* c, const void* d_k, const void*
   if (int rc = kv8_check(c, batch, "kv8_append")) return rc;
   if (int rc = kv8_check_dtype(dtype, "kv8_append")) return rc;
   N730_REQUIRE(d_k && d_v && d_lens, N730_NULL, "kv8_append: null pointer");
+  N730_REQUIRE(kv8_aligned(kv8_esize(dtype), d_k, d_v) && kv8_aligned(4, d_lens, d_new), N730_BAD_ARG,
+               "kv8_append: pointers must lie on whole elements");
   N730_REQUIRE(tokens >= 1 && tokens <= (1 << 24), N730_BAD_ARG, "kv8_append: tokens %d", tokens);
   N730_REQUIRE(ld >= (int64_t)c->n_kv * c->head_dim, N730_BAD_ARG, "kv8_append: row stride %lld < %d heads x %d",
                (long long)ld, c->n_kv, c->head_dim);
@@ -633,6 +637,8 @@ N730_API int n730_kv8_read(const N730KV8Cache* c, void* d_k, void* d_v, int dtyp
   if (int rc = kv8_check(c, batch, "kv8_read")) return rc;
   if (int rc = kv8_check_dtype(dtype, "kv8_read")) return rc;
   N730_REQUIRE(d_k && d_v && d_lens, N730_NULL, "kv8_read: null pointer");
+  N730_REQUIRE(kv8_aligned(kv8_esize(dtype), d_k, d_v) && kv8_aligned(4, d_lens, d_first), N730_BAD_ARG,
+               "kv8_read: pointers must lie on whole elements");
   N730_REQUIRE(tokens >= 1 && tokens <= (1 << 30), N730_BAD_ARG, "kv8_read: tokens %d", tokens);
   N730_REQUIRE(c->n_kv <= 32767, N730_BAD_ARG, "kv8_read: n_kv %d", c->n_kv);
   N730_REQUIRE(ld >= (int64_t)c->n_kv * c->head_dim, N730_BAD_ARG, "kv8_read: row stride %lld < %d heads x %d",
@@ -675,6 +681,8 @@ N730_API int n730_kv8_evict(const N730KV8Cache* c, int batch, int keep, int firs
   if (int rc = evict_check(c, batch, keep)) return rc;
   N730_REQUIRE(d_seen && d_lens && d_lens_out && d_w && d_w_out && d_pos && d_pos_out && d_ws, N730_NULL,
                "kv8_evict: null pointer");
+  N730_REQUIRE(kv8_aligned(4, d_seen, d_lens, d_lens_out) && kv8_aligned(4, d_w, d_w_out, d_pos, d_pos_out), N730_BAD_ARG,
+               "kv8_evict: pointers must lie on whole elements");
   N730_REQUIRE(first >= 0 && recent >= 0 && (int64_t)first + recent <= keep, N730_BAD_ARG,
                "kv8_evict: first %d + recent %d exceed keep %d", first, recent, keep);
   N730_REQUIRE(ldw >= (int64_t)c->max_pages * c->page_size, N730_BAD_ARG,

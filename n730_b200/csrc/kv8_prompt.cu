@@ -470,7 +470,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
     };
     auto load_scale = [&](const int (&row)[MINE]) {
       const int r = lane_row(row);
-      return r >= 0 ? ((lane & 1) ? c.v_scales : c.k_scales)[r >> a.log_block] : -1.f;
+      const float s = r >= 0 ? ((lane & 1) ? c.v_scales : c.k_scales)[r >> a.log_block] : -1.f;
+      return (lane & 1) && s < KV8_TINY ? 0.f : s;
     };
     const int at0 = lrow * 128 + (chunk >> 2) * Cfg::KB;
     auto store = [&](uint8_t* dst, int j, const int (&row)[MINE]) {

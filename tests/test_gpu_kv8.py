@@ -239,6 +239,74 @@ def test_several_tokens(code, dtype, kv, heads, dim, T, lens, new):
     check_attention(d, q, dtype, np.array(lens), None if new is None else np.array(new))
 
 
+@pytest.mark.parametrize("code,dtype,kv,heads,dim,page,T,lens,new", [
+    ("int8", "f16", 2, 8, 128, 64, 300, [1700, 0], None),                   # positions in shares
+    ("e4m3", "bf16", 1, 14, 64, 48, 40, [2900, 700, 0], [40, 3, 0]),        # pages of three blocks
+    ("int8", "bf16", 2, 8, 64, 16, 130, [1111], None),
+    ("int8", "f16", 1, 65, 128, 128, 1, [1500, 0, 127], None),              # one token of many heads
+    ("e4m3", "f16", 8, 32, 64, 64, 160, [900, 0, 129, 511], [160, 160, 0, 97])])
+def test_prompts_over_many_tiles(code, dtype, kv, heads, dim, page, T, lens, new):
+    """Chunks far into a context, with the positions in shares where there are few rows; scores that
+    move the references from tile to tile."""
+    rng = np.random.default_rng(T + page)
+    d = OnDevice(make(rng, len(lens), (max(lens) + T) // page + 1, kv, dim, page, 16, code))
+    q = 2 * rng.standard_normal((len(lens), T, heads, dim))
+    q[:, ::5] *= 6
+    out, _ = check_attention(d, q, dtype, np.array(lens), None if new is None else np.array(new),
+                             weights=rng.random((len(lens), kv, d.ref.cap)))
+    again, _ = run_attention(d, q, dtype, np.array(lens), None if new is None else np.array(new))
+    assert np.array_equal(out, again)
+
+
+@pytest.mark.parametrize("T", [1, 70])
+def test_missing_pages_far_apart(T):
+    """A long table most of whose pages are missing, whole tiles and shares of it among them."""
+    rng = np.random.default_rng(T)
+    d = OnDevice(make(rng, 2, 40, 1, 64, 64, 32, "int8"))
+    d.ref.table[rng.random(d.ref.table.shape) < 0.7] = -1
+    d.ref.table[0, :20] = d.ref.n_pages
+    d.t["table"].copy_(dev(d.ref.table))
+    for dtype in ("f16", "f32"):
+        check_attention(d, rng.standard_normal((2, T, 4, 64)), dtype, np.array([2560 - T, 2011]),
+                        weights=rng.random((2, 1, 2560)))
+
+
+@pytest.mark.parametrize("T,heads", [(1, 6), (30, 6)])
+def test_no_new_rows_and_shared_pages(T, heads):
+    """A batch without a new row keeps its output and weights; two sequences that read the same pages agree."""
+    rng = np.random.default_rng(T)
+    d = OnDevice(make(rng, 3, 3, 2, 64, 64, 16, "int8"))
+    d.ref.table[1] = d.ref.table[0]
+    d.t["table"].copy_(dev(d.ref.table))
+    q = rng.standard_normal((3, T, heads, 64))
+    q[1] = q[0]
+    lens, w = np.array([130, 130, 0]), rng.random((3, 2, 192))
+    w[1] = w[0]
+    check_attention(d, q, "f16", lens, np.zeros(3, int), weights=w)
+    out, w = check_attention(d, q, "f16", lens, weights=w)
+    assert np.array_equal(out[0], out[1]) and np.array_equal(w[0], w[1])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_many_sequences(dtype):
+    """More sequences than CTAs, most of them short or empty."""
+    rng = np.random.default_rng(6)
+    B = 600
+    d = OnDevice(make(rng, B, 3, 1, 64, 16, 16, "e4m3"))
+    lens = rng.integers(0, 47, B) * (rng.random(B) < 0.6)
+    check_attention(d, rng.standard_normal((B, 1, 3, 64)), dtype, lens, (rng.random(B) < 0.8).astype(int),
+                    weights=rng.random((B, 1, 48)))
+
+
+@pytest.mark.parametrize("heads", [80, 200])
+def test_many_heads_of_one_kv_head(heads):
+    """fp32 rows of more heads than a call's rows at a time, one token after the other."""
+    rng = np.random.default_rng(heads)
+    d = OnDevice(make(rng, 2, 3, 1, 64, 64, 16, "int8"))
+    check_attention(d, rng.standard_normal((2, 3, heads, 64)), "f32", np.array([100, 0]), np.array([3, 2]),
+                    weights=rng.random((2, 1, 192)))
+
+
 def test_missing_pages_and_empty_rows():
     """Ids outside the pool are unseen positions; a row that sees none gives zeros."""
     rng = np.random.default_rng(2)
@@ -281,6 +349,78 @@ def test_scales_of_any_size():
             d.t[n].copy_(dev(getattr(d.ref, n)))
         for dtype in ("f16", "f32"):
             check_attention(d, 4 * rng.standard_normal((1, T, 4, 64)), dtype, np.array([190 - T]))
+
+
+@pytest.mark.parametrize("T", [1, 70])
+def test_tiny_scales(T):
+    """V scales down to fp32's smallest: blocks below 2^-100 add nothing, alone or beside others."""
+    rng = np.random.default_rng(14)
+    for tiny in (np.float32(1e-44), np.float32(1e-38), np.float32(2.0 ** -99)):
+        for share in (1.0, 0.5):
+            d = OnDevice(make(rng, 1, 3, 2, 64, 64, 16, "int8"))
+            d.ref.vs[rng.random(d.ref.vs.shape) < share] = tiny
+            d.t["vs"].copy_(dev(d.ref.vs))
+            for dtype in ("bf16", "f32"):
+                check_attention(d, rng.standard_normal((1, T, 4, 64)), dtype, np.array([180 - T]),
+                                weights=rng.random((1, 2, 192)))
+
+
+def test_two_graphs_on_two_streams():
+    """A single token and a prompt with weights, captured with a workspace each and replayed side by side; an
+    eviction captured too.  Every replay gives the eager call's bits."""
+    t = torch()
+    rng = np.random.default_rng(41)
+    sides = []
+    for T, H, lens in ((1, 14, [700, 3, 90]), (60, 6, [500, 0, 130])):
+        d = OnDevice(make(rng, 3, 12, 2, 64, 64, 16, "int8"))
+        q = dev(rng.standard_normal((3, T, H, 64)).astype(np.float16))
+        s = {"d": d, "q": q, "T": T, "H": H, "lens": ints(lens), "w": dev(rng.random((3, 2, 768)).astype(np.float32)),
+             "ws": t.zeros(d.h.attention_workspace(3, T, H, weights=True), dtype=t.uint8, device="cuda"),
+             "st": t.cuda.Stream()}
+        s["out"], s["wo"] = t.zeros_like(q), t.zeros_like(s["w"])
+        n = d.h.evict_workspace(3, 64)
+        s.update(ews=t.zeros(n, dtype=t.uint8, device="cuda"), eb=n, pos=t.arange(768, dtype=t.int32, device="cuda").expand(3, 2, -1).contiguous(),
+                 ew=t.zeros_like(s["w"]), ep=t.zeros(3, 2, 768, dtype=t.int32, device="cuda"), el=ints([0, 0, 0]))
+        sides.append(s)
+
+    def call(s, stream):
+        s["d"].h.attention(s["q"].data_ptr(), s["out"].data_ptr(), "f16", 3, s["T"], s["H"], s["lens"].data_ptr(),
+                           w_in=s["w"].data_ptr(), w_out=s["wo"].data_ptr(), ld_w=768, ws=s["ws"].data_ptr(),
+                           ws_bytes=s["ws"].numel(), stream=stream)
+        s["d"].h.evict(3, 64, s["lens"].data_ptr(), s["el"].data_ptr(), s["wo"].data_ptr(), s["ew"].data_ptr(),
+                       s["pos"].data_ptr(), s["ep"].data_ptr(), 768, seen=s["lens"].data_ptr(), recent=8,
+                       ws=s["ews"].data_ptr(), ws_bytes=s["eb"], stream=stream)
+
+    t.cuda.synchronize()
+    names = ("out", "wo", "ew", "ep", "el")
+    for s in sides:
+        pools = {n: s["d"].t[n].clone() for n in ("k", "v", "ks", "vs")}
+        call(s, 0)
+        t.cuda.synchronize()
+        s["want"] = [s[n].clone() for n in names] + [s["d"].t[n].clone() for n in pools]
+        for n, x in pools.items():
+            s["d"].t[n].copy_(x)
+        for n in names:
+            s[n].zero_()
+        s["pools"] = pools
+    t.cuda.synchronize()
+    for s in sides:
+        s["graph"] = t.cuda.CUDAGraph()
+        with t.cuda.graph(s["graph"], stream=s["st"]):
+            call(s, t.cuda.current_stream().cuda_stream)
+    for _ in range(5):
+        for s in sides:
+            for n, x in s["pools"].items():
+                s["d"].t[n].copy_(x)
+        t.cuda.synchronize()
+        for s in sides:
+            with t.cuda.stream(s["st"]):
+                s["graph"].replay()
+        t.cuda.synchronize()
+        for s in sides:
+            got = [s[n] for n in names] + [s["d"].t[n] for n in s["pools"]]
+            assert all(t.equal(g, w) for g, w in zip(got, s["want"]))
+            assert int(s["ws"][:4].view(t.int32)[0]) == 0  # no wait ran out
 
 
 def test_query_ranges():
@@ -380,6 +520,27 @@ def test_evict_exact(code, dim, page, block, keep, first, recent):
         append(d, rows(rng, len(lens), T, 3, dim), rows(rng, len(lens), T, 3, dim), "f16", lens, n)
         lens, seen = lens + n, seen + n
         w = w + rng.random(w.shape).astype(np.float32)
+
+
+@pytest.mark.parametrize("max_pages,keep", [(700, 20032), (900, 4096), (900, 56000)])
+def test_evict_long(max_pages, keep):
+    """Contexts and budgets beyond what the selection holds on chip."""
+    rng = np.random.default_rng(keep)
+    t = torch()
+    d = OnDevice(make(rng, 1, max_pages, 1, 64, 64, 64, "int8", spare=0))
+    cap = d.ref.cap
+    w = np.round(rng.random((1, 1, cap)) * 5000).astype(np.float32)
+    pos = np.broadcast_to(np.arange(cap, dtype=np.int32), w.shape).copy()
+    lens = np.array([cap - 7])
+    dw, dp, dl = dev(w), dev(pos), ints(lens)
+    ws = t.empty(d.h.evict_workspace(1, keep), dtype=t.uint8, device="cuda")
+    d.h.evict(1, keep, dl.data_ptr(), dl.data_ptr(), dw.data_ptr(), dw.data_ptr(), dp.data_ptr(), dp.data_ptr(), cap,
+              seen=ints(lens).data_ptr(), first=4, recent=100, ws=ws.data_ptr(), ws_bytes=ws.numel())
+    t.cuda.synchronize()
+    lens, w, pos = d.ref.evict(keep, 4, 100, lens, lens, w, pos)
+    d.same_as_reference()
+    assert np.array_equal(dl.cpu().numpy(), lens)
+    assert np.array_equal(dw.cpu().numpy(), w) and np.array_equal(dp.cpu().numpy(), pos)
 
 
 def test_evict_missing_pages():

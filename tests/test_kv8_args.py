@@ -28,7 +28,7 @@ BAD_CACHES = [({"k_codes": 0}, -12), ({"v_codes": 0}, -12), ({"k_scales": 0}, -1
               ({"block_table": 0}, -12), ({"k_codes": A + 8}, -13), ({"code": 2}, -13), ({"head_dim": 96}, -14),
               ({"head_dim": 256}, -14), ({"block": 8}, -13), ({"block": 48}, -13), ({"page_size": 24}, -13),
               ({"page_size": 0}, -13), ({"block": 64, "page_size": 96}, -13), ({"n_kv": 0}, -13), ({"n_pages": 0}, -13),
-              ({"max_pages": 0}, -13), ({"n_pages": 1 << 24, "n_kv": 8}, -13), ({"max_pages": 1 << 25}, -13)]
+              ({"max_pages": 0}, -13), ({"k_scales": A + 2}, -13), ({"block_table": A + 1}, -13), ({"n_pages": 1 << 24, "n_kv": 8}, -13), ({"max_pages": 1 << 25}, -13)]
 
 
 @pytest.mark.parametrize("kw,code", BAD_CACHES)
@@ -61,6 +61,9 @@ def test_append_and_read_arguments():
         refused(lambda: call(A, A, "f16", 1, 0, A), -13)
         refused(lambda: call(A, A, "f16", 1, -3, A), -13)
         refused(lambda: call(A, A, "f16", 1, 1, A, ld=127), -13)
+        refused(lambda: call(A + 1, A, "f16", 1, 1, A), -13)
+        refused(lambda: call(A, A + 2, "f32", 1, 1, A), -13)
+        refused(lambda: call(A, A, "f16", 1, 1, A + 2), -13)
     assert c.lib.n730_kv8_append(c._ref, A, A, 3, 128, 1, 1, A, None, None) == -13
     assert c.lib.n730_kv8_read(c._ref, A, A, -1, 128, 1, 1, None, A, None) == -13
 
@@ -90,6 +93,13 @@ def test_attention_arguments():
     refused(call(ws_bytes=need - 1), -13)
     refused(call(ws=A + 4), -13)
     refused(call(scale=float("nan")), -13)
+    refused(call(q=A + 1), -13)
+    refused(call(out=A + 1), -13)
+    refused(call(dtype="f32", q=A + 2), -13)
+    refused(call(lens=A + 2), -13)
+    refused(call(w_out=A + 1), -13)
+    refused(lambda: cache(max_pages=1 << 20).attention_workspace(4096, 1, 2), -13)  # 2^31 tiles
+    refused(lambda: cache(n_kv=1).attention_workspace(1, 1, 8193), -13)
     refused(call(scale=float("inf")), -13)
     assert c.lib.n730_kv8_attention(c._ref, A, 7, 896, 2, 3, 14, 1.0, A, None, A, 896, None, None, 0, A, need, None) == -13
 
@@ -116,6 +126,8 @@ def test_evict_arguments():
     refused(call(ld_w=255), -13)
     refused(call(ws_bytes=need - 1), -13)
     refused(call(ws=A + 2), -13)
+    refused(call(pos=A + 2), -13)
+    refused(call(w=A + 1), -13)
 
 
 def test_reference_codes_round_to_nearest_even():
