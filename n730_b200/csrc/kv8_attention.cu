@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
     }
     if (whole && a.lse && tid < nrow)
       a.lse[((int64_t)b * c.n_kv + h) * a.rows + f0 + tid] =
-          sm.tot[tid][2] == 0.f ? INFINITY : sm.tot[tid][1] + lg2(sm.tot[tid][2]);
+          sm.tot[tid][2] == 0.f ? INFINITY : sm.tot[tid][1] + log2f(sm.tot[tid][2]);
   }
   cp_wait<0>();
 }
@@ -704,7 +704,7 @@ __device__ __forceinline__ float kf_lse_of(const KFArgs& a, const int2& p, int r
   }
   const float m = warp_max(M), ms = m == -INFINITY ? 0.f : m;
   l = warp_sum(l * ex2(M - ms));
-  return l == 0.f ? INFINITY : m + lg2(l);
+  return l == 0.f ? INFINITY : m + log2f(l);
 }
 
 // sums of weight x V against mo, and of weights l against m, of two sets of parts
@@ -765,7 +765,7 @@ __global__ void __launch_bounds__(KF_THREADS) kv8_finish_kernel(const KFArgs a) 
         }
         kd_answer<HD>(d, b, h, f0 + r, d4 * 4, sum.num, sum.mo, sum.m, sum.l);
         if (a.splits && d.lse && d4 == 0)  // for the prompt's weights
-          d.lse[((int64_t)b * c.n_kv + h) * d.rows + f0 + r] = sum.l == 0.f ? INFINITY : sum.m + lg2(sum.l);
+          d.lse[((int64_t)b * c.n_kv + h) * d.rows + f0 + r] = sum.l == 0.f ? INFINITY : sum.m + log2f(sum.l);
       }
     }
     return;

@@ -16,8 +16,8 @@
 // Tensor memory: scores of A and B, 128 columns each, outputs of A and B, head_dim columns each.
 //
 // Softmax.  The weight x V scale of a position is formed by one FMA and one exp2: its exponent is
-// score * (row, block factor) + log2(V scale) - reference, and the sum of weights gets each block's sum
-// times 2^(reference - maximum) / V scale.  Both references follow the largest values lazily (2^8 of
+// score * (row, block factor) + lv - reference with lv the approximate log2(V scale), and the sum of
+// weights gets each block's sum times 2^(reference - maximum - lv).  Both references follow the largest values lazily (2^8 of
 // slack), so outputs in tensor memory are rescaled only when a row's maximum has grown by that much.
 //
 // Bounds: per 128x128 tile 2 x 1024 cycles of tensor work for head_dim 128 against 1024 of exp2 and about
@@ -43,6 +43,8 @@ constexpr int KW_THREADS = 13 * 32;
 constexpr int KP_RING = 4;        // tiles whose scales are kept: two more than tiles of codes
 constexpr float KP_SLACK = 8.f;   // log2 of how far a weight x V scale may exceed its reference (fp16: 2^16)
 constexpr float KP_SUM_SLACK = 64.f;  // and of how far a weight in the sum (fp32)
+// V scales and references this close leave weight x V scale and the way back to the weight inside fp32's range
+constexpr float KP_NEAR_MIN = 0x1p-24f, KP_NEAR_MAX = 0x1p24f, KP_NEAR_REFS = 40.f, KP_NEAR_BACK = 0x1p64f;
 
 template <int HD>
 struct KPCfg {
@@ -61,8 +63,8 @@ struct KPSmem {
   uint8_t q[KPCfg<HD>::NB * KPCfg<HD>::QB];
   uint8_t k[2][KPCfg<HD>::KV];
   uint8_t v[2][KPCfg<HD>::KV];
-  float sc[KP_RING][3][8];   // by block of 16 positions: K's scale (-infinity: no page), log2 of V's scale, 1 / V's scale
-  int odd[KP_RING][4];       // by warp of the codes: some block has no page, or a V scale of 0
+  float sc[KP_RING][3][8];   // by block of 16 positions: K's scale (-infinity: no page), lv = log2 of V's scale, 2^-lv
+  int odd[KP_RING][4];       // by warp of the codes: some block has no page, or a V scale of 0 or far from 1
   float rowmul[KP_ROWS];
   uint64_t kfull[2], vfull[2], kfree[2], vfree[2], sfull[2], pready[2], odone[2], drain;
   uint32_t tmem;
@@ -115,8 +117,8 @@ __device__ __forceinline__ void tc_mma_ss(uint32_t tmem_d, uint64_t adesc, uint6
                :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(IDESC), "r"(accumulate) : "memory");
 }
 
-// Brings a warp's share of query rows into shared memory: row r (of 32) is scaled by a power of two, so that its largest magnitude lies in [2^13, 2^14) (rows of zeros or with an
-// infinity stay), and written as row r of a K-major, swizzled operand with `block` bytes between 64-channel blocks.
+// Brings a warp's share of 16-bit query rows into shared memory: row r (of 32) is scaled by a power of two, so that its
+// largest magnitude lies in [2^13, 2^14) (rows of zeros or with an infinity stay), and written as row r of a K-major, swizzled operand with `block` bytes between 64-channel blocks.
 // A lane takes 8 channels; `put(r, mul)` is called by one lane a row with what scores of it are to be multiplied by,
 // `at(r)` gives the row's first element, negative for rows that are not there.
 template <int HD, class At, class Put>
@@ -132,7 +134,7 @@ __device__ __forceinline__ void kp_put_rows(const void* q, int dtype, bool vec, 
       const int64_t i = at(r0 + u * RPI + sub);
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[u][e] = 0.f;
-      if (i >= 0 && vec && dtype != N730_F32) {
+      if (i >= 0 && vec) {
         const uint4 y = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(q) + i + ch * 8);
         const uint32_t w[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
@@ -294,7 +296,7 @@ __device__ __forceinline__ void kp_softmax(uint32_t ts, uint32_t to, const float
   }
 }
 
-// The same for any tile: the first `sees` positions are seen, blocks may have no page or a V scale of 0.
+// The same for any tile: the first `sees` positions are seen, blocks may have no page or any V scale.
 template <int HD>
 __device__ __forceinline__ void kp_softmax_any(uint32_t ts, uint32_t to, const float* ksc, const float* lvs, float rm, int sees,
                                                bool outputs, float& m_ref, float& mo_ref, float& l) {
@@ -330,7 +332,9 @@ __device__ __forceinline__ void kp_softmax_any(uint32_t ts, uint32_t to, const f
         const float ks = ksc[blk], lv = lvs[blk];
         // zero V: the weights count in the sum, their product with V is zero
         const bool none = ks == -INFINITY, zero = lv == -INFINITY;  // the same for all rows
-        const float fk = rm * ks, off = zero ? -ms : lv - mos, back = zero ? 1.f : back0 * lvs[8 + blk];
+        float back = zero ? 1.f : back0 * lvs[8 + blk];
+        const bool apart = back > KP_NEAR_BACK;  // the row's sum takes its own exp2
+        const float fk = rm * ks, off = zero ? -ms : lv - mos;
         const int n = none ? 0 : sees - blk * 16;
         float sum = 0.f;
 #pragma unroll
@@ -339,6 +343,12 @@ __device__ __forceinline__ void kp_softmax_any(uint32_t ts, uint32_t to, const f
           const float p1 = i + 1 < n ? ex2(fmaf(v[16 * e + i + 1], fk, off)) : 0.f;
           sum += p0 + p1;
           w[hh * 16 + e * 8 + i / 2] = zero ? 0u : h2u(__floats2half2_rn(p0, p1));
+        }
+        if (__any_sync(0xffffffffu, apart)) {
+          float own = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) own += i < n ? ex2(fmaf(v[16 * e + i], fk, -ms)) : 0.f;
+          if (apart) { sum = own; back = 1.f; }
         }
         l = fmaf(sum, back, l);
       }
@@ -470,8 +480,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
     };
     auto load_scale = [&](const int (&row)[MINE]) {
       const int r = lane_row(row);
-      const float s = r >= 0 ? ((lane & 1) ? c.v_scales : c.k_scales)[r >> a.log_block] : -1.f;
-      return (lane & 1) && s < KV8_TINY ? 0.f : s;
+      return r >= 0 ? ((lane & 1) ? c.v_scales : c.k_scales)[r >> a.log_block] : -1.f;
     };
     const int at0 = lrow * 128 + (chunk >> 2) * Cfg::KB;
     auto store = [&](uint8_t* dst, int j, const int (&row)[MINE]) {
@@ -513,11 +522,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
         const bool mine = lane < 2 * MINE && block(lane >> 1) < BLOCKS, none = lane_row(row) < 0;
         if (mine) {
           float* at = &sm.sc[j % KP_RING][lane & 1][block(lane >> 1)];
-          at[0] = none ? -INFINITY : lane & 1 ? lg2(scale) : scale;
-          if (lane & 1) at[8] = none || scale == 0.f ? 0.f : __frcp_rn(scale);
+          if ((lane & 1) && scale < KV8_TINY) scale = 0.f;
+          const float lv = lg2(scale);
+          at[0] = none ? -INFINITY : lane & 1 ? lv : scale;
+          if (lane & 1) at[8] = none || scale == 0.f ? 0.f : ex2(-lv);  // undoes what lv does, not the scale itself
         }
-        // whether every block has a page and a V scale
-        const bool odd = __any_sync(0xffffffffu, mine && (none || ((lane & 1) && scale == 0.f)));
+        // whether every block has a page and a V scale that is not far from 1
+        const bool odd = __any_sync(0xffffffffu, mine && (none || ((lane & 1) && !(scale > KP_NEAR_MIN && scale < KP_NEAR_MAX))));
         if (lane == 0) sm.odd[j % KP_RING][w] = odd;
       }
       ready(is_k ? &sm.kfull[s] : &sm.vfull[s]);
@@ -606,7 +617,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
     const uint32_t ts = tmem + ((uint32_t)(q * 32) << 16) + Cfg::S0 + x * KP_KEYS;
     const uint32_t to = tmem + ((uint32_t)(q * 32) << 16) + Cfg::O0 + x * HD;
     float m_ref = -INFINITY, mo_ref = -INFINITY, l = 0.f;
-    bool go = true;
+    bool go = true, far = false;
     for (int j = 0; j < nt; ++j) {
       if (!kp_wait_warp(&sm.sfull[x], (uint32_t)(j & 1), abortf)) { go = false; break; }
       tc_fence_after();
@@ -615,10 +626,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
       const int p0 = (j0 + j) * KP_KEYS;
       const bool masked = p0 + KP_KEYS > sees_all;  // some row of the CTA does not see all of the tile
       const int4 odd4 = *reinterpret_cast<const int4*>(sm.odd[j % KP_RING]);
-      if (!masked && !(odd4.x | odd4.y | odd4.z))
+      if (!masked && !far && !(odd4.x | odd4.y | odd4.z)) {
         kp_softmax<HD>(ts, to, ksc, lvs, rm, j > 0, m_ref, mo_ref, l);
-      else
+      } else {
         kp_softmax_any<HD>(ts, to, ksc, lvs, rm, masked ? vis - p0 : KP_KEYS, j > 0, m_ref, mo_ref, l);
+        far = __any_sync(0xffffffffu, fabsf(mo_ref - m_ref) > KP_NEAR_REFS);
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive1(&sm.pready[x]);
@@ -645,7 +658,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
             *reinterpret_cast<float4*>(a.part + slot * HD + cc * 32 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-        } else if (a.vec && a.dtype != N730_F32) {
+        } else if (a.vec) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             uint32_t w[4];
@@ -667,7 +680,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
         }
       }
       if (live && a.splits > 1) reinterpret_cast<float4*>(a.part_ml)[slot] = make_float4(mo_ref, m_ref, l, 0.f);
-      if (live && a.lse && a.splits == 1) a.lse[head * a.rows + f] = l == 0.f ? INFINITY : m_ref + lg2(l);
+      if (live && a.lse && a.splits == 1) a.lse[head * a.rows + f] = l == 0.f ? INFINITY : m_ref + log2f(l);
     }
   }
   tc_fence_before();

@@ -365,6 +365,19 @@ def test_tiny_scales(T):
                                 weights=rng.random((1, 2, 192)))
 
 
+@pytest.mark.parametrize("T", [1, 70])
+def test_scales_far_apart(T):
+    """V scales from 2^-99 to 2^100 in one row's blocks: the softmax weights do not feel them."""
+    rng = np.random.default_rng(15)
+    for lo, hi in ((-99, 100), (-24, 60), (60, 100), (0, 100)):
+        d = OnDevice(make(rng, 1, 6, 2, 64, 64, 16, "int8"))
+        d.ref.vs[:] = np.exp2(rng.choice([lo, hi, 0], d.ref.vs.shape, p=[0.3, 0.2, 0.5])).astype(np.float32)
+        d.t["vs"].copy_(dev(d.ref.vs))
+        for dtype in ("bf16", "f32"):
+            check_attention(d, rng.standard_normal((1, T, 4, 64)), dtype, np.array([380 - T]),
+                            weights=np.zeros((1, 2, 384)))
+
+
 def test_two_graphs_on_two_streams():
     """A single token and a prompt with weights, captured with a workspace each and replayed side by side; an
     eviction captured too.  Every replay gives the eager call's bits."""
