@@ -117,58 +117,53 @@ __device__ __forceinline__ void tc_mma_ss(uint32_t tmem_d, uint64_t adesc, uint6
                :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(IDESC), "r"(accumulate) : "memory");
 }
 
-// Brings a warp's share of 16-bit query rows into shared memory: row r (of 32) is scaled by a power of two, so that its
-// largest magnitude lies in [2^13, 2^14) (rows of zeros or with an infinity stay), and written as row r of a K-major, swizzled operand with `block` bytes between 64-channel blocks.
-// A lane takes 8 channels; `put(r, mul)` is called by one lane a row with what scores of it are to be multiplied by,
-// `at(r)` gives the row's first element, negative for rows that are not there.
-template <int HD, class At, class Put>
-__device__ __forceinline__ void kp_put_rows(const void* q, int dtype, bool vec, float sign, float scale, uint8_t* dst, int block,
-                                            int first, At at, Put put) {
-  constexpr int LPR = HD / 8, RPI = 32 / LPR, U = 4;  // lanes a row, rows an instruction, instructions in flight
+// Rows of a warp's share of the 16-bit queries: a lane holds 8 channels of U rows, RPI rows an instruction.  `at(r)`
+// gives row r's first element, negative for rows that are not there.
+template <int HD>
+struct KPRows { static constexpr int LPR = HD / 8, RPI = 32 / LPR; };
+template <int HD, int U, class At>
+__device__ __forceinline__ void kp_load_rows(const void* q, bool vec, int first, At at, uint4 (&x)[U]) {
+  const int lane = threadIdx.x & 31, sub = lane / KPRows<HD>::LPR, ch = lane % KPRows<HD>::LPR;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t i = at(first + u * KPRows<HD>::RPI + sub);
+    x[u] = make_uint4(0, 0, 0, 0);
+    if (i < 0) continue;
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(q) + i + ch * 8;
+    if (vec) x[u] = *reinterpret_cast<const uint4*>(p);
+    else x[u] = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
+  }
+}
+// Writes them as rows of a K-major, swizzled operand with `block` bytes between 64-channel blocks, each scaled by a
+// power of two, so that its largest magnitude lies in [2^13, 2^14) (rows of zeros or with an infinity stay);
+// `put(r, mul)` is called by one lane a row with what scores of it are to be multiplied by.
+template <int HD, int U, class Put>
+__device__ __forceinline__ void kp_put_rows(const uint4 (&raw)[U], int dtype, float sign, float scale, uint8_t* dst, int block,
+                                            int first, Put put) {
+  constexpr int LPR = KPRows<HD>::LPR;
   const int lane = threadIdx.x & 31, sub = lane / LPR, ch = lane % LPR;
-#pragma unroll 1
-  for (int r0 = first; r0 < first + 32; r0 += U * RPI) {
-    float x[U][8];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t i = at(r0 + u * RPI + sub);
+  for (int u = 0; u < U; ++u) {
+    const uint32_t y[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+    float x[8], m = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[u][e] = 0.f;
-      if (i >= 0 && vec) {
-        const uint4 y = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(q) + i + ch * 8);
-        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (dtype == N730_F16) {
-            const float2 f = __half22float2(u2h(w[e]));
-            x[u][2 * e] = f.x; x[u][2 * e + 1] = f.y;
-          } else {
-            x[u][2 * e] = __uint_as_float(w[e] << 16);
-            x[u][2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-          }
-        }
-      } else if (i >= 0) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[u][e] = kv8_load1(q, i + ch * 8 + e, dtype);
-      }
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = dtype == N730_F16 ? __half22float2(u2h(y[e]))
+                                         : make_float2(__uint_as_float(y[e] << 16), __uint_as_float(y[e] & 0xffff0000u));
+      x[2 * e] = f.x; x[2 * e + 1] = f.y;
+      m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = r0 + u * RPI + sub;
-      float m = 0.f;
+    for (int k = 1; k < LPR; k <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+    const int ex = (int)((__float_as_uint(m) >> 23) & 255u);
+    const int sh = ex == 0 || ex == 255 ? 0 : min(max(140 - ex, -126), 126);
+    const float mul = __uint_as_float((uint32_t)(127 + sh) << 23) * sign;
+    uint32_t w[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[u][e]));
-#pragma unroll
-      for (int k = 1; k < LPR; k <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-      const int ex = (int)((__float_as_uint(m) >> 23) & 255u);
-      const int sh = ex == 0 || ex == 255 ? 0 : min(max(140 - ex, -126), 126);
-      const float mul = __uint_as_float((uint32_t)(127 + sh) << 23) * sign;
-      uint32_t w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = h2u(__floats2half2_rn(x[u][2 * e] * mul, x[u][2 * e + 1] * mul));
-      *reinterpret_cast<uint4*>(dst + (ch >> 3) * block + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-      if (ch == 0) put(r, scale * __uint_as_float((uint32_t)(127 - sh) << 23));
-    }
+    for (int e = 0; e < 4; ++e) w[e] = h2u(__floats2half2_rn(x[2 * e] * mul, x[2 * e + 1] * mul));
+    const int r = first + u * KPRows<HD>::RPI + sub;
+    *reinterpret_cast<uint4*>(dst + (ch >> 3) * block + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (ch == 0) put(r, scale * __uint_as_float((uint32_t)(127 - sh) << 23));
   }
 }
 // 16 codes as fp16 into a row of a swizzled operand, at the row's 128 bytes in the 64-channel block of `chunk`;
@@ -414,14 +409,18 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
                  :: "r"(smem_u32(&sm.tmem)), "r"(Cfg::TMEM) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // ---- Q: a row per warp at a time, scaled by a power of two, K-major and swizzled ----
-  if (warp < 8)  // 32 rows each
-    kp_put_rows<HD>(a.q, a.dtype, a.qvec, a.sign, a.scale_log2e, sm.q, Cfg::QB, warp * 32,
-                    [&](int r) -> int64_t {
-                      const int f = f0 + r;
-                      return r < nrow ? ((int64_t)b * a.tokens + f / a.group) * a.ldq + (int64_t)(h * a.group + f % a.group) * HD : -1;
-                    },
-                    [&](int r, float mul) { sm.rowmul[r] = mul; });
+  if (warp < 8) {  // Q, 32 rows each, K-major and swizzled
+    constexpr int U = 4;
+#pragma unroll 1
+    for (int r0 = warp * 32; r0 < warp * 32 + 32; r0 += U * KPRows<HD>::RPI) {
+      uint4 x[U];
+      kp_load_rows<HD, U>(a.q, a.qvec, r0, [&](int r) -> int64_t {
+        const int f = f0 + r;
+        return r < nrow ? ((int64_t)b * a.tokens + f / a.group) * a.ldq + (int64_t)(h * a.group + f % a.group) * HD : -1;
+      }, x);
+      kp_put_rows<HD, U>(x, a.dtype, a.sign, a.scale_log2e, sm.q, Cfg::QB, r0, [&](int r, float mul) { sm.rowmul[r] = mul; });
+    }
+  }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   tc_fence_before();
   __syncthreads();
@@ -766,24 +765,32 @@ kv8_prompt_weights_kernel(const KPArgs a, const float* w_in, float* w_out, int64
 
   if (warp >= 8 && warp < 12) {
     const int w = warp - 8;
+    constexpr int U = 32 / KPRows<HD>::RPI;  // the share at once: the next tile's rows are on their way during this one's products
+    uint4 x[U];
+    float lse;
+    auto load = [&](int i) {
+      const int first = (i0 + i) * RT;
+      kp_load_rows<HD, U>(a.q, a.qvec, w * 32, [&](int r) -> int64_t {
+        const int f = first + r;
+        return f < rows ? ((int64_t)b * a.tokens + f / a.group) * a.ldq + (int64_t)(h * a.group + f % a.group) * HD : -1;
+      }, x);
+      const int f = first + w * 32 + lane;
+      lse = f < rows ? a.lse[head * a.rows + f] : INFINITY;
+    };
+    if (n > 0) load(0);
+#pragma unroll 1
     for (int i = 0; i < n; ++i) {
       const int s = i & 1;
       // the products of the tile before are done, and its factors read
       if (i >= 2 && !(kp_wait_warp(&sm.qfree[s], (uint32_t)((i / 2 - 1) & 1), abortf) &&
                       kp_wait_warp(&sm.sread[s], (uint32_t)((i / 2 - 1) & 1), abortf)))
         break;
-      const int first = (i0 + i) * RT;
-      kp_put_rows<HD>(a.q, a.dtype, a.qvec, a.sign, a.scale_log2e, sm.q[s], Cfg::KB, w * 32,
-                      [&](int r) -> int64_t {
-                        const int f = first + r;
-                        return f < rows ? ((int64_t)b * a.tokens + f / a.group) * a.ldq + (int64_t)(h * a.group + f % a.group) * HD : -1;
-                      },
-                      [&](int r, float mul) {
-                        sm.row[s][r] = make_float2(mul, first + r < rows ? a.lse[head * a.rows + first + r] : INFINITY);
-                      });
+      kp_put_rows<HD, U>(x, a.dtype, a.sign, a.scale_log2e, sm.q[s], Cfg::KB, w * 32, [&](int r, float mul) { sm.row[s][r].x = mul; });
+      sm.row[s][w * 32 + lane].y = lse;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive1(&sm.qfull[s]);
+      if (i + 1 < n) load(i + 1);
     }
   } else if (warp == 12) {
     const uint64_t kd = umma_desc_sw128(smem_u32(sm.k)), qd = umma_desc_sw128(smem_u32(sm.q[0]));
