@@ -43,7 +43,7 @@ int kv8_attention_launch(const KV8AttnCall& a, cudaStream_t st);
 
 // The tensor-memory kernel for prompts (kv8_prompt.cu): 256 rows of an item a CTA, the positions in
 // `splits` shares whose parts lie as [item tile][split][rg rows].
-struct KV8PromptPlan { int rows, tiles, splits, rg; };
+struct KV8PromptPlan { int rows, tiles, splits, rg, shares; };  // shares: of the rows, for the weights
 KV8PromptPlan kv8_prompt_plan(const N730KV8Cache& c, int batch, int tokens, int heads);
 int kv8_prompt_launch(const KV8AttnCall& k, const KV8PromptPlan& p, int* status, float* part, float* part_ml, float* lse,
                       cudaStream_t st);
@@ -105,20 +105,31 @@ template <int CODE>
 __device__ __forceinline__ uint32_t code_word(uint32_t x) { return CODE == N730_KV8_INT8 ? x ^ 0x80808080u : x; }
 
 // Launch with or without programmatic dependent launch.
-template <typename... KArgs, typename... Args>
-int kv8_launch(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl, Args... args) {
+template <class... KArgs, class... Args>
+int kv8_launch_cluster(void (*k)(KArgs...), dim3 grid, int cluster, dim3 block, size_t smem, cudaStream_t st, bool pdl, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
+  if (pdl) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = cluster;
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
   N730_CUDA(cudaLaunchKernelEx(&cfg, k, args...));
   return N730_OK;
+}
+template <class... KArgs, class... Args>
+int kv8_launch(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl, Args... args) {
+  return kv8_launch_cluster(k, grid, 1, block, smem, st, pdl, args...);
 }
 
 }  // namespace n730

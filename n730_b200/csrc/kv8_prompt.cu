@@ -39,7 +39,8 @@ constexpr int KP_KEYS = 128;      // positions of a tile
 // cost as much as the arithmetic).
 constexpr int KP_THREADS = 12 * 32;
 constexpr int KP_CODE_WARPS = 3, KP_MMA_WARP = 11;
-constexpr int KW_THREADS = 13 * 32;
+constexpr int KW_ROW_WARPS = 8, KW_MMA_WARP = 8 + KW_ROW_WARPS, KW_THREADS = (KW_MMA_WARP + 1) * 32;
+constexpr int KW_SHARES = 8;      // most CTAs of a cluster
 constexpr int KP_RING = 4;        // tiles whose scales are kept: two more than tiles of codes
 constexpr float KP_SLACK = 8.f;   // log2 of how far a weight x V scale may exceed its reference (fp16: 2^16)
 constexpr float KP_SUM_SLACK = 64.f;  // and of how far a weight in the sum (fp32)
@@ -359,6 +360,7 @@ struct KPArgs {
   int dtype, tokens, group, rows, tiles;  // rows = tokens * group; tiles of KP_ROWS rows
   int log_block;
   int splits;                             // shares of the positions, each a CTA
+  int shares;                             // of the rows, for the weights
   bool vec, qvec;                         // out rows, query rows are 16-byte aligned
   float scale_log2e;                      // its absolute value; the sign goes with the queries
   float sign;
@@ -425,6 +427,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_launch_dependents();
   const uint32_t tmem = sm.tmem;
   volatile int* abortf = &sm.abort;
 
@@ -693,10 +696,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
 // ---------------------------------------------------------------------------
 // accumulated weights of a prompt: w[b, h, p] += sum over the KV head's rows of exp2(score - lse)
 // ---------------------------------------------------------------------------
-// One CTA per 128 positions of a KV head walks over the rows that see them, 128 at a time, and forms
-// S^T = K Q^T, so that a position is a TMEM lane and its sum over the rows stays in one thread: warps 8-11
-// bring the rows' queries into shared memory, warp 12 issues the products, warps 0-3 sum the even row
-// tiles, 4-7 the odd ones; the two sums are added at the end (always in the same order).
+// A CTA walks over the rows that see its 128 positions of a KV head, 128 at a time, and forms
+// S^T = K Q^T, so that a position is a TMEM lane and its sum over the rows stays in one thread: warps 8-15
+// bring the rows' queries into shared memory, warp 16 issues the products, warps 0-3 sum the even row
+// tiles, 4-7 the odd ones.  Where the positions give the SMs too few CTAs, a cluster of them shares the rows and
+// the first adds up the sums, always in the same order.
 template <int HD>
 struct KWSmem {
   uint8_t k[KPCfg<HD>::KV];
@@ -718,15 +722,19 @@ kv8_prompt_weights_kernel(const KPArgs a, const float* w_in, float* w_out, int64
   KWSmem<HD>& sm = *reinterpret_cast<KWSmem<HD>*>(aligned_smem(kp_raw));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const N730KV8Cache& c = a.c;
-  const int b = blockIdx.z, h = blockIdx.y, p0 = blockIdx.x * KP_KEYS;
+  const int b = blockIdx.z, h = blockIdx.y, rank = blockIdx.x % a.shares, p0 = blockIdx.x / a.shares * KP_KEYS;
   const int cap = c.max_pages * c.page_size;
-  pdl_wait();
+  // all but lse was there before the attention's grid, which lets this one start when all of it holds its tensor memory
   const int L = kv8_len(a.lens, b, cap), n_new = kv8_new(a.n_new, b, a.tokens), rows = n_new * a.group;
   const int total = (int)min((int64_t)L + n_new, (int64_t)cap);
-  if (p0 >= total) return;
+  if (p0 >= total) {  // the whole cluster
+    pdl_wait();
+    return;
+  }
   const int64_t head = (int64_t)b * c.n_kv + h;
-  // row tiles [i0, i0 + n): the first whose last row sees position p0
-  const int i0 = max(0, p0 - L) * a.group / RT, n = (rows + RT - 1) / RT - i0;
+  // row tiles from the first whose last row sees position p0; this CTA's are [i0, i0 + n)
+  const int t0 = max(0, p0 - L) * a.group / RT, nt = (rows + RT - 1) / RT - t0;
+  const int i0 = t0 + nt * rank / a.shares, n = t0 + nt * (rank + 1) / a.shares - i0;
   const int* bt = c.block_table + (int64_t)b * c.max_pages;
   auto row_of = [&](int p) -> int64_t {
     if (p >= total) return -1;
@@ -735,7 +743,7 @@ kv8_prompt_weights_kernel(const KPArgs a, const float* w_in, float* w_out, int64
   };
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&sm.qfull[i], 4);
+      mbar_init(&sm.qfull[i], KW_ROW_WARPS);
       mbar_init(&sm.qfree[i], 1);
       mbar_init(&sm.sfull[i], 1);
       mbar_init(&sm.sread[i], 4);
@@ -744,7 +752,7 @@ kv8_prompt_weights_kernel(const KPArgs a, const float* w_in, float* w_out, int64
     fence_mbar_init();
     sm.abort = 0;
   }
-  if (warp == 12) {
+  if (warp == KW_MMA_WARP) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                  :: "r"(smem_u32(&sm.tmem)), "r"(COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -763,19 +771,21 @@ kv8_prompt_weights_kernel(const KPArgs a, const float* w_in, float* w_out, int64
   volatile int* abortf = &sm.abort;
   float sum = 0.f;
 
-  if (warp >= 8 && warp < 12) {
-    const int w = warp - 8;
-    constexpr int U = 32 / KPRows<HD>::RPI;  // the share at once: the next tile's rows are on their way during this one's products
+  pdl_wait();
+  if (warp >= 8 && warp < KW_MMA_WARP) {
+    // a warp's rows at once: the next tile's are on their way during this one's products
+    constexpr int WR = RT / KW_ROW_WARPS, U = WR / KPRows<HD>::RPI;
+    const int w0 = (warp - 8) * WR;
     uint4 x[U];
     float lse;
     auto load = [&](int i) {
       const int first = (i0 + i) * RT;
-      kp_load_rows<HD, U>(a.q, a.qvec, w * 32, [&](int r) -> int64_t {
+      kp_load_rows<HD, U>(a.q, a.qvec, w0, [&](int r) -> int64_t {
         const int f = first + r;
         return f < rows ? ((int64_t)b * a.tokens + f / a.group) * a.ldq + (int64_t)(h * a.group + f % a.group) * HD : -1;
       }, x);
-      const int f = first + w * 32 + lane;
-      lse = f < rows ? a.lse[head * a.rows + f] : INFINITY;
+      const int f = first + w0 + lane;
+      lse = lane < WR && f < rows ? a.lse[head * a.rows + f] : INFINITY;
     };
     if (n > 0) load(0);
 #pragma unroll 1
@@ -785,14 +795,14 @@ kv8_prompt_weights_kernel(const KPArgs a, const float* w_in, float* w_out, int64
       if (i >= 2 && !(kp_wait_warp(&sm.qfree[s], (uint32_t)((i / 2 - 1) & 1), abortf) &&
                       kp_wait_warp(&sm.sread[s], (uint32_t)((i / 2 - 1) & 1), abortf)))
         break;
-      kp_put_rows<HD, U>(x, a.dtype, a.sign, a.scale_log2e, sm.q[s], Cfg::KB, w * 32, [&](int r, float mul) { sm.row[s][r].x = mul; });
-      sm.row[s][w * 32 + lane].y = lse;
+      kp_put_rows<HD, U>(x, a.dtype, a.sign, a.scale_log2e, sm.q[s], Cfg::KB, w0, [&](int r, float mul) { sm.row[s][r].x = mul; });
+      if (lane < WR) sm.row[s][w0 + lane].y = lse;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive1(&sm.qfull[s]);
       if (i + 1 < n) load(i + 1);
     }
-  } else if (warp == 12) {
+  } else if (warp == KW_MMA_WARP) {
     const uint64_t kd = umma_desc_sw128(smem_u32(sm.k)), qd = umma_desc_sw128(smem_u32(sm.q[0]));
     bool go = true;
 #pragma unroll 1
@@ -851,11 +861,24 @@ kv8_prompt_weights_kernel(const KPArgs a, const float* w_in, float* w_out, int64
   __syncthreads();
   tc_fence_after();
   if (*abortf && tid == 0) *a.status = 1;
-  if (warp < 4 && p0 + tid < total) {
+  if (tid < KP_KEYS) sm.sum[tid] += sum;
+  if (a.shares > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (rank == 0 && tid < KP_KEYS && p0 + tid < total) {
     const int p = p0 + tid;
-    w_out[head * ldw + p] = (w_in && p < L ? w_in[head * ldw + p] : 0.f) + (sum + sm.sum[tid]);
+    float all = sm.sum[tid];
+    for (int k = 1; k < a.shares; ++k) {
+      uint32_t at;
+      float other;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&sm.sum[tid])), "r"(k));
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other) : "r"(at) : "memory");
+      all += other;
+    }
+    w_out[head * ldw + p] = (w_in && p < L ? w_in[head * ldw + p] : 0.f) + all;
   }
-  if (warp == 12)
+  __syncwarp();
+  // the others' shared memory stays until it is read
+  if (a.shares > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (warp == KW_MMA_WARP)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(COLS) : "memory");
 }
 
@@ -866,6 +889,9 @@ KV8PromptPlan kv8_prompt_plan(const N730KV8Cache& c, int batch, int tokens, int 
   p.rg = KP_ROWS;
   const int64_t ctas = (int64_t)batch * c.n_kv * p.tiles;
   const int64_t key_tiles = ((int64_t)c.max_pages * c.page_size + KP_KEYS - 1) / KP_KEYS;
+  // CTAs of a cluster that share the rows of 128 positions' weights, two row tiles each at least
+  const int64_t idle = num_sms() / std::max<int64_t>(1, (int64_t)batch * c.n_kv * key_tiles);
+  p.shares = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(KW_SHARES, idle), p.rows / (2 * KP_KEYS)));
   // shares of the positions while the SMs would stand idle, of four tiles at least
   p.splits = 1;
   while (ctas * (p.splits + 1) <= num_sms() && key_tiles / (p.splits + 1) >= 4) ++p.splits;
@@ -876,7 +902,7 @@ static KPArgs kp_args(const KV8AttnCall& k, const KV8PromptPlan& p, int* status,
   KPArgs a{};
   a.c = k.c;
   a.q = k.q; a.out = k.out; a.ldq = k.ldq; a.ldo = k.ldo; a.dtype = k.dtype;
-  a.tokens = k.tokens; a.group = k.heads / k.c.n_kv; a.rows = p.rows; a.tiles = p.tiles; a.splits = p.splits;
+  a.tokens = k.tokens; a.group = k.heads / k.c.n_kv; a.rows = p.rows; a.tiles = p.tiles; a.splits = p.splits; a.shares = p.shares;
   a.vec = ((uintptr_t)k.out & 15) == 0 && k.ldo * kv8_esize(k.dtype) % 16 == 0;
   a.qvec = ((uintptr_t)k.q & 15) == 0 && k.ldq * kv8_esize(k.dtype) % 16 == 0;
   a.scale_log2e = fabsf(k.scale) * 1.4426950408889634f;
@@ -898,8 +924,8 @@ static int prompt_weights_launch(const KPArgs& a, const KV8AttnCall& k, cudaStre
   const size_t smem = sizeof(KWSmem<HD>) + 1024;
   if (int rc = smem_attr_once<kv8_prompt_weights_kernel<HD, CODE>>((int)smem)) return rc;
   const int cap = a.c.max_pages * a.c.page_size;
-  return kv8_launch(kv8_prompt_weights_kernel<HD, CODE>, dim3((cap + KP_KEYS - 1) / KP_KEYS, a.c.n_kv, k.batch),
-                    dim3(KW_THREADS), smem, st, false, a, k.w_in, k.w_out, k.ldw);
+  return kv8_launch_cluster(kv8_prompt_weights_kernel<HD, CODE>, dim3((cap + KP_KEYS - 1) / KP_KEYS * a.shares, a.c.n_kv, k.batch),
+                            a.shares, dim3(KW_THREADS), smem, st, a.splits == 1, a, k.w_in, k.w_out, k.ldw);
 }
 
 int kv8_prompt_launch(const KV8AttnCall& k, const KV8PromptPlan& p, int* status, float* part, float* part_ml, float* lse,
