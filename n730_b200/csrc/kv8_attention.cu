@@ -9,8 +9,7 @@
 // joins an item's parts in run order, with as many CTAs as there are items.  Within a
 // CTA each warp takes every fourth tile.  An item counts for KD_ITEM_COST tiles more than it has, the
 // time that starting and ending one takes: without that the CTAs that meet many short sequences were
-// the last to finish.  The next run's first tile is
-// asked for before this one's outputs are joined.
+// the last to finish.  The next run's first tile is asked for before this one's outputs are joined.
 //
 // The products are transposed, so that a key or a channel is a row of mma.m16n8k16's A and the few
 // query rows are its 8 columns: no half of an instruction works on rows that are not there.
@@ -33,6 +32,10 @@
 // fp32 query is split into two fp16 terms, and so is P: fp32 calls lose about 2^-22.  For 16-bit calls P
 // is rounded to fp16 (2^-11 of each weight, below the rounding of the output).  Maxima, sums and
 // outputs are fp32.
+//
+// Bound by HBM: 2 head_dim code bytes and 8 / block of scales a position and KV head.  Whole calls: 128 sequences
+// ragged to 4096, 64 / 8 heads x 128, e4m3, 113.5 us (5.36 TB/s); one of 65501 positions 36.4 us, of which 5 start
+// and 5 join; 32 ragged to 8192 of 28 / 4 heads with weights 52.6 us, 31 here and 13 in the finishing kernel.
 #include <algorithm>
 #include <mutex>
 

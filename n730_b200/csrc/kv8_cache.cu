@@ -290,7 +290,8 @@ struct KV8ReadArgs {
 
 // A thread takes 16 channels of RD_ROWS positions, a warp's lanes whole rows one behind the other (contiguous in a
 // page); its loads do not wait for one another.  Bound by HBM: 1 byte read, 2 or 4 written a value.  With one
-// position a thread 8192 positions of 8 sequences and heads took 67 us (5.1 TB/s), too few bytes in flight.
+// position a thread 8192 positions of 8 sequences and heads took 67 us, too few bytes in flight; with four 63 us
+// (5.45 TB/s).
 constexpr int RD_ROWS = 4;
 
 template <int HD, int CODE>
@@ -355,6 +356,8 @@ __global__ void __launch_bounds__(KV8_THREADS) kv8_read_kernel(const KV8ReadArgs
 // Selection: the keys are read once into shared memory (up to EV_KEYS of them; longer contexts read
 // them again), the keep-th largest is found 11 bits at a time, and ranks of ties, holes and movers come
 // from ballots: a warp owns a run of slots, one scan over the warps' counts a pass.
+// 2304 slots of 4 heads take 14 us, all latency; 8192 of 256 rows 32 us in two waves of CTAs (two CTAs an SM, at 32
+// registers, lost 2 us).  The move is bound by HBM: 32 x 8 heads cut from up to 8192 slots to 2048, 52 to 62 us.
 struct KV8EvictArgs {
   N730KV8Cache c;
   int keep, first, recent, log_block;

@@ -21,7 +21,9 @@
 // slack), so outputs in tensor memory are rescaled only when a row's maximum has grown by that much.
 //
 // Bounds: per 128x128 tile 2 x 1024 cycles of tensor work for head_dim 128 against 1024 of exp2 and about
-// as many of issue slots on the 4 schedulers, for each of A and B.
+// as many of issue slots on the 4 schedulers, for each of A and B.  Measured: 2048 tokens behind 6144 positions, 64 / 8
+// heads x 128, 614 us, 783 TFLOP/s (0.47 of a large bf16 product): about 2.75k cycles of softmax in a period of
+// 4.6k a tile, and 3.5 waves of CTAs.
 //
 // Numerics: 16-bit queries are exact in fp16 after a power-of-two scaling of their row; the softmax
 // weights are rounded to fp16 (2^-11 of each, below the rounding of a 16-bit output).  Sums and outputs are
@@ -700,7 +702,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
 // S^T = K Q^T, so that a position is a TMEM lane and its sum over the rows stays in one thread: warps 8-15
 // bring the rows' queries into shared memory, warp 16 issues the products, warps 0-3 sum the even row
 // tiles, 4-7 the odd ones.  Where the positions give the SMs too few CTAs, a cluster of them shares the rows and
-// the first adds up the sums, always in the same order.
+// the first adds up the sums, always in the same order.  Bound by latency: a tile's rows pass a loader, the products
+// and the sums one behind the other.  4 prompts of 300 tokens, 14 / 2 heads x 64, 6 tiles of positions: 62 us with one
+// CTA for all rows and four warps that bring them, 20 us with three CTAs and eight.
 template <int HD>
 struct KWSmem {
   uint8_t k[KPCfg<HD>::KV];

@@ -51,7 +51,8 @@ class KV8Cache:
                                           stream), "kv8_read")
 
     def attention_workspace(self, batch: int, tokens: int, heads: int, weights: bool = False) -> int:
-        """Bytes of the workspace that ``attention`` wants, zeroed once by the caller."""
+        """Bytes of the workspace that ``attention`` of this size wants (not always more for more tokens), zeroed once by
+        the caller; its first int32 is 1 after a device wait ran out."""
         return _lib.check(self.lib.n730_kv8_attention_ws(self._ref, batch, tokens, heads, int(weights)),
                           "kv8_attention_ws")
 
