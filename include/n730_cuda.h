@@ -207,7 +207,7 @@ int64_t n730_kv8_attention_ws(const N730KV8Cache* c, int batch, int tokens, int 
  * positions: query t of sequence b, RoPE applied, sees positions [0, d_lens[b] + t] - call it after
  * n730_kv8_append with the same d_lens and d_new.  d_q and d_out rows are [n_heads][head_dim]
  * (query head i reads KV head i / (n_heads / n_kv)); out rows from d_new[b] on are left as they
- * were; a query that sees no position gives zeros.  Scores are scaled by `scale`.  16-bit rows round
+ * were; a query that sees no position gives zeros.  d_out must not overlap d_q.  Scores are scaled by `scale`.  16-bit rows round
  * the softmax weights to fp16, and more than 64 rows of a KV head run on the tcgen05 tensor cores;
  * fp32 rows keep fp32 accuracy and run 64 rows of a KV head at a time.
  * d_w_out (may be null) [batch][n_kv][ldw]: for positions below d_lens[b] + d_new[b], d_w (null:
@@ -271,7 +271,9 @@ typedef struct N730ModelConfig {
                             released (n730_model_seq_release) */
   int32_t kv_bits;       /* 0 or 16: fp16 cache.  8: int8 codes with an fp32 scale per 16 positions
                             and KV head (n730_kv8_*): half the cache's bytes, decode with one kernel
-                            per op; page_size must be a multiple of 16 */
+                            per op; page_size must be a multiple of 16, max_batch at most
+                            4096.  A block whose newest rows are dropped (n730_model_set_seq_len)
+                            keeps its scale */
 } N730ModelConfig;
 
 /* weight slots (n730_model_set_qweight); EMBED/LMHEAD take layer = -1 */

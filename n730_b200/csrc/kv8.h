@@ -35,8 +35,12 @@ struct KV8AttnCall {
   const float* w_in; float* w_out;
   int64_t ldw;
   void* ws; int64_t ws_bytes;
+  int* status;  // where a wait that ran out leaves its mark (null: the workspace's first word)
   bool pdl;
 };
+constexpr int KV8_MAX_BATCH = 4096;
+// what n730_kv8_attention refuses of the cache and the sizes
+int kv8_attention_check(const N730KV8Cache* c, int batch, int tokens, int heads);
 int64_t kv8_attention_ws(const N730KV8Cache& c, int batch, int tokens, int heads, bool weights);
 int64_t kv8_attention_ws_upto(const N730KV8Cache& c, int batch, int tokens, int heads);
 int kv8_attention_launch(const KV8AttnCall& a, cudaStream_t st);

@@ -56,7 +56,6 @@ constexpr int KD_CTAS_PER_SM = 3;
 // 52.7, 53.2, 54.7.
 constexpr int KD_ITEM_COST = 16;
 constexpr int KD_MIN_UNITS = 4;  // tiles of a run: fewer would leave warps idle and joins to do
-constexpr int KD_MAX_BATCH = 4096;
 constexpr float KD_SLACK = 8.f;  // log2 of how far a weight may exceed its reference
 constexpr uint64_t KD_WAIT_NS = 1000000000;  // bound of a wait for copies
 
@@ -858,9 +857,9 @@ static KDPlan kd_plan(const N730KV8Cache& c, int batch, int tokens, int heads, i
   return p;
 }
 
-static int kv8_attention_check(const N730KV8Cache* c, int batch, int tokens, int heads) {
+int kv8_attention_check(const N730KV8Cache* c, int batch, int tokens, int heads) {
   if (int rc = kv8_check(c, batch, "kv8_attention")) return rc;
-  N730_REQUIRE(batch <= KD_MAX_BATCH, N730_BAD_ARG, "kv8_attention: batch %d", batch);
+  N730_REQUIRE(batch <= KV8_MAX_BATCH, N730_BAD_ARG, "kv8_attention: batch %d", batch);
   N730_REQUIRE(tokens >= 1 && tokens <= (1 << 20), N730_BAD_ARG, "kv8_attention: tokens %d", tokens);
   N730_REQUIRE(heads >= 1 && heads <= 65535 && heads % c->n_kv == 0, N730_BAD_ARG,
                "kv8_attention: %d heads over %d KV heads", heads, c->n_kv);
@@ -922,7 +921,7 @@ int64_t kv8_attention_ws_upto(const N730KV8Cache& c, int batch, int tokens, int 
 template <int HD, int CODE, int NB, bool LO>
 static int split_launch(const KDArgs& a, const CUtensorMap& km, const CUtensorMap& vm, bool pdl, cudaStream_t st) {
   const size_t fixed = sizeof(KDSmem<HD>) + 1024;
-  if (int rc = smem_attr_once<kv8_split_kernel<HD, CODE, NB, LO>>((int)(fixed + KD_MAX_BATCH * 12))) return rc;
+  if (int rc = smem_attr_once<kv8_split_kernel<HD, CODE, NB, LO>>((int)(fixed + KV8_MAX_BATCH * 12))) return rc;
   return kv8_launch(kv8_split_kernel<HD, CODE, NB, LO>, dim3(a.n_cta), dim3(KD_THREADS), fixed + (size_t)a.batch * 12, st,
                     pdl, a, km, vm);
 }
@@ -961,7 +960,7 @@ int kv8_attention_launch(const KV8AttnCall& k, cudaStream_t st) {
   a.chunk = p.chunk;
   a.scale_log2e = k.scale * 1.4426950408889634f;
   a.lens = k.lens; a.n_new = k.n_new;
-  a.status = reinterpret_cast<int*>(ws);
+  a.status = k.status ? k.status : reinterpret_cast<int*>(ws);
   a.parts = reinterpret_cast<int2*>(ws + 256);
   a.part = reinterpret_cast<float*>(ws + p.part);
   a.part_ml = reinterpret_cast<float*>(ws + p.ml);

@@ -703,7 +703,8 @@ static int finalize(Model* m) {
   if (c.kv_bits == 8) {
     for (int l = 0; l < nl; ++l) {
       m->L[l].kv8.block_table = m->block_table;
-      if (int rc = kv8_check(&m->L[l].kv8, c.max_batch, "model: 8-bit cache")) return rc;
+      if (int rc = kv8_attention_check(&m->L[l].kv8, c.max_batch, 1, c.heads)) return rc;
+      if (int rc = kv8_attention_check(&m->L[l].kv8, 1, c.max_prefill, c.heads)) return rc;
     }
     m->kv8_ws_bytes = std::max(kv8_attention_ws(m->L[0].kv8, c.max_batch, 1, c.heads, false),
                                kv8_attention_ws_upto(m->L[0].kv8, 1, c.max_prefill, c.heads));
@@ -898,6 +899,7 @@ static int kv8_attend(Model* m, const Layer& y, const int* table, const int* len
   k.scale = 1.0f / sqrtf((float)c.head_dim);
   k.lens = lens;
   k.ws = m->kv8_ws; k.ws_bytes = m->kv8_ws_bytes;
+  k.status = gemv_err_word();
   k.pdl = c.use_pdl;
   if (int rc = kv8_attention_launch(k, m->st)) return rc;
   return f16 ? kv8_widen_launch(m->kv8_out, out, (int64_t)rows * ad, c.use_pdl, m->st) : N730_OK;
@@ -1022,15 +1024,15 @@ static int prefill(Model* m, int seq, const int32_t* d_tok, int T, float* d_logi
         if (int rc = kv8_attend(m, y, m->block_table + (size_t)seq * m->max_pages, m->kv8_pos0, m->pqkv, 1, n, m->pattn))
           return rc;
       } else {
-      KVWriteArgs kw = {};
-      kw.qkv = m->pqkv; kw.ld_qkv = m->qkv_dim; kw.cos_t = m->cos_t; kw.sin_t = m->sin_t;
-      kw.block_table = m->block_table + (size_t)seq * m->max_pages; kw.kv = y.kv; kw.d = dims(m);
-      kw.T = n; kw.pos0 = pos0; kw.pdl = c.use_pdl;
-      if (int rc = kv_write_launch(kw, m->st)) return rc;
-      PrefillAttnArgs pa = {};
-      pa.qkv = m->pqkv; pa.ld_qkv = m->qkv_dim; pa.block_table = kw.block_table; pa.kv = y.kv; pa.d = dims(m);
-      pa.T = n; pa.pos0 = pos0; pa.out = m->pattn; pa.pdl = c.use_pdl;
-      if (int rc = attn_prefill_launch(pa, m->st)) return rc;
+        KVWriteArgs kw = {};
+        kw.qkv = m->pqkv; kw.ld_qkv = m->qkv_dim; kw.cos_t = m->cos_t; kw.sin_t = m->sin_t;
+        kw.block_table = m->block_table + (size_t)seq * m->max_pages; kw.kv = y.kv; kw.d = dims(m);
+        kw.T = n; kw.pos0 = pos0; kw.pdl = c.use_pdl;
+        if (int rc = kv_write_launch(kw, m->st)) return rc;
+        PrefillAttnArgs pa = {};
+        pa.qkv = m->pqkv; pa.ld_qkv = m->qkv_dim; pa.block_table = kw.block_table; pa.kv = y.kv; pa.d = dims(m);
+        pa.T = n; pa.pos0 = pos0; pa.out = m->pattn; pa.pdl = c.use_pdl;
+        if (int rc = attn_prefill_launch(pa, m->st)) return rc;
       }
       if (int rc = rowsplit_linear(m, lw.o, m->pattn, ad, n, m->px, h, y.o_bias)) return rc;
       if (int rc = gemv(m, lw.gate_up, m->px, h, n, m->pmlp, c.ffn, y.gate_up_bias, nullptr, 0, y.ln2, 1)) return rc;
@@ -1062,6 +1064,7 @@ N730_API int n730_model_create(const N730ModelConfig* cfg, void** out) {
                c.stream_depth);
   N730_REQUIRE(c.kv_bits == 0 || c.kv_bits == 16 || (c.kv_bits == 8 && (c.page_size <= 0 || c.page_size % KV8_MODEL_BLOCK == 0)),
                N730_BAD_ARG, "model_create: kv_bits %d with pages of %d positions", c.kv_bits, c.page_size);
+  N730_REQUIRE(c.kv_bits != 8 || c.max_batch <= KV8_MAX_BATCH, N730_BAD_ARG, "model_create: kv_bits 8 with a batch of %d", c.max_batch);
   Model* m = new Model();
   m->c = c;
   if (m->c.page_size <= 0) m->c.page_size = 64;

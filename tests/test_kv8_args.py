@@ -140,3 +140,11 @@ def test_reference_codes_round_to_nearest_even():
     want = torch.from_numpy(x).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
     assert np.array_equal(encode(x, "e4m3"), want)
     assert encode(np.float32(1e6), "e4m3") == 126 and encode(np.float32(np.inf), "int8").view(np.int8) == 127
+
+
+def test_model_batch():
+    """A model with an 8-bit cache takes the batches that its attention does."""
+    from n730_b200 import synthetic
+    from n730_b200.engine import Engine
+    with pytest.raises(RuntimeError, match="batch of 4097"):
+        Engine(synthetic.SHAPES["tiny"], max_ctx=64, max_batch=4097, kv_bits=8)
