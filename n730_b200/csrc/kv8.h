@@ -45,9 +45,9 @@ int64_t kv8_attention_ws(const N730KV8Cache& c, int batch, int tokens, int heads
 int64_t kv8_attention_ws_upto(const N730KV8Cache& c, int batch, int tokens, int heads);
 int kv8_attention_launch(const KV8AttnCall& a, cudaStream_t st);
 
-// The tensor-memory kernel for prompts (kv8_prompt.cu): 256 rows of an item a CTA, the positions in
-// `splits` shares whose parts lie as [item tile][split][rg rows].
-struct KV8PromptPlan { int rows, tiles, splits, rg, shares; };  // shares: of the rows, for the weights
+// The tensor-memory kernel for prompts (kv8_prompt.cu): 256 rows of an item a CTA; the positions of the first `tail`
+// tiles are cut into `splits` shares whose parts lie as [item][tail tile][split][rg rows].
+struct KV8PromptPlan { int rows, tiles, tail, splits, rg, shares; };  // shares: of the rows, for the weights
 KV8PromptPlan kv8_prompt_plan(const N730KV8Cache& c, int batch, int tokens, int heads);
 int kv8_prompt_launch(const KV8AttnCall& k, const KV8PromptPlan& p, int* status, float* part, float* part_ml, float* lse,
                       cudaStream_t st);

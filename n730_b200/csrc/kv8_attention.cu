@@ -839,9 +839,9 @@ static KDPlan kd_plan(const N730KV8Cache& c, int batch, int tokens, int heads, i
   if (p.prompt) {
     p.pp = kv8_prompt_plan(c, batch, tokens, heads);
     p.rg = p.pp.rg;
-    p.nrg = p.pp.tiles;
+    p.nrg = p.pp.tail;
     p.part = 256;
-    slots = p.pp.splits > 1 ? items * p.nrg * p.pp.splits : 0;
+    slots = items * p.nrg * p.pp.splits;
   } else {
     // fp32 rows take both terms' products, and up to 8 rows need no second group of columns
     p.rg = dtype == N730_F32 || rows <= 8 ? 8 : 16;
@@ -868,6 +868,9 @@ int kv8_attention_check(const N730KV8Cache* c, int batch, int tokens, int heads)
   // the sequences' tiles are counted in 32 bits on the device
   N730_REQUIRE((int64_t)batch * ((int64_t)c->max_pages * c->page_size / KD_TILE + 1 + KD_ITEM_COST) < (1ll << 31), N730_BAD_ARG,
                "kv8_attention: %d sequences of up to %d pages", batch, c->max_pages);
+  // CTAs of one grid axis
+  N730_REQUIRE((int64_t)batch * tokens * heads <= (1ll << 36), N730_BAD_ARG, "kv8_attention: %d sequences of %d tokens of %d heads",
+               batch, tokens, heads);
   N730_REQUIRE((int64_t)tokens * (heads / c->n_kv) <= (1 << 23), N730_BAD_ARG,
                "kv8_attention: %d tokens of %d heads over %d KV heads", tokens, heads, c->n_kv);
   return N730_OK;

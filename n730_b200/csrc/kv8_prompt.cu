@@ -22,8 +22,8 @@
 //
 // Bounds: per 128x128 tile 2 x 1024 cycles of tensor work for head_dim 128 against 1024 of exp2 and about
 // as many of issue slots on the 4 schedulers, for each of A and B.  Measured: 2048 tokens behind 6144 positions, 64 / 8
-// heads x 128, 614 us, 783 TFLOP/s (0.47 of a large bf16 product): about 2.75k cycles of softmax in a period of
-// 4.6k a tile, and 3.5 waves of CTAs.
+// heads x 128, 575 us, 836 TFLOP/s (0.50 of a large bf16 product): about 2.75k cycles of softmax in a period of
+// 4.6k a tile.
 //
 // Numerics: 16-bit queries are exact in fp16 after a power-of-two scaling of their row; the softmax
 // weights are rounded to fp16 (2^-11 of each, below the rounding of a 16-bit output).  Sums and outputs are
@@ -361,14 +361,14 @@ struct KPArgs {
   int64_t ldq, ldo;
   int dtype, tokens, group, rows, tiles;  // rows = tokens * group; tiles of KP_ROWS rows
   int log_block;
-  int splits;                             // shares of the positions, each a CTA
+  int batch, tail, splits;                // the first `tail` tiles' positions are cut into shares, each a CTA
   int shares;                             // of the rows, for the weights
   bool vec, qvec;                         // out rows, query rows are 16-byte aligned
   float scale_log2e;                      // its absolute value; the sign goes with the queries
   float sign;
   const int* lens; const int* n_new;
   int* status;
-  float* part; float* part_ml;            // [item tile][split][KP_ROWS] rows, as the split kernel's (splits > 1)
+  float* part; float* part_ml;            // [item][tail tile][split][KP_ROWS] rows, as the split kernel's
   float* lse;                             // [batch][n_kv][rows] (may be null)
 };
 
@@ -379,11 +379,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
   KPSmem<HD>& sm = *reinterpret_cast<KPSmem<HD>*>(aligned_smem(kp_raw));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const N730KV8Cache& c = a.c;
-  const int b = blockIdx.z, h = blockIdx.y;
-  const int tile = a.tiles - 1 - (int)blockIdx.x / a.splits, split = (int)blockIdx.x % a.splits;  // the longest first
+  // all items' last tiles first, which see most, the tail's shares at the end
+  const int items = a.batch * c.n_kv, unit = (int)blockIdx.x / items, item = (int)blockIdx.x % items, whole = a.tiles - a.tail;
+  const int b = item / c.n_kv, h = item % c.n_kv;
+  const bool part = unit >= whole;
+  const int splits = part ? a.splits : 1, split = part ? (unit - whole) % a.splits : 0;
+  const int tile = part ? a.tail - 1 - (unit - whole) / a.splits : a.tiles - 1 - unit;
   const int cap = c.max_pages * c.page_size;
   pdl_wait();
-  pdl_launch_dependents();  // the finishing kernel waits for this grid's end
   const int L = kv8_len(a.lens, b, cap), n_new = kv8_new(a.n_new, b, a.tokens);
   const int f0 = tile * KP_ROWS, nrow = min(KP_ROWS, n_new * a.group - f0);
   if (nrow <= 0) return;
@@ -391,7 +394,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
   const int sees_last = (int)min((int64_t)L + (f0 + nrow - 1) / a.group + 1, (int64_t)cap);
   const int sees_all = (int)min((int64_t)L + f0 / a.group + 1, (int64_t)cap);
   const int all_tiles = (sees_last + KP_KEYS - 1) / KP_KEYS;
-  const int j0 = (int)((int64_t)all_tiles * split / a.splits), nt = (int)((int64_t)all_tiles * (split + 1) / a.splits) - j0;
+  const int j0 = (int)((int64_t)all_tiles * split / splits), nt = (int)((int64_t)all_tiles * (split + 1) / splits) - j0;
   const int64_t head = (int64_t)b * c.n_kv + h;
 
   if (tid == 0) {
@@ -647,7 +650,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
     if (go) {
       const float s = l == 0.f ? 0.f : (mo_ref == -INFINITY ? 0.f : ex2(mo_ref - m_ref)) / l;  // a NaN query: NaN
       const int64_t at = ((int64_t)b * a.tokens + f / a.group) * a.ldo + (int64_t)(h * a.group + f % a.group) * HD;
-      const int64_t slot = ((head * a.tiles + tile) * a.splits + split) * KP_ROWS + r;
+      const int64_t slot = ((head * a.tail + tile) * splits + split) * KP_ROWS + r;
 #pragma unroll 1
       for (int cc = 0; cc < HD / 32; ++cc) {
         float v[32];
@@ -658,7 +661,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
           for (int i = 0; i < 32; ++i) v[i] = 0.f;
         }
         if (!live) continue;
-        if (a.splits > 1) {
+        if (part) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
             *reinterpret_cast<float4*>(a.part + slot * HD + cc * 32 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
@@ -683,8 +686,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
           for (int i = 0; i < 32; ++i) kv8_store1(a.out, at + cc * 32 + i, a.dtype, v[i] * s);
         }
       }
-      if (live && a.splits > 1) reinterpret_cast<float4*>(a.part_ml)[slot] = make_float4(mo_ref, m_ref, l, 0.f);
-      if (live && a.lse && a.splits == 1) a.lse[head * a.rows + f] = l == 0.f ? INFINITY : m_ref + log2f(l);
+      if (live && part) reinterpret_cast<float4*>(a.part_ml)[slot] = make_float4(mo_ref, m_ref, l, 0.f);
+      if (live && a.lse && !part) a.lse[head * a.rows + f] = l == 0.f ? INFINITY : m_ref + log2f(l);
     }
   }
   tc_fence_before();
@@ -891,14 +894,18 @@ KV8PromptPlan kv8_prompt_plan(const N730KV8Cache& c, int batch, int tokens, int 
   p.rows = tokens * (heads / c.n_kv);
   p.tiles = (p.rows + KP_ROWS - 1) / KP_ROWS;
   p.rg = KP_ROWS;
-  const int64_t ctas = (int64_t)batch * c.n_kv * p.tiles;
+  const int64_t items = (int64_t)batch * c.n_kv;
   const int64_t key_tiles = ((int64_t)c.max_pages * c.page_size + KP_KEYS - 1) / KP_KEYS;
   // CTAs of a cluster that share the rows of 128 positions' weights, two row tiles each at least
-  const int64_t idle = num_sms() / std::max<int64_t>(1, (int64_t)batch * c.n_kv * key_tiles);
+  const int64_t idle = num_sms() / (items * key_tiles);
   p.shares = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(KW_SHARES, idle), p.rows / (2 * KP_KEYS)));
-  // shares of the positions while the SMs would stand idle, of four tiles at least
+  // The last, partial wave of CTAs (or the only one) leaves SMs idle: its tiles' positions are cut into as many shares
+  // as there are SMs, of four tiles at least.  2048 tokens behind 6144 positions, 64 / 8 heads, 3.46 waves: 614 us
+  // without, 575 with.
   p.splits = 1;
-  while (ctas * (p.splits + 1) <= num_sms() && key_tiles / (p.splits + 1) >= 4) ++p.splits;
+  const int64_t tail = (items * p.tiles % num_sms() + items - 1) / items;
+  while (tail && tail * items * (p.splits + 1) <= num_sms() && key_tiles / (p.splits + 1) >= 4) ++p.splits;
+  p.tail = p.splits > 1 ? (int)tail : 0;
   return p;
 }
 
@@ -906,7 +913,7 @@ static KPArgs kp_args(const KV8AttnCall& k, const KV8PromptPlan& p, int* status,
   KPArgs a{};
   a.c = k.c;
   a.q = k.q; a.out = k.out; a.ldq = k.ldq; a.ldo = k.ldo; a.dtype = k.dtype;
-  a.tokens = k.tokens; a.group = k.heads / k.c.n_kv; a.rows = p.rows; a.tiles = p.tiles; a.splits = p.splits; a.shares = p.shares;
+  a.tokens = k.tokens; a.group = k.heads / k.c.n_kv; a.rows = p.rows; a.tiles = p.tiles; a.splits = p.splits; a.tail = p.tail; a.batch = k.batch; a.shares = p.shares;
   a.vec = ((uintptr_t)k.out & 15) == 0 && k.ldo * kv8_esize(k.dtype) % 16 == 0;
   a.qvec = ((uintptr_t)k.q & 15) == 0 && k.ldq * kv8_esize(k.dtype) % 16 == 0;
   a.scale_log2e = fabsf(k.scale) * 1.4426950408889634f;
@@ -918,10 +925,10 @@ static KPArgs kp_args(const KV8AttnCall& k, const KV8PromptPlan& p, int* status,
 }
 
 template <int HD, int CODE>
-static int prompt_launch(const KPArgs& a, int batch, bool pdl, cudaStream_t st) {
+static int prompt_launch(const KPArgs& a, bool pdl, cudaStream_t st) {
   const size_t smem = sizeof(KPSmem<HD>) + 1024;
   if (int rc = smem_attr_once<kv8_prompt_kernel<HD, CODE>>((int)smem)) return rc;
-  return kv8_launch(kv8_prompt_kernel<HD, CODE>, dim3(a.tiles * a.splits, a.c.n_kv, batch), dim3(KP_THREADS), smem, st, pdl, a);
+  return kv8_launch(kv8_prompt_kernel<HD, CODE>, dim3((a.tiles + a.tail * (a.splits - 1)) * a.batch * a.c.n_kv), dim3(KP_THREADS), smem, st, pdl, a);
 }
 template <int HD, int CODE>
 static int prompt_weights_launch(const KPArgs& a, const KV8AttnCall& k, cudaStream_t st) {
@@ -937,8 +944,8 @@ int kv8_prompt_launch(const KV8AttnCall& k, const KV8PromptPlan& p, int* status,
   const KPArgs a = kp_args(k, p, status, part, part_ml, lse);
   const bool i8 = k.c.code == N730_KV8_INT8;
   if (k.c.head_dim == 128)
-    return i8 ? prompt_launch<128, N730_KV8_INT8>(a, k.batch, k.pdl, st) : prompt_launch<128, N730_KV8_E4M3>(a, k.batch, k.pdl, st);
-  return i8 ? prompt_launch<64, N730_KV8_INT8>(a, k.batch, k.pdl, st) : prompt_launch<64, N730_KV8_E4M3>(a, k.batch, k.pdl, st);
+    return i8 ? prompt_launch<128, N730_KV8_INT8>(a, k.pdl, st) : prompt_launch<128, N730_KV8_E4M3>(a, k.pdl, st);
+  return i8 ? prompt_launch<64, N730_KV8_INT8>(a, k.pdl, st) : prompt_launch<64, N730_KV8_E4M3>(a, k.pdl, st);
 }
 
 int kv8_prompt_weights_launch(const KV8AttnCall& k, const KV8PromptPlan& p, int* status, float* lse, cudaStream_t st) {

@@ -244,6 +244,7 @@ def test_several_tokens(code, dtype, kv, heads, dim, T, lens, new):
     ("e4m3", "bf16", 1, 14, 64, 48, 40, [2900, 700, 0], [40, 3, 0]),        # pages of three blocks
     ("int8", "bf16", 2, 8, 64, 16, 130, [1111], None),
     ("int8", "f16", 1, 65, 128, 128, 1, [1500, 0, 127], None),              # one token of many heads
+    ("int8", "f16", 4, 64, 64, 64, 300, [740, 0], None),                    # shares in a last, partial wave of CTAs
     ("e4m3", "f16", 8, 32, 64, 64, 160, [900, 0, 129, 511], [160, 160, 0, 97])])
 def test_prompts_over_many_tiles(code, dtype, kv, heads, dim, page, T, lens, new):
     """Chunks far into a context, with the positions in shares where there are few rows; scores that

@@ -100,6 +100,7 @@ def test_attention_arguments():
     refused(call(w_out=A + 1), -13)
     refused(lambda: cache(max_pages=1 << 20).attention_workspace(4096, 1, 2), -13)  # 2^31 tiles
     refused(lambda: cache(n_kv=1).attention_workspace(1, 1, 8193), -13)
+    refused(lambda: cache().attention_workspace(4096, 1 << 20, 18), -13)  # more rows than a grid has CTAs for
     refused(call(scale=float("inf")), -13)
     assert c.lib.n730_kv8_attention(c._ref, A, 7, 896, 2, 3, 14, 1.0, A, None, A, 896, None, None, 0, A, need, None) == -13
 
