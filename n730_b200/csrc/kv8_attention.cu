@@ -144,13 +144,9 @@ __device__ __forceinline__ bool wait_copies(uint64_t* bar, uint32_t parity, bool
     if (lost || now() - t0 > KD_WAIT_NS) return false;
   return true;
 }
-template <int BYTES>
-__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool pred) {
-  if (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(pred ? 16 : 0) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" :: "r"(dst), "l"(src), "n"(BYTES), "r"(pred ? BYTES : 0)
-                 : "memory");
+// 4 bytes, or zeros
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool pred) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" :: "r"(dst), "l"(src), "r"(pred ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -318,7 +314,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
     if (lane < 4) {
       const int row = lane < 2 ? row0 : row1;
       const float* s = ((lane & 1) ? c.v_scales : c.k_scales) + (max(row, 0) >> a.log_block);
-      cp_async<4>(smem_u32(&sm.sc[warp][st][lane]), s, row >= 0);
+      cp_async4(smem_u32(&sm.sc[warp][st][lane]), s, row >= 0);
     }
   };
   // the warp's rows of a run's queries: asked for a run ahead and ahead of tiles (two row groups

@@ -109,8 +109,10 @@ __device__ __forceinline__ uint32_t pack4_e4m3(float a, float b, float c, float 
   return lo | (hi << 16);
 }
 __device__ __forceinline__ uint32_t pack4_int8(float a, float b, float c, float d) {
-  auto q = [](float y) { return (uint32_t)min(max(__float2int_rn(y), -127), 127) & 0xffu; };  // NaN -> 0
-  return q(a) | (q(b) << 8) | (q(c) << 16) | (q(d) << 24);
+  // + 1.5 * 2^23 rounds to an integer, ties to even, and leaves it in the low byte: conversions to and from integers run
+  // at a quarter of this rate and bounded the eviction (moving 32 x 8 heads to 2048 slots 55 us)
+  auto q = [](float y) { return __float_as_uint(__fadd_rn(fminf(fmaxf(y, -127.f), 127.f), 12582912.f)); };
+  return __byte_perm(__byte_perm(q(a), q(b), 0x0040), __byte_perm(q(c), q(d), 0x0040), 0x5410);
 }
 template <int CODE>
 __device__ __forceinline__ uint4 kv8_pack(const float (&y)[16]) {
@@ -127,8 +129,10 @@ __device__ __forceinline__ void kv8_unpack(const uint4& c, float (&y)[16]) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     if (CODE == N730_KV8_INT8) {
+      // 128 + q in the low byte of 2^23 is 2^23 + 128 + q
+      const uint32_t u = w[e] ^ 0x80808080u;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) y[4 * e + k] = (float)(int8_t)(w[e] >> (8 * k));
+      for (int k = 0; k < 4; ++k) y[4 * e + k] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + k)) - 8388736.f;
     } else {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
