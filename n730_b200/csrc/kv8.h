@@ -57,6 +57,28 @@ int kv8_prompt_weights_launch(const KV8AttnCall& k, const KV8PromptPlan& p, int*
 // compiler would lose sight of the address space and fall back to generic loads and stores.
 __device__ __forceinline__ uint8_t* aligned_smem(uint8_t* raw) { return raw + ((0u - smem_u32(raw)) & 1023u); }
 
+// a * b + c, a + b and a * b of two fp32 pairs
+__device__ __forceinline__ float2 fma2(const float2& a, const float2& b, const float2& c) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(const float2& a, const float2& b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 w, x, y;\n"
+      " mov.b64 {%0, %1}, w;\n}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(const float2& a, const float2& b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 w, x, y;\n"
+      " mov.b64 {%0, %1}, w;\n}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
 // one element of a row in the caller's type, widened to fp32
 __device__ __forceinline__ float kv8_load1(const void* p, int64_t i, int dtype) {
   if (dtype == N730_F32) return reinterpret_cast<const float*>(p)[i];

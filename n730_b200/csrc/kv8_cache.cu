@@ -108,11 +108,12 @@ __device__ __forceinline__ uint32_t pack4_e4m3(float a, float b, float c, float 
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
   return lo | (hi << 16);
 }
+// Of values that round to -127 .. 127.  + 1.5 * 2^23 rounds to an integer, ties to even, and leaves it in the low byte:
+// conversions to and from integers run at a quarter of this rate and bounded the eviction.
 __device__ __forceinline__ uint32_t pack4_int8(float a, float b, float c, float d) {
-  // + 1.5 * 2^23 rounds to an integer, ties to even, and leaves it in the low byte: conversions to and from integers run
-  // at a quarter of this rate and bounded the eviction (moving 32 x 8 heads to 2048 slots 55 us)
-  auto q = [](float y) { return __float_as_uint(__fadd_rn(fminf(fmaxf(y, -127.f), 127.f), 12582912.f)); };
-  return __byte_perm(__byte_perm(q(a), q(b), 0x0040), __byte_perm(q(c), q(d), 0x0040), 0x5410);
+  const float2 x = add2(make_float2(a, b), both(12582912.f)), y = add2(make_float2(c, d), both(12582912.f));
+  return __byte_perm(__byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x0040),
+                     __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x0040), 0x5410);
 }
 template <int CODE>
 __device__ __forceinline__ uint4 kv8_pack(const float (&y)[16]) {
@@ -132,7 +133,11 @@ __device__ __forceinline__ void kv8_unpack(const uint4& c, float (&y)[16]) {
       // 128 + q in the low byte of 2^23 is 2^23 + 128 + q
       const uint32_t u = w[e] ^ 0x80808080u;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) y[4 * e + k] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + k)) - 8388736.f;
+      for (int k = 0; k < 4; k += 2) {
+        const float2 f = add2(make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + k)),
+                                          __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441 + k))), both(-8388736.f));
+        y[4 * e + k] = f.x; y[4 * e + k + 1] = f.y;
+      }
     } else {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -150,32 +155,35 @@ __device__ __forceinline__ void kv8_unpack(const uint4& c, float (&y)[16]) {
 // scales take the division (which cost more than the row's memory traffic: 4096 rows of 8 heads 13.9 us).
 template <int CODE>
 __device__ __forceinline__ uint4 kv8_encode(const float (&x)[16], float s) {
+  constexpr float top = CODE == N730_KV8_INT8 ? 127.f : 448.f;
   float y[16];
   if (s >= 0x1p-60f && s <= 0x1p60f && (__float_as_uint(s) & 0x7fffffu) != 0x7fffffu) {
-    const float r = __frcp_rn(s), most = 1024.f * s;  // past the largest code either way
+    const float r = __frcp_rn(s), most = top * s;  // its quotient rounds to top, as those past it do
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float v = x[e] == x[e] ? fminf(fmaxf(x[e], -most), most) : 0.f;
-      const float q = __fmul_rn(v, r);
-      y[e] = __fmaf_rn(__fmaf_rn(-q, s, v), r, q);
+    for (int e = 0; e < 16; e += 2) {
+      float2 v;
+      v.x = x[e] == x[e] ? fminf(fmaxf(x[e], -most), most) : 0.f;
+      v.y = x[e + 1] == x[e + 1] ? fminf(fmaxf(x[e + 1], -most), most) : 0.f;
+      const float2 q = mul2(v, both(r)), z = fma2(fma2(make_float2(-q.x, -q.y), both(s), v), both(r), q);
+      y[e] = z.x; y[e + 1] = z.y;
     }
   } else {
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const float v = x[e] == x[e] ? x[e] : 0.f;
-      y[e] = s > 0.f ? __fdiv_rn(v, s) : 0.f;
+      y[e] = s > 0.f ? fminf(fmaxf(__fdiv_rn(v, s), -top), top) : 0.f;
     }
   }
   return kv8_pack<CODE>(y);
 }
-// the code values of a scale `from` on a scale `to`
+// the code values of a scale `from` on a scale `to`, which is not smaller
 template <int CODE>
 __device__ __forceinline__ uint4 kv8_recode(const uint4& c, float from, float to) {
   const float r = __fdiv_rn(from, to > 0.f ? to : 1.f);
   float y[16];
   kv8_unpack<CODE>(c, y);
 #pragma unroll
-  for (int e = 0; e < 16; ++e) y[e] = __fmul_rn(y[e], r);
+  for (int e = 0; e < 16; ++e) y[e] = __fmul_rn(y[e], r);  // a packed product is fused with the addition that rounds it
   return kv8_pack<CODE>(y);
 }
 __device__ __forceinline__ float kv8_amax(const float (&x)[16]) {
@@ -338,7 +346,7 @@ __global__ void __launch_bounds__(KV8_THREADS) kv8_read_kernel(const KV8ReadArgs
     float y[16];
     kv8_unpack<CODE>(q[i], y);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) y[e] = row[i] >= 0 ? y[e] * s[i] : 0.f;
+    for (int e = 0; e < 16; ++e) y[e] = row[i] >= 0 ? y[e] * s[i] : 0.f;  // 0 x 0 is slower: 65.3 us for 63.0
     kv8_store16(which ? a.y[1] : a.y[0], ((int64_t)b * a.tokens + t) * a.ld + (int64_t)h * HD + chunk * 16, a.dtype, a.vec, y);
   }
 }
@@ -361,7 +369,8 @@ __global__ void __launch_bounds__(KV8_THREADS) kv8_read_kernel(const KV8ReadArgs
 // them again), the keep-th largest is found 11 bits at a time, and ranks of ties, holes and movers come
 // from ballots: a warp owns a run of slots, one scan over the warps' counts a pass.
 // 2304 slots of 4 heads take 14 us, all latency; 8192 of 256 rows 32 us in two waves of CTAs (two CTAs an SM, at 32
-// registers, lost 2 us).  The move is bound by HBM: 32 x 8 heads cut from up to 8192 slots to 2048, 52 to 62 us.
+// registers, lost 2 us).  The move is bound by the arithmetic on codes (80 % of the issue slots): 32 x 8 heads cut from
+// up to 8192 slots to 2048, about 43 us; 55 with conversions to and from integers.
 struct KV8EvictArgs {
   N730KV8Cache c;
   int keep, first, recent, log_block;

@@ -189,21 +189,6 @@ __device__ __forceinline__ void kp_put_codes(const uint4& x, uint8_t* rowp, int 
   *reinterpret_cast<uint4*>(rowp + (at ^ 16)) = swap ? make_uint4(y[0], y[1], y[2], y[3]) : make_uint4(y[4], y[5], y[6], y[7]);
 }
 
-// a * b + c and a + b of two fp32 pairs
-__device__ __forceinline__ float2 fma2(const float2& a, const float2& b, const float2& c) {
-  float2 d;
-  asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
-      " fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 add2(const float2& a, const float2& b) {
-  float2 d;
-  asm("{\n .reg .b64 x, y, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 w, x, y;\n"
-      " mov.b64 {%0, %1}, w;\n}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-
 // 8 consecutive columns of this thread's TMEM lane multiplied by f
 __device__ __forceinline__ void tc_scale8(uint32_t taddr, float f) {
   float v[8];
