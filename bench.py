@@ -245,13 +245,15 @@ class CpuReferenceDecoder:
     the values).
     """
 
+    CORE = REPO / "oracle" / "_ref" / "n730core.so"
+
     def __init__(self, shape, ctx, threads=None, ahead=16, seed=0):
         import ctypes as C
         import struct
         import tempfile
         from concurrent.futures import ThreadPoolExecutor
 
-        core_so = REPO / "oracle" / "_ref" / "n730core.so"
+        core_so = self.CORE
         if not core_so.exists():
             raise FileNotFoundError("oracle/_ref/n730core.so missing (built by __graft_entry__.build)")
         self.C = C
@@ -589,7 +591,9 @@ def run_ours(a):
                                 f"every linear, prompt in chunks of {a.prefill_chunk} tokens; wall clock incl. host calls, "
                                 "after one untimed prefill"},
         }
-        if not a.no_cpu_baseline and headline:
+        if not a.no_cpu_baseline and headline and not CpuReferenceDecoder.CORE.exists():
+            out["cpu_baseline"] = {"unavailable": "oracle/_ref/n730core.so is not built (it needs the reference's source)"}
+        elif not a.no_cpu_baseline and headline:
             cs = CpuReferenceDecoder(shape, ctx)
             cs.step()
             t0 = time.perf_counter()
