@@ -886,7 +886,7 @@ KV8PromptPlan kv8_prompt_plan(const N730KV8Cache& c, int batch, int tokens, int 
   p.shares = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(KW_SHARES, idle), p.rows / (2 * KP_KEYS)));
   // The last, partial wave of CTAs (or the only one) leaves SMs idle: its tiles' positions are cut into as many shares
   // as there are SMs, of four tiles at least.  2048 tokens behind 6144 positions, 64 / 8 heads, 3.46 waves: 614 us
-  // without, 575 with.
+  // without, 575 with; shares of three tiles (4 prompts of 300 tokens, 700 positions) 49.8 us for 42.3 without.
   p.splits = 1;
   const int64_t tail = (items * p.tiles % num_sms() + items - 1) / items;
   while (tail && tail * items * (p.splits + 1) <= num_sms() && key_tiles / (p.splits + 1) >= 4) ++p.splits;
