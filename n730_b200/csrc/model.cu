@@ -669,8 +669,9 @@ static int finalize(Model* m) {
   m->pool_pages = (int)pages;
   const size_t per_layer = pages * c.kv_heads * c.page_size * c.head_dim;
   if (c.kv_bits == 8) {
-    // a layer: codes of K and V, then their scales
-    const size_t scales = per_layer / c.head_dim / KV8_MODEL_BLOCK, layer_bytes = 2 * (per_layer + scales * sizeof(float));
+    // a layer: codes of K and V, then their scales; the next one's codes start on a boundary that their copies ask for
+    const size_t scales = per_layer / c.head_dim / KV8_MODEL_BLOCK;
+    const size_t layer_bytes = (2 * (per_layer + scales * sizeof(float)) + 255) / 256 * 256;
     uint8_t* pool = nullptr;
     if (int rc = m->alloc(&pool, layer_bytes * nl)) return rc;
     N730_CUDA(cudaMemsetAsync(pool, 0, layer_bytes * nl, m->st));

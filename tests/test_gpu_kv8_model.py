@@ -132,6 +132,30 @@ def test_batcher_reuses_pages(model):
     e.close()
 
 
+@pytest.fixture(scope="module")
+def odd_model(tmp_path_factory):
+    """One KV head, three layers."""
+    shape = synthetic.ModelShape(256, 3, 4, 1, 64, 512, 1000, 1e6, 1e-6, False)
+    path = tmp_path_factory.mktemp("m8odd") / "odd.n730"
+    synthetic.write_n730(path, shape, "int4_g128", seed=6)
+    blocks = _blocks(path)
+    return shape, blocks, _oracle_weights(blocks)
+
+
+@pytest.mark.parametrize("page,pool", [(16, 33), (48, 11), (80, 0)])
+def test_odd_pools(odd_model, page, pool):
+    """Pages, heads and blocks whose product is odd: every layer's codes still lie where copies can start."""
+    shape, blocks, w = odd_model
+    e = _engine(shape, blocks, page_size=page, kv_pool_pages=pool, max_batch=1)
+    orc = Oracle8(shape, w, 512)
+    rng = np.random.default_rng(page)
+    prompt = rng.integers(0, shape.vocab, 90)
+    assert rel_err(e.forward(prompt), orc.forward(prompt)) <= TOL
+    for tok in rng.integers(0, shape.vocab, 3):
+        assert rel_err(e.decode([tok])[0], orc.forward([tok])) <= TOL
+    e.close()
+
+
 def test_refused_configurations():
     shape = synthetic.SHAPES["tiny"]
     for kw in (dict(kv_bits=4), dict(kv_bits=8, page_size=24), dict(kv_bits=-8)):
