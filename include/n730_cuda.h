@@ -208,8 +208,9 @@ int64_t n730_kv8_attention_ws(const N730KV8Cache* c, int batch, int tokens, int 
  * n730_kv8_append with the same d_lens and d_new.  d_q and d_out rows are [n_heads][head_dim]
  * (query head i reads KV head i / (n_heads / n_kv)); out rows from d_new[b] on are left as they
  * were; a query that sees no position gives zeros.  d_out must not overlap d_q.  Scores are scaled
- * by `scale`.  16-bit rows round the softmax weights to fp16, and more than 64 rows of a KV head run
- * on the tcgen05 tensor cores; fp32 rows keep fp32 accuracy and run 64 rows of a KV head at a time.
+ * by `scale`.  16-bit rows round softmax weight x V scale to fp16 (by 2^-11 of each, and not below 2^-32
+ * of the row's largest), and more than 64 rows of a KV head run on the tcgen05 tensor cores; fp32 rows keep
+ * 2^-22 of each, not below 2^-38 of the row's largest, and run 64 rows of a KV head at a time.
  * d_w_out (may be null) [batch][n_kv][ldw]: for positions below d_lens[b] + d_new[b], d_w (null:
  * zeros; may equal d_w_out) plus the softmax weights summed over the KV head's queries; positions
  * that are new count from zero.  ldw >= max_pages * page_size. */

@@ -90,6 +90,10 @@ __device__ __forceinline__ void kv8_store1(void* p, int64_t i, int dtype, float 
   else if (dtype == N730_F16) reinterpret_cast<__half*>(p)[i] = __float2half_rn(x);
   else reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
 }
+// Softmax weight x V scale (P) is fp16 against a reference: log2 of where a new reference puts the largest P, and of how
+// large P may grow before the reference moves (fp16 ends at 2^16).  What lies below goes down to fp16's smallest normal,
+// 2^-14, at full accuracy: 2^-21 of the largest.
+constexpr float KV8_P_NEW = 7.f, KV8_P_MOST = 15.f;
 // V scales below this count as 0: quotients by them would leave fp32's range
 constexpr float KV8_TINY = 0x1p-100f;
 // whether pointers lie on whole elements of `size` bytes (null ones do)

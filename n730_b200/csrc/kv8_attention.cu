@@ -26,12 +26,14 @@
 //
 // Softmax.  Weights are kept against a reference that follows the maximum only when a score is more
 // than 2^8 above it, so a tile costs one vote and no reduction; a second reference does the same for
-// weight x V scale, which has to fit fp16 whatever the scales are.
+// weight x V scale (P), which has to fit fp16 whatever the scales are: the largest P so far lies between 2^KV8_P_NEW
+// (fp32 rows: 2^KD_P_NEW_LO), where a new reference puts it, and 2^KV8_P_MOST, where the reference moves.
 //
 // Numerics.  Queries are scaled by a power of two per row so that a 16-bit query is exact in fp16; an
-// fp32 query is split into two fp16 terms, and so is P: fp32 calls lose about 2^-22.  For 16-bit calls P
-// is rounded to fp16 (2^-11 of each weight, below the rounding of the output).  Maxima, sums and
-// outputs are fp32.
+// fp32 query is split into two fp16 terms, and so is P, which loses 2^-22 of each down to 2^-16 of a warp's largest P and
+// 2^-38 of that largest below (fp16's smallest step under 2^13).  For 16-bit calls P is rounded to fp16: 2^-11 of each,
+// below the rounding of the output, down to 2^-21 of the largest, 2^-32 of the largest below.  Maxima, sums and outputs
+// are fp32.
 //
 // Bound by HBM: 2 head_dim code bytes and 8 / block of scales a position and KV head.  Whole calls: 128 sequences
 // ragged to 4096, 64 / 8 heads x 128, e4m3, 113.5 us (5.36 TB/s); one of 65501 positions 36.4 us, of which 5 start
@@ -56,7 +58,8 @@ constexpr int KD_CTAS_PER_SM = 3;
 // 52.7, 53.2, 54.7.
 constexpr int KD_ITEM_COST = 16;
 constexpr int KD_MIN_UNITS = 4;  // tiles of a run: fewer would leave warps idle and joins to do
-constexpr float KD_SLACK = 8.f;  // log2 of how far a weight may exceed its reference
+constexpr float KD_SLACK = 8.f;  // log2 of how far a weight in the sum (fp32) may exceed its reference
+constexpr float KD_P_NEW_LO = 13.f;  // as KV8_P_NEW for two-term P, whose second term runs out of fp16's range first
 constexpr uint64_t KD_WAIT_NS = 1000000000;  // bound of a wait for copies
 
 struct KDArgs {
@@ -174,12 +177,13 @@ __device__ __forceinline__ int kd_owner(int64_t u, int64_t U, int64_t N) { retur
 // The answer of row f, channels d..d + 3: sums of weight x V against Mo, of weights l against M.
 template <int HD>
 __device__ __forceinline__ void kd_answer(const KDArgs& a, int b, int h, int f, int d, const float4& num, float Mo, float M, float l) {
-  const float s = l == 0.f ? 0.f : (Mo == -INFINITY ? 0.f : ex2(Mo - M)) / l;  // a NaN query: NaN
+  // by two factors, whose product may leave fp32's normal range when the answer does not; a NaN query: NaN
+  const float s = l == 0.f ? 0.f : 1.f / l, f2 = l == 0.f || Mo == -INFINITY ? 0.f : ex2(Mo - M);
   const int64_t at = ((int64_t)b * a.tokens + a.t0 + f / a.group) * a.ldo + (int64_t)(h * a.group + f % a.group) * HD + d;
-  kv8_store1(a.out, at, a.dtype, num.x * s);
-  kv8_store1(a.out, at + 1, a.dtype, num.y * s);
-  kv8_store1(a.out, at + 2, a.dtype, num.z * s);
-  kv8_store1(a.out, at + 3, a.dtype, num.w * s);
+  kv8_store1(a.out, at, a.dtype, num.x * s * f2);
+  kv8_store1(a.out, at + 1, a.dtype, num.y * s * f2);
+  kv8_store1(a.out, at + 2, a.dtype, num.z * s * f2);
+  kv8_store1(a.out, at + 3, a.dtype, num.w * s * f2);
 }
 
 // NB: 8-row groups of an item's rows worked on together; LO: fp32 rows in two fp16 terms.
@@ -187,6 +191,7 @@ template <int HD, int CODE, int NB, bool LO>
 __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(const KDArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using G = KDGeom<HD>;
   constexpr int RG = 8 * NB, KS = HD / 16, MT = HD / 16, ST = KD_STAGES;
+  constexpr float P_NEW = LO ? KD_P_NEW_LO : KV8_P_NEW;
   constexpr int TT = NB == 1 ? 2 : 1;  // halves of a tile worked on together: independent chains for the tensor cores
   extern __shared__ __align__(1024) uint8_t kd_raw[];
   KDSmem<HD>& sm = *reinterpret_cast<KDSmem<HD>*>(aligned_smem(kd_raw));
@@ -481,7 +486,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
             }
         }
       }
-      // ---- move the references when a weight would exceed them by 2^KD_SLACK ----
+      // ---- move the references when a weight would be too large against them ----
       bool move = false;
 #pragma unroll
       for (int n = 0; n < NB; ++n)
@@ -494,14 +499,14 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
             mx = fmaxf(mx, x);
             mv = fmaxf(mv, x + lv[tt]);
           }
-          move |= mx > m_ref[n][e] + KD_SLACK || mv > mo_ref[n][e] + KD_SLACK;
+          move |= mx > m_ref[n][e] + KD_SLACK || mv > mo_ref[n][e] + KV8_P_MOST;
         }
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float mx = m_ref[n][e], mv = mo_ref[n][e];
+            float mx = m_ref[n][e], mv = -INFINITY;
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt) {
               const float x = fmaxf(y[tt][n][e], y[tt][n][e + 2]);
@@ -513,6 +518,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
               mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, k));
             }
+            mv = fmaxf(mo_ref[n][e], mv - P_NEW);
             if (mx != m_ref[n][e]) {  // from -infinity: the sums are still 0
               l_run[n][e] *= ex2(m_ref[n][e] - mx);
               m_ref[n][e] = mx;

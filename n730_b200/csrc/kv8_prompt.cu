@@ -17,8 +17,8 @@
 //
 // Softmax.  The weight x V scale of a position is formed by one FMA and one exp2: its exponent is
 // score * (row, block factor) + lv - reference with lv the approximate log2(V scale), and the sum of
-// weights gets each block's sum times 2^(reference - maximum - lv).  Both references follow the largest values lazily (2^8 of
-// slack), so outputs in tensor memory are rescaled only when a row's maximum has grown by that much.
+// weights gets each block's sum times 2^(reference - maximum - lv).  Both references follow the largest values lazily (P
+// grows from 2^KV8_P_NEW to 2^KV8_P_MOST meanwhile), so outputs in tensor memory are rescaled only when a row's maximum has grown by that much.
 //
 // Bounds: per 128x128 tile 2 x 1024 cycles of tensor work for head_dim 128 against 1024 of exp2 and about
 // as many of issue slots on the 4 schedulers, for each of A and B.  Measured: 2048 tokens behind 6144 positions, 64 / 8
@@ -26,8 +26,8 @@
 // 4.6k a tile.
 //
 // Numerics: 16-bit queries are exact in fp16 after a power-of-two scaling of their row; the softmax
-// weights are rounded to fp16 (2^-11 of each, below the rounding of a 16-bit output).  Sums and outputs are
-// fp32.  fp32 queries do not come here.
+// weights are rounded to fp16 (2^-11 of each, below the rounding of a 16-bit output, down to 2^-21 of the largest weight
+// x V scale; 2^-32 of that largest below).  Sums and outputs are fp32.  fp32 queries do not come here.
 // Every wait is bounded; one that runs out sets the workspace's status word, ends the CTA's work and
 // still frees the tensor memory.
 #include "kv8.h"
@@ -44,8 +44,7 @@ constexpr int KP_CODE_WARPS = 3, KP_MMA_WARP = 11;
 constexpr int KW_ROW_WARPS = 8, KW_MMA_WARP = 8 + KW_ROW_WARPS, KW_THREADS = (KW_MMA_WARP + 1) * 32;
 constexpr int KW_SHARES = 8;      // most CTAs of a cluster
 constexpr int KP_RING = 4;        // tiles whose scales are kept: two more than tiles of codes
-constexpr float KP_SLACK = 8.f;   // log2 of how far a weight x V scale may exceed its reference (fp16: 2^16)
-constexpr float KP_SUM_SLACK = 64.f;  // and of how far a weight in the sum (fp32)
+constexpr float KP_SUM_SLACK = 64.f;  // log2 of how far a weight in the sum (fp32) may exceed its reference
 // V scales and references this close leave weight x V scale and the way back to the weight inside fp32's range
 constexpr float KP_NEAR_MIN = 0x1p-24f, KP_NEAR_MAX = 0x1p24f, KP_NEAR_REFS = 40.f, KP_NEAR_BACK = 0x1p64f;
 
@@ -222,11 +221,11 @@ __device__ __forceinline__ void tc_ld64(uint32_t taddr, float* v) {
   for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// Moves a row's references to the largest score mx and the largest score + log2(V scale) mv of a tile where those
-// are larger; sums and, when there are any, outputs (at to) are rescaled.  A warp at a time.
+// Moves a row's references to the largest score mx of a tile, and to where its largest score + log2(V scale) mv becomes
+// a P of 2^KV8_P_NEW, where those are larger; sums and, when there are any, outputs (at to) are rescaled.  A warp at a time.
 template <int HD>
 __device__ __forceinline__ void kp_move(uint32_t to, bool outputs, float mx, float mv, float& m_ref, float& mo_ref, float& l) {
-  const float mn = fmaxf(m_ref, mx), mon = fmaxf(mo_ref, mv);
+  const float mn = fmaxf(m_ref, mx), mon = fmaxf(mo_ref, mv - KV8_P_NEW);
   if (mn != m_ref) l *= ex2(m_ref - mn);
   const float f = mon != mo_ref ? ex2(mo_ref - mon) : 1.f;
   m_ref = mn;
@@ -255,7 +254,7 @@ __device__ __forceinline__ void kp_softmax(uint32_t ts, uint32_t to, const float
     mx = fmaxf(mx, y);
     mv = fmaxf(mv, y + lvs[blk]);
   }
-  if (__any_sync(0xffffffffu, mx > m_ref + KP_SUM_SLACK || mv > mo_ref + KP_SLACK))
+  if (__any_sync(0xffffffffu, mx > m_ref + KP_SUM_SLACK || mv > mo_ref + KV8_P_MOST))
     kp_move<HD>(to, outputs, mx, mv, m_ref, mo_ref, l);
   const float mos = mo_ref == -INFINITY ? 0.f : mo_ref, ms = m_ref == -INFINITY ? 0.f : m_ref, back0 = ex2(mos - ms);
 #pragma unroll
@@ -299,7 +298,7 @@ __device__ __forceinline__ void kp_softmax_any(uint32_t ts, uint32_t to, const f
       mv = fmaxf(mv, y + lvs[2 * cc + e]);
     }
   }
-  if (__any_sync(0xffffffffu, mx > m_ref + KP_SUM_SLACK || mv > mo_ref + KP_SLACK))
+  if (__any_sync(0xffffffffu, mx > m_ref + KP_SUM_SLACK || mv > mo_ref + KV8_P_MOST))
     kp_move<HD>(to, outputs, mx, mv, m_ref, mo_ref, l);
   const float mos = mo_ref == -INFINITY ? 0.f : mo_ref, ms = m_ref == -INFINITY ? 0.f : m_ref, back0 = ex2(mos - ms);
 #pragma unroll 1
@@ -633,7 +632,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
       tc_fence_after();
     }
     if (go) {
-      const float s = l == 0.f ? 0.f : (mo_ref == -INFINITY ? 0.f : ex2(mo_ref - m_ref)) / l;  // a NaN query: NaN
+      // by two factors, whose product may leave fp32's normal range when the answer does not; a NaN query: NaN
+      const float s = l == 0.f ? 0.f : 1.f / l, f2 = l == 0.f || mo_ref == -INFINITY ? 0.f : ex2(mo_ref - m_ref);
       const int64_t at = ((int64_t)b * a.tokens + f / a.group) * a.ldo + (int64_t)(h * a.group + f % a.group) * HD;
       const int64_t slot = ((head * a.tail + tile) * splits + split) * KP_ROWS + r;
 #pragma unroll 1
@@ -656,7 +656,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float y0 = v[i + 2 * e] * s, y1 = v[i + 2 * e + 1] * s;
+              const float y0 = v[i + 2 * e] * s * f2, y1 = v[i + 2 * e + 1] * s * f2;
               if (a.dtype == N730_F16) {
                 w[e] = h2u(__floats2half2_rn(y0, y1));
               } else {
@@ -668,7 +668,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) kv8_store1(a.out, at + cc * 32 + i, a.dtype, v[i] * s);
+          for (int i = 0; i < 32; ++i) kv8_store1(a.out, at + cc * 32 + i, a.dtype, v[i] * s * f2);
         }
       }
       if (live && part) reinterpret_cast<float4*>(a.part_ml)[slot] = make_float4(mo_ref, m_ref, l, 0.f);

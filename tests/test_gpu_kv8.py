@@ -379,6 +379,42 @@ def test_scales_far_apart(T):
                             weights=np.zeros((1, 2, 384)))
 
 
+def one_hot_cache(rng, pages, dim=64):
+    """One sequence, one KV head; every 16th key scores 0 and has no V, the others are -100 in channel 0; scales 1."""
+    d = OnDevice(make(rng, 1, pages, 1, dim, 64, 16, "int8", spare=0))
+    d.ref.ks[:], d.ref.vs[:] = 1, 1
+    d.ref.k[..., 0] = np.int8(-100).view(np.uint8)
+    d.ref.v[:] = rng.integers(1, 128, d.ref.v.shape)
+    d.ref.k[:, :, 5::16, 0], d.ref.v[:, :, 5::16] = 0, 0
+    for n in ("k", "v", "ks", "vs"):
+        d.t[n].copy_(dev(getattr(d.ref, n)))
+    return d
+
+
+@pytest.mark.parametrize("dtype,T,depth", [("f32", T, x) for T in (1, 5, 70) for x in (12.5, 13.9, 17.9)] +
+                         [("f16", T, x) for T in (1, 12, 70) for x in (17.9, 18.7)] +
+                         [("bf16", T, x) for T in (1, 12, 70) for x in (18.4, 18.7)])
+def test_long_tail_under_peaks(dtype, T, depth):
+    """All that is answered comes from weights 2^-depth of the largest, all alike, so that their roundings do not cancel:
+    they are held to 2^-11 of each (fp32 rows 2^-22) down to 2^-21 (2^-16) of the largest.
+
+    Queries are one-hot, so scores are exact up to three fp32 roundings of up to `depth`, 3 depth 2^-24, and exp2's
+    2^-22, twice for numerator and denominator; sums of n / 16 products truncate by 2^-23 each at most; below the depths
+    named, P's smallest step leaves 2^-32 (2^-38) of the largest weight x V."""
+    rng = np.random.default_rng(int(10 * depth))
+    n, heads = 2048, 4
+    d = one_hot_cache(rng, n // 64)
+    q = np.zeros((1, T, heads, 64))
+    q[..., 0] = 1
+    scale = float(np.float32(depth * np.log(2) / 100))
+    out, _ = run_attention(d, q, dtype, np.array([n - T]), scale=scale)
+    want, _, mag, _ = d.ref.attention(q, [n - T], [T], scale)
+    u, low = (2.0 ** -22, 2.0 ** -38) if dtype == "f32" else (2.0 ** -11, 2.0 ** -32)
+    dx = 2 * (3 * depth * 2.0 ** -24 + 2.0 ** -22) + n / 16 * 2.0 ** -23
+    peak = 1 / ((n - T) // 16)  # the largest weight, at most
+    near(out, want, HALF[dtype] * np.abs(want) + (u + dx) * mag + n * low * peak * 127)
+
+
 def test_two_graphs_on_two_streams():
     """A single token and a prompt with weights, captured with a workspace each and replayed side by side; an
     eviction captured too.  Every replay gives the eager call's bits."""
