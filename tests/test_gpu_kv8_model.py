@@ -142,7 +142,7 @@ def odd_model(tmp_path_factory):
     return shape, blocks, _oracle_weights(blocks)
 
 
-@pytest.mark.parametrize("page,pool", [(16, 33), (48, 11), (80, 0)])
+@pytest.mark.parametrize("page,pool", [(16, 31), (48, 11), (80, 0)])
 def test_odd_pools(odd_model, page, pool):
     """Pages, heads and blocks whose product is odd: every layer's codes still lie where copies can start."""
     shape, blocks, w = odd_model
