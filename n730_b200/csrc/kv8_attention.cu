@@ -540,12 +540,22 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           float w[4];
+          // weight x V scale: V scale x fm leaves fp32's range where a row sees little or nothing of a block whose scale
+          // is far above its others'; the weight goes first then
+          float f1[2], f2[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float f = vsc[tt] * fm[n][e];
+            const bool in_range = f < 0x1p127f;
+            f1[e] = in_range ? f : vsc[tt];
+            f2[e] = in_range ? 1.f : fm[n][e];
+          }
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float m = m_ref[n][e & 1];
             const float pe = ex2(y[tt][n][e] - (m == -INFINITY ? 0.f : m));
             l_run[n][e & 1] += pe;
-            w[e] = pe * (vsc[tt] * fm[n][e & 1]);
+            w[e] = pe * f1[e & 1] * f2[e & 1];
           }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {

@@ -415,6 +415,43 @@ def test_long_tail_under_peaks(dtype, T, depth):
     near(out, want, HALF[dtype] * np.abs(want) + (u + dx) * mag + n * low * peak * 127)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("T", [1, 12, 40])
+@pytest.mark.parametrize("far", ["behind", "below"])
+def test_one_block_of_large_scale(dtype, T, far):
+    """V scales of 2^-99 and one block of 2^100 that a row does not see, or whose scores lie 2^260 below: the row
+    answers by the others alone.
+
+    The one-hot queries' scores are 0 or about -260 and exact; weights count as in test_long_tail_under_peaks."""
+    rng = np.random.default_rng(T)
+    d = OnDevice(make(rng, 1, 2, 1, 64, 64, 16, "int8", spare=0))
+    d.ref.ks[:], d.ref.vs[:] = 1, 2.0 ** -99
+    pg, off = d.ref.where(0, 48)
+    d.ref.vs[pg, 0, off // 16] = 2.0 ** 100
+    d.ref.k[..., 0] = 0
+    if far == "below":
+        d.ref.k[pg, 0, off:off + 16, 0] = np.int8(-100).view(np.uint8)
+    for n in ("k", "ks", "vs"):
+        d.t[n].copy_(dev(getattr(d.ref, n)))
+    q = np.zeros((1, T, 3, 64))
+    q[..., 0] = 1
+    scale = float(np.float32(2.6 * np.log(2)))
+    L = 48 - T if far == "behind" else 90  # behind: the block's first rows are new, the last query sees position 47
+    lens, new = np.array([L]), np.array([T])
+    if far == "behind":  # rows that do see it follow in the same tile
+        q = np.concatenate([q, q[:, :1]], 1)
+        new = new + 1
+    out, _ = run_attention(d, q, dtype, lens, new, scale=scale)
+    want, p, mag, _ = d.ref.attention(q, lens, new, scale)
+    u, low = (2.0 ** -22, 2.0 ** -38) if dtype == "f32" else (2.0 ** -11, 2.0 ** -32)
+    top = 127 * 2.0 ** -99
+    tol = HALF[dtype] * np.abs(want) + (u + 2.0 ** -19) * mag + 128 * low * top
+    if dtype == "f16":  # smaller than fp16's numbers
+        tol += 2.0 ** -25
+    near(out[:, :T], want[:, :T], tol[:, :T])
+    assert not np.isnan(out).any()
+
+
 def test_two_graphs_on_two_streams():
     """A single token and a prompt with weights, captured with a workspace each and replayed side by side; an
     eviction captured too.  Every replay gives the eager call's bits."""
