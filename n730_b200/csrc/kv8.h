@@ -94,6 +94,9 @@ __device__ __forceinline__ void kv8_store1(void* p, int64_t i, int dtype, float 
 // large P may grow before the reference moves (fp16 ends at 2^16).  What lies below goes down to fp16's smallest normal,
 // 2^-14, at full accuracy: 2^-21 of the largest.
 constexpr float KV8_P_NEW = 7.f, KV8_P_MOST = 15.f;
+// log2 of how far P's reference may lie below the weights': V scales reach 100 and KV8_P_MOST below, scores of blocks
+// whose scale is 0 put the weights' reference anywhere above, and 2^distance has to stay in fp32's range
+constexpr float KV8_REFS_APART = 120.f;
 // V scales below this count as 0: quotients by them would leave fp32's range
 constexpr float KV8_TINY = 0x1p-100f;
 // whether pointers lie on whole elements of `size` bytes (null ones do)

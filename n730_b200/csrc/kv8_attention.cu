@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
               mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, k));
             }
-            mv = fmaxf(mo_ref[n][e], mv - P_NEW);
+            mv = fmaxf(fmaxf(mo_ref[n][e], mx - KV8_REFS_APART), mv - P_NEW);
             if (mx != m_ref[n][e]) {  // from -infinity: the sums are still 0
               l_run[n][e] *= ex2(m_ref[n][e] - mx);
               m_ref[n][e] = mx;

@@ -225,7 +225,7 @@ __device__ __forceinline__ void tc_ld64(uint32_t taddr, float* v) {
 // a P of 2^KV8_P_NEW, where those are larger; sums and, when there are any, outputs (at to) are rescaled.  A warp at a time.
 template <int HD>
 __device__ __forceinline__ void kp_move(uint32_t to, bool outputs, float mx, float mv, float& m_ref, float& mo_ref, float& l) {
-  const float mn = fmaxf(m_ref, mx), mon = fmaxf(mo_ref, mv - KV8_P_NEW);
+  const float mn = fmaxf(m_ref, mx), mon = fmaxf(fmaxf(mo_ref, mn - KV8_REFS_APART), mv - KV8_P_NEW);
   if (mn != m_ref) l *= ex2(m_ref - mn);
   const float f = mon != mo_ref ? ex2(mo_ref - mon) : 1.f;
   m_ref = mn;

@@ -452,6 +452,31 @@ def test_one_block_of_large_scale(dtype, T, far):
     assert not np.isnan(out).any()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("T", [1, 12, 70])
+@pytest.mark.parametrize("depth", [110, 122, 200])
+def test_all_v_far_below_a_block_of_zeros(dtype, T, depth):
+    """The largest scores meet a V scale of 0, the rest weigh 2^-depth: the answer is that small, down to fp32's
+    smallest normal weight, 2^-126, below which it is 0; scores as in test_long_tail_under_peaks."""
+    rng = np.random.default_rng(T)
+    d = one_hot_cache(rng, 8)
+    d.ref.k[..., 0] = np.int8(-100).view(np.uint8)
+    for p0 in range(0, 512, 128):
+        pg, off = d.ref.where(0, p0)
+        d.ref.k[pg, 0, off:off + 16, 0] = 0
+        d.ref.vs[pg, 0, off // 16] = 0
+    for n in ("k", "vs"):
+        d.t[n].copy_(dev(getattr(d.ref, n)))
+    q = np.zeros((1, T, 4, 64))
+    q[..., 0] = 1
+    scale = float(np.float32(depth * np.log(2) / 100))
+    out, _ = run_attention(d, q, dtype, np.array([512 - T]), scale=scale)
+    want, _, mag, _ = d.ref.attention(q, [512 - T], [T], scale)
+    u = 2.0 ** -22 if dtype == "f32" else 2.0 ** -11
+    dx = 2 * (3 * depth * 2.0 ** -24 + 2.0 ** -22) + 32 * 2.0 ** -23
+    near(out, want, HALF[dtype] * np.abs(want) + (u + dx) * mag + (0 if depth < 126 else 2.0 ** -126 * 127 * 512))
+
+
 def test_two_graphs_on_two_streams():
     """A single token and a prompt with weights, captured with a workspace each and replayed side by side; an
     eviction captured too.  Every replay gives the eager call's bits."""
