@@ -234,6 +234,11 @@ int64_t n730_kv8_evict_ws(const N730KV8Cache* c, int batch, int keep);
 int n730_kv8_evict(const N730KV8Cache* c, int batch, int keep, int first, int recent, const int32_t* d_seen,
                    const int32_t* d_lens, int32_t* d_lens_out, const float* d_w, float* d_w_out,
                    const int32_t* d_pos, int32_t* d_pos_out, int64_t ldw, void* d_ws, int64_t ws_bytes, void* stream);
+/* Self-check of the attention's bounded waits: a warp waits at most wait_ns (up to 1 s) for an arrival that never
+ * comes (arrives 0), is there already (1), or comes after half that time, one lane having given up before (2).
+ * Synchronous; 0, or N730_TIMEOUT (-15) in the first and last case, through the device error word; the context stays
+ * usable. */
+int n730_kv8_wait_check(int64_t wait_ns, int arrives, void* stream);
 
 /* ---- whole-model engine (replaces N730CudaTransformer.forward's per-op loop,
  * src-code/inference.py:259-669) ---- */

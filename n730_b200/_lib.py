@@ -65,6 +65,7 @@ _CUDA_SIGS = {
     "n730_kv8_attention": ([vp, vp, i32, i64, i32, i32, i32, f32, vp, vp, vp, i64, vp, vp, i64, vp, i64, vp], i32),
     "n730_kv8_evict_ws": ([vp, i32, i32], i64),
     "n730_kv8_evict": ([vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, i64, vp, i64, vp], i32),
+    "n730_kv8_wait_check": ([i64, i32, vp], i32),
     "n730_qweight_load_blocks": ([C.c_char_p, i32, vp, vp, vp, vp], i32),
     "n730_tp_wait_check": ([i64, i32, vp], i32),
     "n730_attention_forward_noalloc": ([vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp], i32),

@@ -137,6 +137,21 @@ __device__ __forceinline__ uint32_t codes2(uint32_t x) {
 template <int CODE>
 __device__ __forceinline__ uint32_t code_word(uint32_t x) { return CODE == N730_KV8_INT8 ? x ^ 0x80808080u : x; }
 
+// Wait of a whole warp for the phase of `bar`, at most `limit_ns` long; false in every lane when one of them gave up:
+// what that lane reads next may not be there yet.
+__device__ __forceinline__ bool kv8_wait(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
+  bool ok = mbar_try_wait(bar, parity);
+  if (!ok) {
+    auto now = [] { uint64_t t; asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t)); return t; };
+    const uint64_t t0 = now();
+    while (!(ok = mbar_try_wait(bar, parity)))
+      if (now() - t0 > limit_ns) break;
+  }
+  ok = __all_sync(0xffffffffu, ok);
+  __syncwarp();
+  return ok;
+}
+
 // Launch with or without programmatic dependent launch.
 template <class... KArgs, class... Args>
 int kv8_launch_cluster(void (*k)(KArgs...), dim3 grid, int cluster, dim3 block, size_t smem, cudaStream_t st, bool pdl, Args... args) {

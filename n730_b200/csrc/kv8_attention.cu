@@ -139,15 +139,6 @@ __device__ __forceinline__ void copy_rows(uint32_t dst, const CUtensorMap* map, 
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(smem_u32(bar)) : "memory");
 }
-// Bounded wait for the phase of `bar`; no time is spent once a wait of the thread has run out.
-__device__ __forceinline__ bool wait_copies(uint64_t* bar, uint32_t parity, bool lost) {
-  if (mbar_try_wait(bar, parity)) return true;
-  auto now = [] { uint64_t t; asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t)); return t; };
-  const uint64_t t0 = now();
-  while (!mbar_try_wait(bar, parity))
-    if (lost || now() - t0 > KD_WAIT_NS) return false;
-  return true;
-}
 // 4 bytes, or zeros
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool pred) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" :: "r"(dst), "l"(src), "r"(pred ? 4 : 0) : "memory");
@@ -204,7 +195,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
     for (int s = 0; s < ST; ++s) mbar_init(&sm.full[warp][s], 1);
     fence_mbar_init();
   }
-  bool lost = false;   // a wait ran out
+  bool lost = false;   // a wait of the warp ran out: it asks for nothing more
   uint32_t fills = 0;  // tiles this warp has asked for, and used: buffer and phase go by them
   uint32_t uses = 0;
   pdl_wait();
@@ -292,6 +283,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
   };
   // ask for a tile whose half rows are lanes 2 i, 2 i + 1 of `rows`
   auto issue = [&](int rows, int i) {
+    if (lost) return;
     const int st = fills % ST;
     ++fills;
     const int row0 = __shfl_sync(0xffffffffu, rows, 2 * i), row1 = __shfl_sync(0xffffffffu, rows, 2 * i + 1);
@@ -349,7 +341,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
     const KDSeg& after = sm.seg[(turn + 1) % 3];
     if (!run.valid) break;
     const int b = run.b, h = run.h, f0 = run.f0, nrow = run.nrow, L = run.L, total = run.total, ta = run.ta;
-    const int n_tile = tiles_of(run);
+    const int n_tile = lost ? 0 : tiles_of(run);
     int rows_next = lookup(run, 32);
     if (tid == WALKER) next_run(sm.seg[(turn + 1) % 3]);
 
@@ -421,7 +413,8 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
       }
       cp_commit();
       const int st = uses % ST;
-      if (!wait_copies(&sm.full[warp][st], (uses / ST) & 1, lost)) lost = true;
+      lost = !kv8_wait(&sm.full[warp][st], (uses / ST) & 1, KD_WAIT_NS);
+      if (lost) break;
       ++uses;
       cp_wait<ST - 1>();
       __syncwarp();
@@ -688,6 +681,8 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
           sm.tot[tid][2] == 0.f ? INFINITY : sm.tot[tid][1] + log2f(sm.tot[tid][2]);
   }
   cp_wait<0>();
+  if (lost)  // copies in flight end before the shared memory they go to is given up
+    for (; uses != fills; ++uses) kv8_wait(&sm.full[warp][uses % ST], (uses / ST) & 1, KD_WAIT_NS);
 }
 
 // ---------------------------------------------------------------------------
@@ -1015,9 +1010,45 @@ int kv8_attention_launch(const KV8AttnCall& k, cudaStream_t st) {
   return N730_OK;
 }
 
+// One warp waits as the attention's do, on a barrier that nobody (0), a thread beforehand (1) or another warp after half
+// the limit (2) arrives at; in the last case one lane's own limit has run out by then.
+__global__ void kv8_wait_check_kernel(int arrives, uint64_t limit_ns, int* status) {
+  __shared__ uint64_t bar;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    mbar_init(&bar, 1);
+    fence_mbar_init();
+    if (arrives == 1) mbar_arrive_expect_tx(&bar, 0);
+  }
+  __syncthreads();
+  if (warp == 0) {
+    if (!kv8_wait(&bar, 0, arrives == 2 && lane == 7 ? 1 : limit_ns) && lane == 0) *status = DEV_ERR_TIMEOUT;
+  } else if (arrives == 2 && lane == 0) {
+    auto now = [] { uint64_t t; asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t)); return t; };
+    const uint64_t t0 = now();
+    while (now() - t0 < limit_ns / 2) {}
+    mbar_arrive_expect_tx(&bar, 0);
+  }
+}
+
+int* gemv_err_word();
+int gemv_check_error(bool reset);
+
 }  // namespace n730
 
 using namespace n730;
+
+N730_API int n730_kv8_wait_check(int64_t wait_ns, int arrives, void* stream) {
+  N730_REQUIRE(wait_ns > 0 && wait_ns <= 1000000000ll, N730_BAD_ARG, "kv8_wait_check: wait %lld ns", (long long)wait_ns);
+  N730_REQUIRE(arrives >= 0 && arrives <= 2, N730_BAD_ARG, "kv8_wait_check: arrives %d", arrives);
+  int* err = gemv_err_word();
+  if (!err) return N730_OOM;
+  cudaStream_t st = (cudaStream_t)stream;
+  kv8_wait_check_kernel<<<1, 64, 0, st>>>(arrives, (uint64_t)wait_ns, err);
+  N730_CHECK_LAUNCH();
+  N730_CUDA(cudaStreamSynchronize(st));
+  return gemv_check_error(true);
+}
 
 N730_API int64_t n730_kv8_attention_ws(const N730KV8Cache* c, int batch, int tokens, int n_heads, int weights) {
   if (int rc = kv8_attention_check(c, batch, tokens, n_heads)) return rc;

@@ -119,6 +119,16 @@ __device__ __forceinline__ void tc_mma_ss(uint32_t tmem_d, uint64_t adesc, uint6
                :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(IDESC), "r"(accumulate) : "memory");
 }
 
+// After the barrier behind all roles' work, when a wait of the CTA ran out, whichever role's: leaves the mark, and the warp
+// that issued the products waits for those in flight, so that tensor and shared memory can be given up.
+__device__ __forceinline__ void kp_give_up(uint64_t* drain, bool issuer, int* status) {
+  if (threadIdx.x == 0) *status = 1;
+  if (!issuer) return;
+  if (elect_one()) tc_commit(drain);
+  __syncwarp();
+  kv8_wait(drain, 0, 2000000000ull);
+}
+
 // Rows of a warp's share of the 16-bit queries: a lane holds 8 channels of U rows, RPI rows an instruction.  `at(r)`
 // gives row r's first element, negative for rows that are not there.
 template <int HD>
@@ -593,12 +603,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
         }
       }
     }
-    if (!go && nt > 0) {  // what is in flight ends before the tensor memory is freed
-      if (lane == 0) *abortf = 1;
-      if (elect_one()) tc_commit(&sm.drain);
-      wait_bar(&sm.drain, 0);
-      __syncwarp();
-    }
   } else {
     // ---------------- softmax: warps 0-3 of A, 4-7 of B, a thread a row ----------------
     const int x = warp >> 2, q = warp & 3, r = x * (KP_ROWS / 2) + q * 32 + lane, f = f0 + r;
@@ -678,7 +682,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (*abortf && tid == 0) *a.status = 1;
+  if (*abortf) kp_give_up(&sm.drain, warp == KP_MMA_WARP, a.status);
   if (warp == KP_MMA_WARP)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(Cfg::TMEM) : "memory");
 }
@@ -815,12 +819,6 @@ kv8_prompt_weights_kernel(const KPArgs a, const float* w_in, float* w_out, int64
       }
       __syncwarp();
     }
-    if (!go) {
-      if (lane == 0) *abortf = 1;
-      if (elect_one()) tc_commit(&sm.drain);
-      wait_bar(&sm.drain, 0);
-      __syncwarp();
-    }
   } else {
     const int x = warp >> 2, q = warp & 3, p = p0 + q * 32 + lane;
     const int64_t row = row_of(p);
@@ -852,7 +850,7 @@ kv8_prompt_weights_kernel(const KPArgs a, const float* w_in, float* w_out, int64
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (*abortf && tid == 0) *a.status = 1;
+  if (*abortf) kp_give_up(&sm.drain, warp == KW_MMA_WARP, a.status);
   if (tid < KP_KEYS) sm.sum[tid] += sum;
   if (a.shares > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (rank == 0 && tid < KP_KEYS && p0 + tid < total) {

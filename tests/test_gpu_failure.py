@@ -47,3 +47,13 @@ def test_wait_check_rejects_bad_limits():
     lib = _lib.cuda()
     assert lib.n730_tp_wait_check(0, 0, None) == -13
     assert lib.n730_tp_wait_check(20_000_000_000, 0, None) == -13
+
+
+def test_kv8_waits_run_out_and_context_survives():
+    """The 8-bit cache attention's wait: it ends after its limit, one lane that gives up is enough, and the next
+    call is not marked."""
+    lib = _lib.cuda()
+    for arrives, want in ((0, -15), (1, 0), (2, -15), (1, 0)):
+        t0 = time.monotonic()
+        assert lib.n730_kv8_wait_check(200_000_000, arrives, None) == want, arrives
+        assert time.monotonic() - t0 < 2.0

@@ -149,3 +149,9 @@ def test_model_batch():
     from n730_b200.engine import Engine
     with pytest.raises(RuntimeError, match="batch of 4097"):
         Engine(synthetic.SHAPES["tiny"], max_ctx=64, max_batch=4097, kv_bits=8)
+
+
+def test_wait_check_arguments():
+    lib = _lib.cuda()
+    for ns, arrives in ((0, 0), (-1, 1), (1_000_000_001, 0), (1000, 3), (1000, -1)):
+        assert lib.n730_kv8_wait_check(ns, arrives, None) == -13
