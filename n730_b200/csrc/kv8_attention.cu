@@ -57,7 +57,6 @@ constexpr int KD_CTAS_PER_SM = 3;
 // heads): 3 131.8 us, 6 124.9, 10 120.5, 16 116.1, 24 117.1, 40 121.1; batch of 32 with weights 55.6, 53.9, 53.4,
 // 52.7, 53.2, 54.7.
 constexpr int KD_ITEM_COST = 16;
-constexpr float KD_NEAR = 0x1p60f;  // V scales and factors fm below it have a product in fp32's range
 constexpr int KD_MIN_UNITS = 4;  // tiles of a run: fewer would leave warps idle and joins to do
 constexpr float KD_SLACK = 8.f;  // log2 of how far a weight in the sum (fp32) may exceed its reference
 constexpr float KD_P_NEW_LO = 13.f;  // as KV8_P_NEW for two-term P, whose second term runs out of fp16's range first
@@ -403,7 +402,6 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
     for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) { m_ref[n][e] = mo_ref[n][e] = -INFINITY; fm[n][e] = l_run[n][e] = 0.f; }
-    bool apart = false;  // some row's references are KD_NEAR or more apart
 
     for (int qi = 0; qi < n_tile; ++qi) {
       __syncwarp();  // every lane is done with the buffer that the next copies go to
@@ -526,10 +524,6 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
             }
             fm[n][e] = mv == -INFINITY ? 0.f : ex2(mx - mv);
           }
-        apart = false;
-#pragma unroll
-        for (int n = 0; n < NB; ++n) apart |= !(fm[n][0] < KD_NEAR && fm[n][1] < KD_NEAR);
-        apart = __any_sync(0xffffffffu, apart);
       }
       // ---- O^T += V^T P^T ----
 #pragma unroll
@@ -539,23 +533,22 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           float w[4];
+          // weight x V scale: V scale x fm leaves fp32's range where a row sees little or nothing of a block whose scale
+          // is far above its others'; the weight goes first then
+          float f1[2], f2[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float f = vsc[tt] * fm[n][e];
+            const bool in_range = f < 0x1p127f;
+            f1[e] = in_range ? f : vsc[tt];
+            f2[e] = in_range ? 1.f : fm[n][e];
+          }
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float m = m_ref[n][e & 1];
-            w[e] = ex2(y[tt][n][e] - (m == -INFINITY ? 0.f : m));
-            l_run[n][e & 1] += w[e];
-          }
-          if (!apart && vsc[tt] < KD_NEAR) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] *= vsc[tt] * fm[n][e & 1];
-          } else {
-            // V scale x fm leaves fp32's range where a row sees little or nothing of a block whose scale is far above its
-            // others'; the weight goes first then
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float f = vsc[tt] * fm[n][e & 1];
-              w[e] = f < 0x1p127f ? w[e] * f : w[e] * vsc[tt] * fm[n][e & 1];
-            }
+            const float pe = ex2(y[tt][n][e] - (m == -INFINITY ? 0.f : m));
+            l_run[n][e & 1] += pe;
+            w[e] = pe * f1[e & 1] * f2[e & 1];
           }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
