@@ -21,13 +21,11 @@ int kv8_append_launch(const N730KV8Cache& c, const void* k, const void* v, int d
 // *pos + r (one sequence) or pos[r] (a row per sequence).  q16 (may be null): q rounded to fp16 instead.
 int kv8_rope_launch(float* qkv, int64_t ld, int rows, int heads, int n_kv, int head_dim, const float* cos_t,
                     const float* sin_t, const int* pos, bool per_row, __half* q16, bool pdl, cudaStream_t st);
-// fp16 -> fp32
-int kv8_widen_launch(const __half* x, float* y, int64_t n, bool pdl, cudaStream_t st);
 
 struct KV8AttnCall {
   N730KV8Cache c;
   const void* q; void* out;
-  int dtype;
+  int dtype, out_dtype;  // of q; of out
   int64_t ldq, ldo;
   int batch, tokens, heads;
   float scale;

@@ -66,7 +66,7 @@ struct KDArgs {
   N730KV8Cache c;
   const void* q; void* out;
   int64_t ldq, ldo;
-  int dtype, batch, tokens, heads, group, rows, nrg;  // rows = chunk * group; nrg row groups of RG
+  int dtype, odtype, batch, tokens, heads, group, rows, nrg;  // rows = chunk * group; nrg row groups of RG
   int t0, chunk;       // the call's tokens [t0, t0 + chunk) of each sequence
   float scale_log2e;
   const int* lens; const int* n_new;
@@ -171,10 +171,10 @@ __device__ __forceinline__ void kd_answer(const KDArgs& a, int b, int h, int f, 
   // by two factors, whose product may leave fp32's normal range when the answer does not; a NaN query: NaN
   const float s = l == 0.f ? 0.f : 1.f / l, f2 = l == 0.f || Mo == -INFINITY ? 0.f : ex2(Mo - M);
   const int64_t at = ((int64_t)b * a.tokens + a.t0 + f / a.group) * a.ldo + (int64_t)(h * a.group + f % a.group) * HD + d;
-  kv8_store1(a.out, at, a.dtype, num.x * s * f2);
-  kv8_store1(a.out, at + 1, a.dtype, num.y * s * f2);
-  kv8_store1(a.out, at + 2, a.dtype, num.z * s * f2);
-  kv8_store1(a.out, at + 3, a.dtype, num.w * s * f2);
+  kv8_store1(a.out, at, a.odtype, num.x * s * f2);
+  kv8_store1(a.out, at + 1, a.odtype, num.y * s * f2);
+  kv8_store1(a.out, at + 2, a.odtype, num.z * s * f2);
+  kv8_store1(a.out, at + 3, a.odtype, num.w * s * f2);
 }
 
 // NB: 8-row groups of an item's rows worked on together; LO: fp32 rows in two fp16 terms.
@@ -964,7 +964,7 @@ int kv8_attention_launch(const KV8AttnCall& k, cudaStream_t st) {
   uint8_t* ws = reinterpret_cast<uint8_t*>(k.ws);
   KDArgs a{};
   a.c = c;
-  a.q = k.q; a.out = k.out; a.ldq = k.ldq; a.ldo = k.ldo; a.dtype = k.dtype;
+  a.q = k.q; a.out = k.out; a.ldq = k.ldq; a.ldo = k.ldo; a.dtype = k.dtype; a.odtype = k.out_dtype;
   a.batch = k.batch; a.tokens = k.tokens; a.heads = k.heads; a.group = k.heads / c.n_kv;
   a.rows = p.chunk * a.group; a.nrg = p.nrg;
   a.chunk = p.chunk;
@@ -1069,7 +1069,7 @@ N730_API int n730_kv8_attention(const N730KV8Cache* c, const void* d_q, int dtyp
                N730_BAD_ARG, "kv8_attention: workspace of %lld bytes", (long long)ws_bytes);
   KV8AttnCall k{};
   k.c = *c;
-  k.q = d_q; k.out = d_out; k.dtype = dtype; k.ldq = ldq; k.ldo = ldo;
+  k.q = d_q; k.out = d_out; k.dtype = k.out_dtype = dtype; k.ldq = ldq; k.ldo = ldo;
   k.batch = batch; k.tokens = tokens; k.heads = n_heads; k.scale = scale;
   k.lens = d_lens; k.n_new = d_new;
   k.w_in = d_w; k.w_out = d_w_out; k.ldw = ldw;

@@ -621,16 +621,6 @@ int kv8_rope_launch(float* qkv, int64_t ld, int rows, int heads, int n_kv, int h
                     (int)per_row, q16);
 }
 
-__global__ void kv8_widen_kernel(const __half* x, float* y, int64_t n) {
-  pdl_wait();
-  const int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 2;  // n is even: rows of head_dim
-  if (i < n) *reinterpret_cast<float2*>(y + i) = __half22float2(*reinterpret_cast<const __half2*>(x + i));
-}
-
-int kv8_widen_launch(const __half* x, float* y, int64_t n, bool pdl, cudaStream_t st) {
-  return kv8_launch(kv8_widen_kernel, dim3((unsigned)((n / 2 + 255) / 256)), dim3(256), 0, st, pdl, x, y, n);
-}
-
 }  // namespace n730
 
 using namespace n730;

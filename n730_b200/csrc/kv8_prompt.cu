@@ -353,7 +353,7 @@ struct KPArgs {
   N730KV8Cache c;
   const void* q; void* out;
   int64_t ldq, ldo;
-  int dtype, tokens, group, rows, tiles;  // rows = tokens * group; tiles of KP_ROWS rows
+  int dtype, odtype, tokens, group, rows, tiles;  // rows = tokens * group; tiles of KP_ROWS rows
   int log_block;
   int batch, tail, splits;                // the first `tail` tiles' positions are cut into shares, each a CTA
   int shares;                             // of the rows, for the weights
@@ -654,6 +654,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
             *reinterpret_cast<float4*>(a.part + slot * HD + cc * 32 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        } else if (a.vec && a.odtype == N730_F32) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + at + cc * 32 + i) =
+                make_float4(v[i] * s * f2, v[i + 1] * s * f2, v[i + 2] * s * f2, v[i + 3] * s * f2);
         } else if (a.vec) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
@@ -661,7 +666,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float y0 = v[i + 2 * e] * s * f2, y1 = v[i + 2 * e + 1] * s * f2;
-              if (a.dtype == N730_F16) {
+              if (a.odtype == N730_F16) {
                 w[e] = h2u(__floats2half2_rn(y0, y1));
               } else {
                 const __nv_bfloat162 y = __floats2bfloat162_rn(y0, y1);
@@ -672,7 +677,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) kv8_store1(a.out, at + cc * 32 + i, a.dtype, v[i] * s * f2);
+          for (int i = 0; i < 32; ++i) kv8_store1(a.out, at + cc * 32 + i, a.odtype, v[i] * s * f2);
         }
       }
       if (live && part) reinterpret_cast<float4*>(a.part_ml)[slot] = make_float4(mo_ref, m_ref, l, 0.f);
@@ -895,9 +900,9 @@ KV8PromptPlan kv8_prompt_plan(const N730KV8Cache& c, int batch, int tokens, int 
 static KPArgs kp_args(const KV8AttnCall& k, const KV8PromptPlan& p, int* status, float* part, float* part_ml, float* lse) {
   KPArgs a{};
   a.c = k.c;
-  a.q = k.q; a.out = k.out; a.ldq = k.ldq; a.ldo = k.ldo; a.dtype = k.dtype;
+  a.q = k.q; a.out = k.out; a.ldq = k.ldq; a.ldo = k.ldo; a.dtype = k.dtype; a.odtype = k.out_dtype;
   a.tokens = k.tokens; a.group = k.heads / k.c.n_kv; a.rows = p.rows; a.tiles = p.tiles; a.splits = p.splits; a.tail = p.tail; a.batch = k.batch; a.shares = p.shares;
-  a.vec = ((uintptr_t)k.out & 15) == 0 && k.ldo * kv8_esize(k.dtype) % 16 == 0;
+  a.vec = ((uintptr_t)k.out & 15) == 0 && k.ldo * kv8_esize(k.out_dtype) % 16 == 0;
   a.qvec = ((uintptr_t)k.q & 15) == 0 && k.ldq * kv8_esize(k.dtype) % 16 == 0;
   a.scale_log2e = fabsf(k.scale) * 1.4426950408889634f;
   a.sign = k.scale < 0.f ? -1.f : 1.f;

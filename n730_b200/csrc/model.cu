@@ -88,11 +88,11 @@ struct Model {
   std::vector<void*> allocs;
   float *cos_t = nullptr, *sin_t = nullptr;
   __half *k_pool = nullptr, *v_pool = nullptr;
-  // 8-bit cache (kv_bits 8): attention workspace, prefill's first position, fp16 queries and outputs
+  // 8-bit cache (kv_bits 8): attention workspace, prefill's first position, fp16 queries
   uint8_t* kv8_ws = nullptr;
   int64_t kv8_ws_bytes = 0;
   int* kv8_pos0 = nullptr;
-  __half *kv8_q = nullptr, *kv8_out = nullptr;
+  __half* kv8_q = nullptr;
   int* block_table = nullptr;
   int* seq_lens = nullptr;
   std::vector<int> h_seq;
@@ -713,7 +713,6 @@ static int finalize(Model* m) {
     N730_CUDA(cudaMemsetAsync(m->kv8_ws, 0, (size_t)m->kv8_ws_bytes, m->st));
     if (int rc = m->alloc(&m->kv8_pos0, 1)) return rc;
     if (int rc = m->alloc(&m->kv8_q, (size_t)c.max_prefill * c.heads * c.head_dim)) return rc;
-    if (int rc = m->alloc(&m->kv8_out, (size_t)c.max_prefill * c.heads * c.head_dim)) return rc;
   }
   if (int rc = m->alloc(&m->seq_lens, c.max_batch)) return rc;
   N730_CUDA(cudaMemsetAsync(m->seq_lens, 0, c.max_batch * 4, m->st));
@@ -880,7 +879,7 @@ static int kv8_attend(Model* m, const Layer& y, const int* table, const int* len
                       float* out) {
   const N730ModelConfig& c = m->c;
   const int ad = c.heads * c.head_dim, rows = batch * tokens;
-  const bool f16 = tokens > 1;  // prompts: fp16 queries and outputs, which o_proj's GEMM rounds to anyway
+  const bool f16 = tokens > 1;  // prompts: fp16 queries, as over the fp16 cache; what they answer stays fp32
   N730KV8Cache kv = y.kv8;
   kv.block_table = table;
   if (int rc = kv8_rope_launch(qkv, m->qkv_dim, rows, c.heads, c.kv_heads, c.head_dim, m->cos_t, m->sin_t, lens, batch > 1,
@@ -892,8 +891,9 @@ static int kv8_attend(Model* m, const Layer& y, const int* table, const int* len
   KV8AttnCall k{};
   k.c = kv;
   k.q = f16 ? (const void*)m->kv8_q : qkv;
-  k.out = f16 ? (void*)m->kv8_out : out;
+  k.out = out;
   k.dtype = f16 ? N730_F16 : N730_F32;
+  k.out_dtype = N730_F32;
   k.ldq = f16 ? ad : m->qkv_dim;
   k.ldo = ad;
   k.batch = batch; k.tokens = tokens; k.heads = c.heads;
@@ -902,8 +902,7 @@ static int kv8_attend(Model* m, const Layer& y, const int* table, const int* len
   k.ws = m->kv8_ws; k.ws_bytes = m->kv8_ws_bytes;
   k.status = gemv_err_word();
   k.pdl = c.use_pdl;
-  if (int rc = kv8_attention_launch(k, m->st)) return rc;
-  return f16 ? kv8_widen_launch(m->kv8_out, out, (int64_t)rows * ad, c.use_pdl, m->st) : N730_OK;
+  return kv8_attention_launch(k, m->st);
 }
 
 // Enqueue one decode step for sequences [0, B) on m->st (tokens in m->d_tokens).

@@ -14,7 +14,7 @@ import pytest
 from gpu_util import rel_err
 from kv8_ref import Cache, decode
 from n730_b200 import synthetic
-from n730_b200.engine import Engine, load_tensors
+from n730_b200.engine import BIAS_SLOTS, Engine, load_tensors
 from n730_b200.batching import ContinuousBatcher
 from oracle.model import OracleDecoder, apply_rope, attention, rms_norm, swiglu
 from test_gpu_model import _blocks, _oracle_weights
@@ -153,6 +153,28 @@ def test_odd_pools(odd_model, page, pool):
     assert rel_err(e.forward(prompt), orc.forward(prompt)) <= TOL
     for tok in rng.integers(0, shape.vocab, 3):
         assert rel_err(e.decode([tok])[0], orc.forward([tok])) <= TOL
+    e.close()
+
+
+@pytest.mark.parametrize("prompt", [9, 64])
+def test_large_values_with_exact_gemv(model, prompt):
+    """V far beyond fp16's range: with the fp32 GEMV prompts answer like single tokens, by either kernel."""
+    shape, blocks, w = model
+    e = Engine(shape, max_ctx=512, max_batch=1, max_prefill=64, kv_bits=8, exact_gemv=True)
+    load_tensors(e, blocks)
+    w = dict(w)
+    for i in range(shape.layers):
+        name = f"model.layers.{i}.self_attn.v_proj.bias"
+        w[name] = w[name].astype(np.float32).copy()
+        w[name][::16] += 2e5
+        e.set_vector(i, BIAS_SLOTS["self_attn.v_proj"], w[name])
+    e.finalize()
+    orc = Oracle8(shape, w, 512)
+    rng = np.random.default_rng(prompt)
+    ids = rng.integers(0, shape.vocab, prompt)
+    assert rel_err(e.forward(ids), orc.forward(ids)) <= TOL
+    tok = int(rng.integers(0, shape.vocab))
+    assert rel_err(e.decode([tok])[0], orc.forward([tok])) <= TOL
     e.close()
 
 
