@@ -199,10 +199,13 @@ int n730_kv8_append(const N730KV8Cache* c, const void* d_k, const void* d_v, int
  * [n_kv][head_dim] of d_k and d_v; positions outside [0, d_lens[b]) give zeros. */
 int n730_kv8_read(const N730KV8Cache* c, void* d_k, void* d_v, int dtype, int64_t ld, int batch, int tokens,
                   const int32_t* d_first, const int32_t* d_lens, void* stream);
-/* Bytes of workspace (16-byte aligned) of an n730_kv8_attention call of this size (negative: a return
- * code).  Zero it once: its first int32 becomes 1 if a device wait ever runs out (the call's outputs
+/* Bytes of workspace (16-byte aligned) of an n730_kv8_attention call of this size, whatever the type of its
+ * rows (negative: a return code).  Zero it once: its first int32 becomes 1 if a device wait ever runs out (the call's outputs
  * are not valid then), the rest does not matter from call to call. */
 int64_t n730_kv8_attention_ws(const N730KV8Cache* c, int batch, int tokens, int n_heads, int weights);
+/* The same for rows of one type, which is all that a call of that type asks for: with weights, a 16-bit
+ * prompt's is a small part of the other, which has room for fp32 rows' scores. */
+int64_t n730_kv8_attention_ws_of(const N730KV8Cache* c, int dtype, int batch, int tokens, int n_heads, int weights);
 /* Attention of the `tokens` newest rows of each sequence (d_new[b] of them) over its cached
  * positions: query t of sequence b, RoPE applied, sees positions [0, d_lens[b] + t] - call it after
  * n730_kv8_append with the same d_lens and d_new.  d_q and d_out rows are [n_heads][head_dim]

@@ -62,6 +62,7 @@ _CUDA_SIGS = {
     "n730_kv8_append": ([vp, vp, vp, i32, i64, i32, i32, vp, vp, vp], i32),
     "n730_kv8_read": ([vp, vp, vp, i32, i64, i32, i32, vp, vp, vp], i32),
     "n730_kv8_attention_ws": ([vp, i32, i32, i32, i32], i64),
+    "n730_kv8_attention_ws_of": ([vp, i32, i32, i32, i32, i32], i64),
     "n730_kv8_attention": ([vp, vp, i32, i64, i32, i32, i32, f32, vp, vp, vp, i64, vp, vp, i64, vp, i64, vp], i32),
     "n730_kv8_evict_ws": ([vp, i32, i32], i64),
     "n730_kv8_evict": ([vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, i64, vp, i64, vp], i32),

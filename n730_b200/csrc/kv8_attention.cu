@@ -884,7 +884,7 @@ int kv8_attention_check(const N730KV8Cache* c, int batch, int tokens, int heads)
 }
 
 int64_t kv8_attention_ws(const N730KV8Cache& c, int batch, int tokens, int heads, bool weights) {
-  // fp32 calls take more row groups, 16-bit calls larger parts
+  // fp32 calls take more row groups and keep a prompt's scores, 16-bit calls larger parts
   return std::max(kd_plan(c, batch, tokens, heads, N730_F32, weights).bytes,
                   kd_plan(c, batch, tokens, heads, N730_F16, weights).bytes);
 }
@@ -1048,6 +1048,12 @@ N730_API int64_t n730_kv8_attention_ws(const N730KV8Cache* c, int batch, int tok
   return kv8_attention_ws(*c, batch, tokens, n_heads, weights != 0);
 }
 
+N730_API int64_t n730_kv8_attention_ws_of(const N730KV8Cache* c, int dtype, int batch, int tokens, int n_heads, int weights) {
+  if (int rc = kv8_attention_check(c, batch, tokens, n_heads)) return rc;
+  N730_REQUIRE(dtype == N730_F32 || dtype == N730_F16 || dtype == N730_BF16, N730_BAD_ARG, "kv8_attention: dtype %d", dtype);
+  return kd_plan(*c, batch, tokens, n_heads, dtype, weights != 0).bytes;
+}
+
 N730_API int n730_kv8_attention(const N730KV8Cache* c, const void* d_q, int dtype, int64_t ldq, int batch, int tokens,
                                 int n_heads, float scale, const int32_t* d_lens, const int32_t* d_new, void* d_out,
                                 int64_t ldo, const float* d_w, float* d_w_out, int64_t ldw, void* d_ws,
@@ -1065,8 +1071,7 @@ N730_API int n730_kv8_attention(const N730KV8Cache* c, const void* d_q, int dtyp
                "kv8_attention: row stride %lld of the weights is below the table's %lld positions", (long long)ldw,
                (long long)c->max_pages * c->page_size);
   N730_REQUIRE(scale == scale && scale - scale == 0.f, N730_BAD_ARG, "kv8_attention: scale %g", scale);
-  N730_REQUIRE(ws_bytes >= kv8_attention_ws(*c, batch, tokens, n_heads, d_w_out != nullptr) && ((uintptr_t)d_ws & 15) == 0,
-               N730_BAD_ARG, "kv8_attention: workspace of %lld bytes", (long long)ws_bytes);
+  N730_REQUIRE(((uintptr_t)d_ws & 15) == 0, N730_BAD_ARG, "kv8_attention: the workspace must be 16-byte aligned");
   KV8AttnCall k{};
   k.c = *c;
   k.q = d_q; k.out = d_out; k.dtype = k.out_dtype = dtype; k.ldq = ldq; k.ldo = ldo;

@@ -50,9 +50,13 @@ class KV8Cache:
         _lib.check(self.lib.n730_kv8_read(self._ref, k, v, DTYPES[dtype], ld or self.row, batch, tokens, first, lens,
                                           stream), "kv8_read")
 
-    def attention_workspace(self, batch: int, tokens: int, heads: int, weights: bool = False) -> int:
-        """Bytes of the workspace that ``attention`` of this size wants (not always more for more tokens), zeroed once by
-        the caller; its first int32 is 1 after a device wait ran out."""
+    def attention_workspace(self, batch: int, tokens: int, heads: int, weights: bool = False,
+                            dtype: str | None = None) -> int:
+        """Bytes of the workspace that ``attention`` of this size wants (not always more for more tokens), for rows of
+        any type or of ``dtype``, zeroed once by the caller; its first int32 is 1 after a device wait ran out."""
+        if dtype is not None:
+            return _lib.check(self.lib.n730_kv8_attention_ws_of(self._ref, DTYPES[dtype], batch, tokens, heads,
+                                                                int(weights)), "kv8_attention_ws")
         return _lib.check(self.lib.n730_kv8_attention_ws(self._ref, batch, tokens, heads, int(weights)),
                           "kv8_attention_ws")
 

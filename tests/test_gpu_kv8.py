@@ -379,6 +379,21 @@ def test_scales_far_apart(T):
                             weights=np.zeros((1, 2, 384)))
 
 
+@pytest.mark.parametrize("dtype,T", [("f16", 70), ("f32", 70), ("bf16", 3), ("f32", 1), ("f16", 300)])
+def test_workspace_of_a_type(dtype, T):
+    """A call stays within the workspace of its own type."""
+    rng = np.random.default_rng(T)
+    t = torch()
+    d = OnDevice(make(rng, 2, 8, 2, 64, 64, 16, "int8"))
+    for weights in (False, True):
+        need = d.h.attention_workspace(2, T, 14, weights=weights, dtype=dtype)
+        ws = t.full((need + 4096,), 0x5a, dtype=t.uint8, device="cuda")
+        ws[:4] = 0
+        check_attention(d, rng.standard_normal((2, T, 14, 64)), dtype, np.array([100, 0]), ws=ws[:need],
+                        weights=rng.random((2, 2, 512)) if weights else None)
+        assert (ws[need:] == 0x5a).all() and (ws[:4] == 0).all()
+
+
 def one_hot_cache(rng, pages, dim=64):
     """One sequence, one KV head; every 16th key scores 0 and has no V, the others are -100 in channel 0; scales 1."""
     d = OnDevice(make(rng, 1, pages, 1, dim, 64, 16, "int8", spare=0))

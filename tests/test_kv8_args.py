@@ -155,3 +155,19 @@ def test_wait_check_arguments():
     lib = _lib.cuda()
     for ns, arrives in ((0, 0), (-1, 1), (1_000_000_001, 0), (1000, 3), (1000, -1)):
         assert lib.n730_kv8_wait_check(ns, arrives, None) == -13
+
+
+def test_workspace_of_a_type():
+    """A type's own workspace is enough for its calls and no more is asked for; the query without one covers all."""
+    c = cache(max_pages=128, n_kv=8, head_dim=128, n_pages=4096)
+    for batch, tokens, heads, weights in ((32, 300, 64, True), (1, 1, 64, False), (4, 3, 8, True), (2, 70, 16, False)):
+        every = {t: c.attention_workspace(batch, tokens, heads, weights, dtype=t) for t in ("f32", "f16", "bf16")}
+        assert c.attention_workspace(batch, tokens, heads, weights) == max(every.values())
+        assert every["f16"] == every["bf16"]
+        for t, need in every.items():
+            with pytest.raises(_lib.N730Error, match=f"{need} needed"):
+                c.attention(A, A, t, batch, tokens, heads, A, w_out=A if weights else 0, ld_w=8192, ws=A, ws_bytes=need - 1)
+    every = [c.attention_workspace(32, 300, 64, True, dtype=t) for t in ("f16", "f32")]
+    assert every[0] < 20 << 20 < 500 << 20 < every[1]
+    assert c.lib.n730_kv8_attention_ws_of(c._ref, 3, 1, 1, 8, 0) == -13
+    assert c.lib.n730_kv8_attention_ws_of(None, 1, 1, 1, 8, 0) == -12
