@@ -178,6 +178,51 @@ def test_large_values_with_exact_gemv(model, prompt):
     e.close()
 
 
+def test_sampled_steps_moves_and_rollback(model):
+    """Greedy sampled steps, a sequence cut back (its block keeps the scale) and grown again, moved to another slot;
+    prefill chunks of one token."""
+    shape, blocks, w = model
+    e = _engine(shape, blocks, max_batch=3)
+    orc = Oracle8(shape, w, 512)
+    rng = np.random.default_rng(17)
+    ids = rng.integers(0, shape.vocab, 65)  # the second chunk is one token
+    assert rel_err(e.forward(ids, seq=1), orc.forward(ids)) <= TOL
+    e.set_seq_len(1, 41)
+    orc.seq_len = 41
+    ids = rng.integers(0, shape.vocab, 12)
+    assert rel_err(e.forward(ids, seq=1), orc.forward(ids)) <= TOL
+    e.seq_move(0, 1)
+    tok = int(rng.integers(0, shape.vocab))
+    for _ in range(3):
+        y = orc.forward([tok])
+        nxt = int(e.decode_sample([tok], temperature=0.0)[0])
+        assert y[nxt] >= y.max() - TOL * np.abs(y).max()
+        tok = nxt
+    assert e.seq_len(0) == 56
+    e.reset()
+    orc = Oracle8(shape, w, 512)
+    assert rel_err(e.forward(ids), orc.forward(ids)) <= TOL
+    e.close()
+
+
+@pytest.mark.parametrize("kw", [dict(stream_depth=2), dict(exact_gemv=True), dict(per_op_decode=1), dict(per_op_decode=-1)])
+def test_other_paths_agree(model, kw):
+    """Streamed layers give the resident engine's bits, the fp32 GEMV its logits; the decode path is the same whatever
+    is asked for."""
+    shape, blocks, w = model
+    a, b = _engine(shape, blocks, max_batch=2), _engine(shape, blocks, max_batch=2, **kw)
+    rng = np.random.default_rng(19)
+    ids = rng.integers(0, shape.vocab, 70)
+    steps = [(x.forward(ids), x.forward(ids[:9], seq=1), x.decode([3, 5]).copy(), x.decode([7]).copy()) for x in (a, b)]
+    for x, y in zip(*steps):
+        if "exact_gemv" in kw:
+            assert rel_err(y, x) <= TOL
+        else:
+            assert np.array_equal(x, y)
+    a.close()
+    b.close()
+
+
 def test_refused_configurations():
     shape = synthetic.SHAPES["tiny"]
     for kw in (dict(kv_bits=4), dict(kv_bits=8, page_size=24), dict(kv_bits=-8)):
