@@ -93,6 +93,8 @@ def _args():
                     help="persistent decode FFN: 0 auto, 1 one fused phase, -1 two GEMV phases")
     ap.add_argument("--per-op", action="store_true",
                     help="batch-1 decode through the per-op kernels instead of the persistent kernel")
+    ap.add_argument("--kv-bits", type=int, default=16, choices=[16, 8],
+                    help="resident workload: the KV cache in fp16 (the headline) or in int8 codes")
     ap.add_argument("--model", default=SHAPE_NAME, choices=["qwen2-7b", "qwen2-0.5b"],
                     help="resident workload: model shape")
     ap.add_argument("--pmap", default="int4_g128", choices=["int4_g128", "mixed_05b"],
@@ -423,11 +425,11 @@ def run_ours(a):
     shape = SHAPES[a.model]
     if a.layers:
         shape = dataclasses.replace(shape, layers=a.layers)
-    headline = a.model == SHAPE_NAME and a.pmap == "int4_g128"
+    headline = a.model == SHAPE_NAME and a.pmap == "int4_g128" and a.kv_bits == 16
     B, ctx = a.batch, a.ctx
     max_ctx = ctx + 3 * (a.warmup + a.steps) + 64  # device-side steps, then the two e2e passes
     eng = Engine(shape, max_ctx=max_ctx, max_batch=B, max_prefill=a.prefill_chunk, ffn_fuse=a.ffn_fuse,
-                 per_op_decode=a.per_op)
+                 per_op_decode=a.per_op, kv_bits=a.kv_bits)
     build_on_device(shape, a.pmap, eng, seed=rank)
     eng.finalize()
     info = eng.info()
@@ -548,13 +550,15 @@ def run_ours(a):
                 if line.startswith("traffic_bytes_per_launch:"):
                     traffic = int(line.split(":", 1)[1])
         toks = B * a.steps * world
+        per_layer = 5 if a.kv_bits == 16 else 8  # RoPE, append, attention and its join instead of one attention kernel
         kv_bytes = info["kv_bytes_per_pos"] * (ctx + a.warmup + a.steps // 2) * B
         step_bytes = info["weight_bytes"] + kv_bytes
         params = shape.layers * (shape.hidden * (shape.heads + 2 * shape.kv_heads) * shape.head_dim
                                  + shape.heads * shape.head_dim * shape.hidden
                                  + 3 * shape.hidden * shape.ffn) + shape.vocab * shape.hidden
         out = {
-            "metric": METRIC if headline else f"decode tok/s at {a.model}-shape ({a.pmap})",
+            "metric": METRIC if headline else f"decode tok/s at {a.model}-shape ({a.pmap}"
+                                                   + (", 8-bit KV)" if a.kv_bits == 8 else ")"),
             "value": round(toks / t_dev, 2), "unit": "tok/s", "n_gpus": world,
             "steps": a.steps, "warmup": a.warmup, "ms_per_step": round(t_dev / a.steps * 1000, 4),
             "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
@@ -563,7 +567,7 @@ def run_ours(a):
             "config": {"workload": f"{a.model}-shape decoder ({shape.layers} layers), "
                                    + ("all linears INT4 g128 (fp16 scale+zero)" if a.pmap == "int4_g128" else
                                       "attention INT8 per-tensor, FFN INT4 g128, fp16 tied embedding / lm_head")
-                                   + f", batch {B} decode after a {ctx}-token prefill, fp16 paged KV",
+                                   + f", batch {B} decode after a {ctx}-token prefill, {'fp16' if a.kv_bits == 16 else 'int8'} paged KV",
                        "batch": B, "ctx_start": ctx, "parallelism": f"replicas x{world}" if world > 1 else "single",
                        "decode_path": ("persistent kernel" + (", FFN fused" if info["ffn_fused"] else "")
                                        if persistent else "per-op kernels (graph)"),
@@ -582,8 +586,8 @@ def run_ours(a):
                               "achieved_gbs": round(step_bytes / (t_dev / a.steps) / 1e9, 1),
                               "frac": round(step_bytes / (t_dev / a.steps) / 1e9 / peak, 4)},
             "clocks": clk.summary(),
-            "gpu_launches": a.steps * (3 if persistent else 5 * shape.layers + 3),
-            "gpu_launches_e2e_per_step": (3 if persistent else 5 * shape.layers + 3) + 1,
+            "gpu_launches": a.steps * (3 if persistent else per_layer * shape.layers + 3),
+            "gpu_launches_e2e_per_step": (3 if persistent else per_layer * shape.layers + 3) + 1,
             "prefill": {"tokens": B * ctx, "chunk": a.prefill_chunk, "s": round(t_prefill, 4), "tok_per_s": round(B * ctx / t_prefill, 1),
                         "tflops": round(2 * params * B * ctx / t_prefill / 1e12, 1),
                         "path": "tcgen05 GEMM (INT4 fragment tiles dequantised to fp16 into tensor memory as the "
