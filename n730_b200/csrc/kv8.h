@@ -45,6 +45,12 @@ int kv8_attention_launch(const KV8AttnCall& a, cudaStream_t st);
 
 // The tensor-memory kernel for prompts (kv8_prompt.cu): 256 rows of an item a CTA; the positions of the first `tail`
 // tiles are cut into `splits` shares whose parts lie as [item][tail tile][split][rg rows].
+constexpr int KV8_PROMPT_TILE = 128;  // positions of a tile
+// How many of the planned shares a row tile uses whose rows see `sees` positions: each gets four tiles of them at least.
+// The plan knows the table's width alone.
+__device__ __forceinline__ int kv8_shares_used(int sees, int splits) {
+  return min(splits, max(1, (sees + KV8_PROMPT_TILE - 1) / KV8_PROMPT_TILE / 4));
+}
 struct KV8PromptPlan { int rows, tiles, tail, splits, rg, shares; };  // shares: of the rows, for the weights
 KV8PromptPlan kv8_prompt_plan(const N730KV8Cache& c, int batch, int tokens, int heads);
 int kv8_prompt_launch(const KV8AttnCall& k, const KV8PromptPlan& p, int* status, float* part, float* part_ml, float* lse,

@@ -690,7 +690,7 @@ constexpr int KF_POSITIONS = 4 * KF_THREADS;
 struct KFArgs {
   KDArgs d;
   int rg, rb;
-  int splits;  // parts of every item, one behind the other (prompts); 0: by the table
+  int splits;  // room for parts of an item, one behind the other (prompts); 0: by the parts table
   const float* w_in; float* w_out;
   int64_t ldw;
 };
@@ -698,9 +698,6 @@ struct KFArgs {
 // An item's parts: row r of part k lies in the first CTA's second slot (k = 0), the others' first.
 __device__ __forceinline__ int64_t kf_row(const KFArgs& a, const int2& p, int k, int r) {
   return (a.splits ? (int64_t)(p.x + k) : (int64_t)(2 * (p.x + k) + (k == 0))) * a.rg + r;
-}
-__device__ __forceinline__ int2 kf_parts(const KFArgs& a, int64_t item) {
-  return a.splits ? make_int2((int)item * a.splits, a.splits) : a.d.parts[item];
 }
 // A warp's log2 of the softmax sum of row r over the parts (+inf for an empty row).
 __device__ __forceinline__ float kf_lse_of(const KFArgs& a, const int2& p, int r) {
@@ -743,7 +740,14 @@ __global__ void __launch_bounds__(KF_THREADS) kv8_finish_kernel(const KFArgs a) 
   if ((int)blockIdx.x < joins) {
     const int rg = blockIdx.x / (a.rg / a.rb), first = blockIdx.x % (a.rg / a.rb) * a.rb, f0 = rg * a.rg;
     if (f0 + first >= rows_b) return;
-    const int2 p = kf_parts(a, ((int64_t)b * c.n_kv + h) * d.nrg + rg);
+    const int64_t item = ((int64_t)b * c.n_kv + h) * d.nrg + rg;
+    int2 p;
+    if (a.splits) {  // as many as the prompt kernel used for what the rows see
+      const int sees = (int)min((int64_t)kd_len(d, b, cap) + (min(f0 + a.rg, rows_b) - 1) / d.group + 1, (int64_t)cap);
+      p = make_int2((int)item * a.splits, kv8_shares_used(sees, a.splits));
+    } else {
+      p = d.parts[item];
+    }
     if (p.y == 1) return;  // its CTA gave the answer
     const int per_row = a.rb >= WARPS ? 1 : WARPS / a.rb;  // warps
     const int shares = per_row * (32 / LPP), mine = warp % per_row * (32 / LPP) + lane / LPP, d4 = lane % LPP;
@@ -801,7 +805,7 @@ __global__ void __launch_bounds__(KF_THREADS) kv8_finish_kernel(const KFArgs a) 
   if (rows_b) {
     load(0);
     for (int f = warp; f < rows_b; f += KF_THREADS / 32) {
-      const int2 p = kf_parts(a, head * d.nrg + f / a.rg);
+      const int2 p = d.parts[head * d.nrg + f / a.rg];
       const float lse = p.y == 1 ? d.lse[head * d.rows + f] : kf_lse_of(a, p, f % a.rg);
       if (lane == 0) kf_lse[f] = lse;
     }

@@ -36,7 +36,7 @@
 namespace n730 {
 
 constexpr int KP_ROWS = 256;      // query rows of a CTA
-constexpr int KP_KEYS = 128;      // positions of a tile
+constexpr int KP_KEYS = KV8_PROMPT_TILE;  // positions of a tile
 // Twelve warps leave 168 registers a thread: the softmax holds a row's 128 scores (reading tensor memory twice
 // cost as much as the arithmetic).
 constexpr int KP_THREADS = 12 * 32;
@@ -376,9 +376,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
   // all items' last tiles first, which see most, the tail's shares at the end
   const int items = a.batch * c.n_kv, unit = (int)blockIdx.x / items, item = (int)blockIdx.x % items, whole = a.tiles - a.tail;
   const int b = item / c.n_kv, h = item % c.n_kv;
-  const bool part = unit >= whole;
-  const int splits = part ? a.splits : 1, split = part ? (unit - whole) % a.splits : 0;
-  const int tile = part ? a.tail - 1 - (unit - whole) / a.splits : a.tiles - 1 - unit;
+  const bool tail = unit >= whole;
+  const int split = tail ? (unit - whole) % a.splits : 0;
+  const int tile = tail ? a.tail - 1 - (unit - whole) / a.splits : a.tiles - 1 - unit;
   const int cap = c.max_pages * c.page_size;
   pdl_wait();
   const int L = kv8_len(a.lens, b, cap), n_new = kv8_new(a.n_new, b, a.tokens);
@@ -387,8 +387,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
   // positions [p_lo, p_hi) of this share: what the tile's last row sees, cut into whole tiles
   const int sees_last = (int)min((int64_t)L + (f0 + nrow - 1) / a.group + 1, (int64_t)cap);
   const int sees_all = (int)min((int64_t)L + f0 / a.group + 1, (int64_t)cap);
-  const int all_tiles = (sees_last + KP_KEYS - 1) / KP_KEYS;
-  const int j0 = (int)((int64_t)all_tiles * split / splits), nt = (int)((int64_t)all_tiles * (split + 1) / splits) - j0;
+  const int all_tiles = (sees_last + KP_KEYS - 1) / KP_KEYS, used = tail ? kv8_shares_used(sees_last, a.splits) : 1;
+  if (split >= used) return;
+  const bool part = used > 1;
+  const int j0 = (int)((int64_t)all_tiles * split / used), nt = (int)((int64_t)all_tiles * (split + 1) / used) - j0;
   const int64_t head = (int64_t)b * c.n_kv + h;
 
   if (tid == 0) {
@@ -639,7 +641,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv8_prompt_kernel(const KPArgs 
       // by two factors, whose product may leave fp32's normal range when the answer does not; a NaN query: NaN
       const float s = l == 0.f ? 0.f : 1.f / l, f2 = l == 0.f || mo_ref == -INFINITY ? 0.f : ex2(mo_ref - m_ref);
       const int64_t at = ((int64_t)b * a.tokens + f / a.group) * a.ldo + (int64_t)(h * a.group + f % a.group) * HD;
-      const int64_t slot = ((head * a.tail + tile) * splits + split) * KP_ROWS + r;
+      const int64_t slot = ((head * a.tail + tile) * a.splits + split) * KP_ROWS + r;
 #pragma unroll 1
       for (int cc = 0; cc < HD / 32; ++cc) {
         float v[32];
@@ -888,8 +890,9 @@ KV8PromptPlan kv8_prompt_plan(const N730KV8Cache& c, int batch, int tokens, int 
   const int64_t idle = num_sms() / (items * key_tiles);
   p.shares = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(KW_SHARES, idle), p.rows / (2 * KP_KEYS)));
   // The last, partial wave of CTAs (or the only one) leaves SMs idle: its tiles' positions are cut into as many shares
-  // as there are SMs, of four tiles at least.  2048 tokens behind 6144 positions, 64 / 8 heads, 3.46 waves: 614 us
-  // without, 575 with; shares of three tiles (4 prompts of 300 tokens, 700 positions) 49.8 us for 42.3 without.
+  // as there are SMs, of four tiles at least (of the table's here, of those that a row tile sees on the device).  2048
+  // tokens behind 6144 positions, 64 / 8 heads, 3.46 waves: 614 us without, 578 with; shares of three tiles (4 prompts of
+  // 300 tokens, 700 positions) 49.8 us for 42.3 without.
   p.splits = 1;
   const int64_t tail = (items * p.tiles % num_sms() + items - 1) / items;
   while (tail && tail * items * (p.splits + 1) <= num_sms() && key_tiles / (p.splits + 1) >= 4) ++p.splits;

@@ -394,6 +394,22 @@ def test_workspace_of_a_type(dtype, T):
         assert (ws[need:] == 0x5a).all() and (ws[:4] == 0).all()
 
 
+@pytest.mark.parametrize("dim,heads,T,lens", [(64, 4, 70, [0, 300]), (128, 14, 300, [40, 0])])
+def test_short_prompts_in_a_wide_table(dim, heads, T, lens):
+    """A table of 8192 positions: rows that see fewer than eight tiles of 128 are answered without parts."""
+    rng = np.random.default_rng(T)
+    t = torch()
+    d = OnDevice(make(rng, 2, 128, 2, dim, 64, 16, "int8"))
+    need = d.h.attention_workspace(2, T, heads, dtype="f16")
+    ws = t.full((need,), 0x5a, dtype=t.uint8, device="cuda")
+    ws[:4] = 0
+    check_attention(d, rng.standard_normal((2, T, heads, dim)), "f16", np.array(lens), ws=ws)
+    assert (ws[4:] == 0x5a).all()
+    # one sequence sees enough for two shares, the other does not
+    lens = np.array([1300, lens[1]])
+    out, _ = check_attention(d, rng.standard_normal((2, T, heads, dim)), "f16", lens, weights=rng.random((2, 2, 8192)))
+
+
 def one_hot_cache(rng, pages, dim=64):
     """One sequence, one KV head; every 16th key scores 0 and has no V, the others are -100 in channel 0; scales 1."""
     d = OnDevice(make(rng, 1, pages, 1, dim, 64, 16, "int8", spare=0))
