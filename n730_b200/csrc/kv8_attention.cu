@@ -36,8 +36,10 @@
 // are fp32.
 //
 // Bound by HBM: 2 head_dim code bytes and 8 / block of scales a position and KV head.  Whole calls: 128 sequences
-// ragged to 4096, 64 / 8 heads x 128, e4m3, 113.5 us (5.36 TB/s); one of 65501 positions 36.4 us, of which 5 start
-// and 5 join; 32 ragged to 8192 of 28 / 4 heads with weights 52.6 us, 31 here and 13 in the finishing kernel.
+// ragged to 4096, 64 / 8 heads x 128, e4m3, 116.5 us (5.2 TB/s); one of 65501 positions 36.5 us, of which 5 start
+// and 5 join; 32 ragged to 8192 of 28 / 4 heads with weights 53.7 us, 31 here and 13 in the finishing kernel.  fp32 rows
+// take two products for each one: 64 sequences of 2048, 28 / 4 heads, 47.2 us for 39.0 of 16-bit rows, and a prompt of
+// 300 behind 724 543 us, every 8 rows reading the context.
 #include <algorithm>
 #include <mutex>
 
@@ -828,7 +830,9 @@ __global__ void __launch_bounds__(KF_THREADS) kv8_finish_kernel(const KFArgs a) 
 // host
 // ---------------------------------------------------------------------------
 // Rows of an item from which the prompt kernel takes a call: below, its 256-row tiles are mostly empty and
-// the split kernel's 16-row groups read K and V few enough times.
+// the split kernel's 16-row groups read K and V few enough times.  28 / 4 heads x 128, split / prompt kernel: one sequence
+// behind 2048 positions, 63 rows 18.4 / 29.0 us, 252 rows 26.7 / 35.5; 8 behind 4096, 35 rows 41.7 / 45.0, 63 rows
+// 51.2 / 46.5, 252 rows 137 / 55; 32 behind 2048, 35 rows 67.9 / 61.5, 63 rows 86 / 62.
 constexpr int KD_ROWS_MAX = 64;
 
 struct KDPlan {
@@ -949,7 +953,9 @@ static int finish_launch(const KV8AttnCall& k, const KDPlan& p, const KDArgs& a,
   f.splits = p.prompt ? p.pp.splits : 0;
   f.w_in = w_in; f.w_out = k.w_out; f.ldw = k.ldw;
   const int cap = k.c.max_pages * k.c.page_size;
-  // rows of a block: one where that leaves the SMs few blocks, more where most items have one part
+  // rows of a block: one where that leaves the SMs few blocks, more where most items have one part.  From 8 x SMs on; from
+  // 2 x and 32 x: 32 sequences with weights 53.5 (51.5, 53.5) us, 64 of 28 / 4 heads 39.8 (38.9, 42.9), 128 of 64 / 8
+  // heads 115.2 (115.2, 119.3)
   const int64_t all_rows = (int64_t)k.batch * k.c.n_kv * p.nrg * p.rg;
   f.rb = 1;
   while (f.rb < p.rg && all_rows / f.rb > 8 * num_sms()) f.rb *= 2;

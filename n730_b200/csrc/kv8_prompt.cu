@@ -18,12 +18,13 @@
 // Softmax.  The weight x V scale of a position is formed by one FMA and one exp2: its exponent is
 // score * (row, block factor) + lv - reference with lv the approximate log2(V scale), and the sum of
 // weights gets each block's sum times 2^(reference - maximum - lv).  Both references follow the largest values lazily (P
-// grows from 2^KV8_P_NEW to 2^KV8_P_MOST meanwhile), so outputs in tensor memory are rescaled only when a row's maximum has grown by that much.
+// grows from 2^KV8_P_NEW to 2^KV8_P_MOST meanwhile), so outputs in tensor memory are rescaled only when a row's maximum
+// has grown by that much.
 //
-// Bounds: per 128x128 tile 2 x 1024 cycles of tensor work for head_dim 128 against 1024 of exp2 and about
-// as many of issue slots on the 4 schedulers, for each of A and B.  Measured: 2048 tokens behind 6144 positions, 64 / 8
-// heads x 128, 575 us, 836 TFLOP/s (0.50 of a large bf16 product): about 2.75k cycles of softmax in a period of
-// 4.6k a tile.
+// Bounds: per tile of 128 positions and head_dim 128, 2 x 512 cycles of tensor work against 1024 of exp2 and about as many
+// of issue slots on the 4 schedulers, for each of A and B.  Measured: 2048 tokens behind 6144 positions, 64 / 8 heads x
+// 128, 578 us, 832 TFLOP/s (0.50 of a large bf16 product): about 2.75k cycles of softmax in a period of 4.6k a tile, 2.2
+// times what the tensor cores or exp2 would need: latency.
 //
 // Numerics: 16-bit queries are exact in fp16 after a power-of-two scaling of their row; the softmax
 // weights are rounded to fp16 (2^-11 of each, below the rounding of a 16-bit output, down to 2^-21 of the largest weight
@@ -886,7 +887,9 @@ KV8PromptPlan kv8_prompt_plan(const N730KV8Cache& c, int batch, int tokens, int 
   p.rg = KP_ROWS;
   const int64_t items = (int64_t)batch * c.n_kv;
   const int64_t key_tiles = ((int64_t)c.max_pages * c.page_size + KP_KEYS - 1) / KP_KEYS;
-  // CTAs of a cluster that share the rows of 128 positions' weights, two row tiles each at least
+  // CTAs of a cluster that share the rows of 128 positions' weights, two row tiles each at least, and no more than the
+  // table's positions leave SMs for: in a wide table one (4 prompts of 300 tokens, 14 / 2 heads x 64, whole call, 42.4 us in
+  // a table of 704 positions, 66.9 in 8192, 78 in 65536, where the grid's CTAs behind the last position count as well)
   const int64_t idle = num_sms() / (items * key_tiles);
   p.shares = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(KW_SHARES, idle), p.rows / (2 * KP_KEYS)));
   // The last, partial wave of CTAs (or the only one) leaves SMs idle: its tiles' positions are cut into as many shares
