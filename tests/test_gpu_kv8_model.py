@@ -14,7 +14,7 @@ import pytest
 from gpu_util import rel_err
 from kv8_ref import Cache, decode
 from n730_b200 import synthetic
-from n730_b200.engine import BIAS_SLOTS, Engine, load_tensors
+from n730_b200.engine import Engine, load_tensors
 from n730_b200.batching import ContinuousBatcher
 from oracle.model import OracleDecoder, apply_rope, attention, rms_norm, swiglu
 from test_gpu_model import _blocks, _oracle_weights
@@ -159,6 +159,7 @@ def test_odd_pools(odd_model, page, pool):
 @pytest.mark.parametrize("prompt", [9, 64])
 def test_large_values_with_exact_gemv(model, prompt):
     """V far beyond fp16's range: with the fp32 GEMV prompts answer like single tokens, by either kernel."""
+    from n730_b200.engine import BIAS_SLOTS
     shape, blocks, w = model
     e = Engine(shape, max_ctx=512, max_batch=1, max_prefill=64, kv_bits=8, exact_gemv=True)
     load_tensors(e, blocks)
