@@ -38,8 +38,8 @@
 // Bound by HBM: 2 head_dim code bytes and 8 / block of scales a position and KV head.  Whole calls: 128 sequences
 // ragged to 4096, 64 / 8 heads x 128, e4m3, 116.5 us (5.2 TB/s); one of 65501 positions 36.5 us, of which 5 start
 // and 5 join; 32 ragged to 8192 of 28 / 4 heads with weights 53.7 us, 31 here and 13 in the finishing kernel.  fp32 rows
-// take two products for each one: 64 sequences of 2048, 28 / 4 heads, 47.2 us for 39.0 of 16-bit rows, and a prompt of
-// 300 behind 724 543 us, every 8 rows reading the context.
+// take two products for each one: 64 sequences of 2048, 28 / 4 heads, 45.6 us for 39.6 of 16-bit rows, and a prompt of
+// 300 behind 724 499 us, every 8 rows reading the context.
 #include <algorithm>
 #include <mutex>
 
@@ -413,8 +413,14 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS_PER_SM) kv8_split_kernel(c
       }
       cp_commit();
       const int st = uses % ST;
-      lost = !kv8_wait(&sm.full[warp][st], (uses / ST) & 1, KD_WAIT_NS);
-      if (lost) break;
+      // the same twice: as a value the verdict costs the two-term form registers (64 sequences of 2048 fp32 rows 47.1 us
+      // for 45.7, a prompt of 300 541 for 499), as a branch the other form (64 of 16-bit rows 40.7 us for 39.6)
+      if (LO) {
+        if (!kv8_wait(&sm.full[warp][st], (uses / ST) & 1, KD_WAIT_NS)) { lost = true; break; }
+      } else {
+        lost = !kv8_wait(&sm.full[warp][st], (uses / ST) & 1, KD_WAIT_NS);
+        if (lost) break;
+      }
       ++uses;
       cp_wait<ST - 1>();
       __syncwarp();
