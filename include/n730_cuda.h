@@ -199,9 +199,9 @@ int n730_kv8_append(const N730KV8Cache* c, const void* d_k, const void* d_v, int
  * [n_kv][head_dim] of d_k and d_v; positions outside [0, d_lens[b]) give zeros. */
 int n730_kv8_read(const N730KV8Cache* c, void* d_k, void* d_v, int dtype, int64_t ld, int batch, int tokens,
                   const int32_t* d_first, const int32_t* d_lens, void* stream);
-/* Bytes of workspace (16-byte aligned) of an n730_kv8_attention call of this size, whatever the type of its
- * rows (negative: a return code).  Zero it once: its first int32 becomes 1 if a device wait ever runs out (the call's outputs
- * are not valid then), the rest does not matter from call to call. */
+/* Bytes of workspace (16-byte aligned) of an n730_kv8_attention call of this size, whatever the type of
+ * its rows (negative: a return code).  Zero it once: its first int32 becomes 1 if a device wait ever runs
+ * out (the call's outputs are not valid then), the rest does not matter from call to call. */
 int64_t n730_kv8_attention_ws(const N730KV8Cache* c, int batch, int tokens, int n_heads, int weights);
 /* The same for rows of one type, which is all that a call of that type asks for: with weights, a 16-bit
  * prompt's is a small part of the other, which has room for fp32 rows' scores. */
@@ -240,7 +240,7 @@ int n730_kv8_evict(const N730KV8Cache* c, int batch, int keep, int first, int re
 /* Self-check of the attention's bounded waits: a warp waits at most wait_ns (up to 1 s) for an arrival that never
  * comes (arrives 0), is there already (1), or comes after half that time, one lane having given up before (2).
  * Synchronous; 0, or N730_TIMEOUT (-15) in the first and last case, through the device error word; the context stays
- * usable. */
+ * usable.  A single poll may take the hardware some milliseconds, so ask for 0.1 s or more in the last case. */
 int n730_kv8_wait_check(int64_t wait_ns, int arrives, void* stream);
 
 /* ---- whole-model engine (replaces N730CudaTransformer.forward's per-op loop,

@@ -371,8 +371,9 @@ __global__ void __launch_bounds__(KV8_THREADS) kv8_read_kernel(const KV8ReadArgs
 // 2304 slots of 4 heads take 14 us, all latency; 256 rows of up to 8192 32 us in one wave, two CTAs an SM (32 registers):
 // the issue slots are 58 % busy, and warps wait for global memory first, for barriers next.  Table widths count too: from
 // EV_KEYS positions on keys are read again, and the outputs' rows are written to their ends (one sequence of 2304 slots,
-// whole call, 20.5 us in a table of 8192 positions, 24.6 in 32768, 30.4 in 65536).  The move is bound by the arithmetic on codes (80 % of the issue slots): 32 x 8 heads cut from
-// up to 8192 slots to 2048, about 43 us; 55 with conversions to and from integers.
+// whole call, 20.5 us in a table of 8192 positions, 24.6 in 32768, 30.4 in 65536).  The move is bound by the arithmetic on
+// codes (80 % of the issue slots): 32 x 8 heads cut from up to 8192 slots to 2048, about 43 us; 55 with conversions to and
+// from integers.
 struct KV8EvictArgs {
   N730KV8Cache c;
   int keep, first, recent, log_block;
