@@ -164,7 +164,8 @@ __device__ __forceinline__ uint4 kv8_encode(const float (&x)[16], float s) {
       float2 v;
       v.x = x[e] == x[e] ? fminf(fmaxf(x[e], -most), most) : 0.f;
       v.y = x[e + 1] == x[e + 1] ? fminf(fmaxf(x[e + 1], -most), most) : 0.f;
-      const float2 q = mul2(v, both(r)), z = fma2(fma2(make_float2(-q.x, -q.y), both(s), v), both(r), q);
+      // the remainder negated: that way -0 stays -0
+      const float2 q = mul2(v, both(r)), z = fma2(fma2(q, both(s), make_float2(-v.x, -v.y)), both(-r), q);
       y[e] = z.x; y[e + 1] = z.y;
     }
   } else {

@@ -107,6 +107,21 @@ def test_append_edges(code):
     d.same_as_reference()
 
 
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("amp", [1.0, 2.0 ** -70])
+def test_append_zeros_keep_their_sign(code, amp):
+    """Zeros of both signs and values that round to them, by either way of dividing (scales below 2^-60 take the other)."""
+    rng = np.random.default_rng(23)
+    d = OnDevice(make(rng, 2, 2, 2, 64, 32, 16, code))
+    k, v = amp * rows(rng, 2, 20, 2, 64), amp * rows(rng, 2, 20, 2, 64)
+    for x in (k, v):
+        x[..., ::4] = -0.0
+        x[..., 1::8] *= 1e-5
+        x[..., 2::8] = 0.0
+    append(d, k, v, "f32", np.array([0, 7]))
+    d.same_as_reference()
+
+
 @pytest.mark.parametrize("dtype,extra,shift", [("f16", 8, 0), ("f16", 3, 0), ("bf16", 0, 1), ("f32", 5, 3), ("f16", 0, 8)])
 def test_append_and_read_strides(dtype, extra, shift):
     """Rows inside wider rows, at addresses that are not 16-byte aligned."""
