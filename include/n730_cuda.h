@@ -148,6 +148,20 @@ int n730_qgemm(void* qw, const float* d_x, int ldx, int tokens, float* d_y, int 
  * receives u (may be null).  Asynchronous on `stream`. */
 int n730_sample(const float* d_logits, int batch, int vocab, int ld, float temperature, float top_p,
                 uint64_t seed, uint64_t counter, int32_t* d_tokens, float* d_u, void* stream);
+/* Sampling with each row's own settings and given random numbers: for each of `batch` rows of d_logits
+ * (type N730_F32 / F16 / BF16, row stride ld >= vocab, up to 2^24 of each), d_temperature <= 0 gives the first
+ * index of the largest logit; otherwise tokens are ordered by logit (ties by index) with weights
+ * w = exp((logit - largest) / temperature), and kept are the first d_top_k of them (<= 0: all), of those the
+ * shortest prefix whose mass reaches d_top_p times theirs (>= 1 or NaN: all), and of those the ones with
+ * w >= d_min_p (<= 0 or NaN: all); one token always is.  The token is the first whose cumulative mass exceeds
+ * d_u[row] (in [0, 1); outside: the nearest of that) times the kept mass.  Logits of -infinity or NaN are no
+ * tokens (a row of them answers -1); beside one of +infinity only its equals have a weight.  Arrays of settings are
+ * on the device, one value a row; null: temperature 1, no cut.  d_tokens [batch] out; d_prob (may be null): the
+ * token's share of the kept mass; d_kept (may be null): how many tokens were kept.  Weights and masses are
+ * formed in 64 bits.  Asynchronous on `stream`, needs no workspace, can be captured into a graph. */
+int n730_sample_rows(const void* d_logits, int dtype, int batch, int vocab, int64_t ld, const float* d_temperature,
+                     const int32_t* d_top_k, const float* d_top_p, const float* d_min_p, const float* d_u,
+                     int32_t* d_tokens, float* d_prob, int32_t* d_kept, void* stream);
 /* Load packed-weight blocks of a .n730 file onto the current device without an intermediate
  * host copy (replaces the per-call Python reads of inference.py:355-366 and the read + dequant
  * of n730core.cpp:192-248): block i at absolute offset offsets[i] becomes out_handles[i] (as
@@ -242,6 +256,76 @@ int n730_kv8_evict(const N730KV8Cache* c, int batch, int keep, int first, int re
  * Synchronous; 0, or N730_TIMEOUT (-15) in the first and last case, through the device error word; the context stays
  * usable.  A single poll may take the hardware some milliseconds, so ask for 0.1 s or more in the last case. */
 int n730_kv8_wait_check(int64_t wait_ns, int arrives, void* stream);
+
+/* ---- many continuations of one prompt (no counterpart in the reference) ----
+ * Rotary positions.  Channels [0, rotary_dim) of a head are rotated, the others stay: the pair (x0, x1) at
+ * position p becomes factor * (x0 cos a - x1 sin a, x1 cos a + x0 sin a) with a = p * d_freq[i]; pair i is
+ * channels (i, i + rotary_dim / 2) in the half layout, (2 i, 2 i + 1) in the interleaved one.  d_freq:
+ * rotary_dim / 2 doubles on the device, radians per position; angles are formed in 64 bits. */
+enum { N730_ROTARY_HALF = 0, N730_ROTARY_INTERLEAVED = 1 };
+typedef struct N730Rotary {
+  const double* d_freq;
+  int32_t rotary_dim, layout;
+  float factor;
+} N730Rotary;
+/* Frequencies theta^(-2 i / rotary_dim) for N730Rotary (host arrays), scaled for contexts longer than the
+ * `trained` positions.  PLAIN: as they are.  LINEAR: all slowed by `factor`.  BASE: theta * factor^(n / (n - 2))
+ * in theta's place, n = rotary_dim.  RAMP: pairs that make more than `high` turns over the trained positions
+ * stay, those below `low` are slowed, those between go linearly by their number; *out_factor is
+ * 0.1 ln(factor) + 1 (1 otherwise).  BANDS: the same by the number of turns itself, without a factor.
+ * Arguments that a scaling does not use are ignored. */
+enum { N730_ROTARY_PLAIN = 0, N730_ROTARY_LINEAR = 1, N730_ROTARY_BASE = 2, N730_ROTARY_RAMP = 3, N730_ROTARY_BANDS = 4 };
+int n730_rotary_frequencies(int rotary_dim, double theta, int scaling, double factor, double low, double high,
+                            int trained, double* freq, float* out_factor);
+/* Rows of d_x, [n_heads][head_dim] each (head_dim up to 512), rotated at positions d_pos[row] into rows of d_y
+ * (type N730_F32 / F16 / BF16, strides in elements; in place with d_y = d_x and one stride, else they must not
+ * overlap).  Computed in fp32.  Asynchronous on `stream`, as everything below. */
+int n730_rotary(const N730Rotary* r, const void* d_x, int64_t ldx, void* d_y, int64_t ldy, int dtype, int64_t rows,
+                int n_heads, int head_dim, const int32_t* d_pos, void* stream);
+/* A paged 16-bit cache of one layer, [n_pages][n_kv][page_size][head_dim] (the layout of the engine's own),
+ * behind a prefix that all of a call's sequences share: the prefix's position p lies in page
+ * prefix_table[p / page_size], position p of sequence b's own part in page block_table[b * max_pages +
+ * p / page_size], which stands *prefix_len + p tokens behind the start.  *prefix_len (on the device; below 0
+ * counts as 0, above the table's positions as those) may end inside a page.  prefix_pages 0: no prefix.  A page
+ * id outside [0, n_pages) is no page: rows for it are dropped, attention does not see its positions.
+ * page_size is a multiple of 16, head_dim 64 or 128, pools are 16-byte aligned, dtype is N730_F16 or N730_BF16.
+ * The prompt's own rows are appended through a cache whose block table is the prefix's (batch 1, no prefix).
+ * All pointers are device memory of the current device and belong to the caller; calls allocate nothing, can
+ * be captured into a graph, and need a workspace each where they may overlap in time.  d_lens[b]: own positions
+ * cached before the call (below 0 counts as 0, above the table's as those); d_new[b]: rows of the call's
+ * `tokens` that sequence b has (null: all); token t of sequence b is row b * tokens + t. */
+typedef struct N730KV16Cache {
+  void* k;
+  void* v;
+  const int32_t* block_table;
+  const int32_t* prefix_table;
+  const int32_t* prefix_len;
+  int32_t n_pages, max_pages, prefix_pages, n_kv, head_dim, page_size, dtype;
+} N730KV16Cache;
+/* Append rows of K and V, [n_kv][head_dim] each, behind the cached positions, K rotated by r (null: as it is) and
+ * both rounded to the cache's type; with d_q, query rows [n_heads][head_dim] are rotated into d_q_out as well
+ * (in place with d_q_out = d_q).  Positions are d_pos[row] (null: *prefix_len + d_lens[b] + t).  Rows past the
+ * table's capacity are dropped, rows from d_new[b] on left as they were.  d_lens is not changed.  Pages that are
+ * written must not be shared between sequences. */
+int n730_kv16_append(const N730KV16Cache* c, const N730Rotary* r, const void* d_q, int64_t ldq, void* d_q_out,
+                     int64_t ldqo, int n_heads, const void* d_k, const void* d_v, int64_t ld, int dtype, int batch,
+                     int tokens, const int32_t* d_lens, const int32_t* d_new, const int32_t* d_pos, void* stream);
+
+/* Bytes of workspace (16-byte aligned) of an n730_kv16_attention call of this size (negative: a return code).  Zero
+ * it once: its first int32 becomes 1 if a device wait ever runs out (the call's outputs are not valid then), the rest
+ * does not matter from call to call. */
+int64_t n730_kv16_attention_ws(const N730KV16Cache* c, int batch, int tokens, int n_heads);
+/* Attention of the `tokens` newest rows of each sequence (d_new[b] of them) over the prefix and its own positions:
+ * query t of sequence b, RoPE applied, sees the prefix and own positions [0, d_lens[b] + t] - call it after
+ * n730_kv16_append with the same d_lens and d_new.  Keys and values of the prefix are read once for the whole batch.
+ * d_q and d_out rows are [n_heads][head_dim] of the cache's type (query head i reads KV head i / (n_heads / n_kv));
+ * out rows from d_new[b] on are left as they were; a query that sees no position gives zeros.  d_out must not overlap
+ * d_q.  Scores are scaled by `scale`.  Softmax weights are rounded to the cache's type before they meet V; sums and
+ * outputs are fp32 until the end.  What lies behind a sequence's or the prefix's last position may be anything, NaN
+ * included. */
+int n730_kv16_attention(const N730KV16Cache* c, const void* d_q, int64_t ldq, int batch, int tokens, int n_heads,
+                        float scale, const int32_t* d_lens, const int32_t* d_new, void* d_out, int64_t ldo, void* d_ws,
+                        int64_t ws_bytes, void* stream);
 
 /* ---- whole-model engine (replaces N730CudaTransformer.forward's per-op loop,
  * src-code/inference.py:259-669) ---- */

@@ -16,7 +16,7 @@ from pathlib import Path
 LIB_DIR = Path(__file__).resolve().parent / "lib"
 
 vp, fp, bp, pp = C.c_void_p, C.POINTER(C.c_float), C.POINTER(C.c_uint8), C.POINTER(C.c_void_p)
-i32, i64, f32, u64 = C.c_int32, C.c_int64, C.c_float, C.c_uint64
+i32, i64, f32, f64, u64 = C.c_int32, C.c_int64, C.c_float, C.c_double, C.c_uint64
 i64p = C.POINTER(C.c_int64)
 
 _CUDA_SIGS = {
@@ -67,6 +67,12 @@ _CUDA_SIGS = {
     "n730_kv8_evict_ws": ([vp, i32, i32], i64),
     "n730_kv8_evict": ([vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, i64, vp, i64, vp], i32),
     "n730_kv8_wait_check": ([i64, i32, vp], i32),
+    "n730_sample_rows": ([vp, i32, i32, i32, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp], i32),
+    "n730_rotary_frequencies": ([i32, f64, i32, f64, f64, f64, i32, vp, vp], i32),
+    "n730_rotary": ([vp, vp, i64, vp, i64, i32, i64, i32, i32, vp, vp], i32),
+    "n730_kv16_append": ([vp, vp, vp, i64, vp, i64, i32, vp, vp, i64, i32, i32, i32, vp, vp, vp, vp], i32),
+    "n730_kv16_attention_ws": ([vp, i32, i32, i32], i64),
+    "n730_kv16_attention": ([vp, vp, i64, i32, i32, i32, f32, vp, vp, vp, i64, vp, i64, vp], i32),
     "n730_qweight_load_blocks": ([C.c_char_p, i32, vp, vp, vp, vp], i32),
     "n730_tp_wait_check": ([i64, i32, vp], i32),
     "n730_attention_forward_noalloc": ([vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp], i32),
