@@ -1,61 +1,594 @@
-// Attention over the 16-bit paged cache behind a prefix that the batch shares.
+// Attention over the 16-bit paged cache behind a prefix that the batch shares, on the 5th-generation tensor cores.
 //
 //   out[b, t, head] = softmax_p(scale q . k_p) v_p,  p over the prefix and own positions <= lens[b] + t
+//
+// The softmax over a row's positions is cut into parts, each (sum of weights x values, reference, sum of weights), that a
+// finishing kernel joins.  A part is an item of work: up to 128 or 256 query rows of a KV head that read the same keys and
+// values.  Of the prefix these are rows of ALL sequences, row = (b * tokens + t) * G + g, so that a key is read once for
+// the whole batch (once for 256 rows) and the products are full tiles; of a sequence's own part they are its tokens x G
+// rows.  Items of few rows, or of long positions, are cut along the positions so that every SM has some.
+//
+// A CTA takes one item.  Warps 0-3 (and 4-7 with two row tiles): softmax, a thread a row.  The next warp brings K and V
+// by tensor copies, the last one issues S = Q K^T (both from shared memory, K-major) and O += P V (P in tensor memory, V
+// MN-major), of the two row tiles in turn so that one's products run under the other's softmax.  P, rounded to the cache's
+// type, overwrites its scores.  With one row tile two CTAs share an SM to the same end.  Pages are copied as they lie,
+// 16 to 128 rows a copy; positions without a page are copied from behind the pool's end, which gives zeros.
+//
+// Softmax.  A row's reference follows its maximum lazily: it moves when a weight would pass 2^KA_MOST, so outputs in
+// tensor memory are seldom rescaled.  Weights are at most 2^8, the largest at least 1: fp16 holds them to 2^-11, and
+// those below 2^-14 to 2^-25.
+//
+// What lies behind the last position anyone sees may be anything: scores are masked, and those rows of V are zeroed in
+// shared memory before the product (zero weight times NaN is NaN).  Rows of V that some rows of the item see and others
+// do not (tokens of the same call) are zeroed where they are not finite; rows that see them add them by themselves.
+//
+// Every wait is bounded; one that runs out sets the workspace's status word, ends the CTA's work and still frees the
+// tensor memory.
+#include <algorithm>
 #include <cmath>
+#include <mutex>
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
 
 #include "kv16.h"
+#include "tcgen05.cuh"
 
 namespace n730 {
 
-struct KSArgs {
+constexpr int KA_KEYS = 128;       // positions of a tile
+constexpr float KA_MOST = 8.f;     // log2 of how large a weight may grow against its reference
+constexpr int KA_RING = 4;         // tiles whose masks are kept
+constexpr int KA_BAD = 256;        // positions of an item that some of its rows see and others do not: fewer than its rows
+
+template <int HD, int NT>
+struct KACfg {
+  static constexpr int NB = HD / 64;                               // 64-channel blocks
+  static constexpr int ROWS = NT * 128;
+  static constexpr int QB = ROWS * 128, KB = KA_KEYS * 128;        // bytes of a block of Q, of K or V
+  static constexpr int KV = NB * KB;                               // bytes of a tile of K or V
+  static constexpr int STAGES = NT == 2 || HD == 64 ? 2 : 1;       // one row tile of 128 channels: 96 KB, two CTAs an SM
+  static constexpr int COPY_WARP = NT * 4, MMA_WARP = NT * 4 + 1, THREADS = (NT * 4 + 2) * 32;
+  static constexpr uint32_t TMEM = NT == 1 ? 256u : 512u;
+  static constexpr uint32_t S0 = 0, O0 = NT * KA_KEYS;             // columns: scores, outputs
+};
+// kind::f16: D fp32, A and B of the cache's type, M = 128
+template <bool BF>
+constexpr uint32_t ka_idesc(int n, bool mn_major) {
+  return (1u << 4) | (BF ? (1u << 7) | (1u << 10) : 0u) | (mn_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+
+template <int HD, int NT>
+struct KASmem {
+  using Cfg = KACfg<HD, NT>;
+  uint8_t q[Cfg::NB * Cfg::QB];
+  uint8_t k[Cfg::STAGES][Cfg::KV];
+  uint8_t v[Cfg::STAGES][Cfg::KV];
+  uint32_t pages[KA_RING];   // bit i: positions 16 i .. 16 i + 15 of the tile have a page
+  uint64_t qready, kfull[2], vfull[2], kfree[2], vfree[2], sfull[2], pready[2], odone[2], drain;
+  uint32_t tmem;
+  int abort;
+  int n_bad, bad[KA_BAD];
+};
+
+// Parts of one kind (the prefix's or the sequences' own): [unit][split][rows of a unit], a unit being a KV head, or a
+// sequence and a KV head.
+struct KAParts {
+  int tiles, splits, rows;   // row tiles of a unit, shares of the positions, tiles * rows of a tile
+  float* o;
+  float2* ml;                // reference (log2) and sum of weights
+};
+struct KAArgs {
   N730KV16Cache c;
   const void* q; void* out;
   int64_t ldq, ldo;
-  int batch, tokens, heads;
-  float scale;
+  int batch, tokens, heads, group;
+  int prefix_items, box;
+  bool qvec, ovec;
+  float scale_log2e;         // its absolute value; the sign goes with the queries
+  uint32_t sign;
   const int* lens; const int* n_new;
+  int* status;
+  KAParts pre, own;
 };
 
-constexpr int KS_THREADS = 128;
+// shares of the positions that are used: the plan knows the tables' widths alone
+__device__ __forceinline__ int ka_used(int n, int splits) { return min(splits, (n + KA_KEYS - 1) / KA_KEYS); }
 
-// A CTA takes one query row: scores of 128 positions, a thread each, then outputs, a thread a channel.
-__global__ void __launch_bounds__(KS_THREADS) kv16_simple_kernel(const KSArgs a) {
-  __shared__ float q[128], p[KS_THREADS], red[32];
-  __shared__ int64_t row[KS_THREADS];
-  const N730KV16Cache& c = a.c;
-  const int tid = threadIdx.x, D = c.head_dim, b = blockIdx.x / a.tokens, t = blockIdx.x % a.tokens, head = blockIdx.y;
-  if (t >= kv8_new(a.n_new, b, a.tokens)) return;
-  const int h = head / (a.heads / c.n_kv), cap = c.max_pages * c.page_size;
-  const int prefix = kv16_prefix(c), own = min(kv8_len(a.lens, b, cap) + t + 1, cap), n = prefix + own;
-  if (tid < D) q[tid] = kv8_load1(a.q, (int64_t)blockIdx.x * a.ldq + (int64_t)head * D + tid, c.dtype) * a.scale;
-  float m = -INFINITY, l = 0.f, acc = 0.f;
-  for (int j0 = 0; j0 < n; j0 += KS_THREADS) {
-    __syncthreads();
-    const int j = j0 + tid;
-    int page = -1, off = 0;
-    if (j < prefix) { page = c.prefix_table[j / c.page_size]; off = j % c.page_size; }
-    else if (j < n) { page = c.block_table[(int64_t)b * c.max_pages + (j - prefix) / c.page_size]; off = (j - prefix) % c.page_size; }
-    const bool here = (unsigned)page < (unsigned)c.n_pages;
-    row[tid] = here ? (((int64_t)page * c.n_kv + h) * c.page_size + off) * D : -1;
-    float x = -INFINITY;
-    if (here) {
-      x = 0.f;
-      for (int d = 0; d < D; ++d) x = fmaf(q[d], kv8_load1(c.k, row[tid] + d, c.dtype), x);
+template <bool BF>
+__device__ __forceinline__ float2 ka_wide(uint32_t x) {
+  return BF ? make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)) : __half22float2(u2h(x));
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t ka_pack(float a, float b) {
+  if (!BF) return h2u(__floats2half2_rn(a, b));
+  const __nv_bfloat162 y = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+
+// 2-D tensor copy of a box of the pool into shared memory (channel c0, row c1 of the pool)
+__device__ __forceinline__ void ka_copy(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               :: "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// Moves a row's reference to its tile's maximum y where that is larger; its sum and, when there are any, outputs follow.
+template <int HD>
+__device__ __forceinline__ void ka_move(uint32_t to, bool outputs, float y, float& m, float& l) {
+  const float mn = fmaxf(m, y), f = mn == m ? 1.f : ex2(m - mn);
+  m = mn;
+  l *= f;
+  if (!outputs) return;
+#pragma unroll 1
+  for (int cc = 0; cc < HD; cc += 8) tc_scale8(to + cc, f);
+}
+
+// One tile of a row whose positions are all seen: weights over the scores at ts, their sum to l.
+template <int HD, bool BF>
+__device__ __forceinline__ void ka_softmax(uint32_t ts, uint32_t to, float c, bool outputs, float& m, float& l) {
+  float v[KA_KEYS];
+  tc_ld64(ts, v);
+  tc_ld64(ts + 64, v + 64);
+  float mx[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+  for (int i = 4; i < KA_KEYS; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
+  const float y = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+  if (__any_sync(0xffffffffu, y > m + KA_MOST)) ka_move<HD>(to, outputs, y, m, l);
+  const float ms = m == -INFINITY ? 0.f : m;
+  const float2 c2 = both(c), m2 = both(-ms);
+  float2 sum[2] = {both(0.f), both(0.f)};
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    uint32_t w[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float2 x = fma2(make_float2(v[half * 64 + 2 * i], v[half * 64 + 2 * i + 1]), c2, m2);
+      const float2 p = make_float2(ex2(x.x), ex2(x.y));
+      sum[i & 1] = add2(sum[i & 1], p);
+      w[i] = ka_pack<BF>(p.x, p.y);
     }
-    float mx = warp_max(x);
-    if ((tid & 31) == 0) red[tid >> 5] = mx;
-    __syncthreads();
-    mx = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-    const float ms = mx == -INFINITY ? 0.f : mx, f = expf(m - ms), e = here ? expf(x - ms) : 0.f;
-    p[tid] = e;
-    m = mx;
-    l = l * f + block_sum(e, red);
-    acc *= f;
-    if (tid < D)
-      for (int k = 0; k < KS_THREADS; ++k)
-        if (row[k] >= 0) acc = fmaf(p[k], kv8_load1(c.v, row[k] + tid, c.dtype), acc);
+    tc_st32(ts + half * 32, w);
   }
-  if (tid < D) kv8_store1(a.out, (int64_t)blockIdx.x * a.ldo + (int64_t)head * D + tid, c.dtype, l == 0.f ? 0.f : acc / l);
+  const float2 s = add2(sum[0], sum[1]);
+  l += s.x + s.y;
+}
+// The same where the row sees the first `sees` positions, of those the ones that have a page.
+template <int HD, bool BF>
+__device__ __forceinline__ void ka_softmax_some(uint32_t ts, uint32_t to, float c, int sees, uint32_t pages, bool outputs,
+                                                float& m, float& l) {
+  float mx = -INFINITY;
+#pragma unroll 1
+  for (int cc = 0; cc < 4; ++cc) {
+    float v[32];
+    tc_ld32(ts + cc * 32, v);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) mx = fmaxf(mx, cc * 32 + i < sees && (pages >> (2 * cc + i / 16) & 1) ? v[i] : -INFINITY);
+  }
+  const float y = mx * c;
+  const float yy = mx == -INFINITY ? -INFINITY : y;  // c may be 0
+  if (__any_sync(0xffffffffu, yy > m + KA_MOST)) ka_move<HD>(to, outputs, yy, m, l);
+  const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+  for (int c2 = 0; c2 < 2; ++c2) {  // 64 positions: 32 columns of P over scores that have been read
+    uint32_t w[32];
+    float sum = 0.f;
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      float v[32];
+      tc_ld32(ts + c2 * 64 + hh * 32, v);
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        const int at = c2 * 64 + hh * 32 + i;
+        const bool here = pages >> (at >> 4) & 1;
+        const float p0 = at < sees && here ? ex2(fmaf(v[i], c, -ms)) : 0.f;
+        const float p1 = at + 1 < sees && here ? ex2(fmaf(v[i + 1], c, -ms)) : 0.f;
+        sum += p0 + p1;
+        w[hh * 16 + i / 2] = ka_pack<BF>(p0, p1);
+      }
+    }
+    l += sum;
+    tc_st32(ts + c2 * 32, w);
+  }
+}
+
+template <int HD, bool BF, int NT>
+__global__ void __launch_bounds__(KACfg<HD, NT>::THREADS, NT == 1 ? 2 : 1)
+kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  using Cfg = KACfg<HD, NT>;
+  constexpr int ST = Cfg::STAGES;
+  extern __shared__ __align__(1024) uint8_t ka_raw[];
+  KASmem<HD, NT>& sm = *reinterpret_cast<KASmem<HD, NT>*>(aligned_smem(ka_raw));
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const N730KV16Cache& c = a.c;
+  const int cap = c.max_pages * c.page_size, G = a.group;
+
+  // the item: rows [f0, f0 + nrow) of KV head h, positions [0, sees) of which every row sees the first sees_all
+  int i = (int)blockIdx.x;
+  const bool pre = i < a.prefix_items;
+  if (!pre) i -= a.prefix_items;
+  const KAParts& part = pre ? a.pre : a.own;
+  const int tile = part.tiles - 1 - i % part.tiles;
+  i /= part.tiles;
+  const int h = i % c.n_kv;
+  i /= c.n_kv;
+  const int b = pre ? 0 : i % a.batch, split = pre ? i : i / a.batch;
+  const int f0 = tile * Cfg::ROWS;
+  int L = 0, nrow, sees, sees_all;
+  if (pre) {
+    nrow = min(Cfg::ROWS, a.batch * a.tokens * G - f0);
+    sees = sees_all = kv16_prefix(c);
+  } else {
+    L = kv8_len(a.lens, b, cap);
+    nrow = min(Cfg::ROWS, kv8_new(a.n_new, b, a.tokens) * G - f0);
+    sees = min(L + (f0 + nrow - 1) / G + 1, cap);
+    sees_all = min(L + f0 / G + 1, cap);
+  }
+  const int used = ka_used(sees, part.splits);
+  if (nrow <= 0 || split >= used) {
+    if (blockIdx.x == 0) pdl_wait();
+    return;
+  }
+  const int all_tiles = (sees + KA_KEYS - 1) / KA_KEYS;
+  const int j0 = (int)((int64_t)all_tiles * split / used), nt = (int)((int64_t)all_tiles * (split + 1) / used) - j0;
+  const int* table = pre ? c.prefix_table : c.block_table + (int64_t)b * c.max_pages;
+
+  if (tid == 0) {
+    mbar_init(&sm.qready, NT * 4);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&sm.kfull[s], 1);
+      mbar_init(&sm.vfull[s], 1);
+      mbar_init(&sm.kfree[s], 1);
+      mbar_init(&sm.vfree[s], 1);
+      mbar_init(&sm.sfull[s], 1);
+      mbar_init(&sm.pready[s], 4);
+      mbar_init(&sm.odone[s], 1);
+    }
+    mbar_init(&sm.drain, 1);
+    fence_mbar_init();
+    sm.abort = 0;
+    sm.n_bad = 0;
+  }
+  if (warp == Cfg::MMA_WARP) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 :: "r"(smem_u32(&sm.tmem)), "r"(Cfg::TMEM) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_dependents();
+  const uint32_t tmem = sm.tmem;
+  volatile int* abortf = &sm.abort;
+
+  if (warp == Cfg::COPY_WARP) {
+    // ---------------- K and V: a lane a copy, its page looked up by itself ----------------
+    const int chunks = KA_KEYS / a.box, chunk = lane / Cfg::NB, blk = lane % Cfg::NB;
+    const bool mine = chunk < chunks;
+    const int none = c.n_pages * c.n_kv * c.page_size;  // the first row behind the pool
+    auto row_of = [&](int j) {
+      const int p = (j0 + j) * KA_KEYS + chunk * a.box;
+      if (!mine || p >= sees) return none;
+      const int page = table[p / c.page_size];
+      return (unsigned)page < (unsigned)c.n_pages ? (page * c.n_kv + h) * c.page_size + p % c.page_size : none;
+    };
+    const int at = blk * Cfg::KB + chunk * a.box * 128;
+    int row = row_of(0), nk = 0, nv = 0;  // tiles asked for
+    for (int j = 0; j < nt; ++j) {
+      const int s = j % ST;
+      const uint32_t ph = (uint32_t)((j / ST - 1) & 1);
+      // the tile's pages, 16 positions a bit (positions behind the last count as none)
+      const uint32_t has = __ballot_sync(0xffffffffu, row != none && blk == 0);
+      const int next = j + 1 < nt ? row_of(j + 1) : none;
+      if (j >= ST && !kp_wait_warp(&sm.kfree[s], ph, abortf)) break;
+      if (lane == 0) {
+        uint32_t m = 0;
+        for (int k = 0; k < chunks; ++k)
+          if (has >> (k * Cfg::NB) & 1) m |= ((1u << (a.box / 16)) - 1) << (k * (a.box / 16));
+        sm.pages[j % KA_RING] = m;
+        mbar_arrive_expect_tx(&sm.kfull[s], Cfg::KV);
+      }
+      __syncwarp();
+      if (mine) ka_copy(sm.k[s] + at, &kmap, blk * 64, row, &sm.kfull[s]);
+      nk = j + 1;
+      if (j >= ST && !kp_wait_warp(&sm.vfree[s], ph, abortf)) break;
+      if (lane == 0) mbar_arrive_expect_tx(&sm.vfull[s], Cfg::KV);
+      __syncwarp();
+      if (mine) ka_copy(sm.v[s] + at, &vmap, blk * 64, row, &sm.vfull[s]);
+      nv = j + 1;
+      row = next;
+    }
+    // copies in flight land before their memory is given up, whatever else gave up
+    for (int j = max(nk - ST, 0); j < nk; ++j) kv8_wait(&sm.kfull[j % ST], (uint32_t)((j / ST) & 1), 2000000000ull);
+    for (int j = max(nv - ST, 0); j < nv; ++j) kv8_wait(&sm.vfull[j % ST], (uint32_t)((j / ST) & 1), 2000000000ull);
+  } else if (warp == Cfg::MMA_WARP) {
+    // ---------------- products ----------------
+    const uint64_t qd = umma_desc_sw128(smem_u32(sm.q)), kd = umma_desc_sw128(smem_u32(sm.k[0]));
+    const uint64_t vd = umma_desc_mn_sw128(smem_u32(sm.v[0]), Cfg::KB);
+    auto scores = [&](int x, int s) {  // S = Q K^T
+      const uint64_t q0 = qd + (uint64_t)(x * 128 * 128 / 16), k0 = kd + (uint64_t)(s * Cfg::KV / 16);
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+          tc_mma_ss<ka_idesc<BF>(KA_KEYS, false)>(tmem + Cfg::S0 + x * KA_KEYS, q0 + (uint64_t)(((k >> 2) * Cfg::QB + (k & 3) * 32) / 16),
+                                                  k0 + (uint64_t)(((k >> 2) * Cfg::KB + (k & 3) * 32) / 16), k > 0);
+        tc_commit(&sm.sfull[x]);
+        if (x == NT - 1) tc_commit(&sm.kfree[s]);
+      }
+      __syncwarp();
+    };
+    auto outputs = [&](int x, int s, bool first) {  // O += P V
+      const uint64_t v0 = vd + (uint64_t)(s * Cfg::KV / 16);
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < KA_KEYS / 16; ++k)
+          tc_mma_ts<ka_idesc<BF>(HD, true)>(tmem + Cfg::O0 + x * HD, tmem + Cfg::S0 + x * KA_KEYS + k * 8, v0 + (uint64_t)(k * 2048 / 16),
+                                            !(first && k == 0));
+        if (x == NT - 1) tc_commit(&sm.vfree[s]);
+      }
+      __syncwarp();
+    };
+    bool go = kp_wait_warp(&sm.qready, 0, abortf) && kp_wait_warp(&sm.kfull[0], 0, abortf);
+    if (go) {
+      tc_fence_after();
+#pragma unroll
+      for (int x = 0; x < NT; ++x) scores(x, 0);
+    }
+#pragma unroll 1
+    for (int j = 0; go && j < nt; ++j) {
+      const int s = j % ST, s1 = (j + 1) % ST;
+      go = kp_wait_warp(&sm.vfull[s], (uint32_t)((j / ST) & 1), abortf);
+#pragma unroll 1
+      for (int x = 0; go && x < NT; ++x) {
+        go = kp_wait_warp(&sm.pready[x], (uint32_t)(j & 1), abortf);
+        if (!go) break;
+        tc_fence_after();
+        outputs(x, s, j == 0);
+        if (j + 1 < nt) {
+          if (x == 0) go = kp_wait_warp(&sm.kfull[s1], (uint32_t)(((j + 1) / ST) & 1), abortf);
+          if (!go) break;
+          tc_fence_after();
+          scores(x, s1);
+        } else {
+          if (elect_one()) tc_commit(&sm.odone[x]);
+          __syncwarp();
+        }
+      }
+    }
+  } else {
+    // ---------------- softmax: a thread a row ----------------
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q);
+    // where row f of the item lies: its token's row, its head
+    auto token = [&](int f) { return pre ? f / G : b * a.tokens + f / G; };
+    {
+      constexpr int LPR = HD / 8, RPI = 32 / LPR, U = 4;
+      const int sub = lane / LPR, ch = lane % LPR;
+#pragma unroll 1
+      for (int r0 = warp * 32; r0 < warp * 32 + 32; r0 += U * RPI) {
+        uint4 x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int r = r0 + u * RPI + sub, f = f0 + r;
+          x[u] = make_uint4(0, 0, 0, 0);
+          if (r >= nrow) continue;
+          const uint16_t* p = q + (int64_t)token(f) * a.ldq + (int64_t)(h * G + f % G) * HD + ch * 8;
+          if (a.qvec) x[u] = *reinterpret_cast<const uint4*>(p);
+          else x[u] = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int r = r0 + u * RPI + sub;
+          *reinterpret_cast<uint4*>(sm.q + (ch >> 3) * Cfg::QB + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) =
+              make_uint4(x[u].x ^ a.sign, x[u].y ^ a.sign, x[u].z ^ a.sign, x[u].w ^ a.sign);
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive1(&sm.qready);
+    }
+    const int x = warp >> 2, wq = warp & 3, r = x * 128 + wq * 32 + lane, f = f0 + r;
+    const bool live = r < nrow;
+    const int vis = !live ? 0 : pre ? sees : min(L + f / G + 1, cap);
+    const uint32_t ts = tmem + ((uint32_t)(wq * 32) << 16) + Cfg::S0 + x * KA_KEYS;
+    const uint32_t to = tmem + ((uint32_t)(wq * 32) << 16) + Cfg::O0 + x * HD;
+    float m = -INFINITY, l = 0.f;
+    bool go = true;
+    for (int j = 0; j < nt; ++j) {
+      if (!kp_wait_warp(&sm.sfull[x], (uint32_t)(j & 1), abortf)) { go = false; break; }
+      tc_fence_after();
+      const int p0 = (j0 + j) * KA_KEYS;
+      const uint32_t pages = sm.pages[j % KA_RING];
+      if (p0 + KA_KEYS <= sees_all && pages == 0xffu) {
+        ka_softmax<HD, BF>(ts, to, a.scale_log2e, j > 0, m, l);
+      } else {
+        ka_softmax_some<HD, BF>(ts, to, a.scale_log2e, vis - p0, pages, j > 0, m, l);
+        if (x == 0 && p0 + KA_KEYS > sees_all) {  // rows of V that not everyone sees
+          if (!kp_wait_warp(&sm.vfull[j % ST], (uint32_t)((j / ST) & 1), abortf)) { go = false; break; }
+          const int row = wq * 32 + lane, p = p0 + row;
+          uint8_t* v = sm.v[j % ST] + row * 128;
+          bool zero = p >= sees;
+          if (p >= sees_all && !zero) {
+#pragma unroll 1
+            for (int e = 0; e < Cfg::NB * 8; ++e) {  // the row's 16 bytes in any order
+              const uint4 y = *reinterpret_cast<const uint4*>(v + (e >> 3) * Cfg::KB + (e & 7) * 16);
+              const uint32_t inf = BF ? 0x7f80u : 0x7c00u, w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) zero = zero || (w[k] & inf) == inf || (w[k] >> 16 & inf) == inf;
+            }
+            if (zero) sm.bad[atomicAdd(&sm.n_bad, 1)] = p;
+          }
+          if (zero)
+#pragma unroll
+            for (int e = 0; e < Cfg::NB * 8; ++e)
+              *reinterpret_cast<uint4*>(v + (e >> 3) * Cfg::KB + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive1(&sm.pready[x]);
+    }
+    if (go) {
+      go = kp_wait_warp(&sm.odone[x], 0, abortf);
+      tc_fence_after();
+    }
+    if (go) {
+      const int n_bad = *reinterpret_cast<volatile int*>(&sm.n_bad);
+      const int64_t unit = ((int64_t)(pre ? h : b * c.n_kv + h) * part.splits + split) * part.rows + f;
+      if (live) part.ml[unit] = make_float2(m, l);
+      const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+      for (int cc = 0; cc < HD; cc += 32) {
+        float o[32];
+        tc_ld32(to + cc, o);
+        if (live && n_bad) {
+          for (int k = 0; k < n_bad; ++k) {
+            const int p = sm.bad[k], page = table[p / c.page_size];
+            if (p >= vis || (unsigned)page >= (unsigned)c.n_pages) continue;
+            const int64_t at = (((int64_t)page * c.n_kv + h) * c.page_size + p % c.page_size) * HD;
+            const int64_t qa = (int64_t)token(f) * a.ldq + (int64_t)(h * G + f % G) * HD;
+            float dot = 0.f;
+            for (int d = 0; d < HD; ++d) dot = fmaf(kv8_load1(a.q, qa + d, c.dtype), kv8_load1(c.k, at + d, c.dtype), dot);
+            const float w = ex2(fmaf(a.sign ? -dot : dot, a.scale_log2e, -ms));
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = fmaf(w, kv8_load1(c.v, at + cc + e, c.dtype), o[e]);
+          }
+        }
+        __syncwarp();
+        if (live) {
+          float4* dst = reinterpret_cast<float4*>(part.o + unit * HD + cc);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (sm.abort) {
+    if (tid == 0) *a.status = 1;
+    if (warp == Cfg::MMA_WARP) {  // products in flight end before tensor and shared memory are given up
+      if (elect_one()) tc_commit(&sm.drain);
+      __syncwarp();
+      kv8_wait(&sm.drain, 0, 2000000000ull);
+    }
+    __syncthreads();
+  }
+  if (warp == Cfg::MMA_WARP)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(Cfg::TMEM));
+  if (blockIdx.x == 0) pdl_wait();  // the kernel behind this one waits for it alone, and so for the one before
+}
+
+// Joins a row's parts: a warp a row, HD / 32 channels a lane.
+constexpr int KJ_WARPS = 4;
+template <int HD, bool BF>
+__global__ void __launch_bounds__(KJ_WARPS * 32) kv16_join_kernel(const KAArgs a) {
+  constexpr int V = HD / 32;
+  const N730KV16Cache& c = a.c;
+  const int lane = threadIdx.x & 31, G = a.group, cap = c.max_pages * c.page_size;
+  const int64_t row = (int64_t)blockIdx.x * KJ_WARPS + (threadIdx.x >> 5);
+  const int64_t rows = (int64_t)a.batch * a.tokens * a.heads;
+  pdl_wait();
+  if (row >= rows) return;
+  const int head = (int)(row % a.heads);
+  const int64_t tok = row / a.heads;
+  const int b = (int)(tok / a.tokens), t = (int)(tok % a.tokens), h = head / G, g = head % G;
+  const int n_new = kv8_new(a.n_new, b, a.tokens);
+  if (t >= n_new) return;
+  // a row's share of its tile's positions: the tile's last row decides
+  const int np = a.pre.o ? ka_used(kv16_prefix(c), a.pre.splits) : 0;
+  const int tile_rows = a.own.rows / a.own.tiles, f = t * G + g, f0 = f / tile_rows * tile_rows;
+  const int last = (min(f0 + tile_rows, n_new * G) - 1) / G;
+  const int no = ka_used(min(kv8_len(a.lens, b, cap) + last + 1, cap), a.own.splits);
+  const int64_t p0 = (int64_t)h * a.pre.splits * a.pre.rows + tok * G + g;
+  const int64_t o0 = (int64_t)(b * c.n_kv + h) * a.own.splits * a.own.rows + f;
+  auto at = [&](int i) { return i < np ? p0 + (int64_t)i * a.pre.rows : o0 + (int64_t)(i - np) * a.own.rows; };
+  const int n = np + no;
+  float big = -INFINITY;
+  for (int i = lane; i < n; i += 32) big = fmaxf(big, (i < np ? a.pre.ml : a.own.ml)[at(i)].x);
+  big = warp_max(big);
+  float acc[V] = {}, sum = 0.f;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    float w = 0.f, l = 0.f;
+    if (i0 + lane < n) {
+      const float2 ml = (i0 + lane < np ? a.pre.ml : a.own.ml)[at(i0 + lane)];
+      w = ml.x == -INFINITY ? 0.f : ex2(ml.x - big);
+      l = ml.y;
+    }
+    // a part without a seen position has no sum either; a NaN stays one
+    sum += warp_sum(l == 0.f ? 0.f : l * w);
+    const int k1 = min(32, n - i0);
+#pragma unroll 4
+    for (int k = 0; k < k1; ++k) {
+      const float wk = __shfl_sync(0xffffffffu, w, k);
+      const float* o = (i0 + k < np ? a.pre.o : a.own.o) + at(i0 + k) * HD + lane * V;
+      if (V == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(o);
+        acc[0] = fmaf(wk, x.x, acc[0]); acc[1] = fmaf(wk, x.y, acc[1]);
+        acc[2 % V] = fmaf(wk, x.z, acc[2 % V]); acc[3 % V] = fmaf(wk, x.w, acc[3 % V]);
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(o);
+        acc[0] = fmaf(wk, x.x, acc[0]); acc[1] = fmaf(wk, x.y, acc[1]);
+      }
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + tok * a.ldo + (int64_t)head * HD + lane * V;
+  uint32_t y[V / 2];
+#pragma unroll
+  for (int e = 0; e < V / 2; ++e) y[e] = ka_pack<BF>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+  if (a.ovec) {
+    if (V == 4) *reinterpret_cast<uint2*>(out) = make_uint2(y[0], y[V / 2 - 1]);
+    else *reinterpret_cast<uint32_t*>(out) = y[0];
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[e] = (uint16_t)(y[e / 2] >> (16 * (e & 1)));
+  }
+}
+
+// ----------------------------------------------------------------------------- plan
+struct KAPlan {
+  int pre_nt, own_nt;              // row tiles of a CTA
+  int pre_tiles, pre_splits, own_tiles, own_splits;
+  int64_t pre_items, own_items;
+  int64_t pre_o, pre_ml, own_o, own_ml, bytes;  // in the workspace
+};
+
+static KAPlan ka_plan(const N730KV16Cache& c, int batch, int tokens, int heads) {
+  KAPlan p{};
+  const int G = heads / c.n_kv, sms = num_sms();
+  const int64_t pre_rows = (int64_t)batch * tokens * G, own_rows = (int64_t)tokens * G;
+  auto cells = [&](int64_t tiles, int splits) { return tiles * splits; };
+  auto shape = [&](int64_t rows, int64_t units, int64_t positions, int& nt, int& tiles, int& splits) {
+    nt = rows > 128 ? 2 : 1;
+    tiles = (int)((rows + nt * 128 - 1) / (nt * 128));
+    const int64_t items = units * tiles, slots = (int64_t)sms * (nt == 1 ? 2 : 1);
+    const int64_t pos = (positions + KA_KEYS - 1) / KA_KEYS;
+    // a share's time: its tiles and what it costs to begin and end; the parts' way through memory
+    double best = 1e30;
+    splits = 1;
+    for (int s = 1; s <= std::min<int64_t>(pos, 64); ++s) {
+      const double waves = (double)((items * s + slots - 1) / slots);
+      const double us = waves * ((double)((pos + s - 1) / s) * 1.2 + 3.0) + (double)(s > 1 ? s : 0) * units * rows * c.head_dim * 8 / 4e6;
+      if (us < best * 0.98) { best = us; splits = s; }
+    }
+  };
+  if (c.prefix_pages) {
+    shape(pre_rows, c.n_kv, (int64_t)c.prefix_pages * c.page_size, p.pre_nt, p.pre_tiles, p.pre_splits);
+    p.pre_items = (int64_t)c.n_kv * p.pre_tiles * p.pre_splits;
+  }
+  shape(own_rows, (int64_t)batch * c.n_kv, (int64_t)c.max_pages * c.page_size, p.own_nt, p.own_tiles, p.own_splits);
+  p.own_items = (int64_t)batch * c.n_kv * p.own_tiles * p.own_splits;
+  auto room = [&](int64_t bytes) { const int64_t at = p.bytes; p.bytes += (bytes + 255) / 256 * 256; return at; };
+  room(256);
+  const int64_t pr = cells(p.pre_tiles, p.pre_splits) * p.pre_nt * 128 * c.n_kv;
+  const int64_t orows = cells(p.own_tiles, p.own_splits) * p.own_nt * 128 * c.n_kv * batch;
+  p.pre_o = room(pr * c.head_dim * 4);
+  p.pre_ml = room(pr * 8);
+  p.own_o = room(orows * c.head_dim * 4);
+  p.own_ml = room(orows * 8);
+  return p;
 }
 
 static int kv16_attention_check(const N730KV16Cache* c, int batch, int tokens, int heads) {
@@ -64,7 +597,62 @@ static int kv16_attention_check(const N730KV16Cache* c, int batch, int tokens, i
   N730_REQUIRE(batch <= KV8_MAX_BATCH && tokens >= 1 && tokens <= (1 << 20), N730_BAD_ARG, "%s: batch %d, tokens %d", what, batch, tokens);
   N730_REQUIRE(heads >= c->n_kv && heads % c->n_kv == 0 && heads <= 65535, N730_BAD_ARG, "%s: %d heads over %d KV heads", what,
                heads, c->n_kv);
+  N730_REQUIRE((int64_t)batch * tokens * heads < (1ll << 30), N730_BAD_ARG, "%s: 2^30 or more query rows", what);
   return N730_OK;
+}
+
+// cuTensorMapEncodeTiled through the runtime's driver entry point (no libcuda link).
+static PFN_cuTensorMapEncodeTiled_v12000 ka_encoder() {
+  static std::once_flag once;
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+    else
+      cudaGetLastError();
+  });
+  return fn;
+}
+// A pool as a 2-D tensor, one row per position and KV head of a page; a copy takes 64 channels of `box` rows,
+// swizzled over 128 bytes (x is 0 or 64, a multiple of 16 bytes).
+static int ka_map(const N730KV16Cache& c, const void* pool, int box, CUtensorMap* out) {
+  auto enc = ka_encoder();
+  N730_REQUIRE(enc, N730_CUDA_ERR, "kv16_attention: cuTensorMapEncodeTiled is not available");
+  const cuuint64_t dims[2] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.n_pages * c.n_kv * c.page_size};
+  const cuuint64_t strides[1] = {(cuuint64_t)c.head_dim * 2};
+  const cuuint32_t boxes[2] = {64, (cuuint32_t)box}, es[2] = {1, 1};
+  N730_REQUIRE(enc(out, c.dtype == N730_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                   const_cast<void*>(pool), dims, strides, boxes, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS,
+               N730_CUDA_ERR, "kv16_attention: cuTensorMapEncodeTiled failed");
+  return N730_OK;
+}
+
+template <int HD, bool BF, int NT>
+static int ka_launch_one(const KAArgs& a, const CUtensorMap& km, const CUtensorMap& vm, int64_t grid, bool pdl, cudaStream_t st) {
+  const size_t smem = sizeof(KASmem<HD, NT>) + 1024;
+  if (int rc = smem_attr_once<kv16_attention_kernel<HD, BF, NT>>((int)smem)) return rc;
+  return kv8_launch(kv16_attention_kernel<HD, BF, NT>, dim3((unsigned)grid), dim3(KACfg<HD, NT>::THREADS), smem, st, pdl, a, km, vm);
+}
+
+template <int HD, bool BF>
+static int ka_launch(KAArgs& a, const KAPlan& p, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
+  auto one = [&](int nt, int64_t pre, int64_t own, bool pdl) {
+    a.prefix_items = (int)pre;
+    return nt == 1 ? ka_launch_one<HD, BF, 1>(a, km, vm, pre + own, pdl, st) : ka_launch_one<HD, BF, 2>(a, km, vm, pre + own, pdl, st);
+  };
+  // items of the same shape in one grid, the prefix's (longer) first; otherwise the own ones' grid follows on its heels
+  if (!p.pre_items || p.pre_nt == p.own_nt) {
+    if (int rc = one(p.own_nt, p.pre_items, p.own_items, false)) return rc;
+  } else {
+    if (int rc = one(p.pre_nt, p.pre_items, 0, false)) return rc;
+    if (int rc = one(p.own_nt, 0, p.own_items, true)) return rc;
+  }
+  const int64_t rows = (int64_t)a.batch * a.tokens * a.heads;
+  return kv8_launch(kv16_join_kernel<HD, BF>, dim3((unsigned)((rows + KJ_WARPS - 1) / KJ_WARPS)), dim3(KJ_WARPS * 32), 0, st, true, a);
 }
 
 }  // namespace n730
@@ -73,7 +661,7 @@ using namespace n730;
 
 N730_API int64_t n730_kv16_attention_ws(const N730KV16Cache* c, int batch, int tokens, int n_heads) {
   if (int rc = kv16_attention_check(c, batch, tokens, n_heads)) return rc;
-  return 256;
+  return ka_plan(*c, batch, tokens, n_heads).bytes;
 }
 
 N730_API int n730_kv16_attention(const N730KV16Cache* c, const void* d_q, int64_t ldq, int batch, int tokens, int n_heads,
@@ -89,10 +677,34 @@ N730_API int n730_kv16_attention(const N730KV16Cache* c, const void* d_q, int64_
                "%s: pointers must lie on whole elements", what);
   N730_REQUIRE(std::isfinite(scale), N730_BAD_ARG, "%s: scale %g", what, scale);
   N730_REQUIRE(((uintptr_t)d_ws & 15) == 0, N730_BAD_ARG, "%s: the workspace must be 16-byte aligned", what);
-  const int64_t need = n730_kv16_attention_ws(c, batch, tokens, n_heads);
-  N730_REQUIRE(ws_bytes >= need, N730_BAD_ARG, "%s: workspace of %lld bytes, %lld needed", what, (long long)ws_bytes, (long long)need);
-  KSArgs a{*c, d_q, d_out, ldq, ldo, batch, tokens, n_heads, scale, d_lens, d_new};
-  kv16_simple_kernel<<<dim3((unsigned)(batch * tokens), n_heads), KS_THREADS, 0, (cudaStream_t)stream>>>(a);
-  N730_CHECK_LAUNCH();
-  return N730_OK;
+  const KAPlan p = ka_plan(*c, batch, tokens, n_heads);
+  N730_REQUIRE(ws_bytes >= p.bytes, N730_BAD_ARG, "%s: workspace of %lld bytes, %lld needed", what, (long long)ws_bytes,
+               (long long)p.bytes);
+  N730_REQUIRE(p.pre_items + p.own_items < (1ll << 31), N730_BAD_ARG, "%s: 2^31 or more pieces of work", what);
+  uint8_t* ws = reinterpret_cast<uint8_t*>(d_ws);
+  KAArgs a{};
+  a.c = *c;
+  a.q = d_q; a.out = d_out; a.ldq = ldq; a.ldo = ldo;
+  a.batch = batch; a.tokens = tokens; a.heads = n_heads; a.group = n_heads / c->n_kv;
+  a.box = 16;
+  while (a.box < KA_KEYS && c->page_size % (2 * a.box) == 0) a.box *= 2;
+  a.qvec = ((uintptr_t)d_q & 15) == 0 && ldq % 8 == 0;
+  a.ovec = ((uintptr_t)d_out & 7) == 0 && ldo % 4 == 0;
+  a.scale_log2e = std::fabs(scale) * 1.4426950408889634f;
+  a.sign = scale < 0 ? 0x80008000u : 0u;
+  a.lens = d_lens; a.n_new = d_new;
+  a.status = reinterpret_cast<int*>(ws);
+  if (p.pre_items)
+    a.pre = KAParts{p.pre_tiles, p.pre_splits, p.pre_tiles * p.pre_nt * 128, reinterpret_cast<float*>(ws + p.pre_o),
+                    reinterpret_cast<float2*>(ws + p.pre_ml)};
+  a.own = KAParts{p.own_tiles, p.own_splits, p.own_tiles * p.own_nt * 128, reinterpret_cast<float*>(ws + p.own_o),
+                  reinterpret_cast<float2*>(ws + p.own_ml)};
+  CUtensorMap km, vm;
+  int rc = ka_map(*c, c->k, a.box, &km);
+  if (!rc) rc = ka_map(*c, c->v, a.box, &vm);
+  if (rc) return rc;
+  const bool bf = c->dtype == N730_BF16;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (c->head_dim == 128) return bf ? ka_launch<128, true>(a, p, km, vm, st) : ka_launch<128, false>(a, p, km, vm, st);
+  return bf ? ka_launch<64, true>(a, p, km, vm, st) : ka_launch<64, false>(a, p, km, vm, st);
 }
