@@ -7,9 +7,9 @@
 // Angles reach 2^31 radians, where fp32 knows nothing of the fraction of a turn: p * freq / 2 pi is formed in 64
 // bits, whole turns are taken off there, and the rest, at most half a turn, goes to sincospif in 32.
 //
-// Bound by bytes: every element is read and written once.  A CTA takes rows x units (a unit: 8 channels, or both
-// runs of 8 that a half layout pairs), two units a thread; each thread asks for its units before the CTA's angles
-// are computed, once a row and pair and not once a head.
+// Bound by bytes: every element is read and written once.  A thread has one unit of a row (8 channels, or both runs of
+// 8 that a half layout pairs) in up to 16 rows, so that what the unit is costs nothing a row; angles are computed once a
+// row and pair, not once a head, in shared memory.
 #include <cmath>
 
 #include "kv16.h"
@@ -38,8 +38,21 @@ int kv16_check(const N730KV16Cache* c, int batch, const char* what) {
   return N730_OK;
 }
 
-constexpr int RO_THREADS = 256, RO_EACH = 2, RO_UNITS = RO_THREADS * RO_EACH;
-constexpr int RO_V = 8;  // channels of a vector unit
+constexpr int RO_THREADS = 320;  // most threads of a CTA
+constexpr int RO_ROWS = 16;      // most rows of a CTA
+constexpr int RO_V = 8;          // channels of a vector unit
+constexpr int64_t RO_TABLE = 40 * 1024;  // bytes of a CTA's cosines and sines
+
+// n / d for n < 2^31 by a product: integer divisions by what a launch gives took a third of the kernel's time
+struct FastDiv {
+  uint32_t d, m, s;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t x) : d(x), s(0) {
+    while ((1ull << s) < x) ++s;
+    m = (uint32_t)((((1ull << s) - x) << 32) / x + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }
+};
 
 // One group of heads of a row: where it is read, and where it goes.
 struct RotaryPart {
@@ -56,29 +69,45 @@ struct RotaryArgs {
   int head_dim, rd;        // rd: rotated channels (0: none)
   int interleaved, dtype;
   int units_head, units_copy;  // units of a rotated head, of one that is copied
-  int units, rows_cta, chunk;  // units of a row; rows and units of a row that a CTA takes
-  int64_t rows;
-  int has_cache, tokens;
+  int units, chunk;        // units of a row; those that a CTA takes
+  int at_once, rows_cta;   // rows that a CTA works on side by side, and in all
+  int rows, tokens, has_cache;
+  FastDiv by_chunk, by_last, by_head, by_copy, by_tokens, by_page, by_pairs;  // by_last: units of the last chunk
   N730KV16Cache c;
   const int* lens; const int* n_new;
 };
 
-// n (8 or 1) consecutive elements as fp32
-template <int N>
-__device__ __forceinline__ void ro_load(const void* p, int64_t i, int dtype, float* x) {
-  if (N == 1) {
-    x[0] = kv8_load1(p, i, dtype);
-  } else if (dtype == N730_F32) {
-    const float4* s = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
-    const float4 a = s[0], b = s[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+// A run of N consecutive elements as it lies in memory.
+template <int N, int ES> struct RoRun { uint4 w[N * ES / 16]; };
+template <> struct RoRun<1, 2> { uint16_t w; };
+template <> struct RoRun<1, 4> { uint32_t w; };
+template <int N, int ES>
+__device__ __forceinline__ RoRun<N, ES> ro_load(const void* p, int64_t i) {
+  return *reinterpret_cast<const RoRun<N, ES>*>(reinterpret_cast<const uint8_t*>(p) + i * ES);
+}
+__device__ __forceinline__ float2 ro_wide(uint32_t w, bool f16) {
+  return f16 ? __half22float2(*reinterpret_cast<const __half2*>(&w)) : make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ uint32_t ro_pack(float a, float b, bool f16) {
+  if (f16) return h2_bits(__floats2half2_rn(a, b));
+  const __nv_bfloat162 y = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+template <int N, int ES>
+__device__ __forceinline__ void ro_widen(const RoRun<N, ES>& r, bool f16, float* x) {
+  if constexpr (N == 1) {
+    x[0] = ES == 4 ? __uint_as_float(r.w) : ro_wide(r.w, f16).x;
+  } else if constexpr (ES == 4) {
+#pragma unroll
+    for (int e = 0; e < N / 4; ++e) {
+      x[4 * e] = __uint_as_float(r.w[e].x); x[4 * e + 1] = __uint_as_float(r.w[e].y);
+      x[4 * e + 2] = __uint_as_float(r.w[e].z); x[4 * e + 3] = __uint_as_float(r.w[e].w);
+    }
   } else {
-    const uint4 a = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float2 f = dtype == N730_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[e]))
-                                         : make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
+      const float2 f = ro_wide(w[e], f16);
       x[2 * e] = f.x; x[2 * e + 1] = f.y;
     }
   }
@@ -94,123 +123,133 @@ __device__ __forceinline__ void ro_store(void* p, int64_t i, int dtype, const fl
   } else {
     uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (dtype == N730_F16) w[e] = h2_bits(__floats2half2_rn(x[2 * e], x[2 * e + 1]));
-      else {
-        const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
-        w[e] = *reinterpret_cast<const uint32_t*>(&b);
-      }
-    }
+    for (int e = 0; e < 4; ++e) w[e] = ro_pack(x[2 * e], x[2 * e + 1], dtype == N730_F16);
     *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
 // A unit: N consecutive channels (a half layout's rotated ones: two runs of N, rd / 2 apart; N = 1 interleaved: the
-// pair), N = 8 where every run starts on a 16-byte boundary, 1 otherwise.
-template <int N>
-__global__ void __launch_bounds__(RO_THREADS) rotary_kernel(const RotaryArgs a) {
-  extern __shared__ float2 ro_cs[];  // [row of the CTA][pair]
-  __shared__ int64_t row_pos[RO_UNITS];
+// pair), N = 8 where every run starts on a 16-byte boundary, 1 otherwise.  A thread has one unit of a row, the same in
+// each of its rows: what it is and where it lies is found out once.
+template <int N, int ES>
+__global__ void __launch_bounds__(RO_THREADS, 3) rotary_kernel(const RotaryArgs a) {
+  extern __shared__ __align__(16) float2 ro_cs[];  // [row of the CTA][pair]
+  __shared__ int row_pos[RO_ROWS * 32], row_slot[RO_ROWS * 32];  // position; row of the pool, -1: dropped, -2: no row at all
+  constexpr int BATCH = N == 1 || ES == 4 ? 1 : 2;            // rows asked for at a time
   const int tid = threadIdx.x, np = a.rd / 2;
-  const int64_t r0 = (int64_t)blockIdx.x * a.rows_cta;
+  const int r0 = (int)blockIdx.x * a.rows_cta, nr = min(a.rows_cta, a.rows - r0);
   const int u0 = blockIdx.y * a.chunk, uc = min(a.chunk, a.units - u0);
-  const int nr = (int)min((int64_t)a.rows_cta, a.rows - r0);
   const int prefix = a.has_cache ? kv16_prefix(a.c) : 0, cap = a.has_cache ? a.c.max_pages * a.c.page_size : 0;
 
-  float x[RO_EACH][2 * N];
-  void* to[RO_EACH];
-  int64_t at[RO_EACH];      // element that the unit's first run goes to
-  int pair[RO_EACH], type[RO_EACH], gap[RO_EACH];  // pair < 0: copied; gap: elements to the second run, 0: none
-#pragma unroll
-  for (int k = 0; k < RO_EACH; ++k) {
-    const int i = tid + k * RO_THREADS, r = i / uc;
-    to[k] = nullptr;
-    if (r >= nr) continue;
-    int u = u0 + i % uc;
-    const int64_t row = r0 + r;
-    int which = 0, per = a.units_head;
-    if (u >= a.part[0].heads * per) {
-      u -= a.part[0].heads * per;
-      which = 1;
-      if (u >= a.part[1].heads * per) { u -= a.part[1].heads * per; which = 2; per = a.units_copy; }
-    }
-    const int head = u / per, w = u % per;
-    // the unit's first channel: rotated units first, then the channels that stay
-    int ch, rot = -1, g = 0;
-    if (which == 2 || a.rd == 0) {
-      ch = w * N;
-    } else if (a.interleaved) {
-      const int nu = N == 1 ? np : a.rd / N;
-      if (w < nu) { ch = N == 1 ? 2 * w : w * N; rot = ch / 2; g = N == 1 ? 1 : 0; }
-      else ch = a.rd + (w - nu) * N;
-    } else {
-      const int nu = np / N;
-      if (w < nu) { ch = rot = w * N; g = np; }
-      else ch = a.rd + (w - nu) * N;
-    }
-    const RotaryPart& p = a.part[which];
-    int64_t dst = row * p.ldy + (int64_t)head * a.head_dim + ch;
-    void* y = p.y;
-    int type_y = a.dtype;
+  // this thread's unit
+  const int first = (int)(uc == a.chunk ? a.by_chunk : a.by_last).div(tid);  // its first row of the CTA
+  int u = u0 + tid - first * uc, which = 0, per = a.units_head;
+  if (u >= a.part[0].heads * per) {
+    u -= a.part[0].heads * per;
+    which = 1;
+    if (u >= a.part[1].heads * per) { u -= a.part[1].heads * per; which = 2; per = a.units_copy; }
+  }
+  const int head = (int)(which == 2 ? a.by_copy : a.by_head).div(u), w = u - head * per;
+  int ch, rot = -1, gap = 0;  // its first channel, its first pair (-1: it stays), elements to its second run
+  if (which == 2 || a.rd == 0) {
+    ch = w * N;
+  } else if (a.interleaved) {
+    const int nu = N == 1 ? np : a.rd / N;
+    if (w < nu) { ch = N == 1 ? 2 * w : w * N; rot = ch / 2; gap = N == 1 ? 1 : 0; }
+    else ch = a.rd + (w - nu) * N;
+  } else {
+    const int nu = np / N;
+    if (w < nu) { ch = rot = w * N; gap = np; }
+    else ch = a.rd + (w - nu) * N;
+  }
+  const RotaryPart& p = a.part[which];
+  const int col = head * a.head_dim + ch;
+  const bool to_pool = p.y == nullptr, f16 = a.dtype == N730_F16, mine = first < a.at_once;
+
+  RoRun<N, ES> x[BATCH], x2[BATCH];
+  auto load = [&](int k, int r) {
+    const int64_t at = (int64_t)(r0 + r) * p.ldx + col;
+    x[k] = ro_load<N, ES>(p.x, at);
+    if (gap) x2[k] = ro_load<N, ES>(p.x, at + gap);
+  };
+  // rows that are surely there are asked for before what follows is known
+  const bool early = mine && first < nr && (!a.has_cache || a.tokens == 1);
+  if (early) load(0, first);
+
+  for (int r = tid; r < nr; r += blockDim.x) {
+    const int row = r0 + r;
+    int pos = 0, slot = 0;
     if (a.has_cache) {
-      const int b = (int)(row / a.tokens), t = (int)(row % a.tokens);
-      const int slot = kv8_len(a.lens, b, cap) + t;
-      if (t >= kv8_new(a.n_new, b, a.tokens)) continue;
-      if (!y) {
-        if (slot >= cap) continue;
-        const int page = a.c.block_table[(int64_t)b * a.c.max_pages + slot / a.c.page_size];
-        if ((unsigned)page >= (unsigned)a.c.n_pages) continue;
-        y = p.pool ? a.c.v : a.c.k;
-        type_y = a.c.dtype;
-        dst = (((int64_t)page * a.c.n_kv + head) * a.c.page_size + slot % a.c.page_size) * a.head_dim + ch;
+      const int b = (int)a.by_tokens.div(row), t = row - b * a.tokens, len = kv8_len(a.lens, b, cap);
+      pos = prefix + len + t;
+      slot = -1;
+      if (t >= kv8_new(a.n_new, b, a.tokens)) {
+        slot = -2;
+      } else if (len + t < cap) {
+        const int pi = (int)a.by_page.div(len + t), page = a.c.block_table[(int64_t)b * a.c.max_pages + pi];
+        if ((unsigned)page < (unsigned)a.c.n_pages) slot = page * a.c.n_kv * a.c.page_size + len + t - pi * a.c.page_size;
       }
     }
-    const int64_t src = row * p.ldx + (int64_t)head * a.head_dim + ch;
-    ro_load<N>(p.x, src, a.dtype, x[k]);
-    if (g) ro_load<N>(p.x, src + g, a.dtype, x[k] + N);
-    to[k] = y; at[k] = dst; pair[k] = rot < 0 ? -1 : r * np + rot; type[k] = type_y; gap[k] = g;
+    if (a.pos) pos = a.pos[row];
+    row_pos[r] = pos;
+    row_slot[r] = slot;
   }
-
+  __syncthreads();
   if (np) {
-    for (int r = tid; r < nr; r += RO_THREADS) {
-      const int64_t row = r0 + r;
-      row_pos[r] = a.pos ? a.pos[row] : (int64_t)prefix + kv8_len(a.lens, (int)(row / a.tokens), cap) + row % a.tokens;
-    }
-    __syncthreads();
-    for (int i = tid; i < nr * np; i += RO_THREADS) {
-      double turns = (double)row_pos[i / np] * a.freq[i % np] * 0.15915494309189533577;  // 1 / 2 pi
+    for (int i = tid; i < nr * np; i += blockDim.x) {
+      const int r = (int)a.by_pairs.div(i);
+      double turns = (double)row_pos[r] * a.freq[i - r * np] * 0.15915494309189533577;  // 1 / 2 pi
       turns -= rint(turns);
-      float s, c;
-      sincospif(2.f * (float)turns, &s, &c);
-      ro_cs[i] = make_float2(c * a.factor, s * a.factor);
+      float sn, cs;
+      sincospif(2.f * (float)turns, &sn, &cs);
+      ro_cs[i] = make_float2(cs * a.factor, sn * a.factor);
     }
     __syncthreads();
   }
+  if (!mine) return;
 
+  for (int rb = first; rb < nr; rb += BATCH * a.at_once) {
 #pragma unroll
-  for (int k = 0; k < RO_EACH; ++k) {
-    if (!to[k]) continue;
-    if (pair[k] >= 0) {
-      if (gap[k]) {
+    for (int k = 0; k < BATCH; ++k) {
+      const int r = rb + k * a.at_once;
+      if (r < nr && row_slot[r] != -2 && !(early && r == first)) load(k, r);
+    }
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float2 cs = ro_cs[pair[k] + e];
-          const float x0 = x[k][e], x1 = x[k][N + e];
-          x[k][e] = x0 * cs.x - x1 * cs.y;
-          x[k][N + e] = x1 * cs.x + x0 * cs.y;
-        }
-      } else {
+    for (int k = 0; k < BATCH; ++k) {
+      const int r = rb + k * a.at_once;
+      if (r >= nr) break;
+      const int slot = row_slot[r];
+      if (slot == -2 || (to_pool && slot < 0)) continue;
+      float y[2 * N];
+      ro_widen<N, ES>(x[k], f16, y);
+      if (gap) ro_widen<N, ES>(x2[k], f16, y + N);
+      if (rot >= 0) {
+        const float2* cs = ro_cs + r * np + rot;  // on 16 bytes where units are vectors
+        float4 c4;
+        if (gap) {
 #pragma unroll
-        for (int e = 0; e < N / 2; ++e) {
-          const float2 cs = ro_cs[pair[k] + e];
-          const float x0 = x[k][2 * e], x1 = x[k][2 * e + 1];
-          x[k][2 * e] = x0 * cs.x - x1 * cs.y;
-          x[k][2 * e + 1] = x1 * cs.x + x0 * cs.y;
+          for (int e = 0; e < N; ++e) {
+            const float2 t = N == 1 ? cs[0] : e % 2 ? make_float2(c4.z, c4.w) : (c4 = reinterpret_cast<const float4*>(cs)[e / 2], make_float2(c4.x, c4.y));
+            const float y0 = y[e], y1 = y[N + e];
+            y[e] = y0 * t.x - y1 * t.y;
+            y[N + e] = y1 * t.x + y0 * t.y;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < N / 2; ++e) {
+            const float2 t = e % 2 ? make_float2(c4.z, c4.w) : (c4 = reinterpret_cast<const float4*>(cs)[e / 2], make_float2(c4.x, c4.y));
+            const float y0 = y[2 * e], y1 = y[2 * e + 1];
+            y[2 * e] = y0 * t.x - y1 * t.y;
+            y[2 * e + 1] = y1 * t.x + y0 * t.y;
+          }
         }
       }
+      void* dst = to_pool ? (p.pool ? a.c.v : a.c.k) : p.y;
+      const int type = to_pool ? a.c.dtype : a.dtype;
+      const int64_t at = to_pool ? (int64_t)(slot + head * a.c.page_size) * a.head_dim + ch : (int64_t)(r0 + r) * p.ldy + col;
+      ro_store<N>(dst, at, type, y);
+      if (gap) ro_store<N>(dst, at + gap, type, y + N);
     }
-    ro_store<N>(to[k], at[k], type[k], x[k]);
-    if (gap[k]) ro_store<N>(to[k], at[k] + gap[k], type[k], x[k] + N);
   }
 }
 
@@ -239,17 +278,34 @@ static int rotary_launch(RotaryArgs& a, const N730Rotary* r, const char* what, c
   a.units_copy = a.head_dim / n;
   a.units_head = a.rd == 0 ? a.units_copy : a.interleaved && vec ? a.units_copy : a.rd / 2 / n + (a.head_dim - a.rd) / n;
   const int64_t units = (int64_t)(a.part[0].heads + a.part[1].heads) * a.units_head + (int64_t)a.part[2].heads * a.units_copy;
-  N730_REQUIRE(units <= (int64_t)RO_UNITS * 65535, N730_BAD_ARG, "%s: rows of %lld channels", what,
+  N730_REQUIRE(units <= (int64_t)RO_THREADS * 65535, N730_BAD_ARG, "%s: rows of %lld channels", what,
                (long long)(a.part[0].heads + a.part[1].heads + a.part[2].heads) * a.head_dim);
   a.units = (int)units;
-  a.chunk = std::min(a.units, RO_UNITS);
-  a.rows_cta = RO_UNITS / a.chunk;
-  const int64_t grid = (a.rows + a.rows_cta - 1) / a.rows_cta;
-  N730_REQUIRE(grid < (1ll << 31), N730_BAD_ARG, "%s: %lld rows", what, (long long)a.rows);
-  const dim3 g((unsigned)grid, (a.units + a.chunk - 1) / a.chunk);
+  const int most = (a.units + RO_THREADS - 1) / RO_THREADS;
+  a.chunk = (a.units + most - 1) / most;  // even shares
+  const int chunks = (a.units + a.chunk - 1) / a.chunk;
+  // short rows go side by side; a CTA takes several rows where there are more than the SMs hold CTAs (three each)
+  a.at_once = std::min(std::max(RO_THREADS / a.chunk, 1), 32);
+  const int64_t turns = ((int64_t)a.rows + a.at_once - 1) / a.at_once * chunks;
+  a.rows_cta = a.at_once * (int)std::min<int64_t>(std::max<int64_t>(turns / (3 * num_sms()), 1), RO_ROWS);
+  const int threads = (a.chunk * a.at_once + 31) / 32 * 32;
+  a.by_chunk = FastDiv(a.chunk);
+  a.by_last = FastDiv(a.units - (chunks - 1) * a.chunk);
+  a.by_head = FastDiv(a.units_head);
+  a.by_copy = FastDiv(a.units_copy);
+  a.by_tokens = FastDiv(a.tokens);
+  a.by_page = FastDiv(a.has_cache ? a.c.page_size : 1);
+  a.by_pairs = FastDiv(std::max(a.rd / 2, 1));
+  while ((int64_t)a.rows_cta * (a.rd / 2) * sizeof(float2) > RO_TABLE) a.rows_cta -= a.at_once;
+  const dim3 g((a.rows + a.rows_cta - 1) / a.rows_cta, chunks);
   const size_t smem = (size_t)a.rows_cta * (a.rd / 2) * sizeof(float2);
-  if (vec) rotary_kernel<RO_V><<<g, RO_THREADS, smem, st>>>(a);
-  else rotary_kernel<1><<<g, RO_THREADS, smem, st>>>(a);
+  if (vec) {
+    if (es == 4) rotary_kernel<RO_V, 4><<<g, threads, smem, st>>>(a);
+    else rotary_kernel<RO_V, 2><<<g, threads, smem, st>>>(a);
+  } else {
+    if (es == 4) rotary_kernel<1, 4><<<g, threads, smem, st>>>(a);
+    else rotary_kernel<1, 2><<<g, threads, smem, st>>>(a);
+  }
   N730_CHECK_LAUNCH();
   return N730_OK;
 }
@@ -312,7 +368,7 @@ N730_API int n730_rotary(const N730Rotary* r, const void* d_x, int64_t ldx, void
                "%s: pointers must lie on whole elements", what);
   RotaryArgs a{};
   a.part[0] = RotaryPart{d_x, d_y, ldx, ldy, n_heads, 0};
-  a.head_dim = head_dim; a.dtype = dtype; a.rows = rows; a.tokens = 1;
+  a.head_dim = head_dim; a.dtype = dtype; a.rows = (int)rows; a.tokens = 1;
   a.pos = d_pos;
   return rotary_launch(a, r, what, (cudaStream_t)stream);
 }
@@ -344,7 +400,8 @@ N730_API int n730_kv16_append(const N730KV16Cache* c, const N730Rotary* r, const
   }
   a.part[1] = RotaryPart{d_k, nullptr, ld, 0, c->n_kv, 0};
   a.part[2] = RotaryPart{d_v, nullptr, ld, 0, c->n_kv, 1};
-  a.head_dim = c->head_dim; a.dtype = dtype; a.rows = (int64_t)batch * tokens; a.tokens = tokens;
+  N730_REQUIRE((int64_t)batch * tokens < (1ll << 31), N730_BAD_ARG, "%s: %d x %d rows", what, batch, tokens);
+  a.head_dim = c->head_dim; a.dtype = dtype; a.rows = batch * tokens; a.tokens = tokens;
   a.pos = d_pos;
   a.has_cache = 1;
   a.c = *c;
