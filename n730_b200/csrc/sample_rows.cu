@@ -6,17 +6,18 @@
 //   whose mass reaches p times the mass of those k; the tokens with w >= q.  The token is the first whose cumulative
 //   mass exceeds u times the kept mass.
 //
-// A cluster of 8 CTAs takes a row: each keeps an eighth of the logits in shared memory, so that HBM is read once and
-// whatever follows runs on the chip.
+// A cluster of 8 CTAs takes a row: each copies an eighth of the logits into its shared memory, so that HBM is read once
+// and whatever follows runs on the chip.
 //   1. largest and smallest logit;
 //   2. a histogram over RS_BINS linear bins of max - l: how many tokens, and, where the mass of all tokens matters (no
 //      top-k, or a large one), the sum of w / w(bin's edge) - 1 in fixed point.  Bins are narrow, so that this is small
 //      and fp32 holds it to 2^-24 of w or so; a bin's mass is w(edge) * (count + sum), formed in 64 bits.  Both sums are
-//      integers: the order of the atomics does not matter;
-//   3. the first CTA scans the bins.  Where the bins up to the last one that a kept token can lie in hold at most
-//      RS_CAP tokens, these are gathered in its shared memory and sorted, and the rest is a scan over them with weights
-//      in 64 bits.  Where not (flat rows without a top-k), each prefix's end is looked up in its bin by itself: the
-//      bin's tokens are gathered and sorted, or, where they are too many (equal logits, coarse types), found by four
+//      integers: the order of the atomics does not matter.  Each CTA adds up an eighth of the bins over the cluster and
+//      puts them where the first CTA scans them;
+//   3. where the bins up to the last one that a kept token can lie in hold at most RS_CAP tokens, these are gathered in
+//      the first CTA's shared memory and sorted, and the rest is a scan over them with weights in 64 bits; the other
+//      CTAs are gone by then.  Where not (flat rows without a top-k), each prefix's end is looked up in its bin by itself:
+//      the bin's tokens are gathered and sorted, or, where they are too many (equal logits, coarse types), found by four
 //      rounds of 8 bits of the logit, after which the tokens left are equal and go by index.
 // All sums are 64-bit floats in a fixed order or integers: the same inputs give the same token.
 #include <cooperative_groups.h>
@@ -31,10 +32,12 @@ namespace cg = cooperative_groups;
 constexpr int RS_CLUSTER = 8;
 constexpr int RS_THREADS = 512;
 constexpr int RS_WARPS = RS_THREADS / 32;
-constexpr int RS_BINS = 2048;      // and one more for what lies behind the last
+constexpr int RS_BINS = 1536;      // as many as leave room for two CTAs of 19008 fp32 logits (a row of 152064) an SM
+constexpr int RS_SHARE = RS_BINS / RS_CLUSTER;
 constexpr int RS_PER = RS_BINS / RS_THREADS;
-constexpr int RS_CAP = 2048;       // tokens that are sorted at once
+constexpr int RS_CAP = 1024;       // tokens that are sorted at once
 constexpr int RS_EACH = RS_CAP / RS_THREADS;
+constexpr int RS_COUNT = 160;      // lists up to this long are sorted by counting
 constexpr int RS_SURE = 2048;      // tokens of a CTA's bin that the fixed point of the bins' masses has room for at first
 constexpr float RS_SPAN = 32.f;    // bins reach this many logits, or temperatures where that is more, below the largest
 constexpr size_t RS_STAGE_MAX = 160 * 1024;  // longest slice that is kept in shared memory
@@ -42,7 +45,7 @@ constexpr size_t RS_STAGE_MAX = 160 * 1024;  // longest slice that is kept in sh
 struct RSArgs {
   const void* logits;
   int64_t ld;
-  int vocab, dtype, per;           // per: logits of a CTA
+  int vocab, per;                  // per: logits of a CTA
   bool vec;                        // rows lie on 16 bytes
   const float* temperature; const int* top_k; const float* top_p; const float* min_p; const float* u;
   int* tokens; float* prob; int* kept;
@@ -51,27 +54,34 @@ struct RSArgs {
 enum { RS_DONE = 0, RS_MASSES, RS_GATHER, RS_RADIX, RS_OVER, RS_FIND };
 struct RSCommand {
   int op, b0, b1;         // bins [b0, b1]
+  int last;               // GATHER: nothing follows for the other CTAs
   uint32_t prefix, shift; // RADIX: digits found, where the next one starts
   uint32_t key, skip;     // FIND: the skip-th token of this key
   int sure;               // MASSES: tokens of a CTA's bin to have room for
   double z0;              // RADIX: the bin's edge / T
 };
-struct RSStat { float mx, mn; int idx, pad; };
+struct RSStat { float mx, mn; };
 
 struct RSSmem {
-  uint32_t cnt[RS_BINS + 4];       // by bin; also the counts of 256 digits
-  int32_t dev[RS_BINS + 4];        // sums of w / w(edge) - 1; also the digits' masses, low and high words
-  unsigned long long list[RS_CAP]; // (order of the logit, largest first) << 32 | index
+  uint32_t cnt[RS_BINS];             // by bin; also the counts of 256 digits
+  int32_t dev[RS_BINS];              // sums of w / w(edge) - 1; also the digits' masses, low and high words
+  union { unsigned long long list[RS_CAP]; uint32_t bin_cnt[RS_BINS]; uint2 share[2 * RS_SHARE]; };  // list: ~order << 32 | index
+  union { double cum[RS_CAP]; double bin_mass[RS_BINS]; };
   RSCommand cmd;
-  RSStat stat;
+  RSStat stats[RS_CLUSTER];
   RSStat wstat[RS_WARPS];
   double wsum[RS_WARPS];
   uint32_t wcnt[RS_WARPS];
-  double all_mass, pick_mass, pick_w, sel_base;
-  uint32_t all_cnt, most_cnt, n_list, over, sel_cnt, sel_bin_cnt, pick_cnt;
-  int sel_bin, pick, found;
-  uint32_t occur;
+  uint32_t beyond[RS_CLUSTER], most[RS_CLUSTER];  // tokens behind the last bin; of the fullest bin of a share
+  uint32_t own_beyond, own_most;
+  double sel_base, sel_mass, pick_w;
+  uint32_t n_list, over, sel_cnt, sel_in, pick_cnt, occur;
+  int bin_k, bin_p, bin_last, pick, found, first;
 };
+
+__device__ __forceinline__ void rs_arrive() { __syncwarp(); asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void rs_wait() { __syncwarp(); asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void rs_sync() { rs_arrive(); rs_wait(); }
 
 // the order of logits as unsigned numbers (largest largest); logits here are no NaN and no -0
 __device__ __forceinline__ uint32_t rs_order(float x) {
@@ -80,6 +90,9 @@ __device__ __forceinline__ uint32_t rs_order(float x) {
 }
 __device__ __forceinline__ float rs_unorder(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 __device__ __forceinline__ float rs_clean(float x) { return x != x ? -INFINITY : x + 0.f; }
+__device__ __forceinline__ float rs_float(float x) { return x; }
+__device__ __forceinline__ float rs_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float rs_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
 // A row's bins: bin = floor((max - l) * sx), edge(b) = b * width below the largest.
 struct RSGeom {
@@ -119,33 +132,40 @@ __device__ V rs_scan(V v, V* warps, V* total) {
   return before + inc - v;
 }
 
-template <bool STAGED>
+template <class T, bool STAGED>
 struct RSRow {
   RSSmem& s;
-  float* stage;          // this CTA's logits
+  T* stage;              // this CTA's logits
   const RSArgs& a;
-  int64_t base;          // the row's first logit
+  const T* row;          // the row's first logit
   int i0, n;             // this CTA's share
   RSGeom g;
   cg::cluster_group cl;
-  double zmin;           // log of min-p
+  double min_p;
   int sure;              // tokens of a CTA's bin that the masses have room for
+  bool alone;            // the other CTAs are gone
 
-  __device__ float get(int i) const {
-    return STAGED ? stage[i] : rs_clean(kv8_load1(a.logits, base + i0 + i, a.dtype));
+  __device__ float raw(int i) const { return rs_float(STAGED ? stage[i] : row[i0 + i]); }
+  __device__ float get(int i) const { return rs_clean(raw(i)); }
+
+  // Fixed-point unit of the deviations: a CTA's sum of a bin with up to `sure` tokens stays inside 31 bits.
+  __device__ float dev_unit() const {
+    const float most = fmaxf(1.f - expf(-g.width * g.inv_t * 1.01f), 0x1p-20f) * (float)sure;
+    return ldexpf(1.f, (int)floorf(29.f - log2f(most)));
   }
-
   // Sums of w / w(edge) - 1 by bin; with `count`, the bins' tokens as well.
   __device__ void fill(bool count, bool masses) {
     const float unit = dev_unit();
     const bool narrow = g.width * g.inv_t < 0x1p-6f;
+    uint32_t beyond = 0;
 #pragma unroll 4
     for (int i = threadIdx.x; i < n; i += RS_THREADS) {
       const float l = get(i);
       if (l == -INFINITY) continue;
       const int b = rs_bin(l, g);
+      if (b == RS_BINS) { ++beyond; continue; }
       if (count) atomicAdd(&s.cnt[b], 1u);
-      if (masses && b < RS_BINS) {
+      if (masses) {
         // y = (l - max + edge) / T, with the rounding of max - l put back
         const float d = rs_below(l, g), bb = d - g.mx, err = l == g.mx ? 0.f : (g.mx - (d - bb)) - (l + bb);
         const float y = -(fmaf(-(float)b, g.width, d) + err) * g.inv_t;
@@ -153,6 +173,50 @@ struct RSRow {
         atomicAdd(&s.dev[b], __float2int_rn(c * unit));
       }
     }
+    if (count && beyond) atomicAdd(&s.own_beyond, beyond);
+  }
+  // This CTA's share of the bins, added up over the cluster, to the first CTA.  The cluster has filled before.
+  __device__ void reduce(bool masses) {
+    const int t = threadIdx.x, rank = (int)cl.block_rank();
+    uint32_t k = 0, most = 0;
+    int d[RS_CLUSTER / 2] = {};
+    if (t < 2 * RS_SHARE) {
+      const int b = rank * RS_SHARE + t % RS_SHARE, r0 = t / RS_SHARE * (RS_CLUSTER / 2);
+#pragma unroll
+      for (int r = 0; r < RS_CLUSTER / 2; ++r) {
+        const RSSmem* o = cl.map_shared_rank(&s, r0 + r);
+        const uint32_t x = o->cnt[b];
+        k += x;
+        most = max(most, x);
+        if (masses) d[r] = o->dev[b];
+      }
+    }
+    int64_t dd = (int64_t)d[0] + d[1] + d[2] + d[3];
+    // halves meet: deviations in two words
+    if (t >= RS_SHARE && t < 2 * RS_SHARE) {
+      s.share[t] = make_uint2((uint32_t)dd, (uint32_t)(dd >> 32));
+      s.share[t - RS_SHARE].x = k;
+    }
+    if (t == 0) s.own_most = 0;
+    __syncthreads();
+    RSSmem* lead = cl.map_shared_rank(&s, 0);
+    if (most > RS_SURE) atomicMax(&s.own_most, most);
+    uint32_t kk = 0;
+    double mass = 0;
+    if (t < RS_SHARE) {
+      kk = k + s.share[t].x;
+      if (masses && kk) {
+        dd += (int64_t)((unsigned long long)s.share[t + RS_SHARE].y << 32 | s.share[t + RS_SHARE].x);
+        mass = exp(-(double)(rank * RS_SHARE + t) * (double)g.width / g.t) * ((double)kk + (double)dd / dev_unit());
+      }
+    }
+    __syncthreads();
+    rs_sync();  // the first CTA has read its own `share`, which lies where the bins' counts go
+    if (t < RS_SHARE) {
+      lead->bin_cnt[rank * RS_SHARE + t] = kk;
+      lead->bin_mass[rank * RS_SHARE + t] = mass;
+    }
+    if (t == 0) { lead->beyond[rank] = s.own_beyond; lead->most[rank] = s.own_most; }
   }
 
   // A CTA's share of a command.
@@ -163,13 +227,15 @@ struct RSRow {
       for (int i = tid; i < RS_BINS; i += RS_THREADS) s.dev[i] = 0;
       __syncthreads();
       fill(false, true);
+      rs_sync();
+      reduce(true);
     } else if (c.op == RS_GATHER) {
       RSSmem* lead = cl.map_shared_rank(&s, 0);
+#pragma unroll 4
       for (int i = tid; i < n; i += RS_THREADS) {
         const float l = get(i);
-        if (l == -INFINITY) continue;
         const int b = rs_bin(l, g);
-        if (b < c.b0 || b > c.b1) continue;
+        if (l == -INFINITY || b < c.b0 || b > c.b1) continue;
         const uint32_t at = atomicAdd(&lead->n_list, 1u);
         if (at < RS_CAP) lead->list[at] = (unsigned long long)~rs_order(l) << 32 | (uint32_t)(i0 + i);
       }
@@ -193,12 +259,11 @@ struct RSRow {
       }
     } else if (c.op == RS_OVER) {  // tokens of weight >= min-p; bins below b0 are sure to have it
       uint32_t k = 0;
-      const double q = exp(zmin);
       for (int i = tid; i < n; i += RS_THREADS) {
         const float l = get(i);
         if (l == -INFINITY) continue;
         const int b = rs_bin(l, g);
-        k += b < c.b0 || (b <= c.b1 && rs_weight(l, g) >= q);
+        k += b < c.b0 || (b <= c.b1 && rs_weight(l, g) >= min_p);
       }
       uint32_t all;
       rs_scan<uint32_t>(k, s.wcnt, &all);
@@ -210,7 +275,7 @@ struct RSRow {
       for (int i = j0; i < j1; ++i) k += get(i) != -INFINITY && rs_order(get(i)) == c.key;
       const uint32_t before = rs_scan<uint32_t>(k, s.wcnt, &all);
       if (tid == 0) s.occur = all;
-      cl.sync();
+      rs_sync();
       uint32_t first = before;
       for (int r = 0; r < (int)cl.block_rank(); ++r) first += cl.map_shared_rank(&s, r)->occur;
       if (c.skip >= first && c.skip < first + k) {
@@ -222,180 +287,208 @@ struct RSRow {
   }
 
   // ---- the first CTA's side ----
-  uint32_t bin_cnt[RS_PER], cnt_before;   // this thread's bins: tokens, tokens of all bins before
-  double bin_mass[RS_PER], mass_before;
+  uint32_t bin_cnt[RS_PER], cnt_before, all_cnt;   // this thread's bins: tokens, tokens of all bins before; of the row
+  double bin_mass[RS_PER], mass_before, all_mass;
 
+  __device__ void post(const RSCommand& c) {  // to every CTA
+    if (threadIdx.x < RS_CLUSTER) cl.map_shared_rank(&s, threadIdx.x)->cmd = c;
+  }
   __device__ void command(const RSCommand& c) {
     __syncthreads();
-    if (threadIdx.x == 0) { s.cmd = c; s.n_list = 0; s.over = 0; }
-    cl.sync();
+    post(c);
+    if (threadIdx.x == 0) { s.n_list = 0; s.over = 0; }
+    rs_sync();
     serve(c);
-    cl.sync();
+    rs_sync();
+    if (c.last) alone = true;
   }
 
-  // the histogram of all CTAs, scanned
-  __device__ void collect(bool masses) {
-    const int b = threadIdx.x * RS_PER;
-    uint32_t k[RS_PER] = {}, beyond = 0, most = 0;
-    if (threadIdx.x == 0) s.most_cnt = 0;
-    __syncthreads();
-    int64_t d[RS_PER] = {};
-    for (int r = 0; r < RS_CLUSTER; ++r) {
-      const RSSmem* o = cl.map_shared_rank(&s, r);
-      const uint4 x = *reinterpret_cast<const uint4*>(&o->cnt[b]);
-      k[0] += x.x; k[1] += x.y; k[2] += x.z; k[3] += x.w;
-      most = max(most, max(max(x.x, x.y), max(x.z, x.w)));
-      if (masses) {
-        const int4 y = *reinterpret_cast<const int4*>(&o->dev[b]);
-        d[0] += y.x; d[1] += y.y; d[2] += y.z; d[3] += y.w;
-      }
-      if (threadIdx.x == 0) beyond += o->cnt[RS_BINS];
-    }
-    if (most > RS_SURE) atomicMax(&s.most_cnt, most);
-    uint32_t kc = 0;
+  // the bins that the cluster has put here, scanned
+  __device__ void scan_bins() {
+    uint32_t kc = 0, all;
     double mc = 0;
 #pragma unroll
     for (int e = 0; e < RS_PER; ++e) {
-      bin_cnt[e] = k[e];
-      bin_mass[e] = k[e] && masses ? exp(-(double)(b + e) * (double)g.width / g.t) * ((double)k[e] + (double)d[e] / dev_unit()) : 0.0;
+      bin_cnt[e] = s.bin_cnt[threadIdx.x * RS_PER + e];
+      bin_mass[e] = s.bin_mass[threadIdx.x * RS_PER + e];
       kc += bin_cnt[e];
       mc += bin_mass[e];
     }
-    uint32_t all;
-    double mass;
     cnt_before = rs_scan<uint32_t>(kc, s.wcnt, &all);
-    mass_before = rs_scan<double>(mc, s.wsum, &mass);
-    if (threadIdx.x == 0) { s.all_cnt = all + beyond; s.all_mass = mass; }
-    __syncthreads();
+    mass_before = rs_scan<double>(mc, s.wsum, &all_mass);
+    for (int r = 0; r < RS_CLUSTER; ++r) all += s.beyond[r];
+    all_cnt = all;
   }
-  // Fixed-point unit of the deviations: a CTA's sum of a bin with up to `sure` tokens stays inside 31 bits.
-  __device__ float dev_unit() const {
-    const float most = fmaxf(1.f - expf(-g.width * g.inv_t * 1.01f), 0x1p-20f) * (float)sure;
-    return ldexpf(1.f, (int)floorf(29.f - log2f(most)));
+  __device__ uint32_t most() const {
+    uint32_t m = 0;
+    for (int r = 0; r < RS_CLUSTER; ++r) m = max(m, s.most[r]);
+    return m;
+  }
+  // the bins' masses once more, or at last
+  __device__ void recollect(int room) {
+    RSCommand c{};
+    c.op = RS_MASSES; c.sure = room;
+    command(c);
+    scan_bins();
   }
 
   // First bin at which the running count or mass reaches the target (strict: exceeds it); when none does, RS_BINS by
   // count and the last one with a token by mass (a rounding is missing).
-  __device__ int cross(bool by_mass, double target, bool strict) {
-    if (threadIdx.x == 0) { s.sel_bin = RS_BINS; s.pick = 0; }
-    __syncthreads();
+  __device__ void cross(bool by_mass, double target, bool strict, int* bin) {
     uint32_t k = cnt_before;
     double m = mass_before;
+    int at = RS_BINS, full = 0;
 #pragma unroll
     for (int e = 0; e < RS_PER; ++e) {
       k += bin_cnt[e];
       m += bin_mass[e];
-      const double x = by_mass ? m : (double)k;
       if (!bin_cnt[e]) continue;
-      atomicMax(&s.pick, (int)threadIdx.x * RS_PER + e);
-      if (strict ? x > target : x >= target) { atomicMin(&s.sel_bin, (int)threadIdx.x * RS_PER + e); break; }
+      const int b = (int)threadIdx.x * RS_PER + e;
+      const double x = by_mass ? m : (double)k;
+      full = b;
+      if (at == RS_BINS && (strict ? x > target : x >= target)) at = b;
     }
+    at = __reduce_min_sync(0xffffffffu, at);
+    full = __reduce_max_sync(0xffffffffu, full);
+    if ((threadIdx.x & 31) == 0) {
+      if (at < RS_BINS) atomicMin(bin, at);
+      if (by_mass) atomicMax(&s.pick, full);
+    }
+  }
+  __device__ int cross_one(bool by_mass, double target, bool strict) {
     __syncthreads();
-    const int b = by_mass && s.sel_bin == RS_BINS ? s.pick : s.sel_bin;
+    if (threadIdx.x == 0) { s.bin_k = RS_BINS; s.pick = 0; }
     __syncthreads();
-    return b;
+    cross(by_mass, target, strict, &s.bin_k);
+    __syncthreads();
+    return by_mass && s.bin_k == RS_BINS ? s.pick : s.bin_k;
   }
   // tokens and mass of all bins before b, and of b
-  __device__ void at_bin(int b, uint32_t* before, double* mass, uint32_t* in) {
+  __device__ void at_bin(int b, uint32_t* before, double* mass, uint32_t* in, double* in_mass) {
     if ((int)threadIdx.x == min(b, RS_BINS - 1) / RS_PER) {
-      uint32_t k = cnt_before;
-      double m = mass_before;
+      uint32_t k = cnt_before, c = 0;
+      double m = mass_before, cm = 0;
 #pragma unroll
-      for (int e = 0; e < RS_PER; ++e)
-        if ((int)threadIdx.x * RS_PER + e < b) { k += bin_cnt[e]; m += bin_mass[e]; }
+      for (int e = 0; e < RS_PER; ++e) {
+        const int at = (int)threadIdx.x * RS_PER + e;
+        if (at < b) { k += bin_cnt[e]; m += bin_mass[e]; }
+        if (at == b) { c = bin_cnt[e]; cm = bin_mass[e]; }
+      }
       s.sel_cnt = k;
       s.sel_base = m;
-      uint32_t c = 0;
-#pragma unroll
-      for (int e = 0; e < RS_PER; ++e)
-        if ((int)threadIdx.x * RS_PER + e == b) c = bin_cnt[e];
-      s.sel_bin_cnt = b >= RS_BINS ? s.all_cnt - k : c;
+      s.sel_in = b >= RS_BINS ? all_cnt - k : c;
+      s.sel_mass = cm;
     }
     __syncthreads();
-    *before = s.sel_cnt; *mass = s.sel_base; *in = s.sel_bin_cnt;
-    __syncthreads();
+    *before = s.sel_cnt; *mass = s.sel_base; *in = s.sel_in; *in_mass = s.sel_mass;
   }
 
-  // sorts the n first of the list
+  // sorts the first n_list of the list
   __device__ void sort(int n_list) {
-    int np2 = 2;
-    while (np2 < n_list) np2 <<= 1;
-    for (int i = n_list + threadIdx.x; i < np2; i += RS_THREADS) s.list[i] = ~0ull;
-    __syncthreads();
-    for (int size = 2; size <= np2; size <<= 1) {
-      for (int step = size >> 1; step > 0; step >>= 1) {
-        for (int i = threadIdx.x; i < np2 / 2; i += RS_THREADS) {
-          const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
-          const unsigned long long x = s.list[lo], y = s.list[hi];
-          if ((x > y) == ((lo & size) == 0)) { s.list[lo] = y; s.list[hi] = x; }
-        }
-        __syncthreads();
+    const int t = threadIdx.x;
+    if (n_list <= RS_COUNT) {  // each token's place is how many come before it
+      unsigned long long x = 0;
+      int at = 0;
+      if (t < n_list) {
+        x = s.list[t];
+#pragma unroll 8
+        for (int i = 0; i < n_list; ++i) at += s.list[i] < x;
       }
+      __syncthreads();
+      if (t < n_list) s.list[at] = x;
+      __syncthreads();
+      return;
     }
+    // two neighbours a thread: steps of up to 32 stay in a warp
+    int np2 = 256;
+    while (np2 < n_list) np2 <<= 1;
+    for (int i = n_list + t; i < np2; i += RS_THREADS) s.list[i] = ~0ull;
+    __syncthreads();
+    unsigned long long x = ~0ull, y = ~0ull;
+    const bool mine = 2 * t < np2;
+    if (mine) { x = s.list[2 * t]; y = s.list[2 * t + 1]; }
+    for (int size = 2; size <= np2; size <<= 1) {
+      const bool up = ((2 * t) & size) == 0;
+      int step = size >> 1;
+      if (step > 32) {
+        if (mine) { s.list[2 * t] = x; s.list[2 * t + 1] = y; }
+        __syncthreads();
+        for (; step > 32; step >>= 1) {
+          for (int i = t; i < np2 / 2; i += RS_THREADS) {
+            const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
+            const unsigned long long p = s.list[lo], q = s.list[hi];
+            if ((p > q) == ((lo & size) == 0)) { s.list[lo] = q; s.list[hi] = p; }
+          }
+          __syncthreads();
+        }
+        if (mine) { x = s.list[2 * t]; y = s.list[2 * t + 1]; }
+      }
+      for (; step > 1; step >>= 1) {
+        const int o = step >> 1;  // threads between the two
+        const unsigned long long px = __shfl_xor_sync(0xffffffffu, x, o), py = __shfl_xor_sync(0xffffffffu, y, o);
+        const bool keep_small = ((t & o) == 0) == up;
+        x = (px < x) == keep_small ? px : x;
+        y = (py < y) == keep_small ? py : y;
+      }
+      if ((x > y) == up) { const unsigned long long z = x; x = y; y = z; }
+    }
+    if (mine) { s.list[2 * t] = x; s.list[2 * t + 1] = y; }
+    __syncthreads();
   }
   __device__ float list_logit(int i) const { return rs_unorder(~(uint32_t)(s.list[i] >> 32)); }
-  // weights of this thread's share of the sorted list and the mass before them
-  __device__ double list_masses(int n_list, double (&w)[RS_EACH], double* total) {
-    double loc = 0;
+  // s.cum: base and the mass of the sorted list up to and with each token
+  template <int EACH>
+  __device__ void list_masses_of(int n_list, double base) {
+    double w[EACH], loc = 0, total;
 #pragma unroll
-    for (int e = 0; e < RS_EACH; ++e) {
-      const int i = threadIdx.x * RS_EACH + e;
+    for (int e = 0; e < EACH; ++e) {
+      const int i = threadIdx.x * EACH + e;
       w[e] = i < n_list ? rs_weight(list_logit(i), g) : 0.0;
       loc += w[e];
     }
-    return rs_scan<double>(loc, s.wsum, total);
-  }
-  // First of the list's first n tokens at which base + mass reaches the target (strict: exceeds it); n - 1 when none does.
-  __device__ int list_cross(int n_list, const double (&w)[RS_EACH], double before, double target, bool strict) {
-    if (threadIdx.x == 0) s.pick = n_list - 1;
+    double m = base + rs_scan<double>(loc, s.wsum, &total);
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int i = threadIdx.x * EACH + e;
+      m += w[e];
+      if (i < n_list) s.cum[i] = m;
+    }
     __syncthreads();
-    double m = before;
+  }
+  __device__ void list_masses(int n_list, double base) {
+    if (n_list <= RS_THREADS) list_masses_of<1>(n_list, base);
+    else list_masses_of<RS_EACH>(n_list, base);
+  }
+  // how many of the list's first n tokens lie before the target: mass below it (strict: not above it)
+  __device__ int list_before(int n_list, double target, bool strict) {
+    int c = 0;
 #pragma unroll
     for (int e = 0; e < RS_EACH; ++e) {
-      m += w[e];
-      const int i = threadIdx.x * RS_EACH + e;
-      if (i < n_list && (strict ? m > target : m >= target)) { atomicMin(&s.pick, i); break; }
+      const int i = threadIdx.x + e * RS_THREADS;
+      if (e && n_list <= e * RS_THREADS) break;
+      c += __syncthreads_count(i < n_list && (strict ? s.cum[i] <= target : s.cum[i] < target));
     }
-    __syncthreads();
-    const int p = s.pick;
-    __syncthreads();
-    return p;
-  }
-  // mass of the list's tokens up to and with i
-  __device__ double list_mass_at(int i, const double (&w)[RS_EACH], double before) {
-    if ((int)threadIdx.x == i / RS_EACH) {
-      double m = before;
-#pragma unroll
-      for (int e = 0; e < RS_EACH; ++e)
-        if ((int)threadIdx.x * RS_EACH + e <= i) m += w[e];
-      s.pick_mass = m;
-    }
-    __syncthreads();
-    const double m = s.pick_mass;
-    __syncthreads();
-    return m;
+    return c;
   }
 
   // The first token in order at which the running count or mass reaches the target (strict: exceeds it): its index, its
   // weight, and the count and mass up to and with it.
   struct Pick { int idx; double w; uint32_t cnt; double mass; };
-  __device__ Pick select(bool by_mass, double target, bool strict) {
-    const int b = cross(by_mass, target, strict);
+  __device__ Pick select(bool by_mass, double target, bool strict, bool last) {
+    const int b = cross_one(by_mass, target, strict);
     uint32_t before, in;
-    double base;
-    at_bin(b, &before, &base, &in);
+    double base, in_mass;
+    at_bin(b, &before, &base, &in, &in_mass);
     Pick p;
     if (in <= RS_CAP) {
       RSCommand c{};
-      c.op = RS_GATHER; c.b0 = c.b1 = b;
+      c.op = RS_GATHER; c.b0 = c.b1 = b; c.last = last;
       command(c);
       const int n_list = (int)s.n_list;
       sort(n_list);
-      double w[RS_EACH], total;
-      const double m0 = list_masses(n_list, w, &total);
-      const int i = by_mass ? list_cross(n_list, w, base + m0, target, strict)
-                            : min(max((int)(target - before) - 1, 0), n_list - 1);
-      p.mass = list_mass_at(i, w, base + m0);
+      list_masses(n_list, base);
+      const int i = min(max(by_mass ? list_before(n_list, target, strict) : (int)(target - before) - 1, 0), n_list - 1);
+      p.mass = s.cum[i];
       p.idx = (int)(uint32_t)s.list[i];
       p.w = rs_weight(list_logit(i), g);
       p.cnt = before + i + 1;
@@ -407,7 +500,7 @@ struct RSRow {
     c.op = RS_RADIX; c.b0 = b;
     c.z0 = b < RS_BINS ? (double)b * (double)g.width / g.t : 0.0;
     const double unit = b < RS_BINS ? exp(-c.z0) : 0.0;
-    double each = 0;   // of the tokens left: their weight / unit
+    double each = 0;   // of the tokens left: their weight
     uint32_t left = 0;
     for (int round = 0; round < 4; ++round) {
       c.shift = 24 - 8 * round;
@@ -437,10 +530,9 @@ struct RSRow {
       }
       __syncthreads();
       const int at = s.pick < 256 ? s.pick : (int)s.pick_cnt;
+      if ((int)threadIdx.x == at) { s.sel_cnt = before + kb; s.sel_base = base + mb; s.sel_in = k; s.pick_w = k ? mass / k : 0.0; }
       __syncthreads();
-      if ((int)threadIdx.x == at) { s.sel_cnt = before + kb; s.sel_base = base + mb; s.sel_bin_cnt = k; s.pick_w = k ? mass / k : 0.0; }
-      __syncthreads();
-      before = s.sel_cnt; base = s.sel_base; left = s.sel_bin_cnt; each = s.pick_w;
+      before = s.sel_cnt; base = s.sel_base; left = s.sel_in; each = s.pick_w;
       c.prefix = c.prefix << 8 | (uint32_t)(255 - at);
       __syncthreads();
     }
@@ -462,189 +554,167 @@ struct RSRow {
     return p;
   }
 
-  __device__ void answer(int row, int idx, double prob, uint32_t kept) {
+  __device__ void answer(int r, int idx, double prob, uint32_t kept) {
     if (threadIdx.x == 0) {
-      a.tokens[row] = idx;
-      if (a.prob) a.prob[row] = (float)prob;
-      if (a.kept) a.kept[row] = (int)kept;
+      a.tokens[r] = idx;
+      if (a.prob) a.prob[r] = (float)prob;
+      if (a.kept) a.kept[r] = (int)kept;
     }
   }
 
-  // the bins' masses once more, or at last
-  __device__ void recollect(int room) {
-    RSCommand c{};
-    c.op = RS_MASSES; c.sure = room;
-    command(c);
-    collect(true);
-  }
-
-  __device__ void lead(int row, int k, double top_p, double min_p, double u, bool masses) {
-    collect(masses);
-    if (masses && s.most_cnt) recollect((int)s.most_cnt);
-    const uint32_t all = s.all_cnt;
+  __device__ void lead(int r, int k, double top_p, double u, bool masses) {
+    scan_bins();
+    if (masses && most()) recollect((int)most());
+    const uint32_t all = all_cnt;
     const bool cut_k = k > 0 && (uint32_t)k < all;
     const uint32_t cut = cut_k ? (uint32_t)k : all;
     const bool by_p = top_p < 1, by_m = min_p > 0;
     const bool listed = cut_k || !masses;  // the mass that top-p goes by is that of tokens that are all in the list
     // the last bin that a kept token can lie in
-    int last = RS_BINS;
-    if (cut_k) last = cross(false, (double)k, false);
-    if (by_m && !(listed && by_p)) {
-      const double x = -log(min_p) * g.t * (double)g.sx;
-      last = min(last, x < RS_BINS ? (int)fmax(x, 0.0) + 1 : RS_BINS);
-    }
-    if (by_p && !listed) last = min(last, cross(true, top_p * s.all_mass, false));
+    const double over = by_m ? -log(min_p) * g.t * (double)g.sx : 0.0;
+    __syncthreads();
+    if (threadIdx.x == 0) { s.bin_k = s.bin_p = RS_BINS; s.pick = 0; }
+    __syncthreads();
+    if (cut_k) cross(false, (double)k, false, &s.bin_k);
+    if (by_p && !listed) cross(true, top_p * all_mass, false, &s.bin_p);
+    __syncthreads();
+    int last = s.bin_k;
+    if (by_m && !(listed && by_p)) last = min(last, over < RS_BINS ? (int)fmax(over, 0.0) + 1 : RS_BINS);
+    if (by_p && !listed) last = min(last, s.bin_p == RS_BINS ? s.pick : s.bin_p);
     uint32_t before, in;
-    double base;
-    at_bin(last, &before, &base, &in);
+    double base, in_mass;
+    at_bin(last, &before, &base, &in, &in_mass);
     if (before + in <= RS_CAP) {
       RSCommand c{};
-      c.op = RS_GATHER; c.b1 = last;
+      c.op = RS_GATHER; c.b1 = last; c.last = 1;
       command(c);
       const int n_list = (int)s.n_list;
       sort(n_list);
-      double w[RS_EACH], total;
-      const double m0 = list_masses(n_list, w, &total);
+      list_masses(n_list, 0.0);
       int kept = (int)min(cut, (uint32_t)n_list);
       if (by_p) {
         // mass of the cut: of the list's first k, or of the list and the bins behind it
-        const double mass = listed ? list_mass_at(kept - 1, w, m0) : total + (s.all_mass - base - bin_mass_of(last));
-        kept = min(kept, list_cross(kept, w, m0, top_p * mass, false) + 1);
+        const double mass = listed ? s.cum[kept - 1] : s.cum[n_list - 1] + (all_mass - base - in_mass);
+        kept = min(kept, list_before(kept, top_p * mass, false) + 1);
       }
       if (by_m) {
-        uint32_t ok = 0, all_ok;
+        int ok = 0;
 #pragma unroll
-        for (int e = 0; e < RS_EACH; ++e) ok += (int)threadIdx.x * RS_EACH + e < n_list && w[e] >= min_p;
-        rs_scan<uint32_t>(ok, s.wcnt, &all_ok);
-        kept = min(kept, max((int)all_ok, 1));
+        for (int e = 0; e < RS_EACH; ++e) {
+          const int i = threadIdx.x + e * RS_THREADS;
+          if (e && n_list <= e * RS_THREADS) break;
+          ok += __syncthreads_count(i < n_list && rs_weight(list_logit(i), g) >= min_p);
+        }
+        kept = min(kept, max(ok, 1));
       }
-      const double mass = list_mass_at(kept - 1, w, m0);
-      const int i = list_cross(kept, w, m0, u * mass, true);
-      answer(row, (int)(uint32_t)s.list[i], rs_weight(list_logit(i), g) / mass, (uint32_t)kept);
+      const double mass = s.cum[kept - 1];
+      const int i = min(list_before(kept, u * mass, true), kept - 1);
+      answer(r, (int)(uint32_t)s.list[i], rs_weight(list_logit(i), g) / mass, (uint32_t)kept);
       return;
     }
     // long prefixes: each end by itself
-    if (!masses) {  // the k-th token's bin is crowded
-      recollect((int)max(s.most_cnt, (uint32_t)RS_SURE));
-    }
+    if (!masses) recollect((int)max(most(), (uint32_t)RS_SURE));  // the k-th token's bin is crowded
     uint32_t kept = cut;
-    double mass = s.all_mass;
-    if (cut_k) mass = select(false, (double)k, false).mass;
+    double mass = all_mass;
+    if (cut_k) mass = select(false, (double)k, false, false).mass;
     if (by_p) {
-      const Pick p = select(true, top_p * mass, false);
+      const Pick p = select(true, top_p * mass, false, false);
       if (p.cnt < kept) { kept = p.cnt; mass = p.mass; }
     }
     if (by_m) {
-      const double x = -log(min_p) * g.t * (double)g.sx;
-      const int b = x < RS_BINS ? (int)fmax(x, 0.0) : RS_BINS;
+      const int b = over < RS_BINS ? (int)fmax(over, 0.0) : RS_BINS;
       RSCommand c{};
       c.op = RS_OVER; c.b0 = b - 1; c.b1 = min(b + 1, RS_BINS);
       command(c);
-      const uint32_t over = max(s.over, 1u);
+      const uint32_t n_over = max(s.over, 1u);
       __syncthreads();
-      if (over < kept) { kept = over; mass = select(false, (double)over, false).mass; }
+      if (n_over < kept) { kept = n_over; mass = select(false, (double)n_over, false, false).mass; }
     }
-    Pick p = select(true, u * mass, true);
-    if (p.cnt > kept) p = select(false, (double)kept, false);  // the two sums of a bin differ by a rounding
-    answer(row, p.idx, p.w / mass, kept);
-  }
-  __device__ double bin_mass_of(int b) {
-    if (threadIdx.x == 0) s.pick_mass = 0;
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < RS_PER; ++e)
-      if ((int)threadIdx.x * RS_PER + e == b) s.pick_mass = bin_mass[e];
-    __syncthreads();
-    const double m = s.pick_mass;
-    __syncthreads();
-    return m;
+    Pick p = select(true, u * mass, true, !cut_k && !by_p && !by_m);
+    if (p.cnt > kept) p = select(false, (double)kept, false, true);  // the two sums of a bin differ by a rounding
+    answer(r, p.idx, p.w / mass, kept);
   }
 };
 
-template <bool STAGED>
+template <class T, bool STAGED>
 __global__ void __launch_bounds__(RS_THREADS, 2) sample_rows_kernel(const RSArgs a) {
   extern __shared__ __align__(16) uint8_t rs_raw[];
   RSSmem& s = *reinterpret_cast<RSSmem*>(rs_raw);
-  float* stage = reinterpret_cast<float*>(rs_raw + sizeof(RSSmem));
+  T* stage = reinterpret_cast<T*>(rs_raw + (sizeof(RSSmem) + 15) / 16 * 16);
   cg::cluster_group cl = cg::this_cluster();
+  rs_arrive();  // waited for before anything is written to another CTA: it has to be there
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cl.block_rank();
-  const int row = (int)(blockIdx.x / RS_CLUSTER);
+  const int r = (int)(blockIdx.x / RS_CLUSTER);
   const int i0 = min(rank * a.per, a.vocab), n = min(a.per, a.vocab - i0);
-  RSRow<STAGED> r{s, stage, a, (int64_t)row * a.ld, i0, n, RSGeom{}, cl, 0.0, RS_SURE};
+  const T* row = reinterpret_cast<const T*>(a.logits) + (int64_t)r * a.ld;
+  RSRow<T, STAGED> w{s, stage, a, row, i0, n, RSGeom{}, cl, 0.0, RS_SURE, false};
 
-  // 1. this CTA's logits, the largest with its index, the smallest that is a number
-  RSStat st{-INFINITY, INFINITY, 0x7fffffff, 0};
-  auto see = [&](int i, float l) {
-    if (l > st.mx) { st.mx = l; st.idx = i0 + i; }
-    if (l > -INFINITY) st.mn = fminf(st.mn, l);
-    if (STAGED) stage[i] = l;
-  };
-  if (a.vec) {  // 16 bytes a lane; the shares are multiples of 8 logits
-    const int v = a.dtype == N730_F32 ? 4 : 8, nv = n / v;
-    const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.logits) +
-                                                    (r.base + i0) * (a.dtype == N730_F32 ? 4 : 2));
-    constexpr int U = 4;
-    for (int j = tid; j < nv; j += U * RS_THREADS) {
-      uint4 x[U];
-#pragma unroll
-      for (int e = 0; e < U; ++e)
-        if (j + e * RS_THREADS < nv) x[e] = ld_stream_v4(p + j + e * RS_THREADS);
-#pragma unroll
-      for (int e = 0; e < U; ++e) {
-        const int i = (j + e * RS_THREADS) * v;
-        if (j + e * RS_THREADS >= nv) break;
-        const uint32_t y[4] = {x[e].x, x[e].y, x[e].z, x[e].w};
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          if (a.dtype == N730_F32) {
-            see(i + h, rs_clean(__uint_as_float(y[h])));
-          } else {
-            const float2 f = a.dtype == N730_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&y[h]))
-                                                 : make_float2(__uint_as_float(y[h] << 16), __uint_as_float(y[h] & 0xffff0000u));
-            see(i + 2 * h, rs_clean(f.x));
-            see(i + 2 * h + 1, rs_clean(f.y));
-          }
-        }
-      }
-    }
-    for (int i = nv * v + tid; i < n; i += RS_THREADS) see(i, rs_clean(kv8_load1(a.logits, r.base + i0 + i, a.dtype)));
-  } else {
-    for (int i = tid; i < n; i += RS_THREADS) see(i, rs_clean(kv8_load1(a.logits, r.base + i0 + i, a.dtype)));
+  // 1. this CTA's logits, the largest and the smallest that is a number.  Copies of 16 bytes and more; the shares are
+  // multiples of 8 logits, what is left of a row's end comes by itself.
+  constexpr int V = 16 / sizeof(T);
+  const int nv = a.vec ? n / V : 0;
+  if (STAGED) {
+    for (int v = tid; v < nv; v += RS_THREADS)
+      asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" :: "r"(smem_u32(stage + v * V)), "l"(row + i0 + v * V) : "memory");
   }
-  auto join = [](RSStat& x, const RSStat& y) {
-    if (y.mx > x.mx || (y.mx == x.mx && y.idx < x.idx)) { x.mx = y.mx; x.idx = y.idx; }
-    x.mn = fminf(x.mn, y.mn);
+  const float t = a.temperature ? a.temperature[r] : 1.f;
+  const int k = a.top_k ? a.top_k[r] : 0;
+  const float p = a.top_p ? a.top_p[r] : 1.f, q = a.min_p ? a.min_p[r] : 0.f, un = a.u[r];
+  for (int i = tid; i < RS_BINS; i += RS_THREADS) { s.cnt[i] = 0; s.dev[i] = 0; }
+  if (tid == 0) s.own_beyond = 0;
+  RSStat st{-INFINITY, INFINITY};
+  auto see = [&](float l) {  // NaN is neither
+    st.mx = fmaxf(st.mx, l);
+    st.mn = fminf(st.mn, l > -INFINITY ? l : INFINITY);
   };
+  if (STAGED) {
+    for (int i = nv * V + tid; i < n; i += RS_THREADS) {
+      const T x = row[i0 + i];
+      stage[i] = x;
+      see(rs_float(x));
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    for (int v = tid; v < nv; v += RS_THREADS) {  // what this thread has copied
+      const uint4 x = *reinterpret_cast<const uint4*>(stage + v * V);
+      const T* e = reinterpret_cast<const T*>(&x);
+#pragma unroll
+      for (int j = 0; j < V; ++j) see(rs_float(e[j]));
+    }
+  } else {
+    for (int i = tid; i < n; i += RS_THREADS) see(rs_float(row[i0 + i]));
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    RSStat y;
-    y.mx = __shfl_xor_sync(0xffffffffu, st.mx, o);
-    y.mn = __shfl_xor_sync(0xffffffffu, st.mn, o);
-    y.idx = __shfl_xor_sync(0xffffffffu, st.idx, o);
-    join(st, y);
+    st.mx = fmaxf(st.mx, __shfl_xor_sync(0xffffffffu, st.mx, o));
+    st.mn = fminf(st.mn, __shfl_xor_sync(0xffffffffu, st.mn, o));
   }
   if (lane == 0) s.wstat[warp] = st;
-  for (int i = tid; i < RS_BINS + 4; i += RS_THREADS) { s.cnt[i] = 0; s.dev[i] = 0; }
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < RS_WARPS; ++w) join(st, s.wstat[w]);
-    s.stat = st;
+  rs_wait();
+  if (tid < RS_CLUSTER) {
+    for (int v = 0; v < RS_WARPS; ++v) { st.mx = fmaxf(st.mx, s.wstat[v].mx); st.mn = fminf(st.mn, s.wstat[v].mn); }
+    cl.map_shared_rank(&s, tid)->stats[rank] = st;
   }
-  cl.sync();
-  st = cl.map_shared_rank(&s, 0)->stat;
-  for (int k = 1; k < RS_CLUSTER; ++k) join(st, cl.map_shared_rank(&s, k)->stat);
-  const float t = a.temperature ? a.temperature[row] : 1.f;
-  if (st.mx == -INFINITY || !(t > 0.f)) {  // no token, or greedy
-    if (rank == 0) r.answer(row, st.mx == -INFINITY ? -1 : st.idx, st.mx == -INFINITY ? 0.0 : 1.0, st.mx == -INFINITY ? 0u : 1u);
-    cl.sync();  // the others may still read this CTA's statistics
+  if (tid == 0) s.first = 0x7fffffff;
+  rs_sync();
+#pragma unroll
+  for (int c = 0; c < RS_CLUSTER; ++c) { st.mx = fmaxf(st.mx, s.stats[c].mx); st.mn = fminf(st.mn, s.stats[c].mn); }
+  st.mx += 0.f;
+  if (st.mx == -INFINITY || !(t > 0.f)) {  // no token, or greedy: the first of the largest
+    int at = 0x7fffffff;
+    if (st.mx > -INFINITY)
+      for (int i = tid; i < n; i += RS_THREADS)
+        if (w.raw(i) == st.mx) { at = i0 + i; break; }
+    at = (int)__reduce_min_sync(0xffffffffu, (unsigned)at);
+    if (lane == 0 && at != 0x7fffffff) atomicMin(&cl.map_shared_rank(&s, 0)->first, at);
+    rs_sync();
+    if (rank == 0) w.answer(r, st.mx == -INFINITY ? -1 : s.first, st.mx == -INFINITY ? 0.0 : 1.0, st.mx == -INFINITY ? 0u : 1u);
     return;
   }
-  const int k = a.top_k ? a.top_k[row] : 0;
-  const float p = a.top_p ? a.top_p[row] : 1.f, q = a.min_p ? a.min_p[row] : 0.f, un = a.u[row];
   const bool masses = !(k > 0 && k <= RS_CAP / 2);
 
   // 2. the bins
-  RSGeom& g = r.g;
+  RSGeom& g = w.g;
   g.mx = st.mx;
   const float tc = fminf(fmaxf(t, 0x1p-100f), 0x1p100f);
   g.t = tc;
@@ -653,27 +723,45 @@ __global__ void __launch_bounds__(RS_THREADS, 2) sample_rows_kernel(const RSArgs
   const float span = fminf((st.mx - st.mn) * (1.f + 0x1p-20f), RS_SPAN * fmaxf(tc, 1.f));
   g.sx = span > 1e-30f ? (float)RS_BINS / span : 0.f;
   g.width = span > 1e-30f ? span / (float)RS_BINS : 0.f;
-  r.zmin = q > 0.f ? log((double)q) : -INFINITY;
-  r.fill(true, masses);
-  cl.sync();
+  w.min_p = q > 0.f ? (double)q : 0.0;
+  w.fill(true, masses);
+  rs_sync();
+  w.reduce(masses);
+  rs_sync();
 
   // 3. ends of the prefixes and the token
   if (rank == 0) {
     const double up = un > 0.f ? fmin((double)un, 1.0) : 0.0;
-    r.lead(row, k, p < 1.f ? (double)p : 1.0, q > 0.f ? (double)q : 0.0, up, masses);
-    __syncthreads();
-    if (tid == 0) s.cmd.op = RS_DONE;
-    cl.sync();
-  } else {
-    for (;;) {
-      cl.sync();
-      const RSCommand c = cl.map_shared_rank(&s, 0)->cmd;
-      if (c.op == RS_DONE) break;
-      r.serve(c);
-      cl.sync();
+    w.lead(r, k, p < 1.f ? (double)p : 1.0, up, masses);
+    if (!w.alone) {
+      __syncthreads();
+      RSCommand c{};
+      w.post(c);
+      rs_sync();
     }
+    return;
   }
-  cl.sync();  // no CTA leaves while another reads its shared memory
+  for (;;) {
+    rs_sync();
+    const RSCommand c = s.cmd;
+    if (c.op == RS_DONE) return;
+    w.serve(c);
+    rs_arrive();
+    if (c.last) return;  // nobody reads this CTA's memory any more
+    rs_wait();
+  }
+}
+
+template <class T>
+static int rs_launch(const RSArgs& a, int batch, cudaStream_t st) {
+  const size_t fixed = (sizeof(RSSmem) + 15) / 16 * 16, slice = (size_t)a.per * sizeof(T);
+  const dim3 grid((unsigned)batch * RS_CLUSTER), block(RS_THREADS);
+  if (slice <= RS_STAGE_MAX) {
+    if (int rc = smem_attr_once<sample_rows_kernel<T, true>>((int)(fixed + RS_STAGE_MAX))) return rc;
+    return kv8_launch_cluster(sample_rows_kernel<T, true>, grid, RS_CLUSTER, block, fixed + slice, st, false, a);
+  }
+  if (int rc = smem_attr_once<sample_rows_kernel<T, false>>((int)fixed)) return rc;
+  return kv8_launch_cluster(sample_rows_kernel<T, false>, grid, RS_CLUSTER, block, fixed, st, false, a);
 }
 
 }  // namespace n730
@@ -693,17 +781,12 @@ N730_API int n730_sample_rows(const void* d_logits, int dtype, int batch, int vo
                    kv8_aligned(4, d_temperature, d_top_p, d_min_p, d_u, d_prob) && kv8_aligned(4, d_top_k, d_tokens, d_kept),
                N730_BAD_ARG, "%s: pointers must lie on whole elements", what);
   RSArgs a{};
-  a.logits = d_logits; a.ld = ld; a.vocab = vocab; a.dtype = dtype;
+  a.logits = d_logits; a.ld = ld; a.vocab = vocab;
   a.per = ((vocab + RS_CLUSTER - 1) / RS_CLUSTER + 7) / 8 * 8;
   a.vec = ((uintptr_t)d_logits & 15) == 0 && ld * es % 16 == 0;
   a.temperature = d_temperature; a.top_k = d_top_k; a.top_p = d_top_p; a.min_p = d_min_p; a.u = d_u;
   a.tokens = d_tokens; a.prob = d_prob; a.kept = d_kept;
-  const size_t slice = (size_t)a.per * 4;
-  const bool staged = slice <= RS_STAGE_MAX;
-  const dim3 grid((unsigned)batch * RS_CLUSTER), block(RS_THREADS);
-  if (staged) {
-    if (int rc = smem_attr_once<sample_rows_kernel<true>>((int)(sizeof(RSSmem) + RS_STAGE_MAX))) return rc;
-    return kv8_launch_cluster(sample_rows_kernel<true>, grid, RS_CLUSTER, block, sizeof(RSSmem) + slice, (cudaStream_t)stream, false, a);
-  }
-  return kv8_launch_cluster(sample_rows_kernel<false>, grid, RS_CLUSTER, block, sizeof(RSSmem), (cudaStream_t)stream, false, a);
+  cudaStream_t st = (cudaStream_t)stream;
+  return dtype == N730_F32 ? rs_launch<float>(a, batch, st) : dtype == N730_F16 ? rs_launch<__half>(a, batch, st)
+                                                                                : rs_launch<__nv_bfloat16>(a, batch, st);
 }
