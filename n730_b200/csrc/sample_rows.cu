@@ -29,11 +29,11 @@
 namespace n730 {
 namespace cg = cooperative_groups;
 
-constexpr int RS_CLUSTER = 8;
+constexpr int RS_CLUSTER = 8;      // CTAs of a row, one for rows of up to RS_ALONE logits: no exchange, 15 -> 10 us at 1000
+constexpr int RS_ALONE = 16384;
 constexpr int RS_THREADS = 512;
 constexpr int RS_WARPS = RS_THREADS / 32;
 constexpr int RS_BINS = 1536;      // as many as leave room for two CTAs of 19008 fp32 logits (a row of 152064) an SM
-constexpr int RS_SHARE = RS_BINS / RS_CLUSTER;
 constexpr int RS_PER = RS_BINS / RS_THREADS;
 constexpr int RS_CAP = 1024;       // tokens that are sorted at once
 constexpr int RS_EACH = RS_CAP / RS_THREADS;
@@ -65,7 +65,8 @@ struct RSStat { float mx, mn; };
 struct RSSmem {
   uint32_t cnt[RS_BINS];             // by bin; also the counts of 256 digits
   int32_t dev[RS_BINS];              // sums of w / w(edge) - 1; also the digits' masses, low and high words
-  union { unsigned long long list[RS_CAP]; uint32_t bin_cnt[RS_BINS]; uint2 share[2 * RS_SHARE]; };  // list: ~order << 32 | index
+  uint2 share[2 * RS_BINS / RS_CLUSTER];
+  union { unsigned long long list[RS_CAP]; uint32_t bin_cnt[RS_BINS]; };  // list: ~order << 32 | index
   union { double cum[RS_CAP]; double bin_mass[RS_BINS]; };
   RSCommand cmd;
   RSStat stats[RS_CLUSTER];
@@ -79,9 +80,21 @@ struct RSSmem {
   int bin_k, bin_p, bin_last, pick, found, first;
 };
 
-__device__ __forceinline__ void rs_arrive() { __syncwarp(); asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void rs_wait() { __syncwarp(); asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ void rs_sync() { rs_arrive(); rs_wait(); }
+// a row's CTAs meet
+template <int CL>
+__device__ __forceinline__ void rs_arrive() {
+  if (CL == 1) return;
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+template <int CL>
+__device__ __forceinline__ void rs_wait() {
+  if (CL == 1) { __syncthreads(); return; }
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+template <int CL>
+__device__ __forceinline__ void rs_sync() { rs_arrive<CL>(); rs_wait<CL>(); }
 
 // the order of logits as unsigned numbers (largest largest); logits here are no NaN and no -0
 __device__ __forceinline__ uint32_t rs_order(float x) {
@@ -94,20 +107,49 @@ __device__ __forceinline__ float rs_float(float x) { return x; }
 __device__ __forceinline__ float rs_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ float rs_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// A row's bins: bin = floor((max - l) * sx), edge(b) = b * width below the largest.
+// A row's bins: bin = floor((max - l) * sx); edge(b), its upper end, is max - b * width as fp32 rounds it.
 struct RSGeom {
   float mx, sx, width, inv_t;
   double t;
 };
-__device__ __forceinline__ float rs_below(float l, const RSGeom& g) { return l == g.mx ? 0.f : g.mx - l; }
+__device__ __forceinline__ float rs_place(float l, const RSGeom& g) { return (l == g.mx ? 0.f : g.mx - l) * g.sx; }
+// NaN and -infinity have no place below RS_BINS
 __device__ __forceinline__ int rs_bin(float l, const RSGeom& g) {
-  const float x = rs_below(l, g) * g.sx;
+  const float x = rs_place(l, g);
   return x < (float)RS_BINS ? (int)x : RS_BINS;
 }
+__device__ __forceinline__ float rs_edge(float b, const RSGeom& g) { return fmaf(-b, g.width, g.mx); }
 __device__ __forceinline__ double rs_weight(float l, const RSGeom& g) {
   return l == g.mx ? 1.0 : g.mx == INFINITY ? 0.0 : exp(((double)l - (double)g.mx) / g.t);
 }
 
+// Exclusive scans over the block in thread order; the totals.
+__device__ __forceinline__ void rs_scan2(uint32_t& k, double& m, RSSmem& s, uint32_t* all_k, double* all_m) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t ik = k;
+  double im = m;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t nk = __shfl_up_sync(0xffffffffu, ik, o);
+    const double nm = __shfl_up_sync(0xffffffffu, im, o);
+    if (lane >= o) { ik += nk; im += nm; }
+  }
+  __syncthreads();
+  if (lane == 31) { s.wcnt[warp] = ik; s.wsum[warp] = im; }
+  __syncthreads();
+  uint32_t bk = 0, tk = 0;
+  double bm = 0, tm = 0;
+#pragma unroll
+  for (int w = 0; w < RS_WARPS; ++w) {
+    const uint32_t xk = s.wcnt[w];
+    const double xm = s.wsum[w];
+    if (w < warp) { bk += xk; bm += xm; }
+    tk += xk; tm += xm;
+  }
+  *all_k = tk; *all_m = tm;
+  k = bk + ik - k;
+  m = bm + im - m;
+}
 // Exclusive scan over the block in thread order; *total the sum.
 template <class V>
 __device__ V rs_scan(V v, V* warps, V* total) {
@@ -132,8 +174,9 @@ __device__ V rs_scan(V v, V* warps, V* total) {
   return before + inc - v;
 }
 
-template <class T, bool STAGED>
+template <class T, bool STAGED, int CL>
 struct RSRow {
+  static constexpr int V = 16 / sizeof(T), SHARE = RS_BINS / CL;
   RSSmem& s;
   T* stage;              // this CTA's logits
   const RSArgs& a;
@@ -147,6 +190,27 @@ struct RSRow {
 
   __device__ float raw(int i) const { return rs_float(STAGED ? stage[i] : row[i0 + i]); }
   __device__ float get(int i) const { return rs_clean(raw(i)); }
+  // f(first index, V logits) over this CTA's, V = 16 bytes of them, NaN behind the last.
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    for (int i = threadIdx.x * V; i < n; i += RS_THREADS * V) {
+      float l[V];
+      if (STAGED) {
+        const uint4 x = *reinterpret_cast<const uint4*>(stage + i);
+        const T* e = reinterpret_cast<const T*>(&x);
+#pragma unroll
+        for (int j = 0; j < V; ++j) l[j] = rs_float(e[j]);
+        if (i + V > n)
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (i + j >= n) l[j] = NAN;
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) l[j] = i + j < n ? rs_float(row[i0 + i + j]) : NAN;
+      }
+      f(i, l);
+    }
+  }
 
   // Fixed-point unit of the deviations: a CTA's sum of a bin with up to `sure` tokens stays inside 31 bits.
   __device__ float dev_unit() const {
@@ -158,32 +222,58 @@ struct RSRow {
     const float unit = dev_unit();
     const bool narrow = g.width * g.inv_t < 0x1p-6f;
     uint32_t beyond = 0;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < n; i += RS_THREADS) {
-      const float l = get(i);
-      if (l == -INFINITY) continue;
-      const int b = rs_bin(l, g);
-      if (b == RS_BINS) { ++beyond; continue; }
-      if (count) atomicAdd(&s.cnt[b], 1u);
-      if (masses) {
-        // y = (l - max + edge) / T, with the rounding of max - l put back
-        const float d = rs_below(l, g), bb = d - g.mx, err = l == g.mx ? 0.f : (g.mx - (d - bb)) - (l + bb);
-        const float y = -(fmaf(-(float)b, g.width, d) + err) * g.inv_t;
-        const float c = narrow ? y * fmaf(y, fmaf(y, fmaf(y, 1.f / 24, 1.f / 6), 0.5f), 1.f) : expm1f(y);
-        atomicAdd(&s.dev[b], __float2int_rn(c * unit));
+    each([&](int, const float (&l)[V]) {
+      int b[V], c[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float x = rs_place(l[j], g), f = __fadd_rd(x, 8388608.f);  // 2^23 + floor(x)
+        const bool in = x < (float)RS_BINS;
+        beyond += !in && l[j] > -INFINITY;
+        b[j] = in ? __float_as_int(f) & 0x7fffff : -1;
+        if (masses) {
+          // y = (l - edge) / T: the two are near, their difference is exact but for what is below 2^-24 of a bin
+          const float y = l[j] == g.mx ? 0.f : (l[j] - rs_edge(f - 8388608.f, g)) * g.inv_t;
+          const float e = narrow ? y * fmaf(y, fmaf(y, fmaf(y, 1.f / 24, 1.f / 6), 0.5f), 1.f) : expm1f(y);
+          c[j] = __float_as_int(fmaf(e, unit, 12582912.f)) - 0x4b400000;  // to the nearest whole number, below 2^22
+        }
       }
-    }
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (b[j] >= 0) {
+          if (count) atomicAdd(&s.cnt[b[j]], 1u);
+          if (masses) atomicAdd(&s.dev[b[j]], c[j]);
+        }
+    });
     if (count && beyond) atomicAdd(&s.own_beyond, beyond);
   }
   // This CTA's share of the bins, added up over the cluster, to the first CTA.  The cluster has filled before.
   __device__ void reduce(bool masses) {
+    const float unit = dev_unit();
+    auto mass_of = [&](int b, uint32_t k, int64_t d) {
+      return masses && k ? rs_weight(rs_edge((float)b, g), g) * ((double)k + (double)d / unit) : 0.0;
+    };
+    if (CL == 1) {
+      uint32_t most = 0;
+      for (int b = threadIdx.x; b < RS_BINS; b += RS_THREADS) {
+        const uint32_t k = s.cnt[b];
+        most = max(most, k);
+        s.bin_cnt[b] = k;
+        s.bin_mass[b] = mass_of(b, k, s.dev[b]);
+      }
+      if (threadIdx.x == 0) s.own_most = 0;
+      __syncthreads();
+      if (most > RS_SURE) atomicMax(&s.own_most, most);
+      __syncthreads();
+      if (threadIdx.x == 0) { s.beyond[0] = s.own_beyond; s.most[0] = s.own_most; }
+      return;
+    }
     const int t = threadIdx.x, rank = (int)cl.block_rank();
     uint32_t k = 0, most = 0;
-    int d[RS_CLUSTER / 2] = {};
-    if (t < 2 * RS_SHARE) {
-      const int b = rank * RS_SHARE + t % RS_SHARE, r0 = t / RS_SHARE * (RS_CLUSTER / 2);
+    int d[CL] = {};
+    if (t < 2 * SHARE) {  // two threads a bin, half of the CTAs each
+      const int b = rank * SHARE + t % SHARE, r0 = t / SHARE * (CL / 2);
 #pragma unroll
-      for (int r = 0; r < RS_CLUSTER / 2; ++r) {
+      for (int r = 0; r < CL / 2; ++r) {
         const RSSmem* o = cl.map_shared_rank(&s, r0 + r);
         const uint32_t x = o->cnt[b];
         k += x;
@@ -191,31 +281,24 @@ struct RSRow {
         if (masses) d[r] = o->dev[b];
       }
     }
-    int64_t dd = (int64_t)d[0] + d[1] + d[2] + d[3];
-    // halves meet: deviations in two words
-    if (t >= RS_SHARE && t < 2 * RS_SHARE) {
+    int64_t dd = 0;
+#pragma unroll
+    for (int r = 0; r < CL / 2; ++r) dd += d[r];
+    if (t >= SHARE && t < 2 * SHARE) {  // deviations in two words
       s.share[t] = make_uint2((uint32_t)dd, (uint32_t)(dd >> 32));
-      s.share[t - RS_SHARE].x = k;
+      s.share[t - SHARE].x = k;
     }
     if (t == 0) s.own_most = 0;
     __syncthreads();
     RSSmem* lead = cl.map_shared_rank(&s, 0);
     if (most > RS_SURE) atomicMax(&s.own_most, most);
-    uint32_t kk = 0;
-    double mass = 0;
-    if (t < RS_SHARE) {
-      kk = k + s.share[t].x;
-      if (masses && kk) {
-        dd += (int64_t)((unsigned long long)s.share[t + RS_SHARE].y << 32 | s.share[t + RS_SHARE].x);
-        mass = exp(-(double)(rank * RS_SHARE + t) * (double)g.width / g.t) * ((double)kk + (double)dd / dev_unit());
-      }
+    if (t < SHARE) {
+      k += s.share[t].x;
+      dd += (int64_t)((unsigned long long)s.share[t + SHARE].y << 32 | s.share[t + SHARE].x);
+      lead->bin_cnt[rank * SHARE + t] = k;
+      lead->bin_mass[rank * SHARE + t] = mass_of(rank * SHARE + t, k, dd);
     }
     __syncthreads();
-    rs_sync();  // the first CTA has read its own `share`, which lies where the bins' counts go
-    if (t < RS_SHARE) {
-      lead->bin_cnt[rank * RS_SHARE + t] = kk;
-      lead->bin_mass[rank * RS_SHARE + t] = mass;
-    }
     if (t == 0) { lead->beyond[rank] = s.own_beyond; lead->most[rank] = s.own_most; }
   }
 
@@ -227,18 +310,20 @@ struct RSRow {
       for (int i = tid; i < RS_BINS; i += RS_THREADS) s.dev[i] = 0;
       __syncthreads();
       fill(false, true);
-      rs_sync();
+      rs_sync<CL>();
       reduce(true);
     } else if (c.op == RS_GATHER) {
-      RSSmem* lead = cl.map_shared_rank(&s, 0);
-#pragma unroll 4
-      for (int i = tid; i < n; i += RS_THREADS) {
-        const float l = get(i);
-        const int b = rs_bin(l, g);
-        if (l == -INFINITY || b < c.b0 || b > c.b1) continue;
-        const uint32_t at = atomicAdd(&lead->n_list, 1u);
-        if (at < RS_CAP) lead->list[at] = (unsigned long long)~rs_order(l) << 32 | (uint32_t)(i0 + i);
-      }
+      RSSmem* lead = CL == 1 ? &s : cl.map_shared_rank(&s, 0);
+      const float lo = (float)c.b0, hi = c.b1 == RS_BINS ? INFINITY : (float)(c.b1 + 1);  // -infinity's place is infinity
+      each([&](int i, const float (&l)[V]) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float x = rs_place(l[j], g);
+          if (!((x >= lo && x < hi) || (hi == INFINITY && x == hi && l[j] > -INFINITY))) continue;
+          const uint32_t at = atomicAdd(&lead->n_list, 1u);
+          if (at < RS_CAP) lead->list[at] = (unsigned long long)~rs_order(l[j] + 0.f) << 32 | (uint32_t)(i0 + i + j);
+        }
+      });
     } else if (c.op == RS_RADIX) {
       uint32_t* lo = reinterpret_cast<uint32_t*>(s.dev);
       for (int i = tid; i < 256; i += RS_THREADS) s.cnt[i] = lo[i] = lo[256 + i] = 0;
@@ -275,7 +360,7 @@ struct RSRow {
       for (int i = j0; i < j1; ++i) k += get(i) != -INFINITY && rs_order(get(i)) == c.key;
       const uint32_t before = rs_scan<uint32_t>(k, s.wcnt, &all);
       if (tid == 0) s.occur = all;
-      rs_sync();
+      rs_sync<CL>();
       uint32_t first = before;
       for (int r = 0; r < (int)cl.block_rank(); ++r) first += cl.map_shared_rank(&s, r)->occur;
       if (c.skip >= first && c.skip < first + k) {
@@ -291,22 +376,23 @@ struct RSRow {
   double bin_mass[RS_PER], mass_before, all_mass;
 
   __device__ void post(const RSCommand& c) {  // to every CTA
-    if (threadIdx.x < RS_CLUSTER) cl.map_shared_rank(&s, threadIdx.x)->cmd = c;
+    if (threadIdx.x < CL) cl.map_shared_rank(&s, threadIdx.x)->cmd = c;
   }
   __device__ void command(const RSCommand& c) {
     __syncthreads();
     post(c);
     if (threadIdx.x == 0) { s.n_list = 0; s.over = 0; }
-    rs_sync();
+    rs_sync<CL>();
     serve(c);
-    rs_sync();
-    if (c.last) alone = true;
+    rs_sync<CL>();
+    if (c.last || CL == 1) alone = true;
   }
 
   // the bins that the cluster has put here, scanned
   __device__ void scan_bins() {
     uint32_t kc = 0, all;
     double mc = 0;
+    __syncthreads();
 #pragma unroll
     for (int e = 0; e < RS_PER; ++e) {
       bin_cnt[e] = s.bin_cnt[threadIdx.x * RS_PER + e];
@@ -314,14 +400,17 @@ struct RSRow {
       kc += bin_cnt[e];
       mc += bin_mass[e];
     }
-    cnt_before = rs_scan<uint32_t>(kc, s.wcnt, &all);
-    mass_before = rs_scan<double>(mc, s.wsum, &all_mass);
-    for (int r = 0; r < RS_CLUSTER; ++r) all += s.beyond[r];
+    cnt_before = kc;
+    mass_before = mc;
+    rs_scan2(cnt_before, mass_before, s, &all, &all_mass);
+#pragma unroll
+    for (int r = 0; r < CL; ++r) all += s.beyond[r];
     all_cnt = all;
   }
   __device__ uint32_t most() const {
     uint32_t m = 0;
-    for (int r = 0; r < RS_CLUSTER; ++r) m = max(m, s.most[r]);
+#pragma unroll
+    for (int r = 0; r < CL; ++r) m = max(m, s.most[r]);
     return m;
   }
   // the bins' masses once more, or at last
@@ -498,7 +587,7 @@ struct RSRow {
     // crowded: digit by digit, masses in units of the bin edge's weight
     RSCommand c{};
     c.op = RS_RADIX; c.b0 = b;
-    c.z0 = b < RS_BINS ? (double)b * (double)g.width / g.t : 0.0;
+    c.z0 = b > 0 && b < RS_BINS ? ((double)g.mx - (double)rs_edge((float)b, g)) / g.t : 0.0;
     const double unit = b < RS_BINS ? exp(-c.z0) : 0.0;
     double each = 0;   // of the tokens left: their weight
     uint32_t left = 0;
@@ -510,7 +599,7 @@ struct RSRow {
       unsigned long long m = 0;
       const int d = 255 - (int)threadIdx.x;
       if (threadIdx.x < 256)
-        for (int r = 0; r < RS_CLUSTER; ++r) {
+        for (int r = 0; r < CL; ++r) {
           const RSSmem* o = cl.map_shared_rank(&s, r);
           const uint32_t* lo = reinterpret_cast<const uint32_t*>(o->dev);
           k += o->cnt[d];
@@ -636,18 +725,18 @@ struct RSRow {
   }
 };
 
-template <class T, bool STAGED>
+template <class T, bool STAGED, int CL>
 __global__ void __launch_bounds__(RS_THREADS, 2) sample_rows_kernel(const RSArgs a) {
   extern __shared__ __align__(16) uint8_t rs_raw[];
   RSSmem& s = *reinterpret_cast<RSSmem*>(rs_raw);
   T* stage = reinterpret_cast<T*>(rs_raw + (sizeof(RSSmem) + 15) / 16 * 16);
   cg::cluster_group cl = cg::this_cluster();
-  rs_arrive();  // waited for before anything is written to another CTA: it has to be there
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cl.block_rank();
-  const int r = (int)(blockIdx.x / RS_CLUSTER);
+  rs_arrive<CL>();  // waited for before anything is written to another CTA: it has to be there
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = CL == 1 ? 0 : (int)cl.block_rank();
+  const int r = (int)(blockIdx.x / CL);
   const int i0 = min(rank * a.per, a.vocab), n = min(a.per, a.vocab - i0);
   const T* row = reinterpret_cast<const T*>(a.logits) + (int64_t)r * a.ld;
-  RSRow<T, STAGED> w{s, stage, a, row, i0, n, RSGeom{}, cl, 0.0, RS_SURE, false};
+  RSRow<T, STAGED, CL> w{s, stage, a, row, i0, n, RSGeom{}, cl, 0.0, RS_SURE, false};
 
   // 1. this CTA's logits, the largest and the smallest that is a number.  Copies of 16 bytes and more; the shares are
   // multiples of 8 logits, what is left of a row's end comes by itself.
@@ -689,16 +778,22 @@ __global__ void __launch_bounds__(RS_THREADS, 2) sample_rows_kernel(const RSArgs
     st.mn = fminf(st.mn, __shfl_xor_sync(0xffffffffu, st.mn, o));
   }
   if (lane == 0) s.wstat[warp] = st;
-  __syncthreads();
-  rs_wait();
-  if (tid < RS_CLUSTER) {
-    for (int v = 0; v < RS_WARPS; ++v) { st.mx = fmaxf(st.mx, s.wstat[v].mx); st.mn = fminf(st.mn, s.wstat[v].mn); }
-    cl.map_shared_rank(&s, tid)->stats[rank] = st;
-  }
   if (tid == 0) s.first = 0x7fffffff;
-  rs_sync();
+  __syncthreads();
+  rs_wait<CL>();
+  if (warp == 0) {
+    st = s.wstat[lane % RS_WARPS];
 #pragma unroll
-  for (int c = 0; c < RS_CLUSTER; ++c) { st.mx = fmaxf(st.mx, s.stats[c].mx); st.mn = fminf(st.mn, s.stats[c].mn); }
+    for (int o = RS_WARPS / 2; o > 0; o >>= 1) {
+      st.mx = fmaxf(st.mx, __shfl_xor_sync(0xffffffffu, st.mx, o));
+      st.mn = fminf(st.mn, __shfl_xor_sync(0xffffffffu, st.mn, o));
+    }
+    if (lane < CL) cl.map_shared_rank(&s, lane)->stats[rank] = st;
+  }
+  rs_sync<CL>();
+  st = s.stats[0];
+#pragma unroll
+  for (int c = 1; c < CL; ++c) { st.mx = fmaxf(st.mx, s.stats[c].mx); st.mn = fminf(st.mn, s.stats[c].mn); }
   st.mx += 0.f;
   if (st.mx == -INFINITY || !(t > 0.f)) {  // no token, or greedy: the first of the largest
     int at = 0x7fffffff;
@@ -707,7 +802,7 @@ __global__ void __launch_bounds__(RS_THREADS, 2) sample_rows_kernel(const RSArgs
         if (w.raw(i) == st.mx) { at = i0 + i; break; }
     at = (int)__reduce_min_sync(0xffffffffu, (unsigned)at);
     if (lane == 0 && at != 0x7fffffff) atomicMin(&cl.map_shared_rank(&s, 0)->first, at);
-    rs_sync();
+    rs_sync<CL>();
     if (rank == 0) w.answer(r, st.mx == -INFINITY ? -1 : s.first, st.mx == -INFINITY ? 0.0 : 1.0, st.mx == -INFINITY ? 0u : 1u);
     return;
   }
@@ -725,43 +820,48 @@ __global__ void __launch_bounds__(RS_THREADS, 2) sample_rows_kernel(const RSArgs
   g.width = span > 1e-30f ? span / (float)RS_BINS : 0.f;
   w.min_p = q > 0.f ? (double)q : 0.0;
   w.fill(true, masses);
-  rs_sync();
+  rs_sync<CL>();
   w.reduce(masses);
-  rs_sync();
+  rs_sync<CL>();
 
   // 3. ends of the prefixes and the token
-  if (rank == 0) {
+  if (CL == 1 || rank == 0) {
     const double up = un > 0.f ? fmin((double)un, 1.0) : 0.0;
     w.lead(r, k, p < 1.f ? (double)p : 1.0, up, masses);
     if (!w.alone) {
       __syncthreads();
       RSCommand c{};
       w.post(c);
-      rs_sync();
+      rs_sync<CL>();
     }
     return;
   }
   for (;;) {
-    rs_sync();
+    rs_sync<CL>();
     const RSCommand c = s.cmd;
     if (c.op == RS_DONE) return;
     w.serve(c);
-    rs_arrive();
+    rs_arrive<CL>();
     if (c.last) return;  // nobody reads this CTA's memory any more
-    rs_wait();
+    rs_wait<CL>();
   }
 }
 
+template <class T, bool STAGED, int CL>
+static int rs_launch_one(const RSArgs& a, int batch, size_t slice, cudaStream_t st) {
+  const size_t fixed = (sizeof(RSSmem) + 15) / 16 * 16;
+  if (int rc = smem_attr_once<sample_rows_kernel<T, STAGED, CL>>((int)(fixed + (STAGED ? RS_STAGE_MAX : 0)))) return rc;
+  return kv8_launch_cluster(sample_rows_kernel<T, STAGED, CL>, dim3((unsigned)batch * CL), CL, dim3(RS_THREADS), fixed + slice, st,
+                            false, a);
+}
 template <class T>
-static int rs_launch(const RSArgs& a, int batch, cudaStream_t st) {
-  const size_t fixed = (sizeof(RSSmem) + 15) / 16 * 16, slice = (size_t)a.per * sizeof(T);
-  const dim3 grid((unsigned)batch * RS_CLUSTER), block(RS_THREADS);
-  if (slice <= RS_STAGE_MAX) {
-    if (int rc = smem_attr_once<sample_rows_kernel<T, true>>((int)(fixed + RS_STAGE_MAX))) return rc;
-    return kv8_launch_cluster(sample_rows_kernel<T, true>, grid, RS_CLUSTER, block, fixed + slice, st, false, a);
-  }
-  if (int rc = smem_attr_once<sample_rows_kernel<T, false>>((int)fixed)) return rc;
-  return kv8_launch_cluster(sample_rows_kernel<T, false>, grid, RS_CLUSTER, block, fixed, st, false, a);
+static int rs_launch(RSArgs& a, int batch, cudaStream_t st) {
+  const int cl = a.vocab <= RS_ALONE ? 1 : RS_CLUSTER;
+  a.per = ((a.vocab + cl - 1) / cl + 7) / 8 * 8;
+  const size_t slice = (size_t)a.per * sizeof(T);
+  if (cl == 1) return rs_launch_one<T, true, 1>(a, batch, slice, st);
+  if (slice <= RS_STAGE_MAX) return rs_launch_one<T, true, RS_CLUSTER>(a, batch, slice, st);
+  return rs_launch_one<T, false, RS_CLUSTER>(a, batch, 0, st);
 }
 
 }  // namespace n730
@@ -782,7 +882,6 @@ N730_API int n730_sample_rows(const void* d_logits, int dtype, int batch, int vo
                N730_BAD_ARG, "%s: pointers must lie on whole elements", what);
   RSArgs a{};
   a.logits = d_logits; a.ld = ld; a.vocab = vocab;
-  a.per = ((vocab + RS_CLUSTER - 1) / RS_CLUSTER + 7) / 8 * 8;
   a.vec = ((uintptr_t)d_logits & 15) == 0 && ld * es % 16 == 0;
   a.temperature = d_temperature; a.top_k = d_top_k; a.top_p = d_top_p; a.min_p = d_min_p; a.u = d_u;
   a.tokens = d_tokens; a.prob = d_prob; a.kept = d_kept;
