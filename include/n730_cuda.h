@@ -149,7 +149,7 @@ int n730_qgemm(void* qw, const float* d_x, int ldx, int tokens, float* d_y, int 
 int n730_sample(const float* d_logits, int batch, int vocab, int ld, float temperature, float top_p,
                 uint64_t seed, uint64_t counter, int32_t* d_tokens, float* d_u, void* stream);
 /* Sampling with each row's own settings and given random numbers: for each of `batch` rows of d_logits
- * (type N730_F32 / F16 / BF16, row stride ld >= vocab, up to 2^24 of each), d_temperature <= 0 gives the first
+ * (type N730_F32 / F16 / BF16, row stride ld >= vocab; up to 2^24 rows of up to 2^23), d_temperature <= 0 gives the first
  * index of the largest logit; otherwise tokens are ordered by logit (ties by index) with weights
  * w = exp((logit - largest) / temperature), and kept are the first d_top_k of them (<= 0: all), of those the
  * shortest prefix whose mass reaches d_top_p times theirs (>= 1 or NaN: all), and of those the ones with

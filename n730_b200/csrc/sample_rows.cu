@@ -7,19 +7,22 @@
 //   mass exceeds u times the kept mass.
 //
 // A cluster of 8 CTAs takes a row: each copies an eighth of the logits into its shared memory, so that HBM is read once
-// and whatever follows runs on the chip.
-//   1. largest and smallest logit;
-//   2. a histogram over RS_BINS linear bins of max - l: how many tokens, and, where the mass of all tokens matters (no
-//      top-k, or a large one), the sum of w / w(bin's edge) - 1 in fixed point.  Bins are narrow, so that this is small
-//      and fp32 holds it to 2^-24 of w or so; a bin's mass is w(edge) * (count + sum), formed in 64 bits.  Both sums are
-//      integers: the order of the atomics does not matter.  Each CTA adds up an eighth of the bins over the cluster and
-//      puts them where the first CTA scans them;
-//   3. where the bins up to the last one that a kept token can lie in hold at most RS_CAP tokens, these are gathered in
-//      the first CTA's shared memory and sorted, and the rest is a scan over them with weights in 64 bits; the other
-//      CTAs are gone by then.  Where not (flat rows without a top-k), each prefix's end is looked up in its bin by itself:
-//      the bin's tokens are gathered and sorted, or, where they are too many (equal logits, coarse types), found by four
-//      rounds of 8 bits of the logit, after which the tokens left are equal and go by index.
-// All sums are 64-bit floats in a fixed order or integers: the same inputs give the same token.
+// and whatever follows runs on the chip.  (Rows of up to RS_ALONE logits take one CTA.)  The first CTA leads; the others
+// serve its commands, and all meet around each.
+//   1. largest and smallest logit, and each thread's largest.
+//   2. A list: tokens are gathered in the first CTA's shared memory and sorted, the rest is a scan over it with weights in
+//      64 bits.  With min-p and no top-p they are those of weight >= q; with a top-k those up to the bin (of RS_BINS
+//      linear ones of max - l) that k of the threads' largest reach, 4096 of a long row: the first k tokens all lie up to
+//      there, and seldom many more.
+//   3. Rows of neither kind, or whose list is too long: a histogram of all tokens and their masses.  A bin's mass is
+//      w(edge) * sum of w / w(edge), the sum in fixed point; bins are narrow, so w / w(edge) is near 1 and fp32 holds its
+//      distance from 1 to 2^-24 of that.  Shared-memory atomics bound this pass, 10 cycles a warp's worth.  Flat rows take
+//      one, the distances beside the count in a word; where that is too coarse (rows that a few tokens have much of,
+//      crowded or wide bins), or likely to be (rows with a top-p), 43 bits of sum below 21 of count in two words.
+//      Each prefix's end is then looked up in its bin: the bin's tokens are gathered and sorted, or, where they are too
+//      many (equal logits, coarse types), found by four rounds of 8 bits of the logit, after which the tokens left are
+//      equal and go by index.
+// Sums are integers, or 64-bit floats in a fixed order: the same inputs give the same token.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -31,14 +34,15 @@ namespace cg = cooperative_groups;
 
 constexpr int RS_CLUSTER = 8;      // CTAs of a row, one for rows of up to RS_ALONE logits: no exchange, 15 -> 10 us at 1000
 constexpr int RS_ALONE = 16384;
-constexpr int RS_THREADS = 512;
-constexpr int RS_WARPS = RS_THREADS / 32;
+// Threads of a CTA: 512 and all of an SM's registers while a row's CTAs find an SM each (one row of 152064: 12.8 us, 13.5
+// with 256), 256 and two CTAs an SM beyond that (64 rows with a top-k: 30 us, 60 with 512).
+constexpr int RS_THREADS_FEW = 512, RS_THREADS_MANY = 256;
+constexpr int RS_WARPS = RS_THREADS_FEW / 32;  // most warps
 constexpr int RS_BINS = 1536;      // as many as leave room for two CTAs of 19008 fp32 logits (a row of 152064) an SM
-constexpr int RS_PER = RS_BINS / RS_THREADS;
 constexpr int RS_CAP = 1024;       // tokens that are sorted at once
-constexpr int RS_EACH = RS_CAP / RS_THREADS;
 constexpr int RS_COUNT = 160;      // lists up to this long are sorted by counting
-constexpr int RS_SURE = 2048;      // tokens of a CTA's bin that the fixed point of the bins' masses has room for at first
+constexpr uint32_t RS_ROOM1 = 256, RS_ROOM2 = 4095;  // tokens of a CTA's bin that one word, and two, have room for
+constexpr uint32_t RS_FLAT = 65536;  // tokens from which a row is tried with one word: two cost shorter ones little
 constexpr float RS_SPAN = 32.f;    // bins reach this many logits, or temperatures where that is more, below the largest
 constexpr size_t RS_STAGE_MAX = 160 * 1024;  // longest slice that is kept in shared memory
 
@@ -51,33 +55,42 @@ struct RSArgs {
   int* tokens; float* prob; int* kept;
 };
 
-enum { RS_DONE = 0, RS_MASSES, RS_GATHER, RS_RADIX, RS_OVER, RS_FIND };
+// what the bins hold: nothing, threads' largest, all tokens, all tokens and their masses in one word or two
+enum { RS_NONE = 0, RS_LARGEST, RS_COUNTS, RS_ONE_WORD, RS_TWO_WORDS };
+enum { RS_DONE = 0, RS_FILL, RS_GATHER, RS_RADIX, RS_OVER, RS_FIND };
 struct RSCommand {
   int op, b0, b1;         // bins [b0, b1]
   int last;               // GATHER: nothing follows for the other CTAs
+  int mode, sure;         // FILL: what, tokens of a CTA's bin to have room for
   uint32_t prefix, shift; // RADIX: digits found, where the next one starts
   uint32_t key, skip;     // FIND: the skip-th token of this key
-  int sure;               // MASSES: tokens of a CTA's bin to have room for
   double z0;              // RADIX: the bin's edge / T
 };
-struct RSStat { float mx, mn; };
+struct RSStat { float mx, mn; uint32_t n; };  // n: tokens
 
+// What the first CTA knows of its row between two commands.
+struct RSLead {
+  int state, mode, purpose, b, round;
+  uint32_t cut, kept, before, left, prefix;
+  bool cut_k, by_mass, strict;
+  double top_p, u, over, mass, target, base, in_mass, unit, each;  // over: place of weight min-p
+};
 struct RSSmem {
   uint32_t cnt[RS_BINS];             // by bin; also the counts of 256 digits
-  int32_t dev[RS_BINS];              // sums of w / w(edge) - 1; also the digits' masses, low and high words
-  uint2 share[2 * RS_BINS / RS_CLUSTER];
+  uint32_t low[RS_BINS];             // the second word; also the digits' masses, low and high words
   union { unsigned long long list[RS_CAP]; uint32_t bin_cnt[RS_BINS]; };  // list: ~order << 32 | index
-  union { double cum[RS_CAP]; double bin_mass[RS_BINS]; };
+  union { double cum[RS_CAP]; double bin_mass[RS_BINS]; unsigned long long mine[RS_CAP]; };
   RSCommand cmd;
+  RSLead lead;
   RSStat stats[RS_CLUSTER];
   RSStat wstat[RS_WARPS];
   double wsum[RS_WARPS];
   uint32_t wcnt[RS_WARPS];
-  uint32_t beyond[RS_CLUSTER], most[RS_CLUSTER];  // tokens behind the last bin; of the fullest bin of a share
+  uint32_t beyond[RS_CLUSTER], most[RS_CLUSTER];  // tokens behind the last bin; of a share's fullest bin, where it has no room
   uint32_t own_beyond, own_most;
   double sel_base, sel_mass, pick_w;
-  uint32_t n_list, over, sel_cnt, sel_in, pick_cnt, occur;
-  int bin_k, bin_p, bin_last, pick, found, first;
+  uint32_t n_list, n_mine, list_at, over, sel_cnt, sel_in, pick_cnt, occur;
+  int bin_k, bin_p, pick, found, first;
 };
 
 // a row's CTAs meet
@@ -124,6 +137,7 @@ __device__ __forceinline__ double rs_weight(float l, const RSGeom& g) {
 }
 
 // Exclusive scans over the block in thread order; the totals.
+template <int TH>
 __device__ __forceinline__ void rs_scan2(uint32_t& k, double& m, RSSmem& s, uint32_t* all_k, double* all_m) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t ik = k;
@@ -140,7 +154,7 @@ __device__ __forceinline__ void rs_scan2(uint32_t& k, double& m, RSSmem& s, uint
   uint32_t bk = 0, tk = 0;
   double bm = 0, tm = 0;
 #pragma unroll
-  for (int w = 0; w < RS_WARPS; ++w) {
+  for (int w = 0; w < (TH / 32); ++w) {
     const uint32_t xk = s.wcnt[w];
     const double xm = s.wsum[w];
     if (w < warp) { bk += xk; bm += xm; }
@@ -151,7 +165,7 @@ __device__ __forceinline__ void rs_scan2(uint32_t& k, double& m, RSSmem& s, uint
   m = bm + im - m;
 }
 // Exclusive scan over the block in thread order; *total the sum.
-template <class V>
+template <int TH, class V>
 __device__ V rs_scan(V v, V* warps, V* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   V inc = v;
@@ -165,7 +179,7 @@ __device__ V rs_scan(V v, V* warps, V* total) {
   __syncthreads();
   V before = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < RS_WARPS; ++w) {
+  for (int w = 0; w < (TH / 32); ++w) {
     const V x = warps[w];
     if (w < warp) before += x;
     all += x;
@@ -174,8 +188,9 @@ __device__ V rs_scan(V v, V* warps, V* total) {
   return before + inc - v;
 }
 
-template <class T, bool STAGED, int CL>
+template <class T, bool STAGED, int CL, int TH>
 struct RSRow {
+  static constexpr int RS_PER = RS_BINS / TH, RS_EACH = RS_CAP / TH;
   static constexpr int V = 16 / sizeof(T), SHARE = RS_BINS / CL;
   RSSmem& s;
   T* stage;              // this CTA's logits
@@ -185,15 +200,15 @@ struct RSRow {
   RSGeom g;
   cg::cluster_group cl;
   double min_p;
-  int sure;              // tokens of a CTA's bin that the masses have room for
-  bool alone;            // the other CTAs are gone
+  uint32_t all_cnt;      // the row's tokens
+  int sure;              // tokens of a CTA's bin that two words are to have room for
 
   __device__ float raw(int i) const { return rs_float(STAGED ? stage[i] : row[i0 + i]); }
   __device__ float get(int i) const { return rs_clean(raw(i)); }
   // f(first index, V logits) over this CTA's, V = 16 bytes of them, NaN behind the last.
   template <class F>
   __device__ __forceinline__ void each(F f) const {
-    for (int i = threadIdx.x * V; i < n; i += RS_THREADS * V) {
+    for (int i = threadIdx.x * V; i < n; i += TH * V) {
       float l[V];
       if (STAGED) {
         const uint4 x = *reinterpret_cast<const uint4*>(stage + i);
@@ -212,15 +227,19 @@ struct RSRow {
     }
   }
 
-  // Fixed-point unit of the deviations: a CTA's sum of a bin with up to `sure` tokens stays inside 31 bits.
-  __device__ float dev_unit() const {
-    const float most = fmaxf(1.f - expf(-g.width * g.inv_t * 1.01f), 0x1p-20f) * (float)sure;
-    return ldexpf(1.f, (int)floorf(29.f - log2f(most)));
+  // Units of a weight over its bin edge's: one word has 22 bits for RS_ROOM1 distances from 1, two have 43 for `sure`
+  // weights.
+  __device__ float unit_of(int mode) const {
+    if (mode == RS_ONE_WORD) return ldexpf(1.f, (int)floorf(14.f - log2f(fmaxf(expm1f(g.width * g.inv_t * 1.01f), 0x1p-20f))));
+    return ldexpf(1.f, 31 - (32 - __clz(sure / 4096)));
   }
-  // Sums of w / w(edge) - 1 by bin; with `count`, the bins' tokens as well.
-  __device__ void fill(bool count, bool masses) {
-    const float unit = dev_unit();
-    const bool narrow = g.width * g.inv_t < 0x1p-6f;
+  __device__ bool one_word() const { return g.mx < INFINITY && g.width * g.inv_t < 0x1p-4f; }
+
+  // Counts and sums of w / w(edge) by bin; in one word from the lower edge, so that the distance from 1 is not negative.
+  template <int MODE>
+  __device__ __forceinline__ void fill() {
+    const float unit = unit_of(MODE), down = MODE == RS_ONE_WORD ? 1.f : 0.f;
+    const bool narrow = MODE == RS_ONE_WORD || one_word();
     uint32_t beyond = 0;
     each([&](int, const float (&l)[V]) {
       int b[V], c[V];
@@ -230,105 +249,140 @@ struct RSRow {
         const bool in = x < (float)RS_BINS;
         beyond += !in && l[j] > -INFINITY;
         b[j] = in ? __float_as_int(f) & 0x7fffff : -1;
-        if (masses) {
-          // y = (l - edge) / T: the two are near, their difference is exact but for what is below 2^-24 of a bin
-          const float y = l[j] == g.mx ? 0.f : (l[j] - rs_edge(f - 8388608.f, g)) * g.inv_t;
-          const float e = narrow ? y * fmaf(y, fmaf(y, fmaf(y, 1.f / 24, 1.f / 6), 0.5f), 1.f) : expm1f(y);
-          c[j] = __float_as_int(fmaf(e, unit, 12582912.f)) - 0x4b400000;  // to the nearest whole number, below 2^22
-        }
+        if (MODE == RS_COUNTS) continue;
+        // y = (l - edge) / T: the two are near, their difference is exact but for what is below 2^-24 of a bin
+        float y = (l[j] - rs_edge(f - 8388608.f + down, g)) * g.inv_t;
+        if (MODE == RS_ONE_WORD) y = fmaxf(y, 0.f);
+        else y = l[j] == g.mx ? 0.f : fminf(y, 0.f);
+        const float e = narrow ? y * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 1.f / 120, 1.f / 24), 1.f / 6), 0.5f), 1.f) : expm1f(y);
+        if (MODE == RS_ONE_WORD) c[j] = __float_as_int(fmaf(e, unit, 12582912.f)) - 0x4b400000;  // nearest, below 2^22
+        else c[j] = (int)((uint32_t)__float2int_rn(e * unit) + (uint32_t)unit);
       }
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (b[j] >= 0) {
-          if (count) atomicAdd(&s.cnt[b[j]], 1u);
-          if (masses) atomicAdd(&s.dev[b[j]], c[j]);
+      for (int j = 0; j < V; ++j) {
+        if (b[j] < 0) continue;
+        if (MODE == RS_COUNTS) {
+          atomicAdd(&s.cnt[b[j]], 1u);
+        } else if (MODE == RS_ONE_WORD) {
+          atomicAdd(&s.cnt[b[j]], (uint32_t)c[j] + (1u << 22));
+        } else {
+          const uint32_t old = atomicAdd(&s.low[b[j]], (uint32_t)c[j]);
+          atomicAdd(&s.cnt[b[j]], (1u << 11) + (old + (uint32_t)c[j] < old));
         }
+      }
     });
-    if (count && beyond) atomicAdd(&s.own_beyond, beyond);
+    if (beyond) atomicAdd(&s.own_beyond, beyond);
   }
   // This CTA's share of the bins, added up over the cluster, to the first CTA.  The cluster has filled before.
-  __device__ void reduce(bool masses) {
-    const float unit = dev_unit();
-    auto mass_of = [&](int b, uint32_t k, int64_t d) {
-      return masses && k ? rs_weight(rs_edge((float)b, g), g) * ((double)k + (double)d / unit) : 0.0;
+  __device__ __forceinline__ void reduce(int mode) {
+    const float unit = unit_of(mode);
+    const bool one = mode == RS_ONE_WORD, two = mode == RS_TWO_WORDS;
+    auto mass_of = [&](int b, uint32_t k, unsigned long long m) {
+      return k && (one || two) ? rs_weight(rs_edge((float)(b + one), g), g) * ((one ? (double)k : 0.0) + (double)m / unit) : 0.0;
     };
+    auto tokens = [&](uint32_t x) { return one ? x >> 22 : two ? x >> 11 : x; };
+    auto sum = [&](const RSSmem* o, int b, uint32_t x) {
+      return one ? (unsigned long long)(x & 0x3fffffu) : two ? (unsigned long long)(x & 2047u) << 32 | o->low[b] : 0ull;
+    };
+    const uint32_t room = one ? RS_ROOM1 : two ? max((uint32_t)sure, RS_ROOM2) : 0xffffffffu;
     if (CL == 1) {
       uint32_t most = 0;
-      for (int b = threadIdx.x; b < RS_BINS; b += RS_THREADS) {
-        const uint32_t k = s.cnt[b];
+      for (int b = threadIdx.x; b < RS_BINS; b += TH) {
+        const uint32_t x = s.cnt[b], k = tokens(x);
         most = max(most, k);
         s.bin_cnt[b] = k;
-        s.bin_mass[b] = mass_of(b, k, s.dev[b]);
+        s.bin_mass[b] = mass_of(b, k, sum(&s, b, x));
       }
       if (threadIdx.x == 0) s.own_most = 0;
       __syncthreads();
-      if (most > RS_SURE) atomicMax(&s.own_most, most);
+      if (most > room) atomicMax(&s.own_most, most);
       __syncthreads();
       if (threadIdx.x == 0) { s.beyond[0] = s.own_beyond; s.most[0] = s.own_most; }
       return;
     }
     const int t = threadIdx.x, rank = (int)cl.block_rank();
     uint32_t k = 0, most = 0;
-    int d[CL] = {};
-    if (t < 2 * SHARE) {  // two threads a bin, half of the CTAs each
-      const int b = rank * SHARE + t % SHARE, r0 = t / SHARE * (CL / 2);
+    unsigned long long m = 0;
+    if (t < SHARE) {
 #pragma unroll
-      for (int r = 0; r < CL / 2; ++r) {
-        const RSSmem* o = cl.map_shared_rank(&s, r0 + r);
-        const uint32_t x = o->cnt[b];
-        k += x;
-        most = max(most, x);
-        if (masses) d[r] = o->dev[b];
+      for (int r = 0; r < CL; ++r) {
+        const RSSmem* o = cl.map_shared_rank(&s, r);
+        const uint32_t x = o->cnt[rank * SHARE + t];
+        k += tokens(x);
+        most = max(most, tokens(x));
+        m += sum(o, rank * SHARE + t, x);
       }
-    }
-    int64_t dd = 0;
-#pragma unroll
-    for (int r = 0; r < CL / 2; ++r) dd += d[r];
-    if (t >= SHARE && t < 2 * SHARE) {  // deviations in two words
-      s.share[t] = make_uint2((uint32_t)dd, (uint32_t)(dd >> 32));
-      s.share[t - SHARE].x = k;
     }
     if (t == 0) s.own_most = 0;
     __syncthreads();
     RSSmem* lead = cl.map_shared_rank(&s, 0);
-    if (most > RS_SURE) atomicMax(&s.own_most, most);
+    if (most > room) atomicMax(&s.own_most, most);
     if (t < SHARE) {
-      k += s.share[t].x;
-      dd += (int64_t)((unsigned long long)s.share[t + SHARE].y << 32 | s.share[t + SHARE].x);
       lead->bin_cnt[rank * SHARE + t] = k;
-      lead->bin_mass[rank * SHARE + t] = mass_of(rank * SHARE + t, k, dd);
+      lead->bin_mass[rank * SHARE + t] = mass_of(rank * SHARE + t, k, m);
     }
     __syncthreads();
     if (t == 0) { lead->beyond[rank] = s.own_beyond; lead->most[rank] = s.own_most; }
   }
+  // The bins of all CTAs' tokens, or of their threads' largest.
+  __device__ __forceinline__ void histogram(int mode, float largest) {
+    if (mode == RS_ONE_WORD) {
+      fill<RS_ONE_WORD>();
+    } else if (mode == RS_TWO_WORDS) {
+      fill<RS_TWO_WORDS>();
+    } else if (mode == RS_COUNTS) {
+      fill<RS_COUNTS>();
+    } else if (largest > -INFINITY) {
+      const int b = rs_bin(largest, g);
+      atomicAdd(b < RS_BINS ? &s.cnt[b] : &s.own_beyond, 1u);
+    }
+    rs_sync<CL>();
+    reduce(mode);
+  }
 
   // A CTA's share of a command.
-  __device__ void serve(const RSCommand& c) {
+  __device__ __forceinline__ void serve(const RSCommand& c, float of_thread) {
     const int tid = threadIdx.x;
-    if (c.op == RS_MASSES) {
+    if (c.op == RS_FILL) {
       sure = c.sure;
-      for (int i = tid; i < RS_BINS; i += RS_THREADS) s.dev[i] = 0;
+      for (int i = tid; i < RS_BINS; i += TH) s.cnt[i] = s.low[i] = 0;
+      if (tid == 0) s.own_beyond = 0;
       __syncthreads();
-      fill(false, true);
-      rs_sync<CL>();
-      reduce(true);
+      histogram(c.mode, of_thread);
     } else if (c.op == RS_GATHER) {
-      RSSmem* lead = CL == 1 ? &s : cl.map_shared_rank(&s, 0);
+      // into this CTA's own shared memory first: a place in the first CTA's list takes a trip there
       const float lo = (float)c.b0, hi = c.b1 == RS_BINS ? INFINITY : (float)(c.b1 + 1);  // -infinity's place is infinity
+      // nothing below this is wanted
+      const float least = c.b1 == RS_BINS || g.sx == 0.f ? -INFINITY : rs_edge((float)(c.b1 + 2), g);
+      const float largest = c.b0 < 2 || g.sx == 0.f ? INFINITY : rs_edge((float)(c.b0 - 1), g);  // or above this
+      if (tid == 0) s.n_mine = 0;
+      __syncthreads();
       each([&](int i, const float (&l)[V]) {
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < V; ++j) any = any || (l[j] >= least && l[j] <= largest);
+        if (!any) return;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
+          if (!(l[j] >= least && l[j] <= largest)) continue;
           const float x = rs_place(l[j], g);
           if (!((x >= lo && x < hi) || (hi == INFINITY && x == hi && l[j] > -INFINITY))) continue;
-          const uint32_t at = atomicAdd(&lead->n_list, 1u);
-          if (at < RS_CAP) lead->list[at] = (unsigned long long)~rs_order(l[j] + 0.f) << 32 | (uint32_t)(i0 + i + j);
+          const uint32_t at = atomicAdd(&s.n_mine, 1u);
+          if (at < RS_CAP) s.mine[at] = (unsigned long long)~rs_order(l[j] + 0.f) << 32 | (uint32_t)(i0 + i + j);
         }
       });
-    } else if (c.op == RS_RADIX) {
-      uint32_t* lo = reinterpret_cast<uint32_t*>(s.dev);
-      for (int i = tid; i < 256; i += RS_THREADS) s.cnt[i] = lo[i] = lo[256 + i] = 0;
       __syncthreads();
-      for (int i = tid; i < n; i += RS_THREADS) {
+      RSSmem* lead = cl.map_shared_rank(&s, 0);
+      const uint32_t k = s.n_mine;
+      if (tid == 0 && k) s.list_at = atomicAdd(&lead->n_list, k);
+      __syncthreads();
+      for (uint32_t i = tid; i < min(k, (uint32_t)RS_CAP); i += TH)
+        if (s.list_at + i < RS_CAP) lead->list[s.list_at + i] = s.mine[i];
+    } else if (c.op == RS_RADIX) {
+      uint32_t* lo = s.low;
+      for (int i = tid; i < 256; i += TH) s.cnt[i] = lo[i] = lo[256 + i] = 0;
+      __syncthreads();
+      for (int i = tid; i < n; i += TH) {
         const float l = get(i);
         if (l == -INFINITY || rs_bin(l, g) != c.b0) continue;
         const uint32_t o = rs_order(l);
@@ -344,21 +398,21 @@ struct RSRow {
       }
     } else if (c.op == RS_OVER) {  // tokens of weight >= min-p; bins below b0 are sure to have it
       uint32_t k = 0;
-      for (int i = tid; i < n; i += RS_THREADS) {
+      for (int i = tid; i < n; i += TH) {
         const float l = get(i);
         if (l == -INFINITY) continue;
         const int b = rs_bin(l, g);
         k += b < c.b0 || (b <= c.b1 && rs_weight(l, g) >= min_p);
       }
       uint32_t all;
-      rs_scan<uint32_t>(k, s.wcnt, &all);
+      rs_scan<TH, uint32_t>(k, s.wcnt, &all);
       if (tid == 0) atomicAdd(&cl.map_shared_rank(&s, 0)->over, all);
     } else if (c.op == RS_FIND) {
       // tokens of the key in this CTA, then its place among the CTAs', then in thread order (contiguous runs)
-      const int run = (n + RS_THREADS - 1) / RS_THREADS, j0 = min(n, tid * run), j1 = min(n, j0 + run);
+      const int run = (n + TH - 1) / TH, j0 = min(n, tid * run), j1 = min(n, j0 + run);
       uint32_t k = 0, all;
       for (int i = j0; i < j1; ++i) k += get(i) != -INFINITY && rs_order(get(i)) == c.key;
-      const uint32_t before = rs_scan<uint32_t>(k, s.wcnt, &all);
+      const uint32_t before = rs_scan<TH, uint32_t>(k, s.wcnt, &all);
       if (tid == 0) s.occur = all;
       rs_sync<CL>();
       uint32_t first = before;
@@ -372,24 +426,16 @@ struct RSRow {
   }
 
   // ---- the first CTA's side ----
-  uint32_t bin_cnt[RS_PER], cnt_before, all_cnt;   // this thread's bins: tokens, tokens of all bins before; of the row
+  uint32_t bin_cnt[RS_PER], cnt_before;   // this thread's bins: tokens, tokens of all bins before
   double bin_mass[RS_PER], mass_before, all_mass;
 
-  __device__ void post(const RSCommand& c) {  // to every CTA
-    if (threadIdx.x < CL) cl.map_shared_rank(&s, threadIdx.x)->cmd = c;
-  }
-  __device__ void command(const RSCommand& c) {
+  __device__ __forceinline__ void post(const RSCommand& c) {  // to every CTA
     __syncthreads();
-    post(c);
+    if (threadIdx.x < CL) cl.map_shared_rank(&s, threadIdx.x)->cmd = c;
     if (threadIdx.x == 0) { s.n_list = 0; s.over = 0; }
-    rs_sync<CL>();
-    serve(c);
-    rs_sync<CL>();
-    if (c.last || CL == 1) alone = true;
   }
-
-  // the bins that the cluster has put here, scanned
-  __device__ void scan_bins() {
+  // the bins that the cluster has put here, scanned; how many there are of what they count
+  __device__ uint32_t scan_bins() {
     uint32_t kc = 0, all;
     double mc = 0;
     __syncthreads();
@@ -402,23 +448,27 @@ struct RSRow {
     }
     cnt_before = kc;
     mass_before = mc;
-    rs_scan2(cnt_before, mass_before, s, &all, &all_mass);
+    rs_scan2<TH>(cnt_before, mass_before, s, &all, &all_mass);
 #pragma unroll
     for (int r = 0; r < CL; ++r) all += s.beyond[r];
-    all_cnt = all;
+    return all;
   }
-  __device__ uint32_t most() const {
+  // whether a bin has more tokens than its words have room for
+  __device__ bool crowded() const {
     uint32_t m = 0;
 #pragma unroll
-    for (int r = 0; r < CL; ++r) m = max(m, s.most[r]);
+    for (int r = 0; r < CL; ++r) m |= s.most[r];
     return m;
   }
-  // the bins' masses once more, or at last
-  __device__ void recollect(int room) {
-    RSCommand c{};
-    c.op = RS_MASSES; c.sure = room;
-    command(c);
-    scan_bins();
+  // Whether one word a bin holds the masses well enough.  Its rounding, 0.3 units a token, moves a border by that
+  // times sqrt(sum w^2); all borders together may take 2^-12 of the mass.
+  __device__ bool fine(uint32_t counted) {
+    double w2 = 0, all;
+#pragma unroll
+    for (int e = 0; e < RS_PER; ++e) w2 += bin_cnt[e] ? bin_mass[e] * (bin_mass[e] / bin_cnt[e]) : 0.0;
+    rs_scan<TH, double>(w2, s.wsum, &all);
+    const double off = 0.3 / unit_of(RS_ONE_WORD) * sqrt(all) / all_mass;
+    return counted == all_cnt && !crowded() && 2 * off * all_cnt < 0x1p-12;
   }
 
   // First bin at which the running count or mass reaches the target (strict: exceeds it); when none does, RS_BINS by
@@ -488,40 +538,61 @@ struct RSRow {
       __syncthreads();
       return;
     }
-    // two neighbours a thread: steps of up to 32 stay in a warp
+    // two pairs of neighbours a thread: steps of up to 32 stay in a warp
     int np2 = 256;
     while (np2 < n_list) np2 <<= 1;
-    for (int i = n_list + t; i < np2; i += RS_THREADS) s.list[i] = ~0ull;
+    for (int i = n_list + t; i < np2; i += TH) s.list[i] = ~0ull;
     __syncthreads();
-    unsigned long long x = ~0ull, y = ~0ull;
-    const bool mine = 2 * t < np2;
-    if (mine) { x = s.list[2 * t]; y = s.list[2 * t + 1]; }
+    unsigned long long x[2], y[2];
+    auto load = [&] {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int q = t + e * TH;
+        x[e] = y[e] = ~0ull;
+        if (2 * q < np2) { x[e] = s.list[2 * q]; y[e] = s.list[2 * q + 1]; }
+      }
+    };
+    auto store = [&] {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int q = t + e * TH;
+        if (2 * q < np2) { s.list[2 * q] = x[e]; s.list[2 * q + 1] = y[e]; }
+      }
+    };
+    load();
     for (int size = 2; size <= np2; size <<= 1) {
-      const bool up = ((2 * t) & size) == 0;
       int step = size >> 1;
       if (step > 32) {
-        if (mine) { s.list[2 * t] = x; s.list[2 * t + 1] = y; }
+        store();
         __syncthreads();
         for (; step > 32; step >>= 1) {
-          for (int i = t; i < np2 / 2; i += RS_THREADS) {
+          for (int i = t; i < np2 / 2; i += TH) {
             const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
             const unsigned long long p = s.list[lo], q = s.list[hi];
             if ((p > q) == ((lo & size) == 0)) { s.list[lo] = q; s.list[hi] = p; }
           }
           __syncthreads();
         }
-        if (mine) { x = s.list[2 * t]; y = s.list[2 * t + 1]; }
+        load();
       }
       for (; step > 1; step >>= 1) {
         const int o = step >> 1;  // threads between the two
-        const unsigned long long px = __shfl_xor_sync(0xffffffffu, x, o), py = __shfl_xor_sync(0xffffffffu, y, o);
-        const bool keep_small = ((t & o) == 0) == up;
-        x = (px < x) == keep_small ? px : x;
-        y = (py < y) == keep_small ? py : y;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const bool up = ((2 * (t + e * TH)) & size) == 0;
+          const unsigned long long px = __shfl_xor_sync(0xffffffffu, x[e], o), py = __shfl_xor_sync(0xffffffffu, y[e], o);
+          const bool keep_small = ((t & o) == 0) == up;
+          x[e] = (px < x[e]) == keep_small ? px : x[e];
+          y[e] = (py < y[e]) == keep_small ? py : y[e];
+        }
       }
-      if ((x > y) == up) { const unsigned long long z = x; x = y; y = z; }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const bool up = ((2 * (t + e * TH)) & size) == 0;
+        if ((x[e] > y[e]) == up) { const unsigned long long z = x[e]; x[e] = y[e]; y[e] = z; }
+      }
     }
-    if (mine) { s.list[2 * t] = x; s.list[2 * t + 1] = y; }
+    store();
     __syncthreads();
   }
   __device__ float list_logit(int i) const { return rs_unorder(~(uint32_t)(s.list[i] >> 32)); }
@@ -535,7 +606,7 @@ struct RSRow {
       w[e] = i < n_list ? rs_weight(list_logit(i), g) : 0.0;
       loc += w[e];
     }
-    double m = base + rs_scan<double>(loc, s.wsum, &total);
+    double m = base + rs_scan<TH, double>(loc, s.wsum, &total);
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
       const int i = threadIdx.x * EACH + e;
@@ -545,7 +616,7 @@ struct RSRow {
     __syncthreads();
   }
   __device__ void list_masses(int n_list, double base) {
-    if (n_list <= RS_THREADS) list_masses_of<1>(n_list, base);
+    if (n_list <= TH) list_masses_of<1>(n_list, base);
     else list_masses_of<RS_EACH>(n_list, base);
   }
   // how many of the list's first n tokens lie before the target: mass below it (strict: not above it)
@@ -553,94 +624,11 @@ struct RSRow {
     int c = 0;
 #pragma unroll
     for (int e = 0; e < RS_EACH; ++e) {
-      const int i = threadIdx.x + e * RS_THREADS;
-      if (e && n_list <= e * RS_THREADS) break;
+      const int i = threadIdx.x + e * TH;
+      if (e && n_list <= e * TH) break;
       c += __syncthreads_count(i < n_list && (strict ? s.cum[i] <= target : s.cum[i] < target));
     }
     return c;
-  }
-
-  // The first token in order at which the running count or mass reaches the target (strict: exceeds it): its index, its
-  // weight, and the count and mass up to and with it.
-  struct Pick { int idx; double w; uint32_t cnt; double mass; };
-  __device__ Pick select(bool by_mass, double target, bool strict, bool last) {
-    const int b = cross_one(by_mass, target, strict);
-    uint32_t before, in;
-    double base, in_mass;
-    at_bin(b, &before, &base, &in, &in_mass);
-    Pick p;
-    if (in <= RS_CAP) {
-      RSCommand c{};
-      c.op = RS_GATHER; c.b0 = c.b1 = b; c.last = last;
-      command(c);
-      const int n_list = (int)s.n_list;
-      sort(n_list);
-      list_masses(n_list, base);
-      const int i = min(max(by_mass ? list_before(n_list, target, strict) : (int)(target - before) - 1, 0), n_list - 1);
-      p.mass = s.cum[i];
-      p.idx = (int)(uint32_t)s.list[i];
-      p.w = rs_weight(list_logit(i), g);
-      p.cnt = before + i + 1;
-      __syncthreads();
-      return p;
-    }
-    // crowded: digit by digit, masses in units of the bin edge's weight
-    RSCommand c{};
-    c.op = RS_RADIX; c.b0 = b;
-    c.z0 = b > 0 && b < RS_BINS ? ((double)g.mx - (double)rs_edge((float)b, g)) / g.t : 0.0;
-    const double unit = b < RS_BINS ? exp(-c.z0) : 0.0;
-    double each = 0;   // of the tokens left: their weight
-    uint32_t left = 0;
-    for (int round = 0; round < 4; ++round) {
-      c.shift = 24 - 8 * round;
-      command(c);
-      // digits in descending order: thread t < 256 has digit 255 - t
-      uint32_t k = 0;
-      unsigned long long m = 0;
-      const int d = 255 - (int)threadIdx.x;
-      if (threadIdx.x < 256)
-        for (int r = 0; r < CL; ++r) {
-          const RSSmem* o = cl.map_shared_rank(&s, r);
-          const uint32_t* lo = reinterpret_cast<const uint32_t*>(o->dev);
-          k += o->cnt[d];
-          m += (unsigned long long)lo[256 + d] << 32 | lo[d];
-        }
-      uint32_t all_k;
-      double all_m;
-      const double mass = (double)m * 0x1p-40 * unit;
-      const uint32_t kb = rs_scan<uint32_t>(k, s.wcnt, &all_k);
-      const double mb = rs_scan<double>(mass, s.wsum, &all_m);
-      if (threadIdx.x == 0) { s.pick = 256; s.pick_cnt = 0; }
-      __syncthreads();
-      const double x = by_mass ? base + mb + mass : (double)(before + kb + k);
-      if (k) {
-        if (strict ? x > target : x >= target) atomicMin(&s.pick, (int)threadIdx.x);
-        atomicMax(&s.pick_cnt, threadIdx.x);  // the last digit that is there, should rounding leave no crossing
-      }
-      __syncthreads();
-      const int at = s.pick < 256 ? s.pick : (int)s.pick_cnt;
-      if ((int)threadIdx.x == at) { s.sel_cnt = before + kb; s.sel_base = base + mb; s.sel_in = k; s.pick_w = k ? mass / k : 0.0; }
-      __syncthreads();
-      before = s.sel_cnt; base = s.sel_base; left = s.sel_in; each = s.pick_w;
-      c.prefix = c.prefix << 8 | (uint32_t)(255 - at);
-      __syncthreads();
-    }
-    // `left` tokens of the same logit: the j-th of them by index
-    double j = 0;
-    if (!by_mass) j = target - before - 1;
-    else if (each > 0) {
-      j = floor((target - base) / each);
-      if (!strict && j * each >= target - base) j -= 1;  // reaching is enough
-    }
-    const uint32_t skip = (uint32_t)min(max(j, 0.0), (double)left - 1);
-    c.op = RS_FIND; c.key = c.prefix; c.skip = skip;
-    command(c);
-    p.idx = s.found;
-    p.w = rs_weight(rs_unorder(c.prefix), g);
-    p.cnt = before + skip + 1;
-    p.mass = base + (double)(skip + 1) * each;
-    __syncthreads();
-    return p;
   }
 
   __device__ void answer(int r, int idx, double prob, uint32_t kept) {
@@ -650,83 +638,230 @@ struct RSRow {
       if (a.kept) a.kept[r] = (int)kept;
     }
   }
+  // The answer that a sorted list holds which has every kept token; `rest`: mass of the tokens that are not in it.
+  __device__ __forceinline__ void settle(int r, int n_list, uint32_t cut, bool cut_k, double top_p, double u, double rest) {
+    int kept = (int)min(cut, (uint32_t)n_list);
+    if (top_p < 1) {  // the mass it goes by is that of the first k, or of all
+      const double target = top_p * (cut_k ? s.cum[kept - 1] : s.cum[n_list - 1] + rest);
+      kept = min(kept, list_before(kept, target, false) + 1);
+    }
+    if (min_p > 0) {
+      int ok = 0;
+#pragma unroll
+      for (int e = 0; e < RS_EACH; ++e) {
+        const int i = threadIdx.x + e * TH;
+        if (e && n_list <= e * TH) break;
+        ok += __syncthreads_count(i < n_list && rs_weight(list_logit(i), g) >= min_p);
+      }
+      kept = min(kept, max(ok, 1));
+    }
+    const double mass = s.cum[kept - 1];
+    const int i = min(list_before(kept, u * mass, true), kept - 1);
+    answer(r, (int)(uint32_t)s.list[i], rs_weight(list_logit(i), g) / mass, (uint32_t)kept);
+  }
 
-  __device__ void lead(int r, int k, double top_p, double u, bool masses) {
-    scan_bins();
-    if (masses && most()) recollect((int)most());
-    const uint32_t all = all_cnt;
-    const bool cut_k = k > 0 && (uint32_t)k < all;
-    const uint32_t cut = cut_k ? (uint32_t)k : all;
-    const bool by_p = top_p < 1, by_m = min_p > 0;
-    const bool listed = cut_k || !masses;  // the mass that top-p goes by is that of tokens that are all in the list
-    // the last bin that a kept token can lie in
-    const double over = by_m ? -log(min_p) * g.t * (double)g.sx : 0.0;
+  // What the first CTA does between two commands, as a machine whose states are what the last command was for: every
+  // command is served at one place in the code, which keeps a row's state in registers.  Ends are looked up (LOOK) for
+  // a purpose: the first k (mass of), top-p's end, min-p's (mass of), the token, the last kept token.
+  enum { START, LISTED, REFILLED, LAST_LIST, LOOKED, DIGIT, FOUND, COUNTED };
+  enum { OF_K, OF_P, OF_M, OF_TOKEN, OF_LAST };
+  // the next command (DONE: the row is answered); the row's state is in shared memory while a command is served
+  __device__ __forceinline__ RSCommand next(int r) {
+    RSLead m = s.lead;
+    const RSCommand c = step(m, r);
     __syncthreads();
-    if (threadIdx.x == 0) { s.bin_k = s.bin_p = RS_BINS; s.pick = 0; }
-    __syncthreads();
-    if (cut_k) cross(false, (double)k, false, &s.bin_k);
-    if (by_p && !listed) cross(true, top_p * all_mass, false, &s.bin_p);
-    __syncthreads();
-    int last = s.bin_k;
-    if (by_m && !(listed && by_p)) last = min(last, over < RS_BINS ? (int)fmax(over, 0.0) + 1 : RS_BINS);
-    if (by_p && !listed) last = min(last, s.bin_p == RS_BINS ? s.pick : s.bin_p);
-    uint32_t before, in;
-    double base, in_mass;
-    at_bin(last, &before, &base, &in, &in_mass);
-    if (before + in <= RS_CAP) {
-      RSCommand c{};
-      c.op = RS_GATHER; c.b1 = last; c.last = 1;
-      command(c);
+    if (threadIdx.x == 0) s.lead = m;
+    return c;
+  }
+  __device__ __forceinline__ RSCommand step(RSLead& m, int r) {
+    RSCommand c{};
+    const bool by_p = m.top_p < 1, by_m = min_p > 0;
+    if (m.state == START && by_m) m.over = -log(min_p) * g.t * (double)g.sx;
+    const int over_bin = m.over < RS_BINS ? (int)fmax(m.over, 0.0) : RS_BINS;
+    int idx = 0;          // what a look found
+    double w = 0, mass = 0;
+    uint32_t cnt = 0;
+    if (m.state == START) {
+      m.state = LISTED;
+      c.op = RS_GATHER;
+      if (all_cnt <= RS_COUNT) {
+        c.b1 = RS_BINS;
+        c.last = 1;
+        return c;
+      }
+      if (m.mode == RS_NONE) {
+        c.b1 = min(over_bin + 1, RS_BINS);
+        return c;
+      }
+      const uint32_t counted = scan_bins();
+      if (m.mode == RS_LARGEST || m.mode == RS_COUNTS) {
+        c.b1 = cross_one(false, (double)m.cut, false);
+        return c;
+      }
+      m.left = counted;
+      m.state = REFILLED;
+    } else if (m.state == REFILLED) {
+      m.left = scan_bins();
+    }
+    if (m.state == LISTED || m.state == LAST_LIST) {
+      const int n_list = (int)s.n_list;
+      if (n_list <= RS_CAP) {
+        sort(n_list);
+        list_masses(n_list, 0.0);
+        settle(r, n_list, m.cut, m.cut_k, m.top_p, m.u, m.state == LISTED ? 0.0 : all_mass - m.base - m.in_mass);
+        return c;
+      }
+      m.mode = one_word() && !by_p ? RS_ONE_WORD : RS_TWO_WORDS;
+      m.state = REFILLED;
+      c.op = RS_FILL; c.mode = m.mode; c.sure = (int)RS_ROOM2;
+      return c;
+    }
+    if (m.state == REFILLED) {
+      if (m.mode == RS_ONE_WORD ? !fine(m.left) : sure < a.per && (crowded() || m.left != all_cnt)) {
+        c.op = RS_FILL;
+        c.mode = RS_TWO_WORDS;
+        c.sure = m.mode == RS_ONE_WORD ? (int)RS_ROOM2 : max(a.per, (int)RS_ROOM2);
+        m.mode = RS_TWO_WORDS;
+        return c;
+      }
+      // the last bin that a kept token can lie in
+      __syncthreads();
+      if (threadIdx.x == 0) { s.bin_k = s.bin_p = RS_BINS; s.pick = 0; }
+      __syncthreads();
+      if (m.cut_k) cross(false, (double)m.cut, false, &s.bin_k);
+      if (by_p && !m.cut_k) cross(true, m.top_p * all_mass, false, &s.bin_p);
+      __syncthreads();
+      int last = s.bin_k;
+      if (by_m && !(m.cut_k && by_p)) last = min(last, min(over_bin + 1, RS_BINS));
+      if (by_p && !m.cut_k) last = min(last, s.bin_p == RS_BINS ? s.pick : s.bin_p);
+      uint32_t in;
+      at_bin(last, &m.before, &m.base, &in, &m.in_mass);
+      if (m.before + in <= RS_CAP) {
+        m.state = LAST_LIST;
+        c.op = RS_GATHER; c.b1 = last; c.last = 1;
+        return c;
+      }
+      // long prefixes: each end by itself
+      m.kept = m.cut;
+      m.mass = all_mass;
+      m.purpose = m.cut_k ? OF_K : by_p ? OF_P : by_m ? OF_M : OF_TOKEN;
+      if (m.purpose == OF_M) {
+        m.state = COUNTED;
+        c.op = RS_OVER; c.b0 = over_bin - 1; c.b1 = min(over_bin + 1, RS_BINS);
+        return c;
+      }
+    } else if (m.state == LOOKED) {
       const int n_list = (int)s.n_list;
       sort(n_list);
-      list_masses(n_list, 0.0);
-      int kept = (int)min(cut, (uint32_t)n_list);
-      if (by_p) {
-        // mass of the cut: of the list's first k, or of the list and the bins behind it
-        const double mass = listed ? s.cum[kept - 1] : s.cum[n_list - 1] + (all_mass - base - in_mass);
-        kept = min(kept, list_before(kept, top_p * mass, false) + 1);
-      }
-      if (by_m) {
-        int ok = 0;
-#pragma unroll
-        for (int e = 0; e < RS_EACH; ++e) {
-          const int i = threadIdx.x + e * RS_THREADS;
-          if (e && n_list <= e * RS_THREADS) break;
-          ok += __syncthreads_count(i < n_list && rs_weight(list_logit(i), g) >= min_p);
+      list_masses(n_list, m.base);
+      const int i = min(max(m.by_mass ? list_before(n_list, m.target, m.strict) : (int)(m.target - m.before) - 1, 0), n_list - 1);
+      idx = (int)(uint32_t)s.list[i];
+      w = rs_weight(list_logit(i), g);
+      cnt = m.before + i + 1;
+      mass = s.cum[i];
+    } else if (m.state == DIGIT) {
+      // digits in descending order: thread t < 256 has digit 255 - t
+      uint32_t k = 0;
+      unsigned long long x = 0;
+      const int d = 255 - (int)threadIdx.x;
+      if (threadIdx.x < 256)
+        for (int q = 0; q < CL; ++q) {
+          const RSSmem* o = cl.map_shared_rank(&s, q);
+          k += o->cnt[d];
+          x += (unsigned long long)o->low[256 + d] << 32 | o->low[d];
         }
-        kept = min(kept, max(ok, 1));
-      }
-      const double mass = s.cum[kept - 1];
-      const int i = min(list_before(kept, u * mass, true), kept - 1);
-      answer(r, (int)(uint32_t)s.list[i], rs_weight(list_logit(i), g) / mass, (uint32_t)kept);
-      return;
-    }
-    // long prefixes: each end by itself
-    if (!masses) recollect((int)max(most(), (uint32_t)RS_SURE));  // the k-th token's bin is crowded
-    uint32_t kept = cut;
-    double mass = all_mass;
-    if (cut_k) mass = select(false, (double)k, false, false).mass;
-    if (by_p) {
-      const Pick p = select(true, top_p * mass, false, false);
-      if (p.cnt < kept) { kept = p.cnt; mass = p.mass; }
-    }
-    if (by_m) {
-      const int b = over < RS_BINS ? (int)fmax(over, 0.0) : RS_BINS;
-      RSCommand c{};
-      c.op = RS_OVER; c.b0 = b - 1; c.b1 = min(b + 1, RS_BINS);
-      command(c);
-      const uint32_t n_over = max(s.over, 1u);
+      uint32_t kb = k, all_k;
+      const double of_digit = (double)x * 0x1p-40 * m.unit;
+      double mb = of_digit, all_m;
+      rs_scan2<TH>(kb, mb, s, &all_k, &all_m);
+      if (threadIdx.x == 0) { s.pick = 256; s.pick_cnt = 0; }
       __syncthreads();
-      if (n_over < kept) { kept = n_over; mass = select(false, (double)n_over, false, false).mass; }
+      const double at_end = m.by_mass ? m.base + mb + of_digit : (double)(m.before + kb + k);
+      if (k) {
+        if (m.strict ? at_end > m.target : at_end >= m.target) atomicMin(&s.pick, (int)threadIdx.x);
+        atomicMax(&s.pick_cnt, threadIdx.x);  // the last digit that is there, should rounding leave no crossing
+      }
+      __syncthreads();
+      const int at = s.pick < 256 ? s.pick : (int)s.pick_cnt;
+      if ((int)threadIdx.x == at) {
+        s.sel_cnt = m.before + kb;
+        s.sel_base = m.base + mb;
+        s.sel_in = k;
+        s.pick_w = k ? of_digit / k : 0.0;
+      }
+      __syncthreads();
+      m.before = s.sel_cnt; m.base = s.sel_base; m.left = s.sel_in; m.each = s.pick_w;
+      m.prefix = m.prefix << 8 | (uint32_t)(255 - at);
+      if (++m.round < 4) {
+        c.op = RS_RADIX; c.b0 = m.b; c.prefix = m.prefix; c.shift = 24 - 8 * m.round;
+        c.z0 = m.in_mass;
+        return c;
+      }
+      // `left` tokens of the same logit: the j-th of them by index
+      double j = 0;
+      if (!m.by_mass) j = m.target - m.before - 1;
+      else if (m.each > 0) {
+        j = floor((m.target - m.base) / m.each);
+        if (!m.strict && j * m.each >= m.target - m.base) j -= 1;  // reaching is enough
+      }
+      m.left = (uint32_t)fmin(fmax(j, 0.0), (double)m.left - 1);
+      m.state = FOUND;
+      c.op = RS_FIND; c.key = m.prefix; c.skip = m.left;
+      return c;
+    } else if (m.state == FOUND) {
+      idx = s.found;
+      w = rs_weight(rs_unorder(m.prefix), g);
+      cnt = m.before + m.left + 1;
+      mass = m.base + (double)(m.left + 1) * m.each;
+    } else {  // COUNTED: tokens of weight >= min-p
+      const uint32_t n_over = max(s.over, 1u);
+      m.purpose = n_over < m.kept ? OF_M : OF_TOKEN;
+      if (m.purpose == OF_M) m.kept = n_over;
     }
-    Pick p = select(true, u * mass, true, !cut_k && !by_p && !by_m);
-    if (p.cnt > kept) p = select(false, (double)kept, false, true);  // the two sums of a bin differ by a rounding
-    answer(r, p.idx, p.w / mass, kept);
+    if (m.state == LOOKED || m.state == FOUND) {  // what was found, and what it leads to
+      if (m.purpose == OF_TOKEN && cnt > m.kept) {  // the two sums of a bin differ by a rounding
+        m.purpose = OF_LAST;
+      } else if (m.purpose >= OF_TOKEN) {
+        answer(r, idx, w / m.mass, m.kept);
+        return c;
+      } else {
+        if (m.purpose != OF_P || cnt < m.kept) { m.kept = m.purpose == OF_M ? m.kept : cnt; m.mass = mass; }
+        const int was = m.purpose;
+        m.purpose = was == OF_K && by_p ? OF_P : was != OF_M && by_m ? OF_M : OF_TOKEN;
+        if (m.purpose == OF_M) {
+          m.state = COUNTED;
+          c.op = RS_OVER; c.b0 = over_bin - 1; c.b1 = min(over_bin + 1, RS_BINS);
+          return c;
+        }
+      }
+    }
+    // LOOK
+    m.by_mass = m.purpose == OF_P || m.purpose == OF_TOKEN;
+    m.strict = m.purpose == OF_TOKEN;
+    m.target = m.purpose == OF_P ? m.top_p * m.mass : m.purpose == OF_TOKEN ? m.u * m.mass : (double)m.kept;
+    m.b = cross_one(m.by_mass, m.target, m.strict);
+    uint32_t in;
+    double in_mass;
+    at_bin(m.b, &m.before, &m.base, &in, &in_mass);
+    if (in <= RS_CAP) {
+      m.state = LOOKED;
+      c.op = RS_GATHER; c.b0 = c.b1 = m.b;
+      c.last = m.purpose == OF_TOKEN && m.kept == all_cnt;  // no prefix ends before the token that is found
+      return c;
+    }
+    // crowded: digit by digit, masses in units of the bin edge's weight
+    m.state = DIGIT;
+    m.round = 0;
+    m.prefix = 0;
+    m.in_mass = m.b > 0 && m.b < RS_BINS ? ((double)g.mx - (double)rs_edge((float)m.b, g)) / g.t : 0.0;  // edge / T
+    m.unit = m.b < RS_BINS ? exp(-m.in_mass) : 0.0;
+    c.op = RS_RADIX; c.b0 = m.b; c.shift = 24; c.z0 = m.in_mass;
+    return c;
   }
 };
 
-template <class T, bool STAGED, int CL>
-__global__ void __launch_bounds__(RS_THREADS, 2) sample_rows_kernel(const RSArgs a) {
+template <class T, bool STAGED, int CL, int TH>
+__global__ void __launch_bounds__(TH, TH == RS_THREADS_FEW ? 1 : 2) sample_rows_kernel(const RSArgs a) {
   extern __shared__ __align__(16) uint8_t rs_raw[];
   RSSmem& s = *reinterpret_cast<RSSmem*>(rs_raw);
   T* stage = reinterpret_cast<T*>(rs_raw + (sizeof(RSSmem) + 15) / 16 * 16);
@@ -736,69 +871,77 @@ __global__ void __launch_bounds__(RS_THREADS, 2) sample_rows_kernel(const RSArgs
   const int r = (int)(blockIdx.x / CL);
   const int i0 = min(rank * a.per, a.vocab), n = min(a.per, a.vocab - i0);
   const T* row = reinterpret_cast<const T*>(a.logits) + (int64_t)r * a.ld;
-  RSRow<T, STAGED, CL> w{s, stage, a, row, i0, n, RSGeom{}, cl, 0.0, RS_SURE, false};
+  RSRow<T, STAGED, CL, TH> w{s, stage, a, row, i0, n, RSGeom{}, cl, 0.0, 0u, (int)RS_ROOM2};
 
   // 1. this CTA's logits, the largest and the smallest that is a number.  Copies of 16 bytes and more; the shares are
   // multiples of 8 logits, what is left of a row's end comes by itself.
   constexpr int V = 16 / sizeof(T);
   const int nv = a.vec ? n / V : 0;
   if (STAGED) {
-    for (int v = tid; v < nv; v += RS_THREADS)
+    for (int v = tid; v < nv; v += TH)
       asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" :: "r"(smem_u32(stage + v * V)), "l"(row + i0 + v * V) : "memory");
   }
   const float t = a.temperature ? a.temperature[r] : 1.f;
   const int k = a.top_k ? a.top_k[r] : 0;
   const float p = a.top_p ? a.top_p[r] : 1.f, q = a.min_p ? a.min_p[r] : 0.f, un = a.u[r];
-  for (int i = tid; i < RS_BINS; i += RS_THREADS) { s.cnt[i] = 0; s.dev[i] = 0; }
+  for (int i = tid; i < RS_BINS; i += TH) s.cnt[i] = s.low[i] = 0;
   if (tid == 0) s.own_beyond = 0;
-  RSStat st{-INFINITY, INFINITY};
+  RSStat st{-INFINITY, INFINITY, 0};
   auto see = [&](float l) {  // NaN is neither
     st.mx = fmaxf(st.mx, l);
     st.mn = fminf(st.mn, l > -INFINITY ? l : INFINITY);
+    st.n += l > -INFINITY;
   };
   if (STAGED) {
-    for (int i = nv * V + tid; i < n; i += RS_THREADS) {
+    for (int i = nv * V + tid; i < n; i += TH) {
       const T x = row[i0 + i];
       stage[i] = x;
       see(rs_float(x));
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-    for (int v = tid; v < nv; v += RS_THREADS) {  // what this thread has copied
+    for (int v = tid; v < nv; v += TH) {  // what this thread has copied
       const uint4 x = *reinterpret_cast<const uint4*>(stage + v * V);
       const T* e = reinterpret_cast<const T*>(&x);
 #pragma unroll
       for (int j = 0; j < V; ++j) see(rs_float(e[j]));
     }
   } else {
-    for (int i = tid; i < n; i += RS_THREADS) see(rs_float(row[i0 + i]));
+    for (int i = tid; i < n; i += TH) see(rs_float(row[i0 + i]));
   }
+  const float largest = st.mx;  // this thread's
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     st.mx = fmaxf(st.mx, __shfl_xor_sync(0xffffffffu, st.mx, o));
     st.mn = fminf(st.mn, __shfl_xor_sync(0xffffffffu, st.mn, o));
+    st.n += __shfl_xor_sync(0xffffffffu, st.n, o);
   }
   if (lane == 0) s.wstat[warp] = st;
   if (tid == 0) s.first = 0x7fffffff;
   __syncthreads();
   rs_wait<CL>();
   if (warp == 0) {
-    st = s.wstat[lane % RS_WARPS];
+    st = s.wstat[lane % (TH / 32)];
 #pragma unroll
-    for (int o = RS_WARPS / 2; o > 0; o >>= 1) {
+    for (int o = (TH / 32) / 2; o > 0; o >>= 1) {
       st.mx = fmaxf(st.mx, __shfl_xor_sync(0xffffffffu, st.mx, o));
       st.mn = fminf(st.mn, __shfl_xor_sync(0xffffffffu, st.mn, o));
+      st.n += __shfl_xor_sync(0xffffffffu, st.n, o);
     }
     if (lane < CL) cl.map_shared_rank(&s, lane)->stats[rank] = st;
   }
   rs_sync<CL>();
   st = s.stats[0];
 #pragma unroll
-  for (int c = 1; c < CL; ++c) { st.mx = fmaxf(st.mx, s.stats[c].mx); st.mn = fminf(st.mn, s.stats[c].mn); }
+  for (int c = 1; c < CL; ++c) {
+    st.mx = fmaxf(st.mx, s.stats[c].mx);
+    st.mn = fminf(st.mn, s.stats[c].mn);
+    st.n += s.stats[c].n;
+  }
   st.mx += 0.f;
   if (st.mx == -INFINITY || !(t > 0.f)) {  // no token, or greedy: the first of the largest
     int at = 0x7fffffff;
     if (st.mx > -INFINITY)
-      for (int i = tid; i < n; i += RS_THREADS)
+      for (int i = tid; i < n; i += TH)
         if (w.raw(i) == st.mx) { at = i0 + i; break; }
     at = (int)__reduce_min_sync(0xffffffffu, (unsigned)at);
     if (lane == 0 && at != 0x7fffffff) atomicMin(&cl.map_shared_rank(&s, 0)->first, at);
@@ -806,8 +949,6 @@ __global__ void __launch_bounds__(RS_THREADS, 2) sample_rows_kernel(const RSArgs
     if (rank == 0) w.answer(r, st.mx == -INFINITY ? -1 : s.first, st.mx == -INFINITY ? 0.0 : 1.0, st.mx == -INFINITY ? 0u : 1u);
     return;
   }
-  const bool masses = !(k > 0 && k <= RS_CAP / 2);
-
   // 2. the bins
   RSGeom& g = w.g;
   g.mx = st.mx;
@@ -819,49 +960,71 @@ __global__ void __launch_bounds__(RS_THREADS, 2) sample_rows_kernel(const RSArgs
   g.sx = span > 1e-30f ? (float)RS_BINS / span : 0.f;
   g.width = span > 1e-30f ? span / (float)RS_BINS : 0.f;
   w.min_p = q > 0.f ? (double)q : 0.0;
-  w.fill(true, masses);
-  rs_sync<CL>();
-  w.reduce(masses);
-  rs_sync<CL>();
-
-  // 3. ends of the prefixes and the token
-  if (CL == 1 || rank == 0) {
-    const double up = un > 0.f ? fmin((double)un, 1.0) : 0.0;
-    w.lead(r, k, p < 1.f ? (double)p : 1.0, up, masses);
-    if (!w.alone) {
-      __syncthreads();
-      RSCommand c{};
-      w.post(c);
-      rs_sync<CL>();
-    }
-    return;
-  }
-  for (;;) {
+  w.all_cnt = st.n;
+  const bool cut_k = k > 0 && (uint32_t)k < st.n, by_p = p < 1.f;
+  const int mode = st.n <= RS_COUNT || (q > 0.f && !by_p) ? RS_NONE
+                   // the k largest are sure to be few more than k where k is a small part of the threads' largest
+                   : cut_k && k <= RS_CAP / 2             ? (k <= a.vocab / (32 / (int)sizeof(T)) / 4 && k <= TH * CL / 8 ? RS_LARGEST : RS_COUNTS)
+                   : !by_p && w.one_word() && st.n >= RS_FLAT ? RS_ONE_WORD
+                                                          : RS_TWO_WORDS;
+  if (mode != RS_NONE) {
+    w.histogram(mode, largest);
     rs_sync<CL>();
-    const RSCommand c = s.cmd;
+  }
+
+  // 3. commands of the first CTA, until the row is answered
+  if (tid == 0) {
+    RSLead m{};
+    m.state = RSRow<T, STAGED, CL, TH>::START;
+    m.mode = mode;
+    m.cut_k = cut_k;
+    m.cut = cut_k ? (uint32_t)k : st.n;
+    m.top_p = by_p ? (double)p : 1.0;
+    m.u = un > 0.f ? fmin((double)un, 1.0) : 0.0;
+    s.lead = m;
+  }
+  __syncthreads();
+  bool alone = CL == 1;
+  for (;;) {
+    RSCommand c;
+    if (CL == 1 || rank == 0) {
+      c = w.next(r);
+      if (c.op == RS_DONE && alone) return;
+      w.post(c);
+    }
+    rs_sync<CL>();
+    c = s.cmd;
     if (c.op == RS_DONE) return;
-    w.serve(c);
+    w.serve(c, largest);
     rs_arrive<CL>();
-    if (c.last) return;  // nobody reads this CTA's memory any more
+    if (c.last && CL > 1) {
+      if (rank) return;  // nobody reads this CTA's memory any more
+      alone = true;
+    }
     rs_wait<CL>();
   }
 }
 
-template <class T, bool STAGED, int CL>
+template <class T, bool STAGED, int CL, int TH>
 static int rs_launch_one(const RSArgs& a, int batch, size_t slice, cudaStream_t st) {
   const size_t fixed = (sizeof(RSSmem) + 15) / 16 * 16;
-  if (int rc = smem_attr_once<sample_rows_kernel<T, STAGED, CL>>((int)(fixed + (STAGED ? RS_STAGE_MAX : 0)))) return rc;
-  return kv8_launch_cluster(sample_rows_kernel<T, STAGED, CL>, dim3((unsigned)batch * CL), CL, dim3(RS_THREADS), fixed + slice, st,
-                            false, a);
+  if (int rc = smem_attr_once<sample_rows_kernel<T, STAGED, CL, TH>>((int)(fixed + (STAGED ? RS_STAGE_MAX : 0)))) return rc;
+  return kv8_launch_cluster(sample_rows_kernel<T, STAGED, CL, TH>, dim3((unsigned)batch * CL), CL, dim3(TH), fixed + slice, st, false, a);
+}
+template <class T, bool STAGED, int CL>
+static int rs_launch_few(const RSArgs& a, int batch, size_t slice, cudaStream_t st) {
+  // half of the SMs: a cluster lies in one group of SMs, which one CTA an SM does not fill evenly
+  return batch <= num_sms() / 2 / CL ? rs_launch_one<T, STAGED, CL, RS_THREADS_FEW>(a, batch, slice, st)
+                                 : rs_launch_one<T, STAGED, CL, RS_THREADS_MANY>(a, batch, slice, st);
 }
 template <class T>
 static int rs_launch(RSArgs& a, int batch, cudaStream_t st) {
   const int cl = a.vocab <= RS_ALONE ? 1 : RS_CLUSTER;
   a.per = ((a.vocab + cl - 1) / cl + 7) / 8 * 8;
   const size_t slice = (size_t)a.per * sizeof(T);
-  if (cl == 1) return rs_launch_one<T, true, 1>(a, batch, slice, st);
-  if (slice <= RS_STAGE_MAX) return rs_launch_one<T, true, RS_CLUSTER>(a, batch, slice, st);
-  return rs_launch_one<T, false, RS_CLUSTER>(a, batch, 0, st);
+  if (cl == 1) return rs_launch_few<T, true, 1>(a, batch, slice, st);
+  if (slice <= RS_STAGE_MAX) return rs_launch_few<T, true, RS_CLUSTER>(a, batch, slice, st);
+  return rs_launch_few<T, false, RS_CLUSTER>(a, batch, 0, st);
 }
 
 }  // namespace n730
@@ -874,7 +1037,7 @@ N730_API int n730_sample_rows(const void* d_logits, int dtype, int batch, int vo
   const char* what = "sample_rows";
   N730_REQUIRE(d_logits && d_u && d_tokens, N730_NULL, "%s: null pointer", what);
   N730_REQUIRE(dtype == N730_F32 || dtype == N730_F16 || dtype == N730_BF16, N730_BAD_ARG, "%s: dtype %d", what, dtype);
-  N730_REQUIRE(batch >= 1 && batch <= (1 << 24) && vocab >= 1 && vocab <= (1 << 24) && ld >= vocab, N730_BAD_ARG,
+  N730_REQUIRE(batch >= 1 && batch <= (1 << 24) && vocab >= 1 && vocab <= (1 << 23) && ld >= vocab, N730_BAD_ARG,
                "%s: batch %d, vocab %d, row stride %lld", what, batch, vocab, (long long)ld);
   const int es = kv8_esize(dtype);
   N730_REQUIRE(kv8_aligned(es, (const char*)d_logits) &&
