@@ -8,7 +8,7 @@
 // the whole batch (once for 256 rows) and the products are full tiles; of a sequence's own part they are its tokens x G
 // rows.  Items of few rows, or of long positions, are cut along the positions so that every SM has some.
 //
-// A CTA takes one item.  Warps 0-3 (and 4-7 with two row tiles): softmax, a thread a row.  The next warp brings K and V
+// A CTA takes one item.  Eight warps a row tile: softmax, two threads a row.  The next warp brings K and V
 // by tensor copies, the last one issues S = Q K^T (both from shared memory, K-major) and O += P V (P in tensor memory, V
 // MN-major), of the two row tiles in turn so that one's products run under the other's softmax.  P, rounded to the cache's
 // type, overwrites its scores.  With one row tile two CTAs share an SM to the same end.  Pages are copied as they lie,
@@ -48,7 +48,7 @@ struct KACfg {
   static constexpr int QB = ROWS * 128, KB = KA_KEYS * 128;        // bytes of a block of Q, of K or V
   static constexpr int KV = NB * KB;                               // bytes of a tile of K or V
   static constexpr int STAGES = NT == 2 || HD == 64 ? 2 : 1;       // one row tile of 128 channels: 96 KB, two CTAs an SM
-  static constexpr int COPY_WARP = NT * 4, MMA_WARP = NT * 4 + 1, THREADS = (NT * 4 + 2) * 32;
+  static constexpr int COPY_WARP = NT * 8, MMA_WARP = NT * 8 + 1, THREADS = (NT * 8 + 2) * 32;
   static constexpr uint32_t TMEM = NT == 1 ? 256u : 512u;
   static constexpr uint32_t S0 = 0, O0 = NT * KA_KEYS;             // columns: scores, outputs
 };
@@ -69,6 +69,7 @@ struct KASmem {
   uint32_t tmem;
   int abort;
   int n_bad, bad[KA_BAD];
+  float half[2][NT][2][128];  // by tile's parity, row tile, half: what the two threads of a row tell each other
 };
 
 // Parts of one kind (the prefix's or the sequences' own): [unit][split][rows of a unit], a unit being a KV head, or a
@@ -113,7 +114,14 @@ __device__ __forceinline__ void ka_copy(void* dst, const CUtensorMap* map, int c
                : "memory");
 }
 
-// Moves a row's reference to its tile's maximum y where that is larger; its sum and, when there are any, outputs follow.
+// The two threads of a row, in warps w and w + 4 of a row tile, meet: each its half's maximum, both the row's.
+__device__ __forceinline__ float ka_row_max(float y, float* mine, const float* other, int bar) {
+  *mine = y;
+  asm volatile("bar.sync %0, 64;" :: "r"(bar) : "memory");
+  return fmaxf(y, *other);
+}
+// Moves a row's reference to its tile's maximum y where that is larger; the thread's sum and, when there are any, its
+// half of the outputs (at to) follow.
 template <int HD>
 __device__ __forceinline__ void ka_move(uint32_t to, bool outputs, float y, float& m, float& l) {
   const float mn = fmaxf(m, y), f = mn == m ? 1.f : ex2(m - mn);
@@ -121,75 +129,61 @@ __device__ __forceinline__ void ka_move(uint32_t to, bool outputs, float y, floa
   l *= f;
   if (!outputs) return;
 #pragma unroll 1
-  for (int cc = 0; cc < HD; cc += 8) tc_scale8(to + cc, f);
+  for (int cc = 0; cc < HD / 2; cc += 8) tc_scale8(to + cc, f);
 }
 
-// One tile of a row whose positions are all seen: weights over the scores at ts, their sum to l.
+// A thread's half of one tile of a row whose positions are all seen: weights over the scores, their sum to l.  ts: the
+// half's scores; tp: its weights, which lie over the first half's scores.
 template <int HD, bool BF>
-__device__ __forceinline__ void ka_softmax(uint32_t ts, uint32_t to, float c, bool outputs, float& m, float& l) {
-  float v[KA_KEYS];
+__device__ __forceinline__ void ka_softmax(uint32_t ts, uint32_t tp, uint32_t to, float c, bool outputs, float* mine,
+                                           const float* other, int bar, float& m, float& l) {
+  float v[64];
   tc_ld64(ts, v);
-  tc_ld64(ts + 64, v + 64);
   float mx[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-  for (int i = 4; i < KA_KEYS; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
-  const float y = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+  for (int i = 4; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
+  const float y = ka_row_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c, mine, other, bar);
   if (__any_sync(0xffffffffu, y > m + KA_MOST)) ka_move<HD>(to, outputs, y, m, l);
   const float ms = m == -INFINITY ? 0.f : m;
   const float2 c2 = both(c), m2 = both(-ms);
   float2 sum[2] = {both(0.f), both(0.f)};
+  uint32_t w[32];
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    uint32_t w[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const float2 x = fma2(make_float2(v[half * 64 + 2 * i], v[half * 64 + 2 * i + 1]), c2, m2);
-      const float2 p = make_float2(ex2(x.x), ex2(x.y));
-      sum[i & 1] = add2(sum[i & 1], p);
-      w[i] = ka_pack<BF>(p.x, p.y);
-    }
-    tc_st32(ts + half * 32, w);
+  for (int i = 0; i < 32; ++i) {
+    const float2 x = fma2(make_float2(v[2 * i], v[2 * i + 1]), c2, m2);
+    const float2 p = make_float2(ex2(x.x), ex2(x.y));
+    sum[i & 1] = add2(sum[i & 1], p);
+    w[i] = ka_pack<BF>(p.x, p.y);
   }
+  tc_st32(tp, w);
   const float2 s = add2(sum[0], sum[1]);
   l += s.x + s.y;
 }
-// The same where the row sees the first `sees` positions, of those the ones that have a page.
+// The same where the row sees the first `sees` positions of the half, of those the ones that have a page.
 template <int HD, bool BF>
-__device__ __forceinline__ void ka_softmax_some(uint32_t ts, uint32_t to, float c, int sees, uint32_t pages, bool outputs,
-                                                float& m, float& l) {
-  float mx = -INFINITY;
-#pragma unroll 1
-  for (int cc = 0; cc < 4; ++cc) {
-    float v[32];
-    tc_ld32(ts + cc * 32, v);
+__device__ __forceinline__ void ka_softmax_some(uint32_t ts, uint32_t tp, uint32_t to, float c, int sees, uint32_t pages, bool outputs,
+                                                float* mine, const float* other, int bar, float& m, float& l) {
+  float v[64], mx = -INFINITY;
+  tc_ld64(ts, v);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) mx = fmaxf(mx, cc * 32 + i < sees && (pages >> (2 * cc + i / 16) & 1) ? v[i] : -INFINITY);
+  for (int i = 0; i < 64; ++i) {
+    v[i] = i < sees && (pages >> (i / 16) & 1) ? v[i] : -INFINITY;
+    mx = fmaxf(mx, v[i]);
   }
-  const float y = mx * c;
-  const float yy = mx == -INFINITY ? -INFINITY : y;  // c may be 0
-  if (__any_sync(0xffffffffu, yy > m + KA_MOST)) ka_move<HD>(to, outputs, yy, m, l);
+  const float y = ka_row_max(mx == -INFINITY ? mx : mx * c, mine, other, bar);  // c may be 0
+  if (__any_sync(0xffffffffu, y > m + KA_MOST)) ka_move<HD>(to, outputs, y, m, l);
   const float ms = m == -INFINITY ? 0.f : m;
-#pragma unroll 1
-  for (int c2 = 0; c2 < 2; ++c2) {  // 64 positions: 32 columns of P over scores that have been read
-    uint32_t w[32];
-    float sum = 0.f;
+  uint32_t w[32];
+  float sum = 0.f;
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      float v[32];
-      tc_ld32(ts + c2 * 64 + hh * 32, v);
-#pragma unroll
-      for (int i = 0; i < 32; i += 2) {
-        const int at = c2 * 64 + hh * 32 + i;
-        const bool here = pages >> (at >> 4) & 1;
-        const float p0 = at < sees && here ? ex2(fmaf(v[i], c, -ms)) : 0.f;
-        const float p1 = at + 1 < sees && here ? ex2(fmaf(v[i + 1], c, -ms)) : 0.f;
-        sum += p0 + p1;
-        w[hh * 16 + i / 2] = ka_pack<BF>(p0, p1);
-      }
-    }
-    l += sum;
-    tc_st32(ts + c2 * 32, w);
+  for (int i = 0; i < 64; i += 2) {
+    const float p0 = i < sees && (pages >> (i / 16) & 1) ? ex2(fmaf(v[i], c, -ms)) : 0.f;
+    const float p1 = i + 1 < sees && (pages >> (i / 16) & 1) ? ex2(fmaf(v[i + 1], c, -ms)) : 0.f;
+    sum += p0 + p1;
+    w[i / 2] = ka_pack<BF>(p0, p1);
   }
+  l += sum;
+  tc_st32(tp, w);
 }
 
 template <int HD, bool BF, int NT>
@@ -234,14 +228,14 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
   const int* table = pre ? c.prefix_table : c.block_table + (int64_t)b * c.max_pages;
 
   if (tid == 0) {
-    mbar_init(&sm.qready, NT * 4);
+    mbar_init(&sm.qready, NT * 8);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&sm.kfull[s], 1);
       mbar_init(&sm.vfull[s], 1);
       mbar_init(&sm.kfree[s], 1);
       mbar_init(&sm.vfree[s], 1);
       mbar_init(&sm.sfull[s], 1);
-      mbar_init(&sm.pready[s], 4);
+      mbar_init(&sm.pready[s], 8);
       mbar_init(&sm.odone[s], 1);
     }
     mbar_init(&sm.drain, 1);
@@ -356,7 +350,7 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
       }
     }
   } else {
-    // ---------------- softmax: a thread a row ----------------
+    // ---------------- softmax: two threads a row, 64 positions of a tile each ----------------
     const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q);
     // where row f of the item lies: its token's row, its head
     auto token = [&](int f) { return pre ? f / G : b * a.tokens + f / G; };
@@ -364,7 +358,7 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
       constexpr int LPR = HD / 8, RPI = 32 / LPR, U = 4;
       const int sub = lane / LPR, ch = lane % LPR;
 #pragma unroll 1
-      for (int r0 = warp * 32; r0 < warp * 32 + 32; r0 += U * RPI) {
+      for (int r0 = warp * 16; r0 < warp * 16 + 16; r0 += U * RPI) {
         uint4 x[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -386,11 +380,12 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
       __syncwarp();
       if (lane == 0) mbar_arrive1(&sm.qready);
     }
-    const int x = warp >> 2, wq = warp & 3, r = x * 128 + wq * 32 + lane, f = f0 + r;
-    const bool live = r < nrow;
+    const int x = warp >> 3, half = warp >> 2 & 1, wq = warp & 3, r = x * 128 + wq * 32 + lane, f = f0 + r;
+    const bool live = r < nrow, some_live = x * 128 + wq * 32 < nrow;
     const int vis = !live ? 0 : pre ? sees : min(L + f / G + 1, cap);
     const uint32_t ts = tmem + ((uint32_t)(wq * 32) << 16) + Cfg::S0 + x * KA_KEYS;
-    const uint32_t to = tmem + ((uint32_t)(wq * 32) << 16) + Cfg::O0 + x * HD;
+    const uint32_t to = tmem + ((uint32_t)(wq * 32) << 16) + Cfg::O0 + x * HD + half * (HD / 2);
+    const int bar = 1 + x * 4 + wq;  // named barrier of the row's two warps
     float m = -INFINITY, l = 0.f;
     bool go = true;
     for (int j = 0; j < nt; ++j) {
@@ -398,11 +393,16 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
       tc_fence_after();
       const int p0 = (j0 + j) * KA_KEYS;
       const uint32_t pages = sm.pages[j % KA_RING];
-      if (p0 + KA_KEYS <= sees_all && pages == 0xffu) {
-        ka_softmax<HD, BF>(ts, to, a.scale_log2e, j > 0, m, l);
-      } else {
-        ka_softmax_some<HD, BF>(ts, to, a.scale_log2e, vis - p0, pages, j > 0, m, l);
-        if (x == 0 && p0 + KA_KEYS > sees_all) {  // rows of V that not everyone sees
+      float* mine = &sm.half[j & 1][x][half][wq * 32 + lane];
+      const float* other = &sm.half[j & 1][x][half ^ 1][wq * 32 + lane];
+      const bool whole = p0 + KA_KEYS <= sees_all && pages == 0xffu;
+      if (some_live) {  // rows of nobody keep what is there as their weights
+        if (whole) ka_softmax<HD, BF>(ts + half * 64, ts + half * 32, to, a.scale_log2e, j > 0, mine, other, bar, m, l);
+        else ka_softmax_some<HD, BF>(ts + half * 64, ts + half * 32, to, a.scale_log2e, vis - p0 - half * 64, pages >> (4 * half), j > 0,
+                                     mine, other, bar, m, l);
+      }
+      if (!whole) {
+        if (x == 0 && half == 0 && p0 + KA_KEYS > sees_all) {  // rows of V that not everyone sees
           if (!kp_wait_warp(&sm.vfull[j % ST], (uint32_t)((j / ST) & 1), abortf)) { go = false; break; }
           const int row = wq * 32 + lane, p = p0 + row;
           uint8_t* v = sm.v[j % ST] + row * 128;
@@ -432,13 +432,21 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
       go = kp_wait_warp(&sm.odone[x], 0, abortf);
       tc_fence_after();
     }
+    // a warp that gave up leaves its partner nothing to wait for: what the partner needs to get further than the barrier it
+    // may be at does not come without this warp
+    if (!go && some_live) asm volatile("bar.arrive %0, 64;" :: "r"(bar) : "memory");
     if (go) {
       const int n_bad = *reinterpret_cast<volatile int*>(&sm.n_bad);
       const int64_t unit = ((int64_t)(pre ? h : b * c.n_kv + h) * part.splits + split) * part.rows + f;
-      if (live) part.ml[unit] = make_float2(m, l);
+      if (some_live) {  // the row's sum is its two threads'
+        float* sum = &sm.half[nt & 1][x][1][wq * 32 + lane];
+        if (half) *sum = l;
+        asm volatile("bar.sync %0, 64;" :: "r"(bar) : "memory");
+        if (!half && live) part.ml[unit] = make_float2(m, l + *sum);
+      }
       const float ms = m == -INFINITY ? 0.f : m;
 #pragma unroll 1
-      for (int cc = 0; cc < HD; cc += 32) {
+      for (int cc = 0; some_live && cc < HD / 2; cc += 32) {
         float o[32];
         tc_ld32(to + cc, o);
         if (live && n_bad) {
@@ -451,12 +459,12 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
             for (int d = 0; d < HD; ++d) dot = fmaf(kv8_load1(a.q, qa + d, c.dtype), kv8_load1(c.k, at + d, c.dtype), dot);
             const float w = ex2(fmaf(a.sign ? -dot : dot, a.scale_log2e, -ms));
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = fmaf(w, kv8_load1(c.v, at + cc + e, c.dtype), o[e]);
+            for (int e = 0; e < 32; ++e) o[e] = fmaf(w, kv8_load1(c.v, at + half * (HD / 2) + cc + e, c.dtype), o[e]);
           }
         }
         __syncwarp();
         if (live) {
-          float4* dst = reinterpret_cast<float4*>(part.o + unit * HD + cc);
+          float4* dst = reinterpret_cast<float4*>(part.o + unit * HD + half * (HD / 2) + cc);
 #pragma unroll
           for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
         }
