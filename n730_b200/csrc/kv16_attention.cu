@@ -332,6 +332,8 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
     for (int j = 0; go && j < nt; ++j) {
       const int s = j % ST, s1 = (j + 1) % ST;
       go = kp_wait_warp(&sm.vfull[s], (uint32_t)((j / ST) & 1), abortf);
+      // with two stages the next tile's K has been there for long: a wait costs 300 cycles, better here than between products
+      if (ST > 1 && go && j + 1 < nt) go = kp_wait_warp(&sm.kfull[s1], (uint32_t)(((j + 1) / ST) & 1), abortf);
 #pragma unroll 1
       for (int x = 0; go && x < NT; ++x) {
         go = kp_wait_warp(&sm.pready[x], (uint32_t)(j & 1), abortf);
@@ -339,7 +341,7 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
         tc_fence_after();
         outputs(x, s, j == 0);
         if (j + 1 < nt) {
-          if (x == 0) go = kp_wait_warp(&sm.kfull[s1], (uint32_t)(((j + 1) / ST) & 1), abortf);
+          if (ST == 1 && x == 0) go = kp_wait_warp(&sm.kfull[s1], (uint32_t)(((j + 1) / ST) & 1), abortf);
           if (!go) break;
           tc_fence_after();
           scores(x, s1);
