@@ -72,12 +72,14 @@ struct KASmem {
   float half[2][NT][2][128];  // by tile's parity, row tile, half: what the two threads of a row tell each other
 };
 
-// Parts of one kind (the prefix's or the sequences' own): [unit][split][rows of a unit], a unit being a KV head, or a
-// sequence and a KV head.
+// Parts of one kind (the prefix's or the sequences' own): [unit][split][4 channels][rows of a unit], a unit being a KV
+// head, or a sequence and a KV head.  Rows lie side by side: a warp writes and reads its rows' 16 bytes as one piece
+// (written as rows of head_dim floats by a thread each, 256 rows took 10k cycles, half as long as the rest of the item).
 struct KAParts {
-  int tiles, splits, rows;   // row tiles of a unit, shares of the positions, tiles * rows of a tile
-  float* o;
-  float2* ml;                // reference (log2) and sum of weights
+  int tiles, splits, rows;   // row tiles of a unit, shares of the positions, rows in memory
+  int tile_rows;             // rows of a tile
+  float4* o;
+  float2* ml;                // [unit][split][row]: reference (log2) and sum of weights
 };
 struct KAArgs {
   N730KV16Cache c;
@@ -91,6 +93,7 @@ struct KAArgs {
   const int* lens; const int* n_new;
   int* status;
   KAParts pre, own;
+  FastDiv by_group, by_tokens;
 };
 
 // shares of the positions that are used: the plan knows the tables' widths alone
@@ -355,19 +358,20 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
     // ---------------- softmax: two threads a row, 64 positions of a tile each ----------------
     const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q);
     // where row f of the item lies: its token's row, its head
-    auto token = [&](int f) { return pre ? f / G : b * a.tokens + f / G; };
+    auto token = [&](int f) { return (pre ? 0 : b * a.tokens) + (int)a.by_group.div(f); };
+    auto query = [&](int f) { return (int64_t)token(f) * a.ldq + (int64_t)(h * G + f - (int)a.by_group.div(f) * G) * HD; };
     {
-      constexpr int LPR = HD / 8, RPI = 32 / LPR, U = 4;
+      constexpr int LPR = HD / 8, RPI = 32 / LPR, U = 16 / RPI;  // all of the warp's 16 rows at once
       const int sub = lane / LPR, ch = lane % LPR;
-#pragma unroll 1
-      for (int r0 = warp * 16; r0 < warp * 16 + 16; r0 += U * RPI) {
+      const int r0 = warp * 16;
+      {
         uint4 x[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int r = r0 + u * RPI + sub, f = f0 + r;
           x[u] = make_uint4(0, 0, 0, 0);
           if (r >= nrow) continue;
-          const uint16_t* p = q + (int64_t)token(f) * a.ldq + (int64_t)(h * G + f % G) * HD + ch * 8;
+          const uint16_t* p = q + query(f) + ch * 8;
           if (a.qvec) x[u] = *reinterpret_cast<const uint4*>(p);
           else x[u] = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
         }
@@ -384,7 +388,7 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
     }
     const int x = warp >> 3, half = warp >> 2 & 1, wq = warp & 3, r = x * 128 + wq * 32 + lane, f = f0 + r;
     const bool live = r < nrow, some_live = x * 128 + wq * 32 < nrow;
-    const int vis = !live ? 0 : pre ? sees : min(L + f / G + 1, cap);
+    const int vis = !live ? 0 : pre ? sees : min(L + (int)a.by_group.div(f) + 1, cap);
     const uint32_t ts = tmem + ((uint32_t)(wq * 32) << 16) + Cfg::S0 + x * KA_KEYS;
     const uint32_t to = tmem + ((uint32_t)(wq * 32) << 16) + Cfg::O0 + x * HD + half * (HD / 2);
     const int bar = 1 + x * 4 + wq;  // named barrier of the row's two warps
@@ -439,12 +443,12 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
     if (!go && some_live) asm volatile("bar.arrive %0, 64;" :: "r"(bar) : "memory");
     if (go) {
       const int n_bad = *reinterpret_cast<volatile int*>(&sm.n_bad);
-      const int64_t unit = ((int64_t)(pre ? h : b * c.n_kv + h) * part.splits + split) * part.rows + f;
+      const int64_t unit = (int64_t)(pre ? h : b * c.n_kv + h) * part.splits + split;
       if (some_live) {  // the row's sum is its two threads'
         float* sum = &sm.half[nt & 1][x][1][wq * 32 + lane];
         if (half) *sum = l;
         asm volatile("bar.sync %0, 64;" :: "r"(bar) : "memory");
-        if (!half && live) part.ml[unit] = make_float2(m, l + *sum);
+        if (!half && live) part.ml[unit * part.rows + f] = make_float2(m, l + *sum);
       }
       const float ms = m == -INFINITY ? 0.f : m;
 #pragma unroll 1
@@ -456,7 +460,7 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
             const int p = sm.bad[k], page = table[p / c.page_size];
             if (p >= vis || (unsigned)page >= (unsigned)c.n_pages) continue;
             const int64_t at = (((int64_t)page * c.n_kv + h) * c.page_size + p % c.page_size) * HD;
-            const int64_t qa = (int64_t)token(f) * a.ldq + (int64_t)(h * G + f % G) * HD;
+            const int64_t qa = query(f);
             float dot = 0.f;
             for (int d = 0; d < HD; ++d) dot = fmaf(kv8_load1(a.q, qa + d, c.dtype), kv8_load1(c.k, at + d, c.dtype), dot);
             const float w = ex2(fmaf(a.sign ? -dot : dot, a.scale_log2e, -ms));
@@ -466,9 +470,9 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
         }
         __syncwarp();
         if (live) {
-          float4* dst = reinterpret_cast<float4*>(part.o + unit * HD + half * (HD / 2) + cc);
+          float4* dst = part.o + (unit * (HD / 4) + (half * (HD / 2) + cc) / 4) * part.rows + f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          for (int e = 0; e < 8; ++e) dst[(int64_t)e * part.rows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
         }
       }
     }
@@ -490,77 +494,286 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
   if (blockIdx.x == 0) pdl_wait();  // the kernel behind this one waits for it alone, and so for the one before
 }
 
-// Joins a row's parts: a warp a row, HD / 32 channels a lane.
-constexpr int KJ_WARPS = 4;
-template <int HD, bool BF>
-__global__ void __launch_bounds__(KJ_WARPS * 32) kv16_join_kernel(const KAArgs a) {
-  constexpr int V = HD / 32;
+// Attention of single tokens over their own positions: a warp an item (sequence, KV head, share of the positions), its G
+// query rows (up to 8 NB) against 16 positions at a time.  Positions, and then channels, are the products' 16 rows and the
+// queries their columns (mma.m16n8k16): S^T = K Q^T, O^T += V^T P^T, so that nothing is spent on the 128 rows that a
+// tensor-memory tile would have; with single tokens this is bound by the bytes of K and V.  P^T's fragments are those of
+// S^T transposed, 8 x 8 at a time, in registers.  Rows arrive by asynchronous copies, three blocks of 16 positions deep;
+// no warp waits for another, and a CTA is one warp of KO_STAGE * 3 bytes, so that it finds room beside the CTA of the
+// prefix's kernel that is running (1024 items of 64 heads x 128, 144 positions: 46 us by the kernel above, most of that
+// hidden here).
+template <int HD> struct KOCfg { static constexpr int KB = 16 * HD * 2, STAGE = 2 * KB, STAGES = 3; };
+
+template <bool BF>
+__device__ __forceinline__ void ko_mma(float (&c)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1) {
+  if (BF)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1));
+  else
+    mma16816(c, x[0], x[1], x[2], x[3], b0, b1);
+}
+template <bool TRANS>
+__device__ __forceinline__ void ko_load(uint32_t (&x)[4], uint32_t addr) {
+  if (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(addr) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t ko_transpose(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <int HD, bool BF, int NB>
+__global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
+  using Cfg = KOCfg<HD>;
+  constexpr int KS = HD / 16, CH = HD / 8;  // steps of 16 channels; 16-byte pieces of a row
+  extern __shared__ __align__(128) uint8_t ko_smem[];
   const N730KV16Cache& c = a.c;
-  const int lane = threadIdx.x & 31, G = a.group, cap = c.max_pages * c.page_size;
-  const int64_t row = (int64_t)blockIdx.x * KJ_WARPS + (threadIdx.x >> 5);
-  const int64_t rows = (int64_t)a.batch * a.tokens * a.heads;
-  pdl_wait();
-  if (row >= rows) return;
-  const int head = (int)(row % a.heads);
-  const int64_t tok = row / a.heads;
-  const int b = (int)(tok / a.tokens), t = (int)(tok % a.tokens), h = head / G, g = head % G;
-  const int n_new = kv8_new(a.n_new, b, a.tokens);
-  if (t >= n_new) return;
-  // a row's share of its tile's positions: the tile's last row decides
-  const int np = a.pre.o ? ka_used(kv16_prefix(c), a.pre.splits) : 0;
-  const int tile_rows = a.own.rows / a.own.tiles, f = t * G + g, f0 = f / tile_rows * tile_rows;
-  const int last = (min(f0 + tile_rows, n_new * G) - 1) / G;
-  const int no = ka_used(min(kv8_len(a.lens, b, cap) + last + 1, cap), a.own.splits);
-  const int64_t p0 = (int64_t)h * a.pre.splits * a.pre.rows + tok * G + g;
-  const int64_t o0 = (int64_t)(b * c.n_kv + h) * a.own.splits * a.own.rows + f;
-  auto at = [&](int i) { return i < np ? p0 + (int64_t)i * a.pre.rows : o0 + (int64_t)(i - np) * a.own.rows; };
-  const int n = np + no;
-  float big = -INFINITY;
-  for (int i = lane; i < n; i += 32) big = fmaxf(big, (i < np ? a.pre.ml : a.own.ml)[at(i)].x);
-  big = warp_max(big);
-  float acc[V] = {}, sum = 0.f;
-  for (int i0 = 0; i0 < n; i0 += 32) {
-    float w = 0.f, l = 0.f;
-    if (i0 + lane < n) {
-      const float2 ml = (i0 + lane < np ? a.pre.ml : a.own.ml)[at(i0 + lane)];
-      w = ml.x == -INFINITY ? 0.f : ex2(ml.x - big);
-      l = ml.y;
-    }
-    // a part without a seen position has no sum either; a NaN stays one
-    sum += warp_sum(l == 0.f ? 0.f : l * w);
-    const int k1 = min(32, n - i0);
-#pragma unroll 4
-    for (int k = 0; k < k1; ++k) {
-      const float wk = __shfl_sync(0xffffffffu, w, k);
-      const float* o = (i0 + k < np ? a.pre.o : a.own.o) + at(i0 + k) * HD + lane * V;
-      if (V == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(o);
-        acc[0] = fmaf(wk, x.x, acc[0]); acc[1] = fmaf(wk, x.y, acc[1]);
-        acc[2 % V] = fmaf(wk, x.z, acc[2 % V]); acc[3 % V] = fmaf(wk, x.w, acc[3 % V]);
-      } else {
-        const float2 x = *reinterpret_cast<const float2*>(o);
-        acc[0] = fmaf(wk, x.x, acc[0]); acc[1] = fmaf(wk, x.y, acc[1]);
+  const int lane = threadIdx.x, G = a.group, cap = c.max_pages * c.page_size;
+  int i = (int)blockIdx.x;
+  const int h = i % c.n_kv;
+  i /= c.n_kv;
+  const int b = i % a.batch, split = i / a.batch;
+  const int sees = kv8_new(a.n_new, b, 1) ? min(kv8_len(a.lens, b, cap) + 1, cap) : 0;
+  const int used = ka_used(sees, a.own.splits);
+  pdl_launch_dependents();
+  if (split < used) {
+    const int blocks = (sees + 15) / 16, i0 = (int)((int64_t)blocks * split / used), n = (int)((int64_t)blocks * (split + 1) / used) - i0;
+    const int* table = c.block_table + (int64_t)b * c.max_pages;
+    const uint32_t base = smem_u32(ko_smem);
+    // block j of the share: its page, asked for a block ahead
+    auto page_of = [&](int j) { return j < n ? table[(i0 + j) * 16 / c.page_size] : -1; };
+    uint32_t here = 0;  // bit s: the block in stage s has a page
+    const int piece = lane % CH, row0 = lane / CH;
+    auto fetch = [&](int j, int page, int s) {
+      const bool ok = (unsigned)page < (unsigned)c.n_pages;
+      here = ok ? here | 1u << s : here & ~(1u << s);
+      if (j < n) {
+        const int p0 = (i0 + j) * 16;
+        const int64_t src = ((int64_t)(ok ? page : 0) * c.n_kv + h) * c.page_size + p0 % c.page_size;
+#pragma unroll
+        for (int r = row0; r < 16; r += 32 / CH) {
+          const uint32_t bytes = ok && p0 + r < sees ? 16u : 0u;  // behind the last position: zeros
+          const int64_t at = (src + r) * HD + piece * 8;
+          const uint32_t dst = base + s * Cfg::STAGE + r * (HD * 2) + ((piece ^ (r & 7)) << 4);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(reinterpret_cast<const uint16_t*>(c.k) + at), "r"(bytes) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst + Cfg::KB), "l"(reinterpret_cast<const uint16_t*>(c.v) + at), "r"(bytes) : "memory");
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int page = page_of(1);
+    fetch(0, page_of(0), 0);
+    fetch(1, page, 1);
+    page = page_of(2);
+    // the queries as the products' columns: row lane / 4 (+ 8), channels 16 k + 2 (lane % 4) (+ 8)
+    uint32_t q[NB][KS][2];
+    const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)b * a.ldq + (int64_t)h * G * HD + (lane & 3) * 2;
+#pragma unroll
+    for (int y = 0; y < NB; ++y)
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = y * 8 + (lane >> 2);
+          const uint16_t* at = qp + r * HD + k * 16 + e * 8;
+          q[y][k][e] = r >= G ? 0u : (a.qvec ? *reinterpret_cast<const uint32_t*>(at) : at[0] | (uint32_t)at[1] << 16) ^ a.sign;
+        }
+    float o[NB][KS][4] = {}, m[NB][2], l[NB][2] = {};
+#pragma unroll
+    for (int y = 0; y < NB; ++y) m[y][0] = m[y][1] = -INFINITY;
+    // where this lane's rows of the four 8 x 8 pieces lie: K's by position and then channels, V's turned
+    const int kr = lane & 15, kc = lane >> 4, vr = (lane & 7) + (lane >> 4) * 8, vc = lane >> 3 & 1;
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      const int s = j % Cfg::STAGES, p0 = (i0 + j) * 16;
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      __syncwarp();  // everyone's rows are here, and everyone is through with the block before
+      const bool ok = here >> s & 1;
+      fetch(j + 2, page, (j + 2) % Cfg::STAGES);
+      page = page_of(j + 3);
+      if (!ok) continue;
+      const uint32_t kb = base + s * Cfg::STAGE, vb = kb + Cfg::KB;
+      float x[NB][4] = {};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        uint32_t f[4];
+        ko_load<false>(f, kb + kr * (HD * 2) + (((2 * k + kc) ^ (kr & 7)) << 4));
+#pragma unroll
+        for (int y = 0; y < NB; ++y) ko_mma<BF>(x[y], f, q[y][k][0], q[y][k][1]);
+      }
+      uint32_t w[NB][2];
+#pragma unroll
+      for (int y = 0; y < NB; ++y) {
+        float big[2];
+        const int p = p0 + (lane >> 2);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          x[y][e] = p < sees ? x[y][e] * a.scale_log2e : -INFINITY;
+          x[y][2 + e] = p + 8 < sees ? x[y][2 + e] * a.scale_log2e : -INFINITY;
+          big[e] = fmaxf(x[y][e], x[y][2 + e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) big[e] = fmaxf(big[e], __shfl_xor_sync(0xffffffffu, big[e], d));
+        if (__any_sync(0xffffffffu, big[0] > m[y][0] + KA_MOST || big[1] > m[y][1] + KA_MOST)) {
+          float f[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float mn = fmaxf(m[y][e], big[e]);
+            f[e] = mn == m[y][e] ? 1.f : ex2(m[y][e] - mn);
+            m[y][e] = mn;
+            l[y][e] *= f[e];
+          }
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[y][k][e] *= f[e & 1];
+        }
+        float e4[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float ms = m[y][e & 1] == -INFINITY ? 0.f : m[y][e & 1];
+          e4[e] = ex2(x[y][e] - ms);
+          l[y][e & 1] += e4[e];
+        }
+        w[y][0] = ko_transpose(ka_pack<BF>(e4[0], e4[1]));
+        w[y][1] = ko_transpose(ka_pack<BF>(e4[2], e4[3]));
+      }
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        uint32_t f[4];
+        ko_load<true>(f, vb + vr * (HD * 2) + (((2 * k + vc) ^ (vr & 7)) << 4));
+#pragma unroll
+        for (int y = 0; y < NB; ++y) ko_mma<BF>(o[y][k], f, w[y][0], w[y][1]);
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    const int64_t unit = (int64_t)(b * c.n_kv + h) * a.own.splits + split;
+    float* dst = reinterpret_cast<float*>(a.own.o + unit * (HD / 4) * a.own.rows);
+#pragma unroll
+    for (int y = 0; y < NB; ++y)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[y][e] += __shfl_xor_sync(0xffffffffu, l[y][e], d);
+        const int r = y * 8 + (lane & 3) * 2 + e;
+        if (r >= G) continue;
+        if (lane < 4) a.own.ml[unit * a.own.rows + r] = make_float2(m[y][e], l[y][e]);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int ch = k * 16 + u * 8 + (lane >> 2);
+            dst[((int64_t)(ch >> 2) * a.own.rows + r) * 4 + (ch & 3)] = o[y][k][2 * u + e];
+          }
+      }
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + tok * a.ldo + (int64_t)head * HD + lane * V;
-  uint32_t y[V / 2];
+  if (blockIdx.x == 0) pdl_wait();
+}
+
+// Joins the rows' parts.  A CTA takes 32 rows of a KV head, a lane a row, and PIECES groups of 4 channels; its warps take
+// MINE of these each, and every PARTS-th part: with few rows that is 32 channels and a quarter of the parts, so that a
+// part's trip to memory is paid for few times in a row (896 rows of 17 parts: 7 us, 11 with a CTA for all channels), with
+// many all channels and parts (8192 rows of 5 parts: 13 us, 17 the other way).  Outputs change places in shared memory so
+// that they leave as whole rows.
+template <int HD, bool BF, int MINE, int COLS, int PARTS>
+__global__ void __launch_bounds__(COLS * PARTS * 32) kv16_join_kernel(const KAArgs a) {
+  constexpr int PIECES = MINE * COLS;
+  __shared__ uint2 out[32][PIECES + 1];
+  __shared__ float4 other[PARTS > 1 ? PARTS - 1 : 1][PARTS > 1 ? MINE : 1][COLS][32];
+  __shared__ float most[PARTS][32], sums[PARTS][32];
+  __shared__ int64_t to[32];
+  const N730KV16Cache& c = a.c;
+  const int lane = threadIdx.x & 31, col = (threadIdx.x >> 5) % COLS, turn = threadIdx.x / (COLS * 32);
+  const int G = a.group, cap = c.max_pages * c.page_size, h = blockIdx.y, piece = blockIdx.z * PIECES + col * MINE;
+  const int64_t r = (int64_t)blockIdx.x * 32 + lane, rows = (int64_t)a.batch * a.tokens * G;  // row of the KV head
+  bool live = r < rows;
+  const int tok = live ? (int)a.by_group.div((uint32_t)r) : 0, g = (int)(r - (int64_t)tok * G);
+  const int b = (int)a.by_tokens.div(tok), t = tok - b * a.tokens;
+  const int n_new = live ? kv8_new(a.n_new, b, a.tokens) : 0;
+  live = live && t < n_new;
+  // the shares of the row's positions: the last row of its tile decides
+  const int np = live && a.pre.o ? ka_used(kv16_prefix(c), a.pre.splits) : 0;
+  const int f = t * G + g, f0 = f / a.own.tile_rows * a.own.tile_rows;
+  const int last = live ? (int)a.by_group.div(min(f0 + a.own.tile_rows, n_new * G) - 1) : 0;
+  const int no = live ? ka_used(min(kv8_len(a.lens, b, cap) + last + 1, cap), a.own.splits) : 0;
+  const int64_t p0 = (int64_t)h * a.pre.splits, o0 = (int64_t)(b * c.n_kv + h) * a.own.splits;
+  const int n = np + no;  // parts: the prefix's, then the own ones
+  pdl_wait();
+  float big = -INFINITY, sum = 0.f;
+#pragma unroll 4
+  for (int i = turn; i < n; i += PARTS)
+    big = fmaxf(big, (i < np ? a.pre.ml[(p0 + i) * a.pre.rows + r] : a.own.ml[(o0 + i - np) * a.own.rows + f]).x);
+  if (col == 0) most[turn][lane] = big;
+  __syncthreads();
 #pragma unroll
-  for (int e = 0; e < V / 2; ++e) y[e] = ka_pack<BF>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-  if (a.ovec) {
-    if (V == 4) *reinterpret_cast<uint2*>(out) = make_uint2(y[0], y[V / 2 - 1]);
-    else *reinterpret_cast<uint32_t*>(out) = y[0];
-  } else {
+  for (int k = 0; k < PARTS; ++k) big = fmaxf(big, most[k][lane]);
+  float4 acc[MINE];
 #pragma unroll
-    for (int e = 0; e < V; ++e) out[e] = (uint16_t)(y[e / 2] >> (16 * (e & 1)));
+  for (int e = 0; e < MINE; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = turn; i < n; i += PARTS) {
+    const bool of_prefix = i < np;
+    const KAParts& part = of_prefix ? a.pre : a.own;
+    const int64_t unit = of_prefix ? p0 + i : o0 + i - np, row = of_prefix ? r : f;
+    const float2 ml = part.ml[unit * part.rows + row];
+    const float4* src = part.o + (unit * (HD / 4) + piece) * part.rows + row;
+    const float w = ml.x == -INFINITY ? 0.f : ex2(ml.x - big);
+    sum += ml.y == 0.f ? 0.f : ml.y * w;  // a part without a seen position has no sum either; a NaN stays one
+#pragma unroll
+    for (int e = 0; e < MINE; ++e) {
+      const float4 x = src[(int64_t)e * part.rows];
+      acc[e].x = fmaf(w, x.x, acc[e].x); acc[e].y = fmaf(w, x.y, acc[e].y);
+      acc[e].z = fmaf(w, x.z, acc[e].z); acc[e].w = fmaf(w, x.w, acc[e].w);
+    }
+  }
+  if (PARTS > 1 && turn) {
+#pragma unroll
+    for (int e = 0; e < MINE; ++e) other[turn - 1][e][col][lane] = acc[e];
+  }
+  if (col == 0) sums[turn][lane] = sum;
+  if (threadIdx.x < 32) to[lane] = live ? (int64_t)tok * a.ldo + (int64_t)(h * G + g) * HD + blockIdx.z * (PIECES * 4) : -1;
+  __syncthreads();
+  if (!turn) {
+#pragma unroll
+    for (int k = 1; k < PARTS; ++k) {
+      sum += sums[k][lane];
+#pragma unroll
+      for (int e = 0; e < MINE; ++e) {
+        const float4 x = other[k - 1][e][col][lane];
+        acc[e] = make_float4(acc[e].x + x.x, acc[e].y + x.y, acc[e].z + x.z, acc[e].w + x.w);
+      }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int e = 0; e < MINE; ++e)
+      out[lane][col * MINE + e] = make_uint2(ka_pack<BF>(acc[e].x * inv, acc[e].y * inv), ka_pack<BF>(acc[e].z * inv, acc[e].w * inv));
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * PIECES; i += COLS * PARTS * 32) {
+    const int row = i / PIECES, e = i % PIECES;
+    if (to[row] < 0) continue;
+    uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + to[row] + e * 4;
+    const uint2 y = out[row][e];
+    if (a.ovec) {
+      *reinterpret_cast<uint2*>(dst) = y;
+    } else {
+      dst[0] = (uint16_t)y.x; dst[1] = (uint16_t)(y.x >> 16); dst[2] = (uint16_t)y.y; dst[3] = (uint16_t)(y.y >> 16);
+    }
   }
 }
 
 // ----------------------------------------------------------------------------- plan
+constexpr int KO_ROWS = 16;        // query rows of a KV head that the own kernel takes at most
 struct KAPlan {
-  int pre_nt, own_nt;              // row tiles of a CTA
-  int pre_tiles, pre_splits, own_tiles, own_splits;
+  int pre_nt, own_nt;              // row tiles of a CTA; own_nt 0: the kernel for single tokens
+  int pre_tiles, pre_splits, own_tiles, own_splits, own_rows;
   int64_t pre_items, own_items;
   int64_t pre_o, pre_ml, own_o, own_ml, bytes;  // in the workspace
 };
@@ -568,19 +781,18 @@ struct KAPlan {
 static KAPlan ka_plan(const N730KV16Cache& c, int batch, int tokens, int heads) {
   KAPlan p{};
   const int G = heads / c.n_kv, sms = num_sms();
-  const int64_t pre_rows = (int64_t)batch * tokens * G, own_rows = (int64_t)tokens * G;
-  auto cells = [&](int64_t tiles, int splits) { return tiles * splits; };
+  const int64_t pre_rows = (int64_t)batch * tokens * G, own_rows = (int64_t)tokens * G, own_units = (int64_t)batch * c.n_kv;
   auto shape = [&](int64_t rows, int64_t units, int64_t positions, int& nt, int& tiles, int& splits) {
     nt = rows > 128 ? 2 : 1;
     tiles = (int)((rows + nt * 128 - 1) / (nt * 128));
     const int64_t items = units * tiles, slots = (int64_t)sms * (nt == 1 ? 2 : 1);
     const int64_t pos = (positions + KA_KEYS - 1) / KA_KEYS;
-    // a share's time: its tiles and what it costs to begin and end; the parts' way through memory
+    // a share's time in us: its tiles and what it costs to begin and end; the parts' way through memory
     double best = 1e30;
     splits = 1;
     for (int s = 1; s <= std::min<int64_t>(pos, 64); ++s) {
       const double waves = (double)((items * s + slots - 1) / slots);
-      const double us = waves * ((double)((pos + s - 1) / s) * 1.2 + 3.0) + (double)(s > 1 ? s : 0) * units * rows * c.head_dim * 8 / 4e6;
+      const double us = waves * ((double)((pos + s - 1) / s) * 1.9 + 4.5) + s * 0.15 + (double)s * units * rows * c.head_dim * 8 / 6e6;
       if (us < best * 0.98) { best = us; splits = s; }
     }
   };
@@ -588,12 +800,22 @@ static KAPlan ka_plan(const N730KV16Cache& c, int batch, int tokens, int heads) 
     shape(pre_rows, c.n_kv, (int64_t)c.prefix_pages * c.page_size, p.pre_nt, p.pre_tiles, p.pre_splits);
     p.pre_items = (int64_t)c.n_kv * p.pre_tiles * p.pre_splits;
   }
-  shape(own_rows, (int64_t)batch * c.n_kv, (int64_t)c.max_pages * c.page_size, p.own_nt, p.own_tiles, p.own_splits);
-  p.own_items = (int64_t)batch * c.n_kv * p.own_tiles * p.own_splits;
+  const int64_t cap = (int64_t)c.max_pages * c.page_size;
+  shape(own_rows, own_units, cap, p.own_nt, p.own_tiles, p.own_splits);
+  p.own_rows = p.own_tiles * p.own_nt * 128;
+  // single tokens: a warp each where that fills a share of the SMs, in one grid with the prefix's items otherwise (one launch
+  // less)
+  if (tokens == 1 && G <= KO_ROWS && own_units >= sms / 4) {
+    p.own_nt = 0;
+    p.own_tiles = 1;
+    p.own_rows = KO_ROWS;
+    p.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({(cap + KA_KEYS - 1) / KA_KEYS, 8ll * sms / own_units, 32}));
+  }
+  p.own_items = own_units * p.own_tiles * p.own_splits;
   auto room = [&](int64_t bytes) { const int64_t at = p.bytes; p.bytes += (bytes + 255) / 256 * 256; return at; };
   room(256);
-  const int64_t pr = cells(p.pre_tiles, p.pre_splits) * p.pre_nt * 128 * c.n_kv;
-  const int64_t orows = cells(p.own_tiles, p.own_splits) * p.own_nt * 128 * c.n_kv * batch;
+  const int64_t pr = (int64_t)p.pre_tiles * p.pre_splits * p.pre_nt * 128 * c.n_kv;
+  const int64_t orows = own_units * p.own_splits * p.own_rows;
   p.pre_o = room(pr * c.head_dim * 4);
   p.pre_ml = room(pr * 8);
   p.own_o = room(orows * c.head_dim * 4);
@@ -655,14 +877,23 @@ static int ka_launch(KAArgs& a, const KAPlan& p, const CUtensorMap& km, const CU
     return nt == 1 ? ka_launch_one<HD, BF, 1>(a, km, vm, pre + own, pdl, st) : ka_launch_one<HD, BF, 2>(a, km, vm, pre + own, pdl, st);
   };
   // items of the same shape in one grid, the prefix's (longer) first; otherwise the own ones' grid follows on its heels
-  if (!p.pre_items || p.pre_nt == p.own_nt) {
+  if (p.own_nt == 0) {
+    if (p.pre_items)
+      if (int rc = one(p.pre_nt, p.pre_items, 0, false)) return rc;
+    const int smem = KOCfg<HD>::STAGE * KOCfg<HD>::STAGES;
+    auto own = [&](auto kernel) { return kv8_launch(kernel, dim3((unsigned)p.own_items), dim3(32), smem, st, p.pre_items > 0, a); };
+    if (int rc = a.group <= 8 ? own(kv16_own_kernel<HD, BF, 1>) : own(kv16_own_kernel<HD, BF, 2>)) return rc;
+  } else if (!p.pre_items || p.pre_nt == p.own_nt) {
     if (int rc = one(p.own_nt, p.pre_items, p.own_items, false)) return rc;
   } else {
     if (int rc = one(p.pre_nt, p.pre_items, 0, false)) return rc;
     if (int rc = one(p.own_nt, 0, p.own_items, true)) return rc;
   }
-  const int64_t rows = (int64_t)a.batch * a.tokens * a.heads;
-  return kv8_launch(kv16_join_kernel<HD, BF>, dim3((unsigned)((rows + KJ_WARPS - 1) / KJ_WARPS)), dim3(KJ_WARPS * 32), 0, st, true, a);
+  const int64_t rows = (int64_t)a.batch * a.tokens * a.group;
+  const unsigned blocks = (unsigned)((rows + 31) / 32);
+  if ((int64_t)blocks * a.c.n_kv >= num_sms())
+    return kv8_launch(kv16_join_kernel<HD, BF, 4, HD / 16, 1>, dim3(blocks, a.c.n_kv), dim3(HD / 16 * 32), 0, st, true, a);
+  return kv8_launch(kv16_join_kernel<HD, BF, 2, 4, 4>, dim3(blocks, a.c.n_kv, HD / 32), dim3(512), 0, st, true, a);
 }
 
 }  // namespace n730
@@ -705,10 +936,12 @@ N730_API int n730_kv16_attention(const N730KV16Cache* c, const void* d_q, int64_
   a.lens = d_lens; a.n_new = d_new;
   a.status = reinterpret_cast<int*>(ws);
   if (p.pre_items)
-    a.pre = KAParts{p.pre_tiles, p.pre_splits, p.pre_tiles * p.pre_nt * 128, reinterpret_cast<float*>(ws + p.pre_o),
+    a.pre = KAParts{p.pre_tiles, p.pre_splits, p.pre_tiles * p.pre_nt * 128, p.pre_nt * 128, reinterpret_cast<float4*>(ws + p.pre_o),
                     reinterpret_cast<float2*>(ws + p.pre_ml)};
-  a.own = KAParts{p.own_tiles, p.own_splits, p.own_tiles * p.own_nt * 128, reinterpret_cast<float*>(ws + p.own_o),
+  a.own = KAParts{p.own_tiles, p.own_splits, p.own_rows, p.own_nt ? p.own_nt * 128 : KO_ROWS, reinterpret_cast<float4*>(ws + p.own_o),
                   reinterpret_cast<float2*>(ws + p.own_ml)};
+  a.by_group = FastDiv(a.group);
+  a.by_tokens = FastDiv(tokens);
   CUtensorMap km, vm;
   int rc = ka_map(*c, c->k, a.box, &km);
   if (!rc) rc = ka_map(*c, c->v, a.box, &vm);

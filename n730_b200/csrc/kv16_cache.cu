@@ -43,17 +43,6 @@ constexpr int RO_ROWS = 16;      // most rows of a CTA
 constexpr int RO_V = 8;          // channels of a vector unit
 constexpr int64_t RO_TABLE = 40 * 1024;  // bytes of a CTA's cosines and sines
 
-// n / d for n < 2^31 by a product: integer divisions by what a launch gives took a third of the kernel's time
-struct FastDiv {
-  uint32_t d, m, s;
-  FastDiv() = default;
-  explicit FastDiv(uint32_t x) : d(x), s(0) {
-    while ((1ull << s) < x) ++s;
-    m = (uint32_t)((((1ull << s) - x) << 32) / x + 1);
-  }
-  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }
-};
-
 // One group of heads of a row: where it is read, and where it goes.
 struct RotaryPart {
   const void* x; void* y;  // y null: into the cache's pool
