@@ -230,6 +230,29 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
   const int j0 = (int)((int64_t)all_tiles * split / used), nt = (int)((int64_t)all_tiles * (split + 1) / used) - j0;
   const int* table = pre ? c.prefix_table : c.block_table + (int64_t)b * c.max_pages;
 
+  // the queries are asked for first: 16 rows of a softmax warp, 16 bytes a lane
+  constexpr int QR = 32 / (HD / 8), QU = 16 / QR;  // rows an instruction, instructions
+  const int qsub = lane / (HD / 8), qch = lane % (HD / 8);
+  // where row f of the item lies: its token's row, its head
+  auto query = [&](int f) {
+    const int t = (int)a.by_group.div(f);
+    return (int64_t)((pre ? 0 : b * a.tokens) + t) * a.ldq + (int64_t)(h * G + f - t * G) * HD;
+  };
+  uint4 qx[QU];
+  if (warp < NT * 8) {
+#pragma unroll
+    for (int u = 0; u < QU; ++u) {
+      const int r = warp * 16 + u * QR + qsub;
+      qx[u] = make_uint4(0, 0, 0, 0);
+      if (r >= nrow) continue;
+      const uint16_t* p = reinterpret_cast<const uint16_t*>(a.q) + query(f0 + r) + qch * 8;
+      if (a.qvec) qx[u] = *reinterpret_cast<const uint4*>(p);
+      else qx[u] = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
+    }
+  } else if (warp == Cfg::COPY_WARP && lane == 0) {
+    asm volatile("prefetch.tensormap [%0];" :: "l"(reinterpret_cast<uint64_t>(&kmap)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" :: "l"(reinterpret_cast<uint64_t>(&vmap)) : "memory");
+  }
   if (tid == 0) {
     mbar_init(&sm.qready, NT * 8);
     for (int s = 0; s < 2; ++s) {
@@ -356,36 +379,15 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
     }
   } else {
     // ---------------- softmax: two threads a row, 64 positions of a tile each ----------------
-    const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q);
-    // where row f of the item lies: its token's row, its head
-    auto token = [&](int f) { return (pre ? 0 : b * a.tokens) + (int)a.by_group.div(f); };
-    auto query = [&](int f) { return (int64_t)token(f) * a.ldq + (int64_t)(h * G + f - (int)a.by_group.div(f) * G) * HD; };
-    {
-      constexpr int LPR = HD / 8, RPI = 32 / LPR, U = 16 / RPI;  // all of the warp's 16 rows at once
-      const int sub = lane / LPR, ch = lane % LPR;
-      const int r0 = warp * 16;
-      {
-        uint4 x[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int r = r0 + u * RPI + sub, f = f0 + r;
-          x[u] = make_uint4(0, 0, 0, 0);
-          if (r >= nrow) continue;
-          const uint16_t* p = q + query(f) + ch * 8;
-          if (a.qvec) x[u] = *reinterpret_cast<const uint4*>(p);
-          else x[u] = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int r = r0 + u * RPI + sub;
-          *reinterpret_cast<uint4*>(sm.q + (ch >> 3) * Cfg::QB + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) =
-              make_uint4(x[u].x ^ a.sign, x[u].y ^ a.sign, x[u].z ^ a.sign, x[u].w ^ a.sign);
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive1(&sm.qready);
+    for (int u = 0; u < QU; ++u) {
+      const int r = warp * 16 + u * QR + qsub;
+      *reinterpret_cast<uint4*>(sm.q + (qch >> 3) * Cfg::QB + r * 128 + (((qch & 7) ^ (r & 7)) << 4)) =
+          make_uint4(qx[u].x ^ a.sign, qx[u].y ^ a.sign, qx[u].z ^ a.sign, qx[u].w ^ a.sign);
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) mbar_arrive1(&sm.qready);
     const int x = warp >> 3, half = warp >> 2 & 1, wq = warp & 3, r = x * 128 + wq * 32 + lane, f = f0 + r;
     const bool live = r < nrow, some_live = x * 128 + wq * 32 < nrow;
     const int vis = !live ? 0 : pre ? sees : min(L + (int)a.by_group.div(f) + 1, cap);
