@@ -496,8 +496,8 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
   if (blockIdx.x == 0) pdl_wait();  // the kernel behind this one waits for it alone, and so for the one before
 }
 
-// Attention of single tokens over their own positions: a warp an item (sequence, KV head, share of the positions), its G
-// query rows (up to 8 NB) against 16 positions at a time.  Positions, and then channels, are the products' 16 rows and the
+// Attention of single tokens and drafts over their own positions: a warp an item (sequence, KV head, 8 NB of its query rows,
+// share of the positions), 16 positions at a time.  Positions, and then channels, are the products' 16 rows and the
 // queries their columns (mma.m16n8k16): S^T = K Q^T, O^T += V^T P^T, so that nothing is spent on the 128 rows that a
 // tensor-memory tile would have; with single tokens this is bound by the bytes of K and V.  P^T's fragments are those of
 // S^T transposed, 8 x 8 at a time, in registers.  Rows arrive by asynchronous copies, three blocks of 16 positions deep;
@@ -537,10 +537,14 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
   const N730KV16Cache& c = a.c;
   const int lane = threadIdx.x, G = a.group, cap = c.max_pages * c.page_size;
   int i = (int)blockIdx.x;
+  const int f0 = i % a.own.tiles * a.own.tile_rows;  // the first of its rows
+  i /= a.own.tiles;
   const int h = i % c.n_kv;
   i /= c.n_kv;
   const int b = i % a.batch, split = i / a.batch;
-  const int sees = kv8_new(a.n_new, b, 1) ? min(kv8_len(a.lens, b, cap) + 1, cap) : 0;
+  const int L = kv8_len(a.lens, b, cap), nrow = min(8 * NB, kv8_new(a.n_new, b, a.tokens) * G - f0);
+  auto vis_of = [&](int f) { return min(L + (int)a.by_group.div(f) + 1, cap); };
+  const int sees = nrow > 0 ? vis_of(f0 + nrow - 1) : 0, sees_all = vis_of(f0);  // of any row, of every one
   const int used = ka_used(sees, a.own.splits);
   pdl_launch_dependents();
   if (split < used) {
@@ -574,17 +578,24 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
     page = page_of(2);
     // the queries as the products' columns: row lane / 4 (+ 8), channels 16 k + 2 (lane % 4) (+ 8)
     uint32_t q[NB][KS][2];
-    const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)b * a.ldq + (int64_t)h * G * HD + (lane & 3) * 2;
 #pragma unroll
-    for (int y = 0; y < NB; ++y)
+    for (int y = 0; y < NB; ++y) {
+      const int r = y * 8 + (lane >> 2), t = (int)a.by_group.div(f0 + r);
+      const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(b * a.tokens + t) * a.ldq +
+                           (int64_t)(h * G + f0 + r - t * G) * HD + (lane & 3) * 2;
 #pragma unroll
       for (int k = 0; k < KS; ++k)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int r = y * 8 + (lane >> 2);
-          const uint16_t* at = qp + r * HD + k * 16 + e * 8;
-          q[y][k][e] = r >= G ? 0u : (a.qvec ? *reinterpret_cast<const uint32_t*>(at) : at[0] | (uint32_t)at[1] << 16) ^ a.sign;
+          const uint16_t* at = qp + k * 16 + e * 8;
+          q[y][k][e] = r >= nrow ? 0u : (a.qvec ? *reinterpret_cast<const uint32_t*>(at) : at[0] | (uint32_t)at[1] << 16) ^ a.sign;
         }
+    }
+    int vis[NB][2];  // of the rows whose scores this lane holds
+#pragma unroll
+    for (int y = 0; y < NB; ++y)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) vis[y][e] = vis_of(min(f0 + y * 8 + (lane & 3) * 2 + e, f0 + nrow - 1));
     float o[NB][KS][4] = {}, m[NB][2], l[NB][2] = {};
 #pragma unroll
     for (int y = 0; y < NB; ++y) m[y][0] = m[y][1] = -INFINITY;
@@ -609,14 +620,15 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
         for (int y = 0; y < NB; ++y) ko_mma<BF>(x[y], f, q[y][k][0], q[y][k][1]);
       }
       uint32_t w[NB][2];
+      float e4[NB][4];
 #pragma unroll
       for (int y = 0; y < NB; ++y) {
         float big[2];
         const int p = p0 + (lane >> 2);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          x[y][e] = p < sees ? x[y][e] * a.scale_log2e : -INFINITY;
-          x[y][2 + e] = p + 8 < sees ? x[y][2 + e] * a.scale_log2e : -INFINITY;
+          x[y][e] = p < vis[y][e] ? x[y][e] * a.scale_log2e : -INFINITY;
+          x[y][2 + e] = p + 8 < vis[y][e] ? x[y][2 + e] * a.scale_log2e : -INFINITY;
           big[e] = fmaxf(x[y][e], x[y][2 + e]);
         }
 #pragma unroll
@@ -637,15 +649,45 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[y][k][e] *= f[e & 1];
         }
-        float e4[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float ms = m[y][e & 1] == -INFINITY ? 0.f : m[y][e & 1];
-          e4[e] = ex2(x[y][e] - ms);
-          l[y][e & 1] += e4[e];
+          e4[y][e] = ex2(x[y][e] - ms);
+          l[y][e & 1] += e4[y][e];
         }
-        w[y][0] = ko_transpose(ka_pack<BF>(e4[0], e4[1]));
-        w[y][1] = ko_transpose(ka_pack<BF>(e4[2], e4[3]));
+        w[y][0] = ko_transpose(ka_pack<BF>(e4[y][0], e4[y][1]));
+        w[y][1] = ko_transpose(ka_pack<BF>(e4[y][2], e4[y][3]));
+      }
+      if (p0 + 16 > sees_all && sees > sees_all) {
+        // rows of V that some of the rows do not see: zeroed where not finite, added by the rows that see them
+        const uint32_t inf = BF ? 0x7f80u : 0x7c00u;
+#pragma unroll 1
+        for (int p = max(sees_all, p0); p < min(sees, p0 + 16); ++p) {
+          uint8_t* row = ko_smem + s * Cfg::STAGE + Cfg::KB + (p - p0) * (HD * 2);
+          uint32_t bad = 0;
+          for (int e = lane; e < HD / 2; e += 32) {
+            const uint32_t y = *reinterpret_cast<const uint32_t*>(row + e * 4);
+            bad |= (y & inf) == inf || (y >> 16 & inf) == inf;
+          }
+          if (!__any_sync(0xffffffffu, bad)) continue;
+          for (int e = lane; e < HD / 2; e += 32) *reinterpret_cast<uint32_t*>(row + e * 4) = 0u;
+          const int pg = table[p / c.page_size];
+          const int64_t at = (((int64_t)pg * c.n_kv + h) * c.page_size + p % c.page_size) * HD + (lane >> 2);
+          const int from = ((p - p0) & 7) * 4 + (lane & 3);
+#pragma unroll
+          for (int y = 0; y < NB; ++y)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float lo = __shfl_sync(0xffffffffu, e4[y][e], from), hi = __shfl_sync(0xffffffffu, e4[y][2 + e], from);
+              if (p >= vis[y][e]) continue;
+#pragma unroll
+              for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                  o[y][k][2 * u + e] = fmaf(p - p0 < 8 ? lo : hi, kv8_load1(c.v, at + k * 16 + u * 8, c.dtype), o[y][k][2 * u + e]);
+            }
+        }
+        __syncwarp();
       }
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
@@ -665,14 +707,14 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[y][e] += __shfl_xor_sync(0xffffffffu, l[y][e], d);
         const int r = y * 8 + (lane & 3) * 2 + e;
-        if (r >= G) continue;
-        if (lane < 4) a.own.ml[unit * a.own.rows + r] = make_float2(m[y][e], l[y][e]);
+        if (r >= nrow) continue;
+        if (lane < 4) a.own.ml[unit * a.own.rows + f0 + r] = make_float2(m[y][e], l[y][e]);
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int ch = k * 16 + u * 8 + (lane >> 2);
-            dst[((int64_t)(ch >> 2) * a.own.rows + r) * 4 + (ch & 3)] = o[y][k][2 * u + e];
+            dst[((int64_t)(ch >> 2) * a.own.rows + f0 + r) * 4 + (ch & 3)] = o[y][k][2 * u + e];
           }
       }
   }
@@ -772,7 +814,7 @@ __global__ void __launch_bounds__(COLS * PARTS * 32) kv16_join_kernel(const KAAr
 }
 
 // ----------------------------------------------------------------------------- plan
-constexpr int KO_ROWS = 16;        // query rows of a KV head that the own kernel takes at most
+constexpr int KO_ROWS = 16, KO_MOST = 64;  // query rows of a KV head that a warp of the own kernel takes, and that it is used for
 struct KAPlan {
   int pre_nt, own_nt;              // row tiles of a CTA; own_nt 0: the kernel for single tokens
   int pre_tiles, pre_splits, own_tiles, own_splits, own_rows;
@@ -805,13 +847,12 @@ static KAPlan ka_plan(const N730KV16Cache& c, int batch, int tokens, int heads) 
   const int64_t cap = (int64_t)c.max_pages * c.page_size;
   shape(own_rows, own_units, cap, p.own_nt, p.own_tiles, p.own_splits);
   p.own_rows = p.own_tiles * p.own_nt * 128;
-  // single tokens: a warp each where that fills a share of the SMs, in one grid with the prefix's items otherwise (one launch
-  // less)
-  if (tokens == 1 && G <= KO_ROWS && own_units >= sms / 4) {
+  // few rows: warps of 16 where they fill a share of the SMs, in one grid with the prefix's items otherwise (one launch less)
+  if (own_rows <= KO_MOST && own_units >= sms / 4) {
     p.own_nt = 0;
-    p.own_tiles = 1;
-    p.own_rows = KO_ROWS;
-    p.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({(cap + KA_KEYS - 1) / KA_KEYS, 8ll * sms / own_units, 32}));
+    p.own_tiles = (int)((own_rows + KO_ROWS - 1) / KO_ROWS);
+    p.own_rows = p.own_tiles * KO_ROWS;
+    p.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({(cap + KA_KEYS - 1) / KA_KEYS, 8ll * sms / (own_units * p.own_tiles), 32}));
   }
   p.own_items = own_units * p.own_tiles * p.own_splits;
   auto room = [&](int64_t bytes) { const int64_t at = p.bytes; p.bytes += (bytes + 255) / 256 * 256; return at; };
@@ -884,7 +925,7 @@ static int ka_launch(KAArgs& a, const KAPlan& p, const CUtensorMap& km, const CU
       if (int rc = one(p.pre_nt, p.pre_items, 0, false)) return rc;
     const int smem = KOCfg<HD>::STAGE * KOCfg<HD>::STAGES;
     auto own = [&](auto kernel) { return kv8_launch(kernel, dim3((unsigned)p.own_items), dim3(32), smem, st, p.pre_items > 0, a); };
-    if (int rc = a.group <= 8 ? own(kv16_own_kernel<HD, BF, 1>) : own(kv16_own_kernel<HD, BF, 2>)) return rc;
+    if (int rc = a.group * a.tokens <= 8 ? own(kv16_own_kernel<HD, BF, 1>) : own(kv16_own_kernel<HD, BF, 2>)) return rc;
   } else if (!p.pre_items || p.pre_nt == p.own_nt) {
     if (int rc = one(p.own_nt, p.pre_items, p.own_items, false)) return rc;
   } else {

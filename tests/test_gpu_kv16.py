@@ -425,3 +425,47 @@ def test_step_in_a_graph():
             near(io["out"].float().cpu().numpy().reshape(q.shape), *d.ref.attention(q, n, [1] * B, D ** -0.5))
             assert int(ws[:4].view(t.int32)[0]) == 0
             lens += 1
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("T,heads,dim,page", [(1, 8, 64, 64), (3, 14, 64, 16), (1, 32, 128, 48), (5, 14, 128, 64), (4, 32, 64, 32)])
+def test_attention_many_sequences(dtype, T, heads, dim, page):
+    """Enough sequences that each one's own part is a warp's: stale memory, pages that are none, ragged counts."""
+    rng = np.random.default_rng(T * heads + page)
+    B, kv, prefix = 24, 2, 70
+    ref = Cache(B, -(-150 // page), -(-prefix // page), prefix, kv, dim, page, dtype, rng, fill=np.nan)
+    lens, new = rng.integers(0, 140, B), rng.integers(0, T + 1, B)
+    lens[:4] = 0, 15, 16, 127
+    for ids, n in [(ref.prefix_table, prefix)] + [(ref.table[b], lens[b] + new[b]) for b in range(B)]:
+        for p in range(n):
+            pg, off = ref.slot(ids, p)
+            ref.k[pg, :, off], ref.v[pg, :, off] = rounded(rng.standard_normal((2, kv, dim)), dtype)
+    ref.table[5:9, 0], ref.table[9, -1] = -1, ref.n_pages
+    check(OnDevice(ref), rng.standard_normal((B, T, heads, dim)), lens, new)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("T,heads", [(6, 4), (5, 14)])
+def test_attention_many_sequences_future_values(dtype, T, heads):
+    """The same where rows that later tokens of the call see are not finite."""
+    rng = np.random.default_rng(T + heads)
+    B, kv, dim = 20, 2, 64
+    ref = Cache(B, 3, 1, 40, kv, dim, 64, dtype, rng)
+    lens = rng.integers(0, 180 - T, B)
+    lens[:3] = 0, 62, 126
+    for b in range(0, B, 2):
+        for t, what in ((2, np.nan), (4, np.inf)):
+            pg, off = ref.slot(ref.table[b], lens[b] + t)
+            ref.v[pg, :, off, ::3] = what
+    d = OnDevice(ref)
+    q = rng.standard_normal((B, T, heads, dim))
+    got = attend(d, q, lens, None)
+    clean = Cache.__new__(Cache)
+    clean.__dict__ = dict(ref.__dict__, v=np.nan_to_num(ref.v, posinf=0, neginf=0))
+    want, bound = clean.attention(rounded(q, dtype), lens, [T] * B, dim ** -0.5)
+    for b in range(B):
+        n = 2 if b % 2 == 0 else T
+        near(got[b, :n], want[b, :n], bound[b, :n], f"sequence {b}")
+        if b % 2 == 0:
+            assert not np.isfinite(got[b, 2:, :, ::3]).any() and np.isfinite(got[b, 2:, :, 1::3]).all()
+            near(got[b, 2:, :, 1::3], want[b, 2:, :, 1::3], bound[b, 2:, :, 1::3], f"sequence {b}, other channels")
