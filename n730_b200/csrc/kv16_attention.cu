@@ -551,31 +551,43 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
     const int blocks = (sees + 15) / 16, i0 = (int)((int64_t)blocks * split / used), n = (int)((int64_t)blocks * (split + 1) / used) - i0;
     const int* table = c.block_table + (int64_t)b * c.max_pages;
     const uint32_t base = smem_u32(ko_smem);
-    // block j of the share: its page, asked for a block ahead
-    auto page_of = [&](int j) { return j < n ? table[(i0 + j) * 16 / c.page_size] : -1; };
+    // the share's blocks in order: the page of the next one to be fetched is known by then, asked for a block ahead
+    int at_page = i0 * 16 / c.page_size, at_off = i0 * 16 - at_page * c.page_size, left = n;
+    auto next_page = [&] {
+      const int page = left > 0 ? table[at_page] : -1;
+      --left;
+      return page;
+    };
     uint32_t here = 0;  // bit s: the block in stage s has a page
     const int piece = lane % CH, row0 = lane / CH;
+    uint32_t to[16 * CH / 32];  // where this lane's 16 bytes of its rows go
+#pragma unroll
+    for (int u = 0; u < 16 * CH / 32; ++u) {
+      const int r = row0 + u * (32 / CH);
+      to[u] = base + r * (HD * 2) + ((piece ^ (r & 7)) << 4);
+    }
     auto fetch = [&](int j, int page, int s) {
       const bool ok = (unsigned)page < (unsigned)c.n_pages;
       here = ok ? here | 1u << s : here & ~(1u << s);
       if (j < n) {
-        const int p0 = (i0 + j) * 16;
-        const int64_t src = ((int64_t)(ok ? page : 0) * c.n_kv + h) * c.page_size + p0 % c.page_size;
+        const int64_t at = ((int64_t)(((ok ? page : 0) * c.n_kv + h) * c.page_size + at_off) + row0) * HD + piece * 8;
+        const uint16_t* k = reinterpret_cast<const uint16_t*>(c.k) + at;
+        const uint16_t* v = reinterpret_cast<const uint16_t*>(c.v) + at;
+        const int rows = ok ? sees - (i0 + j) * 16 - row0 : 0;  // of this lane's; behind the last position: zeros
 #pragma unroll
-        for (int r = row0; r < 16; r += 32 / CH) {
-          const uint32_t bytes = ok && p0 + r < sees ? 16u : 0u;  // behind the last position: zeros
-          const int64_t at = (src + r) * HD + piece * 8;
-          const uint32_t dst = base + s * Cfg::STAGE + r * (HD * 2) + ((piece ^ (r & 7)) << 4);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(reinterpret_cast<const uint16_t*>(c.k) + at), "r"(bytes) : "memory");
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst + Cfg::KB), "l"(reinterpret_cast<const uint16_t*>(c.v) + at), "r"(bytes) : "memory");
+        for (int u = 0; u < 16 * CH / 32; ++u) {
+          const uint32_t bytes = u * (32 / CH) < rows ? 16u : 0u;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(to[u] + s * Cfg::STAGE), "l"(k + u * (32 / CH) * HD), "r"(bytes) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(to[u] + s * Cfg::STAGE + Cfg::KB), "l"(v + u * (32 / CH) * HD), "r"(bytes) : "memory");
         }
+        at_off += 16;
+        if (at_off == c.page_size) { at_off = 0; ++at_page; }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    int page = page_of(1);
-    fetch(0, page_of(0), 0);
-    fetch(1, page, 1);
-    page = page_of(2);
+    fetch(0, next_page(), 0);
+    fetch(1, next_page(), 1);
+    int page = next_page();
     // the queries as the products' columns: row lane / 4 (+ 8), channels 16 k + 2 (lane % 4) (+ 8)
     uint32_t q[NB][KS][2];
 #pragma unroll
@@ -602,22 +614,22 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
     // where this lane's rows of the four 8 x 8 pieces lie: K's by position and then channels, V's turned
     const int kr = lane & 15, kc = lane >> 4, vr = (lane & 7) + (lane >> 4) * 8, vc = lane >> 3 & 1;
 #pragma unroll 1
-    for (int j = 0; j < n; ++j) {
-      const int s = j % Cfg::STAGES, p0 = (i0 + j) * 16;
+    for (int j = 0, s = 0; j < n; ++j, s = s == Cfg::STAGES - 1 ? 0 : s + 1) {
+      const int p0 = (i0 + j) * 16;
       asm volatile("cp.async.wait_group 1;" ::: "memory");
       __syncwarp();  // everyone's rows are here, and everyone is through with the block before
       const bool ok = here >> s & 1;
-      fetch(j + 2, page, (j + 2) % Cfg::STAGES);
-      page = page_of(j + 3);
+      fetch(j + 2, page, s == 0 ? Cfg::STAGES - 1 : s - 1);
+      page = next_page();
       if (!ok) continue;
       const uint32_t kb = base + s * Cfg::STAGE, vb = kb + Cfg::KB;
-      float x[NB][4] = {};
+      float x[NB][4] = {}, x2[NB][4] = {};  // two sums: half as long a chain of products
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         uint32_t f[4];
         ko_load<false>(f, kb + kr * (HD * 2) + (((2 * k + kc) ^ (kr & 7)) << 4));
 #pragma unroll
-        for (int y = 0; y < NB; ++y) ko_mma<BF>(x[y], f, q[y][k][0], q[y][k][1]);
+        for (int y = 0; y < NB; ++y) ko_mma<BF>(k & 1 ? x2[y] : x[y], f, q[y][k][0], q[y][k][1]);
       }
       uint32_t w[NB][2];
       float e4[NB][4];
@@ -627,15 +639,15 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
         const int p = p0 + (lane >> 2);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          x[y][e] = p < vis[y][e] ? x[y][e] * a.scale_log2e : -INFINITY;
-          x[y][2 + e] = p + 8 < vis[y][e] ? x[y][2 + e] * a.scale_log2e : -INFINITY;
+          x[y][e] = p < vis[y][e] ? (x[y][e] + x2[y][e]) * a.scale_log2e : -INFINITY;
+          x[y][2 + e] = p + 8 < vis[y][e] ? (x[y][2 + e] + x2[y][2 + e]) * a.scale_log2e : -INFINITY;
           big[e] = fmaxf(x[y][e], x[y][2 + e]);
         }
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) big[e] = fmaxf(big[e], __shfl_xor_sync(0xffffffffu, big[e], d));
         if (__any_sync(0xffffffffu, big[0] > m[y][0] + KA_MOST || big[1] > m[y][1] + KA_MOST)) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) big[e] = fmaxf(big[e], __shfl_xor_sync(0xffffffffu, big[e], d));
           float f[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
@@ -814,7 +826,7 @@ __global__ void __launch_bounds__(COLS * PARTS * 32) kv16_join_kernel(const KAAr
 }
 
 // ----------------------------------------------------------------------------- plan
-constexpr int KO_ROWS = 16, KO_MOST = 64;  // query rows of a KV head that a warp of the own kernel takes, and that it is used for
+constexpr int KO_ROWS = 16, KO_MOST = 32;  // query rows of a KV head that a warp of the own kernel takes, and that it is used for
 struct KAPlan {
   int pre_nt, own_nt;              // row tiles of a CTA; own_nt 0: the kernel for single tokens
   int pre_tiles, pre_splits, own_tiles, own_splits, own_rows;
