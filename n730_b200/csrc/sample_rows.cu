@@ -15,10 +15,9 @@
 //      linear ones of max - l) that k of the threads' largest reach, 4096 of a long row: the first k tokens all lie up to
 //      there, and seldom many more.
 //   3. Rows of neither kind, or whose list is too long: a histogram of all tokens and their masses.  A bin's mass is
-//      w(edge) * sum of w / w(edge), the sum in fixed point; bins are narrow, so w / w(edge) is near 1 and fp32 holds its
-//      distance from 1 to 2^-24 of that.  Shared-memory atomics bound this pass, 10 cycles a warp's worth.  Flat rows take
-//      one, the distances beside the count in a word; where that is too coarse (rows that a few tokens have much of,
-//      crowded or wide bins), or likely to be (rows with a top-p), 43 bits of sum below 21 of count in two words.
+//      w(edge) * sum of w / w(edge), the sum in fixed point, 43 bits below 21 of count in two words; bins are narrow, so
+//      w / w(edge) is near 1 and fp32 holds its distance from 1 to 2^-24 of that.  (One word of 22 bits below 10 was no
+//      faster: shared-memory atomics cost 5 cycles a warp's worth, a token's arithmetic twice that.)
 //      Each prefix's end is then looked up in its bin: the bin's tokens are gathered and sorted, or, where they are too
 //      many (equal logits, coarse types), found by four rounds of 8 bits of the logit, after which the tokens left are
 //      equal and go by index.
@@ -34,15 +33,15 @@ namespace cg = cooperative_groups;
 
 constexpr int RS_CLUSTER = 8;      // CTAs of a row, one for rows of up to RS_ALONE logits: no exchange, 15 -> 10 us at 1000
 constexpr int RS_ALONE = 16384;
-// Threads of a CTA: 512 and all of an SM's registers while a row's CTAs find an SM each (one row of 152064: 12.8 us, 13.5
-// with 256), 256 and two CTAs an SM beyond that (64 rows with a top-k: 30 us, 60 with 512).
+// Threads of a CTA: 512 and all of an SM's registers while a row's CTAs find an SM each (one row of 152064 without a cut:
+// 23.5 us, 24.6 with 256), 256 beyond that and two CTAs an SM (64 rows with a top-k: 30 us, 60 with 512), three of 16-bit
+// logits, which shared memory has room for (192 rows without a cut: 150 us, 173 with two).
 constexpr int RS_THREADS_FEW = 512, RS_THREADS_MANY = 256;
 constexpr int RS_WARPS = RS_THREADS_FEW / 32;  // most warps
 constexpr int RS_BINS = 1536;      // as many as leave room for two CTAs of 19008 fp32 logits (a row of 152064) an SM
 constexpr int RS_CAP = 1024;       // tokens that are sorted at once
 constexpr int RS_COUNT = 160;      // lists up to this long are sorted by counting
-constexpr uint32_t RS_ROOM1 = 256, RS_ROOM2 = 4095;  // tokens of a CTA's bin that one word, and two, have room for
-constexpr uint32_t RS_FLAT = 65536;  // tokens from which a row is tried with one word: two cost shorter ones little
+constexpr uint32_t RS_ROOM = 4000;  // tokens of a CTA's bin that the sums have room for
 constexpr float RS_SPAN = 32.f;    // bins reach this many logits, or temperatures where that is more, below the largest
 constexpr size_t RS_STAGE_MAX = 160 * 1024;  // longest slice that is kept in shared memory
 
@@ -55,13 +54,13 @@ struct RSArgs {
   int* tokens; float* prob; int* kept;
 };
 
-// what the bins hold: nothing, threads' largest, all tokens, all tokens and their masses in one word or two
-enum { RS_NONE = 0, RS_LARGEST, RS_COUNTS, RS_ONE_WORD, RS_TWO_WORDS };
+// what the bins hold: nothing, threads' largest, all tokens, all tokens and their masses
+enum { RS_NONE = 0, RS_LARGEST, RS_COUNTS, RS_MASSES };
 enum { RS_DONE = 0, RS_FILL, RS_GATHER, RS_RADIX, RS_OVER, RS_FIND };
 struct RSCommand {
   int op, b0, b1;         // bins [b0, b1]
   int last;               // GATHER: nothing follows for the other CTAs
-  int mode, sure;         // FILL: what, tokens of a CTA's bin to have room for
+  int sure;               // FILL: tokens of a CTA's bin to have room for
   uint32_t prefix, shift; // RADIX: digits found, where the next one starts
   uint32_t key, skip;     // FIND: the skip-th token of this key
   double z0;              // RADIX: the bin's edge / T
@@ -86,8 +85,7 @@ struct RSSmem {
   RSStat wstat[RS_WARPS];
   double wsum[RS_WARPS];
   uint32_t wcnt[RS_WARPS];
-  uint32_t beyond[RS_CLUSTER], most[RS_CLUSTER];  // tokens behind the last bin; of a share's fullest bin, where it has no room
-  uint32_t own_beyond, own_most;
+  uint32_t most[RS_CLUSTER], own_most;  // tokens of a share's fullest bin, where it has no room for them
   double sel_base, sel_mass, pick_w;
   uint32_t n_list, n_mine, list_at, over, sel_cnt, sel_in, pick_cnt, occur;
   int bin_k, bin_p, pick, found, first;
@@ -120,21 +118,28 @@ __device__ __forceinline__ float rs_float(float x) { return x; }
 __device__ __forceinline__ float rs_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ float rs_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// A row's bins: bin = floor((max - l) * sx); edge(b), its upper end, is max - b * width as fp32 rounds it.
+// A row's bins: bin = floor((max - l) * sx); edge(b), its upper end, is max - b * width as fp32 rounds it.  A place is
+// off by `slack` bins where logits lie far from 0: bins are then not what their edges say, but their masses go by the edges
+// and stay right.
 struct RSGeom {
-  float mx, sx, width, inv_t;
+  float mx, sx, top, width, inv_t;  // top: max * sx
   double t;
+  bool far;                         // the largest logit is too large for products by sx, or infinite: logits go by their
+  float from;                       // distance from it, RS_LEAST at least
 };
-__device__ __forceinline__ float rs_place(float l, const RSGeom& g) { return (l == g.mx ? 0.f : g.mx - l) * g.sx; }
+constexpr float RS_LEAST = -3e38f, RS_FAR = 0x1p100f;
+__device__ __forceinline__ float rs_place(float l, const RSGeom& g) { return fmaf(-l, g.sx, g.top); }
 // NaN and -infinity have no place below RS_BINS
 __device__ __forceinline__ int rs_bin(float l, const RSGeom& g) {
   const float x = rs_place(l, g);
-  return x < (float)RS_BINS ? (int)x : RS_BINS;
+  return x < (float)RS_BINS ? max((int)x, 0) : RS_BINS;
 }
 __device__ __forceinline__ float rs_edge(float b, const RSGeom& g) { return fmaf(-b, g.width, g.mx); }
-__device__ __forceinline__ double rs_weight(float l, const RSGeom& g) {
-  return l == g.mx ? 1.0 : g.mx == INFINITY ? 0.0 : exp(((double)l - (double)g.mx) / g.t);
+__device__ __forceinline__ int rs_slack(const RSGeom& g) { return 1 + (int)fminf(fabsf(g.top) * 0x1p-22f, (float)RS_BINS); }
+__device__ __forceinline__ float rs_seen(float l, const RSGeom& g) {
+  return !g.far || !(l > -INFINITY) ? l : l == g.from ? 0.f : fmaxf(l - g.from, RS_LEAST);
 }
+__device__ __forceinline__ double rs_weight(float l, const RSGeom& g) { return l == g.mx ? 1.0 : exp(((double)l - (double)g.mx) / g.t); }
 
 // Exclusive scans over the block in thread order; the totals.
 template <int TH>
@@ -204,7 +209,7 @@ struct RSRow {
   int sure;              // tokens of a CTA's bin that two words are to have room for
 
   __device__ float raw(int i) const { return rs_float(STAGED ? stage[i] : row[i0 + i]); }
-  __device__ float get(int i) const { return rs_clean(raw(i)); }
+  __device__ float get(int i) const { return rs_seen(rs_clean(raw(i)), g); }
   // f(first index, V logits) over this CTA's, V = 16 bytes of them, NaN behind the last.
   template <class F>
   __device__ __forceinline__ void each(F f) const {
@@ -223,68 +228,55 @@ struct RSRow {
 #pragma unroll
         for (int j = 0; j < V; ++j) l[j] = i + j < n ? rs_float(row[i0 + i + j]) : NAN;
       }
+      if (g.far)
+#pragma unroll
+        for (int j = 0; j < V; ++j) l[j] = rs_seen(l[j], g);
       f(i, l);
     }
   }
 
-  // Units of a weight over its bin edge's: one word has 22 bits for RS_ROOM1 distances from 1, two have 43 for `sure`
-  // weights.
-  __device__ float unit_of(int mode) const {
-    if (mode == RS_ONE_WORD) return ldexpf(1.f, (int)floorf(14.f - log2f(fmaxf(expm1f(g.width * g.inv_t * 1.01f), 0x1p-20f))));
-    return ldexpf(1.f, 31 - (32 - __clz(sure / 4096)));
-  }
-  __device__ bool one_word() const { return g.mx < INFINITY && g.width * g.inv_t < 0x1p-4f; }
+  // Units of a weight over its bin edge's: 43 bits have room for `sure` of them.
+  __device__ float unit_of() const { return ldexpf(1.f, 31 - (32 - __clz(sure / 4001))); }
 
-  // Counts and sums of w / w(edge) by bin; in one word from the lower edge, so that the distance from 1 is not negative.
-  template <int MODE>
+  // Counts, and sums of w / w(edge), by bin.
+  template <bool MASSES>
   __device__ __forceinline__ void fill() {
-    const float unit = unit_of(MODE), down = MODE == RS_ONE_WORD ? 1.f : 0.f;
-    const bool narrow = MODE == RS_ONE_WORD || one_word();
-    uint32_t beyond = 0;
+    const float unit = unit_of();
+    const bool narrow = g.width * g.inv_t < 0x1p-4f;
     each([&](int, const float (&l)[V]) {
       int b[V], c[V];
+      uint32_t old[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float x = rs_place(l[j], g), f = __fadd_rd(x, 8388608.f);  // 2^23 + floor(x)
-        const bool in = x < (float)RS_BINS;
-        beyond += !in && l[j] > -INFINITY;
-        b[j] = in ? __float_as_int(f) & 0x7fffff : -1;
-        if (MODE == RS_COUNTS) continue;
+        const float x = fmaxf(rs_place(l[j], g), 0.f), f = __fadd_rd(x, 8388608.f);  // 2^23 + floor(x)
+        b[j] = l[j] > -INFINITY && x < (float)RS_BINS ? __float_as_int(f) & 0x7fffff : -1;
+        if (!MASSES) continue;
         // y = (l - edge) / T: the two are near, their difference is exact but for what is below 2^-24 of a bin
-        float y = (l[j] - rs_edge(f - 8388608.f + down, g)) * g.inv_t;
-        if (MODE == RS_ONE_WORD) y = fmaxf(y, 0.f);
-        else y = l[j] == g.mx ? 0.f : fminf(y, 0.f);
+        const float y = (l[j] - rs_edge(f - 8388608.f, g)) * g.inv_t;
         const float e = narrow ? y * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 1.f / 120, 1.f / 24), 1.f / 6), 0.5f), 1.f) : expm1f(y);
-        if (MODE == RS_ONE_WORD) c[j] = __float_as_int(fmaf(e, unit, 12582912.f)) - 0x4b400000;  // nearest, below 2^22
-        else c[j] = (int)((uint32_t)__float2int_rn(e * unit) + (uint32_t)unit);
+        c[j] = (int)((uint32_t)__float2int_rn(e * unit) + (uint32_t)unit);
       }
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         if (b[j] < 0) continue;
-        if (MODE == RS_COUNTS) {
-          atomicAdd(&s.cnt[b[j]], 1u);
-        } else if (MODE == RS_ONE_WORD) {
-          atomicAdd(&s.cnt[b[j]], (uint32_t)c[j] + (1u << 22));
-        } else {
-          const uint32_t old = atomicAdd(&s.low[b[j]], (uint32_t)c[j]);
-          atomicAdd(&s.cnt[b[j]], (1u << 11) + (old + (uint32_t)c[j] < old));
-        }
+        if (MASSES) old[j] = atomicAdd(&s.low[b[j]], (uint32_t)c[j]);
+        else atomicAdd(&s.cnt[b[j]], 1u << 11);
       }
+      if (MASSES)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (b[j] >= 0) atomicAdd(&s.cnt[b[j]], (1u << 11) + (old[j] + (uint32_t)c[j] < old[j]));
     });
-    if (beyond) atomicAdd(&s.own_beyond, beyond);
   }
   // This CTA's share of the bins, added up over the cluster, to the first CTA.  The cluster has filled before.
-  __device__ __forceinline__ void reduce(int mode) {
-    const float unit = unit_of(mode);
-    const bool one = mode == RS_ONE_WORD, two = mode == RS_TWO_WORDS;
+  __device__ __forceinline__ void reduce(bool masses) {
+    const float unit = unit_of();
     auto mass_of = [&](int b, uint32_t k, unsigned long long m) {
-      return k && (one || two) ? rs_weight(rs_edge((float)(b + one), g), g) * ((one ? (double)k : 0.0) + (double)m / unit) : 0.0;
+      return k && masses ? rs_weight(rs_edge((float)b, g), g) * ((double)m / unit) : 0.0;
     };
-    auto tokens = [&](uint32_t x) { return one ? x >> 22 : two ? x >> 11 : x; };
-    auto sum = [&](const RSSmem* o, int b, uint32_t x) {
-      return one ? (unsigned long long)(x & 0x3fffffu) : two ? (unsigned long long)(x & 2047u) << 32 | o->low[b] : 0ull;
-    };
-    const uint32_t room = one ? RS_ROOM1 : two ? max((uint32_t)sure, RS_ROOM2) : 0xffffffffu;
+    auto tokens = [](uint32_t x) { return x >> 11; };
+    auto sum = [](const RSSmem* o, int b, uint32_t x) { return (unsigned long long)(x & 2047u) << 32 | o->low[b]; };
+    const uint32_t room = masses ? max((uint32_t)sure, RS_ROOM) : 0xffffffffu;
     if (CL == 1) {
       uint32_t most = 0;
       for (int b = threadIdx.x; b < RS_BINS; b += TH) {
@@ -297,7 +289,7 @@ struct RSRow {
       __syncthreads();
       if (most > room) atomicMax(&s.own_most, most);
       __syncthreads();
-      if (threadIdx.x == 0) { s.beyond[0] = s.own_beyond; s.most[0] = s.own_most; }
+      if (threadIdx.x == 0) s.most[0] = s.own_most;
       return;
     }
     const int t = threadIdx.x, rank = (int)cl.block_rank();
@@ -322,22 +314,20 @@ struct RSRow {
       lead->bin_mass[rank * SHARE + t] = mass_of(rank * SHARE + t, k, m);
     }
     __syncthreads();
-    if (t == 0) { lead->beyond[rank] = s.own_beyond; lead->most[rank] = s.own_most; }
+    if (t == 0) lead->most[rank] = s.own_most;
   }
   // The bins of all CTAs' tokens, or of their threads' largest.
   __device__ __forceinline__ void histogram(int mode, float largest) {
-    if (mode == RS_ONE_WORD) {
-      fill<RS_ONE_WORD>();
-    } else if (mode == RS_TWO_WORDS) {
-      fill<RS_TWO_WORDS>();
+    if (mode == RS_MASSES) {
+      fill<true>();
     } else if (mode == RS_COUNTS) {
-      fill<RS_COUNTS>();
+      fill<false>();
     } else if (largest > -INFINITY) {
-      const int b = rs_bin(largest, g);
-      atomicAdd(b < RS_BINS ? &s.cnt[b] : &s.own_beyond, 1u);
+      const int b = rs_bin(rs_seen(largest, g), g);
+      if (b < RS_BINS) atomicAdd(&s.cnt[b], 1u << 11);
     }
     rs_sync<CL>();
-    reduce(mode);
+    reduce(mode == RS_MASSES);
   }
 
   // A CTA's share of a command.
@@ -346,15 +336,14 @@ struct RSRow {
     if (c.op == RS_FILL) {
       sure = c.sure;
       for (int i = tid; i < RS_BINS; i += TH) s.cnt[i] = s.low[i] = 0;
-      if (tid == 0) s.own_beyond = 0;
       __syncthreads();
-      histogram(c.mode, of_thread);
+      histogram(RS_MASSES, of_thread);
     } else if (c.op == RS_GATHER) {
       // into this CTA's own shared memory first: a place in the first CTA's list takes a trip there
       const float lo = (float)c.b0, hi = c.b1 == RS_BINS ? INFINITY : (float)(c.b1 + 1);  // -infinity's place is infinity
       // nothing below this is wanted
-      const float least = c.b1 == RS_BINS || g.sx == 0.f ? -INFINITY : rs_edge((float)(c.b1 + 2), g);
-      const float largest = c.b0 < 2 || g.sx == 0.f ? INFINITY : rs_edge((float)(c.b0 - 1), g);  // or above this
+      const float least = c.b1 == RS_BINS || g.sx == 0.f ? -INFINITY : rs_edge((float)(c.b1 + 1 + rs_slack(g)), g);
+      const float largest = c.b0 < 2 || g.sx == 0.f ? INFINITY : rs_edge((float)(c.b0 - rs_slack(g)), g);  // or above this
       if (tid == 0) s.n_mine = 0;
       __syncthreads();
       each([&](int i, const float (&l)[V]) {
@@ -366,7 +355,7 @@ struct RSRow {
         for (int j = 0; j < V; ++j) {
           if (!(l[j] >= least && l[j] <= largest)) continue;
           const float x = rs_place(l[j], g);
-          if (!((x >= lo && x < hi) || (hi == INFINITY && x == hi && l[j] > -INFINITY))) continue;
+          if (!((x >= lo && x < hi) || (lo == 0.f && x < 0.f) || (hi == INFINITY && x == hi && l[j] > -INFINITY))) continue;
           const uint32_t at = atomicAdd(&s.n_mine, 1u);
           if (at < RS_CAP) s.mine[at] = (unsigned long long)~rs_order(l[j] + 0.f) << 32 | (uint32_t)(i0 + i + j);
         }
@@ -434,8 +423,8 @@ struct RSRow {
     if (threadIdx.x < CL) cl.map_shared_rank(&s, threadIdx.x)->cmd = c;
     if (threadIdx.x == 0) { s.n_list = 0; s.over = 0; }
   }
-  // the bins that the cluster has put here, scanned; how many there are of what they count
-  __device__ uint32_t scan_bins() {
+  // the bins that the cluster has put here, scanned
+  __device__ void scan_bins() {
     uint32_t kc = 0, all;
     double mc = 0;
     __syncthreads();
@@ -449,9 +438,6 @@ struct RSRow {
     cnt_before = kc;
     mass_before = mc;
     rs_scan2<TH>(cnt_before, mass_before, s, &all, &all_mass);
-#pragma unroll
-    for (int r = 0; r < CL; ++r) all += s.beyond[r];
-    return all;
   }
   // whether a bin has more tokens than its words have room for
   __device__ bool crowded() const {
@@ -460,17 +446,6 @@ struct RSRow {
     for (int r = 0; r < CL; ++r) m |= s.most[r];
     return m;
   }
-  // Whether one word a bin holds the masses well enough.  Its rounding, 0.3 units a token, moves a border by that
-  // times sqrt(sum w^2); all borders together may take 2^-12 of the mass.
-  __device__ bool fine(uint32_t counted) {
-    double w2 = 0, all;
-#pragma unroll
-    for (int e = 0; e < RS_PER; ++e) w2 += bin_cnt[e] ? bin_mass[e] * (bin_mass[e] / bin_cnt[e]) : 0.0;
-    rs_scan<TH, double>(w2, s.wsum, &all);
-    const double off = 0.3 / unit_of(RS_ONE_WORD) * sqrt(all) / all_mass;
-    return counted == all_cnt && !crowded() && 2 * off * all_cnt < 0x1p-12;
-  }
-
   // First bin at which the running count or mass reaches the target (strict: exceeds it); when none does, RS_BINS by
   // count and the last one with a token by mass (a rounding is missing).
   __device__ void cross(bool by_mass, double target, bool strict, int* bin) {
@@ -681,27 +656,21 @@ struct RSRow {
     int idx = 0;          // what a look found
     double w = 0, mass = 0;
     uint32_t cnt = 0;
-    if (m.state == START) {
-      m.state = LISTED;
+    const int near = rs_slack(g);
+    const bool first = m.state == START;
+    if (first) {
       c.op = RS_GATHER;
-      if (all_cnt <= RS_COUNT) {
-        c.b1 = RS_BINS;
-        c.last = 1;
-        return c;
-      }
+      m.state = m.mode == RS_MASSES ? REFILLED : LISTED;
       if (m.mode == RS_NONE) {
-        c.b1 = min(over_bin + 1, RS_BINS);
+        c.last = all_cnt <= RS_COUNT;
+        c.b1 = c.last ? RS_BINS : min(over_bin + near, RS_BINS);
         return c;
       }
-      const uint32_t counted = scan_bins();
-      if (m.mode == RS_LARGEST || m.mode == RS_COUNTS) {
-        c.b1 = cross_one(false, (double)m.cut, false);
-        return c;
-      }
-      m.left = counted;
-      m.state = REFILLED;
-    } else if (m.state == REFILLED) {
-      m.left = scan_bins();
+    }
+    if (first || m.state == REFILLED) scan_bins();
+    if (first && m.state == LISTED) {
+      c.b1 = cross_one(false, (double)m.cut, false);
+      return c;
     }
     if (m.state == LISTED || m.state == LAST_LIST) {
       const int n_list = (int)s.n_list;
@@ -711,17 +680,13 @@ struct RSRow {
         settle(r, n_list, m.cut, m.cut_k, m.top_p, m.u, m.state == LISTED ? 0.0 : all_mass - m.base - m.in_mass);
         return c;
       }
-      m.mode = one_word() && !by_p ? RS_ONE_WORD : RS_TWO_WORDS;
       m.state = REFILLED;
-      c.op = RS_FILL; c.mode = m.mode; c.sure = (int)RS_ROOM2;
+      c.op = RS_FILL; c.sure = (int)RS_ROOM;
       return c;
     }
     if (m.state == REFILLED) {
-      if (m.mode == RS_ONE_WORD ? !fine(m.left) : sure < a.per && (crowded() || m.left != all_cnt)) {
-        c.op = RS_FILL;
-        c.mode = RS_TWO_WORDS;
-        c.sure = m.mode == RS_ONE_WORD ? (int)RS_ROOM2 : max(a.per, (int)RS_ROOM2);
-        m.mode = RS_TWO_WORDS;
+      if (crowded() && sure < a.per) {
+        c.op = RS_FILL; c.sure = a.per;
         return c;
       }
       // the last bin that a kept token can lie in
@@ -732,7 +697,7 @@ struct RSRow {
       if (by_p && !m.cut_k) cross(true, m.top_p * all_mass, false, &s.bin_p);
       __syncthreads();
       int last = s.bin_k;
-      if (by_m && !(m.cut_k && by_p)) last = min(last, min(over_bin + 1, RS_BINS));
+      if (by_m && !(m.cut_k && by_p)) last = min(last, min(over_bin + near, RS_BINS));
       if (by_p && !m.cut_k) last = min(last, s.bin_p == RS_BINS ? s.pick : s.bin_p);
       uint32_t in;
       at_bin(last, &m.before, &m.base, &in, &m.in_mass);
@@ -747,7 +712,7 @@ struct RSRow {
       m.purpose = m.cut_k ? OF_K : by_p ? OF_P : by_m ? OF_M : OF_TOKEN;
       if (m.purpose == OF_M) {
         m.state = COUNTED;
-        c.op = RS_OVER; c.b0 = over_bin - 1; c.b1 = min(over_bin + 1, RS_BINS);
+        c.op = RS_OVER; c.b0 = over_bin - near; c.b1 = min(over_bin + near, RS_BINS);
         return c;
       }
     } else if (m.state == LOOKED) {
@@ -830,7 +795,7 @@ struct RSRow {
         m.purpose = was == OF_K && by_p ? OF_P : was != OF_M && by_m ? OF_M : OF_TOKEN;
         if (m.purpose == OF_M) {
           m.state = COUNTED;
-          c.op = RS_OVER; c.b0 = over_bin - 1; c.b1 = min(over_bin + 1, RS_BINS);
+          c.op = RS_OVER; c.b0 = over_bin - near; c.b1 = min(over_bin + near, RS_BINS);
           return c;
         }
       }
@@ -861,7 +826,7 @@ struct RSRow {
 };
 
 template <class T, bool STAGED, int CL, int TH>
-__global__ void __launch_bounds__(TH, TH == RS_THREADS_FEW ? 1 : 2) sample_rows_kernel(const RSArgs a) {
+__global__ void __launch_bounds__(TH, TH == RS_THREADS_FEW ? 1 : sizeof(T) == 2 ? 3 : 2) sample_rows_kernel(const RSArgs a) {
   extern __shared__ __align__(16) uint8_t rs_raw[];
   RSSmem& s = *reinterpret_cast<RSSmem*>(rs_raw);
   T* stage = reinterpret_cast<T*>(rs_raw + (sizeof(RSSmem) + 15) / 16 * 16);
@@ -871,7 +836,7 @@ __global__ void __launch_bounds__(TH, TH == RS_THREADS_FEW ? 1 : 2) sample_rows_
   const int r = (int)(blockIdx.x / CL);
   const int i0 = min(rank * a.per, a.vocab), n = min(a.per, a.vocab - i0);
   const T* row = reinterpret_cast<const T*>(a.logits) + (int64_t)r * a.ld;
-  RSRow<T, STAGED, CL, TH> w{s, stage, a, row, i0, n, RSGeom{}, cl, 0.0, 0u, (int)RS_ROOM2};
+  RSRow<T, STAGED, CL, TH> w{s, stage, a, row, i0, n, RSGeom{}, cl, 0.0, 0u, (int)RS_ROOM};
 
   // 1. this CTA's logits, the largest and the smallest that is a number.  Copies of 16 bytes and more; the shares are
   // multiples of 8 logits, what is left of a row's end comes by itself.
@@ -885,7 +850,6 @@ __global__ void __launch_bounds__(TH, TH == RS_THREADS_FEW ? 1 : 2) sample_rows_
   const int k = a.top_k ? a.top_k[r] : 0;
   const float p = a.top_p ? a.top_p[r] : 1.f, q = a.min_p ? a.min_p[r] : 0.f, un = a.u[r];
   for (int i = tid; i < RS_BINS; i += TH) s.cnt[i] = s.low[i] = 0;
-  if (tid == 0) s.own_beyond = 0;
   RSStat st{-INFINITY, INFINITY, 0};
   auto see = [&](float l) {  // NaN is neither
     st.mx = fmaxf(st.mx, l);
@@ -951,13 +915,20 @@ __global__ void __launch_bounds__(TH, TH == RS_THREADS_FEW ? 1 : 2) sample_rows_
   }
   // 2. the bins
   RSGeom& g = w.g;
+  g.from = st.mx;
+  g.far = fabsf(st.mx) >= RS_FAR;
+  if (g.far) {
+    st.mn = rs_seen(st.mn, g);
+    st.mx = 0.f;
+  }
   g.mx = st.mx;
   const float tc = fminf(fmaxf(t, 0x1p-100f), 0x1p100f);
   g.t = tc;
   g.inv_t = 1.f / tc;
   // a little more than the row's spread: the smallest logit lies in the last bin, not behind it
-  const float span = fminf((st.mx - st.mn) * (1.f + 0x1p-20f), RS_SPAN * fmaxf(tc, 1.f));
+  const float span = fminf((st.mx - st.mn) * (1.f + 0x1p-10f), RS_SPAN * fmaxf(tc, 1.f));
   g.sx = span > 1e-30f ? (float)RS_BINS / span : 0.f;
+  g.top = st.mx * g.sx;
   g.width = span > 1e-30f ? span / (float)RS_BINS : 0.f;
   w.min_p = q > 0.f ? (double)q : 0.0;
   w.all_cnt = st.n;
@@ -965,8 +936,7 @@ __global__ void __launch_bounds__(TH, TH == RS_THREADS_FEW ? 1 : 2) sample_rows_
   const int mode = st.n <= RS_COUNT || (q > 0.f && !by_p) ? RS_NONE
                    // the k largest are sure to be few more than k where k is a small part of the threads' largest
                    : cut_k && k <= RS_CAP / 2             ? (k <= a.vocab / (32 / (int)sizeof(T)) / 4 && k <= TH * CL / 8 ? RS_LARGEST : RS_COUNTS)
-                   : !by_p && w.one_word() && st.n >= RS_FLAT ? RS_ONE_WORD
-                                                          : RS_TWO_WORDS;
+                                                          : RS_MASSES;
   if (mode != RS_NONE) {
     w.histogram(mode, largest);
     rs_sync<CL>();
