@@ -288,7 +288,7 @@ static int rotary_launch(RotaryArgs& a, const N730Rotary* r, const char* what, c
   a.by_page = FastDiv(a.has_cache ? a.c.page_size : 1);
   a.by_pairs = FastDiv(std::max(a.rd / 2, 1));
   while ((int64_t)a.rows_cta * (a.rd / 2) * sizeof(float2) > RO_TABLE) a.rows_cta -= a.at_once;
-  const dim3 g((a.rows + a.rows_cta - 1) / a.rows_cta, chunks);
+  const dim3 g((unsigned)(((int64_t)a.rows + a.rows_cta - 1) / a.rows_cta), chunks);
   const size_t smem = (size_t)a.rows_cta * (a.rd / 2) * sizeof(float2);
   if (vec) {
     if (es == 4) rotary_kernel<RO_V, 4><<<g, threads, smem, st>>>(a);
