@@ -848,7 +848,7 @@ static KAPlan ka_plan(const N730KV16Cache& c, int batch, int tokens, int heads) 
     splits = 1;
     for (int s = 1; s <= std::min<int64_t>(pos, 64); ++s) {
       const double waves = (double)((items * s + slots - 1) / slots);
-      const double us = waves * ((double)((pos + s - 1) / s) * 1.9 + 4.5) + s * 0.15 + (double)s * units * rows * c.head_dim * 8 / 6e6;
+      const double us = waves * ((double)((pos + s - 1) / s) * 1.9 + 4.5) + s * 0.10 + (double)s * units * rows * c.head_dim * 8 / 1e7;
       if (us < best * 0.98) { best = us; splits = s; }
     }
   };
@@ -859,7 +859,9 @@ static KAPlan ka_plan(const N730KV16Cache& c, int batch, int tokens, int heads) 
   const int64_t cap = (int64_t)c.max_pages * c.page_size;
   shape(own_rows, own_units, cap, p.own_nt, p.own_tiles, p.own_splits);
   p.own_rows = p.own_tiles * p.own_nt * 128;
-  // few rows: warps of 16 where they fill a share of the SMs, in one grid with the prefix's items otherwise (one launch less)
+  // few rows: warps of 16 where they fill a share of the SMs (128 sequences of 64 heads, 8 rows each: 83 us for 123; with 3
+  // groups of rows, 16 sequences of 5 tokens and 28 heads, 38 for 36), in one grid with the prefix's items otherwise (one
+  // launch less: 4 sequences of 14 heads 10 us for 12)
   if (own_rows <= KO_MOST && own_units >= sms / 4) {
     p.own_nt = 0;
     p.own_tiles = (int)((own_rows + KO_ROWS - 1) / KO_ROWS);
