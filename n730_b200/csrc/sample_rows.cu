@@ -7,7 +7,7 @@
 //   mass exceeds u times the kept mass.
 //
 // A cluster of 8 CTAs takes a row: each copies an eighth of the logits into its shared memory, so that HBM is read once
-// and whatever follows runs on the chip.  (Rows of up to RS_ALONE logits take one CTA.)  The first CTA leads; the others
+// and whatever follows runs on the chip.  (Short rows, and many of them, take 4, 2 or one CTA.)  The first CTA leads; the others
 // serve its commands, and all meet around each.
 //   1. largest and smallest logit, and each thread's largest.
 //   2. A list: tokens are gathered in the first CTA's shared memory and sorted, the rest is a scan over it with weights in
@@ -31,8 +31,7 @@
 namespace n730 {
 namespace cg = cooperative_groups;
 
-constexpr int RS_CLUSTER = 8;      // CTAs of a row, one for rows of up to RS_ALONE logits: no exchange, 15 -> 10 us at 1000
-constexpr int RS_ALONE = 16384;
+constexpr int RS_CLUSTER = 8;      // most CTAs of a row
 // Threads of a CTA: 512 and all of an SM's registers while a row's CTAs find an SM each (one row of 152064 without a cut:
 // 23.5 us, 24.6 with 256), 256 beyond that and two CTAs an SM (64 rows with a top-k: 30 us, 60 with 512), three of 16-bit
 // logits, which shared memory has room for (192 rows without a cut: 150 us, 173 with two).
@@ -43,6 +42,7 @@ constexpr int RS_CAP = 1024;       // tokens that are sorted at once
 constexpr int RS_COUNT = 160;      // lists up to this long are sorted by counting
 constexpr uint32_t RS_ROOM = 4000;  // tokens of a CTA's bin that the sums have room for
 constexpr float RS_SPAN = 32.f;    // bins reach this many logits, or temperatures where that is more, below the largest
+constexpr size_t RS_HALF = 76 * 1024;  // longest slice of which two fit an SM
 constexpr size_t RS_STAGE_MAX = 160 * 1024;  // longest slice that is kept in shared memory
 
 struct RSArgs {
@@ -293,25 +293,23 @@ struct RSRow {
       return;
     }
     const int t = threadIdx.x, rank = (int)cl.block_rank();
-    uint32_t k = 0, most = 0;
-    unsigned long long m = 0;
-    if (t < SHARE) {
+    RSSmem* lead = cl.map_shared_rank(&s, 0);
+    if (t == 0) s.own_most = 0;
+    __syncthreads();
+    for (int b = rank * SHARE + t; b < (rank + 1) * SHARE; b += TH) {
+      uint32_t k = 0, most = 0;
+      unsigned long long m = 0;
 #pragma unroll
       for (int r = 0; r < CL; ++r) {
         const RSSmem* o = cl.map_shared_rank(&s, r);
-        const uint32_t x = o->cnt[rank * SHARE + t];
+        const uint32_t x = o->cnt[b];
         k += tokens(x);
         most = max(most, tokens(x));
-        m += sum(o, rank * SHARE + t, x);
+        m += sum(o, b, x);
       }
-    }
-    if (t == 0) s.own_most = 0;
-    __syncthreads();
-    RSSmem* lead = cl.map_shared_rank(&s, 0);
-    if (most > room) atomicMax(&s.own_most, most);
-    if (t < SHARE) {
-      lead->bin_cnt[rank * SHARE + t] = k;
-      lead->bin_mass[rank * SHARE + t] = mass_of(rank * SHARE + t, k, m);
+      if (most > room) atomicMax(&s.own_most, most);
+      lead->bin_cnt[b] = k;
+      lead->bin_mass[b] = mass_of(b, k, m);
     }
     __syncthreads();
     if (t == 0) lead->most[rank] = s.own_most;
@@ -982,19 +980,35 @@ static int rs_launch_one(const RSArgs& a, int batch, size_t slice, cudaStream_t 
   return kv8_launch_cluster(sample_rows_kernel<T, STAGED, CL, TH>, dim3((unsigned)batch * CL), CL, dim3(TH), fixed + slice, st, false, a);
 }
 template <class T, bool STAGED, int CL>
-static int rs_launch_few(const RSArgs& a, int batch, size_t slice, cudaStream_t st) {
-  // half of the SMs: a cluster lies in one group of SMs, which one CTA an SM does not fill evenly
-  return batch <= num_sms() / 2 / CL ? rs_launch_one<T, STAGED, CL, RS_THREADS_FEW>(a, batch, slice, st)
-                                 : rs_launch_one<T, STAGED, CL, RS_THREADS_MANY>(a, batch, slice, st);
+static int rs_launch_many(const RSArgs& a, int batch, size_t slice, bool many, cudaStream_t st) {
+  return many ? rs_launch_one<T, STAGED, CL, RS_THREADS_MANY>(a, batch, slice, st)
+              : rs_launch_one<T, STAGED, CL, RS_THREADS_FEW>(a, batch, slice, st);
 }
+// CTAs of a row: what takes the fewest waves of CTAs times a CTA's time, in us: 12 of meetings (6 without other CTAs), and
+// the logits' share.  Measured, 1, 2, 4 and 8 CTAs: 256 rows of 32000 fp32 logits 40, 42, 53, 86 us; 8 rows of them without
+// a top-k 19 and 13 (1 and 8); 64 rows of 151936 52 and 50 (4 and 8); 8 rows of 1000 8 and 11.
 template <class T>
 static int rs_launch(RSArgs& a, int batch, cudaStream_t st) {
-  const int cl = a.vocab <= RS_ALONE ? 1 : RS_CLUSTER;
-  a.per = ((a.vocab + cl - 1) / cl + 7) / 8 * 8;
-  const size_t slice = (size_t)a.per * sizeof(T);
-  if (cl == 1) return rs_launch_few<T, true, 1>(a, batch, slice, st);
-  if (slice <= RS_STAGE_MAX) return rs_launch_few<T, true, RS_CLUSTER>(a, batch, slice, st);
-  return rs_launch_few<T, false, RS_CLUSTER>(a, batch, 0, st);
+  auto slice = [&](int cl) { return (size_t)(((a.vocab + cl - 1) / cl + 7) / 8 * 8) * sizeof(T); };
+  // 256 threads unless one CTA takes an SM's shared memory, or half of the SMs are enough (a cluster lies in one group of
+  // SMs, which one CTA an SM does not fill evenly)
+  auto many = [&](int cl) { return slice(cl) <= RS_HALF && (int64_t)batch * cl > num_sms() / 2; };
+  int best = RS_CLUSTER;
+  double least = 1e30;
+  for (int cl = RS_CLUSTER; cl >= 1; cl /= 2) {
+    if (slice(cl) > RS_STAGE_MAX) break;
+    const int an_sm = !many(cl) ? 1 : sizeof(T) == 2 && slice(cl) <= RS_HALF / 2 ? 3 : 2;
+    const int64_t slots = (int64_t)num_sms() * an_sm, waves = ((int64_t)batch * cl + slots - 1) / slots;
+    const double us = waves * ((cl == 1 ? 6. : 12.) + (double)a.vocab / cl * (many(cl) ? 0.44e-3 : 0.27e-3));
+    if (us < least) { least = us; best = cl; }
+  }
+  a.per = (int)(slice(best) / sizeof(T));
+  const bool m = many(best);
+  if (slice(best) > RS_STAGE_MAX) return rs_launch_many<T, false, RS_CLUSTER>(a, batch, 0, (int64_t)batch * best > num_sms() / 2, st);
+  if (best == 1) return rs_launch_many<T, true, 1>(a, batch, slice(1), m, st);
+  if (best == 2) return rs_launch_many<T, true, 2>(a, batch, slice(2), m, st);
+  if (best == 4) return rs_launch_many<T, true, 4>(a, batch, slice(4), m, st);
+  return rs_launch_many<T, true, RS_CLUSTER>(a, batch, slice(RS_CLUSTER), m, st);
 }
 
 }  // namespace n730

@@ -208,3 +208,31 @@ def test_graph_and_stream():
         t.cuda.synchronize()
         want = draw(y, "f32", None, None, 0.9, None, u.cpu().numpy())[0][0]
         assert np.array_equal(tok.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("dtype,B,V", [("f32", 74, 50000), ("f16", 74, 160000), ("bf16", 90, 20000), ("f32", 200, 5000)])
+def test_rows_in_smaller_clusters(dtype, B, V):
+    """Many rows: 4, 2 and one CTA a row, every kind of cut among them."""
+    rng = np.random.default_rng(V)
+    t, k = rng.choice([0.0, 0.5, 0.9, 1.3], B), rng.choice([0, 0, 30, 300, 3000], B)
+    check(rows(rng, B, V, peaks=24), dtype, t, k, rng.choice([1.0, 0.9, 0.99], B), rng.choice([0.0, 0.0, 0.02], B), rng.random(B))
+
+
+def test_two_calls_at_once():
+    """On two streams, each with its own outputs: nothing is shared between calls."""
+    t = torch()
+    rng = np.random.default_rng(15)
+    x = [dev(rows(rng, 30, 32000, peaks=20).astype(np.float32)) for _ in range(2)]
+    u, k = dev(rng.random(30).astype(np.float32)), dev(np.where(np.arange(30) % 2, 40, 0).astype(np.int32))
+    p = dev(np.full(30, 0.95, np.float32))
+    out = [[t.zeros(30, dtype=t.int32, device="cuda") for _ in range(2)] for _ in range(2)]
+    st = [t.cuda.Stream() for _ in range(2)]
+    t.cuda.synchronize()
+    for i in range(40):
+        for a in range(2):
+            sampling.sample_rows(x[a].data_ptr(), "f32", 30, 32000, u.data_ptr(), out[a][i % 2].data_ptr(), top_k=k.data_ptr(),
+                                 top_p=p.data_ptr(), stream=st[a].cuda_stream)
+    t.cuda.synchronize()
+    for a in range(2):
+        want = draw(x[a].cpu().numpy(), "f32", None, k.cpu().numpy(), 0.95, None, u.cpu().numpy())[0][0]
+        assert np.array_equal(out[a][0].cpu().numpy(), want) and np.array_equal(out[a][1].cpu().numpy(), want)
