@@ -736,7 +736,7 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
 // Joins the rows' parts.  A CTA takes 32 rows of a KV head, a lane a row, and PIECES groups of 4 channels; its warps take
 // MINE of these each, and every PARTS-th part: with few rows that is 32 channels and a quarter of the parts, so that a
 // part's trip to memory is paid for few times in a row (896 rows of 17 parts: 7 us, 11 with a CTA for all channels), with
-// many all channels and parts (8192 rows of 5 parts: 13 us, 17 the other way).  Outputs change places in shared memory so
+// many all channels and parts (8192 rows of 5 parts: 10 us, 17 the other way).  Outputs change places in shared memory so
 // that they leave as whole rows.
 template <int HD, bool BF, int MINE, int COLS, int PARTS>
 __global__ void __launch_bounds__(COLS * PARTS * 32) kv16_join_kernel(const KAArgs a) {

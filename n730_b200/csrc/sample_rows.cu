@@ -24,6 +24,7 @@
 // Sums are integers, or 64-bit floats in a fixed order: the same inputs give the same token.
 #include <cooperative_groups.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "kv8.h"
@@ -33,8 +34,9 @@ namespace cg = cooperative_groups;
 
 constexpr int RS_CLUSTER = 8;      // most CTAs of a row
 // Threads of a CTA: 512 and all of an SM's registers while a row's CTAs find an SM each (one row of 152064 without a cut:
-// 23.5 us, 24.6 with 256), 256 beyond that and two CTAs an SM (64 rows with a top-k: 30 us, 60 with 512), three of 16-bit
-// logits, which shared memory has room for (192 rows without a cut: 150 us, 173 with two).
+// 21.7 us, 24.1 with 256), 256 beyond that.  Then two CTAs an SM, or three of 16-bit logits, which shared memory has room
+// for, where that saves more waves than registers that do not suffice cost (192 rows of 152064
+// bf16 logits without a cut: 139 us, 157 with two; 40 rows of 100000, where it does not: 39, and 31 with two).
 constexpr int RS_THREADS_FEW = 512, RS_THREADS_MANY = 256;
 constexpr int RS_WARPS = RS_THREADS_FEW / 32;  // most warps
 constexpr int RS_BINS = 1536;      // as many as leave room for two CTAs of 19008 fp32 logits (a row of 152064) an SM
@@ -823,8 +825,8 @@ struct RSRow {
   }
 };
 
-template <class T, bool STAGED, int CL, int TH>
-__global__ void __launch_bounds__(TH, TH == RS_THREADS_FEW ? 1 : sizeof(T) == 2 ? 3 : 2) sample_rows_kernel(const RSArgs a) {
+template <class T, bool STAGED, int CL, int TH, int CTAS>
+__global__ void __launch_bounds__(TH, CTAS) sample_rows_kernel(const RSArgs a) {
   extern __shared__ __align__(16) uint8_t rs_raw[];
   RSSmem& s = *reinterpret_cast<RSSmem*>(rs_raw);
   T* stage = reinterpret_cast<T*>(rs_raw + (sizeof(RSSmem) + 15) / 16 * 16);
@@ -973,16 +975,17 @@ __global__ void __launch_bounds__(TH, TH == RS_THREADS_FEW ? 1 : sizeof(T) == 2 
   }
 }
 
-template <class T, bool STAGED, int CL, int TH>
+template <class T, bool STAGED, int CL, int TH, int CTAS>
 static int rs_launch_one(const RSArgs& a, int batch, size_t slice, cudaStream_t st) {
   const size_t fixed = (sizeof(RSSmem) + 15) / 16 * 16;
-  if (int rc = smem_attr_once<sample_rows_kernel<T, STAGED, CL, TH>>((int)(fixed + (STAGED ? RS_STAGE_MAX : 0)))) return rc;
-  return kv8_launch_cluster(sample_rows_kernel<T, STAGED, CL, TH>, dim3((unsigned)batch * CL), CL, dim3(TH), fixed + slice, st, false, a);
+  if (int rc = smem_attr_once<sample_rows_kernel<T, STAGED, CL, TH, CTAS>>((int)(fixed + (STAGED ? RS_STAGE_MAX : 0)))) return rc;
+  return kv8_launch_cluster(sample_rows_kernel<T, STAGED, CL, TH, CTAS>, dim3((unsigned)batch * CL), CL, dim3(TH), fixed + slice, st, false, a);
 }
 template <class T, bool STAGED, int CL>
-static int rs_launch_many(const RSArgs& a, int batch, size_t slice, bool many, cudaStream_t st) {
-  return many ? rs_launch_one<T, STAGED, CL, RS_THREADS_MANY>(a, batch, slice, st)
-              : rs_launch_one<T, STAGED, CL, RS_THREADS_FEW>(a, batch, slice, st);
+static int rs_launch_many(const RSArgs& a, int batch, size_t slice, int ctas, cudaStream_t st) {
+  if (ctas == 1) return rs_launch_one<T, STAGED, CL, RS_THREADS_FEW, 1>(a, batch, slice, st);
+  if (sizeof(T) == 2 && ctas == 3) return rs_launch_one<T, STAGED, CL, RS_THREADS_MANY, sizeof(T) == 2 ? 3 : 2>(a, batch, slice, st);
+  return rs_launch_one<T, STAGED, CL, RS_THREADS_MANY, 2>(a, batch, slice, st);
 }
 // CTAs of a row: what takes the fewest waves of CTAs times a CTA's time, in us: 12 of meetings (6 without other CTAs), and
 // the logits' share.  Measured, 1, 2, 4 and 8 CTAs: 256 rows of 32000 fp32 logits 40, 42, 53, 86 us; 8 rows of them without
@@ -990,25 +993,27 @@ static int rs_launch_many(const RSArgs& a, int batch, size_t slice, bool many, c
 template <class T>
 static int rs_launch(RSArgs& a, int batch, cudaStream_t st) {
   auto slice = [&](int cl) { return (size_t)(((a.vocab + cl - 1) / cl + 7) / 8 * 8) * sizeof(T); };
-  // 256 threads unless one CTA takes an SM's shared memory, or half of the SMs are enough (a cluster lies in one group of
-  // SMs, which one CTA an SM does not fill evenly)
-  auto many = [&](int cl) { return slice(cl) <= RS_HALF && (int64_t)batch * cl > num_sms() / 2; };
+  // CTAs of an SM: one of 512 threads where it takes an SM's shared memory, or half of the SMs are enough (a cluster lies in
+  // one group of SMs, which one CTA an SM does not fill evenly)
+  auto ctas = [&](int cl) {
+    const double n = (double)batch * cl / num_sms();
+    if (slice(cl) > RS_HALF || n <= 0.5) return 1;
+    return sizeof(T) == 2 && slice(cl) <= RS_HALF / 2 && 1.25 * std::max(1.0, n / 3) < std::max(1.0, n / 2) ? 3 : 2;
+  };
   int best = RS_CLUSTER;
   double least = 1e30;
   for (int cl = RS_CLUSTER; cl >= 1; cl /= 2) {
     if (slice(cl) > RS_STAGE_MAX) break;
-    const int an_sm = !many(cl) ? 1 : sizeof(T) == 2 && slice(cl) <= RS_HALF / 2 ? 3 : 2;
-    const int64_t slots = (int64_t)num_sms() * an_sm, waves = ((int64_t)batch * cl + slots - 1) / slots;
-    const double us = waves * ((cl == 1 ? 6. : 12.) + (double)a.vocab / cl * (many(cl) ? 0.44e-3 : 0.27e-3));
+    const double us = std::max((double)batch * cl / (num_sms() * ctas(cl)), 1.0) * ((cl == 1 ? 6. : 12.) + (double)a.vocab / cl * (ctas(cl) > 1 ? 0.44e-3 : 0.27e-3));
     if (us < least) { least = us; best = cl; }
   }
   a.per = (int)(slice(best) / sizeof(T));
-  const bool m = many(best);
-  if (slice(best) > RS_STAGE_MAX) return rs_launch_many<T, false, RS_CLUSTER>(a, batch, 0, (int64_t)batch * best > num_sms() / 2, st);
-  if (best == 1) return rs_launch_many<T, true, 1>(a, batch, slice(1), m, st);
-  if (best == 2) return rs_launch_many<T, true, 2>(a, batch, slice(2), m, st);
-  if (best == 4) return rs_launch_many<T, true, 4>(a, batch, slice(4), m, st);
-  return rs_launch_many<T, true, RS_CLUSTER>(a, batch, slice(RS_CLUSTER), m, st);
+  const int n = ctas(best);
+  if (slice(best) > RS_STAGE_MAX) return rs_launch_one<T, false, RS_CLUSTER, RS_THREADS_FEW, 1>(a, batch, 0, st);
+  if (best == 1) return rs_launch_many<T, true, 1>(a, batch, slice(1), n, st);
+  if (best == 2) return rs_launch_many<T, true, 2>(a, batch, slice(2), n, st);
+  if (best == 4) return rs_launch_many<T, true, 4>(a, batch, slice(4), n, st);
+  return rs_launch_many<T, true, RS_CLUSTER>(a, batch, slice(RS_CLUSTER), n, st);
 }
 
 }  // namespace n730

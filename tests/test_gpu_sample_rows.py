@@ -210,7 +210,8 @@ def test_graph_and_stream():
         assert np.array_equal(tok.cpu().numpy(), want)
 
 
-@pytest.mark.parametrize("dtype,B,V", [("f32", 74, 50000), ("f16", 74, 160000), ("bf16", 90, 20000), ("f32", 200, 5000)])
+@pytest.mark.parametrize("dtype,B,V", [("f32", 74, 50000), ("f32", 74, 80000), ("f16", 74, 160000), ("bf16", 90, 20000), ("f32", 200, 5000),
+                                       ("bf16", 400, 900), ("f16", 60, 156000), ("bf16", 90, 28000), ("f16", 186, 28000), ("bf16", 93, 19000), ("f32", 52, 78001)])
 def test_rows_in_smaller_clusters(dtype, B, V):
     """Many rows: 4, 2 and one CTA a row, every kind of cut among them."""
     rng = np.random.default_rng(V)
