@@ -23,9 +23,9 @@
 // do not (tokens of the same call) are zeroed where they are not finite; rows that see them add them by themselves.
 //
 // Bound by the chain of a tile rather than by bytes or the tensor pipe: 128 sequences of 64 heads x 128 behind 16384
-// positions take 82 us in all, 41 of products at the tensor cores' rate; the prefix's kernel alone 80 us, 830 TFLOP/s, a
-// tile 4.1k cycles, of which the softmax is 2.2k, the products 1.0k and hand-offs the rest.  32 of 28 heads behind 8131:
-// 24 us, 6 of them the bytes of K and V.
+// positions take 82 us in all (69 GFLOP, 840 TFLOP/s; 41 us at the tensor cores' measured rate), a tile 4.1k cycles, of
+// which the softmax is 2.2k, the products 1.0k and hand-offs the rest.  32 of 28 heads behind 8131: 24 us, 6 of them the
+// bytes of K and V.
 //
 // Every wait is bounded; one that runs out sets the workspace's status word, ends the CTA's work and still frees the
 // tensor memory.

@@ -9,8 +9,8 @@
 //
 // Bound by bytes: every element is read and written once.  A thread has one unit of a row (8 channels, or both runs of
 // 8 that a half layout pairs) in up to 16 rows, so that what the unit is costs nothing a row; angles are computed once a
-// row and pair, not once a head, in shared memory.  2048 rows of 28 fp32 heads x 128: 11.5 us, 5.1 TB/s; a prompt of 4133
-// rows of 36 fp16 heads x 128: 18 us, 4.2 TB/s with its inputs in L2, 23 without.
+// row and pair, not once a head, in shared memory.  2048 rows of 28 fp32 heads x 128 take 11.5 us (5.1 TB/s), a
+// prompt of 4133 rows of 36 fp16 heads x 128 18 us (4.2 TB/s), both partly from L2; the prompt from memory 23.
 #include <cmath>
 
 #include "kv16.h"
