@@ -28,7 +28,7 @@ int kv16_check(const N730KV16Cache* c, int batch, const char* what) {
                "%s: n_kv %d, n_pages %d, max_pages %d, prefix_pages %d", what, c->n_kv, c->n_pages, c->max_pages,
                c->prefix_pages);
   N730_REQUIRE(c->prefix_pages == 0 || (c->prefix_table && c->prefix_len), N730_NULL, "%s: null prefix", what);
-  N730_REQUIRE((int64_t)c->n_pages * c->n_kv * c->page_size < (1ll << 31), N730_BAD_ARG,
+  N730_REQUIRE((int64_t)c->n_pages * c->n_kv <= ((1ll << 31) - 1) / c->page_size, N730_BAD_ARG,
                "%s: the pool holds 2^31 or more rows", what);
   N730_REQUIRE((int64_t)c->max_pages * c->page_size <= (1ll << 29) && (int64_t)c->prefix_pages * c->page_size <= (1ll << 29),
                N730_BAD_ARG, "%s: a table's pages hold more than 2^29 positions", what);

@@ -50,6 +50,12 @@ def test_bad_cache(kw, code):
     refused(lambda: c.attention(A, A, 1, 1, heads, A, ws=A, ws_bytes=1 << 40), code)
 
 
+def test_pool_of_more_rows_than_64_bits_count():
+    """2^30 pages of 2^14 heads and 2^20 positions: their product is 2^64."""
+    c = cache(n_pages=1 << 30, n_kv=1 << 14, page_size=1 << 20, max_pages=1, prefix_pages=1)
+    refused(lambda: c.attention_workspace(1, 1, 1 << 14), -13)
+
+
 def test_null_cache():
     lib = _lib.cuda()
     assert lib.n730_kv16_append(None, None, None, 0, None, 0, 0, A, A, 128, 1, 1, 1, A, None, None, None) == -12
