@@ -46,6 +46,7 @@ constexpr int RS_CAP = 1024;       // tokens that are sorted at once
 constexpr int RS_COUNT = 160;      // lists up to this long are sorted by counting
 constexpr uint32_t RS_ROOM = 4000;  // tokens of a CTA's bin that the sums have room for
 constexpr float RS_SPAN = 32.f;    // bins reach this many logits, or temperatures where that is more, below the largest
+constexpr float RS_TEMPS = 40.f;   // tokens this many temperatures below the largest have e^-40 of its weight, which counts as none
 constexpr size_t RS_HALF = 76 * 1024;  // longest slice of which two fit an SM
 constexpr size_t RS_STAGE_MAX = 160 * 1024;  // longest slice that is kept in shared memory
 
@@ -122,16 +123,19 @@ __device__ __forceinline__ float rs_float(float x) { return x; }
 __device__ __forceinline__ float rs_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ float rs_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// A row's bins: bin = floor((max - l) * sx); edge(b), its upper end, is max - b * width as fp32 rounds it.  A place is
-// off by `slack` bins where logits lie far from 0: bins are then not what their edges say, but their masses go by the edges
-// and stay right.
+// A row's bins: bin = floor((max - l) * sx); edge(b), its upper end, is max - b * width as fp32 rounds it.  max * sx is
+// rounded once, which moves all of a row's places by as much as 2^-24 of it, and an edge by 2^-24 of itself: rows whose
+// largest logit is 2^21 bins or more from 0 (or a bin of T / 38 or more: places, edges and logits would leave the bins that
+// they belong to, the last ones for no bin at all) go by the logits' distances from it, which are exact for all that have a
+// weight.  For the others this is 1/8 of a bin each: what a place and an edge say is off by one bin at most.
 struct RSGeom {
   float mx, sx, top, width, inv_t;  // top: max * sx
   double t;
-  bool far;                         // the largest logit is too large for products by sx, or infinite: logits go by their
-  float from;                       // distance from it, RS_LEAST at least
+  bool far;                         // logits go by their distance from `from`, the largest, RS_LEAST at least
+  float from;
 };
-constexpr float RS_LEAST = -3e38f, RS_FAR = 0x1p100f;
+constexpr float RS_LEAST = -3e38f, RS_FAR = 0x1p21f;  // RS_FAR: bins
+constexpr int RS_SLACK = 1;
 __device__ __forceinline__ float rs_place(float l, const RSGeom& g) { return fmaf(-l, g.sx, g.top); }
 // NaN and -infinity have no place below RS_BINS
 __device__ __forceinline__ int rs_bin(float l, const RSGeom& g) {
@@ -139,7 +143,6 @@ __device__ __forceinline__ int rs_bin(float l, const RSGeom& g) {
   return x < (float)RS_BINS ? max((int)x, 0) : RS_BINS;
 }
 __device__ __forceinline__ float rs_edge(float b, const RSGeom& g) { return fmaf(-b, g.width, g.mx); }
-__device__ __forceinline__ int rs_slack(const RSGeom& g) { return 1 + (int)fminf(fabsf(g.top) * 0x1p-22f, (float)RS_BINS); }
 __device__ __forceinline__ float rs_seen(float l, const RSGeom& g) {
   return !g.far || !(l > -INFINITY) ? l : l == g.from ? 0.f : fmaxf(l - g.from, RS_LEAST);
 }
@@ -257,7 +260,7 @@ struct RSRow {
         if (!MASSES) continue;
         // y = (l - edge) / T: the two are near, their difference is exact but for what is below 2^-24 of a bin
         const float y = (l[j] - rs_edge(f - 8388608.f, g)) * g.inv_t;
-        const float e = narrow ? y * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 1.f / 120, 1.f / 24), 1.f / 6), 0.5f), 1.f) : expm1f(y);
+        const float e = narrow ? y * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 1.f / 120, 1.f / 24), 1.f / 6), 0.5f), 1.f) : expm1f(fminf(y, 0x1p-6f));
         c[j] = (int)((uint32_t)__float2int_rn(e * unit) + (uint32_t)unit);
       }
 #pragma unroll
@@ -344,8 +347,8 @@ struct RSRow {
       // into this CTA's own shared memory first: a place in the first CTA's list takes a trip there
       const float lo = (float)c.b0, hi = c.b1 == RS_BINS ? INFINITY : (float)(c.b1 + 1);  // -infinity's place is infinity
       // nothing below this is wanted
-      const float least = c.b1 == RS_BINS || g.sx == 0.f ? -INFINITY : rs_edge((float)(c.b1 + 1 + rs_slack(g)), g);
-      const float largest = c.b0 < 2 || g.sx == 0.f ? INFINITY : rs_edge((float)(c.b0 - rs_slack(g)), g);  // or above this
+      const float least = c.b1 == RS_BINS || g.sx == 0.f ? -INFINITY : rs_edge((float)(c.b1 + 1 + RS_SLACK), g);
+      const float largest = c.b0 < 2 || g.sx == 0.f ? INFINITY : rs_edge((float)(c.b0 - RS_SLACK), g);  // or above this
       if (tid == 0) s.n_mine = 0;
       __syncthreads();
       each([&](int i, const float (&l)[V]) {
@@ -658,7 +661,7 @@ struct RSRow {
     int idx = 0;          // what a look found
     double w = 0, mass = 0;
     uint32_t cnt = 0;
-    const int near = rs_slack(g);
+    const int near = RS_SLACK;
     const bool first = m.state == START;
     if (first) {
       c.op = RS_GATHER;
@@ -917,18 +920,15 @@ __global__ void __launch_bounds__(TH, CTAS) sample_rows_kernel(const RSArgs a) {
   }
   // 2. the bins
   RSGeom& g = w.g;
-  g.from = st.mx;
-  g.far = fabsf(st.mx) >= RS_FAR;
-  if (g.far) {
-    st.mn = rs_seen(st.mn, g);
-    st.mx = 0.f;
-  }
-  g.mx = st.mx;
   const float tc = fminf(fmaxf(t, 0x1p-100f), 0x1p100f);
+  // a little more than the row's spread: the smallest logit lies in the last bin, not behind it
+  const float spread = (st.mx - st.mn) * (1.f + 0x1p-10f), span = fminf(spread, RS_SPAN * fmaxf(tc, 1.f));
+  g.from = st.mx;
+  g.far = fabsf(st.mx) * (float)RS_BINS > RS_FAR * fminf(spread, RS_TEMPS * tc);
+  if (g.far) st.mx = 0.f;
+  g.mx = st.mx;
   g.t = tc;
   g.inv_t = 1.f / tc;
-  // a little more than the row's spread: the smallest logit lies in the last bin, not behind it
-  const float span = fminf((st.mx - st.mn) * (1.f + 0x1p-10f), RS_SPAN * fmaxf(tc, 1.f));
   g.sx = span > 1e-30f ? (float)RS_BINS / span : 0.f;
   g.top = st.mx * g.sx;
   g.width = span > 1e-30f ? span / (float)RS_BINS : 0.f;
