@@ -15,8 +15,10 @@
 //      linear ones of max - l) that k of the threads' largest reach, 4096 of a long row: the first k tokens all lie up to
 //      there, and seldom many more.
 //   3. Rows of neither kind, or whose list is too long: a histogram of all tokens and their masses.  A bin's mass is
-//      w(edge) * sum of w / w(edge), the sum in fixed point, 43 bits below 21 of count in two words; bins are narrow, so
-//      w / w(edge) is near 1 and fp32 holds its distance from 1 to 2^-24 of that.  (One word of 22 bits below 10 was no
+//      w(edge) * sum of w / w(edge), the sum in fixed point, 43 bits below 21 of count in two words; these bins reach 40
+//      temperatures, not further, so each is T / 38 wide or less and w / w(edge) lies within 3 % of 1, where fp32 holds its
+//      distance from 1 to 2^-24 of that.  (Bins of 32 logits whatever T: at T = 0.001 a token's mass was rounded against an
+//      edge's 10^9 times its own, 7e-4 of a row's mass in all.  One word of 22 bits below 10 was no
 //      faster: shared-memory atomics cost 5 cycles a warp's worth, a token's arithmetic twice that.)
 //      Each prefix's end is then looked up in its bin: the bin's tokens are gathered and sorted, or, where they are too
 //      many (equal logits, coarse types), found by four rounds of 8 bits of the logit, after which the tokens left are
@@ -45,8 +47,8 @@ constexpr int RS_BINS = 1536;      // as many as leave room for two CTAs of 1900
 constexpr int RS_CAP = 1024;       // tokens that are sorted at once
 constexpr int RS_COUNT = 160;      // lists up to this long are sorted by counting
 constexpr uint32_t RS_ROOM = 4000;  // tokens of a CTA's bin that the sums have room for
-constexpr float RS_SPAN = 32.f;    // bins reach this many logits, or temperatures where that is more, below the largest
-constexpr float RS_TEMPS = 40.f;   // tokens this many temperatures below the largest have e^-40 of its weight, which counts as none
+constexpr float RS_SPAN = 32.f;    // bins of counts reach this many logits, or temperatures where that is more, below the largest
+constexpr float RS_TEMPS = 40.f;   // bins of masses this many temperatures: e^-40 of the largest's weight counts as none
 constexpr size_t RS_HALF = 76 * 1024;  // longest slice of which two fit an SM
 constexpr size_t RS_STAGE_MAX = 160 * 1024;  // longest slice that is kept in shared memory
 
@@ -90,6 +92,7 @@ struct RSSmem {
   RSStat wstat[RS_WARPS];
   double wsum[RS_WARPS];
   uint32_t wcnt[RS_WARPS];
+  float spread;                      // largest logit less smallest, and a little more
   uint32_t most[RS_CLUSTER], own_most;  // tokens of a share's fullest bin, where it has no room for them
   double sel_base, sel_mass, pick_w;
   uint32_t n_list, n_mine, list_at, over, sel_cnt, sel_in, pick_cnt, occur;
@@ -137,6 +140,14 @@ struct RSGeom {
 constexpr float RS_LEAST = -3e38f, RS_FAR = 0x1p21f;  // RS_FAR: bins
 constexpr int RS_SLACK = 1;
 __device__ __forceinline__ float rs_place(float l, const RSGeom& g) { return fmaf(-l, g.sx, g.top); }
+// the row's bins reach `most` logits below the largest, or the whole row where that is less
+__device__ __forceinline__ void rs_reach(RSGeom& g, float spread, float most) {
+  const float span = fminf(spread, most);
+  const bool some = span > 1e-33f;  // below that, 1/700 of the smallest temperature, all logits count as one
+  g.sx = some ? (float)RS_BINS / span : 0.f;
+  g.top = g.mx * g.sx;
+  g.width = some ? span / (float)RS_BINS : 0.f;
+}
 // NaN and -infinity have no place below RS_BINS
 __device__ __forceinline__ int rs_bin(float l, const RSGeom& g) {
   const float x = rs_place(l, g);
@@ -249,7 +260,6 @@ struct RSRow {
   template <bool MASSES>
   __device__ __forceinline__ void fill() {
     const float unit = unit_of();
-    const bool narrow = g.width * g.inv_t < 0x1p-4f;
     each([&](int, const float (&l)[V]) {
       int b[V], c[V];
       uint32_t old[V];
@@ -260,7 +270,7 @@ struct RSRow {
         if (!MASSES) continue;
         // y = (l - edge) / T: the two are near, their difference is exact but for what is below 2^-24 of a bin
         const float y = (l[j] - rs_edge(f - 8388608.f, g)) * g.inv_t;
-        const float e = narrow ? y * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 1.f / 120, 1.f / 24), 1.f / 6), 0.5f), 1.f) : expm1f(fminf(y, 0x1p-6f));
+        const float e = y * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 1.f / 120, 1.f / 24), 1.f / 6), 0.5f), 1.f);  // exp(y) - 1
         c[j] = (int)((uint32_t)__float2int_rn(e * unit) + (uint32_t)unit);
       }
 #pragma unroll
@@ -340,6 +350,7 @@ struct RSRow {
     const int tid = threadIdx.x;
     if (c.op == RS_FILL) {
       sure = c.sure;
+      rs_reach(g, s.spread, RS_TEMPS * (float)g.t);
       for (int i = tid; i < RS_BINS; i += TH) s.cnt[i] = s.low[i] = 0;
       __syncthreads();
       histogram(RS_MASSES, of_thread);
@@ -656,12 +667,22 @@ struct RSRow {
   __device__ __forceinline__ RSCommand step(RSLead& m, int r) {
     RSCommand c{};
     const bool by_p = m.top_p < 1, by_m = min_p > 0;
-    if (m.state == START && by_m) m.over = -log(min_p) * g.t * (double)g.sx;
+    if ((m.state == START || m.state == REFILLED) && by_m) m.over = -log(min_p) * g.t * (double)g.sx;
     const int over_bin = m.over < RS_BINS ? (int)fmax(m.over, 0.0) : RS_BINS;
     int idx = 0;          // what a look found
     double w = 0, mass = 0;
     uint32_t cnt = 0;
     const int near = RS_SLACK;
+    auto ended = [&](uint32_t cnt, double mass) {  // a prefix's end, and what it leads to
+      if (m.purpose != OF_P || cnt < m.kept) { m.kept = m.purpose == OF_M ? m.kept : cnt; m.mass = mass; }
+      const int was = m.purpose;
+      m.purpose = was == OF_K && by_p ? OF_P : was != OF_M && by_m ? OF_M : OF_TOKEN;
+    };
+    auto count_over = [&] {
+      m.state = COUNTED;
+      c.op = RS_OVER; c.b0 = over_bin - near; c.b1 = min(over_bin + near, RS_BINS);
+      return c;
+    };
     const bool first = m.state == START;
     if (first) {
       c.op = RS_GATHER;
@@ -715,11 +736,7 @@ struct RSRow {
       m.kept = m.cut;
       m.mass = all_mass;
       m.purpose = m.cut_k ? OF_K : by_p ? OF_P : by_m ? OF_M : OF_TOKEN;
-      if (m.purpose == OF_M) {
-        m.state = COUNTED;
-        c.op = RS_OVER; c.b0 = over_bin - near; c.b1 = min(over_bin + near, RS_BINS);
-        return c;
-      }
+      if (m.purpose == OF_M) return count_over();
     } else if (m.state == LOOKED) {
       const int n_list = (int)s.n_list;
       sort(n_list);
@@ -795,24 +812,23 @@ struct RSRow {
         answer(r, idx, w / m.mass, m.kept);
         return c;
       } else {
-        if (m.purpose != OF_P || cnt < m.kept) { m.kept = m.purpose == OF_M ? m.kept : cnt; m.mass = mass; }
-        const int was = m.purpose;
-        m.purpose = was == OF_K && by_p ? OF_P : was != OF_M && by_m ? OF_M : OF_TOKEN;
-        if (m.purpose == OF_M) {
-          m.state = COUNTED;
-          c.op = RS_OVER; c.b0 = over_bin - near; c.b1 = min(over_bin + near, RS_BINS);
-          return c;
-        }
+        ended(cnt, mass);
+        if (m.purpose == OF_M) return count_over();
       }
     }
     // LOOK
-    m.by_mass = m.purpose == OF_P || m.purpose == OF_TOKEN;
-    m.strict = m.purpose == OF_TOKEN;
-    m.target = m.purpose == OF_P ? m.top_p * m.mass : m.purpose == OF_TOKEN ? m.u * m.mass : (double)m.kept;
-    m.b = cross_one(m.by_mass, m.target, m.strict);
     uint32_t in;
     double in_mass;
-    at_bin(m.b, &m.before, &m.base, &in, &in_mass);
+    for (;;) {
+      m.by_mass = m.purpose == OF_P || m.purpose == OF_TOKEN;
+      m.strict = m.purpose == OF_TOKEN;
+      m.target = m.purpose == OF_P ? m.top_p * m.mass : m.purpose == OF_TOKEN ? m.u * m.mass : (double)m.kept;
+      m.b = cross_one(m.by_mass, m.target, m.strict);
+      at_bin(m.b, &m.before, &m.base, &in, &in_mass);
+      if (m.b < RS_BINS || m.purpose >= OF_TOKEN) break;
+      ended(m.kept, m.base);  // by count, and behind the bins, where nothing has a mass: which token it is does not matter
+      if (m.purpose == OF_M) return count_over();
+    }
     if (in <= RS_CAP) {
       m.state = LOOKED;
       c.op = RS_GATHER; c.b0 = c.b1 = m.b;
@@ -922,16 +938,14 @@ __global__ void __launch_bounds__(TH, CTAS) sample_rows_kernel(const RSArgs a) {
   RSGeom& g = w.g;
   const float tc = fminf(fmaxf(t, 0x1p-100f), 0x1p100f);
   // a little more than the row's spread: the smallest logit lies in the last bin, not behind it
-  const float spread = (st.mx - st.mn) * (1.f + 0x1p-10f), span = fminf(spread, RS_SPAN * fmaxf(tc, 1.f));
+  const float spread = (st.mx - st.mn) * (1.f + 0x1p-10f);
+  if (tid == 0) s.spread = spread;
   g.from = st.mx;
   g.far = fabsf(st.mx) * (float)RS_BINS > RS_FAR * fminf(spread, RS_TEMPS * tc);
   if (g.far) st.mx = 0.f;
   g.mx = st.mx;
   g.t = tc;
   g.inv_t = 1.f / tc;
-  g.sx = span > 1e-30f ? (float)RS_BINS / span : 0.f;
-  g.top = st.mx * g.sx;
-  g.width = span > 1e-30f ? span / (float)RS_BINS : 0.f;
   w.min_p = q > 0.f ? (double)q : 0.0;
   w.all_cnt = st.n;
   const bool cut_k = k > 0 && (uint32_t)k < st.n, by_p = p < 1.f;
@@ -939,6 +953,7 @@ __global__ void __launch_bounds__(TH, CTAS) sample_rows_kernel(const RSArgs a) {
                    // the k largest are sure to be few more than k where k is a small part of the threads' largest
                    : cut_k && k <= RS_CAP / 2             ? (k <= a.vocab / (32 / (int)sizeof(T)) / 4 && k <= TH * CL / 8 ? RS_LARGEST : RS_COUNTS)
                                                           : RS_MASSES;
+  rs_reach(g, spread, mode == RS_MASSES ? RS_TEMPS * tc : RS_SPAN * fmaxf(tc, 1.f));
   if (mode != RS_NONE) {
     w.histogram(mode, largest);
     rs_sync<CL>();
