@@ -967,7 +967,7 @@ __global__ void __launch_bounds__(TH, CTAS) sample_rows_kernel(const RSArgs a) {
     m.cut_k = cut_k;
     m.cut = cut_k ? (uint32_t)k : st.n;
     m.top_p = by_p ? (double)p : 1.0;
-    m.u = un > 0.f ? fmin((double)un, 1.0) : 0.0;
+    m.u = un > 0.f ? (double)fminf(un, 1.f - 0x1p-24f) : 0.0;  // not 1: the last kept token may have no mass
     s.lead = m;
   }
   __syncthreads();
