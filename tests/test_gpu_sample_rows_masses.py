@@ -57,3 +57,10 @@ def test_masses_at_all_temperatures(dtype, T):
     q = np.array([0, 0, 0, 0, 0, 1e-4, 0, 1e-3, 0, 1e-20])
     check(rows(rng, 10, 50257), dtype, T, k, p, q, rng.random(10), slack=MASSES)
     check(rows(rng, 10, 33000, peaks=24), dtype, T, k, p, q, rng.random(10), slack=MASSES)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_the_longest_row(dtype):
+    """2^23 logits: half a unit is 2^-23 of an edge's weight there, and a sum is off by 2^-22 of itself."""
+    rng = np.random.default_rng(23)
+    check(2.2 * rng.standard_normal((2, 1 << 23)) + 5, dtype, [1.0, 0.3], [0, 300000], [0.99, 1.0], 0.0, rng.random(2), slack=2.0 ** -21)
