@@ -149,16 +149,19 @@ int n730_qgemm(void* qw, const float* d_x, int ldx, int tokens, float* d_y, int 
 int n730_sample(const float* d_logits, int batch, int vocab, int ld, float temperature, float top_p,
                 uint64_t seed, uint64_t counter, int32_t* d_tokens, float* d_u, void* stream);
 /* Sampling with each row's own settings and given random numbers: for each of `batch` rows of d_logits
- * (type N730_F32 / F16 / BF16, row stride ld >= vocab; up to 2^24 rows of up to 2^23), d_temperature <= 0 gives the first
- * index of the largest logit; otherwise tokens are ordered by logit (ties by index) with weights
+ * (type N730_F32 / F16 / BF16, row stride ld >= vocab; up to 2^24 rows of up to 2^23), d_temperature <= 0 or NaN gives the
+ * first index of the largest logit; otherwise tokens are ordered by logit (ties by index) with weights
  * w = exp((logit - largest) / temperature), and kept are the first d_top_k of them (<= 0: all), of those the
  * shortest prefix whose mass reaches d_top_p times theirs (>= 1 or NaN: all), and of those the ones with
  * w >= d_min_p (<= 0 or NaN: all); one token always is.  The token is the first whose cumulative mass exceeds
- * d_u[row] (in [0, 1); outside: the nearest of that) times the kept mass.  Logits of -infinity or NaN are no
+ * d_u[row] (in [0, 1); outside: the nearest of that, NaN: 0) times the kept mass.  Logits of -infinity or NaN are no
  * tokens (a row of them answers -1); beside one of +infinity only its equals have a weight.  Arrays of settings are
  * on the device, one value a row; null: temperature 1, no cut.  d_tokens [batch] out; d_prob (may be null): the
- * token's share of the kept mass; d_kept (may be null): how many tokens were kept.  Weights and masses are
- * formed in 64 bits.  Asynchronous on `stream`, needs no workspace, can be captured into a graph. */
+ * token's share of the kept mass; d_kept (may be null): how many tokens were kept.  Rows that a list of up to 1024
+ * tokens settles (a top-k up to 512, a min-p without a top-p, few tokens) go by weights and sums in 64 bits.  The others go
+ * by sums that are held to 2^-25 of themselves (2^-22 beyond 2^20 logits), so a border nearer than twice that to a
+ * token's may go either way, and tokens more than 40 temperatures below the largest have no mass there.  The same
+ * inputs give the same answer.  Asynchronous on `stream`, needs no workspace, can be captured into a graph. */
 int n730_sample_rows(const void* d_logits, int dtype, int batch, int vocab, int64_t ld, const float* d_temperature,
                      const int32_t* d_top_k, const float* d_top_p, const float* d_min_p, const float* d_u,
                      int32_t* d_tokens, float* d_prob, int32_t* d_kept, void* stream);
@@ -304,7 +307,8 @@ typedef struct N730KV16Cache {
 } N730KV16Cache;
 /* Append rows of K and V, [n_kv][head_dim] each, behind the cached positions, K rotated by r (null: as it is) and
  * both rounded to the cache's type; with d_q, query rows [n_heads][head_dim] are rotated into d_q_out as well
- * (in place with d_q_out = d_q).  Positions are d_pos[row] (null: *prefix_len + d_lens[b] + t).  Rows past the
+ * (in place with d_q_out = d_q), in the rows' own type: n730_kv16_attention reads queries of the cache's type and has
+ * none to compare, so rows that go on to it have to be of that type here.  Positions are d_pos[row] (null: *prefix_len + d_lens[b] + t).  Rows past the
  * table's capacity are dropped, rows from d_new[b] on left as they were.  d_lens is not changed.  Pages that are
  * written must not be shared between sequences. */
 int n730_kv16_append(const N730KV16Cache* c, const N730Rotary* r, const void* d_q, int64_t ldq, void* d_q_out,

@@ -27,8 +27,9 @@
 // which the softmax is 2.2k, the products 1.0k and hand-offs the rest.  32 of 28 heads behind 8131: 24 us, 6 of them the
 // bytes of K and V.
 //
-// Every wait is bounded; one that runs out sets the workspace's status word, ends the CTA's work and still frees the
-// tensor memory.
+// Every wait for an mbarrier is bounded; one that runs out sets the workspace's status word, ends the CTA's work and still
+// frees the tensor memory.  The named barriers of a row's two warps have no limit of their own: a warp that gives up arrives
+// once for its partner, which then finds the abort flag at its next wait.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -506,7 +507,7 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
 // queries their columns (mma.m16n8k16): S^T = K Q^T, O^T += V^T P^T, so that nothing is spent on the 128 rows that a
 // tensor-memory tile would have; with single tokens this is bound by the bytes of K and V.  P^T's fragments are those of
 // S^T transposed, 8 x 8 at a time, in registers.  Rows arrive by asynchronous copies, three blocks of 16 positions deep;
-// no warp waits for another, and a CTA is one warp of KO_STAGE * 3 bytes, so that it finds room beside the CTA of the
+// no warp waits for another, and a CTA is one warp with KOCfg's three stages, so that it finds room beside the CTA of the
 // prefix's kernel that is running (1024 items of 64 heads x 128, 144 positions: 46 us by the kernel above, most of that
 // hidden here).
 template <int HD> struct KOCfg { static constexpr int KB = 16 * HD * 2, STAGE = 2 * KB, STAGES = 3; };

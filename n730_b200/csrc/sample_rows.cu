@@ -23,8 +23,9 @@
 //      Each prefix's end is then looked up in its bin: the bin's tokens are gathered and sorted, or, where they are too
 //      many (equal logits, coarse types), found by four rounds of 8 bits of the logit, after which the tokens left are
 //      equal and go by index.
-// One row of 152064 with a top-k is bound by six meetings of the cluster, 1.2 us each (11.7 us); many rows without one by
-// a token's arithmetic: 192 rows of 152064 bf16 logits 139 us, 42 % of issue slots, 0.42 TB/s.
+// One row of 152064 with a top-k is bound by six meetings of the cluster, 1.2 us each (11.6 us).  192 rows of 152064 bf16
+// logits without one take 136 us, 0.43 TB/s at 39 % of the issue slots: a token's polynomial and two dependent atomics, behind
+// a pass for the largest, and CTAs that wait while the first one looks ends up (barriers are the longest stall).
 // Sums are integers, or 64-bit floats in a fixed order: the same inputs give the same token.
 #include <cooperative_groups.h>
 
@@ -38,9 +39,9 @@ namespace cg = cooperative_groups;
 
 constexpr int RS_CLUSTER = 8;      // most CTAs of a row
 // Threads of a CTA: 512 and all of an SM's registers while a row's CTAs find an SM each (one row of 152064 without a cut:
-// 21.7 us, 24.1 with 256), 256 beyond that.  Then two CTAs an SM, or three of 16-bit logits, which shared memory has room
+// 20.8 us, 22.3 with 256), 256 beyond that.  Then two CTAs an SM, or three of 16-bit logits, which shared memory has room
 // for, where that saves more waves than registers that do not suffice cost (192 rows of 152064
-// bf16 logits without a cut: 139 us, 157 with two; 40 rows of 100000, where it does not: 39, and 31 with two).
+// bf16 logits without a cut: 136 us, 152 with two; 40 rows of 100000, where it does not: 38, and 31 with two).
 constexpr int RS_THREADS_FEW = 512, RS_THREADS_MANY = 256;
 constexpr int RS_WARPS = RS_THREADS_FEW / 32;  // most warps
 constexpr int RS_BINS = 1536;      // as many as leave room for two CTAs of 19008 fp32 logits (a row of 152064) an SM
@@ -1005,8 +1006,8 @@ static int rs_launch_many(const RSArgs& a, int batch, size_t slice, int ctas, cu
   return rs_launch_one<T, STAGED, CL, RS_THREADS_MANY, 2>(a, batch, slice, st);
 }
 // CTAs of a row: what takes the fewest waves of CTAs times a CTA's time, in us: 12 of meetings (6 without other CTAs), and
-// the logits' share.  Measured, 1, 2, 4 and 8 CTAs: 256 rows of 32000 fp32 logits 40, 42, 53, 86 us; 8 rows of them without
-// a top-k 19 and 13 (1 and 8); 64 rows of 151936 52 and 50 (4 and 8); 8 rows of 1000 8 and 11.
+// the logits' share.  Measured, 1, 2, 4 and 8 CTAs: 256 rows of 32000 fp32 logits 39, 42, 53, 86 us; 8 rows of them without
+// a top-k 18 and 11 (1 and 8); 64 rows of 151936 49 and 48 (4 and 8); 8 rows of 1000 with a top-k 8 and 10.
 template <class T>
 static int rs_launch(RSArgs& a, int batch, cudaStream_t st) {
   auto slice = [&](int cl) { return (size_t)(((a.vocab + cl - 1) / cl + 7) / 8 * 8) * sizeof(T); };

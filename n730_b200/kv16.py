@@ -74,7 +74,8 @@ class KV16Cache:
     def append(self, k: int, v: int, dtype: str, batch: int, tokens: int, lens: int, *, new: int = 0, ld: int = 0,
                rotary: Rotary | None = None, pos: int = 0, q: int = 0, q_out: int = 0, heads: int = 0, ldq: int = 0,
                ldqo: int = 0, stream: int = 0):
-        """Rows k (rotated) and v behind lens[b] cached positions; with q, its rows rotated into q_out."""
+        """Rows k (rotated) and v behind lens[b] cached positions; with q, its rows rotated into q_out.  All rows are of
+        ``dtype``, q_out too; ``attention`` reads queries of the cache's own."""
         row = heads * self.c.head_dim
         _lib.check(self.lib.n730_kv16_append(self._ref, rotary._ref if rotary else 0, q, ldq or row, q_out, ldqo or row, heads,
                                              k, v, ld or self.row, DTYPES[dtype], batch, tokens, lens, new, pos, stream),
@@ -87,7 +88,8 @@ class KV16Cache:
 
     def attention(self, q: int, out: int, batch: int, tokens: int, heads: int, lens: int, *, new: int = 0,
                   scale: float | None = None, ldq: int = 0, ldo: int = 0, ws: int = 0, ws_bytes: int = 0, stream: int = 0):
-        """Queries of the newest rows over the prefix and the own positions; scale defaults to head_dim ** -0.5."""
+        """Queries of the newest rows, of the cache's type as out is, over the prefix and the own positions; scale defaults
+        to head_dim ** -0.5."""
         dim = self.c.head_dim
         _lib.check(self.lib.n730_kv16_attention(self._ref, q, ldq or heads * dim, batch, tokens, heads,
                                                 dim ** -0.5 if scale is None else scale, lens, new, out, ldo or heads * dim,
