@@ -324,9 +324,9 @@ int64_t n730_kv16_attention_ws(const N730KV16Cache* c, int batch, int tokens, in
  * n730_kv16_append with the same d_lens and d_new.  Keys and values of the prefix are read once for the whole batch.
  * d_q and d_out rows are [n_heads][head_dim] of the cache's type (query head i reads KV head i / (n_heads / n_kv));
  * out rows from d_new[b] on are left as they were; a query that sees no position gives zeros.  d_out must not overlap
- * d_q.  Scores are scaled by `scale`.  Softmax weights are rounded to the cache's type before they meet V; sums and
- * outputs are fp32 until the end.  What lies behind a sequence's or the prefix's last position may be anything, NaN
- * included. */
+ * d_q.  Scores are scaled by `scale`; they may be as large as fp32 holds, but rows with one beyond 10^7 are slow.
+ * Softmax weights are rounded to the cache's type before they meet V; sums and outputs are fp32 until the end.  What
+ * lies behind a sequence's or the prefix's last position may be anything, NaN included. */
 int n730_kv16_attention(const N730KV16Cache* c, const void* d_q, int64_t ldq, int batch, int tokens, int n_heads,
                         float scale, const int32_t* d_lens, const int32_t* d_new, void* d_out, int64_t ldo, void* d_ws,
                         int64_t ws_bytes, void* stream);

@@ -16,7 +16,11 @@
 //
 // Softmax.  A row's reference follows its maximum lazily: it moves when a weight would pass 2^KA_MOST, so outputs in
 // tensor memory are seldom rescaled.  Weights are at most 2^8, the largest at least 1: fp16 holds them to 2^-11, and
-// those below 2^-14 to 2^-25.
+// those below 2^-14 to 2^-25.  Score x scale less the reference is rounded once, so whatever the reference was rounded to, a
+// part's sums go with it exactly.  Its rounding stays in every weight's exponent, half a step of it at most: beyond
+// 2^24 that is more than weights have room for.  A row that meets such a reference is marked (no number for a reference),
+// and the joining kernel forms it again by itself, score x scale rounded first.  (To do that in the softmax cost 3 to 8 % of
+// every call: 81 us -> 84 to 88.  A token whose 28 rows are all marked takes 7 ms behind 16384 positions.)
 //
 // What lies behind the last position anyone sees may be anything: scores are masked, and those rows of V are zeroed in
 // shared memory before the product (zero weight times NaN is NaN).  Rows of V that some rows of the item see and others
@@ -44,6 +48,7 @@ namespace n730 {
 
 constexpr int KA_KEYS = 128;       // positions of a tile
 constexpr float KA_MOST = 8.f;     // log2 of how large a weight may grow against its reference
+constexpr float KA_FAR = 0x1p24f;  // references beyond this leave nothing of a score behind its own rounding
 constexpr int KA_RING = 4;         // tiles whose masks are kept
 constexpr int KA_BAD = 256;        // positions of an item that some of its rows see and others do not: fewer than its rows
 
@@ -76,6 +81,7 @@ struct KASmem {
   int abort;
   int n_bad, bad[KA_BAD];
   float half[2][NT][2][128];  // by tile's parity, row tile, half: what the two threads of a row tell each other
+  uint8_t far[Cfg::ROWS];     // whether a row has met a reference beyond KA_FAR
 };
 
 // Parts of one kind (the prefix's or the sequences' own): [unit][split][4 channels][rows of a unit], a unit being a KV
@@ -130,12 +136,13 @@ __device__ __forceinline__ float ka_row_max(float y, float* mine, const float* o
   return fmaxf(y, *other);
 }
 // Moves a row's reference to its tile's maximum y where that is larger; the thread's sum and, when there are any, its
-// half of the outputs (at to) follow.
+// half of the outputs (at to) follow.  far: the row's mark.
 template <int HD>
-__device__ __forceinline__ void ka_move(uint32_t to, bool outputs, float y, float& m, float& l) {
+__device__ __forceinline__ void ka_move(uint32_t to, bool outputs, float y, float& m, float& l, uint8_t* far) {
   const float mn = fmaxf(m, y), f = mn == m ? 1.f : ex2(m - mn);
   m = mn;
   l *= f;
+  if (fabsf(mn) > KA_FAR && fabsf(mn) < INFINITY) *far = 1;
   if (!outputs) return;
 #pragma unroll 1
   for (int cc = 0; cc < HD / 2; cc += 8) tc_scale8(to + cc, f);
@@ -145,14 +152,14 @@ __device__ __forceinline__ void ka_move(uint32_t to, bool outputs, float y, floa
 // half's scores; tp: its weights, which lie over the first half's scores.
 template <int HD, bool BF>
 __device__ __forceinline__ void ka_softmax(uint32_t ts, uint32_t tp, uint32_t to, float c, bool outputs, float* mine,
-                                           const float* other, int bar, float& m, float& l) {
+                                           const float* other, int bar, uint8_t* far, float& m, float& l) {
   float v[64];
   tc_ld64(ts, v);
   float mx[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
   for (int i = 4; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
   const float y = ka_row_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c, mine, other, bar);
-  if (__any_sync(0xffffffffu, y > m + KA_MOST)) ka_move<HD>(to, outputs, y, m, l);
+  if (__any_sync(0xffffffffu, y > m + KA_MOST)) ka_move<HD>(to, outputs, y, m, l, far);
   const float ms = m == -INFINITY ? 0.f : m;
   const float2 c2 = both(c), m2 = both(-ms);
   float2 sum[2] = {both(0.f), both(0.f)};
@@ -171,7 +178,7 @@ __device__ __forceinline__ void ka_softmax(uint32_t ts, uint32_t tp, uint32_t to
 // The same where the row sees the first `sees` positions of the half, of those the ones that have a page.
 template <int HD, bool BF>
 __device__ __forceinline__ void ka_softmax_some(uint32_t ts, uint32_t tp, uint32_t to, float c, int sees, uint32_t pages, bool outputs,
-                                                float* mine, const float* other, int bar, float& m, float& l) {
+                                                float* mine, const float* other, int bar, uint8_t* far, float& m, float& l) {
   float v[64], mx = -INFINITY;
   tc_ld64(ts, v);
 #pragma unroll
@@ -180,7 +187,7 @@ __device__ __forceinline__ void ka_softmax_some(uint32_t ts, uint32_t tp, uint32
     mx = fmaxf(mx, v[i]);
   }
   const float y = ka_row_max(mx == -INFINITY ? mx : mx * c, mine, other, bar);  // c may be 0
-  if (__any_sync(0xffffffffu, y > m + KA_MOST)) ka_move<HD>(to, outputs, y, m, l);
+  if (__any_sync(0xffffffffu, y > m + KA_MOST)) ka_move<HD>(to, outputs, y, m, l, far);
   const float ms = m == -INFINITY ? 0.f : m;
   uint32_t w[32];
   float sum = 0.f;
@@ -401,6 +408,7 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
     const uint32_t to = tmem + ((uint32_t)(wq * 32) << 16) + Cfg::O0 + x * HD + half * (HD / 2);
     const int bar = 1 + x * 4 + wq;  // named barrier of the row's two warps
     float m = -INFINITY, l = 0.f;
+    sm.far[r] = 0;  // by both of its threads, who meet before either may set it
     bool go = true;
     for (int j = 0; j < nt; ++j) {
       if (!kp_wait_warp(&sm.sfull[x], (uint32_t)(j & 1), abortf)) { go = false; break; }
@@ -411,9 +419,9 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
       const float* other = &sm.half[j & 1][x][half ^ 1][wq * 32 + lane];
       const bool whole = p0 + KA_KEYS <= sees_all && pages == 0xffu;
       if (some_live) {  // rows of nobody keep what is there as their weights
-        if (whole) ka_softmax<HD, BF>(ts + half * 64, ts + half * 32, to, a.scale_log2e, j > 0, mine, other, bar, m, l);
+        if (whole) ka_softmax<HD, BF>(ts + half * 64, ts + half * 32, to, a.scale_log2e, j > 0, mine, other, bar, &sm.far[r], m, l);
         else ka_softmax_some<HD, BF>(ts + half * 64, ts + half * 32, to, a.scale_log2e, vis - p0 - half * 64, pages >> (4 * half), j > 0,
-                                     mine, other, bar, m, l);
+                                     mine, other, bar, &sm.far[r], m, l);
       }
       if (!whole) {
         if (x == 0 && half == 0 && p0 + KA_KEYS > sees_all) {  // rows of V that not everyone sees
@@ -456,7 +464,7 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
         float* sum = &sm.half[nt & 1][x][1][wq * 32 + lane];
         if (half) *sum = l;
         asm volatile("bar.sync %0, 64;" :: "r"(bar) : "memory");
-        if (!half && live) part.ml[unit * part.rows + f] = make_float2(m, l + *sum);
+        if (!half && live) part.ml[unit * part.rows + f] = make_float2(sm.far[r] ? NAN : m, l + *sum);
       }
       const float ms = m == -INFINITY ? 0.f : m;
 #pragma unroll 1
@@ -645,9 +653,10 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
         const int p = p0 + (lane >> 2);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          x[y][e] = p < vis[y][e] ? (x[y][e] + x2[y][e]) * a.scale_log2e : -INFINITY;
-          x[y][2 + e] = p + 8 < vis[y][e] ? (x[y][2 + e] + x2[y][2 + e]) * a.scale_log2e : -INFINITY;
+          x[y][e] = p < vis[y][e] ? x[y][e] + x2[y][e] : -INFINITY;
+          x[y][2 + e] = p + 8 < vis[y][e] ? x[y][2 + e] + x2[y][2 + e] : -INFINITY;
           big[e] = fmaxf(x[y][e], x[y][2 + e]);
+          big[e] = big[e] == -INFINITY ? big[e] : big[e] * a.scale_log2e;  // the scale may be 0
         }
         if (__any_sync(0xffffffffu, big[0] > m[y][0] + KA_MOST || big[1] > m[y][1] + KA_MOST)) {
 #pragma unroll
@@ -670,7 +679,9 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float ms = m[y][e & 1] == -INFINITY ? 0.f : m[y][e & 1];
-          e4[y][e] = ex2(x[y][e] - ms);
+          // in one step with the reference, as the kernel above; beyond KA_FAR in a step of its own
+          const float2 f = fabsf(ms) > KA_FAR ? make_float2(a.scale_log2e, 1.f) : make_float2(1.f, a.scale_log2e);
+          e4[y][e] = x[y][e] == -INFINITY ? 0.f : ex2(fmaf(x[y][e] * f.x, f.y, -ms));
           l[y][e & 1] += e4[y][e];
         }
         w[y][0] = ko_transpose(ka_pack<BF>(e4[y][0], e4[y][1]));
@@ -739,18 +750,82 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
   if (blockIdx.x == 0) pdl_wait();
 }
 
+// A marked row by itself, by all warps of a CTA: 4 positions at a time each, a lane its share of the channels.  CH of the row's
+// channels, from `ch` on.  Inline: a call's stack cost every launch of the joining kernel 1 us.
+template <int HD, bool BF, int CH, int WARPS>
+__device__ __forceinline__ void ka_again(const KAArgs& a, int b, int t, int h, int g, int ch, float (&part)[WARPS][CH + 2]) {
+  constexpr int QL = HD / 32, VL = CH / 32, N = 4;
+  const N730KV16Cache& c = a.c;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int cap = c.max_pages * c.page_size, prefix = kv16_prefix(c), all = prefix + min(kv8_len(a.lens, b, cap) + t + 1, cap);
+  const int64_t at = (int64_t)(b * a.tokens + t), col = (int64_t)(h * a.group + g) * HD;
+  const float scale = a.sign ? -a.scale_log2e : a.scale_log2e;
+  float q[QL], m = -INFINITY, l = 0.f, o[VL] = {};
+#pragma unroll
+  for (int e = 0; e < QL; ++e) q[e] = kv8_load1(a.q, at * a.ldq + col + lane * QL + e, c.dtype);
+#pragma unroll 1
+  for (int i0 = warp * N; i0 < all; i0 += WARPS * N) {
+    int64_t row[N];  // -1: a position that is none
+    float x[N], mn = m;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int i = i0 + k, p = i < prefix ? i : i - prefix;
+      const int page = i >= all ? -1 : i < prefix ? c.prefix_table[p / c.page_size] : c.block_table[(int64_t)b * c.max_pages + p / c.page_size];
+      row[k] = (unsigned)page < (unsigned)c.n_pages ? (((int64_t)page * c.n_kv + h) * c.page_size + p % c.page_size) * HD : -1;
+      x[k] = 0.f;
+      if (row[k] >= 0)
+#pragma unroll
+        for (int e = 0; e < QL; ++e) x[k] = fmaf(q[e], kv8_load1(c.k, row[k] + lane * QL + e, c.dtype), x[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      x[k] = row[k] < 0 ? -INFINITY : warp_sum(x[k]) * scale;
+      mn = fmaxf(mn, x[k]);
+    }
+    const float f = mn == m ? 1.f : ex2(m - mn);
+    m = mn;
+    l *= f;
+#pragma unroll
+    for (int e = 0; e < VL; ++e) o[e] *= f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      if (row[k] < 0) continue;
+      const float w = x[k] == -INFINITY ? 0.f : ex2(x[k] - m);
+      l += w;
+#pragma unroll
+      for (int e = 0; e < VL; ++e) o[e] = fmaf(w, kv8_load1(c.v, row[k] + ch + lane * VL + e, c.dtype), o[e]);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < VL; ++e) part[warp][lane * VL + e] = o[e];
+  if (lane == 0) { part[warp][CH] = m; part[warp][CH + 1] = l; }
+  __syncthreads();
+  if ((int)threadIdx.x >= CH) return;
+  m = -INFINITY;
+  for (int w = 0; w < WARPS; ++w) m = fmaxf(m, part[w][CH]);
+  float sum = 0.f, y = 0.f;
+  for (int w = 0; w < WARPS; ++w) {
+    const float f = part[w][CH] == -INFINITY ? 0.f : ex2(part[w][CH] - m);
+    sum += part[w][CH + 1] == 0.f ? 0.f : part[w][CH + 1] * f;
+    y = fmaf(part[w][threadIdx.x], f, y);
+  }
+  kv8_store1(a.out, at * a.ldo + col + ch + threadIdx.x, BF ? N730_BF16 : N730_F16, sum == 0.f ? 0.f : y / sum);
+}
+
 // Joins the rows' parts.  A CTA takes 32 rows of a KV head, a lane a row, and PIECES groups of 4 channels; its warps take
 // MINE of these each, and every PARTS-th part: with few rows that is 32 channels and a quarter of the parts, so that a
 // part's trip to memory is paid for few times in a row (896 rows of 17 parts: 7 us, 11 with a CTA for all channels), with
 // many all channels and parts (8192 rows of 5 parts: 10 us, 17 the other way).  Outputs change places in shared memory so
 // that they leave as whole rows.
 template <int HD, bool BF, int MINE, int COLS, int PARTS>
-__global__ void __launch_bounds__(COLS * PARTS * 32) kv16_join_kernel(const KAArgs a) {
+__global__ void __launch_bounds__(COLS * PARTS * 32) kv16_join_kernel(const __grid_constant__ KAArgs a) {
   constexpr int PIECES = MINE * COLS;
   __shared__ uint2 out[32][PIECES + 1];
   __shared__ float4 other[PARTS > 1 ? PARTS - 1 : 1][PARTS > 1 ? MINE : 1][COLS][32];
   __shared__ float most[PARTS][32], sums[PARTS][32];
   __shared__ int64_t to[32];
+  __shared__ float marked[COLS * PARTS][PIECES * 4 + 2];
   const N730KV16Cache& c = a.c;
   const int lane = threadIdx.x & 31, col = (threadIdx.x >> 5) % COLS, turn = threadIdx.x / (COLS * 32);
   const int G = a.group, cap = c.max_pages * c.page_size, h = blockIdx.y, piece = blockIdx.z * PIECES + col * MINE;
@@ -769,13 +844,20 @@ __global__ void __launch_bounds__(COLS * PARTS * 32) kv16_join_kernel(const KAAr
   const int n = np + no;  // parts: the prefix's, then the own ones
   pdl_wait();
   float big = -INFINITY, sum = 0.f;
+  bool again = false;  // a part has no number for a reference
 #pragma unroll 4
-  for (int i = turn; i < n; i += PARTS)
-    big = fmaxf(big, (i < np ? a.pre.ml[(p0 + i) * a.pre.rows + r] : a.own.ml[(o0 + i - np) * a.own.rows + f]).x);
-  if (col == 0) most[turn][lane] = big;
+  for (int i = turn; i < n; i += PARTS) {
+    const float m = (i < np ? a.pre.ml[(p0 + i) * a.pre.rows + r] : a.own.ml[(o0 + i - np) * a.own.rows + f]).x;
+    big = fmaxf(big, m);
+    again = again || m != m;
+  }
+  if (col == 0) most[turn][lane] = again ? NAN : big;
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < PARTS; ++k) big = fmaxf(big, most[k][lane]);
+  for (int k = 0; k < PARTS; ++k) {
+    big = fmaxf(big, most[k][lane]);
+    again = again || most[k][lane] != most[k][lane];
+  }
   float4 acc[MINE];
 #pragma unroll
   for (int e = 0; e < MINE; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -800,7 +882,7 @@ __global__ void __launch_bounds__(COLS * PARTS * 32) kv16_join_kernel(const KAAr
     for (int e = 0; e < MINE; ++e) other[turn - 1][e][col][lane] = acc[e];
   }
   if (col == 0) sums[turn][lane] = sum;
-  if (threadIdx.x < 32) to[lane] = live ? (int64_t)tok * a.ldo + (int64_t)(h * G + g) * HD + blockIdx.z * (PIECES * 4) : -1;
+  if (threadIdx.x < 32) to[lane] = live && !again ? (int64_t)tok * a.ldo + (int64_t)(h * G + g) * HD + blockIdx.z * (PIECES * 4) : -1;
   __syncthreads();
   if (!turn) {
 #pragma unroll
@@ -828,6 +910,11 @@ __global__ void __launch_bounds__(COLS * PARTS * 32) kv16_join_kernel(const KAAr
     } else {
       dst[0] = (uint16_t)y.x; dst[1] = (uint16_t)(y.x >> 16); dst[2] = (uint16_t)y.y; dst[3] = (uint16_t)(y.y >> 16);
     }
+  }
+  for (unsigned marks = __ballot_sync(0xffffffffu, again); marks; marks &= marks - 1) {  // the same in every warp
+    const int k = __ffs(marks) - 1;
+    ka_again<HD, BF, PIECES * 4, COLS * PARTS>(a, __shfl_sync(0xffffffffu, b, k), __shfl_sync(0xffffffffu, t, k), h,
+                                               __shfl_sync(0xffffffffu, g, k), blockIdx.z * (PIECES * 4), marked);
   }
 }
 
