@@ -1066,7 +1066,8 @@ N730_API int n730_kv16_attention(const N730KV16Cache* c, const void* d_q, int64_
                (long long)ldo, n_heads, c->head_dim);
   N730_REQUIRE(kv8_aligned(2, (const char*)d_q, (const char*)d_out) && kv8_aligned(4, d_lens, d_new), N730_BAD_ARG,
                "%s: pointers must lie on whole elements", what);
-  N730_REQUIRE(std::isfinite(scale), N730_BAD_ARG, "%s: scale %g", what, scale);
+  const float scale_log2e = scale * 1.4426950408889634f;
+  N730_REQUIRE(std::isfinite(scale_log2e), N730_BAD_ARG, "%s: scale %g", what, scale);
   N730_REQUIRE(((uintptr_t)d_ws & 15) == 0, N730_BAD_ARG, "%s: the workspace must be 16-byte aligned", what);
   const KAPlan p = ka_plan(*c, batch, tokens, n_heads);
   N730_REQUIRE(ws_bytes >= p.bytes, N730_BAD_ARG, "%s: workspace of %lld bytes, %lld needed", what, (long long)ws_bytes,
@@ -1081,7 +1082,7 @@ N730_API int n730_kv16_attention(const N730KV16Cache* c, const void* d_q, int64_
   while (a.box < KA_KEYS && c->page_size % (2 * a.box) == 0) a.box *= 2;
   a.qvec = ((uintptr_t)d_q & 15) == 0 && ldq % 8 == 0;
   a.ovec = ((uintptr_t)d_out & 7) == 0 && ldo % 4 == 0;
-  a.scale_log2e = std::fabs(scale) * 1.4426950408889634f;
+  a.scale_log2e = std::fabs(scale_log2e);
   a.sign = scale < 0 ? 0x80008000u : 0u;
   a.lens = d_lens; a.n_new = d_new;
   a.status = reinterpret_cast<int*>(ws);
