@@ -15,8 +15,8 @@
 // 16 to 128 rows a copy; positions without a page are copied from behind the pool's end, which gives zeros.
 //
 // Softmax.  A row's reference follows its maximum lazily: it moves when a weight would pass 2^KA_MOST, so outputs in
-// tensor memory are seldom rescaled.  Weights are at most 2^8, the largest at least 1: fp16 holds them to 2^-11, and
-// those below 2^-14 to 2^-25.  Score x scale less the reference is rounded once, so whatever the reference was rounded to, a
+// tensor memory are seldom rescaled.  Weights of fp16 are at most 2^8, the largest at least 1, held to 2^-11 and below 2^-14
+// to 2^-25; of bf16 at most 1, the largest at least 2^-8.  Score x scale less the reference is rounded once, so whatever the reference was rounded to, a
 // part's sums go with it exactly.  Its rounding stays in every weight's exponent, half a step of it at most: beyond
 // 2^24 that is more than weights have room for.  A row that meets such a reference is marked (no number for a reference),
 // and the joining kernel forms it again by itself, score x scale rounded first.  (To do that in the softmax cost 3 to 8 % of
@@ -47,7 +47,10 @@
 namespace n730 {
 
 constexpr int KA_KEYS = 128;       // positions of a tile
-constexpr float KA_MOST = 8.f;     // log2 of how large a weight may grow against its reference
+// log2 of where a new reference puts the largest weight, and of how large a weight may grow before the reference moves.  fp16
+// has room above 1 and little below; bf16 has as much below, and values whose multiples by 2^8 fp32 does not hold.
+template <bool BF> constexpr float KA_NEW = BF ? -8.f : 0.f;
+template <bool BF> constexpr float KA_MOST = BF ? 0.f : 8.f;
 constexpr float KA_FAR = 0x1p24f;  // references beyond this leave nothing of a score behind its own rounding
 constexpr int KA_RING = 4;         // tiles whose masks are kept
 constexpr int KA_BAD = 256;        // positions of an item that some of its rows see and others do not: fewer than its rows
@@ -135,11 +138,11 @@ __device__ __forceinline__ float ka_row_max(float y, float* mine, const float* o
   asm volatile("bar.sync %0, 64;" :: "r"(bar) : "memory");
   return fmaxf(y, *other);
 }
-// Moves a row's reference to its tile's maximum y where that is larger; the thread's sum and, when there are any, its
+// Moves a row's reference to where its tile's maximum y asks for it, if that is further up; the thread's sum and, when there are any, its
 // half of the outputs (at to) follow.  far: the row's mark.
-template <int HD>
+template <int HD, bool BF>
 __device__ __forceinline__ void ka_move(uint32_t to, bool outputs, float y, float& m, float& l, uint8_t* far) {
-  const float mn = fmaxf(m, y), f = mn == m ? 1.f : ex2(m - mn);
+  const float mn = fmaxf(m, y - KA_NEW<BF>), f = mn == m ? 1.f : ex2(m - mn);
   m = mn;
   l *= f;
   if (fabsf(mn) > KA_FAR && fabsf(mn) < INFINITY) *far = 1;
@@ -159,7 +162,7 @@ __device__ __forceinline__ void ka_softmax(uint32_t ts, uint32_t tp, uint32_t to
 #pragma unroll
   for (int i = 4; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
   const float y = ka_row_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c, mine, other, bar);
-  if (__any_sync(0xffffffffu, y > m + KA_MOST)) ka_move<HD>(to, outputs, y, m, l, far);
+  if (__any_sync(0xffffffffu, y > m + KA_MOST<BF>)) ka_move<HD, BF>(to, outputs, y, m, l, far);
   const float ms = m == -INFINITY ? 0.f : m;
   const float2 c2 = both(c), m2 = both(-ms);
   float2 sum[2] = {both(0.f), both(0.f)};
@@ -187,7 +190,7 @@ __device__ __forceinline__ void ka_softmax_some(uint32_t ts, uint32_t tp, uint32
     mx = fmaxf(mx, v[i]);
   }
   const float y = ka_row_max(mx == -INFINITY ? mx : mx * c, mine, other, bar);  // c may be 0
-  if (__any_sync(0xffffffffu, y > m + KA_MOST)) ka_move<HD>(to, outputs, y, m, l, far);
+  if (__any_sync(0xffffffffu, y > m + KA_MOST<BF>)) ka_move<HD, BF>(to, outputs, y, m, l, far);
   const float ms = m == -INFINITY ? 0.f : m;
   uint32_t w[32];
   float sum = 0.f;
@@ -658,7 +661,7 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
           big[e] = fmaxf(x[y][e], x[y][2 + e]);
           big[e] = big[e] == -INFINITY ? big[e] : big[e] * a.scale_log2e;  // the scale may be 0
         }
-        if (__any_sync(0xffffffffu, big[0] > m[y][0] + KA_MOST || big[1] > m[y][1] + KA_MOST)) {
+        if (__any_sync(0xffffffffu, big[0] > m[y][0] + KA_MOST<BF> || big[1] > m[y][1] + KA_MOST<BF>)) {
 #pragma unroll
           for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -666,7 +669,7 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
           float f[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float mn = fmaxf(m[y][e], big[e]);
+            const float mn = fmaxf(m[y][e], big[e] - KA_NEW<BF>);
             f[e] = mn == m[y][e] ? 1.f : ex2(m[y][e] - mn);
             m[y][e] = mn;
             l[y][e] *= f[e];
