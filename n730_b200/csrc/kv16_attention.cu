@@ -103,8 +103,8 @@ struct KAArgs {
   int batch, tokens, heads, group;
   int prefix_items, box;
   bool qvec, ovec;
-  float scale_log2e;         // its absolute value; the sign goes with the queries
-  uint32_t sign;
+  float scale_log2e;         // its absolute value, and 1 for a scale of 0: both go with the queries, whose bits are
+  uint32_t sign, keep;       // taken as (q ^ sign) & keep
   const int* lens; const int* n_new;
   int* status;
   KAParts pre, own;
@@ -189,7 +189,7 @@ __device__ __forceinline__ void ka_softmax_some(uint32_t ts, uint32_t tp, uint32
     v[i] = i < sees && (pages >> (i / 16) & 1) ? v[i] : -INFINITY;
     mx = fmaxf(mx, v[i]);
   }
-  const float y = ka_row_max(mx == -INFINITY ? mx : mx * c, mine, other, bar);  // c may be 0
+  const float y = ka_row_max(mx * c, mine, other, bar);
   if (__any_sync(0xffffffffu, y > m + KA_MOST<BF>)) ka_move<HD, BF>(to, outputs, y, m, l, far);
   const float ms = m == -INFINITY ? 0.f : m;
   uint32_t w[32];
@@ -399,7 +399,7 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
     for (int u = 0; u < QU; ++u) {
       const int r = warp * 16 + u * QR + qsub;
       *reinterpret_cast<uint4*>(sm.q + (qch >> 3) * Cfg::QB + r * 128 + (((qch & 7) ^ (r & 7)) << 4)) =
-          make_uint4(qx[u].x ^ a.sign, qx[u].y ^ a.sign, qx[u].z ^ a.sign, qx[u].w ^ a.sign);
+          make_uint4((qx[u].x ^ a.sign) & a.keep, (qx[u].y ^ a.sign) & a.keep, (qx[u].z ^ a.sign) & a.keep, (qx[u].w ^ a.sign) & a.keep);
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
@@ -482,7 +482,7 @@ kv16_attention_kernel(const KAArgs a, const __grid_constant__ CUtensorMap kmap, 
             const int64_t qa = query(f);
             float dot = 0.f;
             for (int d = 0; d < HD; ++d) dot = fmaf(kv8_load1(a.q, qa + d, c.dtype), kv8_load1(c.k, at + d, c.dtype), dot);
-            const float w = ex2(fmaf(a.sign ? -dot : dot, a.scale_log2e, -ms));
+            const float w = ex2(fmaf(!a.keep ? 0.f : a.sign ? -dot : dot, a.scale_log2e, -ms));
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = fmaf(w, kv8_load1(c.v, at + half * (HD / 2) + cc + e, c.dtype), o[e]);
           }
@@ -617,7 +617,7 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const uint16_t* at = qp + k * 16 + e * 8;
-          q[y][k][e] = r >= nrow ? 0u : (a.qvec ? *reinterpret_cast<const uint32_t*>(at) : at[0] | (uint32_t)at[1] << 16) ^ a.sign;
+          q[y][k][e] = r >= nrow ? 0u : ((a.qvec ? *reinterpret_cast<const uint32_t*>(at) : at[0] | (uint32_t)at[1] << 16) ^ a.sign) & a.keep;
         }
     }
     int vis[NB][2];  // of the rows whose scores this lane holds
@@ -628,6 +628,12 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
     float o[NB][KS][4] = {}, m[NB][2], l[NB][2] = {};
 #pragma unroll
     for (int y = 0; y < NB; ++y) m[y][0] = m[y][1] = -INFINITY;
+    // scores x scale less the reference: in one step, as the kernel above; beyond KA_FAR the product in a step of its own
+    float c0[NB][2], c1[NB][2];
+#pragma unroll
+    for (int y = 0; y < NB; ++y)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) { c0[y][e] = 1.f; c1[y][e] = a.scale_log2e; }
     // where this lane's rows of the four 8 x 8 pieces lie: K's by position and then channels, V's turned
     const int kr = lane & 15, kc = lane >> 4, vr = (lane & 7) + (lane >> 4) * 8, vc = lane >> 3 & 1;
 #pragma unroll 1
@@ -658,8 +664,7 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
         for (int e = 0; e < 2; ++e) {
           x[y][e] = p < vis[y][e] ? x[y][e] + x2[y][e] : -INFINITY;
           x[y][2 + e] = p + 8 < vis[y][e] ? x[y][2 + e] + x2[y][2 + e] : -INFINITY;
-          big[e] = fmaxf(x[y][e], x[y][2 + e]);
-          big[e] = big[e] == -INFINITY ? big[e] : big[e] * a.scale_log2e;  // the scale may be 0
+          big[e] = fmaxf(x[y][e], x[y][2 + e]) * a.scale_log2e;
         }
         if (__any_sync(0xffffffffu, big[0] > m[y][0] + KA_MOST<BF> || big[1] > m[y][1] + KA_MOST<BF>)) {
 #pragma unroll
@@ -673,6 +678,9 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
             f[e] = mn == m[y][e] ? 1.f : ex2(m[y][e] - mn);
             m[y][e] = mn;
             l[y][e] *= f[e];
+            const bool far = fabsf(mn) > KA_FAR && mn > -INFINITY;
+            c0[y][e] = far ? a.scale_log2e : 1.f;
+            c1[y][e] = far ? 1.f : a.scale_log2e;
           }
 #pragma unroll
           for (int k = 0; k < KS; ++k)
@@ -682,9 +690,7 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float ms = m[y][e & 1] == -INFINITY ? 0.f : m[y][e & 1];
-          // in one step with the reference, as the kernel above; beyond KA_FAR in a step of its own
-          const float2 f = fabsf(ms) > KA_FAR ? make_float2(a.scale_log2e, 1.f) : make_float2(1.f, a.scale_log2e);
-          e4[y][e] = x[y][e] == -INFINITY ? 0.f : ex2(fmaf(x[y][e] * f.x, f.y, -ms));
+          e4[y][e] = ex2(fmaf(x[y][e] * c0[y][e & 1], c1[y][e & 1], -ms));
           l[y][e & 1] += e4[y][e];
         }
         w[y][0] = ko_transpose(ka_pack<BF>(e4[y][0], e4[y][1]));
@@ -1085,7 +1091,8 @@ N730_API int n730_kv16_attention(const N730KV16Cache* c, const void* d_q, int64_
   while (a.box < KA_KEYS && c->page_size % (2 * a.box) == 0) a.box *= 2;
   a.qvec = ((uintptr_t)d_q & 15) == 0 && ldq % 8 == 0;
   a.ovec = ((uintptr_t)d_out & 7) == 0 && ldo % 4 == 0;
-  a.scale_log2e = std::fabs(scale_log2e);
+  a.scale_log2e = scale_log2e == 0.f ? 1.f : std::fabs(scale_log2e);
+  a.keep = scale_log2e == 0.f ? 0u : ~0u;
   a.sign = scale < 0 ? 0x80008000u : 0u;
   a.lens = d_lens; a.n_new = d_new;
   a.status = reinterpret_cast<int*>(ws);
