@@ -20,7 +20,8 @@
 // part's sums go with it exactly.  Its rounding stays in every weight's exponent, half a step of it at most: beyond
 // 2^24 that is more than weights have room for.  A row that meets such a reference is marked (no number for a reference),
 // and the joining kernel forms it again by itself, score x scale rounded first.  (To do that in the softmax cost 3 to 8 % of
-// every call: 81 us -> 84 to 88.  A token whose 28 rows are all marked takes 7 ms behind 16384 positions.)
+// every call: 81 us -> 84 to 88, a second pass over the item in the same kernel 2 to 8 %.  128 sequences of 64 heads behind
+// 16384 positions, all rows marked, take 10 ms.)
 //
 // What lies behind the last position anyone sees may be anything: scores are masked, and those rows of V are zeroed in
 // shared memory before the product (zero weight times NaN is NaN).  Rows of V that some rows of the item see and others
@@ -759,53 +760,55 @@ __global__ void __launch_bounds__(32) kv16_own_kernel(const KAArgs a) {
   if (blockIdx.x == 0) pdl_wait();
 }
 
-// A marked row by itself, by all warps of a CTA: 4 positions at a time each, a lane its share of the channels.  CH of the row's
-// channels, from `ch` on.  Inline: a call's stack cost every launch of the joining kernel 1 us.
+// A marked row by itself, by all warps of a CTA: 32 positions at a time each, then a lane its share of the channels for the
+// few weights that are left.  CH of the row's channels, from `ch` on.  Inline: a call's stack cost every launch of the joining
+// kernel 1 us.
 template <int HD, bool BF, int CH, int WARPS>
 __device__ __forceinline__ void ka_again(const KAArgs& a, int b, int t, int h, int g, int ch, float (&part)[WARPS][CH + 2]) {
-  constexpr int QL = HD / 32, VL = CH / 32, N = 4;
+  constexpr int VL = CH / 32, LANES = HD / 8, GROUP = 32 / LANES;  // lanes of a row of K, rows at a time
   const N730KV16Cache& c = a.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int cap = c.max_pages * c.page_size, prefix = kv16_prefix(c), all = prefix + min(kv8_len(a.lens, b, cap) + t + 1, cap);
   const int64_t at = (int64_t)(b * a.tokens + t), col = (int64_t)(h * a.group + g) * HD;
+  float q[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) q[e] = kv8_load1(a.q, at * a.ldq + col + lane % LANES * 8 + e, c.dtype);
   const float scale = a.sign ? -a.scale_log2e : a.scale_log2e;
-  float q[QL], m = -INFINITY, l = 0.f, o[VL] = {};
-#pragma unroll
-  for (int e = 0; e < QL; ++e) q[e] = kv8_load1(a.q, at * a.ldq + col + lane * QL + e, c.dtype);
+  float m = -INFINITY, l = 0.f, o[VL] = {};
 #pragma unroll 1
-  for (int i0 = warp * N; i0 < all; i0 += WARPS * N) {
-    int64_t row[N];  // -1: a position that is none
-    float x[N], mn = m;
+  for (int i0 = warp * 32; i0 < all; i0 += WARPS * 32) {
+    const int i = i0 + lane, p = i < prefix ? i : i - prefix;
+    const int page = i >= all ? -1 : i < prefix ? c.prefix_table[p / c.page_size] : c.block_table[(int64_t)b * c.max_pages + p / c.page_size];
+    const int64_t row = (unsigned)page < (unsigned)c.n_pages ? (((int64_t)page * c.n_kv + h) * c.page_size + p % c.page_size) * HD : -1;
+    float x = -INFINITY;
+#pragma unroll 4
+    for (int k = 0; k < LANES; ++k) {  // GROUP positions at a time
+      const int64_t from = max(__shfl_sync(0xffffffffu, row, k * GROUP + lane / LANES), (int64_t)0);  // the pool's first row for none
+      const uint4 y = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(c.k) + from + lane % LANES * 8);
+      const float2 y0 = ka_wide<BF>(y.x), y1 = ka_wide<BF>(y.y), y2 = ka_wide<BF>(y.z), y3 = ka_wide<BF>(y.w);
+      float d = fmaf(q[0], y0.x, q[1] * y0.y);
+      d = fmaf(q[2], y1.x, d); d = fmaf(q[3], y1.y, d); d = fmaf(q[4], y2.x, d);
+      d = fmaf(q[5], y2.y, d); d = fmaf(q[6], y3.x, d); d = fmaf(q[7], y3.y, d);
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int i = i0 + k, p = i < prefix ? i : i - prefix;
-      const int page = i >= all ? -1 : i < prefix ? c.prefix_table[p / c.page_size] : c.block_table[(int64_t)b * c.max_pages + p / c.page_size];
-      row[k] = (unsigned)page < (unsigned)c.n_pages ? (((int64_t)page * c.n_kv + h) * c.page_size + p % c.page_size) * HD : -1;
-      x[k] = 0.f;
-      if (row[k] >= 0)
-#pragma unroll
-        for (int e = 0; e < QL; ++e) x[k] = fmaf(q[e], kv8_load1(c.k, row[k] + lane * QL + e, c.dtype), x[k]);
+      for (int e = 1; e < LANES; e <<= 1) d += __shfl_xor_sync(0xffffffffu, d, e);
+      d = __shfl_sync(0xffffffffu, d, lane % GROUP * LANES);
+      if (lane / GROUP == k && row >= 0) x = d * scale;
     }
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      x[k] = row[k] < 0 ? -INFINITY : warp_sum(x[k]) * scale;
-      mn = fmaxf(mn, x[k]);
-    }
-    const float f = mn == m ? 1.f : ex2(m - mn);
+    const float mn = fmaxf(m, warp_max(x)), f = mn == m ? 1.f : ex2(m - mn), w = x == -INFINITY ? 0.f : ex2(x - mn);
     m = mn;
-    l *= f;
+    l = l * f + w;
 #pragma unroll
     for (int e = 0; e < VL; ++e) o[e] *= f;
+    for (unsigned some = __ballot_sync(0xffffffffu, !(w == 0.f)); some; some &= some - 1) {
+      const int k = __ffs(some) - 1;
+      const int64_t from = __shfl_sync(0xffffffffu, row, k) + ch + lane * VL;
+      const float wk = __shfl_sync(0xffffffffu, w, k);
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      if (row[k] < 0) continue;
-      const float w = x[k] == -INFINITY ? 0.f : ex2(x[k] - m);
-      l += w;
-#pragma unroll
-      for (int e = 0; e < VL; ++e) o[e] = fmaf(w, kv8_load1(c.v, row[k] + ch + lane * VL + e, c.dtype), o[e]);
+      for (int e = 0; e < VL; ++e) o[e] = fmaf(wk, kv8_load1(c.v, from + e, c.dtype), o[e]);
     }
   }
-  __syncthreads();
+  l = warp_sum(l);
+  __syncthreads();  // the row before is through with its parts
 #pragma unroll
   for (int e = 0; e < VL; ++e) part[warp][lane * VL + e] = o[e];
   if (lane == 0) { part[warp][CH] = m; part[warp][CH + 1] = l; }
