@@ -16,12 +16,12 @@
 //
 // Softmax.  A row's reference follows its maximum lazily: it moves when a weight would pass 2^KA_MOST, so outputs in
 // tensor memory are seldom rescaled.  Weights of fp16 are at most 2^8, the largest at least 1, held to 2^-11 and below 2^-14
-// to 2^-25; of bf16 at most 1, the largest at least 2^-8.  Score x scale less the reference is rounded once, so whatever the reference was rounded to, a
-// part's sums go with it exactly.  Its rounding stays in every weight's exponent, half a step of it at most: beyond
-// 2^24 that is more than weights have room for.  A row that meets such a reference is marked (no number for a reference),
-// and the joining kernel forms it again by itself, score x scale rounded first.  (To do that in the softmax cost 3 to 8 % of
-// every call: 81 us -> 84 to 88, a second pass over the item in the same kernel 2 to 8 %.  128 sequences of 64 heads behind
-// 16384 positions, all rows marked, take 10 ms.)
+// to 2^-25; of bf16 at most 1, the largest at least 2^-8.  Score x scale less the reference is rounded once, so whatever the
+// reference was rounded to, a part's sums go with it exactly.  Its rounding stays in every weight's exponent, half a step of it
+// at most: beyond 2^24 that is more than weights have room for.  A row that meets such a reference is marked (no number for a
+// reference), and the joining kernel forms it again by itself, score x scale rounded first.  (To do that in the softmax cost 3
+// to 8 % of every call: 81 us -> 84 to 88, a second pass over the item in the same kernel 2 to 8 %.  128 sequences of 64 heads
+// behind 16384 positions, all rows marked, take 10 ms.)
 //
 // What lies behind the last position anyone sees may be anything: scores are masked, and those rows of V are zeroed in
 // shared memory before the product (zero weight times NaN is NaN).  Rows of V that some rows of the item see and others
