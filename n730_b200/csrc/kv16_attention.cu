@@ -964,9 +964,9 @@ static KAPlan ka_plan(const N730KV16Cache& c, int batch, int tokens, int heads) 
   const int64_t cap = (int64_t)c.max_pages * c.page_size;
   shape(own_rows, own_units, cap, p.own_nt, p.own_tiles, p.own_splits);
   p.own_rows = p.own_tiles * p.own_nt * 128;
-  // few rows: warps of 16 where they fill a share of the SMs (128 sequences of 64 heads, 8 rows each: 83 us for 123; with 3
-  // groups of rows, 16 sequences of 5 tokens and 28 heads, 38 for 36), in one grid with the prefix's items otherwise (one
-  // launch less: 4 sequences of 14 heads 10 us for 12)
+  // few rows: warps of 16 where they fill a share of the SMs (128 sequences of 64 heads, 8 rows each: 82 us for 117; with 3
+  // groups of rows, 16 sequences of 5 tokens and 28 heads, 35.1 for 34.8), in one grid with the prefix's items otherwise (one
+  // launch less: 4 sequences of 14 heads 10.2 us for 10.5)
   if (own_rows <= KO_MOST && own_units >= sms / 4) {
     p.own_nt = 0;
     p.own_tiles = (int)((own_rows + KO_ROWS - 1) / KO_ROWS);
